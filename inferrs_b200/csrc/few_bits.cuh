@@ -1,0 +1,79 @@
+// Numbers in few bits: what the kernels of 4-bit matrices and 8-bit keys and values share.
+//
+// A 4-bit matrix [rows, width] (sign, two bits of exponent, one of mantissa; a power of two per 32 numbers of a row):
+//   codes   byte [row][k / 2], the earlier number in the low half; a row takes 64 bytes per 128 numbers, zeros behind width
+//   scales  byte [row / 128][k / 128][row % 32][row / 32 % 4][k / 32 % 4] = exponent + 127 (255: no number at all), an even
+//           number of 128-column tiles, zeros behind width.  512 bytes are what the block-scaled product wants beside a
+//           tile of 128 rows and 128 columns: copied into tensor memory as they stand.
+// 8-bit keys and values: e4m3 codes [page][head][place][dim], a float32 scale per vector [page][head][place].
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace few {
+
+__host__ __device__ __forceinline__ long code_pitch(int width) { return (long)((width + 127) / 128) * 64; }
+__host__ __device__ __forceinline__ int scale_tiles(int width) { return (width + 255) / 256 * 2; }
+// where the four scales of row `row` and columns 128 t .. 128 t + 127 are
+__device__ __forceinline__ long scale_word(int row, int t, int tiles) {
+    return ((long)(row >> 7) * tiles + t) * 128 + (row & 31) * 4 + (row >> 5 & 3);
+}
+
+// The scale byte of a block from the bits of its largest magnitude: the exponent that puts it into 3.5 .. 7 (up to 7 the
+// nearest code, 6, is off by at most a seventh; beyond, the next power of two is nearer).  0 for a block of zeros or of
+// numbers too small for any exponent, 255 where there is an infinity or no number.
+__device__ __forceinline__ unsigned scale_byte(unsigned largest_bits) {
+    const unsigned e = largest_bits >> 23;
+    if (e == 255u) return 255u;
+    const int b = (int)e - 2 + ((largest_bits & 0x7FFFFFu) > 0x600000u);
+    return b < 0 ? 0u : (unsigned)b;
+}
+// 2^(byte - 127), and its reciprocal (both exact; bytes of scale_byte: 0 .. 253)
+__device__ __forceinline__ float scale_value(unsigned byte) {
+    return byte == 255u ? __uint_as_float(0x7FC00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+__device__ __forceinline__ float scale_reciprocal(unsigned byte) {
+    return byte == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - byte) << 23);
+}
+// two numbers as codes, nearest with ties to even, beyond 6 as 6; the first in the low half of the byte
+__device__ __forceinline__ unsigned codes2(float first, float second) {
+    unsigned r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(first), "f"(second));
+    return r;
+}
+// the value of a 4-bit code
+__device__ __forceinline__ float code_value(unsigned c) {
+    const unsigned m = c & 7u;
+    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+    return c & 8u ? -v : v;
+}
+
+// ---- 8-bit keys and values ----------------------------------------------------------------------------------------------
+// four numbers as e4m3 codes, nearest with ties to even, beyond 448 as 448 (no number stays none)
+__device__ __forceinline__ unsigned codes8x4(float a, float b, float c, float d) {
+    unsigned short lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
+    return (unsigned)lo | (unsigned)hi << 16;
+}
+// two codes (the low half first) as f16 pairs: exact
+__device__ __forceinline__ unsigned values8x2(unsigned short c) {
+    unsigned r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+    return r;
+}
+__device__ __forceinline__ float value8(unsigned char c) {
+    const unsigned v = values8x2(c);
+    return __low2float(*reinterpret_cast<const __half2*>(&v));
+}
+// What a vector with the largest magnitude `a` is multiplied by before its numbers are rounded, and its scale.  A vector
+// whose numbers are all below 2^-100 counts as zeros; one with an infinity or no number reads back as no numbers.
+__device__ __forceinline__ void vector_scale(float a, float& by, float& scale) {
+    const bool some = !(a < 7.888609052210118e-31f);
+    by = some ? 448.0f / a : 0.0f;
+    scale = some ? a / 448.0f : 0.0f;
+}
+
+}  // namespace few

@@ -1,0 +1,211 @@
+// Keys and values in 8 bits: how a step's join the paged cache, and attention over it for any head size.
+// (The layout is in few_bits.cuh.)
+#include "few_bits.cuh"
+
+// The first row (plus one) that was left out because its position lay outside the rotation tables; 0: none.
+__device__ int ib_kv8_row_fault_word = 0;
+IB_EXPORT int ib_kv8_row_fault(int reset) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, ib_kv8_row_fault_word, sizeof(int));
+    if (e != cudaSuccess) return -(int)e;
+    if (reset && v != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(ib_kv8_row_fault_word, &zero, sizeof(int));
+    }
+    return v;
+}
+IB_EXPORT int ib_kv8_row_fault_async(int* out, cudaStream_t stream) {
+    return (int)cudaMemcpyFromSymbolAsync(out, ib_kv8_row_fault_word, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+}
+
+namespace few {
+
+constexpr int STORE_WARPS = 4;
+
+struct StoreArgs {
+    long ldx;
+    int n_heads, n_kv, d, flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages;   // flags: 1 norm q, 2 norm k
+    float eps;
+};
+
+// A warp per head of a row: norm, rotation in float32; queries are stored in their type, keys and values as codes
+// with a scale per vector.
+template <typename T, typename WT>
+__global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
+    const T* __restrict__ qkv, const WT* __restrict__ q_weight, const WT* __restrict__ k_weight,
+    const float* __restrict__ cos_table, const float* __restrict__ sin_table, const int* __restrict__ positions,
+    const int* __restrict__ row_request, const int* __restrict__ block_table, unsigned char* __restrict__ k_pages,
+    unsigned char* __restrict__ v_pages, float* __restrict__ k_scale, float* __restrict__ v_scale, T* __restrict__ q_out,
+    const StoreArgs a) {
+    extern __shared__ float smem[];
+    ib_grid_dependency_launch();
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.d;
+    const int head = blockIdx.y * STORE_WARPS + warp;
+    float* sh = smem + warp * 2 * d;      // the head as it came, and turned
+    float* turned = sh + d;
+    const int pos = positions[row];
+    const bool fault = pos < 0 || (a.rot_dim > 0 && pos >= a.table_rows);
+    ib_grid_dependency_wait();
+    qkv = ib_after_wait(qkv);
+    if (fault) {
+        if (threadIdx.x == 0) atomicCAS(&ib_kv8_row_fault_word, 0, row + 1);
+        return;
+    }
+    if (head >= a.n_heads + 2 * a.n_kv) return;
+    const int kind = head < a.n_heads ? 0 : (head < a.n_heads + a.n_kv ? 1 : 2);   // 0 q, 1 k, 2 v
+    long place = -1;
+    if (kind != 0) {
+        const int page = pos / a.page_size < a.max_pages ? block_table[(long)row_request[row] * a.max_pages + pos / a.page_size] : -1;
+        if (page < 0 || page >= a.n_pages) return;      // a request that stands in to fill a batch
+        place = ((long)page * a.n_kv + (head - a.n_heads) % a.n_kv) * a.page_size + pos % a.page_size;
+    }
+    const T* src = qkv + (long)row * a.ldx + (long)head * d;
+    float ss = 0.0f;
+    for (int j = lane; j < d; j += 32) { sh[j] = ib_to_float(src[j]); ss += sh[j] * sh[j]; }
+    const float* out = sh;
+    if (kind != 2) {
+        if (a.flags >> kind & 1) {
+            const float inv = 1.0f / sqrtf(ib_warp_sum(ss) / (float)d + a.eps);
+            const WT* w = kind == 0 ? q_weight : k_weight;
+            for (int j = lane; j < d; j += 32) sh[j] = sh[j] * inv * (w ? ib_to_float(w[j]) : 1.0f);
+        }
+        __syncwarp();
+        const int half = a.rot_dim / 2;
+        const float *c = cos_table + (long)pos * half, *s = sin_table + (long)pos * half;
+        // element i of the first half turns with element i + rot_dim / 2, or (interleaved) element 2i with 2i + 1.  The
+        // products are rounded before they are added up, so that the codes do not depend on how a compiler joins them.
+        for (int j = lane; j < d; j += 32) {
+            float o = sh[j];
+            if (j < a.rot_dim) {
+                const int i = a.interleaved ? j >> 1 : (j < half ? j : j - half);
+                const bool first = a.interleaved ? !(j & 1) : j < half;
+                const float other = a.interleaved ? sh[j ^ 1] : sh[first ? j + half : j - half];
+                o = first ? __fsub_rn(__fmul_rn(o, c[i]), __fmul_rn(other, s[i])) : __fadd_rn(__fmul_rn(o, c[i]), __fmul_rn(other, s[i]));
+            }
+            turned[j] = o;
+        }
+        out = turned;
+    }
+    __syncwarp();
+    if (kind == 0) {
+        T* dst = q_out + ((long)row * a.n_heads + head) * d;
+        for (int j = lane; j < d; j += 32) dst[j] = ib_from_float<T>(out[j]);
+        return;
+    }
+    unsigned m = 0;
+    for (int j = lane; j < d; j += 32) m = max(m, __float_as_uint(out[j]) & 0x7FFFFFFFu);   // no number counts as the largest
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float by, scale;
+    vector_scale(__uint_as_float(m), by, scale);
+    unsigned char* dst = (kind == 1 ? k_pages : v_pages) + place * d;
+    for (int j = 4 * lane; j < d; j += 128)
+        *reinterpret_cast<unsigned*>(dst + j) = codes8x4(out[j] * by, out[j + 1] * by, out[j + 2] * by, out[j + 3] * by);
+    if (lane == 0) (kind == 1 ? k_scale : v_scale)[place] = scale;
+}
+
+// Attention of every (row, head) by a block of its own: eight warps take every eighth key of the row's, each with a running
+// maximum and sum in float32, and join what they have in shared memory.  Any head size up to 512, float32 throughout.
+constexpr int SLOW_WARPS = 8, SLOW_PER_LANE = 16;
+
+struct AttendArgs {
+    int max_pages, page_size, n_pages, n_req, n_heads, n_kv, d, span;
+    float scale;
+    long out_ld;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * SLOW_WARPS) kv8_attention_kernel(
+    const T* __restrict__ q, const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
+    const float* __restrict__ k_scale, const float* __restrict__ v_scale, const int* __restrict__ block_table,
+    const int* __restrict__ row_request, const int* __restrict__ positions, T* __restrict__ out, const AttendArgs a) {
+    __shared__ float part[SLOW_WARPS][512], part_m[SLOW_WARPS], part_l[SLOW_WARPS];
+    ib_grid_dependency_sync();
+    const int row = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.d;
+    const int kvh = head / (a.n_heads / a.n_kv), pos = positions[row], req = row_request[row];
+    const int lo = ib_first_visible(pos, a.span);
+    const bool known = req >= 0 && req < a.n_req;
+    float qv[SLOW_PER_LANE], acc[SLOW_PER_LANE], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SLOW_PER_LANE; ++i) {
+        const int j = lane + 32 * i;
+        qv[i] = j < d ? ib_to_float(q[((long)row * a.n_heads + head) * d + j]) * a.scale : 0.0f;
+        acc[i] = 0.0f;
+    }
+    for (int t = lo + warp; known && t <= pos; t += SLOW_WARPS) {
+        const int page = t / a.page_size < a.max_pages ? block_table[(long)req * a.max_pages + t / a.page_size] : -1;
+        if (page < 0 || page >= a.n_pages) continue;
+        const long place = ((long)page * a.n_kv + kvh) * a.page_size + t % a.page_size;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SLOW_PER_LANE; ++i) {
+            const int j = lane + 32 * i;
+            if (j < d) s = fmaf(qv[i], value8(k_pages[place * d + j]), s);
+        }
+        s = ib_warp_sum(s) * k_scale[place];
+        const float m2 = fmaxf(m, s), fade = m == -INFINITY ? 0.0f : expf(m - m2), p = expf(s - m2);
+        const float pv = p * v_scale[place];
+        l = l * fade + p;
+        m = m2;
+#pragma unroll
+        for (int i = 0; i < SLOW_PER_LANE; ++i) {
+            const int j = lane + 32 * i;
+            if (j < d) acc[i] = acc[i] * fade + pv * value8(v_pages[place * d + j]);
+        }
+    }
+    if (lane == 0) { part_m[warp] = m; part_l[warp] = l; }
+#pragma unroll
+    for (int i = 0; i < SLOW_PER_LANE; ++i) if (lane + 32 * i < d) part[warp][lane + 32 * i] = acc[i];
+    __syncthreads();
+    float top = -INFINITY, sum = 0.0f;
+    for (int w = 0; w < SLOW_WARPS; ++w) if (part_l[w] != 0.0f) top = fmaxf(top, part_m[w]);
+    for (int w = 0; w < SLOW_WARPS; ++w) if (part_l[w] != 0.0f) sum += part_l[w] * expf(part_m[w] - top);
+    for (int j = threadIdx.x; j < d; j += 32 * SLOW_WARPS) {
+        float o = 0.0f;
+        for (int w = 0; w < SLOW_WARPS; ++w) if (part_l[w] != 0.0f) o += part[w][j] * expf(part_m[w] - top);
+        out[(long)row * a.out_ld + (long)head * d + j] = ib_from_float<T>(sum != 0.0f ? o / sum : 0.0f);   // a row that sees no key: zeros
+    }
+}
+
+}  // namespace few
+
+// The step's rows qkv [n, queries | keys | values of n_heads, n_kv, n_kv heads of d numbers] (float32 or bfloat16): per-head
+// norm (norm_flags: 1 queries, 2 keys) and rotation, queries to q_out, keys and values as 8-bit codes into their pages.
+IB_EXPORT int ib_qk_norm_rope_store_kv8(const void* qkv, int is_f32, long ldx, int n, int n_heads, int n_kv, int d,
+                                        const void* q_weight, const void* k_weight, int w_is_f32, int norm_flags, float eps,
+                                        const float* cos_table, const float* sin_table, int rot_dim, int interleaved, int table_rows,
+                                        const int* positions, const int* row_request, const int* block_table, int max_pages,
+                                        int page_size, int n_pages, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+                                        void* q_out, cudaStream_t stream) {
+    using namespace few;
+    if (n < 0 || n_heads <= 0 || n_kv <= 0 || d <= 0 || d % 4 || d > 1024 || rot_dim < 0 || rot_dim > d || rot_dim % 2 || page_size <= 0) return IB_ERR_ARGUMENT;
+    if (n == 0) return IB_OK;
+    const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, eps};
+    const dim3 grid(n, (n_heads + 2 * n_kv + STORE_WARPS - 1) / STORE_WARPS);
+    const size_t smem = (size_t)STORE_WARPS * 2 * d * sizeof(float);
+#define GO(T, WT) ib_launch(kv8_store_kernel<T, WT>, grid, dim3(32 * STORE_WARPS), smem, stream, (const T*)qkv, (const WT*)q_weight, \
+    (const WT*)k_weight, cos_table, sin_table, positions, row_request, block_table, (unsigned char*)k_pages, (unsigned char*)v_pages, \
+    k_scale, v_scale, (T*)q_out, a)
+    if (is_f32) { if (w_is_f32) GO(float, float); else GO(float, __nv_bfloat16); }
+    else { if (w_is_f32) GO(__nv_bfloat16, float); else GO(__nv_bfloat16, __nv_bfloat16); }
+#undef GO
+    return ib_launch_status();
+}
+
+IB_EXPORT int ib_paged_attention_kv8_generic(const void* q, int is_f32, const void* k_pages, const void* v_pages,
+                                             const float* k_scale, const float* v_scale, const int* block_table, int max_pages,
+                                             int page_size, int n_pages, int n_req, const int* row_request, const int* positions, int n,
+                                             int n_heads, int n_kv, int d, float scale, int span, void* out, long out_ld,
+                                             cudaStream_t stream) {
+    using namespace few;
+    if (n < 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || d <= 0 || page_size <= 0) return IB_ERR_ARGUMENT;
+    if (d > 512 || n_heads > 65535) return IB_ERR_UNSUPPORTED;
+    if (n == 0) return IB_OK;
+    const AttendArgs a = {max_pages, page_size, n_pages, n_req, n_heads, n_kv, d, span, scale, out_ld};
+    const dim3 grid(n, n_heads);
+#define GO(T) ib_launch(kv8_attention_kernel<T>, grid, dim3(32 * SLOW_WARPS), 0, stream, (const T*)q, (const unsigned char*)k_pages, \
+    (const unsigned char*)v_pages, k_scale, v_scale, block_table, row_request, positions, (T*)out, a)
+    if (is_f32) GO(float); else GO(__nv_bfloat16);
+#undef GO
+    return ib_launch_status();
+}

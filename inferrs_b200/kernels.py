@@ -2374,6 +2374,10 @@ def set_pdl(on: bool, act_dtype: torch.dtype = torch.bfloat16):
         gemm_tcgen05_set_pdl(on)
     else:
         _split_lib().ib_gemm_split_set_pdl(int(bool(on)))
+    global _FEW_BITS_PDL
+    _FEW_BITS_PDL = bool(on)
+    if _FEW_BITS_LIB is not None:      # a program without matrices in 4 bits or a cache in 8 never builds that library
+        _FEW_BITS_LIB.ib_few_bits_set_pdl(int(_FEW_BITS_PDL))
 
 
 # up to this many rows the own tcgen05 product is the faster one in a decode step (the environment variable is
@@ -2393,6 +2397,244 @@ def gemm_chain_error(reset: bool = True) -> int:
     if code != 0 and reset:
         _CHAIN_WS.clear()    # a chain that gave up may have left marks in its workspace: the next chain gets a fresh one
     return code
+
+
+# ---- numbers in few bits: matrices of 4-bit numbers, keys and values in 8 bits (csrc/few_bits.cuh) ---------------------
+_FEW_BITS_LIB, _FEW_BITS_PDL = None, False
+_FEW_BITS_SIGNATURES = {
+    "ib_quantize_mx4": [c_void_p, c_int, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    "ib_dequantize_mx4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_long, c_void_p],
+    "ib_product_mx4": [c_void_p, c_int, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_long,
+                       c_void_p],
+    "ib_qk_norm_rope_store_kv8": [c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float,
+                                  c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "ib_paged_attention_kv8_generic": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                       c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_long,
+                                       c_void_p],
+    "ib_kv8_row_fault": [c_int],
+    "ib_kv8_row_fault_async": [c_void_p, c_void_p],
+}
+_BF16_F32 = (torch.bfloat16, torch.float32)
+
+
+def _few_bits():
+    global _FEW_BITS_LIB
+    if _FEW_BITS_LIB is None:
+        lib = load_library("few_bits")
+        for fn, args in _FEW_BITS_SIGNATURES.items():
+            getattr(lib, fn).argtypes = args
+            getattr(lib, fn).restype = c_int
+        lib.ib_few_bits_set_pdl.argtypes = [c_int]
+        lib.ib_few_bits_set_pdl.restype = None
+        lib.ib_few_bits_set_pdl(int(_FEW_BITS_PDL))
+        _FEW_BITS_LIB = lib
+    return _FEW_BITS_LIB
+
+
+def mx4_shapes(rows: int, width: int):
+    """The shapes of a 4-bit matrix's codes and scales."""
+    return (rows, (width + 127) // 128 * 64), ((rows + 127) // 128, (width + 255) // 256 * 2, 32, 4, 4)
+
+
+@dataclass
+class Mx4Matrix:
+    """A matrix [rows, width] of 4-bit numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with a power of two per 32 numbers of
+    a row, in the layout that the kernels read (uint8):
+
+    codes   [rows, 64 per 128 of width], two numbers a byte, the earlier one in the low half, zeros behind ``width``
+    scales  [tile of 128 rows, tile of 128 columns (an even number), row % 32, row / 32 % 4, block of 32 % 4], the exponent
+            + 127 (255: the block holds no numbers), any but 255 behind ``width``"""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    width: int
+
+    def __post_init__(self):
+        _need(self.codes, "codes", (torch.uint8,), 2)
+        _need(self.scales, "scales", (torch.uint8,), 5)
+        want = mx4_shapes(self.rows, self.width) if self.rows >= 0 and self.width > 0 else (None, None)
+        if (tuple(self.codes.shape), tuple(self.scales.shape)) != want:
+            raise KernelError(f"a 4-bit matrix [{self.rows}, {self.width}] has codes and scales of shapes {want}, got "
+                              f"{tuple(self.codes.shape)} and {tuple(self.scales.shape)}")
+        if self.codes.data_ptr() % 32 or self.scales.data_ptr() % 16:
+            raise KernelError("a 4-bit matrix's codes start on 32 bytes, its scales on 16")
+
+    @classmethod
+    def empty(cls, rows: int, width: int, device) -> "Mx4Matrix":
+        if rows < 0 or width <= 0:
+            raise KernelError(f"a 4-bit matrix has rows of at least one number, got [{rows}, {width}]")
+        codes, scales = mx4_shapes(rows, width)
+        return cls(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device),
+                   rows, width)
+
+    @property
+    def shape(self):
+        return (self.rows, self.width)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def bytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def quantize_mx4(x: torch.Tensor, out: Optional[Mx4Matrix] = None) -> Mx4Matrix:
+    """The rows of ``x`` [rows, width] (float32 or bfloat16; they may lie apart) in 4 bits.  With a the largest magnitude of 32
+    neighbours, e = floor(log2 a) - 2, one more where a > 7 * 2^e, they are rounded to multiples of 2^e: to the nearest of
+    the eight magnitudes, ties to the even code, beyond 6 to 6.  e is kept within -127 and 127.  A block that holds an
+    infinity or no number reads back as no numbers."""
+    ld = _need_rows(x, "x", _BF16_F32)
+    rows, width = x.shape
+    if out is None:
+        out = Mx4Matrix.empty(rows, width, x.device)
+    elif out.shape != (rows, width):
+        raise KernelError(f"quantize_mx4: x {(rows, width)} for a matrix {out.shape}")
+    _check(_few_bits().ib_quantize_mx4(x.data_ptr(), x.dtype == torch.float32, ld, rows, width, out.codes.data_ptr(),
+                                       out.scales.data_ptr(), _stream()), "quantize_mx4")
+    return out
+
+
+def dequantize_mx4(w: Mx4Matrix, out: torch.Tensor):
+    """out [rows, width] = the values that ``w`` stands for (float32 or bfloat16; rows may lie apart).  Both types hold them
+    exactly, but for bfloat16's limits at the ends of the range."""
+    ld = _need_rows(out, "out", _BF16_F32)
+    if out.shape != w.shape:
+        raise KernelError(f"dequantize_mx4: a matrix {w.shape} into {tuple(out.shape)}")
+    _check(_few_bits().ib_dequantize_mx4(w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.width, out.data_ptr(),
+                                         out.dtype == torch.float32, ld, _stream()), "dequantize_mx4")
+
+
+def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor):
+    """out = x @ w.T.  ``x`` is a tensor [rows, width] (float32 or bfloat16; its rows may lie apart), whose numbers keep
+    their precision, or an :class:`Mx4Matrix`; sums are float32.  ``out`` [rows, features] may be float32 or bfloat16 and its
+    rows may lie apart."""
+    ldy = _need_rows(out, "out", _BF16_F32)
+    coded = isinstance(x, Mx4Matrix)
+    ldx = x.width if coded else _need_rows(x, "x", _BF16_F32)
+    n, k = x.shape
+    if k != w.width or out.shape != (n, w.rows):
+        raise KernelError(f"linear_mx4: x {(n, k)}, w {w.shape}, out {tuple(out.shape)}")
+    kind = 2 if coded else int(x.dtype == torch.float32)
+    _check(_few_bits().ib_product_mx4((x.codes if coded else x).data_ptr(), kind, ldx, x.scales.data_ptr() if coded else None,
+                                      w.codes.data_ptr(), w.scales.data_ptr(), n, w.rows, k, out.data_ptr(),
+                                      out.dtype == torch.float32, ldy, _stream()), "linear_mx4")
+
+
+@dataclass
+class Kv8Pages:
+    """Pages of keys and values in 8 bits: codes [pages, heads, page size, dim] (float8_e4m3fn) and one float32 scale per vector
+    [pages, heads, page size].  A number is its code times its vector's scale."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    def __post_init__(self):
+        for name, t in (("k", self.k), ("v", self.v)):
+            _need(t, name, (torch.float8_e4m3fn,), 4)
+            if t.data_ptr() % 16:
+                raise KernelError(f"{name}: pages of 8-bit numbers start on 16 bytes")
+        for name, t in (("k_scale", self.k_scale), ("v_scale", self.v_scale)):
+            _need(t, name, (torch.float32,), 3)
+        if self.v.shape != self.k.shape or self.k_scale.shape != self.k.shape[:3] or self.v_scale.shape != self.k.shape[:3]:
+            raise KernelError(f"8-bit pages: keys {tuple(self.k.shape)} with scales {tuple(self.k_scale.shape)}, values "
+                              f"{tuple(self.v.shape)} with scales {tuple(self.v_scale.shape)}")
+        if self.k.shape[3] % 4:
+            raise KernelError(f"8-bit pages hold heads of a multiple of four numbers, got {self.k.shape[3]}")
+
+    @classmethod
+    def zeros(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device) -> "Kv8Pages":
+        codes = torch.zeros((2, n_pages, n_kv_heads, page_size, head_dim), dtype=torch.uint8, device=device)
+        scales = torch.zeros((2, n_pages, n_kv_heads, page_size), dtype=torch.float32, device=device)
+        codes = codes.view(torch.float8_e4m3fn)
+        return cls(codes[0], codes[1], scales[0], scales[1])
+
+
+def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, q_weight: Optional[torch.Tensor],
+                           k_weight: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor],
+                           sin: Optional[torch.Tensor], rot_dim: int, positions: torch.Tensor, row_request: torch.Tensor,
+                           block_table: torch.Tensor, pages: Kv8Pages, q_out: torch.Tensor, interleaved: bool = False):
+    """:func:`qk_norm_rope_store` for a cache in 8 bits: per-head norm of q and k (where a weight is given), rotation by
+    position, q to ``q_out`` in its type, k and v into their pages.  With a the largest magnitude of a head's vector its
+    scale is a / 448 and a number is x * (448 / a) rounded to the nearest code, ties to even.  A vector below 2^-100 is
+    stored as zeros; one with an infinity or no number reads back as no numbers.
+
+    qkv [N, at least (n_heads + 2 n_kv_heads) * d] (float32 or bfloat16, columns behind them are not read); block_table
+    int32 [R, max_pages].  A row whose position lies outside the rotation tables is left out
+    (:func:`few_bits_faults`); a row whose page is not in the cache writes its query only."""
+    act = q_out.dtype
+    ld = _need_rows(qkv, "qkv", (act,))
+    _need(q_out, "q_out", _BF16_F32, 3)
+    _need(positions, "positions", _I, 1)
+    _need(row_request, "row_request", _I, 1)
+    _need(block_table, "block_table", _I, 2)
+    n, cols = qkv.shape[0], (n_heads + 2 * n_kv_heads) * head_dim
+    n_pages, nkv, page_size, d = pages.k.shape
+    if qkv.shape[1] < cols or q_out.shape != (n, n_heads, head_dim) or positions.shape[0] != n or row_request.shape[0] != n \
+            or (nkv, d) != (n_kv_heads, head_dim):
+        raise KernelError(f"qk_norm_rope_store_kv8: qkv {tuple(qkv.shape)} (want {cols} columns), q_out {tuple(q_out.shape)}, "
+                          f"positions {tuple(positions.shape)}, pages {tuple(pages.k.shape)}")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        _need(w, "norm weight", _W, 1)
+        if w.shape[0] != head_dim or w.dtype != weights[0].dtype:
+            raise KernelError(f"qk_norm_rope_store_kv8: norm weights of {head_dim} numbers of one type, got {tuple(w.shape)}, "
+                              f"{w.dtype}")
+    if rot_dim:
+        _need(cos, "cos", (torch.float32,), 2)
+        _need(sin, "sin", (torch.float32,), 2)
+        if cos.shape[1] != rot_dim // 2 or sin.shape != cos.shape or rot_dim % 2 or not 0 < rot_dim <= head_dim:
+            raise KernelError(f"rotation tables {tuple(cos.shape)} do not match rot_dim {rot_dim}")
+    _check(_few_bits().ib_qk_norm_rope_store_kv8(
+        qkv.data_ptr(), act == torch.float32, ld, n, n_heads, n_kv_heads, head_dim, _p(q_weight), _p(k_weight),
+        bool(weights) and weights[0].dtype == torch.float32, int(q_weight is not None) | int(k_weight is not None) << 1,
+        float(eps), cos.data_ptr() if rot_dim else None, sin.data_ptr() if rot_dim else None, rot_dim, int(bool(interleaved)),
+        cos.shape[0] if rot_dim else 0, positions.data_ptr(), row_request.data_ptr(), block_table.data_ptr(),
+        block_table.shape[1], page_size, n_pages, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),
+        pages.v_scale.data_ptr(), q_out.data_ptr(), _stream()), "qk_norm_rope_store_kv8")
+
+
+def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Tensor, row_request: torch.Tensor,
+                        positions: torch.Tensor, scale: float, window: Optional[int], out: torch.Tensor, max_kv_len: int):
+    """out[r, h*d:(h+1)*d] = attention of row r's head h over its request's cached keys in 8 bits up to positions[r].
+    ``window``: see :func:`span_argument`.  ``max_kv_len``: no position is beyond it; how the keys are cut goes by it.  A row
+    that sees no key (a negative position, a request without pages) gets zeros.  The rows of ``out`` may lie apart."""
+    act = out.dtype
+    _need(q, "q", (act,), 3)
+    out_ld = _need_rows(out, "out", _BF16_F32)
+    _need(block_table, "block_table", _I, 2)
+    _need(row_request, "row_request", _I, 1)
+    _need(positions, "positions", _I, 1)
+    n, nh, d = q.shape
+    n_pages, nkv, page_size, dk = pages.k.shape
+    if dk != d or nh % nkv or out.shape != (n, nh * d) or row_request.shape[0] != n or positions.shape[0] != n:
+        raise KernelError(f"paged_attention_kv8: q {tuple(q.shape)}, pages {tuple(pages.k.shape)}, out {tuple(out.shape)}, "
+                          f"positions {tuple(positions.shape)}")
+    code = _few_bits().ib_paged_attention_kv8_generic(
+        q.data_ptr(), act == torch.float32, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),
+        pages.v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, n_pages, block_table.shape[0],
+        row_request.data_ptr(), positions.data_ptr(), n, nh, nkv, d, float(scale), int(window) if window else 0,
+        out.data_ptr(), out_ld, _stream())
+    if code == -1:
+        raise KernelError(f"paged_attention_kv8 takes heads of up to 512 numbers, got {d}")
+    _check(code, "paged_attention_kv8")
+
+
+# names of the words that :func:`few_bits_faults` reads
+FEW_BITS_WORDS = ("a row's position outside the rotation tables (8-bit cache)",)
+
+
+def few_bits_faults(reset: bool = True) -> dict:
+    """The error words of the kernels in few bits that are set, {name: value} (a row: its number plus one).  Waits for
+    the device; empty where the library was never needed."""
+    if _FEW_BITS_LIB is None:
+        return {}
+    values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)),)
+    return {name: v for name, v in zip(FEW_BITS_WORDS, values) if v}
 
 
 # ---- the kernels' error words, all of them ------------------------------------------------------------------
