@@ -50,6 +50,38 @@ __device__ __forceinline__ float code_value(unsigned c) {
     return c & 8u ? -v : v;
 }
 
+// eight neighbours of a row (zeros behind the first n), 16 bytes at a time where the rows allow it
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, bool wide, float (&v)[8]);
+template <> __device__ __forceinline__ void load8<float>(const float* p, int n, bool wide, float (&v)[8]) {
+    if (wide && n >= 8) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+    }
+}
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, int n, bool wide, float (&v)[8]) {
+    if (wide && n >= 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
+    }
+}
+// the bits of the largest magnitude of a block of 32 of which four neighbouring lanes hold eight numbers each; no number
+// counts as larger than an infinity
+__device__ __forceinline__ unsigned block_largest(const float (&v)[8]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+
 // ---- 8-bit keys and values ----------------------------------------------------------------------------------------------
 // four numbers as e4m3 codes, nearest with ties to even, beyond 448 as 448 (no number stays none)
 __device__ __forceinline__ unsigned codes8x4(float a, float b, float c, float d) {
@@ -67,6 +99,21 @@ __device__ __forceinline__ unsigned values8x2(unsigned short c) {
 __device__ __forceinline__ float value8(unsigned char c) {
     const unsigned v = values8x2(c);
     return __low2float(*reinterpret_cast<const __half2*>(&v));
+}
+// Numbers as pieces (see gemm_mx4.cu): the first piece's scale byte of a block from the bits of its largest magnitude (the
+// largest then lies in 128 .. 256; every further piece's byte is five less, down to 0), and eight numbers' next piece, in
+// whose place 32 times what it leaves of them stays.
+template <int PARTS> __device__ __forceinline__ unsigned pieces_byte(unsigned largest_bits) {
+    const int e = (int)(largest_bits >> 23);
+    return e == 255 ? 255u : (unsigned)max(e - 7, 5 * (PARTS - 1));
+}
+__device__ __forceinline__ uint2 take_piece(float (&v)[8]) {
+    uint2 c;
+    c.x = codes8x4(v[0], v[1], v[2], v[3]);
+    c.y = codes8x4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 32.0f * (v[j] - value8((unsigned char)((j < 4 ? c.x : c.y) >> (8 * (j & 3)))));
+    return c;
 }
 // What a vector with the largest magnitude `a` is multiplied by before its numbers are rounded, and its scale.  A vector
 // whose numbers are all below 2^-100 counts as zeros; one with an infinity or no number reads back as no numbers.

@@ -2404,8 +2404,10 @@ _FEW_BITS_LIB, _FEW_BITS_PDL = None, False
 _FEW_BITS_SIGNATURES = {
     "ib_quantize_mx4": [c_void_p, c_int, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "ib_dequantize_mx4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_long, c_void_p],
-    "ib_product_mx4": [c_void_p, c_int, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_long,
-                       c_void_p],
+    "ib_gemm_mx4": [c_void_p, c_int, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_long,
+                    c_void_p, c_int, c_void_p],
+    "ib_gemm_mx4_error": [c_int],
+    "ib_gemm_mx4_error_async": [c_void_p, c_void_p],
     "ib_qk_norm_rope_store_kv8": [c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float,
                                   c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -2425,6 +2427,8 @@ def _few_bits():
         for fn, args in _FEW_BITS_SIGNATURES.items():
             getattr(lib, fn).argtypes = args
             getattr(lib, fn).restype = c_int
+        lib.ib_gemm_mx4_workspace.argtypes = [c_int, c_int, c_int]
+        lib.ib_gemm_mx4_workspace.restype = c_long
         lib.ib_few_bits_set_pdl.argtypes = [c_int]
         lib.ib_few_bits_set_pdl.restype = None
         lib.ib_few_bits_set_pdl(int(_FEW_BITS_PDL))
@@ -2518,9 +2522,12 @@ def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor):
     if k != w.width or out.shape != (n, w.rows):
         raise KernelError(f"linear_mx4: x {(n, k)}, w {w.shape}, out {tuple(out.shape)}")
     kind = 2 if coded else int(x.dtype == torch.float32)
-    _check(_few_bits().ib_product_mx4((x.codes if coded else x).data_ptr(), kind, ldx, x.scales.data_ptr() if coded else None,
-                                      w.codes.data_ptr(), w.scales.data_ptr(), n, w.rows, k, out.data_ptr(),
-                                      out.dtype == torch.float32, ldy, _stream()), "linear_mx4")
+    lib, workspace = _few_bits(), None
+    if not coded:
+        workspace = torch.empty((lib.ib_gemm_mx4_workspace(kind, n, k),), dtype=torch.uint8, device=out.device)
+    _check(lib.ib_gemm_mx4((x.codes if coded else x).data_ptr(), kind, ldx, x.scales.data_ptr() if coded else None,
+                           w.codes.data_ptr(), w.scales.data_ptr(), n, w.rows, k, out.data_ptr(), out.dtype == torch.float32, ldy,
+                           None if coded else workspace.data_ptr(), 0, _stream()), "linear_mx4")
 
 
 @dataclass
@@ -2625,7 +2632,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
 
 
 # names of the words that :func:`few_bits_faults` reads
-FEW_BITS_WORDS = ("a row's position outside the rotation tables (8-bit cache)",)
+FEW_BITS_WORDS = ("a row's position outside the rotation tables (8-bit cache)", "matrix product (4-bit weights)")
 
 
 def few_bits_faults(reset: bool = True) -> dict:
@@ -2633,7 +2640,7 @@ def few_bits_faults(reset: bool = True) -> dict:
     the device; empty where the library was never needed."""
     if _FEW_BITS_LIB is None:
         return {}
-    values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)),)
+    values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)), _FEW_BITS_LIB.ib_gemm_mx4_error(int(reset)))
     return {name: v for name, v in zip(FEW_BITS_WORDS, values) if v}
 
 
