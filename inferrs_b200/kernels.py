@@ -2414,6 +2414,9 @@ _FEW_BITS_SIGNATURES = {
     "ib_paged_attention_kv8_generic": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                        c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_long,
                                        c_void_p],
+    "ib_paged_attention_kv8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                               c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                               c_void_p, c_long, c_int, c_int, c_void_p],
     "ib_kv8_row_fault": [c_int],
     "ib_kv8_row_fault_async": [c_void_p, c_void_p],
 }
@@ -2605,11 +2608,26 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
         pages.v_scale.data_ptr(), q_out.data_ptr(), _stream()), "qk_norm_rope_store_kv8")
 
 
+KV8_HEAD_DIMS = (64, 128, 256)   # head sizes that the tensor cores' kernel takes
+
+
+def kv8_tile_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Tokens of a prompt that a tile of :func:`paged_attention_kv8` holds at most: 32 (token, head) pairs of a key/value head,
+    16 with heads of 256."""
+    return max(1, (16 if head_dim == 256 else 32) // (n_heads // n_kv_heads))
+
+
 def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Tensor, row_request: torch.Tensor,
-                        positions: torch.Tensor, scale: float, window: Optional[int], out: torch.Tensor, max_kv_len: int):
+                        positions: torch.Tensor, scale: float, window: Optional[int], out: torch.Tensor, max_kv_len: int,
+                        tiles=None):
     """out[r, h*d:(h+1)*d] = attention of row r's head h over its request's cached keys in 8 bits up to positions[r].
     ``window``: see :func:`span_argument`.  ``max_kv_len``: no position is beyond it; how the keys are cut goes by it.  A row
-    that sees no key (a negative position, a request without pages) gets zeros.  The rows of ``out`` may lie apart."""
+    that sees no key (a negative position, a request without pages) gets zeros.  The rows of ``out`` may lie apart.
+
+    bfloat16 heads of 64, 128 and 256 numbers run on the tensor cores, the rest in float32 one row and head at a time.
+    ``tiles`` = (tile_req, tile_row0, n_tiles, q_start, tokens) lets rows of one request share what they read: tile i holds
+    up to ``tokens`` (at most :func:`kv8_tile_tokens`) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
+    request r's rows end at q_start[r + 1]."""
     act = out.dtype
     _need(q, "q", (act,), 3)
     out_ld = _need_rows(out, "out", _BF16_F32)
@@ -2621,11 +2639,29 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     if dk != d or nh % nkv or out.shape != (n, nh * d) or row_request.shape[0] != n or positions.shape[0] != n:
         raise KernelError(f"paged_attention_kv8: q {tuple(q.shape)}, pages {tuple(pages.k.shape)}, out {tuple(out.shape)}, "
                           f"positions {tuple(positions.shape)}")
-    code = _few_bits().ib_paged_attention_kv8_generic(
-        q.data_ptr(), act == torch.float32, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),
-        pages.v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, n_pages, block_table.shape[0],
-        row_request.data_ptr(), positions.data_ptr(), n, nh, nkv, d, float(scale), int(window) if window else 0,
-        out.data_ptr(), out_ld, _stream())
+    n_req, max_pages = block_table.shape
+    span = int(window) if window else 0
+    lib, stream = _few_bits(), _stream()
+    code = -1
+    if act == torch.bfloat16 and d in KV8_HEAD_DIMS:
+        tile_req = tile_row0 = q_start = None
+        n_tiles, tokens = n, 1
+        if tiles is not None:
+            tile_req, tile_row0, n_tiles, q_start, tokens = tiles
+            for name, t in (("tile_req", tile_req), ("tile_row0", tile_row0), ("q_start", q_start)):
+                _need(t, name, _I, 1)
+            if min(tile_req.shape[0], tile_row0.shape[0]) < n_tiles or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d):
+                raise KernelError(f"paged_attention_kv8: {n_tiles} tiles of {tokens} tokens in lists of {tile_req.shape[0]}")
+        code = lib.ib_paged_attention_kv8(
+            q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
+            block_table.data_ptr(), max_pages, page_size, n_pages, n_req, row_request.data_ptr(), positions.data_ptr(), n,
+            _p(tile_req), _p(tile_row0), _p(q_start), n_tiles, tokens, nh, nkv, d, float(scale), span, out.data_ptr(), out_ld, 0,
+            int(max_kv_len), stream)
+    if code == -1:
+        code = lib.ib_paged_attention_kv8_generic(
+            q.data_ptr(), act == torch.float32, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),
+            pages.v_scale.data_ptr(), block_table.data_ptr(), max_pages, page_size, n_pages, n_req, row_request.data_ptr(),
+            positions.data_ptr(), n, nh, nkv, d, float(scale), span, out.data_ptr(), out_ld, stream)
     if code == -1:
         raise KernelError(f"paged_attention_kv8 takes heads of up to 512 numbers, got {d}")
     _check(code, "paged_attention_kv8")

@@ -468,3 +468,31 @@ def test_on_a_stream_of_its_own_and_in_a_captured_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, (y, y4, out)))
+
+
+@pytest.mark.parametrize("heads,kv,d,span", [(8, 2, 128, 0), (32, 8, 128, 20), (16, 16, 64, 0), (20, 4, 64, -16), (2, 1, 256, 0), (5, 1, 128, 7)])
+def test_attention_of_prompts_over_eight_bit_pages(heads, kv, d, span):
+    """Tiles of a prompt's tokens, some short, some places of the list without a tile, beside rows one by one."""
+    from inferrs_b200 import kernels as K
+    portions, cached = (37, 1, 12), (100, 5, 0)
+    lengths = [c + p for c, p in zip(cached, portions)]
+    pages, table = filled(lengths, kv, d, 16, 2)
+    n = sum(portions)
+    q = rand((n, heads, d), 3).bfloat16()
+    pos = torch.cat([torch.arange(c, c + p) for c, p in zip(cached, portions)]).int().cuda()
+    req = torch.cat([torch.full((p,), i) for i, p in enumerate(portions)]).int().cuda()
+    starts = [0, 37, 38, 50]
+    tokens = K.kv8_tile_tokens(heads, kv, d)
+    tile_list = [(i, r) for i in range(3) for r in range(starts[i], starts[i + 1], tokens)]
+    tile_list.insert(1, (-1, 0))
+    tile_req, tile_row0 = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in zip(*tile_list))
+    q_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    out, one = (torch.full((n, heads * d), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    scale = d ** -0.5
+    K.paged_attention_kv8(q, pages, table, req, pos, scale, span, out, max(lengths), tiles=(tile_req, tile_row0, len(tile_list), q_start, tokens))
+    K.paged_attention_kv8(q, pages, table, req, pos, scale, span, one, max(lengths))
+    want, weight, size = plain.attention(q, pages.k.double(), pages.v.double(), pages.k_scale.double(), pages.v_scale.double(),
+                                         table, req, pos, scale, span)
+    limit = attention_limit(want, weight, size, d, max(lengths), torch.bfloat16)
+    for got in (out, one):
+        assert bool(((got.double().view(n, heads, d) - want).abs() <= limit).all())
