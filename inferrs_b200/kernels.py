@@ -2624,7 +2624,8 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     ``window``: see :func:`span_argument`.  ``max_kv_len``: no position is beyond it; how the keys are cut goes by it.  A row
     that sees no key (a negative position, a request without pages) gets zeros.  The rows of ``out`` may lie apart.
 
-    bfloat16 heads of 64, 128 and 256 numbers run on the tensor cores, the rest in float32 one row and head at a time.
+    bfloat16 heads of 64, 128 and 256 numbers in pages of a multiple of 16 places run on the tensor cores, the rest in float32
+    one row and head at a time.
     ``tiles`` = (tile_req, tile_row0, n_tiles, q_start, tokens) lets rows of one request share what they read: tile i holds
     up to ``tokens`` (at most :func:`kv8_tile_tokens`) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
     request r's rows end at q_start[r + 1]."""
