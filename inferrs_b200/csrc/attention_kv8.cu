@@ -468,12 +468,30 @@ static int launch(const Args& a, int tiles, cudaStream_t stream) {
 // is a tile of its own (row_request says whose); else tile i holds up to tile_tokens rows of request tile_req[i] (-1: none)
 // from row tile_row0[i] on, and request r's rows end at q_start[r + 1].  splits: CTAs that share a tile's keys (1, 2, 4, 8, 16; 0: chosen here by max_len, which
 // no position is beyond).
-IB_EXPORT int ib_paged_attention_kv8(const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale,
-                                     const int* block_table, int max_pages, int page_size, int n_pages, int n_req,
-                                     const int* row_request, const int* positions, int n, const int* tile_req, const int* tile_row0,
-                                     const int* q_start, int n_tiles, int tile_tokens, int n_heads, int n_kv, int d, float scale, int span,
-                                     void* out, long out_ld, int splits, int max_len, cudaStream_t stream) {
+struct IbAttentionKv8 {
+    const void *q, *k_pages, *v_pages;
+    const float *k_scale, *v_scale;
+    const int *block_table, *row_request, *positions, *tile_req, *tile_row0, *q_start;
+    void* out;
+    cudaStream_t stream;
+    long max_pages, page_size, n_pages, n_req, n, n_tiles, tile_tokens, n_heads, n_kv, d, span, out_ld, splits, max_len;
+    double scale;
+};
+IB_EXPORT int ib_paged_attention_kv8(const IbAttentionKv8* c) {
     using namespace kv8;
+    if (c->n > 0x7FFFFFFF || c->n_heads > 65536 || c->max_pages > 0x7FFFFFFF || c->n_pages > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
+    const void *q = c->q, *k_pages = c->k_pages, *v_pages = c->v_pages;
+    const float *k_scale = c->k_scale, *v_scale = c->v_scale;
+    const int *block_table = c->block_table, *row_request = c->row_request, *positions = c->positions, *tile_req = c->tile_req,
+              *tile_row0 = c->tile_row0, *q_start = c->q_start;
+    void* out = c->out;
+    const cudaStream_t stream = c->stream;
+    const long out_ld = c->out_ld;
+    const int max_pages = (int)c->max_pages, page_size = (int)c->page_size, n_pages = (int)c->n_pages, n_req = (int)c->n_req, n = (int)c->n,
+              n_tiles = (int)c->n_tiles, n_heads = (int)c->n_heads, n_kv = (int)c->n_kv, d = (int)c->d, span = (int)c->span,
+              max_len = (int)(c->max_len < 0x7FFFFFFF ? c->max_len : 0x7FFFFFFF);
+    int tile_tokens = (int)c->tile_tokens, splits = (int)c->splits;
+    const float scale = (float)c->scale;
     if (n < 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || page_size <= 0 || splits < 0 || splits > 16 || (splits & (splits - 1))) return IB_ERR_ARGUMENT;
     if (d != 64 && d != 128 && d != 256) return IB_ERR_UNSUPPORTED;
     if ((long)n_pages * n_kv * page_size > 0x7FFFFFFFL || page_size % KEYS) return IB_ERR_UNSUPPORTED;

@@ -77,9 +77,20 @@ static inline int blocks_for(long threads) {
 }  // namespace few
 
 // x [rows, width] (float32 or bfloat16, rows ldx elements apart) to codes and scales
-IB_EXPORT int ib_quantize_mx4(const void* x, int x_is_f32, long ldx, int rows, int width, void* codes, void* scales,
-                              cudaStream_t stream) {
+struct IbQuantizeMx4 {
+    const void* x;
+    void *codes, *scales;
+    cudaStream_t stream;
+    long x_is_f32, ldx, rows, width;
+};
+IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     using namespace few;
+    if (q->rows > 0x7FFFFFFF || q->width > (1 << 24)) return IB_ERR_UNSUPPORTED;
+    const void* x = q->x;
+    void *codes = q->codes, *scales = q->scales;
+    const cudaStream_t stream = q->stream;
+    const long ldx = q->ldx;
+    const int x_is_f32 = (int)q->x_is_f32, rows = (int)q->rows, width = (int)q->width;
     if (rows < 0 || width <= 0 || ldx < width) return IB_ERR_ARGUMENT;
     if (rows == 0) return IB_OK;
     const size_t e = x_is_f32 ? 4 : 2;
@@ -94,6 +105,7 @@ IB_EXPORT int ib_dequantize_mx4(const void* codes, const void* scales, int rows,
                                 cudaStream_t stream) {
     using namespace few;
     if (rows < 0 || width <= 0 || ldo < width) return IB_ERR_ARGUMENT;
+    if (width > (1 << 24)) return IB_ERR_UNSUPPORTED;
     if (rows == 0) return IB_OK;
     const size_t e = out_is_f32 ? 4 : 2;
     const int wide = (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * e) % 16 == 0) ? 1 : 0;

@@ -15,9 +15,11 @@
 // TMA brings tiles of 128 weight rows and of tokens into a ring of 128-byte-swizzled stages (4-bit weights beside 8-bit
 // pieces are spread to a byte each on the way), and 512-byte tiles of scales, which the issuing thread copies into tensor
 // memory in front of the products that use them (every stage has its own columns, so none is overwritten early).
-// Accumulators are float32 in tensor memory.  Roles: warp 0 copies, warp 1 products, warps 2..5 read back.
+// Accumulators are float32 in tensor memory.  Roles: warp 0 copies, warp 1 products, warps 2..5 read back.  Up to eight
+// bfloat16 rows are brought to pieces inside the product, by warps 6..9 of every CTA while the weights stream in; more rows by
+// a kernel of their own, and the product starts while that one runs.
 //
-// With few output tiles K is cut over a cluster (1, 1, splits): every CTA sends its partial sums to their owners (each has
+// Where low tiles would keep the tensor core longer than the weights take, K is cut over a cluster (1, 1, splits): every CTA sends its partial sums to their owners (each has
 // an equal share of the tile's rows) through distributed shared memory, one cluster barrier follows, and the owner adds
 // them in the order of the ranks.  Every wait is bounded and reports through this file's error word.
 #include <cuda.h>
@@ -30,6 +32,7 @@ namespace mx4 {
 using namespace sm100;
 
 constexpr int BM = 128, THREADS = 192, A_BYTES = BM * 128;
+constexpr int INSIDE_ROWS = 8;        // up to so many bfloat16 rows are brought to pieces inside the product
 // what a kernel's rows are: the number of pieces of a number, CODES for 4-bit rows
 enum { CODES = 1, PIECES_BF16 = 2, PIECES_F32 = 5 };
 
@@ -44,6 +47,9 @@ struct Params {
     int y_is_f32, n_tok, n_out, num_kb;      // num_kb: stages that K takes
     const unsigned char *w_scales, *x_scales;
     int scale_tiles;                         // 128-column tiles of scales per 128 rows
+    const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
+    long ldx;
+    int k, wide;                             // wide: rows start on 16 bytes
 };
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -86,51 +92,195 @@ __device__ __forceinline__ void umma_scaled(unsigned d, unsigned long long a, un
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
 }
 
-// the plan of a kernel's shared and tensor memory
-template <int KIND, int BN, int STAGES> struct Plan {
-    static constexpr int TOKENS = BN / KIND;                            // of a tile
+// the plan of a stage's shared and tensor memory
+template <int KIND, int BN> struct Plan {
+    static constexpr int TOKENS = BN / KIND;                             // of a tile
     static constexpr int B_BYTES = BN * 128;
-    static constexpr int K_TILES = KIND != CODES ? 1 : 2;               // 128-column tiles of scales a stage
+    static constexpr int K_TILES = KIND != CODES ? 1 : 2;                // 128-column tiles of scales a stage
     static constexpr int B_GROUPS = (BN + 127) / 128;                    // 128-row tiles of scales
     static constexpr int SA_BYTES = 512 * K_TILES, SB_BYTES = 512 * K_TILES * B_GROUPS;
-    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
     static constexpr int SCALE_COLS = 4 * K_TILES * (1 + B_GROUPS);      // of tensor memory a stage
-    static constexpr int WANT = BN + STAGES * SCALE_COLS;
-    static constexpr int TMEM_COLS = WANT <= 32 ? 32 : WANT <= 64 ? 64 : WANT <= 128 ? 128 : WANT <= 256 ? 256 : 512;
-    static_assert(WANT <= 512, "tensor memory");
     static_assert(KIND != PIECES_F32 || BN == 80, "read back sixteen tokens at a time");
-    static constexpr bool SPLITS = TOKENS <= 64;                         // K may be cut over a cluster
-    static constexpr int RECV_BYTES = SPLITS ? TOKENS * BM * 4 : 0;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + RECV_BYTES + 16 * STAGES + 64 + 1024;
+    static constexpr int tmem_cols(int stages) {
+        int c = 32;
+        while (c < BN + stages * SCALE_COLS) c *= 2;
+        return c;
+    }
 };
 
-template <int KIND, int BN, int STAGES>
-__global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                       const __grid_constant__ CUtensorMap map_x, const Params p) {
-    using P = Plan<KIND, BN, STAGES>;
+__device__ __forceinline__ void store(const Params& p, int t, int f, float v) {
+    if (p.y_is_f32) reinterpret_cast<float*>(p.y)[(long)t * p.ldy + f] = v;
+    else reinterpret_cast<__nv_bfloat16*>(p.y)[(long)t * p.ldy + f] = __float2bfloat16_rn(v);
+}
+
+// One stage's products, issued by one thread: scales into the stage's columns of tensor memory (`scales`), then four products
+// of 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones.
+template <int KIND, int BN>
+__device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, unsigned char* a, unsigned char* b, unsigned char* sa_tile,
+                                               unsigned char* sb_tile, bool accumulate) {
+    using P = Plan<KIND, BN>;
+    constexpr unsigned FORMATS = KIND != CODES ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);   // e2m1 and e4m3, e2m1 twice
+    constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(BM >> 4) << 24);
+    fence_after();
+    const unsigned sa = scales, sb = sa + 4 * P::K_TILES;
+#pragma unroll
+    for (int j = 0; j < P::K_TILES; ++j) {
+        scales_to_tmem(sa + 4 * j, smem_u32(sa_tile + 512 * j));
+#pragma unroll
+        for (int g = 0; g < P::B_GROUPS; ++g)     // the column tiles one after the other, the row tiles of each side by side
+            scales_to_tmem(sb + 4 * (j * P::B_GROUPS + g), smem_u32(sb_tile + g * P::SA_BYTES + 512 * j));
+    }
+    const unsigned long long da = desc_k_major(smem_u32(a)), db = desc_k_major(smem_u32(b));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned tile = KIND != CODES ? 0 : k >> 1, id = KIND != CODES ? k : (k & 1) * 2;
+        umma_scaled<KIND>(tmem, da + 2 * k, db + 2 * k, IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile,
+                          accumulate || k != 0);
+    }
+}
+
+__device__ __forceinline__ unsigned f16_pair(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// two numbers (f16) to their first pieces and 32 times what they leave of them to the second ones
+__device__ __forceinline__ void two_pieces(unsigned v, unsigned short& first, unsigned short& second) {
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(first) : "r"(v));
+    const unsigned back = few::values8x2(first);
+    const __half2 k32 = __float2half2_rn(32.0f);
+    const __half2 left = __hmul2(k32, __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&back)));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(second) : "r"(*reinterpret_cast<const unsigned*>(&left)));
+}
+
+// ---- up to 64 rows: what counts is that every SM streams its share of the weights -----------------------------------------------
+// A tile may cover fewer rows of W than the product's 128 (a multiple of eight; what the tensor core reads beyond them belongs
+// to other tiles and its results are not stored), so that the tiles can be as many as the SMs, or twice as many.  Its scales are then
+// not a 512-byte tile of the matrix's: warps 6..9 put every fourth stage's together, and bring x's numbers to pieces where
+// the kernel does that itself.
+struct Shape {
+    int tile_rows, stages, splits, tmem_cols;
+};
+
+// What a helper warp holds of its next stage: four rows' words of scales a lane and K tile, and (INSIDE) eight numbers of every
+// other row of x: four threads have a block of 32, a warp two rows at a time.  The numbers go through f16, which holds a
+// bfloat16 number's eight bits from 256 down to 2^-17 and below that what the second piece may still need.
+template <int KIND, int BN, bool INSIDE>
+__device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, int row0, unsigned char* b_tiles, unsigned char* sa_tiles,
+                                            unsigned char* sb_tiles, int kb0, int nkb, unsigned full0, unsigned empty0) {
+    using P = Plan<KIND, BN>;
+    constexpr int PASSES = INSIDE ? P::TOKENS / 2 : 1;
+    const int lane = threadIdx.x & 31, g = lane & 15, rows = (p.n_out + 127) / 128 * 128 - row0;      // of scales there are
+    const unsigned* scales = reinterpret_cast<const unsigned*>(p.w_scales);
+    unsigned words[P::K_TILES][4];
+    auto fetch_scales = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < P::K_TILES; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = 32 * c + lane;
+                words[j][c] = i < nkb && r < sh.tile_rows && r < rows ? scales[few::scale_word(row0 + r, (kb0 + i) * P::K_TILES + j, p.scale_tiles)] : 0u;
+            }
+    };
+    // No more helpers than stages: a warp that has filled stage i knows the products of stage i - stages done; its next stage's
+    // place was last but one used by stage i + helpers - 2 stages, and only if that one is done too does the parity of the place's
+    // barrier say which use it speaks of.
+    const int helpers = sh.stages < 4 ? sh.stages : 4;
+    int i = (int)(threadIdx.x - THREADS) >> 5;
+    if (i >= helpers) return true;
+    fetch_scales(i);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    uint4 raw[PASSES];
+    const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(lane >> 4) * p.ldx + 8 * g);
+    auto fetch_x = [&](int i) {
+        const int c = (kb0 + i) * 128;
+#pragma unroll
+        for (int j = 0; j < PASSES; ++j) {
+            raw[j] = make_uint4(0, 0, 0, 0);
+            if (2 * j + (lane >> 4) >= p.n_tok || i >= nkb) continue;
+            const __nv_bfloat16* src = x + 2L * j * p.ldx + c;
+            const int n = p.k - c - 8 * g;
+            if (p.wide && n >= 8) {
+                raw[j] = *reinterpret_cast<const uint4*>(src);
+            } else {
+                unsigned short* to = reinterpret_cast<unsigned short*>(&raw[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (e < n) to[e] = *reinterpret_cast<const unsigned short*>(src + e);
+            }
+        }
+    };
+    if constexpr (INSIDE) fetch_x(i);
+    for (; i < nkb; i += helpers) {
+        const int s = i % sh.stages;
+        if (i >= sh.stages && !mbar_wait(empty0 + 8 * s, ((i / sh.stages) - 1) & 1, 4)) return false;
+#pragma unroll
+        for (int j = 0; j < P::K_TILES; ++j)
+            *reinterpret_cast<uint4*>(sa_tiles + s * P::SA_BYTES + 512 * j + 16 * lane) = make_uint4(words[j][0], words[j][1], words[j][2], words[j][3]);
+        fetch_scales(i + helpers);
+        if constexpr (INSIDE) {
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                if (2 * j >= p.n_tok) break;                  // columns of no token: whatever the stage holds
+                const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+                unsigned m = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7FFF7FFFu);
+                m = max(m & 0xFFFFu, m >> 16);
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const unsigned byte = few::pieces_byte<PIECES_BF16>(m << 16);
+                const float by = byte == 255u ? 0.0f : few::scale_reciprocal(byte);
+                unsigned short h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    two_pieces(byte == 255u ? 0u : f16_pair(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xFFFF0000u) * by), h[e], l[e]);
+                const int r = 2 * (2 * j + (lane >> 4));
+                unsigned char* to = b_tiles + s * P::B_BYTES + (g & 1) * 8;
+                *reinterpret_cast<uint2*>(to + r * 128 + ((g >> 1) ^ (r & 7)) * 16) = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+                *reinterpret_cast<uint2*>(to + (r + 1) * 128 + ((g >> 1) ^ ((r + 1) & 7)) * 16) = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
+                if ((lane & 3) == 0) {
+                    unsigned char* sc = sb_tiles + s * P::SB_BYTES + r * 16 + (g >> 2);
+                    sc[0] = (unsigned char)byte;
+                    sc[16] = (unsigned char)(byte == 255u ? 255u : byte - 5u);
+                }
+            }
+            fetch_x(i + helpers);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads them behind the barrier
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full0 + 8 * s);
+    }
+    return true;
+}
+
+// INSIDE: the kernel brings x's rows to pieces itself
+template <int KIND, int BN, bool INSIDE>
+__global__ void __launch_bounds__(THREADS + 128) few_rows_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                 const __grid_constant__ CUtensorMap map_x, const Params p, const Shape sh) {
+    using P = Plan<KIND, BN>;
     extern __shared__ unsigned char raw_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
-    unsigned char* a_tiles = smem;
-    unsigned char* b_tiles = a_tiles + STAGES * A_BYTES;
-    unsigned char* sa_tiles = b_tiles + STAGES * P::B_BYTES;
-    unsigned char* sb_tiles = sa_tiles + STAGES * P::SA_BYTES;
-    float* recv = reinterpret_cast<float*>(sb_tiles + STAGES * P::SB_BYTES);     // [rank of the sender][token][rows owned]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(reinterpret_cast<unsigned char*>(recv) + P::RECV_BYTES);
-    const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * STAGES + 1);
+    const int stages = sh.stages, splits = sh.splits, a_bytes = sh.tile_rows * 128;
+    unsigned char* b_tiles = smem;
+    unsigned char* a_tiles = b_tiles + stages * P::B_BYTES;
+    unsigned char* sa_tiles = a_tiles + stages * a_bytes;
+    unsigned char* sb_tiles = sa_tiles + stages * P::SA_BYTES;
+    float* recv = reinterpret_cast<float*>(sb_tiles + stages * P::SB_BYTES);     // [rank of the sender][token][rows owned]
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(reinterpret_cast<unsigned char*>(recv) + (splits > 1 ? P::TOKENS * sh.tile_rows * 4 : 0));
+    const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + stages), accum = smem_u32(bars + 2 * stages);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * stages + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile_f = blockIdx.x, tile_t = blockIdx.y, splits = gridDim.z;
+    const int row0 = blockIdx.x * sh.tile_rows, tile_t = blockIdx.y;
     const int kb0 = (int)((long)blockIdx.z * p.num_kb / splits), nkb = (int)((long)(blockIdx.z + 1) * p.num_kb / splits) - kb0;   // >= 1
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accum, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(sh.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
@@ -138,24 +288,153 @@ __global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ C
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
-    if (P::SPLITS && splits > 1) cluster_arrive();       // "this CTA runs": looked at before the first store to it
+    if (splits > 1) cluster_arrive();       // "this CTA runs": looked at before the first store to it
 
     if (warp == 0) {
         if (lane == 0) {
             const unsigned long long pol = policy_evict_first();
-            constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
+            const unsigned w_tx = KIND == CODES ? a_bytes : a_bytes / 2;     // what a tile of weights counts on its barrier
             auto load_w = [&](int i, int s) {
-                mbar_expect_tx(full0 + 8 * s, W_TX + P::B_BYTES + P::SA_BYTES + P::SB_BYTES);
-                tma_load_2d_hint(smem_u32(a_tiles + s * A_BYTES), &map_w, (kb0 + i) * 128, tile_f * BM, full0 + 8 * s, pol);
-                bulk_load(smem_u32(sa_tiles + s * P::SA_BYTES), p.w_scales + ((long)tile_f * p.scale_tiles + (long)(kb0 + i) * P::K_TILES) * 512,
-                          P::SA_BYTES, full0 + 8 * s);
+                mbar_expect_tx(full0 + 8 * s, w_tx + (INSIDE ? 0 : P::B_BYTES + P::SB_BYTES));
+                tma_load_2d_hint(smem_u32(a_tiles + s * a_bytes), &map_w, (kb0 + i) * 128, row0, full0 + 8 * s, pol);
             };
             auto load_x = [&](int i, int s) {
+                if constexpr (INSIDE) return;
                 tma_load_2d(smem_u32(b_tiles + s * P::B_BYTES), &map_x, (kb0 + i) * 128, tile_t * BN, full0 + 8 * s);
 #pragma unroll
                 for (int g = 0; g < P::B_GROUPS; ++g)
                     bulk_load(smem_u32(sb_tiles + s * P::SB_BYTES + g * P::SA_BYTES),
                               p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)(kb0 + i) * P::K_TILES) * 512,
+                              P::SA_BYTES, full0 + 8 * s);
+            };
+            const int head = nkb < stages ? nkb : stages;    // the first weights are on their way before the kernel ahead is done
+            for (int i = 0; i < head; ++i) load_w(i, i);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int i = 0; i < head; ++i) load_x(i, i);
+            for (int i = head; i < nkb; ++i) {
+                const int s = i % stages;
+                if (!mbar_wait(empty0 + 8 * s, ((i / stages) - 1) & 1, 1)) { ok = false; break; }
+                load_w(i, s);
+                load_x(i, s);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            for (int i = 0; i < nkb; ++i) {
+                const int s = i % stages;
+                if (!mbar_wait(full0 + 8 * s, (i / stages) & 1, 2)) { ok = false; break; }
+                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a_tiles + s * a_bytes, b_tiles + s * P::B_BYTES,
+                                         sa_tiles + s * P::SA_BYTES, sb_tiles + s * P::SB_BYTES, i != 0);
+                umma_commit(empty0 + 8 * s);
+            }
+            umma_commit(accum);
+        }
+    } else if (warp >= 6) {
+        ok = fill_stages<KIND, BN, INSIDE>(p, sh, row0, b_tiles, sa_tiles, sb_tiles, kb0, nkb, full0, empty0);
+    }
+
+    const int q = warp & 3, row = q * 32 + lane;
+    const unsigned rank = blockIdx.z;
+    const int owned = sh.tile_rows / splits;           // rows of the tile that a CTA of the cluster adds up and stores
+    const int t0 = tile_t * P::TOKENS, tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
+    const int rows = p.n_out - row0 < sh.tile_rows ? p.n_out - row0 : sh.tile_rows;
+    if (splits > 1) cluster_wait();
+    if (warp >= 2 && warp < 6) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the kernel ahead
+        ok = mbar_wait(accum, 0, 3);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_after();
+        if (ok && g_error == 0 && q * 32 < sh.tile_rows) {
+            constexpr int COLS = KIND == PIECES_F32 ? 80 : 16, STEP = COLS / KIND;     // accumulator columns at a time, their tokens
+#pragma unroll 1
+            for (int c = 0; c * STEP < tokens; ++c) {
+                float v[COLS / 16][16];
+#pragma unroll
+                for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + ((unsigned)(q * 32) << 16) + COLS * c + 16 * i, v[i]);
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) {
+                    float r = 0.0f;
+#pragma unroll
+                    for (int i = KIND - 1; i >= 0; --i) r += v[(KIND * j + i) / 16][(KIND * j + i) % 16];
+                    const int t = c * STEP + j;
+                    if (t >= tokens) break;
+                    if (splits > 1) {
+                        if (row < sh.tile_rows)
+                            st_remote_f32(smem_u32(recv + ((size_t)rank * P::TOKENS + t) * owned + row % owned), (unsigned)(row / owned), r);
+                    } else if (row < rows) {
+                        store(p, t0 + t, row0 + row, r);
+                    }
+                }
+            }
+        }
+    }
+    if (splits > 1) {
+        cluster_arrive();
+        cluster_wait();                      // every part of the rows that this CTA owns is in its shared memory
+        if (warp >= 2 && warp < 6 && g_error == 0) {
+            for (int i = (int)threadIdx.x - 64; i < tokens * owned; i += 128) {
+                const int t = i / owned, r = i % owned, f = (int)rank * owned + r;
+                if (f >= rows) continue;
+                float sum = 0.0f;
+                for (int part = 0; part < splits; ++part) sum += recv[((size_t)part * P::TOKENS + t) * owned + r];
+                store(p, t0 + t, row0 + f, sum);
+            }
+        }
+    }
+    // after a wait that ran out the copies in flight are given time to land before the shared memory is given back
+    if (!ok) for (const unsigned long long t = global_ns(); global_ns() - t < 20000000ull;) {}
+    fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.tmem_cols));
+}
+
+// ---- more rows ------------------------------------------------------------------------------------------------------------------
+template <int KIND, int BN, int STAGES>
+__global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                       const __grid_constant__ CUtensorMap map_x, const Params p) {
+    using P = Plan<KIND, BN>;
+    extern __shared__ unsigned char raw_smem[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
+    unsigned char* a_tiles = smem;
+    unsigned char* b_tiles = a_tiles + STAGES * A_BYTES;
+    unsigned char* sa_tiles = b_tiles + STAGES * P::B_BYTES;
+    unsigned char* sb_tiles = sa_tiles + STAGES * P::SA_BYTES;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sb_tiles + STAGES * P::SB_BYTES);
+    const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * STAGES + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_f = blockIdx.x, tile_t = blockIdx.y, nkb = p.num_kb;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        mbar_init(accum, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::tmem_cols(STAGES)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const unsigned tmem = *tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
+            auto load_w = [&](int i, int s) {
+                mbar_expect_tx(full0 + 8 * s, W_TX + P::SA_BYTES + P::B_BYTES + P::SB_BYTES);
+                tma_load_2d(smem_u32(a_tiles + s * A_BYTES), &map_w, i * 128, tile_f * BM, full0 + 8 * s);
+                bulk_load(smem_u32(sa_tiles + s * P::SA_BYTES), p.w_scales + ((long)tile_f * p.scale_tiles + (long)i * P::K_TILES) * 512,
+                          P::SA_BYTES, full0 + 8 * s);
+            };
+            auto load_x = [&](int i, int s) {
+                tma_load_2d(smem_u32(b_tiles + s * P::B_BYTES), &map_x, i * 128, tile_t * BN, full0 + 8 * s);
+#pragma unroll
+                for (int g = 0; g < P::B_GROUPS; ++g)
+                    bulk_load(smem_u32(sb_tiles + s * P::SB_BYTES + g * P::SA_BYTES),
+                              p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)i * P::K_TILES) * 512,
                               P::SA_BYTES, full0 + 8 * s);
             };
             const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
@@ -171,79 +450,35 @@ __global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ C
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr unsigned FORMATS = KIND != CODES ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);   // e2m1 and e4m3, e2m1 twice
-            constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(BM >> 4) << 24);
             for (int i = 0; i < nkb; ++i) {
                 const int s = i % STAGES;
                 if (!mbar_wait(full0 + 8 * s, (i / STAGES) & 1, 2)) { ok = false; break; }
-                fence_after();
-                const unsigned sa = tmem + BN + s * P::SCALE_COLS, sb = sa + 4 * P::K_TILES;
-#pragma unroll
-                for (int j = 0; j < P::K_TILES; ++j) {
-                    scales_to_tmem(sa + 4 * j, smem_u32(sa_tiles + s * P::SA_BYTES + 512 * j));
-#pragma unroll
-                    for (int g = 0; g < P::B_GROUPS; ++g)     // the column tiles one after the other, the row tiles of each side by side
-                        scales_to_tmem(sb + 4 * (j * P::B_GROUPS + g), smem_u32(sb_tiles + s * P::SB_BYTES + g * P::SA_BYTES + 512 * j));
-                }
-                const unsigned long long da = desc_k_major(smem_u32(a_tiles + s * A_BYTES));
-                const unsigned long long db = desc_k_major(smem_u32(b_tiles + s * P::B_BYTES));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {                 // 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones
-                    const unsigned tile = KIND != CODES ? 0 : k >> 1, id = KIND != CODES ? k : (k & 1) * 2;
-                    umma_scaled<KIND>(tmem, da + 2 * k, db + 2 * k, IDESC | (id << 4) | (id << 29), sa + 4 * tile,
-                                      sb + 4 * P::B_GROUPS * tile, (i | k) != 0);
-                }
+                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a_tiles + s * A_BYTES, b_tiles + s * P::B_BYTES,
+                                         sa_tiles + s * P::SA_BYTES, sb_tiles + s * P::SB_BYTES, i != 0);
                 umma_commit(empty0 + 8 * s);
             }
             umma_commit(accum);
         }
-    }
-
-    const int q = warp & 3, row = q * 32 + lane, feature = tile_f * BM + row;
-    const unsigned rank = blockIdx.z;
-    const int owned = BM / splits;           // rows of the tile that a CTA of the cluster adds up and stores
-    const int t0 = tile_t * P::TOKENS, tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
-    auto store = [&](int t, int f, float v) {
-        if (p.y_is_f32) reinterpret_cast<float*>(p.y)[(long)(t0 + t) * p.ldy + f] = v;
-        else reinterpret_cast<__nv_bfloat16*>(p.y)[(long)(t0 + t) * p.ldy + f] = __float2bfloat16_rn(v);
-    };
-    if (P::SPLITS && splits > 1) cluster_wait();
-    if (warp >= 2) {
+    } else {
+        const int q = warp & 3, feature = tile_f * BM + q * 32 + lane;
+        const int t0 = tile_t * P::TOKENS, tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
         asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the kernel ahead
         ok = mbar_wait(accum, 0, 3);
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
         if (ok && g_error == 0) {
-            constexpr int COLS = KIND == PIECES_F32 ? 80 : 16, STEP = COLS / KIND;     // accumulator columns at a time, their tokens
+            constexpr int STEP = 16 / KIND;     // tokens of sixteen columns
 #pragma unroll 1
             for (int c = 0; c * STEP < tokens; ++c) {
-                float v[COLS / 16][16];
-#pragma unroll
-                for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + ((unsigned)(q * 32) << 16) + COLS * c + 16 * i, v[i]);
+                float v[16];
+                tmem_ld16(tmem + ((unsigned)(q * 32) << 16) + 16 * c, v);
 #pragma unroll
                 for (int j = 0; j < STEP; ++j) {
                     float r = 0.0f;
 #pragma unroll
-                    for (int i = KIND - 1; i >= 0; --i) r += v[(KIND * j + i) / 16][(KIND * j + i) % 16];
-                    const int t = c * STEP + j;
-                    if (t >= tokens) break;
-                    if (P::SPLITS && splits > 1)
-                        st_remote_f32(smem_u32(recv + ((size_t)rank * P::TOKENS + t) * owned + row % owned), (unsigned)(row / owned), r);
-                    else if (feature < p.n_out) store(t, feature, r);
+                    for (int i = KIND - 1; i >= 0; --i) r += v[KIND * j + i];
+                    if (c * STEP + j < tokens && feature < p.n_out) store(p, t0 + c * STEP + j, feature, r);
                 }
-            }
-        }
-    }
-    if (P::SPLITS && splits > 1) {
-        cluster_arrive();
-        cluster_wait();                      // every part of the rows that this CTA owns is in its shared memory
-        if (warp >= 2 && g_error == 0) {
-            for (int i = (int)threadIdx.x - 64; i < tokens * owned; i += 128) {
-                const int t = i / owned, r = i % owned, f = tile_f * BM + (int)rank * owned + r;
-                if (f >= p.n_out) continue;
-                float sum = 0.0f;
-                for (int part = 0; part < splits; ++part) sum += recv[((size_t)part * P::TOKENS + t) * owned + r];
-                store(t, f, sum);
             }
         }
     }
@@ -251,7 +486,7 @@ __global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ C
     if (!ok) for (const unsigned long long t = global_ns(); global_ns() - t < 20000000ull;) {}
     fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::TMEM_COLS));
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::tmem_cols(STAGES)));
 }
 
 // Where the scales of a row's first piece stand: the tiles of 80 columns that five pieces a number take have tiles of 128
@@ -300,53 +535,112 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base
     return r == CUDA_SUCCESS ? IB_OK : IB_ERR_UNSUPPORTED;
 }
 
-// How many CTAs share a tile's K: as many as run at once (two an SM up to 32 columns of tokens' pieces, one beyond), each
-// with at least two stages of it.
-static int splits_for(int tiles, int num_kb, int resident) {
-    int s = 1;
-    while (s < 8 && tiles * s * 2 <= 148 * resident && num_kb >= 4 * s) s *= 2;
+// the tensor maps of both operands: weights in boxes of box_w rows, x (not where it is brought to pieces inside) of box_x
+template <int KIND>
+static int make_maps(CUtensorMap* map_w, CUtensorMap* map_x, const void* w, const void* x, int n, int m, int k, int box_w, int box_x, Params& p) {
+    const long kp = (long)(k + 127) / 128 * 128;
+    p.scale_tiles = few::scale_tiles(k);
+    p.num_kb = (int)(KIND != CODES ? kp / 128 : (kp + 255) / 256);
+    int r = KIND != CODES ? make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, w, kp, m, kp / 2, 128, box_w)
+                          : make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, kp / 2, m, kp / 2, 128, box_w);
+    if (r || x == nullptr) { *map_x = *map_w; return r; }
+    return KIND != CODES ? make_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp, (long)KIND * n, kp, 128, box_x)
+                         : make_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp / 2, n, kp / 2, 128, box_x);
+}
+
+constexpr int SMS = 148, FEW_SMEM = 100 * 1024;      // of a CTA of the kernel for few rows: two share an SM
+
+// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA's tensor core takes
+// about a cycle per number of K for a tile of any height (half for 4-bit rows), the weights come at 44 bytes a cycle
+// and SM, and parts cost their meeting, about 2,800 cycles.
+template <int KIND, int BN>
+static Shape shape_for(int m, int num_kb, int tiles_t, int tile_rows, int splits) {
+    using P = Plan<KIND, BN>;
+    auto lowered = [](long rows) { return rows > 128 ? 128 : (int)(rows + 7) / 8 * 8; };
+    Shape s = {tile_rows > 0 ? tile_rows : 128, 1, splits > 0 ? splits : 1, 0};
+    if (tile_rows == 0 && splits == 0) {
+        long best = -1;
+        for (int parts = 1; parts <= 8 && (parts == 1 || 2 * parts <= num_kb); parts *= 2) {
+            const long rounds = ((long)(m + 127) / 128 * tiles_t * parts + SMS - 1) / SMS, columns = rounds * SMS / ((long)parts * tiles_t);
+            const int rows = lowered((m + columns - 1) / columns);
+            const long k_cycles = (long)num_kb * 128 / parts, bytes_cycles = (long)rows * num_kb * (KIND == CODES ? 136 : 68) / parts / 44;
+            const long cost = rounds * (k_cycles > bytes_cycles ? k_cycles : bytes_cycles) + (parts > 1 ? 2800 : 0);
+            if (best < 0 || cost < best) { best = cost; s.tile_rows = rows; s.splits = parts; }
+        }
+    }
+    const int stage = s.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES;
+    s.stages = (FEW_SMEM - 3072 - (s.splits > 1 ? P::TOKENS * s.tile_rows * 4 : 0)) / stage;
+    const int columns = (256 - BN) / P::SCALE_COLS;
+    s.stages = s.stages < columns ? s.stages : columns;
+    s.stages = s.stages < 16 ? s.stages : 16;
+    const int own = (num_kb + s.splits - 1) / s.splits;
+    s.stages = s.stages < own ? s.stages : own;
+    s.stages = s.stages < 1 ? 1 : s.stages;
+    s.tmem_cols = P::tmem_cols(s.stages);
     return s;
 }
 
-template <int KIND, int BN, int STAGES>
-static int launch(const void* w, const void* w_scales, const void* x, const void* x_scales, int n, int m, int k, Params p, int splits, cudaStream_t stream) {
-    using P = Plan<KIND, BN, STAGES>;
-    static IbDeviceSet done;
-    if (int r = ib_allow_dynamic_smem(done, gemm_kernel<KIND, BN, STAGES>, P::SMEM)) return r;
-    CUtensorMap map_w, map_x;
-    const long kp = (long)(k + 127) / 128 * 128;
-    int r;
-    if (KIND != CODES) {
-        if ((r = make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, w, kp, m, kp / 2, 128, BM))) return r;
-        if ((r = make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp, (long)KIND * n, kp, 128, BN))) return r;
-        p.num_kb = (int)(kp / 128);
-    } else {
-        if ((r = make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, kp / 2, m, kp / 2, 128, BM))) return r;
-        if ((r = make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp / 2, n, kp / 2, 128, BN))) return r;
-        p.num_kb = (int)((kp + 255) / 256);
-    }
-    p.w_scales = (const unsigned char*)w_scales;
-    p.x_scales = (const unsigned char*)x_scales;
-    p.scale_tiles = few::scale_tiles(k);
-    const int tiles_f = (m + BM - 1) / BM, tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
+template <int KIND, int BN, bool INSIDE>
+static int launch_few(const void* w, const void* x, int n, int m, int k, Params p, int tile_rows, int splits, cudaStream_t stream, bool early) {
+    using P = Plan<KIND, BN>;
+    const int tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
     if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
-    if (!P::SPLITS || tiles_t > 1) splits = 1;
-    else if (splits <= 0) splits = splits_for(tiles_f, p.num_kb, P::SMEM <= 113 * 1024 ? 2 : 1);
-    if (splits > 8 || splits > p.num_kb || BM % splits) return IB_ERR_ARGUMENT;
+    const Shape sh = shape_for<KIND, BN>(m, (k + (KIND == CODES ? 255 : 127)) / (KIND == CODES ? 256 : 128), tiles_t, tile_rows, splits);
+    CUtensorMap map_w, map_x;
+    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, sh.tile_rows, BN, p)) return r;
+    if (sh.splits > 8 || sh.splits > p.num_kb || sh.tile_rows % sh.splits) return IB_ERR_ARGUMENT;
+    size_t smem = 1024 + (size_t)sh.stages * (sh.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) +
+                  (sh.splits > 1 ? P::TOKENS * sh.tile_rows * 4 : 0) + 16 * sh.stages + 64;
+    // the products read 128 rows of A from where the last stage's tile starts, and no less than 128 rows of B are kept readable
+    const size_t a_end = 1024 + (size_t)sh.stages * P::B_BYTES + (size_t)(sh.stages - 1) * sh.tile_rows * 128 + A_BYTES;
+    const size_t b_end = 1024 + (size_t)(sh.stages - 1) * P::B_BYTES + 128 * 128;
+    smem = smem < a_end ? a_end : smem;
+    smem = smem < b_end ? b_end : smem;
+    // no more CTAs on an SM than have their columns of tensor memory at once: CTAs of clusters that wait for columns could wait
+    // for one another
+    const size_t alone = (size_t)227 * 1024 / (512 / sh.tmem_cols + 1) + 1;
+    smem = smem < alone ? alone : smem;
+    static IbDeviceSet done;
+    if (int r = ib_allow_dynamic_smem(done, few_rows_kernel<KIND, BN, INSIDE>, 200 * 1024)) return r;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles_f, tiles_t, splits);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = P::SMEM;
+    cfg.gridDim = dim3((m + sh.tile_rows - 1) / sh.tile_rows, tiles_t, sh.splits);
+    cfg.blockDim = dim3(THREADS + 128);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = splits;
+    attr[0].val.clusterDim.z = sh.splits;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ib_pdl_enabled ? 2 : 1;
+    cfg.numAttrs = ib_pdl_enabled || early ? 2 : 1;      // early: the kernel ahead is pieces_kernel
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<KIND, BN, INSIDE>, map_w, map_x, p, sh);
+    return e == cudaSuccess ? ib_launch_status() : (int)e;
+}
+
+template <int KIND, int BN, int STAGES>
+static int launch(const void* w, const void* x, int n, int m, int k, Params p, cudaStream_t stream, bool early) {
+    using P = Plan<KIND, BN>;
+    static_assert(BN + STAGES * P::SCALE_COLS <= 512, "tensor memory");
+    constexpr size_t SMEM = (size_t)STAGES * (A_BYTES + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) + 16 * STAGES + 64 + 1024;
+    static IbDeviceSet done;
+    if (int r = ib_allow_dynamic_smem(done, gemm_kernel<KIND, BN, STAGES>, SMEM)) return r;
+    const int tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
+    if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
+    CUtensorMap map_w, map_x;
+    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, BM, BN, p)) return r;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((m + BM - 1) / BM, tiles_t);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ib_pdl_enabled || early ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, p);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
@@ -354,11 +648,10 @@ static int launch(const void* w, const void* w_scales, const void* x, const void
 static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((k + 127) / 128 * 128) + 511) / 512 * 512; }
 
 template <typename T, int PARTS>
-static int make_pieces(const void* x, long ldx, int n, int k, unsigned char* pieces, unsigned char* scales, cudaStream_t stream) {
-    const int wide = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * sizeof(T) % 16 == 0) ? 1 : 0;
+static int make_pieces(const void* x, long ldx, int n, int k, int wide, unsigned char* pieces, cudaStream_t stream) {
     const long threads = (long)n * ((k + 127) / 128 * 16), blocks = (threads + 255) / 256;
     ib_launch(pieces_kernel<T, PARTS>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide,
-              (uint2*)pieces, (unsigned*)scales);
+              (uint2*)pieces, (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }
 
@@ -380,42 +673,61 @@ IB_EXPORT int ib_gemm_mx4_error_async(int* out, cudaStream_t stream) {
 
 // the bytes of workspace that ib_gemm_mx4 wants: pieces, then their scales (from a multiple of 512 on)
 IB_EXPORT long ib_gemm_mx4_workspace(int x_kind, int n, int k) {
-    if (x_kind == 2) return 0;
+    if (x_kind == 2 || (x_kind == 0 && n <= mx4::INSIDE_ROWS)) return 0;
     const long scale_rows = x_kind == 1 ? (n + 15) / 16 * 128L : (2L * n + 255) / 256 * 256;      // whole tiles of tokens
     return mx4::pieces_bytes(x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16, n, k) + scale_rows / 128 * few::scale_tiles(k) * 512;
 }
 
 // y [n, m] = x w^T.  x_kind 0: bfloat16 rows, 1: float32 rows (both ldx elements apart, `workspace` on 16 bytes), 2: a 4-bit
-// matrix (x its codes, x_scales its scales).  splits: CTAs that share a tile's K (0: chosen here; 1, 2, 4, 8).
-IB_EXPORT int ib_gemm_mx4(const void* x, int x_kind, long ldx, const void* x_scales, const void* w, const void* w_scales, int n, int m,
-                          int k, void* y, int y_is_f32, long ldy, void* workspace, int splits, cudaStream_t stream) {
+// matrix (x its codes, x_scales its scales).  tile_rows: rows of w
+// a tile of the kernel for few rows (a multiple of 8 up to 128), splits: CTAs that share a tile's K (1, 2, 4, 8); both 0: chosen here.
+struct IbGemmMx4 {
+    const void *x, *x_scales, *w, *w_scales;
+    void *y, *workspace;
+    cudaStream_t stream;
+    long x_kind, ldx, n, m, k, y_is_f32, ldy, tile_rows, splits;
+};
+IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     using namespace mx4;
-    if (n < 0 || m < 0 || k <= 0 || ldy < m || x_kind < 0 || x_kind > 2 || ldx < k || splits < 0) return IB_ERR_ARGUMENT;
+    if (c->n > (1 << 24) || c->m > (1 << 24) || c->k > (1 << 24)) return IB_ERR_UNSUPPORTED;
+    const void *x = c->x, *x_scales = c->x_scales, *w = c->w, *w_scales = c->w_scales;
+    void *y = c->y, *workspace = c->workspace;
+    const cudaStream_t stream = c->stream;
+    const long ldx = c->ldx, ldy = c->ldy;
+    const int x_kind = (int)c->x_kind, n = (int)c->n, m = (int)c->m, k = (int)c->k, y_is_f32 = (int)c->y_is_f32, tile_rows = (int)c->tile_rows,
+              splits = (int)c->splits;
+    if (n < 0 || m < 0 || k <= 0 || ldy < m || x_kind < 0 || x_kind > 2 || ldx < k || splits < 0 || tile_rows < 0 || tile_rows > 128 || tile_rows % 8) return IB_ERR_ARGUMENT;
     if (n == 0 || m == 0) return IB_OK;
-    if (n > (1 << 24) || k > (1 << 24)) return IB_ERR_UNSUPPORTED;
     Params p = {};
     p.y = y;
     p.ldy = ldy;
     p.y_is_f32 = y_is_f32;
     p.n_tok = n;
     p.n_out = m;
+    p.x = x;
+    p.ldx = ldx;
+    p.k = k;
+    p.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_kind ? 4 : 2) % 16 == 0;
+    p.w_scales = (const unsigned char*)w_scales;
+    if (x_kind == 0 && n <= INSIDE_ROWS) return launch_few<PIECES_BF16, 16, true>(w, nullptr, n, m, k, p, tile_rows, splits, stream, false);
+    if (x_kind == 2) {
+        p.x_scales = (const unsigned char*)x_scales;
+        if (n <= 16) return launch_few<CODES, 16, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
+        if (n <= 32) return launch_few<CODES, 32, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
+        if (n <= 64) return launch_few<CODES, 64, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
+        if (n <= 128) return launch<CODES, 128, 4>(w, x, n, m, k, p, stream, false);
+        return launch<CODES, 256, 4>(w, x, n, m, k, p, stream, false);
+    }
     unsigned char* pieces = (unsigned char*)workspace;
-    if (x_kind == 0) {
-        unsigned char* scales = pieces + pieces_bytes(PIECES_BF16, n, k);
-        if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, pieces, scales, stream)) return r;
-        if (n <= 16) return launch<PIECES_BF16, 32, 4>(w, w_scales, pieces, scales, n, m, k, p, splits, stream);
-        if (n <= 32) return launch<PIECES_BF16, 64, 3>(w, w_scales, pieces, scales, n, m, k, p, splits, stream);
-        if (n <= 64) return launch<PIECES_BF16, 128, 5>(w, w_scales, pieces, scales, n, m, k, p, splits, stream);
-        return launch<PIECES_BF16, 256, 4>(w, w_scales, pieces, scales, n, m, k, p, splits, stream);
-    }
     if (x_kind == 1) {
-        unsigned char* scales = pieces + pieces_bytes(PIECES_F32, n, k);
-        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, pieces, scales, stream)) return r;
-        return launch<PIECES_F32, 80, 4>(w, w_scales, pieces, scales, n, m, k, p, splits, stream);
+        p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
+        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, p.wide, pieces, stream)) return r;
+        return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
     }
-    if (n <= 16) return launch<CODES, 16, 5>(w, w_scales, x, x_scales, n, m, k, p, splits, stream);
-    if (n <= 32) return launch<CODES, 32, 4>(w, w_scales, x, x_scales, n, m, k, p, splits, stream);
-    if (n <= 64) return launch<CODES, 64, 3>(w, w_scales, x, x_scales, n, m, k, p, splits, stream);
-    if (n <= 128) return launch<CODES, 128, 4>(w, w_scales, x, x_scales, n, m, k, p, splits, stream);
-    return launch<CODES, 256, 4>(w, w_scales, x, x_scales, n, m, k, p, splits, stream);
+    p.x_scales = pieces + pieces_bytes(PIECES_BF16, n, k);
+    if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, p.wide, pieces, stream)) return r;
+    if (n <= 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    if (n <= 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    if (n <= 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    return launch<PIECES_BF16, 256, 4>(w, pieces, n, m, k, p, stream, true);
 }

@@ -171,13 +171,31 @@ __global__ void __launch_bounds__(32 * SLOW_WARPS) kv8_attention_kernel(
 
 // The step's rows qkv [n, queries | keys | values of n_heads, n_kv, n_kv heads of d numbers] (float32 or bfloat16): per-head
 // norm (norm_flags: 1 queries, 2 keys) and rotation, queries to q_out, keys and values as 8-bit codes into their pages.
-IB_EXPORT int ib_qk_norm_rope_store_kv8(const void* qkv, int is_f32, long ldx, int n, int n_heads, int n_kv, int d,
-                                        const void* q_weight, const void* k_weight, int w_is_f32, int norm_flags, float eps,
-                                        const float* cos_table, const float* sin_table, int rot_dim, int interleaved, int table_rows,
-                                        const int* positions, const int* row_request, const int* block_table, int max_pages,
-                                        int page_size, int n_pages, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
-                                        void* q_out, cudaStream_t stream) {
+struct IbStoreKv8 {
+    const void *qkv, *q_weight, *k_weight;
+    const float *cos_table, *sin_table;
+    const int *positions, *row_request, *block_table;
+    void *k_pages, *v_pages;
+    float *k_scale, *v_scale;
+    void* q_out;
+    cudaStream_t stream;
+    long is_f32, ldx, n, n_heads, n_kv, d, w_is_f32, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages;
+    double eps;
+};
+IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
     using namespace few;
+    if (s->n > 0x7FFFFFFF || s->n_heads > 65536 || s->n_kv > 65536 || s->table_rows > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
+    const void *qkv = s->qkv, *q_weight = s->q_weight, *k_weight = s->k_weight;
+    const float *cos_table = s->cos_table, *sin_table = s->sin_table;
+    const int *positions = s->positions, *row_request = s->row_request, *block_table = s->block_table;
+    void *k_pages = s->k_pages, *v_pages = s->v_pages, *q_out = s->q_out;
+    float *k_scale = s->k_scale, *v_scale = s->v_scale;
+    const cudaStream_t stream = s->stream;
+    const long ldx = s->ldx;
+    const int is_f32 = (int)s->is_f32, n = (int)s->n, n_heads = (int)s->n_heads, n_kv = (int)s->n_kv, d = (int)s->d, w_is_f32 = (int)s->w_is_f32,
+              norm_flags = (int)s->norm_flags, rot_dim = (int)s->rot_dim, interleaved = (int)s->interleaved, table_rows = (int)s->table_rows,
+              max_pages = (int)s->max_pages, page_size = (int)s->page_size, n_pages = (int)s->n_pages;
+    const float eps = (float)s->eps;
     if (n < 0 || n_heads <= 0 || n_kv <= 0 || d <= 0 || d % 4 || d > 1024 || rot_dim < 0 || rot_dim > d || rot_dim % 2 || page_size <= 0) return IB_ERR_ARGUMENT;
     if (n == 0) return IB_OK;
     const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, eps};

@@ -8,6 +8,7 @@ functions: without a CUDA device, ``nvcc`` or a successful build they raise.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -215,10 +216,11 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _need_rows(t: torch.Tensor, name: str, dtypes) -> int:
     """Like :func:`_need` for a matrix whose rows may lie apart (columns of a wider one): the distance of two rows."""
-    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+    stride = t.stride()
+    if not (len(stride) == 2 and t.is_cuda and t.dtype in dtypes and stride[1] == 1 and stride[0] >= t.shape[1]):
         raise KernelError(f"{name} must be a CUDA matrix of {dtypes} with rows of neighbouring elements, got {t.dtype} "
                           f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.stride(0)
+    return stride[0]
 
 
 _W = (torch.float32, torch.bfloat16)
@@ -2402,25 +2404,35 @@ def gemm_chain_error(reset: bool = True) -> int:
 # ---- numbers in few bits: matrices of 4-bit numbers, keys and values in 8 bits (csrc/few_bits.cuh) ---------------------
 _FEW_BITS_LIB, _FEW_BITS_PDL = None, False
 _FEW_BITS_SIGNATURES = {
-    "ib_quantize_mx4": [c_void_p, c_int, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    "ib_quantize_mx4": [ctypes.c_char_p],
     "ib_dequantize_mx4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_long, c_void_p],
-    "ib_gemm_mx4": [c_void_p, c_int, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_long,
-                    c_void_p, c_int, c_void_p],
+    "ib_gemm_mx4": [ctypes.c_char_p],
     "ib_gemm_mx4_error": [c_int],
     "ib_gemm_mx4_error_async": [c_void_p, c_void_p],
-    "ib_qk_norm_rope_store_kv8": [c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float,
-                                  c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
-                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "ib_qk_norm_rope_store_kv8": [ctypes.c_char_p],
+    "ib_paged_attention_kv8": [ctypes.c_char_p],
     "ib_paged_attention_kv8_generic": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                        c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_long,
                                        c_void_p],
-    "ib_paged_attention_kv8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
-                               c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                               c_void_p, c_long, c_int, c_int, c_void_p],
     "ib_kv8_row_fault": [c_int],
     "ib_kv8_row_fault_async": [c_void_p, c_void_p],
 }
+# The calls of a decode step take their arguments as one structure of 8-byte fields (IbQuantizeMx4, IbGemmMx4, IbStoreKv8,
+# IbAttentionKv8 in csrc/), packed at once: ctypes converts single arguments at 0.12 us each, 3.3 us for a call of 28.
+_QUANTIZE_CALL = struct.Struct("=8q").pack
+_GEMM_CALL = struct.Struct("=16q").pack
+_STORE_CALL = struct.Struct("=28qd").pack
+_ATTENTION_CALL = struct.Struct("=27qd").pack
 _BF16_F32 = (torch.bfloat16, torch.float32)
+_F8, _F32, _I32 = torch.float8_e4m3fn, torch.float32, torch.int32
+
+
+def _lists(*tensors) -> bool:
+    """Whether all are lists of 32-bit integers on the GPU (what :func:`_need` asks, without saying which is not)."""
+    for t in tensors:
+        if not (t.dtype is _I32 and t.is_cuda and t.dim() == 1 and t.is_contiguous()):
+            return False
+    return True
 
 
 def _few_bits():
@@ -2459,8 +2471,10 @@ class Mx4Matrix:
     width: int
 
     def __post_init__(self):
-        _need(self.codes, "codes", (torch.uint8,), 2)
-        _need(self.scales, "scales", (torch.uint8,), 5)
+        c, s = self.codes, self.scales
+        if not (c.dtype is torch.uint8 and s.dtype is torch.uint8 and c.is_cuda and s.is_cuda and c.is_contiguous() and s.is_contiguous()):
+            _need(c, "codes", (torch.uint8,), 2)
+            _need(s, "scales", (torch.uint8,), 5)
         want = mx4_shapes(self.rows, self.width) if self.rows >= 0 and self.width > 0 else (None, None)
         if (tuple(self.codes.shape), tuple(self.scales.shape)) != want:
             raise KernelError(f"a 4-bit matrix [{self.rows}, {self.width}] has codes and scales of shapes {want}, got "
@@ -2499,8 +2513,8 @@ def quantize_mx4(x: torch.Tensor, out: Optional[Mx4Matrix] = None) -> Mx4Matrix:
         out = Mx4Matrix.empty(rows, width, x.device)
     elif out.shape != (rows, width):
         raise KernelError(f"quantize_mx4: x {(rows, width)} for a matrix {out.shape}")
-    _check(_few_bits().ib_quantize_mx4(x.data_ptr(), x.dtype == torch.float32, ld, rows, width, out.codes.data_ptr(),
-                                       out.scales.data_ptr(), _stream()), "quantize_mx4")
+    _check(_few_bits().ib_quantize_mx4(_QUANTIZE_CALL(x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), _stream(),
+                                                      x.dtype is torch.float32, ld, rows, width)), "quantize_mx4")
     return out
 
 
@@ -2514,23 +2528,28 @@ def dequantize_mx4(w: Mx4Matrix, out: torch.Tensor):
                                          out.dtype == torch.float32, ld, _stream()), "dequantize_mx4")
 
 
-def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor):
+MX4_INSIDE_ROWS = 8      # up to so many bfloat16 rows the product needs no workspace (INSIDE_ROWS in csrc/gemm_mx4.cu)
+
+
+def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: int = 0):
     """out = x @ w.T.  ``x`` is a tensor [rows, width] (float32 or bfloat16; its rows may lie apart), whose numbers keep
     their precision, or an :class:`Mx4Matrix`; sums are float32.  ``out`` [rows, features] may be float32 or bfloat16 and its
-    rows may lie apart."""
+    rows may lie apart.  Up to 64 rows (float32: any number) the kernel's tiles may be set: ``tile_rows`` rows of w (a multiple
+    of 8 up to 128) and ``splits`` CTAs that share K (1, 2, 4 or 8, a divisor of tile_rows); 0 lets the library choose."""
     ldy = _need_rows(out, "out", _BF16_F32)
     coded = isinstance(x, Mx4Matrix)
     ldx = x.width if coded else _need_rows(x, "x", _BF16_F32)
     n, k = x.shape
     if k != w.width or out.shape != (n, w.rows):
         raise KernelError(f"linear_mx4: x {(n, k)}, w {w.shape}, out {tuple(out.shape)}")
-    kind = 2 if coded else int(x.dtype == torch.float32)
-    lib, workspace = _few_bits(), None
-    if not coded:
+    kind = 2 if coded else int(x.dtype is torch.float32)
+    lib, workspace, at = _few_bits(), None, 0
+    if kind == 1 or (kind == 0 and n > MX4_INSIDE_ROWS):
         workspace = torch.empty((lib.ib_gemm_mx4_workspace(kind, n, k),), dtype=torch.uint8, device=out.device)
-    _check(lib.ib_gemm_mx4((x.codes if coded else x).data_ptr(), kind, ldx, x.scales.data_ptr() if coded else None,
-                           w.codes.data_ptr(), w.scales.data_ptr(), n, w.rows, k, out.data_ptr(), out.dtype == torch.float32, ldy,
-                           None if coded else workspace.data_ptr(), 0, _stream()), "linear_mx4")
+        at = workspace.data_ptr()
+    _check(lib.ib_gemm_mx4(_GEMM_CALL((x.codes if coded else x).data_ptr(), x.scales.data_ptr() if coded else 0, w.codes.data_ptr(),
+                                      w.scales.data_ptr(), out.data_ptr(), at, _stream(), kind, ldx, n, w.rows, k,
+                                      out.dtype is torch.float32, ldy, tile_rows, splits)), "linear_mx4")
 
 
 @dataclass
@@ -2544,7 +2563,14 @@ class Kv8Pages:
     v_scale: torch.Tensor
 
     def __post_init__(self):
-        for name, t in (("k", self.k), ("v", self.v)):
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        shape = k.shape
+        if k.dtype is _F8 and v.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and len(shape) == 4 and v.shape == shape \
+                and ks.shape == vs.shape == shape[:3] and shape[3] % 4 == 0 and k.is_cuda and v.is_cuda and ks.is_cuda and vs.is_cuda \
+                and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() \
+                and (k.data_ptr() | v.data_ptr()) % 16 == 0:
+            return
+        for name, t in (("k", self.k), ("v", self.v)):          # something is wrong: say what
             _need(t, name, (torch.float8_e4m3fn,), 4)
             if t.data_ptr() % 16:
                 raise KernelError(f"{name}: pages of 8-bit numbers start on 16 bytes")
@@ -2578,10 +2604,12 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
     (:func:`few_bits_faults`); a row whose page is not in the cache writes its query only."""
     act = q_out.dtype
     ld = _need_rows(qkv, "qkv", (act,))
-    _need(q_out, "q_out", _BF16_F32, 3)
-    _need(positions, "positions", _I, 1)
-    _need(row_request, "row_request", _I, 1)
-    _need(block_table, "block_table", _I, 2)
+    if not (_lists(positions, row_request) and act in _BF16_F32 and q_out.is_cuda and q_out.dim() == 3 and q_out.is_contiguous()
+            and block_table.dtype is _I32 and block_table.is_cuda and block_table.dim() == 2 and block_table.is_contiguous()):
+        _need(q_out, "q_out", _BF16_F32, 3)
+        _need(positions, "positions", _I, 1)
+        _need(row_request, "row_request", _I, 1)
+        _need(block_table, "block_table", _I, 2)
     n, cols = qkv.shape[0], (n_heads + 2 * n_kv_heads) * head_dim
     n_pages, nkv, page_size, d = pages.k.shape
     if qkv.shape[1] < cols or q_out.shape != (n, n_heads, head_dim) or positions.shape[0] != n or row_request.shape[0] != n \
@@ -2599,13 +2627,14 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
         _need(sin, "sin", (torch.float32,), 2)
         if cos.shape[1] != rot_dim // 2 or sin.shape != cos.shape or rot_dim % 2 or not 0 < rot_dim <= head_dim:
             raise KernelError(f"rotation tables {tuple(cos.shape)} do not match rot_dim {rot_dim}")
-    _check(_few_bits().ib_qk_norm_rope_store_kv8(
-        qkv.data_ptr(), act == torch.float32, ld, n, n_heads, n_kv_heads, head_dim, _p(q_weight), _p(k_weight),
-        bool(weights) and weights[0].dtype == torch.float32, int(q_weight is not None) | int(k_weight is not None) << 1,
-        float(eps), cos.data_ptr() if rot_dim else None, sin.data_ptr() if rot_dim else None, rot_dim, int(bool(interleaved)),
-        cos.shape[0] if rot_dim else 0, positions.data_ptr(), row_request.data_ptr(), block_table.data_ptr(),
-        block_table.shape[1], page_size, n_pages, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),
-        pages.v_scale.data_ptr(), q_out.data_ptr(), _stream()), "qk_norm_rope_store_kv8")
+    _check(_few_bits().ib_qk_norm_rope_store_kv8(_STORE_CALL(
+        qkv.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        cos.data_ptr() if rot_dim else 0, sin.data_ptr() if rot_dim else 0, positions.data_ptr(), row_request.data_ptr(),
+        block_table.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
+        q_out.data_ptr(), _stream(), act is torch.float32, ld, n, n_heads, n_kv_heads, head_dim,
+        bool(weights) and weights[0].dtype is torch.float32, (q_weight is not None) | (k_weight is not None) << 1, rot_dim,
+        bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, eps)),
+        "qk_norm_rope_store_kv8")
 
 
 KV8_HEAD_DIMS = (64, 128, 256)   # head sizes that the tensor cores' kernel takes
@@ -2630,11 +2659,13 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     up to ``tokens`` (at most :func:`kv8_tile_tokens`) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
     request r's rows end at q_start[r + 1]."""
     act = out.dtype
-    _need(q, "q", (act,), 3)
     out_ld = _need_rows(out, "out", _BF16_F32)
-    _need(block_table, "block_table", _I, 2)
-    _need(row_request, "row_request", _I, 1)
-    _need(positions, "positions", _I, 1)
+    if not (_lists(row_request, positions) and q.dtype is act and q.is_cuda and q.dim() == 3 and q.is_contiguous()
+            and block_table.dtype is _I32 and block_table.is_cuda and block_table.dim() == 2 and block_table.is_contiguous()):
+        _need(q, "q", (act,), 3)
+        _need(block_table, "block_table", _I, 2)
+        _need(row_request, "row_request", _I, 1)
+        _need(positions, "positions", _I, 1)
     n, nh, d = q.shape
     n_pages, nkv, page_size, dk = pages.k.shape
     if dk != d or nh % nkv or out.shape != (n, nh * d) or row_request.shape[0] != n or positions.shape[0] != n:
@@ -2645,7 +2676,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     lib, stream = _few_bits(), _stream()
     code = -1
     if act == torch.bfloat16 and d in KV8_HEAD_DIMS:
-        tile_req = tile_row0 = q_start = None
+        tile_req = tile_row0 = q_start = 0
         n_tiles, tokens = n, 1
         if tiles is not None:
             tile_req, tile_row0, n_tiles, q_start, tokens = tiles
@@ -2653,11 +2684,11 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
                 _need(t, name, _I, 1)
             if min(tile_req.shape[0], tile_row0.shape[0]) < n_tiles or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d):
                 raise KernelError(f"paged_attention_kv8: {n_tiles} tiles of {tokens} tokens in lists of {tile_req.shape[0]}")
-        code = lib.ib_paged_attention_kv8(
+            tile_req, tile_row0, q_start = tile_req.data_ptr(), tile_row0.data_ptr(), q_start.data_ptr()
+        code = lib.ib_paged_attention_kv8(_ATTENTION_CALL(
             q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-            block_table.data_ptr(), max_pages, page_size, n_pages, n_req, row_request.data_ptr(), positions.data_ptr(), n,
-            _p(tile_req), _p(tile_row0), _p(q_start), n_tiles, tokens, nh, nkv, d, float(scale), span, out.data_ptr(), out_ld, 0,
-            int(max_kv_len), stream)
+            block_table.data_ptr(), row_request.data_ptr(), positions.data_ptr(), tile_req, tile_row0, q_start, out.data_ptr(),
+            stream, max_pages, page_size, n_pages, n_req, n, n_tiles, tokens, nh, nkv, d, span, out_ld, 0, max_kv_len, scale))
     if code == -1:
         code = lib.ib_paged_attention_kv8_generic(
             q.data_ptr(), act == torch.float32, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(),

@@ -131,6 +131,28 @@ def test_product_with_weights_in_four_bits(n, k, m, kind):
     assert K.few_bits_faults() == {}
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32", "mx4"])
+@pytest.mark.parametrize("n,k,m", [(1, 4096, 300), (8, 2080, 1000), (16, 4096, 520), (30, 3000, 700), (60, 4100, 400)])
+def test_product_of_few_rows_cut_every_way(n, k, m, kind):
+    """Tiles of every height, K in every number of parts, rings that are shorter and longer than what they carry."""
+    from inferrs_b200 import kernels as K
+    x, w = rand((n, k), 13).to(DT.get(kind, torch.bfloat16)), K.quantize_mx4(0.02 * rand((m, k), 14))
+    dense = torch.empty((m, k), device="cuda")
+    K.dequantize_mx4(w, dense)
+    given = K.quantize_mx4(x) if kind == "mx4" else x
+    x = plain.values4(x)[0] if kind == "mx4" else x.double()
+    want = x @ dense.double().t()
+    limit = product_limit(x, dense.double(), kind, torch.float32, want)
+    for tile_rows, splits in ((128, 1), (128, 2), (128, 4), (128, 8), (88, 1), (88, 8), (64, 2), (40, 4), (24, 1), (8, 1), (8, 8)):
+        out = torch.full((n, m), float("nan"), device="cuda")
+        K.linear_mx4(given, w, out, tile_rows, splits)
+        assert bool(((out.double() - want).abs() <= limit).all()), (tile_rows, splits)
+    assert K.few_bits_faults() == {}
+    for bad in ((4, 1), (136, 1), (128, 16), (24, 16), (128, -1)):
+        with pytest.raises(K.KernelError):
+            K.linear_mx4(given, w, out, *bad)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("pad_x,pad_y", [(8, 8), (1, 3)])
 def test_product_of_rows_that_lie_apart(pad_x, pad_y, kind):
