@@ -70,14 +70,26 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+// Operand descriptors by their low word, which holds where a tile starts in units of 16 bytes: the thread that issues the products
+// has about five cycles for an instruction, and what it computes for a stage decides how fast stages follow one another.
+__device__ __forceinline__ unsigned long long from_words(unsigned lo, unsigned hi) {
+    unsigned long long d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+// One lane of the warp, the same every time.  The warp runs the loop around what that lane issues as a whole, so that addresses and
+// descriptors stay uniform registers, which the instructions want.
+__device__ __forceinline__ bool elected() {
+    unsigned r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+constexpr unsigned TILE_HI = (unsigned)(1024 >> 4) | 1u << 14 | 2u << 29, TILE_LO = 1u << 16;       // desc_k_major in sm100.cuh
+constexpr unsigned SCALE_HI = (unsigned)(128 >> 4) | 1u << 14;
 // 512 bytes of scales (32 rows of 16 bytes, eight rows 128 bytes apart) into four columns of tensor memory, the same in
 // every quarter of the lanes
-__device__ __forceinline__ void scales_to_tmem(unsigned tmem, unsigned smem_addr) {
-    unsigned long long d = 0;
-    d |= (unsigned long long)((smem_addr & 0x3FFFF) >> 4);
-    d |= (unsigned long long)(128 >> 4) << 32;
-    d |= (unsigned long long)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+__device__ __forceinline__ void scales_to_tmem(unsigned tmem, unsigned lo) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from_words(lo, SCALE_HI)) : "memory");
 }
 template <int KIND>
 __device__ __forceinline__ void umma_scaled(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sa,
@@ -114,28 +126,27 @@ __device__ __forceinline__ void store(const Params& p, int t, int f, float v) {
 }
 
 // One stage's products, issued by one thread: scales into the stage's columns of tensor memory (`scales`), then four products
-// of 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones.
+// of 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones.  a, b, sa, sb: where the stage's tiles start, in units of
+// 16 bytes.
 template <int KIND, int BN>
-__device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, unsigned char* a, unsigned char* b, unsigned char* sa_tile,
-                                               unsigned char* sb_tile, bool accumulate) {
+__device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, unsigned a, unsigned b, unsigned sa_tile, unsigned sb_tile,
+                                               bool accumulate) {
     using P = Plan<KIND, BN>;
     constexpr unsigned FORMATS = KIND != CODES ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);   // e2m1 and e4m3, e2m1 twice
     constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(BM >> 4) << 24);
-    fence_after();
     const unsigned sa = scales, sb = sa + 4 * P::K_TILES;
 #pragma unroll
     for (int j = 0; j < P::K_TILES; ++j) {
-        scales_to_tmem(sa + 4 * j, smem_u32(sa_tile + 512 * j));
+        scales_to_tmem(sa + 4 * j, sa_tile + 32 * j);
 #pragma unroll
         for (int g = 0; g < P::B_GROUPS; ++g)     // the column tiles one after the other, the row tiles of each side by side
-            scales_to_tmem(sb + 4 * (j * P::B_GROUPS + g), smem_u32(sb_tile + g * P::SA_BYTES + 512 * j));
+            scales_to_tmem(sb + 4 * (j * P::B_GROUPS + g), sb_tile + g * (P::SA_BYTES / 16) + 32 * j);
     }
-    const unsigned long long da = desc_k_major(smem_u32(a)), db = desc_k_major(smem_u32(b));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const unsigned tile = KIND != CODES ? 0 : k >> 1, id = KIND != CODES ? k : (k & 1) * 2;
-        umma_scaled<KIND>(tmem, da + 2 * k, db + 2 * k, IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile,
-                          accumulate || k != 0);
+        umma_scaled<KIND>(tmem, from_words(TILE_LO + a + 2 * k, TILE_HI), from_words(TILE_LO + b + 2 * k, TILE_HI),
+                          IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile, accumulate || k != 0);
     }
 }
 
@@ -155,49 +166,61 @@ __device__ __forceinline__ void two_pieces(unsigned v, unsigned short& first, un
 // ---- up to 64 rows: what counts is that every SM streams its share of the weights -----------------------------------------------
 // A tile may cover fewer rows of W than the product's 128 (a multiple of eight; what the tensor core reads beyond them belongs
 // to other tiles and its results are not stored), so that the tiles can be as many as the SMs, or twice as many.  Its scales are then
-// not a 512-byte tile of the matrix's: warps 6..9 put every fourth stage's together, and bring x's numbers to pieces where
-// the kernel does that itself.
+// not a 512-byte tile of the matrix's: helper warps put them together, a warp every fourth stage's, and, where the kernel brings
+// x's numbers to pieces itself, two warps every fourth stage's pieces.
+__device__ __forceinline__ void copy4(unsigned dst, const void* src, bool in) {        // four bytes, or zeros
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// the thread's arrival at a barrier when its copies so far are there (counted in the barrier's arrivals)
+__device__ __forceinline__ void arrive_with_copies(unsigned bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 struct Shape {
     int tile_rows, stages, splits, tmem_cols;
 };
 
-// What a helper warp holds of its next stage: four rows' words of scales a lane and K tile, and (INSIDE) eight numbers of every
-// other row of x: four threads have a block of 32, a warp two rows at a time.  The numbers go through f16, which holds a
+// (INSIDE) A thread takes eight numbers of a row of x, four threads a block of 32, a warp two rows at a time and every other
+// two; what it needs of its next stage is on its way.  The numbers go through f16, which holds a
 // bfloat16 number's eight bits from 256 down to 2^-17 and below that what the second piece may still need.
 template <int KIND, int BN, bool INSIDE>
 __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, int row0, unsigned char* b_tiles, unsigned char* sa_tiles,
                                             unsigned char* sb_tiles, int kb0, int nkb, unsigned full0, unsigned empty0) {
     using P = Plan<KIND, BN>;
-    constexpr int PASSES = INSIDE ? P::TOKENS / 2 : 1;
+    constexpr int PASSES = INSIDE ? P::TOKENS / 4 : 1;         // of a warp
+    const int which = (int)(threadIdx.x - THREADS) >> 5, half = which >> 2;
     const int lane = threadIdx.x & 31, g = lane & 15, rows = (p.n_out + 127) / 128 * 128 - row0;      // of scales there are
     const unsigned* scales = reinterpret_cast<const unsigned*>(p.w_scales);
-    unsigned words[P::K_TILES][4];
-    auto fetch_scales = [&](int i) {
+    // a stage's scales are on their way with its weights (the weights' scales come from as far as the weights do)
+    auto fetch_scales = [&](int i, int s) {
 #pragma unroll
         for (int j = 0; j < P::K_TILES; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int r = 32 * c + lane;
-                words[j][c] = i < nkb && r < sh.tile_rows && r < rows ? scales[few::scale_word(row0 + r, (kb0 + i) * P::K_TILES + j, p.scale_tiles)] : 0u;
+                const bool in = r < sh.tile_rows && r < rows;
+                copy4(smem_u32(sa_tiles + s * P::SA_BYTES + 512 * j + 16 * lane + 4 * c),
+                      scales + (in ? few::scale_word(row0 + r, (kb0 + i) * P::K_TILES + j, p.scale_tiles) : 0), in);
             }
+        arrive_with_copies(full0 + 8 * s);
     };
     // No more helpers than stages: a warp that has filled stage i knows the products of stage i - stages done; its next stage's
     // place was last but one used by stage i + helpers - 2 stages, and only if that one is done too does the parity of the place's
     // barrier say which use it speaks of.
     const int helpers = sh.stages < 4 ? sh.stages : 4;
-    int i = (int)(threadIdx.x - THREADS) >> 5;
+    int i = which & 3;
     if (i >= helpers) return true;
-    fetch_scales(i);
+    for (int a = i; half == 0 && a < nkb && a < sh.stages; a += helpers) fetch_scales(a, a);      // before the kernel ahead is done
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint4 raw[PASSES];
-    const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(lane >> 4) * p.ldx + 8 * g);
+    const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(2 * half + (lane >> 4)) * p.ldx + 8 * g);
     auto fetch_x = [&](int i) {
         const int c = (kb0 + i) * 128;
 #pragma unroll
         for (int j = 0; j < PASSES; ++j) {
             raw[j] = make_uint4(0, 0, 0, 0);
-            if (2 * j + (lane >> 4) >= p.n_tok || i >= nkb) continue;
-            const __nv_bfloat16* src = x + 2L * j * p.ldx + c;
+            if (4 * j + 2 * half + (lane >> 4) >= p.n_tok || i >= nkb) continue;
+            const __nv_bfloat16* src = x + 4L * j * p.ldx + c;
             const int n = p.k - c - 8 * g;
             if (p.wide && n >= 8) {
                 raw[j] = *reinterpret_cast<const uint4*>(src);
@@ -209,17 +232,16 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
         }
     };
     if constexpr (INSIDE) fetch_x(i);
-    for (; i < nkb; i += helpers) {
-        const int s = i % sh.stages;
-        if (i >= sh.stages && !mbar_wait(empty0 + 8 * s, ((i / sh.stages) - 1) & 1, 4)) return false;
-#pragma unroll
-        for (int j = 0; j < P::K_TILES; ++j)
-            *reinterpret_cast<uint4*>(sa_tiles + s * P::SA_BYTES + 512 * j + 16 * lane) = make_uint4(words[j][0], words[j][1], words[j][2], words[j][3]);
-        fetch_scales(i + helpers);
+    int s = i;
+    unsigned phase = 1;                  // of the place's barrier at this stage's turn
+    for (; i < nkb; i += helpers, s += helpers) {
+        if (s >= sh.stages) { s -= sh.stages; phase ^= 1; }
+        if (i >= sh.stages && !mbar_wait(empty0 + 8 * s, phase, 4)) return false;
+        if (half == 0 && i >= sh.stages) fetch_scales(i, s);
         if constexpr (INSIDE) {
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
-                if (2 * j >= p.n_tok) break;                  // columns of no token: whatever the stage holds
+                if (4 * j + 2 * half >= p.n_tok) break;       // columns of no token: whatever the stage holds
                 const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
                 unsigned m = 0;
 #pragma unroll
@@ -233,7 +255,7 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     two_pieces(byte == 255u ? 0u : f16_pair(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xFFFF0000u) * by), h[e], l[e]);
-                const int r = 2 * (2 * j + (lane >> 4));
+                const int r = 2 * (4 * j + 2 * half + (lane >> 4));
                 unsigned char* to = b_tiles + s * P::B_BYTES + (g & 1) * 8;
                 *reinterpret_cast<uint2*>(to + r * 128 + ((g >> 1) ^ (r & 7)) * 16) = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
                 *reinterpret_cast<uint2*>(to + (r + 1) * 128 + ((g >> 1) ^ ((r + 1) & 7)) * 16) = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
@@ -244,17 +266,18 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
                 }
             }
             fetch_x(i + helpers);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads them behind the barrier
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full0 + 8 * s);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads them behind the barrier
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full0 + 8 * s);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     return true;
 }
 
 // INSIDE: the kernel brings x's rows to pieces itself
 template <int KIND, int BN, bool INSIDE>
-__global__ void __launch_bounds__(THREADS + 128) few_rows_kernel(const __grid_constant__ CUtensorMap map_w,
+__global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                  const __grid_constant__ CUtensorMap map_x, const Params p, const Shape sh) {
     using P = Plan<KIND, BN>;
     extern __shared__ unsigned char raw_smem[];
@@ -275,7 +298,7 @@ __global__ void __launch_bounds__(THREADS + 128) few_rows_kernel(const __grid_co
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, INSIDE ? 35 : 33); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accum, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -291,44 +314,50 @@ __global__ void __launch_bounds__(THREADS + 128) few_rows_kernel(const __grid_co
     if (splits > 1) cluster_arrive();       // "this CTA runs": looked at before the first store to it
 
     if (warp == 0) {
-        if (lane == 0) {
-            const unsigned long long pol = policy_evict_first();
-            const unsigned w_tx = KIND == CODES ? a_bytes : a_bytes / 2;     // what a tile of weights counts on its barrier
-            auto load_w = [&](int i, int s) {
-                mbar_expect_tx(full0 + 8 * s, w_tx + (INSIDE ? 0 : P::B_BYTES + P::SB_BYTES));
-                tma_load_2d_hint(smem_u32(a_tiles + s * a_bytes), &map_w, (kb0 + i) * 128, row0, full0 + 8 * s, pol);
-            };
-            auto load_x = [&](int i, int s) {
-                if constexpr (INSIDE) return;
-                tma_load_2d(smem_u32(b_tiles + s * P::B_BYTES), &map_x, (kb0 + i) * 128, tile_t * BN, full0 + 8 * s);
+        const bool leader = elected();
+        const unsigned long long pol = policy_evict_first();
+        const unsigned w_tx = KIND == CODES ? a_bytes : a_bytes / 2;     // what a tile of weights counts on its barrier
+        auto load_w = [&](int i, int s) {
+            if (!leader) return;
+            mbar_expect_tx(full0 + 8 * s, w_tx + (INSIDE ? 0 : P::B_BYTES + P::SB_BYTES));
+            tma_load_2d_hint(smem_u32(a_tiles) + s * a_bytes, &map_w, (kb0 + i) * 128, row0, full0 + 8 * s, pol);
+        };
+        auto load_x = [&](int i, int s) {
+            if (INSIDE || !leader) return;
+            tma_load_2d(smem_u32(b_tiles) + s * P::B_BYTES, &map_x, (kb0 + i) * 128, tile_t * BN, full0 + 8 * s);
 #pragma unroll
-                for (int g = 0; g < P::B_GROUPS; ++g)
-                    bulk_load(smem_u32(sb_tiles + s * P::SB_BYTES + g * P::SA_BYTES),
-                              p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)(kb0 + i) * P::K_TILES) * 512,
-                              P::SA_BYTES, full0 + 8 * s);
-            };
-            const int head = nkb < stages ? nkb : stages;    // the first weights are on their way before the kernel ahead is done
-            for (int i = 0; i < head; ++i) load_w(i, i);
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (int i = 0; i < head; ++i) load_x(i, i);
-            for (int i = head; i < nkb; ++i) {
-                const int s = i % stages;
-                if (!mbar_wait(empty0 + 8 * s, ((i / stages) - 1) & 1, 1)) { ok = false; break; }
-                load_w(i, s);
-                load_x(i, s);
-            }
+            for (int g = 0; g < P::B_GROUPS; ++g)
+                bulk_load(smem_u32(sb_tiles) + s * P::SB_BYTES + g * P::SA_BYTES,
+                          p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)(kb0 + i) * P::K_TILES) * 512,
+                          P::SA_BYTES, full0 + 8 * s);
+        };
+        const int head = nkb < stages ? nkb : stages;    // the first weights are on their way before the kernel ahead is done
+        for (int i = 0; i < head; ++i) load_w(i, i);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int i = 0; i < head; ++i) load_x(i, i);
+        unsigned phase = 0;
+        for (int i = head, s = 0; i < nkb; ++i) {
+            if (!mbar_wait(empty0 + 8 * s, phase, 1)) { ok = false; break; }
+            load_w(i, s);
+            load_x(i, s);
+            if (++s == stages) { s = 0; phase ^= 1; }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            for (int i = 0; i < nkb; ++i) {
-                const int s = i % stages;
-                if (!mbar_wait(full0 + 8 * s, (i / stages) & 1, 2)) { ok = false; break; }
-                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a_tiles + s * a_bytes, b_tiles + s * P::B_BYTES,
-                                         sa_tiles + s * P::SA_BYTES, sb_tiles + s * P::SB_BYTES, i != 0);
+        const bool leader = elected();
+        const unsigned a0 = smem_u32(a_tiles) >> 4, b0 = smem_u32(b_tiles) >> 4, sa0 = smem_u32(sa_tiles) >> 4, sb0 = smem_u32(sb_tiles) >> 4;
+        unsigned phase = 0;
+        for (int i = 0, s = 0; i < nkb; ++i) {
+            if (!mbar_wait(full0 + 8 * s, phase, 2)) { ok = false; break; }
+            fence_after();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the scales came by plain copies
+            if (leader) {
+                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a0 + s * (a_bytes >> 4), b0 + s * (P::B_BYTES / 16),
+                                         sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0);
                 umma_commit(empty0 + 8 * s);
             }
-            umma_commit(accum);
+            if (++s == stages) { s = 0; phase ^= 1; }
         }
+        if (leader) umma_commit(accum);
     } else if (warp >= 6) {
         ok = fill_stages<KIND, BN, INSIDE>(p, sh, row0, b_tiles, sa_tiles, sb_tiles, kb0, nkb, full0, empty0);
     }
@@ -390,7 +419,7 @@ __global__ void __launch_bounds__(THREADS + 128) few_rows_kernel(const __grid_co
 
 // ---- more rows ------------------------------------------------------------------------------------------------------------------
 template <int KIND, int BN, int STAGES>
-__global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
+__global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
                                                        const __grid_constant__ CUtensorMap map_x, const Params p) {
     using P = Plan<KIND, BN>;
     extern __shared__ unsigned char raw_smem[];
@@ -407,7 +436,7 @@ __global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ C
     const int tile_f = blockIdx.x, tile_t = blockIdx.y, nkb = p.num_kb;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accum, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -420,45 +449,54 @@ __global__ void __launch_bounds__(THREADS) gemm_kernel(const __grid_constant__ C
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
-    if (warp == 0) {
-        if (lane == 0) {
-            constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
-            auto load_w = [&](int i, int s) {
-                mbar_expect_tx(full0 + 8 * s, W_TX + P::SA_BYTES + P::B_BYTES + P::SB_BYTES);
-                tma_load_2d(smem_u32(a_tiles + s * A_BYTES), &map_w, i * 128, tile_f * BM, full0 + 8 * s);
-                bulk_load(smem_u32(sa_tiles + s * P::SA_BYTES), p.w_scales + ((long)tile_f * p.scale_tiles + (long)i * P::K_TILES) * 512,
-                          P::SA_BYTES, full0 + 8 * s);
-            };
-            auto load_x = [&](int i, int s) {
-                tma_load_2d(smem_u32(b_tiles + s * P::B_BYTES), &map_x, i * 128, tile_t * BN, full0 + 8 * s);
+    // Copies are issued by two threads, one for the operands and one for their scales: a thread takes 165 cycles a tile and 50 a
+    // plain copy, five of which together would take longer than the products of a stage.
+    if (warp == 0 || warp == 6) {
+        const bool leader = elected(), tiles = warp == 0;
+        constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
+        auto load_w = [&](int i, int s) {
+            if (!leader) return;
+            mbar_expect_tx(full0 + 8 * s, tiles ? W_TX + P::B_BYTES : P::SA_BYTES + P::SB_BYTES);
+            if (tiles) tma_load_2d(smem_u32(a_tiles) + s * A_BYTES, &map_w, i * 128, tile_f * BM, full0 + 8 * s);
+            else bulk_load(smem_u32(sa_tiles) + s * P::SA_BYTES, p.w_scales + ((long)tile_f * p.scale_tiles + (long)i * P::K_TILES) * 512,
+                           P::SA_BYTES, full0 + 8 * s);
+        };
+        auto load_x = [&](int i, int s) {
+            if (!leader) return;
+            if (tiles) {
+                tma_load_2d(smem_u32(b_tiles) + s * P::B_BYTES, &map_x, i * 128, tile_t * BN, full0 + 8 * s);
+            } else {
 #pragma unroll
                 for (int g = 0; g < P::B_GROUPS; ++g)
-                    bulk_load(smem_u32(sb_tiles + s * P::SB_BYTES + g * P::SA_BYTES),
+                    bulk_load(smem_u32(sb_tiles) + s * P::SB_BYTES + g * P::SA_BYTES,
                               p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)i * P::K_TILES) * 512,
                               P::SA_BYTES, full0 + 8 * s);
-            };
-            const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
-            for (int i = 0; i < head; ++i) load_w(i, i);
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (int i = 0; i < head; ++i) load_x(i, i);
-            for (int i = head; i < nkb; ++i) {
-                const int s = i % STAGES;
-                if (!mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, 1)) { ok = false; break; }
-                load_w(i, s);
-                load_x(i, s);
             }
+        };
+        const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
+        for (int i = 0; i < head; ++i) load_w(i, i);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int i = 0; i < head; ++i) load_x(i, i);
+        for (int i = head; i < nkb; ++i) {
+            const int s = i % STAGES;
+            if (!mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, 1)) { ok = false; break; }
+            load_w(i, s);
+            load_x(i, s);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            for (int i = 0; i < nkb; ++i) {
-                const int s = i % STAGES;
-                if (!mbar_wait(full0 + 8 * s, (i / STAGES) & 1, 2)) { ok = false; break; }
-                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a_tiles + s * A_BYTES, b_tiles + s * P::B_BYTES,
-                                         sa_tiles + s * P::SA_BYTES, sb_tiles + s * P::SB_BYTES, i != 0);
+        const bool leader = elected();
+        const unsigned a0 = smem_u32(a_tiles) >> 4, b0 = smem_u32(b_tiles) >> 4, sa0 = smem_u32(sa_tiles) >> 4, sb0 = smem_u32(sb_tiles) >> 4;
+        for (int i = 0; i < nkb; ++i) {
+            const int s = i % STAGES;
+            if (!mbar_wait(full0 + 8 * s, (i / STAGES) & 1, 2)) { ok = false; break; }
+            fence_after();
+            if (leader) {
+                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a0 + s * (A_BYTES / 16), b0 + s * (P::B_BYTES / 16),
+                                         sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0);
                 umma_commit(empty0 + 8 * s);
             }
-            umma_commit(accum);
         }
+        if (leader) umma_commit(accum);
     } else {
         const int q = warp & 3, feature = tile_f * BM + q * 32 + lane;
         const int t0 = tile_t * P::TOKENS, tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
@@ -550,21 +588,27 @@ static int make_maps(CUtensorMap* map_w, CUtensorMap* map_x, const void* w, cons
 
 constexpr int SMS = 148, FEW_SMEM = 100 * 1024;      // of a CTA of the kernel for few rows: two share an SM
 
-// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA's tensor core takes
-// about a cycle per number of K for a tile of any height (half for 4-bit rows), the weights come at 44 bytes a cycle
-// and SM, and parts cost their meeting, about 2,800 cycles.
+// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA takes about 350 cycles
+// a stage whatever its tile's height (the issue of its copies and products) after a start of 4,000, two share an SM, their bytes
+// come at 44 a cycle, and parts cost their meeting, which grows with the rows of x.  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row
+// 32 x 1 10.9, 64 x 2 8.5, 128 x 4 6.9, 128 x 8 8.1; sixteen rows 11.8, 11.2, 9.9, 11.0; 48 rows 15.7, 18.7, 20.0 (128 x 4).
+// 4,096 x 24,576, one row: 88 x 1 13.3, 128 x 1 13.7; 48 rows 22.2, 25.3.
 template <int KIND, int BN>
-static Shape shape_for(int m, int num_kb, int tiles_t, int tile_rows, int splits) {
+static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int splits) {
     using P = Plan<KIND, BN>;
     auto lowered = [](long rows) { return rows > 128 ? 128 : (int)(rows + 7) / 8 * 8; };
     Shape s = {tile_rows > 0 ? tile_rows : 128, 1, splits > 0 ? splits : 1, 0};
     if (tile_rows == 0 && splits == 0) {
         long best = -1;
         for (int parts = 1; parts <= 8 && (parts == 1 || 2 * parts <= num_kb); parts *= 2) {
-            const long rounds = ((long)(m + 127) / 128 * tiles_t * parts + SMS - 1) / SMS, columns = rounds * SMS / ((long)parts * tiles_t);
+            // tiles of 128 rows, lowered until as many rounds of CTAs as they take are full (clusters find room on 128 SMs or so)
+            const long sms = parts > 1 ? 128 : SMS, per_part = (long)tiles_t * parts, all = (long)(m + 127) / 128 * per_part;
+            const long columns = (all + sms - 1) / sms * sms / per_part;
             const int rows = lowered((m + columns - 1) / columns);
-            const long k_cycles = (long)num_kb * 128 / parts, bytes_cycles = (long)rows * num_kb * (KIND == CODES ? 136 : 68) / parts / 44;
-            const long cost = rounds * (k_cycles > bytes_cycles ? k_cycles : bytes_cycles) + (parts > 1 ? 2800 : 0);
+            const long ctas = (long)(m + rows - 1) / rows * per_part, each = (ctas + sms - 1) / sms, together = each < 2 ? each : 2;
+            const long bytes_cycles = (long)rows * (KIND == CODES ? 136 : 68) / 44 * together, stages = (num_kb + parts - 1) / parts;
+            const long cost = (each + 1) / 2 * (4000 + stages * (bytes_cycles > 350 ? bytes_cycles : 350)) +
+                              (parts == 1 ? 0 : (parts == 2 ? 1000 : parts == 4 ? 2000 : 5500) + 200 * (n < P::TOKENS ? n : P::TOKENS));
             if (best < 0 || cost < best) { best = cost; s.tile_rows = rows; s.splits = parts; }
         }
     }
@@ -585,7 +629,7 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     using P = Plan<KIND, BN>;
     const int tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
     if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
-    const Shape sh = shape_for<KIND, BN>(m, (k + (KIND == CODES ? 255 : 127)) / (KIND == CODES ? 256 : 128), tiles_t, tile_rows, splits);
+    const Shape sh = shape_for<KIND, BN>(n, m, (k + (KIND == CODES ? 255 : 127)) / (KIND == CODES ? 256 : 128), tiles_t, tile_rows, splits);
     CUtensorMap map_w, map_x;
     if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, sh.tile_rows, BN, p)) return r;
     if (sh.splits > 8 || sh.splits > p.num_kb || sh.tile_rows % sh.splits) return IB_ERR_ARGUMENT;
@@ -604,7 +648,7 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     if (int r = ib_allow_dynamic_smem(done, few_rows_kernel<KIND, BN, INSIDE>, 200 * 1024)) return r;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((m + sh.tile_rows - 1) / sh.tile_rows, tiles_t, sh.splits);
-    cfg.blockDim = dim3(THREADS + 128);
+    cfg.blockDim = dim3(THREADS + (INSIDE ? 256 : 128));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -633,7 +677,7 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, BM, BN, p)) return r;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((m + BM - 1) / BM, tiles_t);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(THREADS + 32);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
