@@ -43,11 +43,11 @@ __device__ __forceinline__ unsigned codes2(float first, float second) {
     asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(first), "f"(second));
     return r;
 }
-// the value of a 4-bit code
-__device__ __forceinline__ float code_value(unsigned c) {
-    const unsigned m = c & 7u;
-    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    return c & 8u ? -v : v;
+// the values of two codes, the low half of the byte first
+__device__ __forceinline__ __half2 values4x2(unsigned byte) {
+    unsigned r;
+    asm("{\n\t.reg .b8 t, u, v, w;\n\tmov.b32 {t, u, v, w}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(r) : "r"(byte));
+    return *reinterpret_cast<const __half2*>(&r);
 }
 
 // eight neighbours of a row (zeros behind the first n), 16 bytes at a time where the rows allow it

@@ -24,11 +24,105 @@ constexpr int STORE_WARPS = 4;
 
 struct StoreArgs {
     long ldx;
-    int n_heads, n_kv, d, flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages;   // flags: 1 norm q, 2 norm k
+    int n_heads, n_kv, d, flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req;   // flags: 1 norm q, 2 norm k
     float eps;
 };
 
-// A warp per head of a row: norm, rotation in float32; queries are stored in their type, keys and values as codes
+// Heads of 64, 128 or 256 numbers that turn as a whole, element i with i + d / 2, in bfloat16: a lane holds four numbers of the
+// first half of a head and the four they turn with, a warp 256 / D heads at a time and STEPS times, whose loads are all on their way
+// before the first is used; what belongs to the row (its place, its angles) is fetched once.  2,048 rows of 32 + 8 + 8 heads of 128:
+// 47 MB, 51 us with a warp a head through shared memory, TIME like this.
+template <int D, int STEPS, typename WT>
+__global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
+    const __nv_bfloat16* __restrict__ qkv, const WT* __restrict__ q_weight, const WT* __restrict__ k_weight,
+    const float* __restrict__ cos_table, const float* __restrict__ sin_table, const int* __restrict__ positions,
+    const int* __restrict__ row_request, const int* __restrict__ block_table, unsigned char* __restrict__ k_pages,
+    unsigned char* __restrict__ v_pages, float* __restrict__ k_scale, float* __restrict__ v_scale, __nv_bfloat16* __restrict__ q_out,
+    const StoreArgs a) {
+    constexpr int LANES = D / 8, HEADS = 32 / LANES;            // of a head; heads a step
+    ib_grid_dependency_launch();
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = 4 * (lane % LANES);
+    const int head0 = ((int)blockIdx.y * STORE_WARPS + warp) * HEADS * STEPS + lane / LANES, heads = a.n_heads + 2 * a.n_kv;
+    const int pos = positions[row], req = row_request[row];
+    const bool fault = pos < 0 || pos >= a.table_rows;
+    const float4 c = fault ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(cos_table + (long)pos * (D / 2) + i);
+    const float4 s = fault ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(sin_table + (long)pos * (D / 2) + i);
+    ib_grid_dependency_wait();
+    qkv = ib_after_wait(qkv);
+    if (fault) {
+        if (threadIdx.x == 0) atomicCAS(&ib_kv8_row_fault_word, 0, row + 1);
+        return;
+    }
+    uint2 raw[STEPS][2];
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+        const int head = head0 + t * HEADS;
+        const __nv_bfloat16* src = qkv + (long)row * a.ldx + (long)head * D + i;
+        raw[t][0] = head < heads ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
+        raw[t][1] = head < heads ? *reinterpret_cast<const uint2*>(src + D / 2) : make_uint2(0, 0);
+    }
+    const int page = req >= 0 && req < a.n_req && pos / a.page_size < a.max_pages ? block_table[(long)req * a.max_pages + pos / a.page_size] : -1;
+    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+        const int head = head0 + t * HEADS, kind = head < a.n_heads ? 0 : (head < a.n_heads + a.n_kv ? 1 : 2);   // 0 q, 1 k, 2 v
+        float x[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x[h][0] = __uint_as_float(raw[t][h].x << 16);
+            x[h][1] = __uint_as_float(raw[t][h].x & 0xFFFF0000u);
+            x[h][2] = __uint_as_float(raw[t][h].y << 16);
+            x[h][3] = __uint_as_float(raw[t][h].y & 0xFFFF0000u);
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss += x[0][e] * x[0][e] + x[1][e] * x[1][e];
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (kind != 2) {
+            if (a.flags >> kind & 1) {
+                const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+                const WT* w = kind == 0 ? q_weight : k_weight;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[0][e] = x[0][e] * inv * (w ? ib_to_float(w[i + e]) : 1.0f);
+                    x[1][e] = x[1][e] * inv * (w ? ib_to_float(w[D / 2 + i + e]) : 1.0f);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {       // products are rounded before they are added up, as everywhere in this file
+                const float first = x[0][e], second = x[1][e];
+                x[0][e] = __fsub_rn(__fmul_rn(first, cs[e]), __fmul_rn(second, sn[e]));
+                x[1][e] = __fadd_rn(__fmul_rn(second, cs[e]), __fmul_rn(first, sn[e]));
+            }
+        }
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, max(__float_as_uint(x[0][e]) & 0x7FFFFFFFu, __float_as_uint(x[1][e]) & 0x7FFFFFFFu));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (head >= heads) continue;
+        if (kind == 0) {
+            __nv_bfloat16* dst = q_out + ((long)row * a.n_heads + head) * D + i;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[h][0], x[h][1]), hi = __floats2bfloat162_rn(x[h][2], x[h][3]);
+                *reinterpret_cast<uint2*>(dst + h * (D / 2)) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+            }
+        } else if (page >= 0 && page < a.n_pages) {       // else a request that stands in to fill a batch
+            const long place = ((long)page * a.n_kv + (head - a.n_heads) % a.n_kv) * a.page_size + pos % a.page_size;
+            float by, scale;
+            vector_scale(__uint_as_float(m), by, scale);
+            unsigned char* dst = (kind == 1 ? k_pages : v_pages) + place * D + i;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<unsigned*>(dst + h * (D / 2)) = codes8x4(x[h][0] * by, x[h][1] * by, x[h][2] * by, x[h][3] * by);
+            if (i == 0) (kind == 1 ? k_scale : v_scale)[place] = scale;
+        }
+    }
+}
+
+// Everything else, a warp per head of a row: norm, rotation in float32; queries are stored in their type, keys and values as codes
 // with a scale per vector.
 template <typename T, typename WT>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
@@ -55,7 +149,8 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
     const int kind = head < a.n_heads ? 0 : (head < a.n_heads + a.n_kv ? 1 : 2);   // 0 q, 1 k, 2 v
     long place = -1;
     if (kind != 0) {
-        const int page = pos / a.page_size < a.max_pages ? block_table[(long)row_request[row] * a.max_pages + pos / a.page_size] : -1;
+        const int req = row_request[row];
+        const int page = req >= 0 && req < a.n_req && pos / a.page_size < a.max_pages ? block_table[(long)req * a.max_pages + pos / a.page_size] : -1;
         if (page < 0 || page >= a.n_pages) return;      // a request that stands in to fill a batch
         place = ((long)page * a.n_kv + (head - a.n_heads) % a.n_kv) * a.page_size + pos % a.page_size;
     }
@@ -179,7 +274,7 @@ struct IbStoreKv8 {
     float *k_scale, *v_scale;
     void* q_out;
     cudaStream_t stream;
-    long is_f32, ldx, n, n_heads, n_kv, d, w_is_f32, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages;
+    long is_f32, ldx, n, n_heads, n_kv, d, w_is_f32, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req;
     double eps;
 };
 IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
@@ -194,11 +289,27 @@ IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
     const long ldx = s->ldx;
     const int is_f32 = (int)s->is_f32, n = (int)s->n, n_heads = (int)s->n_heads, n_kv = (int)s->n_kv, d = (int)s->d, w_is_f32 = (int)s->w_is_f32,
               norm_flags = (int)s->norm_flags, rot_dim = (int)s->rot_dim, interleaved = (int)s->interleaved, table_rows = (int)s->table_rows,
-              max_pages = (int)s->max_pages, page_size = (int)s->page_size, n_pages = (int)s->n_pages;
+              max_pages = (int)s->max_pages, page_size = (int)s->page_size, n_pages = (int)s->n_pages, n_req = (int)s->n_req;
     const float eps = (float)s->eps;
     if (n < 0 || n_heads <= 0 || n_kv <= 0 || d <= 0 || d % 4 || d > 1024 || rot_dim < 0 || rot_dim > d || rot_dim % 2 || page_size <= 0) return IB_ERR_ARGUMENT;
     if (n == 0) return IB_OK;
-    const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, eps};
+    const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req, eps};
+    const int heads = n_heads + 2 * n_kv;
+    if (!is_f32 && !interleaved && rot_dim == d && (d == 64 || d == 128 || d == 256) && reinterpret_cast<uintptr_t>(qkv) % 8 == 0 && ldx % 4 == 0 &&
+        (reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) % 16 == 0) {
+        // few rows: every warp a step of its own; many: three, so that what belongs to a row is fetched less often
+        const int steps = (long)n * heads * d < 148L * 64 * 256 ? 1 : 3, per_block = STORE_WARPS * (256 / d) * steps;
+        const dim3 grid(n, (heads + per_block - 1) / per_block);
+#define GO(D, S, WT) ib_launch(kv8_store_whole_kernel<D, S, WT>, grid, dim3(32 * STORE_WARPS), 0, stream, (const __nv_bfloat16*)qkv, (const WT*)q_weight, \
+    (const WT*)k_weight, cos_table, sin_table, positions, row_request, block_table, (unsigned char*)k_pages, (unsigned char*)v_pages, \
+    k_scale, v_scale, (__nv_bfloat16*)q_out, a)
+#define GO_D(S, WT) (d == 64 ? GO(64, S, WT) : d == 128 ? GO(128, S, WT) : GO(256, S, WT))
+        if (w_is_f32) { if (steps == 1) GO_D(1, float); else GO_D(3, float); }
+        else { if (steps == 1) GO_D(1, __nv_bfloat16); else GO_D(3, __nv_bfloat16); }
+#undef GO_D
+#undef GO
+        return ib_launch_status();
+    }
     const dim3 grid(n, (n_heads + 2 * n_kv + STORE_WARPS - 1) / STORE_WARPS);
     const size_t smem = (size_t)STORE_WARPS * 2 * d * sizeof(float);
 #define GO(T, WT) ib_launch(kv8_store_kernel<T, WT>, grid, dim3(32 * STORE_WARPS), smem, stream, (const T*)qkv, (const WT*)q_weight, \

@@ -2421,7 +2421,7 @@ _FEW_BITS_SIGNATURES = {
 # IbAttentionKv8 in csrc/), packed at once: ctypes converts single arguments at 0.12 us each, 3.3 us for a call of 28.
 _QUANTIZE_CALL = struct.Struct("=8q").pack
 _GEMM_CALL = struct.Struct("=16q").pack
-_STORE_CALL = struct.Struct("=28qd").pack
+_STORE_CALL = struct.Struct("=29qd").pack
 _ATTENTION_CALL = struct.Struct("=27qd").pack
 _BF16_F32 = (torch.bfloat16, torch.float32)
 _F8, _F32, _I32 = torch.float8_e4m3fn, torch.float32, torch.int32
@@ -2633,7 +2633,7 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
         block_table.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
         q_out.data_ptr(), _stream(), act is torch.float32, ld, n, n_heads, n_kv_heads, head_dim,
         bool(weights) and weights[0].dtype is torch.float32, (q_weight is not None) | (k_weight is not None) << 1, rot_dim,
-        bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, eps)),
+        bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, block_table.shape[0], eps)),
         "qk_norm_rope_store_kv8")
 
 
