@@ -122,11 +122,21 @@ IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     return ib_launch_status();
 }
 
-IB_EXPORT int ib_dequantize_mx4(const void* codes, const void* scales, int rows, int width, void* out, int out_is_f32, long ldo,
-                                cudaStream_t stream) {
+struct IbDequantizeMx4 {
+    const void *codes, *scales;
+    void* out;
+    cudaStream_t stream;
+    long out_is_f32, ldo, rows, width;
+};
+IB_EXPORT int ib_dequantize_mx4(const IbDequantizeMx4* q) {
     using namespace few;
+    if (q->rows > 0x7FFFFFFF || q->width > (1 << 24)) return IB_ERR_UNSUPPORTED;
+    const void *codes = q->codes, *scales = q->scales;
+    void* out = q->out;
+    const cudaStream_t stream = q->stream;
+    const long ldo = q->ldo;
+    const int out_is_f32 = (int)q->out_is_f32, rows = (int)q->rows, width = (int)q->width;
     if (rows < 0 || width <= 0 || ldo < width) return IB_ERR_ARGUMENT;
-    if (width > (1 << 24)) return IB_ERR_UNSUPPORTED;
     if (rows == 0) return IB_OK;
     const size_t e = out_is_f32 ? 4 : 2;
     const int wide = (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * e) % 16 == 0) ? 1 : 0;

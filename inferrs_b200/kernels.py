@@ -2405,7 +2405,7 @@ def gemm_chain_error(reset: bool = True) -> int:
 _FEW_BITS_LIB, _FEW_BITS_PDL = None, False
 _FEW_BITS_SIGNATURES = {
     "ib_quantize_mx4": [ctypes.c_char_p],
-    "ib_dequantize_mx4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_long, c_void_p],
+    "ib_dequantize_mx4": [ctypes.c_char_p],
     "ib_gemm_mx4": [ctypes.c_char_p],
     "ib_gemm_mx4_error": [c_int],
     "ib_gemm_mx4_error_async": [c_void_p, c_void_p],
@@ -2417,9 +2417,9 @@ _FEW_BITS_SIGNATURES = {
     "ib_kv8_row_fault": [c_int],
     "ib_kv8_row_fault_async": [c_void_p, c_void_p],
 }
-# The calls of a decode step take their arguments as one structure of 8-byte fields (IbQuantizeMx4, IbGemmMx4, IbStoreKv8,
+# These calls take their arguments as one structure of 8-byte fields (IbQuantizeMx4, IbDequantizeMx4, IbGemmMx4, IbStoreKv8,
 # IbAttentionKv8 in csrc/), packed at once: ctypes converts single arguments at 0.12 us each, 3.3 us for a call of 28.
-_QUANTIZE_CALL = struct.Struct("=8q").pack
+_QUANTIZE_CALL = _DEQUANTIZE_CALL = struct.Struct("=8q").pack
 _GEMM_CALL = struct.Struct("=16q").pack
 _STORE_CALL = struct.Struct("=29qd").pack
 _ATTENTION_CALL = struct.Struct("=27qd").pack
@@ -2456,50 +2456,67 @@ def mx4_shapes(rows: int, width: int):
     return (rows, (width + 127) // 128 * 64), ((rows + 127) // 128, (width + 255) // 256 * 2, 32, 4, 4)
 
 
-@dataclass
 class Mx4Matrix:
     """A matrix [rows, width] of 4-bit numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with a power of two per 32 numbers of
     a row, in the layout that the kernels read (uint8):
 
     codes   [rows, 64 per 128 of width], two numbers a byte, the earlier one in the low half, zeros behind ``width``
     scales  [tile of 128 rows, tile of 128 columns (an even number), row % 32, row / 32 % 4, block of 32 % 4], the exponent
-            + 127 (255: the block holds no numbers), any but 255 behind ``width``"""
+            + 127 (255: the block holds no numbers), any but 255 behind ``width``
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    width: int
+    The constructor takes both; :meth:`empty` has them in one piece of memory (``codes`` and ``scales`` are views of it, made
+    when they are asked for)."""
 
-    def __post_init__(self):
-        c, s = self.codes, self.scales
-        if not (c.dtype is torch.uint8 and s.dtype is torch.uint8 and c.is_cuda and s.is_cuda and c.is_contiguous() and s.is_contiguous()):
-            _need(c, "codes", (torch.uint8,), 2)
-            _need(s, "scales", (torch.uint8,), 5)
-        want = mx4_shapes(self.rows, self.width) if self.rows >= 0 and self.width > 0 else (None, None)
-        if (tuple(self.codes.shape), tuple(self.scales.shape)) != want:
-            raise KernelError(f"a 4-bit matrix [{self.rows}, {self.width}] has codes and scales of shapes {want}, got "
-                              f"{tuple(self.codes.shape)} and {tuple(self.scales.shape)}")
-        if self.codes.data_ptr() % 32 or self.scales.data_ptr() % 16:
+    __slots__ = ("rows", "width", "device", "codes_at", "scales_at", "_codes", "_scales", "_memory")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int):
+        if not (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_cuda and scales.is_cuda
+                and codes.is_contiguous() and scales.is_contiguous()):
+            _need(codes, "codes", (torch.uint8,), 2)
+            _need(scales, "scales", (torch.uint8,), 5)
+        want = mx4_shapes(rows, width) if rows >= 0 and width > 0 else (None, None)
+        if (codes.shape, scales.shape) != want:
+            raise KernelError(f"a 4-bit matrix [{rows}, {width}] has codes and scales of shapes {want}, got "
+                              f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        self.rows, self.width, self.device = rows, width, codes.device
+        self.codes_at, self.scales_at = codes.data_ptr(), scales.data_ptr()
+        self._codes, self._scales, self._memory = codes, scales, None
+        if self.codes_at % 32 or self.scales_at % 16:
             raise KernelError("a 4-bit matrix's codes start on 32 bytes, its scales on 16")
 
     @classmethod
     def empty(cls, rows: int, width: int, device) -> "Mx4Matrix":
         if rows < 0 or width <= 0:
             raise KernelError(f"a 4-bit matrix has rows of at least one number, got [{rows}, {width}]")
-        codes, scales = mx4_shapes(rows, width)
-        return cls(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device),
-                   rows, width)
+        of_codes = rows * ((width + 127) // 128 * 64)
+        m = cls.__new__(cls)
+        m.rows, m.width, m._codes, m._scales = rows, width, None, None
+        m._memory = torch.empty(of_codes + (rows + 127) // 128 * ((width + 255) // 256) * 1024, dtype=torch.uint8, device=device)
+        m.device, m.codes_at = m._memory.device, m._memory.data_ptr()
+        m.scales_at = m.codes_at + of_codes
+        return m
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            shape = mx4_shapes(self.rows, self.width)[0]
+            self._codes = self._memory[:shape[0] * shape[1]].view(shape)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            codes, scales = mx4_shapes(self.rows, self.width)
+            self._scales = self._memory[codes[0] * codes[1]:].view(scales)
+        return self._scales
 
     @property
     def shape(self):
         return (self.rows, self.width)
 
-    @property
-    def device(self):
-        return self.codes.device
-
     def bytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        codes, scales = mx4_shapes(self.rows, self.width)
+        return codes[0] * codes[1] + scales[0] * scales[1] * 512
 
 
 def quantize_mx4(x: torch.Tensor, out: Optional[Mx4Matrix] = None) -> Mx4Matrix:
@@ -2511,10 +2528,10 @@ def quantize_mx4(x: torch.Tensor, out: Optional[Mx4Matrix] = None) -> Mx4Matrix:
     rows, width = x.shape
     if out is None:
         out = Mx4Matrix.empty(rows, width, x.device)
-    elif out.shape != (rows, width):
+    elif out.rows != rows or out.width != width:
         raise KernelError(f"quantize_mx4: x {(rows, width)} for a matrix {out.shape}")
-    _check(_few_bits().ib_quantize_mx4(_QUANTIZE_CALL(x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), _stream(),
-                                                      x.dtype is torch.float32, ld, rows, width)), "quantize_mx4")
+    _check(_few_bits().ib_quantize_mx4(_QUANTIZE_CALL(x.data_ptr(), out.codes_at, out.scales_at, _stream(), x.dtype is _F32, ld,
+                                                      rows, width)), "quantize_mx4")
     return out
 
 
@@ -2524,8 +2541,8 @@ def dequantize_mx4(w: Mx4Matrix, out: torch.Tensor):
     ld = _need_rows(out, "out", _BF16_F32)
     if out.shape != w.shape:
         raise KernelError(f"dequantize_mx4: a matrix {w.shape} into {tuple(out.shape)}")
-    _check(_few_bits().ib_dequantize_mx4(w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.width, out.data_ptr(),
-                                         out.dtype == torch.float32, ld, _stream()), "dequantize_mx4")
+    _check(_few_bits().ib_dequantize_mx4(_DEQUANTIZE_CALL(w.codes_at, w.scales_at, out.data_ptr(), _stream(), out.dtype is _F32, ld,
+                                                          w.rows, w.width)), "dequantize_mx4")
 
 
 MX4_INSIDE_ROWS = 8      # up to so many bfloat16 rows the product needs no workspace (INSIDE_ROWS in csrc/gemm_mx4.cu)
@@ -2542,14 +2559,14 @@ def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: i
     n, k = x.shape
     if k != w.width or out.shape != (n, w.rows):
         raise KernelError(f"linear_mx4: x {(n, k)}, w {w.shape}, out {tuple(out.shape)}")
-    kind = 2 if coded else int(x.dtype is torch.float32)
+    kind = 2 if coded else int(x.dtype is _F32)
     lib, workspace, at = _few_bits(), None, 0
     if kind == 1 or (kind == 0 and n > MX4_INSIDE_ROWS):
-        workspace = torch.empty((lib.ib_gemm_mx4_workspace(kind, n, k),), dtype=torch.uint8, device=out.device)
+        workspace = torch.empty(lib.ib_gemm_mx4_workspace(kind, n, k), dtype=torch.uint8, device=out.device)
         at = workspace.data_ptr()
-    _check(lib.ib_gemm_mx4(_GEMM_CALL((x.codes if coded else x).data_ptr(), x.scales.data_ptr() if coded else 0, w.codes.data_ptr(),
-                                      w.scales.data_ptr(), out.data_ptr(), at, _stream(), kind, ldx, n, w.rows, k,
-                                      out.dtype is torch.float32, ldy, tile_rows, splits)), "linear_mx4")
+    _check(lib.ib_gemm_mx4(_GEMM_CALL(x.codes_at if coded else x.data_ptr(), x.scales_at if coded else 0, w.codes_at, w.scales_at,
+                                      out.data_ptr(), at, _stream(), kind, ldx, n, w.rows, k, out.dtype is _F32, ldy, tile_rows,
+                                      splits)), "linear_mx4")
 
 
 @dataclass
@@ -2616,23 +2633,27 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
             or (nkv, d) != (n_kv_heads, head_dim):
         raise KernelError(f"qk_norm_rope_store_kv8: qkv {tuple(qkv.shape)} (want {cols} columns), q_out {tuple(q_out.shape)}, "
                           f"positions {tuple(positions.shape)}, pages {tuple(pages.k.shape)}")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        _need(w, "norm weight", _W, 1)
-        if w.shape[0] != head_dim or w.dtype != weights[0].dtype:
+    w_type = None
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        w_type = w_type or w.dtype
+        if not (w.dtype is w_type and w.is_cuda and w.shape == (head_dim,) and w.is_contiguous() and w_type in _W):
+            _need(w, "norm weight", _W, 1)
             raise KernelError(f"qk_norm_rope_store_kv8: norm weights of {head_dim} numbers of one type, got {tuple(w.shape)}, "
                               f"{w.dtype}")
     if rot_dim:
-        _need(cos, "cos", (torch.float32,), 2)
-        _need(sin, "sin", (torch.float32,), 2)
+        if not (cos.dtype is _F32 and sin.dtype is _F32 and cos.is_cuda and sin.is_cuda and cos.dim() == 2
+                and cos.is_contiguous() and sin.is_contiguous()):
+            _need(cos, "cos", (torch.float32,), 2)
+            _need(sin, "sin", (torch.float32,), 2)
         if cos.shape[1] != rot_dim // 2 or sin.shape != cos.shape or rot_dim % 2 or not 0 < rot_dim <= head_dim:
             raise KernelError(f"rotation tables {tuple(cos.shape)} do not match rot_dim {rot_dim}")
     _check(_few_bits().ib_qk_norm_rope_store_kv8(_STORE_CALL(
         qkv.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
         cos.data_ptr() if rot_dim else 0, sin.data_ptr() if rot_dim else 0, positions.data_ptr(), row_request.data_ptr(),
         block_table.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-        q_out.data_ptr(), _stream(), act is torch.float32, ld, n, n_heads, n_kv_heads, head_dim,
-        bool(weights) and weights[0].dtype is torch.float32, (q_weight is not None) | (k_weight is not None) << 1, rot_dim,
+        q_out.data_ptr(), _stream(), act is _F32, ld, n, n_heads, n_kv_heads, head_dim, w_type is _F32, (q_weight is not None) | (k_weight is not None) << 1, rot_dim,
         bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, block_table.shape[0], eps)),
         "qk_norm_rope_store_kv8")
 
