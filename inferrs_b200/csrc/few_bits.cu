@@ -117,8 +117,8 @@ IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     const int wide = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * e) % 16 == 0) ? 1 : 0;
     const dim3 grid(blocks_for(rows, width));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (x_is_f32) ib_launch(quantize_kernel<float>, grid, dim3(256), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
-    else ib_launch(quantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
+    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(256), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
+    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
     return ib_launch_status();
 }
 
@@ -142,7 +142,7 @@ IB_EXPORT int ib_dequantize_mx4(const IbDequantizeMx4* q) {
     const int wide = (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * e) % 16 == 0) ? 1 : 0;
     const dim3 grid(blocks_for(rows, width));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (out_is_f32) ib_launch(dequantize_kernel<float>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (float*)out, ldo);
-    else ib_launch(dequantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (__nv_bfloat16*)out, ldo);
+    if (out_is_f32) ib_launch_early(dequantize_kernel<float>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (float*)out, ldo);
+    else ib_launch_early(dequantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (__nv_bfloat16*)out, ldo);
     return ib_launch_status();
 }

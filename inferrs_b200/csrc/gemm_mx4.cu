@@ -50,6 +50,7 @@ struct Params {
     const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
     long ldx;
     int k, wide;                             // wide: rows start on 16 bytes
+    int wait_first;                          // the kernel ahead may have written the weights: nothing is read before it is done
 };
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -311,6 +312,7 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
+    if (p.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (splits > 1) cluster_arrive();       // "this CTA runs": looked at before the first store to it
 
     if (warp == 0) {
@@ -449,6 +451,7 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
+    if (p.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
     // Copies are issued by two threads, one for the operands and one for their scales: a thread takes 165 cycles a tile and 50 a
     // plain copy, five of which together would take longer than the products of a stage.
     if (warp == 0 || warp == 6) {
@@ -659,7 +662,8 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ib_pdl_enabled || early ? 2 : 1;      // early: the kernel ahead is pieces_kernel
+    cfg.numAttrs = 2;
+    p.wait_first = !ib_pdl_enabled && !early;      // early: the kernel ahead is pieces_kernel
     const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<KIND, BN, INSIDE>, map_w, map_x, p, sh);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
@@ -684,7 +688,8 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ib_pdl_enabled || early ? 1 : 0;
+    cfg.numAttrs = 1;
+    p.wait_first = !ib_pdl_enabled && !early;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, p);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
@@ -694,7 +699,7 @@ static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((
 template <typename T, int PARTS>
 static int make_pieces(const void* x, long ldx, int n, int k, int wide, unsigned char* pieces, cudaStream_t stream) {
     const long threads = (long)n * ((k + 127) / 128 * 16), blocks = (threads + 255) / 256;
-    ib_launch(pieces_kernel<T, PARTS>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide,
+    ib_launch_early(pieces_kernel<T, PARTS>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide,
               (uint2*)pieces, (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }

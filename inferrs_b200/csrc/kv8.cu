@@ -24,7 +24,7 @@ constexpr int STORE_WARPS = 4;
 
 struct StoreArgs {
     long ldx;
-    int n_heads, n_kv, d, flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req;   // flags: 1 norm q, 2 norm k
+    int n_heads, n_kv, d, flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req, wait_first;   // flags: 1 norm q, 2 norm k
     float eps;
 };
 
@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
     ib_grid_dependency_launch();
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = 4 * (lane % LANES);
     const int head0 = ((int)blockIdx.y * STORE_WARPS + warp) * HEADS * STEPS + lane / LANES, heads = a.n_heads + 2 * a.n_kv;
+    if (a.wait_first) ib_grid_dependency_wait();
     const int pos = positions[row], req = row_request[row];
     const bool fault = pos < 0 || pos >= a.table_rows;
     const float4 c = fault ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(cos_table + (long)pos * (D / 2) + i);
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
     const int head = blockIdx.y * STORE_WARPS + warp;
     float* sh = smem + warp * 2 * d;      // the head as it came, and turned
     float* turned = sh + d;
+    if (a.wait_first) ib_grid_dependency_wait();
     const int pos = positions[row];
     const bool fault = pos < 0 || (a.rot_dim > 0 && pos >= a.table_rows);
     ib_grid_dependency_wait();
@@ -293,14 +295,14 @@ IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
     const float eps = (float)s->eps;
     if (n < 0 || n_heads <= 0 || n_kv <= 0 || d <= 0 || d % 4 || d > 1024 || rot_dim < 0 || rot_dim > d || rot_dim % 2 || page_size <= 0) return IB_ERR_ARGUMENT;
     if (n == 0) return IB_OK;
-    const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req, eps};
+    const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req, !ib_pdl_enabled, eps};
     const int heads = n_heads + 2 * n_kv;
     if (!is_f32 && !interleaved && rot_dim == d && (d == 64 || d == 128 || d == 256) && reinterpret_cast<uintptr_t>(qkv) % 8 == 0 && ldx % 4 == 0 &&
         (reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) % 16 == 0) {
         // few rows: every warp a step of its own; many: three, so that what belongs to a row is fetched less often
         const int steps = (long)n * heads * d < 148L * 64 * 256 ? 1 : 3, per_block = STORE_WARPS * (256 / d) * steps;
         const dim3 grid(n, (heads + per_block - 1) / per_block);
-#define GO(D, S, WT) ib_launch(kv8_store_whole_kernel<D, S, WT>, grid, dim3(32 * STORE_WARPS), 0, stream, (const __nv_bfloat16*)qkv, (const WT*)q_weight, \
+#define GO(D, S, WT) ib_launch_early(kv8_store_whole_kernel<D, S, WT>, grid, dim3(32 * STORE_WARPS), 0, stream, (const __nv_bfloat16*)qkv, (const WT*)q_weight, \
     (const WT*)k_weight, cos_table, sin_table, positions, row_request, block_table, (unsigned char*)k_pages, (unsigned char*)v_pages, \
     k_scale, v_scale, (__nv_bfloat16*)q_out, a)
 #define GO_D(S, WT) (d == 64 ? GO(64, S, WT) : d == 128 ? GO(128, S, WT) : GO(256, S, WT))
@@ -312,7 +314,7 @@ IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
     }
     const dim3 grid(n, (n_heads + 2 * n_kv + STORE_WARPS - 1) / STORE_WARPS);
     const size_t smem = (size_t)STORE_WARPS * 2 * d * sizeof(float);
-#define GO(T, WT) ib_launch(kv8_store_kernel<T, WT>, grid, dim3(32 * STORE_WARPS), smem, stream, (const T*)qkv, (const WT*)q_weight, \
+#define GO(T, WT) ib_launch_early(kv8_store_kernel<T, WT>, grid, dim3(32 * STORE_WARPS), smem, stream, (const T*)qkv, (const WT*)q_weight, \
     (const WT*)k_weight, cos_table, sin_table, positions, row_request, block_table, (unsigned char*)k_pages, (unsigned char*)v_pages, \
     k_scale, v_scale, (T*)q_out, a)
     if (is_f32) { if (w_is_f32) GO(float, float); else GO(float, __nv_bfloat16); }
@@ -332,7 +334,7 @@ IB_EXPORT int ib_paged_attention_kv8_generic(const void* q, int is_f32, const vo
     if (n == 0) return IB_OK;
     const AttendArgs a = {max_pages, page_size, n_pages, n_req, n_heads, n_kv, d, span, scale, out_ld};
     const dim3 grid(n, n_heads);
-#define GO(T) ib_launch(kv8_attention_kernel<T>, grid, dim3(32 * SLOW_WARPS), 0, stream, (const T*)q, (const unsigned char*)k_pages, \
+#define GO(T) ib_launch_early(kv8_attention_kernel<T>, grid, dim3(32 * SLOW_WARPS), 0, stream, (const T*)q, (const unsigned char*)k_pages, \
     (const unsigned char*)v_pages, k_scale, v_scale, block_table, row_request, positions, (T*)out, a)
     if (is_f32) GO(float); else GO(__nv_bfloat16);
 #undef GO
