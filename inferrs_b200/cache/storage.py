@@ -17,6 +17,7 @@ from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..kernels import Kv8Pages
 from .manager import GroupLayout
 
 
@@ -44,17 +45,31 @@ class StateNeed:
     dtype: torch.dtype = torch.float32
 
 
+def bytes_of_vectors(need: KVNeed, dtype: torch.dtype, bits: Optional[int]) -> int:
+    """Bytes of one token's keys and values in one cache."""
+    if bits == 8:
+        return need.n_kv_heads * 2 * (need.head_dim + 4)
+    return need.n_kv_heads * (need.head_dim * (need.planes - 1) + (need.value_dim or need.head_dim)) \
+        * torch.empty((), dtype=dtype).element_size()
+
+
 class CacheStorage:
     def __init__(self, kv_needs: Dict[int, KVNeed], state_needs: Dict[int, StateNeed], page_size: int,
                  n_pages: int, max_requests: int, dtype: torch.dtype, device: torch.device,
                  n_pages_per_group: Optional[Sequence[int]] = None,
-                 side_state_needs: Optional[Dict[Tuple[int, Any], StateNeed]] = None):
-        """``side_state_needs``: per-request states beside a mixer's own, keyed by (cache id, the description that
+                 side_state_needs: Optional[Dict[Tuple[int, Any], StateNeed]] = None, bits: Optional[int] = None):
+        """``bits`` 8: keys and values in 8 bits (``pages8``; ``pages`` then has nothing to give).
+        ``side_state_needs``: per-request states beside a mixer's own, keyed by (cache id, the description that
         owns the state): the inputs that a short convolution in front of a sub-layer or behind a projection keeps."""
         self.page_size = page_size
         self.max_requests = max_requests
         self.dtype = dtype
         self.device = device
+        self.bits = bits
+        if bits not in (None, 8):
+            raise ValueError(f"keys and values are cached in the activations' type or in 8 bits, got {bits} bits")
+        if bits == 8 and any(k.planes != 2 or k.value_dim not in (None, k.head_dim) or k.head_dim % 4 for k in kv_needs.values()):
+            raise ValueError("a cache in 8 bits holds keys and values of one size, a multiple of four numbers")
         # caches with equal needs form a group, in order of first appearance
         keys: List[KVNeed] = []
         self.group_of: Dict[int, int] = {}
@@ -84,10 +99,19 @@ class CacheStorage:
         if any(k.value_dim is not None and k.planes != 2 for k in keys):
             raise ValueError("values of a size of their own need a cache of two planes")
         self.kv: List[torch.Tensor] = []
+        # in 8 bits: codes in ``kv``, and one float32 scale per vector [caches in group, 2, pages, kv_heads, page_size]
+        self.scales: List[torch.Tensor] = []
+        self._pages8: Dict[int, Kv8Pages] = {}
         # values whose heads have another size than the keys': [caches in group, pages, kv_heads, page_size, value_dim]
         # (the group's tensor in ``kv`` then holds the keys alone)
         self.values: List[Optional[torch.Tensor]] = []
         for g, k in enumerate(keys):
+            if bits == 8:
+                shape = (len(members[g]), 2, self.n_pages[g], k.n_kv_heads, page_size, k.head_dim)
+                self.kv.append(torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn))
+                self.scales.append(torch.zeros(shape[:-1], dtype=torch.float32, device=device))
+                self.values.append(None)
+                continue
             own_values = k.value_dim is not None and k.value_dim != k.head_dim
             self.kv.append(torch.zeros((len(members[g]), 1 if own_values else k.planes, self.n_pages[g], k.n_kv_heads,
                                         page_size, k.head_dim), dtype=dtype, device=device))
@@ -105,11 +129,22 @@ class CacheStorage:
         """(key pages, value pages, group index) of one cache; pages are [n_pages, kv_heads, page_size, head_dim]
         (value pages end in the group's ``value_dim`` where it has one).
         A cache of one plane gives the same pages twice."""
+        if self.bits is not None:
+            raise ValueError(f"this cache holds {self.bits} bits a number: ask pages8")
         g = self.group_of[cache_id]
         t = self.kv[g][self.index_in_group[cache_id]]
         if self.values[g] is not None:
             return t[0], self.values[g][self.index_in_group[cache_id]], g
         return t[0], t[t.shape[0] - 1], g
+
+    def pages8(self, cache_id: int) -> Tuple[Kv8Pages, int]:
+        """(pages of keys and values in 8 bits, group index) of one cache."""
+        g = self.group_of[cache_id]
+        if cache_id not in self._pages8:
+            i = self.index_in_group[cache_id]
+            codes, scales = self.kv[g][i], self.scales[g][i]
+            self._pages8[cache_id] = Kv8Pages(codes[0], codes[1], scales[0], scales[1])
+        return self._pages8[cache_id], g
 
     def state(self, cache_id: int) -> torch.Tensor:
         return self.states[cache_id]
@@ -138,12 +173,11 @@ class CacheStorage:
 
     def bytes_per_token(self) -> int:
         """Bytes of keys and values that one token adds, over all groups."""
-        e = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(self.members[g]) * k.n_kv_heads * (k.head_dim * (k.planes - 1) + (k.value_dim or k.head_dim)) * e
-                   for g, k in enumerate(self.needs))
+        return sum(len(self.members[g]) * bytes_of_vectors(k, self.dtype, self.bits) for g, k in enumerate(self.needs))
 
     def total_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.kv) + \
             sum(t.numel() * t.element_size() for t in self.values if t is not None) + \
+            sum(t.numel() * t.element_size() for t in self.scales) + \
             sum(t.numel() * t.element_size() for t in self.states.values()) + \
             sum(t.numel() * t.element_size() for t in self.side_states.values())

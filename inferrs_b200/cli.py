@@ -14,7 +14,7 @@ inferrs/src/bench.rs:21-38 ``bench``).  The model is a local folder (the referen
 (``replay`` is the trace replay program, ``bin/trace_run``, under this command's roof: ``engine/trace.py``.)
 
 Beyond the reference's options: ``--prefill-chunk`` (the most tokens of one prompt in a step), ``--ignore-eos``,
-``--min-p``, ``--random-weights SEED`` (the model argument is then a config.json, or a folder with one, and the
+``--weight-bits 4`` and ``--cache-bits 8`` (a model in few bits), ``--min-p``, ``--random-weights SEED`` (the model argument is then a config.json, or a folder with one, and the
 weights are made on the device), ``--random-prompt LEN`` and ``--prompt-file``.
 """
 from __future__ import annotations
@@ -31,6 +31,10 @@ from typing import List, Optional
 def _shared(ap: argparse.ArgumentParser):
     ap.add_argument("model", help="folder with config.json and model.safetensors (or *.safetensors shards)")
     ap.add_argument("--dtype", default="bf16", help="weight and activation type: bf16 or f32 (default bf16)")
+    ap.add_argument("--weight-bits", type=int, default=None, choices=(4,),
+                    help="keep the layers' projections in 4 bits with a power of two per 32 weights (default: as loaded)")
+    ap.add_argument("--cache-bits", type=int, default=None, choices=(8,),
+                    help="cache keys and values in 8 bits with a scale per vector (default: the activations' type)")
     ap.add_argument("--max-seq-len", type=int, default=0, help="maximum sequence length (0 = model default)")
     ap.add_argument("--block-size", type=int, default=16, help="KV cache block size in tokens")
     ap.add_argument("--max-blocks", type=int, default=0,
@@ -57,7 +61,7 @@ def _engine(args):
     common = dict(dtype=args.dtype, block_size=args.block_size, num_blocks=args.max_blocks or None,
                   paged_attention=args.paged_attention, max_batch_size=args.max_batch_size,
                   max_tokens_per_step=args.max_tokens_per_step, max_seq_len=args.max_seq_len,
-                  prefill_chunk=args.prefill_chunk or None)
+                  prefill_chunk=args.prefill_chunk or None, weight_bits=args.weight_bits, cache_bits=args.cache_bits)
     if args.random_weights is not None:
         path = os.path.join(args.model, "config.json") if os.path.isdir(args.model) else args.model
         with open(path, "r", encoding="utf-8") as f:

@@ -30,7 +30,6 @@ namespace kv8 {
 
 using namespace sm100;
 
-
 constexpr int WARPS = 4, THREADS = 32 * WARPS, KEYS = 16;
 constexpr float NONE = -1e30f;        // below every score
 constexpr float SLACK = 8.0f;         // how far a number may outgrow its reference
@@ -95,7 +94,7 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
     extern __shared__ __align__(16) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    int tile = blockIdx.y;
+    int tile = a.tile_req != nullptr ? gridDim.y - 1 - blockIdx.y : blockIdx.y;      // a list's longest tile stands last in it
     const int rank = blockIdx.x % a.splits, kv_chunk = blockIdx.x / a.splits;
     if (a.ranked) {      // up to 32 single tokens: the longest request's CTAs come first, so that no long one starts last
         const int mine = lane < a.n_rows ? a.positions[lane] : -2;

@@ -31,7 +31,7 @@ struct StoreArgs {
 // Heads of 64, 128 or 256 numbers that turn as a whole, element i with i + d / 2, in bfloat16: a lane holds four numbers of the
 // first half of a head and the four they turn with, a warp 256 / D heads at a time and STEPS times, whose loads are all on their way
 // before the first is used; what belongs to the row (its place, its angles) is fetched once.  2,048 rows of 32 + 8 + 8 heads of 128:
-// 47 MB, 51 us with a warp a head through shared memory, TIME like this.
+// 47 MB, 51 us with a warp a head through shared memory, 16 us like this.
 template <int D, int STEPS, typename WT>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
     const __nv_bfloat16* __restrict__ qkv, const WT* __restrict__ q_weight, const WT* __restrict__ k_weight,

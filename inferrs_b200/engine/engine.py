@@ -32,6 +32,9 @@ class Engine:
     """
     model_dir            folder with config.json and model.safetensors (or shards)
     dtype                "bf16" (default) or "f32"
+    weight_bits          4: the layers' projections keep their weights in 4 bits with a power of two per 32 of them
+    cache_bits           8: keys and values are cached in 8 bits with a scale per vector (both: see
+                         :class:`~inferrs_b200.runtime.Runtime`; a ``runtime`` that is given brings its own)
     block_size           tokens per cache page (reference: --block-size, 16)
     num_blocks           pages in the cache; None: sized from ``paged_attention``
     paged_attention      fraction of the device's free memory, after the weights, given to the cache
@@ -53,8 +56,9 @@ class Engine:
                  num_blocks: Optional[int] = None, paged_attention: float = 0.9, max_batch_size: int = 32,
                  max_tokens_per_step: int = 2048, max_seq_len: int = 0, prefill_chunk: Optional[int] = None,
                  config: Optional[dict] = None, random_weights: Optional[int] = None,
-                 runtime: Optional[Runtime] = None, overlap: bool = True):
-        self.rt = runtime if runtime is not None else Runtime.cuda(parse_dtype(dtype))
+                 runtime: Optional[Runtime] = None, overlap: bool = True, weight_bits: Optional[int] = None,
+                 cache_bits: Optional[int] = None):
+        self.rt = runtime if runtime is not None else Runtime.cuda(parse_dtype(dtype), weight_bits, cache_bits)
         if model_dir is not None:
             spec, weights, cfg = load_model_dir(model_dir, self.rt)
         elif config is not None and random_weights is not None:

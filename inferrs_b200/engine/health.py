@@ -42,8 +42,9 @@ class KernelHealth:
             return None
         self.event.synchronize()
         self.event = None
-        words = self.host[:len(kernels.ERROR_WORDS)].tolist()
-        return {name: int(v) for name, v in zip(kernels.ERROR_WORDS, words) if v}
+        names = kernels.ERROR_WORDS + kernels.FEW_BITS_WORDS
+        words = self.host[:len(names)].tolist()
+        return {name: int(v) for name, v in zip(names, words) if v}
 
     def reset(self) -> Dict[str, int]:
         """Clear the words on the device (waits for it); returns what was set."""

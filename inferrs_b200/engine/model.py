@@ -192,6 +192,11 @@ class Model:
                     if getattr(sub, "sum_norm", None) is not None else None
                 # a sub-layer without a part (an arrangement may allow it) is its norms alone
                 part = part_class(sub.category, sub.part)(sub.part, weights, rt) if sub.part is not None else None
+                for bits, can in ((rt.weight_bits, "few_bit_weights"), (rt.cache_bits if sub.category == "mixer" else None,
+                                                                        "few_bit_cache")):
+                    if bits is not None and part is not None and not getattr(part, can, False):
+                        raise ModelError(f"layer {i}: a {sub.part.kind} has no form with "
+                                         f"{'weights in 4 bits' if can == 'few_bit_weights' else 'a cache in 8 bits'}")
                 built.append(BuiltSubLayer(sub.category, part, norm, post, sum_norm))
             arrangement = part_class("arrangement", _Arrangement(layer.arrangement))
             if getattr(arrangement, "needs_weights", False):

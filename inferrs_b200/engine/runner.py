@@ -17,7 +17,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import torch
 
 from ..cache.manager import CacheManager, OutOfPages
-from ..cache.storage import CacheStorage
+from ..cache.storage import CacheStorage, bytes_of_vectors
 from ..parts.spec import ModelSpec
 from ..runtime import Runtime
 from .batch import StepContext, StepEntry, build_context
@@ -44,7 +44,7 @@ class ModelRunner:
             n_pages = self._pages_for_fraction(kv_needs, page_size, cache_fraction, max_requests,
                                                min(max_context or spec.max_positions, spec.max_positions))
         self.storage = CacheStorage(kv_needs, state_needs, page_size, n_pages, max_requests, rt.dtype, rt.device,
-                                    side_state_needs=side_state_needs(spec))
+                                    side_state_needs=side_state_needs(spec), bits=rt.cache_bits)
         self.manager = CacheManager(self.storage.layouts, page_size, self.storage.n_pages, max_requests)
         self.page_size = page_size
         self.steps_run = 0
@@ -73,9 +73,7 @@ class ModelRunner:
         import gc
         gc.collect()
         torch.cuda.empty_cache()        # what the loader and the fusing of tensors have given back
-        elem = torch.empty((), dtype=self.rt.dtype).element_size()
-        per_page = sum(n.n_kv_heads * (n.head_dim * (n.planes - 1) + (getattr(n, 'value_dim', None) or n.head_dim))
-                       * page_size * elem for n in kv_needs.values())
+        per_page = sum(bytes_of_vectors(n, self.rt.dtype, self.rt.cache_bits) * page_size for n in kv_needs.values())
         free, _total = torch.cuda.mem_get_info(self.rt.device)
         pages = int(free * fraction) // max(per_page, 1)
         # no request can use more than max_context tokens: more pages than that per slot are never touched

@@ -2653,8 +2653,8 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
         qkv.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
         cos.data_ptr() if rot_dim else 0, sin.data_ptr() if rot_dim else 0, positions.data_ptr(), row_request.data_ptr(),
         block_table.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-        q_out.data_ptr(), _stream(), act is _F32, ld, n, n_heads, n_kv_heads, head_dim, w_type is _F32, (q_weight is not None) | (k_weight is not None) << 1, rot_dim,
-        bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, block_table.shape[0], eps)),
+        q_out.data_ptr(), _stream(), act is _F32, ld, n, n_heads, n_kv_heads, head_dim, w_type is _F32,
+        (q_weight is not None) | (k_weight is not None) << 1, rot_dim, bool(interleaved), cos.shape[0] if rot_dim else 0, block_table.shape[1], page_size, n_pages, block_table.shape[0], eps)),
         "qk_norm_rope_store_kv8")
 
 
@@ -2744,7 +2744,8 @@ ERROR_WORDS = ("a row's position outside the rotation tables", "prefill attentio
 
 def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
     """Ask for every error word of the kernel libraries, in the order of ``ERROR_WORDS``, to be copied into ``host``
-    (pinned int32, at least ``len(ERROR_WORDS)`` long) behind the work that the current stream holds.  The caller
+    (pinned int32, at least ``len(ERROR_WORDS)`` long; with room for them, those of the kernels in few bits follow) behind
+    the work that the current stream holds.  The caller
     records an event after this call and reads ``host`` once the event has come."""
     if host.dtype != torch.int32 or host.numel() < len(ERROR_WORDS) or not host.is_pinned():
         raise KernelError("error_words_async wants a pinned int32 tensor with room for every word")
@@ -2756,6 +2757,13 @@ def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
     else:
         calls.append(_split_lib().ib_gemm_split_error_async)     # in the place of the bfloat16 products
         host[len(calls):len(ERROR_WORDS)] = 0
+    if host.numel() >= len(ERROR_WORDS) + len(FEW_BITS_WORDS):       # those of the kernels in few bits behind them
+        host[len(ERROR_WORDS):len(ERROR_WORDS) + len(FEW_BITS_WORDS)] = 0
+        if _FEW_BITS_LIB is not None:
+            for i, fn in enumerate((_FEW_BITS_LIB.ib_kv8_row_fault_async, _FEW_BITS_LIB.ib_gemm_mx4_error_async)):
+                code = fn(at + 4 * (len(ERROR_WORDS) + i), stream)
+                if code != 0:
+                    raise KernelError(f"error_words_async: CUDA error {code}")
     for i, fn in enumerate(calls):
         code = fn(at + 4 * i, stream)
         if code != 0:
@@ -2778,6 +2786,7 @@ def reset_error_words(act_dtype: torch.dtype) -> dict:
         v = fn(True)
         if v:
             found[name] = v
+    found.update(few_bits_faults(reset=True))
     for counters in _DECODE_COUNTERS.values():
         counters.zero_()
     return found

@@ -28,6 +28,8 @@ from .spec import AttentionSpec, TensorDecl
 
 class Attention:
     graph_safe = True  # launches depend only on shapes, never on the step's host-side values
+    few_bit_weights = True
+    few_bit_cache = True      # (plain attention: what the constructor refuses has no kernels for a cache in 8 bits)
 
     @staticmethod
     def declare(spec: AttentionSpec) -> List[TensorDecl]:
@@ -128,6 +130,16 @@ class Attention:
             raise ValueError("query and key norms must share eps")
         if spec.window and spec.chunk:
             raise ValueError("an attention layer has a sliding window or chunks, not both")
+        if rt.cache_bits is not None and (
+                self.fused or not spec.own_kv or spec.value_is_key or spec.value_blend is not None or spec.value_publish is not None
+                or spec.value_dim not in (None, spec.head_dim) or spec.head_dim % 4 or spec.norm_after_rotation or spec.keep_first
+                or any(x is not None for x in (spec.q_bias, spec.k_bias, spec.v_bias, spec.distance_bias, spec.head_mix,
+                                               spec.head_scale, spec.sink, spec.sink_score, spec.distance_slopes, spec.score_cap,
+                                               spec.head_gate))
+                or any(x is not None and x.weight is None for x in (spec.q_norm, spec.k_norm))):
+            raise ValueError("keys and values in 8 bits: attention with its own keys and values, norms per head with weights "
+                             "before the rotation, a window or chunks; no biases, blends, factors, penalties, sinks, caps or gates "
+                             "per head")
         self.spec = spec
         self.rt = rt
         self.value_dim = spec.value_dim or spec.head_dim
@@ -147,7 +159,7 @@ class Attention:
         # projection before it or another kernel stores, behind the product
         bias = self._fused_bias(spec, weights, rt)
         behind = self.fused or spec.value_blend is not None or spec.value_publish is not None
-        self.qkv = Linear(fuse_rows(mats), rt, bias=bias if behind else None)
+        self.qkv = Linear(fuse_rows(mats), rt, bias=bias if behind else None, bits=rt.weight_bits)
         self.store_bias = None if behind else bias
         f32 = lambda name: weights[name].to(torch.float32).contiguous()     # noqa: E731
         self.head_scale = None if spec.head_scale is None else f32(spec.head_scale)
@@ -160,7 +172,7 @@ class Attention:
         self.conv = None if spec.qkv_conv is None else \
             torch.cat([f32(n) for n in spec.qkv_conv], dim=0).t().contiguous()
         self.blend_weight = None if spec.value_blend is None else f32(spec.value_blend[1]).reshape(1)
-        self.o = Linear(weights[spec.o_proj], rt, bias=None if spec.o_bias is None else weights[spec.o_bias])
+        self.o = Linear(weights[spec.o_proj], rt, bias=None if spec.o_bias is None else weights[spec.o_bias], bits=rt.weight_bits)
         # scores penalised by distance and mixed across heads: the mixing is linear, so it is done on the queries
         # (one vector per key/value head and query head, see kernels.mix_queries), and the penalty, mixed the same
         # way, is a table [heads, distances] that the attention kernel takes off the scores
@@ -229,7 +241,8 @@ class Attention:
     # A block whose sub-layers all read the same rows may make this part's two products in one with the others'
     # (see ParallelBlock).
     def joins_products(self) -> bool:
-        return self.qkv is not None and self.qkv.bias is None and self.spec.gate_proj is None and not self.talking
+        return self.qkv is not None and self.qkv.bias is None and self.qkv.mx4 is None and self.spec.gate_proj is None \
+            and not self.talking
 
     def hand_over_products(self):
         products = (self.qkv.weight, self.o.weight, self.o.bias)
@@ -243,6 +256,9 @@ class Attention:
         """From the projected rows to the heads side by side in ``out`` (whose rows may lie apart)."""
         s = self.spec
         n = qkv.shape[0]
+        if self.rt.cache_bits is not None:
+            self._attend_kv8(ctx, cache_id, qkv, out)
+            return
         k_pages, v_pages, group = ctx.storage.pages(cache_id)
         table = ctx.block_tables[group]
         q = torch.empty((n, s.n_heads, s.head_dim), dtype=self.rt.dtype, device=qkv.device)
@@ -277,6 +293,23 @@ class Attention:
         else:
             gate = None if s.head_gate is None else qkv[:, self.head_gate_col:self.head_gate_col + s.n_heads]
             kernels.paged_attention(q, k_pages, v_pages, table, ctx, s.scale, self.span, out, **self._options(gate))
+
+    def _attend_kv8(self, ctx, cache_id: int, qkv: torch.Tensor, out: torch.Tensor):
+        """The same over a cache in 8 bits: a step of single tokens one row each, a step with portions of prompts in tiles."""
+        s = self.spec
+        pages, group = ctx.storage.pages8(cache_id)
+        table = ctx.block_tables[group]
+        q = torch.empty((qkv.shape[0], s.n_heads, s.head_dim), dtype=self.rt.dtype, device=qkv.device)
+        kernels.qk_norm_rope_store_kv8(qkv, s.n_heads, s.n_kv_heads, s.head_dim, self.q_weight, self.k_weight, self.eps, self.cos,
+                                       self.sin, self.rot_dim, ctx.positions, ctx.row_request, table, pages, q,
+                                       interleaved=self.interleaved)
+        tiles = None
+        if not ctx.decode_only:
+            tokens = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim)
+            tile_req, tile_row0, n_tiles = ctx.attention_tiles(tokens)
+            tiles = (tile_req, tile_row0, n_tiles, ctx.q_start, tokens)
+        kernels.paged_attention_kv8(q, pages, table, ctx.row_request, ctx.positions, s.scale, self.span, out, ctx.max_kv_len,
+                                    tiles=tiles)
 
     def _options(self, gate):
         """The fields of :class:`~inferrs_b200.kernels.ScoreOptions` that this layer uses."""

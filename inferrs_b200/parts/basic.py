@@ -355,15 +355,17 @@ class Linear:
     float32 runs: exact bfloat16 pieces on the tensor cores over K of 512 and more, the FFMA kernel
     otherwise.  bfloat16 runs: tensor-core product with float32 accumulation for a bfloat16 weight; a
     weight that is stored in float32 keeps its precision and goes through the FFMA kernel with the
-    bfloat16 activations widened on the fly.
+    bfloat16 activations widened on the fly.  With ``bits`` 4 the weight is brought to 4 bits here (``mx4``; ``weight`` is
+    then None) and meets activations of either type at their full precision.
     """
 
-    def __init__(self, weight: torch.Tensor, rt: Runtime, bias: Optional[torch.Tensor] = None):
+    def __init__(self, weight: torch.Tensor, rt: Runtime, bias: Optional[torch.Tensor] = None, bits: Optional[int] = None):
         """``bias`` [out] (or shorter: it is added to the first columns) is kept in float32 and added by a kernel of
-        its own after the product; a product with a bias folds no norms."""
+        its own after the product; a product with a bias, or with 4-bit weights, folds no norms."""
         if weight.dim() != 2:
             raise ValueError(f"a linear weight must be a matrix, got shape {tuple(weight.shape)}")
-        self.weight = weight.contiguous()
+        self.weight = weight.contiguous() if bits is None else None
+        self.mx4 = kernels.quantize_mx4(weight.contiguous()) if bits == 4 else None
         self.rt = rt
         self.n_out, self.n_in = weight.shape
         if bias is not None and (bias.dim() != 1 or bias.shape[0] > self.n_out):
@@ -374,11 +376,17 @@ class Linear:
         """``x`` may be :class:`~inferrs_b200.kernels.ScaledRows`; with a ``sink`` the result is added to the residual
         stream there and the next norm's scaled rows come back instead of the result."""
         out = torch.empty((x.shape[0], self.n_out), dtype=out_dtype or self.rt.dtype, device=x.device)
-        scaled = kernels.linear(x, self.weight, out, self.rt.dtype, sink=sink)
+        if self.mx4 is not None:
+            if sink is not None or isinstance(x, kernels.ScaledRows):
+                raise ValueError("a product with 4-bit weights folds no norms; ask folds_norms first")
+            kernels.linear_mx4(x, self.mx4, out)
+            scaled = None
+        else:
+            scaled = kernels.linear(x, self.weight, out, self.rt.dtype, sink=sink)
         if self.bias is not None:
             kernels.bias_add(out, self.bias)
         return out if sink is None else scaled
 
     def folds_norms(self, n_rows: int) -> bool:
         """Whether this product takes scaled rows and feeds a sink at this number of rows."""
-        return self.bias is None and kernels.folded_norm_supported(n_rows, self.rt.dtype, self.weight)
+        return self.mx4 is None and self.bias is None and kernels.folded_norm_supported(n_rows, self.rt.dtype, self.weight)

@@ -18,9 +18,10 @@ class GatedDense:
     Gate and up weights are stacked at load: one product feeds the gate kernel, or, for a few rows, one
     kernel does both products and the gate.  With the activation ``clamped_swish`` the gate kernel is
     min(g, limit) sigmoid(slope min(g, limit)) (clamp(u, -limit, limit) + 1), with ``gelu_tanh`` it is
-    gelu_tanh(g) u."""
+    gelu_tanh(g) u.  Weights in 4 bits: the product, then the gate kernel."""
 
     graph_safe = True  # launches depend only on shapes, never on the step's host-side values
+    few_bit_weights = True
 
     @staticmethod
     def declare(spec: GatedDenseSpec) -> List[TensorDecl]:
@@ -38,8 +39,8 @@ class GatedDense:
         self.gelu = spec.activation == "gelu_tanh"
         self.spec = spec
         self.rt = rt
-        self.gate_up = Linear(fuse_rows([weights[spec.gate_proj], weights[spec.up_proj]]), rt)
-        self.down = Linear(weights[spec.down_proj], rt)
+        self.gate_up = Linear(fuse_rows([weights[spec.gate_proj], weights[spec.up_proj]]), rt, bits=rt.weight_bits)
+        self.down = Linear(weights[spec.down_proj], rt, bits=rt.weight_bits)
 
     def takes_scaled_rows(self, n_rows: int) -> bool:
         return not (self.clamped or self.gelu) and self.gate_up.folds_norms(n_rows) \
@@ -54,6 +55,8 @@ class GatedDense:
             kernels.clamped_gate(self.gate_up(h), a, 0.0, 0.0, activation=kernels.GATE_ACT_GELU_TANH)
         elif self.clamped:
             kernels.clamped_gate(self.gate_up(h), a, self.spec.limit, self.spec.slope)
+        elif self.gate_up.mx4 is not None:
+            kernels.silu_gate(self.gate_up(h), a)
         else:
             kernels.gated_linear(h, self.gate_up.weight, a, self.rt.dtype)
         return self.down(a, sink=sink)
