@@ -47,6 +47,7 @@ struct Params {
     int y_is_f32, n_tok, n_out, num_kb;      // num_kb: stages that K takes
     const unsigned char *w_scales, *x_scales;
     int scale_tiles;                         // 128-column tiles of scales per 128 rows
+    int x_groups;                            // 128-row tiles of x's scales
     const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
     long ldx;
     int k, wide;                             // wide: rows start on 16 bytes
@@ -470,10 +471,12 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
                 tma_load_2d(smem_u32(b_tiles) + s * P::B_BYTES, &map_x, i * 128, tile_t * BN, full0 + 8 * s);
             } else {
 #pragma unroll
-                for (int g = 0; g < P::B_GROUPS; ++g)
+                for (int g = 0; g < P::B_GROUPS; ++g) {
+                    const int group = tile_t * P::B_GROUPS + g;      // (the last tile may have none of its own here: any will do)
                     bulk_load(smem_u32(sb_tiles) + s * P::SB_BYTES + g * P::SA_BYTES,
-                              p.x_scales + ((long)(tile_t * P::B_GROUPS + g) * p.scale_tiles + (long)i * P::K_TILES) * 512,
+                              p.x_scales + ((long)(group < p.x_groups ? group : p.x_groups - 1) * p.scale_tiles + (long)i * P::K_TILES) * 512,
                               P::SA_BYTES, full0 + 8 * s);
+                }
             }
         };
         const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
@@ -581,6 +584,7 @@ template <int KIND>
 static int make_maps(CUtensorMap* map_w, CUtensorMap* map_x, const void* w, const void* x, int n, int m, int k, int box_w, int box_x, Params& p) {
     const long kp = (long)(k + 127) / 128 * 128;
     p.scale_tiles = few::scale_tiles(k);
+    p.x_groups = KIND == CODES ? (n + 127) / 128 : KIND == PIECES_F32 ? (n + 15) / 16 : (2 * n + 255) / 256 * 2;
     p.num_kb = (int)(KIND != CODES ? kp / 128 : (kp + 255) / 256);
     int r = KIND != CODES ? make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, w, kp, m, kp / 2, 128, box_w)
                           : make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, kp / 2, m, kp / 2, 128, box_w);
