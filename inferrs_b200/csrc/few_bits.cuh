@@ -131,7 +131,12 @@ __device__ __forceinline__ uint2 take_piece(float (&v)[8]) {
     c.x = codes8x4(v[0], v[1], v[2], v[3]);
     c.y = codes8x4(v[4], v[5], v[6], v[7]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 32.0f * (v[j] - value8((unsigned char)((j < 4 ? c.x : c.y) >> (8 * (j & 3)))));
+    for (int j = 0; j < 4; ++j) {
+        const unsigned two = values8x2((unsigned short)((j < 2 ? c.x : c.y) >> (16 * (j & 1))));
+        const float2 taken = __half22float2(*reinterpret_cast<const __half2*>(&two));
+        v[2 * j] = 32.0f * (v[2 * j] - taken.x);
+        v[2 * j + 1] = 32.0f * (v[2 * j + 1] - taken.y);
+    }
     return c;
 }
 // What a vector with the largest magnitude `a` is multiplied by before its numbers are rounded, and its scale.  A vector

@@ -44,7 +44,7 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int cod
 struct Params {
     void* y;
     long ldy;
-    int y_is_f32, n_tok, n_out, num_kb;      // num_kb: stages that K takes
+    int y_is_f32, y_wide, n_tok, n_out, num_kb;      // num_kb: stages that K takes
     const unsigned char *w_scales, *x_scales;
     int scale_tiles;                         // 128-column tiles of scales per 128 rows
     int x_groups;                            // 128-row tiles of x's scales
@@ -114,7 +114,7 @@ template <int KIND, int BN> struct Plan {
     static constexpr int B_GROUPS = (BN + 127) / 128;                    // 128-row tiles of scales
     static constexpr int SA_BYTES = 512 * K_TILES, SB_BYTES = 512 * K_TILES * B_GROUPS;
     static constexpr int SCALE_COLS = 4 * K_TILES * (1 + B_GROUPS);      // of tensor memory a stage
-    static_assert(KIND != PIECES_F32 || BN == 80, "read back sixteen tokens at a time");
+    static_assert(KIND != PIECES_F32 || BN % 80 == 0, "read back sixteen tokens at a time");
     static constexpr int tmem_cols(int stages) {
         int c = 32;
         while (c < BN + stages * SCALE_COLS) c *= 2;
@@ -129,10 +129,10 @@ __device__ __forceinline__ void store(const Params& p, int t, int f, float v) {
 
 // One stage's products, issued by one thread: scales into the stage's columns of tensor memory (`scales`), then four products
 // of 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones.  a, b, sa, sb: where the stage's tiles start, in units of
-// 16 bytes.
+// 16 bytes; shift: columns of scales in front of x's.
 template <int KIND, int BN>
 __device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, unsigned a, unsigned b, unsigned sa_tile, unsigned sb_tile,
-                                               bool accumulate) {
+                                               bool accumulate, unsigned shift = 0) {
     using P = Plan<KIND, BN>;
     constexpr unsigned FORMATS = KIND != CODES ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);   // e2m1 and e4m3, e2m1 twice
     constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(BM >> 4) << 24);
@@ -148,7 +148,7 @@ __device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, u
     for (int k = 0; k < 4; ++k) {
         const unsigned tile = KIND != CODES ? 0 : k >> 1, id = KIND != CODES ? k : (k & 1) * 2;
         umma_scaled<KIND>(tmem, from_words(TILE_LO + a + 2 * k, TILE_HI), from_words(TILE_LO + b + 2 * k, TILE_HI),
-                          IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile, accumulate || k != 0);
+                          IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile + shift, accumulate || k != 0);
     }
 }
 
@@ -420,7 +420,71 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.tmem_cols));
 }
 
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMNS]) {
+#pragma unroll
+    for (int c = 0; c < COLUMNS / 16; ++c)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(r[16 * c]), "=r"(r[16 * c + 1]), "=r"(r[16 * c + 2]), "=r"(r[16 * c + 3]), "=r"(r[16 * c + 4]), "=r"(r[16 * c + 5]),
+                       "=r"(r[16 * c + 6]), "=r"(r[16 * c + 7]), "=r"(r[16 * c + 8]), "=r"(r[16 * c + 9]), "=r"(r[16 * c + 10]), "=r"(r[16 * c + 11]),
+                       "=r"(r[16 * c + 12]), "=r"(r[16 * c + 13]), "=r"(r[16 * c + 14]), "=r"(r[16 * c + 15])
+                     : "r"(from + 16 * c));
+    tmem_ld_wait();
+}
+
 // ---- more rows ------------------------------------------------------------------------------------------------------------------
+// A pair of CTAs (a cluster) covers 256 rows of W and one tile of tokens: each loads its own 128 rows of W and half of the tokens,
+// which it sends to both.  The pairs stay and take tile after tile; two accumulators take turns, so that four warps read one back
+// and store it while the other is being filled.
+constexpr int PAIR = 2, STORE_BYTES = 4096;      // a warp's piece of shared memory for results on their way out
+template <int KIND, int BN, int STAGES> struct Many {
+    using P = Plan<KIND, BN>;
+    static constexpr int SMEM = STAGES * (A_BYTES + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) + 4 * STORE_BYTES + 16 * STAGES + 64 + 1024;
+    static_assert(2 * BN + STAGES * P::SCALE_COLS <= 512 && SMEM <= 227 * 1024 && SMEM > 114 * 1024, "memories of an SM");
+    static_assert(P::B_GROUPS == PAIR, "a CTA of the pair fetches one tile of x's scales");
+    static_assert(BN % 32 == 0 && BN / PAIR % 8 == 0, "halves of a tile are whole groups of eight rows");
+};
+// The same piece of tokens, or of their scales, to both CTAs of the pair, each at the same place and counted on its own barrier.
+__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.multicast::cluster [%0], [%1, {%3, %4}], [%2], %5;"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ void bulk_load_pair(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.multicast::cluster [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "h"((unsigned short)3) : "memory");
+}
+// one arrival at the barrier of either CTA when the products so far are done
+__device__ __forceinline__ void umma_commit_pair(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+
+// A warp stores `count` tokens' results of its 32 rows of W, a lane a row: through shared memory, so that a token's results go out in
+// pieces of 16 bytes where y allows it.
+template <typename T, int COUNT>
+__device__ __forceinline__ void store_rows(const Params& p, unsigned char* mine, const float (&v)[COUNT], int t0, int count, int f0, int lane, bool wide) {
+    T* rows = reinterpret_cast<T*>(mine);
+    static_assert(COUNT * 32 * sizeof(T) <= STORE_BYTES, "a warp's piece");
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        if constexpr (sizeof(T) == 4) rows[32 * j + lane] = v[j];
+        else rows[32 * j + lane] = __float2bfloat16_rn(v[j]);
+    }
+    __syncwarp();
+    constexpr int LANES = 2 * sizeof(T), PER = 32 / LANES;      // lanes that a token's results take, tokens at a time
+    T* y = reinterpret_cast<T*>(p.y) + (long)t0 * p.ldy + f0;
+    if (wide) {
+        const int r = lane / LANES, c = lane % LANES;
+#pragma unroll
+        for (int j = 0; j < COUNT; j += PER)
+            if (j + r < count)
+                *reinterpret_cast<uint4*>(y + (long)(j + r) * p.ldy + c * (16 / (int)sizeof(T))) = *reinterpret_cast<const uint4*>(rows + 32 * (j + r) + c * (16 / (int)sizeof(T)));
+    } else if (f0 + lane < p.n_out) {
+        for (int j = 0; j < count; ++j) y[(long)j * p.ldy + lane] = rows[32 * j + lane];
+    }
+    __syncwarp();
+}
+
 template <int KIND, int BN, int STAGES>
 __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
                                                        const __grid_constant__ CUtensorMap map_x, const Params p) {
@@ -431,98 +495,149 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     unsigned char* b_tiles = a_tiles + STAGES * A_BYTES;
     unsigned char* sa_tiles = b_tiles + STAGES * P::B_BYTES;
     unsigned char* sb_tiles = sa_tiles + STAGES * P::SA_BYTES;
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sb_tiles + STAGES * P::SB_BYTES);
-    const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * STAGES + 1);
+    unsigned char* stores = sb_tiles + STAGES * P::SB_BYTES;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(stores + 4 * STORE_BYTES);
+    // full: this CTA's stage has landed; empty: both CTAs are done with theirs; filled, drained: an accumulator
+    const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), filled0 = smem_u32(bars + 2 * STAGES), drained0 = filled0 + 16;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * STAGES + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile_f = blockIdx.x, tile_t = blockIdx.y, nkb = p.num_kb;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nkb = p.num_kb;
+    const int rank = blockIdx.x & 1, pairs_f = (p.n_out + PAIR * BM - 1) / (PAIR * BM), tiles = pairs_f * ((p.n_tok + P::TOKENS - 1) / P::TOKENS);
+    const int first = blockIdx.x / PAIR, step = gridDim.x / PAIR, stages = (tiles - first + step - 1) / step * nkb;      // of this pair
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
-        mbar_init(accum, 1);
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, PAIR); }
+        for (int b = 0; b < 2; ++b) { mbar_init(filled0 + 8 * b, 1); mbar_init(drained0 + 8 * b, 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::tmem_cols(STAGES)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
+    cluster_arrive();      // nothing is sent to the other CTA before its barriers stand
+    cluster_wait();
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
     if (p.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
     // Copies are issued by two threads, one for the operands and one for their scales: a thread takes 165 cycles a tile and 50 a
-    // plain copy, five of which together would take longer than the products of a stage.
+    // plain copy, which together would take longer than the products of a stage.
     if (warp == 0 || warp == 6) {
-        const bool leader = elected(), tiles = warp == 0;
+        const bool leader = elected(), operands = warp == 0;
         constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
+        const int last_f = (p.n_out + BM - 1) / BM - 1;
+        int tile = first, row_w = 0, row_x = 0;
+        const unsigned char *at_w = nullptr, *at_x = nullptr;
+        auto enter = [&]() {      // (a tile may lie behind the last row of W, and its scales behind x's: any will do, nothing of it is stored)
+            const int tile_f = tile % pairs_f * PAIR + rank, tile_t = tile / pairs_f;
+            row_w = tile_f * BM;
+            row_x = tile_t * BN + rank * (BN / PAIR);
+            const int group = (KIND == CODES ? tile_t * BN / 128 : tile_t * P::B_GROUPS) + rank;
+            at_w = p.w_scales + (long)(tile_f < last_f ? tile_f : last_f) * p.scale_tiles * 512;
+            at_x = p.x_scales + (long)(group < p.x_groups ? group : p.x_groups - 1) * p.scale_tiles * 512;
+        };
         auto load_w = [&](int i, int s) {
             if (!leader) return;
-            mbar_expect_tx(full0 + 8 * s, tiles ? W_TX + P::B_BYTES : P::SA_BYTES + P::SB_BYTES);
-            if (tiles) tma_load_2d(smem_u32(a_tiles) + s * A_BYTES, &map_w, i * 128, tile_f * BM, full0 + 8 * s);
-            else bulk_load(smem_u32(sa_tiles) + s * P::SA_BYTES, p.w_scales + ((long)tile_f * p.scale_tiles + (long)i * P::K_TILES) * 512,
-                           P::SA_BYTES, full0 + 8 * s);
+            if (operands) {
+                mbar_expect_tx(full0 + 8 * s, W_TX + P::B_BYTES);
+                tma_load_2d(smem_u32(a_tiles) + s * A_BYTES, &map_w, i * 128, row_w, full0 + 8 * s);
+            } else {
+                mbar_expect_tx(full0 + 8 * s, P::SA_BYTES + P::SB_BYTES);
+                bulk_load(smem_u32(sa_tiles) + s * P::SA_BYTES, at_w + i * P::SA_BYTES, P::SA_BYTES, full0 + 8 * s);
+            }
         };
         auto load_x = [&](int i, int s) {
             if (!leader) return;
-            if (tiles) {
-                tma_load_2d(smem_u32(b_tiles) + s * P::B_BYTES, &map_x, i * 128, tile_t * BN, full0 + 8 * s);
-            } else {
-#pragma unroll
-                for (int g = 0; g < P::B_GROUPS; ++g) {
-                    const int group = tile_t * P::B_GROUPS + g;      // (the last tile may have none of its own here: any will do)
-                    bulk_load(smem_u32(sb_tiles) + s * P::SB_BYTES + g * P::SA_BYTES,
-                              p.x_scales + ((long)(group < p.x_groups ? group : p.x_groups - 1) * p.scale_tiles + (long)i * P::K_TILES) * 512,
-                              P::SA_BYTES, full0 + 8 * s);
-                }
-            }
+            if (operands) tma_load_2d_pair(smem_u32(b_tiles) + s * P::B_BYTES + rank * (P::B_BYTES / PAIR), &map_x, i * 128, row_x, full0 + 8 * s);
+            else bulk_load_pair(smem_u32(sb_tiles) + s * P::SB_BYTES + rank * P::SA_BYTES, at_x + i * P::SA_BYTES, P::SA_BYTES, full0 + 8 * s);
         };
         const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
+        enter();
         for (int i = 0; i < head; ++i) load_w(i, i);
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        for (int i = 0; i < head; ++i) load_x(i, i);
-        for (int i = head; i < nkb; ++i) {
-            const int s = i % STAGES;
-            if (!mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, 1)) { ok = false; break; }
-            load_w(i, s);
-            load_x(i, s);
+        int i = 0;
+        unsigned phase = 1;
+        for (int it = 0; it < stages && ok; it += STAGES, phase ^= 1) {
+#pragma unroll
+            for (int s = 0; s < STAGES; ++s) {
+                if (it + s >= stages) break;
+                if (it + s >= head) {
+                    if (!mbar_wait(empty0 + 8 * s, phase, 1)) { ok = false; break; }
+                    load_w(i, s);
+                }
+                load_x(i, s);
+                if (++i == nkb) { i = 0; tile += step; enter(); }
+            }
+        }
+        // the other CTA's last arrivals have come: none is on its way to a CTA that has ended
+        for (int s = 0; ok && s < STAGES; ++s) {
+            const int uses = (stages - s + STAGES - 1) / STAGES;
+            ok = uses == 0 || mbar_wait(empty0 + 8 * s, (uses - 1) & 1, 1);
         }
     } else if (warp == 1) {
         const bool leader = elected();
         const unsigned a0 = smem_u32(a_tiles) >> 4, b0 = smem_u32(b_tiles) >> 4, sa0 = smem_u32(sa_tiles) >> 4, sb0 = smem_u32(sb_tiles) >> 4;
-        for (int i = 0; i < nkb; ++i) {
-            const int s = i % STAGES;
-            if (!mbar_wait(full0 + 8 * s, (i / STAGES) & 1, 2)) { ok = false; break; }
-            fence_after();
-            if (leader) {
-                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a0 + s * (A_BYTES / 16), b0 + s * (P::B_BYTES / 16),
-                                         sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0);
-                umma_commit(empty0 + 8 * s);
+        // a tile of 4-bit rows may start amid a tile of 128 rows of scales, 32 of them a column
+        auto shift_of = [&](int tile) { return KIND == CODES ? (unsigned)(tile / pairs_f * BN / 32 & 3) : 0u; };
+        int i = 0, tile = first;
+        unsigned phase = 0, turn = 0, shift = shift_of(tile);
+        bool landed = mbar_try_wait(full0, 0);      // the next stage's answer is on its way while a stage is issued
+        for (int it = 0; it < stages && ok; it += STAGES, phase ^= 1) {
+#pragma unroll
+            for (int s = 0; s < STAGES; ++s) {
+                if (it + s >= stages) break;
+                const unsigned buffer = turn & 1;
+                if (i == 0 && !mbar_wait(drained0 + 8 * buffer, (turn >> 1 & 1) ^ 1, 4)) { ok = false; break; }
+                if (!landed && !mbar_wait(full0 + 8 * s, phase, 2)) { ok = false; break; }
+                landed = mbar_test_wait(full0 + 8 * ((s + 1) % STAGES), s + 1 == STAGES ? phase ^ 1 : phase);
+                fence_after();
+                if (leader) {
+                    multiply_stage<KIND, BN>(tmem + buffer * BN, tmem + 2 * BN + s * P::SCALE_COLS, a0 + s * (A_BYTES / 16), b0 + s * (P::B_BYTES / 16),
+                                             sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0, shift);
+                    umma_commit_pair(empty0 + 8 * s);
+                    if (i == nkb - 1) umma_commit(filled0 + 8 * buffer);
+                }
+                if (++i == nkb) { i = 0; tile += step; ++turn; shift = shift_of(tile); }
             }
         }
-        if (leader) umma_commit(accum);
     } else {
-        const int q = warp & 3, feature = tile_f * BM + q * 32 + lane;
-        const int t0 = tile_t * P::TOKENS, tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
+        const int q = warp & 3;
+        unsigned char* mine = stores + q * STORE_BYTES;
         asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the kernel ahead
-        ok = mbar_wait(accum, 0, 3);
-        ok = __all_sync(0xffffffffu, ok);
-        fence_after();
-        if (ok && g_error == 0) {
-            constexpr int STEP = 16 / KIND;     // tokens of sixteen columns
+        int turn = 0;
+        for (int tile = first; tile < tiles; tile += step, ++turn) {
+            const unsigned buffer = turn & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(filled0 + 8 * buffer, turn >> 1 & 1, 3)) && *(volatile int*)&g_error == 0;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const int f0 = (tile % pairs_f * PAIR + rank) * BM + q * 32, t0 = tile / pairs_f * P::TOKENS;
+            const int tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
+            const bool wide = p.y_wide && f0 + 32 <= p.n_out;
+            constexpr int STEP = KIND == PIECES_F32 ? 16 : 32 / KIND, COLUMNS = STEP * KIND;      // tokens and columns at a time
 #pragma unroll 1
             for (int c = 0; c * STEP < tokens; ++c) {
-                float v[16];
-                tmem_ld16(tmem + ((unsigned)(q * 32) << 16) + 16 * c, v);
+                unsigned r[COLUMNS];
+                const unsigned from = tmem + buffer * BN + ((unsigned)(q * 32) << 16) + COLUMNS * c;
+                tmem_columns<COLUMNS>(from, r);
+                float v[STEP];
 #pragma unroll
                 for (int j = 0; j < STEP; ++j) {
-                    float r = 0.0f;
+                    v[j] = 0.0f;
 #pragma unroll
-                    for (int i = KIND - 1; i >= 0; --i) r += v[KIND * j + i];
-                    if (c * STEP + j < tokens && feature < p.n_out) store(p, t0 + c * STEP + j, feature, r);
+                    for (int i = KIND - 1; i >= 0; --i) v[j] += __uint_as_float(r[KIND * j + i]);
                 }
+                if ((c + 1) * STEP >= tokens) {      // all is in registers
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(drained0 + 8 * buffer);
+                }
+                const int count = tokens - c * STEP < STEP ? tokens - c * STEP : STEP;
+                if (f0 >= p.n_out) continue;
+                if (p.y_is_f32) store_rows<float, STEP>(p, mine, v, t0 + c * STEP, count, f0, lane, wide);
+                else store_rows<__nv_bfloat16, STEP>(p, mine, v, t0 + c * STEP, count, f0, lane, wide);
             }
         }
     }
@@ -530,40 +645,58 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     if (!ok) for (const unsigned long long t = global_ns(); global_ns() - t < 20000000ull;) {}
     fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::tmem_cols(STAGES)));
+    cluster_arrive();      // the other CTA may still be told that this one is done with a stage, or send to it
+    cluster_wait();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // Where the scales of a row's first piece stand: the tiles of 80 columns that five pieces a number take have tiles of 128
 // rows of scales of their own; tiles of two pieces a number start where tiles of scales do.
-template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(int row) {
-    return PARTS == PIECES_F32 ? row / 16 * 128 + row % 16 * PARTS : row * PARTS;
+template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(int row, int tokens) {
+    return row / tokens * ((tokens * PARTS + 127) / 128 * 128) + row % tokens * PARTS;
 }
 // Rows as pieces: row PARTS * t + i of `pieces` [PARTS * n, kp] holds piece i of row t, kp = width rounded up to 128.  A
-// thread takes eight numbers, four threads a block of 32, sixteen a word of four scales.
+// warp takes 256 columns of two rows: a lane eight numbers of each, four lanes a block of 32, sixteen a word of four scales.  Memory
+// bounds it where the conversions leave it time: 2,048 x 12,288 bfloat16 numbers, 101 MB, PIECES_US.
+constexpr int PIECES_ROWS = 2;
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
+__global__ void __launch_bounds__(256) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide, int tokens,
                                                      uint2* __restrict__ pieces, unsigned* __restrict__ scales) {
     ib_grid_dependency_sync();
-    const int tiles = few::scale_tiles(width), per_row = (width + 127) / 128 * 16;
-    const long total = (long)rows * per_row;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (total + 31) / 32 * 32; i += (long)gridDim.x * 256) {
-        const bool in = i < total;
-        const int row = in ? (int)(i / per_row) : 0, g = (int)(i - (long)row * per_row);
-        float v[8];
-        few::load8<T>(x + (long)row * ldx + 8 * g, in ? width - 8 * g : 0, wide != 0, v);
-        const unsigned m = few::block_largest(v);
-        const unsigned byte = few::pieces_byte<PARTS>(m);
+    const int columns = (width + 255) / 256, per_row = (width + 127) / 128 * 16, lane = threadIdx.x & 31;
+    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row0 = (int)(w / columns) * PIECES_ROWS, g = (int)(w % columns) * 32 + lane;
+    float v[PIECES_ROWS][8];
+#pragma unroll
+    for (int r = 0; r < PIECES_ROWS; ++r)
+        few::load8<T>(x + (long)(row0 + r) * ldx + 8 * g, row0 + r < rows ? width - 8 * g : 0, wide != 0, v[r]);
+#pragma unroll
+    for (int r = 0; r < PIECES_ROWS; ++r) {
+        const unsigned byte = few::pieces_byte<PARTS>(few::block_largest(v[r]));
         const float by = byte == 255u ? 0.0f : few::scale_reciprocal(byte);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.0f : v[j] * by;
+        for (int j = 0; j < 8; ++j) v[r][j] = byte == 255u ? 0.0f : v[r][j] * by;
+        uint2 c[PARTS];
+        if constexpr (PARTS == PIECES_BF16) {
+            unsigned short h[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) two_pieces(f16_pair(v[r][2 * j], v[r][2 * j + 1]), h[j], l[j]);
+            c[0] = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+            c[1] = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
+        } else {
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) c[part] = few::take_piece(v[r]);
+        }
+        unsigned word = byte << (8 * (lane >> 2 & 3));
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        if (row0 + r >= rows || g >= per_row) continue;
+        const int at = pieces_scale_row<PARTS>(row0 + r, tokens);
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-            const uint2 c = few::take_piece(v);
-            unsigned word = (byte == 255u ? 255u : byte - 5u * part) << (8 * (threadIdx.x >> 2 & 3));
-            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-            word |= __shfl_xor_sync(0xffffffffu, word, 8);
-            if (in) pieces[((long)row * PARTS + part) * per_row + g] = c;
-            if (in && (threadIdx.x & 15) == 0) scales[few::scale_word(pieces_scale_row<PARTS>(row) + part, g >> 4, tiles)] = word;
+            pieces[((long)(row0 + r) * PARTS + part) * per_row + g] = c[part];
+            // every further piece's byte is five less; 255 stays (no byte is below five times the pieces in front of its own)
+            if ((lane & 15) == 0) scales[few::scale_word(at + part, g >> 4, 2 * columns)] = __vsub4(word, __vcmpne4(word, 0xFFFFFFFFu) & (0x01010101u * (5 * part)));
         }
     }
 }
@@ -584,7 +717,6 @@ template <int KIND>
 static int make_maps(CUtensorMap* map_w, CUtensorMap* map_x, const void* w, const void* x, int n, int m, int k, int box_w, int box_x, Params& p) {
     const long kp = (long)(k + 127) / 128 * 128;
     p.scale_tiles = few::scale_tiles(k);
-    p.x_groups = KIND == CODES ? (n + 127) / 128 : KIND == PIECES_F32 ? (n + 15) / 16 : (2 * n + 255) / 256 * 2;
     p.num_kb = (int)(KIND != CODES ? kp / 128 : (kp + 255) / 256);
     int r = KIND != CODES ? make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, w, kp, m, kp / 2, 128, box_w)
                           : make_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, kp / 2, m, kp / 2, 128, box_w);
@@ -675,36 +807,47 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
 template <int KIND, int BN, int STAGES>
 static int launch(const void* w, const void* x, int n, int m, int k, Params p, cudaStream_t stream, bool early) {
     using P = Plan<KIND, BN>;
-    static_assert(BN + STAGES * P::SCALE_COLS <= 512, "tensor memory");
-    constexpr size_t SMEM = (size_t)STAGES * (A_BYTES + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) + 16 * STAGES + 64 + 1024;
+    constexpr int SMEM = Many<KIND, BN, STAGES>::SMEM;
     static IbDeviceSet done;
     if (int r = ib_allow_dynamic_smem(done, gemm_kernel<KIND, BN, STAGES>, SMEM)) return r;
-    const int tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
-    if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
+    const long tiles = (long)((n + P::TOKENS - 1) / P::TOKENS) * ((m + PAIR * BM - 1) / (PAIR * BM));
+    if (tiles > (1 << 30)) return IB_ERR_UNSUPPORTED;
     CUtensorMap map_w, map_x;
-    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, BM, BN, p)) return r;
+    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, BM, BN / PAIR, p)) return r;
+    p.x_groups = KIND == CODES ? (n + 127) / 128 : (n + P::TOKENS - 1) / P::TOKENS * P::B_GROUPS;
+    p.y_wide = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy * (p.y_is_f32 ? 4 : 2) % 16 == 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((m + BM - 1) / BM, tiles_t);
+    cfg.gridDim = dim3((unsigned)(PAIR * (tiles < SMS / PAIR ? tiles : SMS / PAIR)));
     cfg.blockDim = dim3(THREADS + 32);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     p.wait_first = !ib_pdl_enabled && !early;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, p);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
 
+// tokens of a tile of the product that rows as pieces go through
+static int tile_tokens(int x_kind, int n) {
+    if (x_kind == 1) return n <= 64 ? 16 : 32;
+    return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 96;
+}
 static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((k + 127) / 128 * 128) + 511) / 512 * 512; }
 
 template <typename T, int PARTS>
-static int make_pieces(const void* x, long ldx, int n, int k, int wide, unsigned char* pieces, cudaStream_t stream) {
-    const long threads = (long)n * ((k + 127) / 128 * 16), blocks = (threads + 255) / 256;
-    ib_launch_early(pieces_kernel<T, PARTS>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide,
-              (uint2*)pieces, (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
+static int make_pieces(const void* x, long ldx, int n, int k, int wide, int tokens, unsigned char* pieces, cudaStream_t stream) {
+    const long blocks = ((long)(n + PIECES_ROWS - 1) / PIECES_ROWS * ((k + 255) / 256) + 7) / 8;
+    if (blocks > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
+    ib_launch_early(pieces_kernel<T, PARTS>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide, tokens, (uint2*)pieces,
+                    (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }
 
@@ -727,7 +870,8 @@ IB_EXPORT int ib_gemm_mx4_error_async(int* out, cudaStream_t stream) {
 // the bytes of workspace that ib_gemm_mx4 wants: pieces, then their scales (from a multiple of 512 on)
 IB_EXPORT long ib_gemm_mx4_workspace(int x_kind, int n, int k) {
     if (x_kind == 2 || (x_kind == 0 && n <= mx4::INSIDE_ROWS)) return 0;
-    const long scale_rows = x_kind == 1 ? (n + 15) / 16 * 128L : (2L * n + 255) / 256 * 256;      // whole tiles of tokens
+    const long tokens = mx4::tile_tokens(x_kind, n), parts = x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16;
+    const long scale_rows = (n + tokens - 1) / tokens * ((tokens * parts + 127) / 128 * 128);      // whole tiles of tokens
     return mx4::pieces_bytes(x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16, n, k) + scale_rows / 128 * few::scale_tiles(k) * 512;
 }
 
@@ -768,19 +912,20 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
         if (n <= 16) return launch_few<CODES, 16, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
         if (n <= 32) return launch_few<CODES, 32, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
         if (n <= 64) return launch_few<CODES, 64, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
-        if (n <= 128) return launch<CODES, 128, 4>(w, x, n, m, k, p, stream, false);
-        return launch<CODES, 256, 4>(w, x, n, m, k, p, stream, false);
+        return launch<CODES, 192, 4>(w, x, n, m, k, p, stream, false);
     }
     unsigned char* pieces = (unsigned char*)workspace;
+    const int tokens = tile_tokens(x_kind, n);
     if (x_kind == 1) {
         p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
-        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, p.wide, pieces, stream)) return r;
-        return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, p.wide, tokens, pieces, stream)) return r;
+        if (tokens == 16) return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+        return launch<PIECES_F32, 160, 5>(w, pieces, n, m, k, p, stream, true);
     }
     p.x_scales = pieces + pieces_bytes(PIECES_BF16, n, k);
-    if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, p.wide, pieces, stream)) return r;
-    if (n <= 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    if (n <= 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    if (n <= 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    return launch<PIECES_BF16, 256, 4>(w, pieces, n, m, k, p, stream, true);
+    if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, p.wide, tokens, pieces, stream)) return r;
+    if (tokens == 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    if (tokens == 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    if (tokens == 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
+    return launch<PIECES_BF16, 192, 5>(w, pieces, n, m, k, p, stream, true);
 }
