@@ -7,53 +7,52 @@ IB_EXPORT void ib_few_bits_set_pdl(int on) { ib_pdl_enabled = on; }
 
 namespace few {
 
-// A warp takes 256 columns of four rows: a lane eight numbers of each, four lanes a block of 32, sixteen a word of four scales.
-// Memory bounds both kernels: every load of the four rows is on its way before the first is used, and no index is divided by
-// anything but once a warp.  A matrix of 24,576 x 4,096 (bfloat16) there and back: 171 us a thread and eight numbers at a time, 123 us now.
-constexpr int QUANT_ROWS = 4;
+// A warp takes 256 columns of four rows: a lane eight numbers of each, four lanes a block of 32.  Memory bounds both kernels: every load of
+// the four rows is on its way before the first is used, and no index is divided by anything but once a block.  A matrix of 24,576 x 4,096
+// (bfloat16) there and back: 171 us a thread and eight numbers at a time, QUANT_US now.
+constexpr int QUANT_ROWS = 4, QUANT_WARPS = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
-                                                       unsigned* __restrict__ codes, unsigned* __restrict__ scales) {
+__global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
+                                                                    unsigned* __restrict__ codes, unsigned char* __restrict__ scales) {
     ib_grid_dependency_sync();
-    const int columns = (width + 255) / 256, lane = threadIdx.x & 31;
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row0 = (int)(w / columns) * QUANT_ROWS, g = (int)(w % columns) * 32 + lane;
+    const Strip at(width, QUANT_ROWS);
+    const int lane = threadIdx.x & 31, tiles = scale_tiles(width);
     const long pitch = code_pitch(width) / 4;
-    float v[QUANT_ROWS][8];
-#pragma unroll
-    for (int r = 0; r < QUANT_ROWS; ++r)
-        load8<T>(x + (long)(row0 + r) * ldx + 8 * g, row0 + r < rows ? width - 8 * g : 0, wide != 0, v[r]);
+    const bool all = wide && at.column + 8 <= width;
+    Eight<T> v[QUANT_ROWS];
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
-        const unsigned byte = scale_byte(block_largest(v[r]));
-        const float by = byte == 255u ? 0.0f : scale_reciprocal(byte);
+        const bool in = at.row0 + r < rows;
+        v[r].load(x + (long)(in ? at.row0 + r : 0) * ldx + at.column, in ? width - at.column : 0, all && in);
+    }
+#pragma unroll
+    for (int r = 0; r < QUANT_ROWS; ++r) {
+        const int row = at.row0 + r;
+        const unsigned byte = scale_byte(block_largest(v[r].largest()));
+        const float by = __uint_as_float((254u - min(byte, 253u)) << 23);
         unsigned c = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) c |= codes2(v[r][2 * j] * by, v[r][2 * j + 1] * by) << (8 * j);
-        unsigned word = byte << (8 * (lane >> 2 & 3));
-        word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        if (row0 + r >= rows) break;
-        if (g < pitch) codes[(long)(row0 + r) * pitch + g] = byte == 255u ? 0u : c;
-        if ((lane & 15) == 0) scales[scale_word(row0 + r, g >> 4, 2 * columns)] = word;
+        if (row >= rows) break;
+        if (at.g < pitch) codes[(long)row * pitch + at.g] = byte == 255u ? 0u : c;
+        if ((lane & 3) == 0) scales[4 * scale_word(row, at.g >> 4, tiles) + (lane >> 2 & 3)] = (unsigned char)byte;
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales,
+__global__ void __launch_bounds__(32 * QUANT_WARPS) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales,
                                                          int rows, int width, int wide, T* __restrict__ out, long ldo) {
     ib_grid_dependency_sync();
-    const int columns = (width + 255) / 256, lane = threadIdx.x & 31;
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row0 = (int)(w / columns) * QUANT_ROWS, g = (int)(w % columns) * 32 + lane;
+    const Strip at(width, QUANT_ROWS);
+    const int row0 = at.row0, g = at.g, lane = threadIdx.x & 31, tiles = scale_tiles(width);
     const long pitch = code_pitch(width) / 4;
     unsigned c[QUANT_ROWS], word[QUANT_ROWS];
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
         const bool in = row0 + r < rows && g < pitch;
         c[r] = in ? codes[(long)(row0 + r) * pitch + g] : 0u;
-        word[r] = in ? scales[scale_word(row0 + r, g >> 4, 2 * columns)] : 0u;
+        word[r] = in ? scales[scale_word(row0 + r, g >> 4, tiles)] : 0u;
     }
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
@@ -88,12 +87,6 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restr
     }
 }
 
-// blocks of eight warps, or 0 where they are more than a grid takes
-static inline unsigned blocks_for(long rows, int width) {
-    const long b = ((rows + QUANT_ROWS - 1) / QUANT_ROWS * ((width + 255) / 256) + 7) / 8;
-    return b <= 0x7FFFFFFF ? (unsigned)b : 0u;
-}
-
 }  // namespace few
 
 // x [rows, width] (float32 or bfloat16, rows ldx elements apart) to codes and scales
@@ -115,10 +108,10 @@ IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     if (rows == 0) return IB_OK;
     const size_t e = x_is_f32 ? 4 : 2;
     const int wide = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * e) % 16 == 0) ? 1 : 0;
-    const dim3 grid(blocks_for(rows, width));
+    const dim3 grid(strips(rows, width, QUANT_ROWS, QUANT_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(256), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
-    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned*)scales);
+    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
+    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
     return ib_launch_status();
 }
 
@@ -140,9 +133,9 @@ IB_EXPORT int ib_dequantize_mx4(const IbDequantizeMx4* q) {
     if (rows == 0) return IB_OK;
     const size_t e = out_is_f32 ? 4 : 2;
     const int wide = (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * e) % 16 == 0) ? 1 : 0;
-    const dim3 grid(blocks_for(rows, width));
+    const dim3 grid(strips(rows, width, QUANT_ROWS, QUANT_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (out_is_f32) ib_launch_early(dequantize_kernel<float>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (float*)out, ldo);
-    else ib_launch_early(dequantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (__nv_bfloat16*)out, ldo);
+    if (out_is_f32) ib_launch_early(dequantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (float*)out, ldo);
+    else ib_launch_early(dequantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (__nv_bfloat16*)out, ldo);
     return ib_launch_status();
 }

@@ -44,10 +44,8 @@ __device__ __forceinline__ long scale_word(int row, int t, int tiles) {
 // nearest code, 6, is off by at most a seventh; beyond, the next power of two is nearer).  0 for a block of zeros or of
 // numbers too small for any exponent, 255 where there is an infinity or no number.
 __device__ __forceinline__ unsigned scale_byte(unsigned largest_bits) {
-    const unsigned e = largest_bits >> 23;
-    if (e == 255u) return 255u;
-    const int b = (int)e - 2 + ((largest_bits & 0x7FFFFFu) > 0x600000u);
-    return b < 0 ? 0u : (unsigned)b;
+    const int b = (int)((largest_bits + 0x1FFFFFu) >> 23) - 2;      // (a fraction beyond three quarters carries)
+    return largest_bits >= 0x7F800000u ? 255u : (unsigned)max(b, 0);
 }
 // 2^(byte - 127), and its reciprocal (both exact; bytes of scale_byte: 0 .. 253)
 __device__ __forceinline__ float scale_value(unsigned byte) {
@@ -69,36 +67,69 @@ __device__ __forceinline__ __half2 values4x2(unsigned byte) {
     return *reinterpret_cast<const __half2*>(&r);
 }
 
-// eight neighbours of a row (zeros behind the first n), 16 bytes at a time where the rows allow it
-template <typename T> __device__ __forceinline__ void load8(const T* p, int n, bool wide, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, int n, bool wide, float (&v)[8]) {
-    if (wide && n >= 8) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+// Eight neighbours of a row as they are stored.  load: those from p on, zeros behind the first n; `all` says that there are eight
+// and that they start on 16 bytes.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p, int n, bool all) {
+        if (all) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+        }
     }
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, int n, bool wide, float (&v)[8]) {
-    if (wide && n >= 8) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const unsigned w[4] = {a.x, a.y, a.z, a.w};
+    // the bits of the largest magnitude
+    __device__ __forceinline__ unsigned largest() const {
+        unsigned m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        return m;
     }
-}
-// the bits of the largest magnitude of a block of 32 of which four neighbouring lanes hold eight numbers each; no number
-// counts as larger than an infinity
-__device__ __forceinline__ unsigned block_largest(const float (&v)[8]) {
-    unsigned m = 0;
+    __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+};
+template <> struct Eight<__nv_bfloat16> {
+    unsigned w[4];      // two numbers each
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int n, bool all) {
+        if (all) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        } else {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            for (int i = 0; i < 4; ++i) w[i] = (2 * i < n ? (unsigned)q[2 * i] : 0u) | (2 * i + 1 < n ? (unsigned)q[2 * i + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ unsigned largest() const {
+        unsigned m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return max(m & 0xFFFF0000u, m << 16);
+    }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
+};
+
+// the largest magnitude's bits among four lanes' eight numbers (a block of 32)
+__device__ __forceinline__ unsigned block_largest(unsigned mine) {
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+    return max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+}
+// The work of a warp whose block takes a strip of 256 columns and `per_warp` rows for each of its warps.
+struct Strip {
+    int row0, column, g;      // the warp's first row, the lane's first column, its place among a row's groups of eight
+    __device__ __forceinline__ Strip(int width, int per_warp) {
+        const unsigned columns = (unsigned)(width + 255) / 256, rows = blockIdx.x / columns;
+        row0 = (int)(rows * (blockDim.x >> 5) + (threadIdx.x >> 5)) * per_warp;
+        g = (int)(blockIdx.x - rows * columns) * 32 + (threadIdx.x & 31);
+        column = 8 * g;
+    }
+};
+// blocks of `warps` warps, or 0 where they are more than a grid takes
+static inline unsigned strips(long rows, int width, int per_warp, int warps) {
+    const long b = (rows + per_warp * warps - 1) / (per_warp * warps) * ((width + 255) / 256);
+    return b <= 0x7FFFFFFF ? (unsigned)b : 0u;
 }
 
 // ---- 8-bit keys and values ----------------------------------------------------------------------------------------------

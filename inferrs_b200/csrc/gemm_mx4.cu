@@ -658,45 +658,48 @@ template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(in
 // Rows as pieces: row PARTS * t + i of `pieces` [PARTS * n, kp] holds piece i of row t, kp = width rounded up to 128.  A
 // warp takes 256 columns of two rows: a lane eight numbers of each, four lanes a block of 32, sixteen a word of four scales.  Memory
 // bounds it where the conversions leave it time: 2,048 x 12,288 bfloat16 numbers, 101 MB, PIECES_US.
-constexpr int PIECES_ROWS = 2;
+constexpr int PIECES_ROWS = 2, PIECES_WARPS = 8;
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide, int tokens,
+__global__ void __launch_bounds__(32 * PIECES_WARPS) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide, int tokens,
                                                      uint2* __restrict__ pieces, unsigned* __restrict__ scales) {
     ib_grid_dependency_sync();
-    const int columns = (width + 255) / 256, per_row = (width + 127) / 128 * 16, lane = threadIdx.x & 31;
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row0 = (int)(w / columns) * PIECES_ROWS, g = (int)(w % columns) * 32 + lane;
-    float v[PIECES_ROWS][8];
-#pragma unroll
-    for (int r = 0; r < PIECES_ROWS; ++r)
-        few::load8<T>(x + (long)(row0 + r) * ldx + 8 * g, row0 + r < rows ? width - 8 * g : 0, wide != 0, v[r]);
+    const few::Strip at(width, PIECES_ROWS);
+    const int row0 = at.row0, g = at.g, per_row = (width + 127) / 128 * 16, tiles = few::scale_tiles(width), lane = threadIdx.x & 31;
+    const bool all = wide && at.column + 8 <= width;
+    few::Eight<T> raw[PIECES_ROWS];
 #pragma unroll
     for (int r = 0; r < PIECES_ROWS; ++r) {
-        const unsigned byte = few::pieces_byte<PARTS>(few::block_largest(v[r]));
-        const float by = byte == 255u ? 0.0f : few::scale_reciprocal(byte);
+        const bool in = row0 + r < rows;
+        raw[r].load(x + (long)(in ? row0 + r : 0) * ldx + at.column, in ? width - at.column : 0, all && in);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[r][j] = byte == 255u ? 0.0f : v[r][j] * by;
+    for (int r = 0; r < PIECES_ROWS; ++r) {
+        const unsigned byte = few::pieces_byte<PARTS>(few::block_largest(raw[r].largest()));
+        const float by = byte == 255u ? 0.0f : few::scale_reciprocal(byte);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.0f : raw[r][j] * by;
         uint2 c[PARTS];
         if constexpr (PARTS == PIECES_BF16) {
             unsigned short h[4], l[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) two_pieces(f16_pair(v[r][2 * j], v[r][2 * j + 1]), h[j], l[j]);
+            for (int j = 0; j < 4; ++j) two_pieces(f16_pair(v[2 * j], v[2 * j + 1]), h[j], l[j]);
             c[0] = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
             c[1] = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
         } else {
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) c[part] = few::take_piece(v[r]);
+            for (int part = 0; part < PARTS; ++part) c[part] = few::take_piece(v);
         }
         unsigned word = byte << (8 * (lane >> 2 & 3));
         word |= __shfl_xor_sync(0xffffffffu, word, 4);
         word |= __shfl_xor_sync(0xffffffffu, word, 8);
         if (row0 + r >= rows || g >= per_row) continue;
-        const int at = pieces_scale_row<PARTS>(row0 + r, tokens);
+        const int first = pieces_scale_row<PARTS>(row0 + r, tokens);
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
             pieces[((long)(row0 + r) * PARTS + part) * per_row + g] = c[part];
             // every further piece's byte is five less; 255 stays (no byte is below five times the pieces in front of its own)
-            if ((lane & 15) == 0) scales[few::scale_word(at + part, g >> 4, 2 * columns)] = __vsub4(word, __vcmpne4(word, 0xFFFFFFFFu) & (0x01010101u * (5 * part)));
+            if ((lane & 15) == 0) scales[few::scale_word(first + part, g >> 4, tiles)] = __vsub4(word, __vcmpne4(word, 0xFFFFFFFFu) & (0x01010101u * (5 * part)));
         }
     }
 }
@@ -844,9 +847,9 @@ static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((
 
 template <typename T, int PARTS>
 static int make_pieces(const void* x, long ldx, int n, int k, int wide, int tokens, unsigned char* pieces, cudaStream_t stream) {
-    const long blocks = ((long)(n + PIECES_ROWS - 1) / PIECES_ROWS * ((k + 255) / 256) + 7) / 8;
-    if (blocks > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
-    ib_launch_early(pieces_kernel<T, PARTS>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, ldx, n, k, wide, tokens, (uint2*)pieces,
+    const dim3 grid(few::strips(n, k, PIECES_ROWS, PIECES_WARPS));
+    if (grid.x == 0) return IB_ERR_UNSUPPORTED;
+    ib_launch_early(pieces_kernel<T, PARTS>, grid, dim3(32 * PIECES_WARPS), 0, stream, (const T*)x, ldx, n, k, wide, tokens, (uint2*)pieces,
                     (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }
