@@ -463,19 +463,6 @@ static int launch(const Args& a, int tiles, cudaStream_t stream) {
 
 }  // namespace kv8
 
-// Attention of bfloat16 rows over pages (a multiple of 16 places) of 8-bit keys and values, heads of 64, 128 or 256 numbers.  tile_req null: every row
-// is a tile of its own (row_request says whose); else tile i holds up to tile_tokens rows of request tile_req[i] (-1: none)
-// from row tile_row0[i] on, and request r's rows end at q_start[r + 1].  splits: CTAs that share a tile's keys (1, 2, 4, 8, 16; 0: chosen here by max_len, which
-// no position is beyond).
-struct IbAttentionKv8 {
-    const void *q, *k_pages, *v_pages;
-    const float *k_scale, *v_scale;
-    const int *block_table, *row_request, *positions, *tile_req, *tile_row0, *q_start;
-    void* out;
-    cudaStream_t stream;
-    long max_pages, page_size, n_pages, n_req, n, n_tiles, tile_tokens, n_heads, n_kv, d, span, out_ld, splits, max_len;
-    double scale;
-};
 IB_EXPORT int ib_paged_attention_kv8(const IbAttentionKv8* c) {
     using namespace kv8;
     if (c->n > 0x7FFFFFFF || c->n_heads > 65536 || c->max_pages > 0x7FFFFFFF || c->n_pages > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
@@ -499,7 +486,8 @@ IB_EXPORT int ib_paged_attention_kv8(const IbAttentionKv8* c) {
     if (tiles == 0 || n == 0) return IB_OK;
     if (tile_req == nullptr) tile_tokens = 1;
     const int cols = tile_tokens * group;
-    if (tile_tokens < 1 || (tile_tokens > 1 && cols > 32)) return IB_ERR_ARGUMENT;
+    if (tile_tokens < 1) return IB_ERR_ARGUMENT;
+    if (tile_tokens > 1 && cols > 32) return ib_kv8_prompt(c);
     const int nt = cols <= 8 ? 1 : cols <= 16 || d == 256 ? 2 : tile_tokens > 1 ? 4 : 2;
     if (tile_tokens > 1 && cols > 8 * nt) return IB_ERR_ARGUMENT;
     const int chunks = (cols + 8 * nt - 1) / (8 * nt);

@@ -1,0 +1,502 @@
+// Attention of a prompt's tokens over paged keys and values in 8 bits, on the fifth-generation tensor cores (bfloat16
+// queries, heads of 128 numbers).
+//
+// A CTA owns 256 (token, head) rows of one key/value head as two tiles of 128 that take turns, and walks the keys in tiles
+// of 128, as attention_pair_tcgen05.cu does for bfloat16 pages:
+//   S  = Q K^T   in tensor memory, one region of 128 x 128 float32 per tile of rows;
+//   P  = by one thread a row, 64 keys at a time, written as f16 pairs over columns of S that have been read;
+//   O += P V     P from tensor memory, accumulated there over all keys.
+// What the codes change:
+//   keys and values   come through registers: warps 8 to 11 load a tile's codes while the tile before is in use, turn them into f16
+//       and store them in the swizzled form that the products read.  An e4m3 number's bits, moved seven to the left with the sign in its
+//       place, are the f16 number 2^-8 times as large, its small ones included: four integer instructions for two numbers, where the
+//       conversion instruction would compete with the exponentials (both run at a quarter of the other units' rate or less).
+//       The 2^8 go into the factors of the scores and of the result.
+//   queries           a row is multiplied by the power of two that brings its largest number to 2^13 .. 2^14, as in attention_kv8.cu.
+//   scores            s = S * key scale * factor of the row.
+//   softmax           the reference R of a row is one for y = s + log2(value scale), P = 2^(y - R): weights of values of very different
+//       scales keep their precision in f16.  The sum takes P / value scale in float32, so there is one exponential a
+//       score, where all value scales of a tile of keys are 0 (their y counts as s - 80) or in 2^-80 .. 2^16; in other tiles it is
+//       2^(s - R), an exponential of its own.
+// Both products take 2,048 cycles of the tensor pipe a tile of keys, the exponentials as many of theirs, the warps that convert fewer;
+// PROMPT_MEASURED.
+// All waits are bounded and report through this file's error word.
+#include "few_bits.cuh"
+#include "sm100.cuh"
+
+namespace kv8p {
+
+using namespace sm100;
+
+constexpr int D = 128, ROWS = 128, KEYS = 128, SLICE = 16;
+constexpr int CONVERT = 4, FIRST_CONVERT = 8, ISSUER = FIRST_CONVERT + CONVERT, THREADS = 32 * (ISSUER + 1);
+constexpr int HALF_BYTES = 128 * 128, TILE_BYTES = 2 * HALF_BYTES;      // [128][64] f16 numbers, swizzled; a tile of 128 x 128
+constexpr float SLACK = 8.0f, LEAST = -80.0f;                           // see attention_kv8.cu
+constexpr float LARGE_SCALE = 65536.0f;
+
+// what the softmax needs to know of a tile's keys
+struct Scales {
+    float key[KEYS], log_value[KEYS], inverse[KEYS], value[KEYS];        // log2 of the value scale (-80 for 0, -inf: no such key), 2^-that
+    int apart[CONVERT];                                                  // per converting warp: whether a value scale is out of bounds
+};
+constexpr int SMEM = 6 * TILE_BYTES + 2 * (int)sizeof(Scales) + 20 * 8 + 1024;
+static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+
+__device__ int g_error = 0;
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int code) { return mbar_wait_bounded(bar, parity, &g_error, code); }
+
+struct Args {
+    const __nv_bfloat16* q;
+    const unsigned char *k_pages, *v_pages;
+    const float *k_scale, *v_scale;
+    const int *block_table, *positions, *tile_req, *tile_row0, *q_start;
+    __nv_bfloat16* out;
+    long out_ld;
+    int max_pages, page_size, n_pages, n_req, n_rows, n_heads, n_kv, tokens, span, wide;
+    float scale;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two float32 operations in one instruction
+__device__ __forceinline__ unsigned long long two(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 apart(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned f16_pair(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// codes in the high bytes of two halves to f16 numbers 2^-8 times as large
+__device__ __forceinline__ unsigned widened(unsigned h) { return (h >> 1 & 0x3F803F80u) | (h & 0x80008000u); }
+// where chunk c (eight f16 numbers) of a row stands in a tile
+__device__ __forceinline__ unsigned place(int row, int c) { return (unsigned)((c >> 3) * HALF_BYTES + row * 128 + ((c & 7) ^ (row & 7)) * 16); }
+
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
+    extern __shared__ unsigned char raw_smem[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
+    unsigned char *sq = smem, *sk = sq + 2 * TILE_BYTES, *sv = sk + 2 * TILE_BYTES;      // queries; two stages of keys, two of values
+    Scales* scales = reinterpret_cast<Scales*>(sv + 2 * TILE_BYTES);                     // of the values' stages
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(scales + 2);
+    const unsigned q_full = smem_u32(bars);
+    const unsigned k_full0 = smem_u32(bars + 1), k_empty0 = smem_u32(bars + 3), v_full0 = smem_u32(bars + 5), v_empty0 = smem_u32(bars + 7);
+    const unsigned s_full0 = smem_u32(bars + 9);      // per tile of rows: S of the next tile of keys is there
+    const unsigned p_full0 = smem_u32(bars + 11);     // per tile of rows and half of the keys (2 t + h): its P is there
+    const unsigned h_done0 = smem_u32(bars + 15);     // per tile of rows: the first half's products are done
+    const unsigned o_full0 = smem_u32(bars + 17);     // per tile of rows: O holds every key
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 19);
+
+    ib_grid_dependency_sync();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the last tiles of a prompt see the most keys: they come first, so that the grid's tail is short
+    const int tile = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv), kvh = (int)(blockIdx.x % a.n_kv);
+    const int req = a.tile_req[tile], row0 = a.tile_row0[tile], group = a.n_heads / a.n_kv;
+    const int n_tok = req >= 0 && req < a.n_req ? min(a.tokens, a.q_start[req + 1] - row0) : 0;
+    if (n_tok <= 0 || row0 < 0 || row0 + n_tok > a.n_rows) return;          // a place of the list without a tile
+    const int tpt = ROWS / group;                                            // tokens of a tile of rows
+    const int p0 = a.positions[row0], pmax = a.positions[row0 + n_tok - 1];
+    const int lo_min = ib_first_visible(p0, a.span), t_begin = lo_min / KEYS;
+    const int n_tok_t[2] = {n_tok < tpt ? n_tok : tpt, n_tok > tpt ? n_tok - tpt : 0};
+    int n_tiles_t[2];                                                        // tiles of keys that a tile of rows walks (none without a key)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = n_tok_t[t] > 0 ? a.positions[row0 + t * tpt + n_tok_t[t] - 1] : -1;
+        n_tiles_t[t] = last >= lo_min ? last / KEYS + 1 - t_begin : 0;
+    }
+    const int n_tiles = max(n_tiles_t[0], n_tiles_t[1]);
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 8);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(k_full0 + 8 * s, CONVERT); mbar_init(k_empty0 + 8 * s, 1);
+            mbar_init(v_full0 + 8 * s, CONVERT); mbar_init(v_empty0 + 8 * s, 1);
+            mbar_init(s_full0 + 8 * s, 1); mbar_init(o_full0 + 8 * s, 1); mbar_init(h_done0 + 8 * s, 1);
+            mbar_init(p_full0 + 16 * s, 4); mbar_init(p_full0 + 16 * s + 8, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == ISSUER) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const unsigned tmem = *tmem_slot;      // columns 128 t: S and P of tile t; 256 + 128 t: O of tile t
+    bool ok = true;
+    // what was stored in shared memory is seen by the products of whoever hears of it through `bar`
+    auto handed_over = [&](unsigned bar) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+
+    if (warp >= FIRST_CONVERT && warp < ISSUER) {
+        // A warp brings 32 keys of every tile, two slices of 16 that lie in one page each: a lane 16 numbers of a row, four rows at a
+        // time.  What no row of the tile sees, and what is not in the cache, is zeros.
+        const int first = 32 * (warp - FIRST_CONVERT), row = lane >> 2 & 3, c = (lane & 3) | (lane >> 4) << 2;
+        const int* table = a.block_table + (long)req * a.max_pages;
+        struct Slice { long vector; int begin, end; };      // the first vector of the slice, the places of it that are read
+        auto look_up = [&](int i, int half) -> Slice {
+            const int j = (t_begin + i) * KEYS + first + SLICE * half, p = j / a.page_size;
+            const int page = i < n_tiles && j <= pmax && p < a.max_pages ? table[p] : -1;
+            if (page < 0 || page >= a.n_pages) return {0, 0, 0};
+            return {((long)page * a.n_kv + kvh) * a.page_size + (j - p * a.page_size), max(lo_min - j, 0), min(pmax - j + 1, SLICE)};
+        };
+        uint4 k_raw[8], v_raw[8];
+        float k_s = 0.0f, v_s = 0.0f;
+        bool here = false;                                   // whether the lane's key is one
+        auto load = [&](uint4 (&raw)[8], const unsigned char* pages, const Slice (&at)[2]) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const Slice& s = at[x >> 2];
+                const int r = 4 * (x & 3) + row;
+                raw[x] = r >= s.begin && r < s.end ? *reinterpret_cast<const uint4*>(pages + (s.vector + r) * D + 16 * c) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto store = [&](const uint4 (&raw)[8], unsigned char* to) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const int r = first + 4 * x + row;
+                const unsigned w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                unsigned h[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[2 * e] = widened(__byte_perm(w[e], 0, 0x1404));
+                    h[2 * e + 1] = widened(__byte_perm(w[e], 0, 0x3424));
+                }
+                *reinterpret_cast<uint4*>(to + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(to + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+            }
+        };
+        auto load_scales = [&](const Slice (&at)[2]) {       // of the lane's key
+            const int r = lane & 15;
+            const bool second = lane >= SLICE;
+            const long vector = second ? at[1].vector : at[0].vector;
+            here = r >= (second ? at[1].begin : at[0].begin) && r < (second ? at[1].end : at[0].end);
+            k_s = here ? a.k_scale[vector + r] : 0.0f;
+            v_s = here ? a.v_scale[vector + r] : 0.0f;
+        };
+        Slice at[2] = {look_up(0, 0), look_up(0, 1)};
+        load(k_raw, a.k_pages, at);
+        load(v_raw, a.v_pages, at);
+        load_scales(at);
+        at[0] = look_up(1, 0);
+        at[1] = look_up(1, 1);
+        for (int i = 0; i < n_tiles; ++i) {
+            const int s = i & 1;
+            if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
+            if (!ok) break;
+            store(k_raw, sk + s * TILE_BYTES);
+            handed_over(k_full0 + 8 * s);
+            load(k_raw, a.k_pages, at);
+            if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
+            if (!ok) break;
+            store(v_raw, sv + s * TILE_BYTES);
+            const float log_value = fmaxf(lg2(v_s), LEAST);
+            const bool out_of_bounds = here && v_s != 0.0f && !(v_s >= 8.271806125530277e-25f && v_s <= LARGE_SCALE);
+            scales[s].key[first + lane] = k_s;
+            scales[s].value[first + lane] = v_s;
+            scales[s].log_value[first + lane] = here ? (v_s == v_s ? log_value : v_s) : -INFINITY;
+            scales[s].inverse[first + lane] = ex2(-log_value);
+            const bool any = __any_sync(0xffffffffu, out_of_bounds);
+            if (lane == 0) scales[s].apart[warp - FIRST_CONVERT] = any;
+            handed_over(v_full0 + 8 * s);
+            load(v_raw, a.v_pages, at);
+            load_scales(at);
+            at[0] = look_up(i + 2, 0);
+            at[1] = look_up(i + 2, 1);
+        }
+    } else if (warp == ISSUER) {
+        // M = 128, N = 128, f16 in, float32 out
+        const unsigned idesc_qk = (1u << 4) | ((unsigned)(KEYS >> 3) << 17) | ((unsigned)(ROWS >> 4) << 24), idesc_pv = idesc_qk | (1u << 16);
+        if (lane == 0 && n_tiles > 0) {
+            auto issue_qk = [&](int t, int i) {
+                const int s = i & 1;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const unsigned off = (k >> 2) * HALF_BYTES + (k & 3) * 32;
+                    umma(tmem + t * 128, desc_k_major(smem_u32(sq + t * TILE_BYTES) + off), desc_k_major(smem_u32(sk + s * TILE_BYTES) + off), idesc_qk, k != 0);
+                }
+                umma_commit(s_full0 + 8 * t);
+            };
+            auto issue_pv = [&](int t, int i, int h) {      // 16 keys are eight columns of P and 16 rows of V
+                const int s = i & 1;
+#pragma unroll
+                for (int k = 4 * h; k < 4 * h + 4; ++k)
+                    umma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, desc_mn_major(smem_u32(sv + s * TILE_BYTES) + k * 16 * 128, HALF_BYTES), idesc_pv, (i | k) != 0);
+            };
+            ok = mbar_wait(q_full, 0, 2) && mbar_wait(k_full0, 0, 2);
+            if (ok) {
+                fence_after();
+                for (int t = 0; t < 2; ++t)
+                    if (n_tiles_t[t] > 0) issue_qk(t, 0);
+                umma_commit(k_empty0);
+            }
+            for (int i = 0; i < n_tiles && ok; ++i) {
+                const int s = i & 1;
+                bool have_v = false, have_k = false;
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (i < n_tiles_t[t]) {
+                        if (!mbar_wait(p_full0 + 16 * t, i & 1, 4)) { ok = false; break; }
+                        if (!have_v && !mbar_wait(v_full0 + 8 * s, (i >> 1) & 1, 3)) { ok = false; break; }
+                        have_v = true;
+                        fence_after();
+                        issue_pv(t, i, 0);
+                        umma_commit(h_done0 + 8 * t);
+                        if (!mbar_wait(p_full0 + 16 * t + 8, i & 1, 4)) { ok = false; break; }
+                        fence_after();
+                        issue_pv(t, i, 1);
+                        if (i == n_tiles_t[t] - 1) umma_commit(o_full0 + 8 * t);
+                    }
+                    if (i + 1 < n_tiles_t[t]) {
+                        if (!have_k && !mbar_wait(k_full0 + 8 * (s ^ 1), ((i + 1) >> 1) & 1, 2)) { ok = false; break; }
+                        have_k = true;
+                        fence_after();
+                        issue_qk(t, i + 1);
+                    }
+                }
+                if (!ok) break;
+                umma_commit(v_empty0 + 8 * s);
+                if (i + 1 < n_tiles) umma_commit(k_empty0 + 8 * (s ^ 1));
+            }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+    } else if (warp < FIRST_CONVERT) {
+        const int t = warp >> 2, r = (warp & 3) * 32 + lane, ti = r / group, head = kvh * group + r - ti * group;
+        const bool valid = ti < n_tok_t[t];
+        const long row = row0 + t * tpt + ti;
+        const int pos = valid ? a.positions[row] : -1, lo = valid ? ib_first_visible(pos, a.span) : 0;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, s_addr = tmem + lanes + t * 128, o_addr = s_addr + 256;
+        // the row's query
+        float factor;
+        {
+            uint4 raw[16];
+            unsigned largest = 0;
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + (row * a.n_heads + head) * D);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                raw[x] = valid ? src[x] : make_uint4(0, 0, 0, 0);
+                largest = __vmaxu2(__vmaxu2(largest, raw[x].x & 0x7FFF7FFFu), __vmaxu2(raw[x].y & 0x7FFF7FFFu, __vmaxu2(raw[x].z & 0x7FFF7FFFu, raw[x].w & 0x7FFF7FFFu)));
+            }
+            largest = max(largest & 0xFFFF0000u, largest << 16);
+            const int e = (int)(largest >> 23), up = largest == 0 ? 0 : 140 - e < 127 ? 140 - e : 127;
+            const float by = __uint_as_float((unsigned)(up + 127) << 23);
+            factor = e == 255 ? __uint_as_float(0x7FC00000u) : 256.0f * (a.scale * 1.4426950408889634f / by);      // a query that is none
+            unsigned char* to = sq + t * TILE_BYTES;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const unsigned w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                unsigned h[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) h[y] = f16_pair(__uint_as_float(w[y] << 16) * by, __uint_as_float(w[y] & 0xFFFF0000u) * by);
+                *reinterpret_cast<uint4*>(to + place(r, x)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            handed_over(q_full);
+        }
+        const unsigned long long factor2 = two(factor, factor);
+        float ref = -INFINITY, l = 0.0f;      // what P and O are relative to, and the sum
+        const int my_tiles = n_tiles_t[t];
+        for (int i = 0; i < my_tiles; ++i) {
+            const Scales& of = scales[i & 1];
+            if (ok && !mbar_wait(v_full0 + 8 * (i & 1), (i >> 1) & 1, 5)) ok = false;
+            if (ok && !mbar_wait(s_full0 + 8 * t, i & 1, 5)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const int4 far = *reinterpret_cast<const int4*>(of.apart);
+            const bool scales_apart = (far.x | far.y | far.z | far.w) != 0;
+#pragma unroll 1
+            for (int h = 0; h < 2 && ok; ++h) {
+                const int in = 64 * h, key0 = (t_begin + i) * KEYS + in;
+                unsigned v[2][32];
+                tmem_ld32_issue(s_addr + in, v[0]);
+                tmem_ld32_issue(s_addr + in + 32, v[1]);
+                tmem_ld_wait();
+                // y = S * key scale * factor + log2 value scale
+#pragma unroll
+                for (int j = 0; j < 64; j += 4) {
+                    unsigned* x = v[j >> 5] + (j & 31);
+                    const float4 ks = *reinterpret_cast<const float4*>(of.key + in + j), lv = *reinterpret_cast<const float4*>(of.log_value + in + j);
+                    const float2 y0 = apart(fma2(mul2(two(__uint_as_float(x[0]), __uint_as_float(x[1])), two(ks.x, ks.y)), factor2, two(lv.x, lv.y)));
+                    const float2 y1 = apart(fma2(mul2(two(__uint_as_float(x[2]), __uint_as_float(x[3])), two(ks.z, ks.w)), factor2, two(lv.z, lv.w)));
+                    x[0] = __float_as_uint(y0.x); x[1] = __float_as_uint(y0.y); x[2] = __float_as_uint(y1.x); x[3] = __float_as_uint(y1.y);
+                }
+                if (!(key0 >= lo && key0 + 63 <= pos)) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (key0 + j < lo || key0 + j > pos) v[j >> 5][j & 31] = 0xff800000u;
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    mx4[j & 3] = max3(mx4[j & 3], __uint_as_float(v[0][2 * j]), __uint_as_float(v[0][2 * j + 1]));
+                    mx4[(j + 2) & 3] = max3(mx4[(j + 2) & 3], __uint_as_float(v[1][2 * j]), __uint_as_float(v[1][2 * j + 1]));
+                }
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                const bool move = mx > ref + SLACK || (ref == -INFINITY && mx > -INFINITY);
+                if ((i | h) != 0 && __any_sync(0xffffffffu, move)) {
+                    // O stands still while its rows are scaled: in the first half, for S of this tile is there and all products
+                    // before it are done; in the second the first half's have to be
+                    if (h == 1 && !mbar_wait(h_done0 + 8 * t, i & 1, 6)) ok = false;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    fence_after();
+                    const float fade = move ? (ref == -INFINITY ? 0.0f : ex2(ref - mx)) : 1.0f;
+#pragma unroll 1
+                    for (int x = 0; x < D; x += 16) {
+                        float o[16];
+                        tmem_ld16(o_addr + x, o);
+                        unsigned w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * fade);
+                        tmem_st16(o_addr + x, w);
+                    }
+                    l *= fade;
+                }
+                if (move) ref = mx;
+                const float less = ref == -INFINITY ? 0.0f : -ref;
+                const unsigned long long less2 = two(less, less);
+                unsigned long long sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    unsigned w[16];
+                    if (!scales_apart) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 inv = *reinterpret_cast<const float4*>(of.inverse + in + 32 * b + j);
+                            float2 x0 = apart(add2(two(__uint_as_float(v[b][j]), __uint_as_float(v[b][j + 1])), less2));
+                            float2 x1 = apart(add2(two(__uint_as_float(v[b][j + 2]), __uint_as_float(v[b][j + 3])), less2));
+                            x0.x = ex2(x0.x); x0.y = ex2(x0.y); x1.x = ex2(x1.x); x1.y = ex2(x1.y);
+                            sum2[0] = fma2(two(x0.x, x0.y), two(inv.x, inv.y), sum2[0]);
+                            sum2[1] = fma2(two(x1.x, x1.y), two(inv.z, inv.w), sum2[1]);
+                            w[j / 2] = f16_pair(x0.x, x0.y);
+                            w[j / 2 + 1] = f16_pair(x1.x, x1.y);
+                        }
+                    } else {
+                        unsigned again[32];      // S, which P has not reached yet
+                        tmem_ld32_issue(s_addr + in + 32 * b, again);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float e[2], p[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int key = in + 32 * b + j + x;
+                                const bool hidden = v[b][j + x] == 0xff800000u;
+                                const float s = __uint_as_float(again[j + x]) * of.key[key] * factor + less;
+                                e[x] = hidden ? 0.0f : ex2(s);
+                                p[x] = hidden ? 0.0f : ex2(s + lg2(of.value[key]));
+                            }
+                            sum2[0] = add2(sum2[0], two(e[0], e[1]));
+                            w[j / 2] = f16_pair(p[0], p[1]);
+                        }
+                    }
+                    tmem_st16(s_addr + 32 * h + 16 * b, w);
+                }
+                const float2 sum = apart(add2(sum2[0], sum2[1]));
+                l += sum.x + sum.y;
+                tmem_st_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full0 + 16 * t + 8 * h);
+            }
+            if (!ok) break;
+        }
+        if (ok && my_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * t, 0, 6));
+        if (ok) {
+            fence_after();
+            const float inv = l != 0.0f ? 256.0f / l : 0.0f;      // a row that sees no key: zeros
+            __nv_bfloat16* dst = a.out + row * a.out_ld + (long)head * D;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 16) {
+                float o[16];
+                if (my_tiles > 0) tmem_ld16(o_addr + x, o);
+                unsigned w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = inv == 0.0f ? 0u : pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv);
+                if (!valid) continue;
+                if (a.wide) {
+                    *reinterpret_cast<uint4*>(dst + x) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(dst + x + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        reinterpret_cast<unsigned short*>(dst + x)[2 * j] = (unsigned short)w[j];
+                        reinterpret_cast<unsigned short*>(dst + x)[2 * j + 1] = (unsigned short)(w[j] >> 16);
+                    }
+                }
+            }
+        }
+    }
+    // after a wait that ran out the products in flight are given time to end before the shared memory is given back
+    if (!ok) for (const unsigned long long since = global_ns(); global_ns() - since < 20000000ull;) {}
+    fence_before();
+    __syncthreads();
+    if (warp == ISSUER) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace kv8p
+
+IB_EXPORT int ib_attention_kv8_error(int reset) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, kv8p::g_error, sizeof(int));
+    if (e != cudaSuccess) return -(int)e;
+    if (reset && v != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(kv8p::g_error, &zero, sizeof(int));
+    }
+    return v;
+}
+IB_EXPORT int ib_attention_kv8_error_async(int* out, cudaStream_t stream) {
+    return (int)cudaMemcpyFromSymbolAsync(out, kv8p::g_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+}
+
+// Tile i holds up to 2 * (128 / group) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, the request's rows
+// end at q_start[r + 1], and their positions grow.
+int ib_kv8_prompt(const IbAttentionKv8* c) {
+    using namespace kv8p;
+    const int group = (int)(c->n_heads / c->n_kv);
+    if (c->d != D || group > ROWS || c->tile_tokens > 2 * (ROWS / group) || reinterpret_cast<uintptr_t>(c->q) % 16) return IB_ERR_UNSUPPORTED;
+    if (c->n_tiles * c->n_kv > 0x7FFFFFFF) return IB_ERR_UNSUPPORTED;
+    static IbDeviceSet done;
+    if (int r = ib_allow_dynamic_smem(done, prompt_kernel, SMEM)) return r;
+    const Args a = {(const __nv_bfloat16*)c->q, (const unsigned char*)c->k_pages, (const unsigned char*)c->v_pages, c->k_scale, c->v_scale,
+                    c->block_table, c->positions, c->tile_req, c->tile_row0, c->q_start, (__nv_bfloat16*)c->out, c->out_ld,
+                    (int)c->max_pages, (int)c->page_size, (int)c->n_pages, (int)c->n_req, (int)c->n, (int)c->n_heads, (int)c->n_kv, (int)c->tile_tokens,
+                    (int)c->span, reinterpret_cast<uintptr_t>(c->out) % 16 == 0 && c->out_ld % 8 == 0, (float)c->scale};
+    ib_launch(prompt_kernel, dim3((unsigned)(c->n_tiles * c->n_kv)), dim3(THREADS), SMEM, c->stream, a);
+    return ib_launch_status();
+}

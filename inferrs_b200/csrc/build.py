@@ -45,7 +45,7 @@ LIBRARIES: Dict[str, dict] = {
     "core_bf16": {"sources": _CORE_SOURCES, "flags": ["-DIB_ACT_BF16=1"], "link": []},
     "gemm_bf16": {"sources": ["gemm_tcgen05.cu", "gemm_chain.cu"], "flags": ["-DIB_ACT_BF16=1"], "link": []},
     # matrices in 4 bits, keys and values in 8: float32 and bfloat16 rows both
-    "few_bits": {"sources": ["few_bits.cu", "gemm_mx4.cu", "kv8.cu", "attention_kv8.cu"], "flags": ["-DIB_ACT_BF16=1"], "link": []},
+    "few_bits": {"sources": ["few_bits.cu", "gemm_mx4.cu", "kv8.cu", "attention_kv8.cu", "attention_kv8_prompt.cu"], "flags": ["-DIB_ACT_BF16=1"], "link": []},
     "gemm_f32": {"sources": ["gemm_split_tcgen05.cu"], "flags": ["-DIB_ACT_BF16=0"], "link": []},
     # host code only (the cache's book-keeping and the step description): the C++ compiler alone builds it
     "host_runtime": {"sources": ["host_runtime.cpp"], "flags": [], "link": [], "host": True},

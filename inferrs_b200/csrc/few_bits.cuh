@@ -179,3 +179,19 @@ __device__ __forceinline__ void vector_scale(float a, float& by, float& scale) {
 }
 
 }  // namespace few
+
+// Attention of bfloat16 rows over pages (a multiple of 16 places) of 8-bit keys and values, heads of 64, 128 or 256 numbers.  tile_req null: every row
+// is a tile of its own (row_request says whose); else tile i holds up to tile_tokens rows of request tile_req[i] (-1: none)
+// from row tile_row0[i] on, and request r's rows end at q_start[r + 1]; tiles of more than 32 (row, head) pairs of a key/value head
+// run on attention_kv8_prompt.cu's kernel.  splits: CTAs that share a tile's keys (1, 2, 4, 8, 16; 0: chosen here by max_len, which
+// no position is beyond).
+struct IbAttentionKv8 {
+    const void *q, *k_pages, *v_pages;
+    const float *k_scale, *v_scale;
+    const int *block_table, *row_request, *positions, *tile_req, *tile_row0, *q_start;
+    void* out;
+    cudaStream_t stream;
+    long max_pages, page_size, n_pages, n_req, n, n_tiles, tile_tokens, n_heads, n_kv, d, span, out_ld, splits, max_len;
+    double scale;
+};
+int ib_kv8_prompt(const IbAttentionKv8* c);

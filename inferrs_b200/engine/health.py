@@ -20,7 +20,7 @@ class KernelHealth:
     def __init__(self, dtype: torch.dtype, every: int = 16):
         self.dtype = dtype
         self.every = every                   # steps between two looks when no request ends
-        self.host = torch.zeros((8,), dtype=torch.int32).pin_memory()
+        self.host = torch.zeros((len(kernels.ERROR_WORDS + kernels.FEW_BITS_WORDS),), dtype=torch.int32).pin_memory()
         self.event: Optional[torch.cuda.Event] = None
 
     @property

@@ -2661,10 +2661,17 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
 KV8_HEAD_DIMS = (64, 128, 256)   # head sizes that the tensor cores' kernel takes
 
 
-def kv8_tile_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+KV8_PROMPT_MIN_CTAS = 64         # see kv8_tile_tokens
+
+
+def kv8_tile_tokens(n_heads: int, n_kv_heads: int, head_dim: int, n_rows: int = 0) -> int:
     """Tokens of a prompt that a tile of :func:`paged_attention_kv8` holds at most: 32 (token, head) pairs of a key/value head,
-    16 with heads of 256."""
-    return max(1, (16 if head_dim == 256 else 32) // (n_heads // n_kv_heads))
+    16 with heads of 256.  With heads of 128 and ``n_rows`` rows, where tiles of 256 pairs (two of 128 that take turns on a CTA, which
+    walks all keys) give at least ``KV8_PROMPT_MIN_CTAS`` CTAs: those."""
+    group = n_heads // n_kv_heads
+    if head_dim == 128 and group <= 128 and n_rows // (2 * (128 // group)) * n_kv_heads >= KV8_PROMPT_MIN_CTAS:
+        return 2 * (128 // group)
+    return max(1, (16 if head_dim == 256 else 32) // group)
 
 
 def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Tensor, row_request: torch.Tensor,
@@ -2677,7 +2684,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     bfloat16 heads of 64, 128 and 256 numbers in pages of a multiple of 16 places run on the tensor cores, the rest in float32
     one row and head at a time.
     ``tiles`` = (tile_req, tile_row0, n_tiles, q_start, tokens) lets rows of one request share what they read: tile i holds
-    up to ``tokens`` (at most :func:`kv8_tile_tokens`) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
+    up to ``tokens`` (at most :func:`kv8_tile_tokens` of any number of rows) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
     request r's rows end at q_start[r + 1]."""
     act = out.dtype
     out_ld = _need_rows(out, "out", _BF16_F32)
@@ -2703,7 +2710,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
             tile_req, tile_row0, n_tiles, q_start, tokens = tiles
             for name, t in (("tile_req", tile_req), ("tile_row0", tile_row0), ("q_start", q_start)):
                 _need(t, name, _I, 1)
-            if min(tile_req.shape[0], tile_row0.shape[0]) < n_tiles or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d):
+            if min(tile_req.shape[0], tile_row0.shape[0]) < n_tiles or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d, 1 << 30):
                 raise KernelError(f"paged_attention_kv8: {n_tiles} tiles of {tokens} tokens in lists of {tile_req.shape[0]}")
             tile_req, tile_row0, q_start = tile_req.data_ptr(), tile_row0.data_ptr(), q_start.data_ptr()
         code = lib.ib_paged_attention_kv8(_ATTENTION_CALL(
@@ -2721,7 +2728,8 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
 
 
 # names of the words that :func:`few_bits_faults` reads
-FEW_BITS_WORDS = ("a row's position outside the rotation tables (8-bit cache)", "matrix product (4-bit weights)")
+FEW_BITS_WORDS = ("a row's position outside the rotation tables (8-bit cache)", "matrix product (4-bit weights)",
+                  "prefill attention (8-bit cache)")
 
 
 def few_bits_faults(reset: bool = True) -> dict:
@@ -2729,7 +2737,8 @@ def few_bits_faults(reset: bool = True) -> dict:
     the device; empty where the library was never needed."""
     if _FEW_BITS_LIB is None:
         return {}
-    values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)), _FEW_BITS_LIB.ib_gemm_mx4_error(int(reset)))
+    values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)), _FEW_BITS_LIB.ib_gemm_mx4_error(int(reset)),
+              _FEW_BITS_LIB.ib_attention_kv8_error(int(reset)))
     return {name: v for name, v in zip(FEW_BITS_WORDS, values) if v}
 
 
@@ -2760,7 +2769,8 @@ def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
     if host.numel() >= len(ERROR_WORDS) + len(FEW_BITS_WORDS):       # those of the kernels in few bits behind them
         host[len(ERROR_WORDS):len(ERROR_WORDS) + len(FEW_BITS_WORDS)] = 0
         if _FEW_BITS_LIB is not None:
-            for i, fn in enumerate((_FEW_BITS_LIB.ib_kv8_row_fault_async, _FEW_BITS_LIB.ib_gemm_mx4_error_async)):
+            for i, fn in enumerate((_FEW_BITS_LIB.ib_kv8_row_fault_async, _FEW_BITS_LIB.ib_gemm_mx4_error_async,
+                                    _FEW_BITS_LIB.ib_attention_kv8_error_async)):
                 code = fn(at + 4 * (len(ERROR_WORDS) + i), stream)
                 if code != 0:
                     raise KernelError(f"error_words_async: CUDA error {code}")

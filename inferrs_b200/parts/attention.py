@@ -295,7 +295,7 @@ class Attention:
             kernels.paged_attention(q, k_pages, v_pages, table, ctx, s.scale, self.span, out, **self._options(gate))
 
     def _attend_kv8(self, ctx, cache_id: int, qkv: torch.Tensor, out: torch.Tensor):
-        """The same over a cache in 8 bits: a step of single tokens one row each, a step with portions of prompts in tiles."""
+        """The same over a cache in 8 bits: single tokens one row each, portions of prompts in tiles."""
         s = self.spec
         pages, group = ctx.storage.pages8(cache_id)
         table = ctx.block_tables[group]
@@ -303,13 +303,23 @@ class Attention:
         kernels.qk_norm_rope_store_kv8(qkv, s.n_heads, s.n_kv_heads, s.head_dim, self.q_weight, self.k_weight, self.eps, self.cos,
                                        self.sin, self.rot_dim, ctx.positions, ctx.row_request, table, pages, q,
                                        interleaved=self.interleaved)
-        tiles = None
-        if not ctx.decode_only:
-            tokens = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim)
-            tile_req, tile_row0, n_tiles = ctx.attention_tiles(tokens)
-            tiles = (tile_req, tile_row0, n_tiles, ctx.q_start, tokens)
-        kernels.paged_attention_kv8(q, pages, table, ctx.row_request, ctx.positions, s.scale, self.span, out, ctx.max_kv_len,
-                                    tiles=tiles)
+
+        def attend(tiles=None):
+            kernels.paged_attention_kv8(q, pages, table, ctx.row_request, ctx.positions, s.scale, self.span, out, ctx.max_kv_len,
+                                        tiles=tiles)
+
+        few = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim)
+        if ctx.decode_only or self.rt.dtype != torch.bfloat16:
+            attend()
+            return
+        tokens = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim, ctx.extra.get("dispatch_rows", ctx.n_rows))
+        if tokens > few:      # a large tile would hold one of the single tokens: those go row by row
+            rows, reqs, n_single = ctx.single_rows()
+            if n_single:
+                attend((reqs, rows, n_single, ctx.q_start, 1))
+        tile_req, tile_row0, n_tiles = ctx.attention_tiles(tokens, portions_only=tokens > few)
+        if n_tiles:
+            attend((tile_req, tile_row0, n_tiles, ctx.q_start, tokens))
 
     def _options(self, gate):
         """The fields of :class:`~inferrs_b200.kernels.ScoreOptions` that this layer uses."""
