@@ -18,8 +18,10 @@
 //       scales keep their precision in f16.  The sum takes P / value scale in float32, so there is one exponential a
 //       score, where all value scales of a tile of keys are 0 (their y counts as s - 80) or in 2^-80 .. 2^16; in other tiles it is
 //       2^(s - R), an exponential of its own.
-// Both products take 2,048 cycles of the tensor pipe a tile of keys, the exponentials as many of theirs, the warps that convert fewer;
-// PROMPT_MEASURED.
+// Both products take 2,048 cycles of the tensor pipe a tile of keys, the exponentials as many of theirs; a tile takes 7,500 (3.9 us): a
+// softmax warp's own instruction stream, one warp of either tile of rows on each of the SM's four schedulers, 0.4 instructions a cycle
+// (without the scales 6,000, without the conversions 7,000, without the exponentials 7,000).  A prompt of 2,048 tokens, 32 heads on 8: 84 us,
+// 410 TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
 // All waits are bounded and report through this file's error word.
 #include "few_bits.cuh"
 #include "sm100.cuh"
