@@ -14,18 +14,17 @@ namespace few {
 constexpr int QUANT_ROWS = 4, QUANT_WARPS = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
+__global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width,
                                                                     unsigned* __restrict__ codes, unsigned char* __restrict__ scales) {
     ib_grid_dependency_sync();
     const Strip at(width, QUANT_ROWS);
     const int lane = threadIdx.x & 31, tiles = scale_tiles(width);
     const long pitch = code_pitch(width) / 4;
-    const bool all = wide && at.column + 8 <= width;
     Eight<T> v[QUANT_ROWS];
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
         const bool in = at.row0 + r < rows;
-        v[r].load(x + (long)(in ? at.row0 + r : 0) * ldx + at.column, in ? width - at.column : 0, all && in);
+        v[r].load(x + (long)(in ? at.row0 + r : 0) * ldx + at.column, in ? width - at.column : 0);
     }
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
@@ -43,7 +42,7 @@ __global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __r
 
 template <typename T>
 __global__ void __launch_bounds__(32 * QUANT_WARPS) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales,
-                                                         int rows, int width, int wide, T* __restrict__ out, long ldo) {
+                                                         int rows, int width, T* __restrict__ out, long ldo) {
     ib_grid_dependency_sync();
     const Strip at(width, QUANT_ROWS);
     const int row0 = at.row0, g = at.g, lane = threadIdx.x & 31, tiles = scale_tiles(width);
@@ -59,32 +58,13 @@ __global__ void __launch_bounds__(32 * QUANT_WARPS) dequantize_kernel(const unsi
     for (int r = 0; r < QUANT_ROWS; ++r) {
         if (row0 + r >= rows || 8 * g >= width) break;
         const float s = scale_value(word[r] >> (8 * (lane >> 2 & 3)) & 255u);
-        float v[8];
+        Eight<T> v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 two = __half22float2(values4x2(c[r] >> (8 * j)));
-            v[2 * j] = two.x * s;
-            v[2 * j + 1] = two.y * s;
+            v.set(j, two.x * s, two.y * s);
         }
-        T* o = out + (long)(row0 + r) * ldo + 8 * g;
-        if (wide && 8 * g + 8 <= width) {
-            if constexpr (sizeof(T) == 2) {
-                uint4 to;
-                unsigned* p = &to.x;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-                    p[j] = *reinterpret_cast<unsigned*>(&b);
-                }
-                *reinterpret_cast<uint4*>(o) = to;
-            } else {
-                reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) if (8 * g + j < width) o[j] = ib_from_float<T>(v[j]);
-        }
+        v.store(out + (long)(row0 + r) * ldo + 8 * g, width - 8 * g);
     }
 }
 
@@ -107,12 +87,10 @@ IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     const int x_is_f32 = (int)q->x_is_f32, rows = (int)q->rows, width = (int)q->width;
     if (rows < 0 || width <= 0 || ldx < width) return IB_ERR_ARGUMENT;
     if (rows == 0) return IB_OK;
-    const size_t e = x_is_f32 ? 4 : 2;
-    const int wide = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * e) % 16 == 0) ? 1 : 0;
     const dim3 grid(strips(rows, width, QUANT_ROWS, QUANT_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
-    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
+    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const float*)x, ldx, rows, width, (unsigned*)codes, (unsigned char*)scales);
+    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, (unsigned*)codes, (unsigned char*)scales);
     return ib_launch_status();
 }
 
@@ -132,11 +110,9 @@ IB_EXPORT int ib_dequantize_mx4(const IbDequantizeMx4* q) {
     const int out_is_f32 = (int)q->out_is_f32, rows = (int)q->rows, width = (int)q->width;
     if (rows < 0 || width <= 0 || ldo < width) return IB_ERR_ARGUMENT;
     if (rows == 0) return IB_OK;
-    const size_t e = out_is_f32 ? 4 : 2;
-    const int wide = (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * e) % 16 == 0) ? 1 : 0;
     const dim3 grid(strips(rows, width, QUANT_ROWS, QUANT_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (out_is_f32) ib_launch_early(dequantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (float*)out, ldo);
-    else ib_launch_early(dequantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, wide, (__nv_bfloat16*)out, ldo);
+    if (out_is_f32) ib_launch_early(dequantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, (float*)out, ldo);
+    else ib_launch_early(dequantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const unsigned*)codes, (const unsigned*)scales, rows, width, (__nv_bfloat16*)out, ldo);
     return ib_launch_status();
 }

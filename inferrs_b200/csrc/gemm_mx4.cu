@@ -50,7 +50,7 @@ struct Params {
     int x_groups;                            // 128-row tiles of x's scales
     const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
     long ldx;
-    int k, wide;                             // wide: rows start on 16 bytes
+    int k;
     int wait_first;                          // the kernel ahead may have written the weights: nothing is read before it is done
 };
 
@@ -214,23 +214,14 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
     if (i >= helpers) return true;
     for (int a = i; half == 0 && a < nkb && a < sh.stages; a += helpers) fetch_scales(a, a);      // before the kernel ahead is done
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    uint4 raw[PASSES];
+    few::Eight<__nv_bfloat16> raw[PASSES];
     const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(2 * half + (lane >> 4)) * p.ldx + 8 * g);
     auto fetch_x = [&](int i) {
         const int c = (kb0 + i) * 128;
 #pragma unroll
         for (int j = 0; j < PASSES; ++j) {
-            raw[j] = make_uint4(0, 0, 0, 0);
-            if (4 * j + 2 * half + (lane >> 4) >= p.n_tok || i >= nkb) continue;
-            const __nv_bfloat16* src = x + 4L * j * p.ldx + c;
-            const int n = p.k - c - 8 * g;
-            if (p.wide && n >= 8) {
-                raw[j] = *reinterpret_cast<const uint4*>(src);
-            } else {
-                unsigned short* to = reinterpret_cast<unsigned short*>(&raw[j]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) if (e < n) to[e] = *reinterpret_cast<const unsigned short*>(src + e);
-            }
+            const bool in = 4 * j + 2 * half + (lane >> 4) < p.n_tok && i < nkb;
+            raw[j].load(x + (in ? 4L * j * p.ldx + c : 0), in ? p.k - c - 8 * g : 0);
         }
     };
     if constexpr (INSIDE) fetch_x(i);
@@ -244,7 +235,7 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
                 if (4 * j + 2 * half >= p.n_tok) break;       // columns of no token: whatever the stage holds
-                const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+                const unsigned (&w)[4] = raw[j].w;
                 unsigned m = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7FFF7FFFu);
@@ -660,17 +651,16 @@ template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(in
 // bounds it where the conversions leave it time: 2,048 x 12,288 bfloat16 numbers, 101 MB, 29 us.
 constexpr int PIECES_ROWS = 2, PIECES_WARPS = 8;
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(32 * PIECES_WARPS) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide, int tokens,
+__global__ void __launch_bounds__(32 * PIECES_WARPS) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int tokens,
                                                      uint2* __restrict__ pieces, unsigned* __restrict__ scales) {
     ib_grid_dependency_sync();
     const few::Strip at(width, PIECES_ROWS);
     const int row0 = at.row0, g = at.g, per_row = (width + 127) / 128 * 16, tiles = few::scale_tiles(width), lane = threadIdx.x & 31;
-    const bool all = wide && at.column + 8 <= width;
     few::Eight<T> raw[PIECES_ROWS];
 #pragma unroll
     for (int r = 0; r < PIECES_ROWS; ++r) {
         const bool in = row0 + r < rows;
-        raw[r].load(x + (long)(in ? row0 + r : 0) * ldx + at.column, in ? width - at.column : 0, all && in);
+        raw[r].load(x + (long)(in ? row0 + r : 0) * ldx + at.column, in ? width - at.column : 0);
     }
 #pragma unroll
     for (int r = 0; r < PIECES_ROWS; ++r) {
@@ -846,10 +836,10 @@ static int tile_tokens(int x_kind, int n) {
 static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((k + 127) / 128 * 128) + 511) / 512 * 512; }
 
 template <typename T, int PARTS>
-static int make_pieces(const void* x, long ldx, int n, int k, int wide, int tokens, unsigned char* pieces, cudaStream_t stream) {
+static int make_pieces(const void* x, long ldx, int n, int k, int tokens, unsigned char* pieces, cudaStream_t stream) {
     const dim3 grid(few::strips(n, k, PIECES_ROWS, PIECES_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    ib_launch_early(pieces_kernel<T, PARTS>, grid, dim3(32 * PIECES_WARPS), 0, stream, (const T*)x, ldx, n, k, wide, tokens, (uint2*)pieces,
+    ib_launch_early(pieces_kernel<T, PARTS>, grid, dim3(32 * PIECES_WARPS), 0, stream, (const T*)x, ldx, n, k, tokens, (uint2*)pieces,
                     (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }
@@ -907,7 +897,6 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     p.x = x;
     p.ldx = ldx;
     p.k = k;
-    p.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_kind ? 4 : 2) % 16 == 0;
     p.w_scales = (const unsigned char*)w_scales;
     if (x_kind == 0 && n <= INSIDE_ROWS) return launch_few<PIECES_BF16, 16, true>(w, nullptr, n, m, k, p, tile_rows, splits, stream, false);
     if (x_kind == 2) {
@@ -921,12 +910,12 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     const int tokens = tile_tokens(x_kind, n);
     if (x_kind == 1) {
         p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
-        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, p.wide, tokens, pieces, stream)) return r;
+        if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, tokens, pieces, stream)) return r;
         if (tokens == 16) return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
         return launch<PIECES_F32, 160, 5>(w, pieces, n, m, k, p, stream, true);
     }
     p.x_scales = pieces + pieces_bytes(PIECES_BF16, n, k);
-    if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, p.wide, tokens, pieces, stream)) return r;
+    if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, tokens, pieces, stream)) return r;
     if (tokens == 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
     if (tokens == 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
     if (tokens == 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);

@@ -518,3 +518,28 @@ def test_attention_of_prompts_over_eight_bit_pages(heads, kv, d, span):
     limit = attention_limit(want, weight, size, d, max(lengths), torch.bfloat16)
     for got in (out, one):
         assert bool(((got.double().view(n, heads, d) - want).abs() <= limit).all())
+
+
+# ---- rows that start anywhere in memory ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("pad,offset", [(1, 0), (2, 0), (3, 1), (4, 0), (4, 2), (6, 1), (8, 0), (8, 1), (8, 4), (12, 4)])
+def test_rows_that_start_anywhere(pad, offset, dtype):
+    """The same bits as rows side by side give, nothing written beside the rows."""
+    from inferrs_b200 import kernels as K
+    width = 271
+    whole = rand((37, width + pad + offset), 5).to(DT[dtype])
+    x = whole[:, offset:offset + width]
+    w, same = K.quantize_mx4(x), K.quantize_mx4(x.contiguous())
+    assert torch.equal(w.codes, same.codes)
+    room = torch.full_like(whole, 7.0)
+    straight = torch.empty((37, width), dtype=DT[dtype], device="cuda")
+    K.dequantize_mx4(w, room[:, offset:offset + width])
+    K.dequantize_mx4(same, straight)          # (scales behind the last row are not written: what counts are the values)
+    assert torch.equal(room[:, offset:offset + width], straight)
+    assert bool((room[:, :offset] == 7).all()) and bool((room[:, offset + width:] == 7).all())
+    m = K.quantize_mx4(rand((130, width), 6))
+    for rows in (1, 7, 37):
+        got, want = (torch.empty((rows, 130), device="cuda") for _ in range(2))
+        K.linear_mx4(x[:rows], m, got)
+        K.linear_mx4(x[:rows].contiguous(), m, want)
+        assert torch.equal(got, want)
