@@ -2409,6 +2409,8 @@ _FEW_BITS_SIGNATURES = {
     "ib_gemm_mx4": [ctypes.c_char_p],
     "ib_gemm_mx4_error": [c_int],
     "ib_gemm_mx4_error_async": [c_void_p, c_void_p],
+    "ib_attention_kv8_error": [c_int],
+    "ib_attention_kv8_error_async": [c_void_p, c_void_p],
     "ib_qk_norm_rope_store_kv8": [ctypes.c_char_p],
     "ib_paged_attention_kv8": [ctypes.c_char_p],
     "ib_paged_attention_kv8_generic": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
