@@ -15,13 +15,14 @@
 // TMA brings tiles of 128 weight rows and of tokens into a ring of 128-byte-swizzled stages (4-bit weights beside 8-bit
 // pieces are spread to a byte each on the way), and 512-byte tiles of scales, which the issuing thread copies into tensor
 // memory in front of the products that use them (every stage has its own columns, so none is overwritten early).
-// Accumulators are float32 in tensor memory.  Roles: warp 0 copies, warp 1 products, warps 2..5 read back.  Up to eight
-// bfloat16 rows are brought to pieces inside the product, by warps 6..9 of every CTA while the weights stream in; more rows by
-// a kernel of their own, and the product starts while that one runs.
+// Accumulators are float32 in tensor memory.  Roles: warp 0 copies (warp 6 the scales, where they are tiles), warp 1 issues
+// products, warps 2..5 read back.  Up to eight bfloat16 rows are brought to pieces inside the product, by warps 6.. of every CTA while
+// the weights stream in; more rows by a kernel of their own, and the product starts while that one runs.
 //
-// Where low tiles would keep the tensor core longer than the weights take, K is cut over a cluster (1, 1, splits): every CTA sends its partial sums to their owners (each has
-// an equal share of the tile's rows) through distributed shared memory, one cluster barrier follows, and the owner adds
-// them in the order of the ranks.  Every wait is bounded and reports through this file's error word.
+// Up to 64 rows (few_rows_kernel), where low tiles would keep the tensor core longer than the weights take, K is cut over a cluster
+// (1, 1, splits): every CTA sends its partial sums to their owners (each has an equal share of the tile's rows) through
+// distributed shared memory, one cluster barrier follows, and the owner adds them in the order of the ranks.  More rows
+// (gemm_kernel): pairs of CTAs.  Every wait is bounded and reports through this file's error word.
 #include <cuda.h>
 
 #include "few_bits.cuh"
@@ -47,7 +48,6 @@ struct Params {
     int y_is_f32, y_wide, n_tok, n_out, num_kb;      // num_kb: stages that K takes
     const unsigned char *w_scales, *x_scales;
     int scale_tiles;                         // 128-column tiles of scales per 128 rows
-    int x_groups;                            // 128-row tiles of x's scales
     const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
     long ldx;
     int k;
@@ -90,21 +90,24 @@ constexpr unsigned TILE_HI = (unsigned)(1024 >> 4) | 1u << 14 | 2u << 29, TILE_L
 constexpr unsigned SCALE_HI = (unsigned)(128 >> 4) | 1u << 14;
 // 512 bytes of scales (32 rows of 16 bytes, eight rows 128 bytes apart) into four columns of tensor memory, the same in
 // every quarter of the lanes
+template <int CTAS>
 __device__ __forceinline__ void scales_to_tmem(unsigned tmem, unsigned lo) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from_words(lo, SCALE_HI)) : "memory");
+    if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from_words(lo, SCALE_HI)) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from_words(lo, SCALE_HI)) : "memory");
 }
-template <int KIND>
+#define MX4_MMA(GROUP, KIND_VEC)                                                                                                   \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                                  \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND_VEC " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"                          \
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory")
+template <int KIND, int CTAS>
 __device__ __forceinline__ void umma_scaled(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sa,
                                             unsigned sb, unsigned accumulate) {
-    if constexpr (KIND != CODES)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+    if constexpr (KIND != CODES && CTAS == 1) MX4_MMA("1", "mxf8f6f4.block_scale.scale_vec::1X");
+    else if constexpr (KIND != CODES) MX4_MMA("2", "mxf8f6f4.block_scale.scale_vec::1X");
+    else if constexpr (CTAS == 1) MX4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+    else MX4_MMA("2", "mxf4.block_scale.scale_vec::2X");
 }
+#undef MX4_MMA
 
 // the plan of a stage's shared and tensor memory
 template <int KIND, int BN> struct Plan {
@@ -130,24 +133,24 @@ __device__ __forceinline__ void store(const Params& p, int t, int f, float v) {
 // One stage's products, issued by one thread: scales into the stage's columns of tensor memory (`scales`), then four products
 // of 32 bytes of each row: 32 numbers spread to bytes, or 64 packed ones.  a, b, sa, sb: where the stage's tiles start, in units of
 // 16 bytes; shift: columns of scales in front of x's.
-template <int KIND, int BN>
+template <int KIND, int BN, int CTAS>
 __device__ __forceinline__ void multiply_stage(unsigned tmem, unsigned scales, unsigned a, unsigned b, unsigned sa_tile, unsigned sb_tile,
                                                bool accumulate, unsigned shift = 0) {
     using P = Plan<KIND, BN>;
     constexpr unsigned FORMATS = KIND != CODES ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);   // e2m1 and e4m3, e2m1 twice
-    constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(BM >> 4) << 24);
+    constexpr unsigned IDESC = FORMATS | ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)(CTAS * BM >> 4) << 24);
     const unsigned sa = scales, sb = sa + 4 * P::K_TILES;
 #pragma unroll
     for (int j = 0; j < P::K_TILES; ++j) {
-        scales_to_tmem(sa + 4 * j, sa_tile + 32 * j);
+        scales_to_tmem<CTAS>(sa + 4 * j, sa_tile + 32 * j);
 #pragma unroll
         for (int g = 0; g < P::B_GROUPS; ++g)     // the column tiles one after the other, the row tiles of each side by side
-            scales_to_tmem(sb + 4 * (j * P::B_GROUPS + g), sb_tile + g * (P::SA_BYTES / 16) + 32 * j);
+            scales_to_tmem<CTAS>(sb + 4 * (j * P::B_GROUPS + g), sb_tile + g * (P::SA_BYTES / 16) + 32 * j);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const unsigned tile = KIND != CODES ? 0 : k >> 1, id = KIND != CODES ? k : (k & 1) * 2;
-        umma_scaled<KIND>(tmem, from_words(TILE_LO + a + 2 * k, TILE_HI), from_words(TILE_LO + b + 2 * k, TILE_HI),
+        umma_scaled<KIND, CTAS>(tmem, from_words(TILE_LO + a + 2 * k, TILE_HI), from_words(TILE_LO + b + 2 * k, TILE_HI),
                           IDESC | (id << 4) | (id << 29), sa + 4 * tile, sb + 4 * P::B_GROUPS * tile + shift, accumulate || k != 0);
     }
 }
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
             fence_after();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the scales came by plain copies
             if (leader) {
-                multiply_stage<KIND, BN>(tmem, tmem + BN + s * P::SCALE_COLS, a0 + s * (a_bytes >> 4), b0 + s * (P::B_BYTES / 16),
+                multiply_stage<KIND, BN, 1>(tmem, tmem + BN + s * P::SCALE_COLS, a0 + s * (a_bytes >> 4), b0 + s * (P::B_BYTES / 16),
                                          sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0);
                 umma_commit(empty0 + 8 * s);
             }
@@ -424,30 +427,46 @@ __device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMN
 }
 
 // ---- more rows ------------------------------------------------------------------------------------------------------------------
-// A pair of CTAs (a cluster) covers 256 rows of W and one tile of tokens: each loads its own 128 rows of W and half of the tokens,
-// which it sends to both.  The pairs stay and take tile after tile; two accumulators take turns, so that four warps read one back
-// and store it while the other is being filled.
+// A pair of CTAs (a cluster) multiplies 256 rows of W with one tile of tokens: each loads its own 128 rows and half of the tokens, the
+// first one issues products that read the shared memories of both and leave each CTA its own rows' results. The halves are what
+// counts: an SM's shared memory moves 128 bytes a cycle, and a stage of 128 x 192 alone has it take in and read out 64 KB (4-bit weights
+// and pieces) or 80 KB (4-bit rows), 512 and 640 cycles where the products take 384 (measured: 500 and 650); here it is 40 and 56 KB.
+// The pairs stay and take tile after tile; two accumulators take turns, so that four warps read one back and store it while the
+// other is being filled.  A stage then takes 395 cycles (pieces) and 410 .. 490 (4-bit rows, 28 KB a CTA from L2), and what bounds it is the clock
+// at which the tensor cores run under load, 1.3 to 1.6 GHz: 2,048 x 12,288 x 4,096 (bfloat16 rows) 130 us behind the 29 that bring x to
+// pieces, 3.2 PFLOP/s of 8-bit products (CTAs by themselves, one tile each: 170); 4-bit rows 2,048 x 4,096 x 24,576 72 to 81 us, 5.1 to 5.7
+// PFLOP/s (200).  Four CTAs that share x's tiles have room on 132 SMs and gain nothing.
 constexpr int PAIR = 2, STORE_BYTES = 4096;      // a warp's piece of shared memory for results on their way out
 template <int KIND, int BN, int STAGES> struct Many {
     using P = Plan<KIND, BN>;
-    static constexpr int SMEM = STAGES * (A_BYTES + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) + 4 * STORE_BYTES + 16 * STAGES + 64 + 1024;
+    static constexpr int B_BYTES = P::B_BYTES / PAIR;
+    static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES + P::SA_BYTES + P::SB_BYTES) + 4 * STORE_BYTES + 16 * STAGES + 64 + 1024;
     static_assert(2 * BN + STAGES * P::SCALE_COLS <= 512 && SMEM <= 227 * 1024 && SMEM > 114 * 1024, "memories of an SM");
-    static_assert(P::B_GROUPS == PAIR, "a CTA of the pair fetches one tile of x's scales");
     static_assert(BN % 32 == 0 && BN / PAIR % 8 == 0, "halves of a tile are whole groups of eight rows");
 };
-// The same piece of tokens, or of their scales, to both CTAs of the pair, each at the same place and counted on its own barrier.
-__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.multicast::cluster [%0], [%1, {%3, %4}], [%2], %5;"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "h"((unsigned short)3) : "memory");
-}
-__device__ __forceinline__ void bulk_load_pair(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.multicast::cluster [%0], [%1], %2, [%3], %4;"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "h"((unsigned short)3) : "memory");
-}
 // one arrival at the barrier of either CTA when the products so far are done
 __device__ __forceinline__ void umma_commit_pair(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+// where the first CTA has what stands at `local` here
+__device__ __forceinline__ unsigned at_first(unsigned local) {
+    unsigned there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(local));
+    return there;
+}
+// (relaxed: what it tells of is in registers; a release would wait for the results on their way to y)
+__device__ __forceinline__ void arrive_there(unsigned bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// into this CTA's shared memory, counted on a barrier of either CTA
+__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 // A warp stores `count` tokens' results of its 32 rows of W, a lane a row: through shared memory, so that a token's results go out in
@@ -478,17 +497,20 @@ __device__ __forceinline__ void store_rows(const Params& p, unsigned char* mine,
 
 template <int KIND, int BN, int STAGES>
 __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                       const __grid_constant__ CUtensorMap map_x, const Params p) {
+                                                            const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sw,
+                                                            const __grid_constant__ CUtensorMap map_sx, const Params p) {
     using P = Plan<KIND, BN>;
+    using M = Many<KIND, BN, STAGES>;
     extern __shared__ unsigned char raw_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
     unsigned char* a_tiles = smem;
     unsigned char* b_tiles = a_tiles + STAGES * A_BYTES;
-    unsigned char* sa_tiles = b_tiles + STAGES * P::B_BYTES;
+    unsigned char* sa_tiles = b_tiles + STAGES * M::B_BYTES;
     unsigned char* sb_tiles = sa_tiles + STAGES * P::SA_BYTES;
     unsigned char* stores = sb_tiles + STAGES * P::SB_BYTES;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(stores + 4 * STORE_BYTES);
-    // full: this CTA's stage has landed; empty: both CTAs are done with theirs; filled, drained: an accumulator
+    // full (the first CTA's): a stage has landed in both; empty: the products are done with it; filled: an accumulator holds a tile; drained
+    // (the first CTA's): both have read theirs
     const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), filled0 = smem_u32(bars + 2 * STAGES), drained0 = filled0 + 16;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * STAGES + 4);
 
@@ -497,13 +519,13 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     const int first = blockIdx.x / PAIR, step = gridDim.x / PAIR, stages = (tiles - first + step - 1) / step * nkb;      // of this pair
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, PAIR); }
-        for (int b = 0; b < 2; ++b) { mbar_init(filled0 + 8 * b, 1); mbar_init(drained0 + 8 * b, 4); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(filled0 + 8 * b, 1); mbar_init(drained0 + 8 * b, 4 * PAIR); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
@@ -513,36 +535,32 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     const unsigned tmem = *tmem_slot;
     bool ok = true;
     if (p.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
-    // Copies are issued by two threads, one for the operands and one for their scales: a thread takes 165 cycles a tile and 50 a
-    // plain copy, which together would take longer than the products of a stage.
+    // Copies are issued by two threads a CTA, one for the operands and one for their scales; those of the first CTA announce what both bring.
     if (warp == 0 || warp == 6) {
         const bool leader = elected(), operands = warp == 0;
         constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
-        const int last_f = (p.n_out + BM - 1) / BM - 1;
-        int tile = first, row_w = 0, row_x = 0;
-        const unsigned char *at_w = nullptr, *at_x = nullptr;
-        auto enter = [&]() {      // (a tile may lie behind the last row of W, and its scales behind x's: any will do, nothing of it is stored)
-            const int tile_f = tile % pairs_f * PAIR + rank, tile_t = tile / pairs_f;
-            row_w = tile_f * BM;
+        const unsigned full = at_first(full0);
+        int tile = first, tile_f = 0, row_x = 0, group = 0;
+        auto enter = [&]() {      // (what lies behind the last rows reads as zeros)
+            const int tile_t = tile / pairs_f;
+            tile_f = tile % pairs_f * PAIR + rank;
             row_x = tile_t * BN + rank * (BN / PAIR);
-            const int group = (KIND == CODES ? tile_t * BN / 128 : tile_t * P::B_GROUPS) + rank;
-            at_w = p.w_scales + (long)(tile_f < last_f ? tile_f : last_f) * p.scale_tiles * 512;
-            at_x = p.x_scales + (long)(group < p.x_groups ? group : p.x_groups - 1) * p.scale_tiles * 512;
+            group = KIND == CODES ? tile_t * BN / 128 : tile_t * P::B_GROUPS;
         };
         auto load_w = [&](int i, int s) {
             if (!leader) return;
             if (operands) {
-                mbar_expect_tx(full0 + 8 * s, W_TX + P::B_BYTES);
-                tma_load_2d(smem_u32(a_tiles) + s * A_BYTES, &map_w, i * 128, row_w, full0 + 8 * s);
+                if (rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR * (W_TX + M::B_BYTES));
+                tma_load_2d_pair(smem_u32(a_tiles) + s * A_BYTES, &map_w, i * 128, tile_f * BM, full + 8 * s);
             } else {
-                mbar_expect_tx(full0 + 8 * s, P::SA_BYTES + P::SB_BYTES);
-                bulk_load(smem_u32(sa_tiles) + s * P::SA_BYTES, at_w + i * P::SA_BYTES, P::SA_BYTES, full0 + 8 * s);
+                if (rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR * (P::SA_BYTES + P::SB_BYTES));
+                tma_load_3d_pair(smem_u32(sa_tiles) + s * P::SA_BYTES, &map_sw, 0, i * P::K_TILES, tile_f, full + 8 * s);
             }
         };
         auto load_x = [&](int i, int s) {
             if (!leader) return;
-            if (operands) tma_load_2d_pair(smem_u32(b_tiles) + s * P::B_BYTES + rank * (P::B_BYTES / PAIR), &map_x, i * 128, row_x, full0 + 8 * s);
-            else bulk_load_pair(smem_u32(sb_tiles) + s * P::SB_BYTES + rank * P::SA_BYTES, at_x + i * P::SA_BYTES, P::SA_BYTES, full0 + 8 * s);
+            if (operands) tma_load_2d_pair(smem_u32(b_tiles) + s * M::B_BYTES, &map_x, i * 128, row_x, full + 8 * s);
+            else tma_load_3d_pair(smem_u32(sb_tiles) + s * P::SB_BYTES, &map_sx, 0, i * P::K_TILES, group, full + 8 * s);      // (every CTA's rows meet all tokens)
         };
         const int head = nkb < STAGES ? nkb : STAGES;    // the first weights are on their way before the kernel ahead is done
         enter();
@@ -562,12 +580,12 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
                 if (++i == nkb) { i = 0; tile += step; enter(); }
             }
         }
-        // the other CTA's last arrivals have come: none is on its way to a CTA that has ended
+        // the last arrivals have come: none is on its way to a CTA that has ended
         for (int s = 0; ok && s < STAGES; ++s) {
             const int uses = (stages - s + STAGES - 1) / STAGES;
             ok = uses == 0 || mbar_wait(empty0 + 8 * s, (uses - 1) & 1, 1);
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         const bool leader = elected();
         const unsigned a0 = smem_u32(a_tiles) >> 4, b0 = smem_u32(b_tiles) >> 4, sa0 = smem_u32(sa_tiles) >> 4, sb0 = smem_u32(sb_tiles) >> 4;
         // a tile of 4-bit rows may start amid a tile of 128 rows of scales, 32 of them a column
@@ -585,15 +603,15 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
                 landed = mbar_test_wait(full0 + 8 * ((s + 1) % STAGES), s + 1 == STAGES ? phase ^ 1 : phase);
                 fence_after();
                 if (leader) {
-                    multiply_stage<KIND, BN>(tmem + buffer * BN, tmem + 2 * BN + s * P::SCALE_COLS, a0 + s * (A_BYTES / 16), b0 + s * (P::B_BYTES / 16),
+                    multiply_stage<KIND, BN, PAIR>(tmem + buffer * BN, tmem + 2 * BN + s * P::SCALE_COLS, a0 + s * (A_BYTES / 16), b0 + s * (M::B_BYTES / 16),
                                              sa0 + s * (P::SA_BYTES / 16), sb0 + s * (P::SB_BYTES / 16), i != 0, shift);
                     umma_commit_pair(empty0 + 8 * s);
-                    if (i == nkb - 1) umma_commit(filled0 + 8 * buffer);
+                    if (i == nkb - 1) umma_commit_pair(filled0 + 8 * buffer);
                 }
                 if (++i == nkb) { i = 0; tile += step; ++turn; shift = shift_of(tile); }
             }
         }
-    } else {
+    } else if (warp != 1) {
         const int q = warp & 3;
         unsigned char* mine = stores + q * STORE_BYTES;
         asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the kernel ahead
@@ -623,7 +641,7 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
                 if ((c + 1) * STEP >= tokens) {      // all is in registers
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(drained0 + 8 * buffer);
+                    if (lane == 0) arrive_there(at_first(drained0 + 8 * buffer));
                 }
                 const int count = tokens - c * STEP < STEP ? tokens - c * STEP : STEP;
                 if (f0 >= p.n_out) continue;
@@ -638,11 +656,10 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     __syncthreads();
     cluster_arrive();      // the other CTA may still be told that this one is done with a stage, or send to it
     cluster_wait();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Where the scales of a row's first piece stand: the tiles of 80 columns that five pieces a number take have tiles of 128
-// rows of scales of their own; tiles of two pieces a number start where tiles of scales do.
+// Where the scales of a row's first piece stand: the pieces of a tile of tokens have tiles of 128 rows of scales of their own.
 template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(int row, int tokens) {
     return row / tokens * ((tokens * PARTS + 127) / 128 * 128) + row % tokens * PARTS;
 }
@@ -716,6 +733,17 @@ static int make_maps(CUtensorMap* map_w, CUtensorMap* map_x, const void* w, cons
     if (r || x == nullptr) { *map_x = *map_w; return r; }
     return KIND != CODES ? make_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp, (long)KIND * n, kp, 128, box_x)
                          : make_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, kp / 2, n, kp / 2, 128, box_x);
+}
+
+// tiles of 512 bytes of scales, `tiles` for each of `groups` tiles of 128 rows, in boxes of box_tiles by box_groups
+static int make_scale_map(CUtensorMap* map, const void* base, int tiles, int groups, int box_tiles, int box_groups) {
+    EncodeTiled fn = encode_fn();
+    if (fn == nullptr) return IB_ERR_UNSUPPORTED;
+    cuuint64_t dims[3] = {128, (cuuint64_t)tiles, (cuuint64_t)groups}, strides[2] = {512, (cuuint64_t)tiles * 512};
+    cuuint32_t box[3] = {128, (cuuint32_t)box_tiles, (cuuint32_t)box_groups}, step[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? IB_OK : IB_ERR_UNSUPPORTED;
 }
 
 constexpr int SMS = 148, FEW_SMEM = 100 * 1024;      // of a CTA of the kernel for few rows: two share an SM
@@ -805,9 +833,11 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     if (int r = ib_allow_dynamic_smem(done, gemm_kernel<KIND, BN, STAGES>, SMEM)) return r;
     const long tiles = (long)((n + P::TOKENS - 1) / P::TOKENS) * ((m + PAIR * BM - 1) / (PAIR * BM));
     if (tiles > (1 << 30)) return IB_ERR_UNSUPPORTED;
-    CUtensorMap map_w, map_x;
+    CUtensorMap map_w, map_x, map_sw, map_sx;
     if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, BM, BN / PAIR, p)) return r;
-    p.x_groups = KIND == CODES ? (n + 127) / 128 : (n + P::TOKENS - 1) / P::TOKENS * P::B_GROUPS;
+    if (int r = make_scale_map(&map_sw, p.w_scales, p.scale_tiles, (m + BM - 1) / BM, P::K_TILES, 1)) return r;
+    if (int r = make_scale_map(&map_sx, p.x_scales, p.scale_tiles, KIND == CODES ? (n + 127) / 128 : (n + P::TOKENS - 1) / P::TOKENS * P::B_GROUPS, P::K_TILES,
+                               P::B_GROUPS)) return r;
     p.y_wide = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy * (p.y_is_f32 ? 4 : 2) % 16 == 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(PAIR * (tiles < SMS / PAIR ? tiles : SMS / PAIR)));
@@ -824,7 +854,7 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     p.wait_first = !ib_pdl_enabled && !early;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, map_sw, map_sx, p);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
 
@@ -904,7 +934,7 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
         if (n <= 16) return launch_few<CODES, 16, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
         if (n <= 32) return launch_few<CODES, 32, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
         if (n <= 64) return launch_few<CODES, 64, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
-        return launch<CODES, 192, 4>(w, x, n, m, k, p, stream, false);
+        return launch<CODES, 192, 5>(w, x, n, m, k, p, stream, false);
     }
     unsigned char* pieces = (unsigned char*)workspace;
     const int tokens = tile_tokens(x_kind, n);
@@ -912,12 +942,12 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
         p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
         if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, tokens, pieces, stream)) return r;
         if (tokens == 16) return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-        return launch<PIECES_F32, 160, 5>(w, pieces, n, m, k, p, stream, true);
+        return launch<PIECES_F32, 160, 6>(w, pieces, n, m, k, p, stream, true);
     }
     p.x_scales = pieces + pieces_bytes(PIECES_BF16, n, k);
     if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, tokens, pieces, stream)) return r;
     if (tokens == 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
     if (tokens == 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
     if (tokens == 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    return launch<PIECES_BF16, 192, 5>(w, pieces, n, m, k, p, stream, true);
+    return launch<PIECES_BF16, 192, 6>(w, pieces, n, m, k, p, stream, true);
 }
