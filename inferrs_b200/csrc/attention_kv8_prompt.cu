@@ -11,18 +11,20 @@
 //       and store them in the swizzled form that the products read.  An e4m3 number's bits, moved seven to the left with the sign in its
 //       place, are the f16 number 2^-8 times as large, its small ones included: four integer instructions for two numbers, where the
 //       conversion instruction would compete with the exponentials (both run at a quarter of the other units' rate or less).
-//       The 2^8 go into the factors of the scores and of the result.
 //   queries           a row is multiplied by the power of two that brings its largest number to 2^13 .. 2^14, as in attention_kv8.cu.
-//   scores            s = S * key scale * factor of the row.
-//   softmax           the reference R of a row is one for y = s + log2(value scale), P = 2^(y - R): weights of values of very different
-//       scales keep their precision in f16.  The sum takes P / value scale in float32, so there is one exponential a
-//       score, where all value scales of a tile of keys are 0 (their y counts as s - 80) or in 2^-80 .. 2^16; in other tiles it is
-//       2^(s - R), an exponential of its own.
-// Both products take 2,048 cycles of the tensor pipe a tile of keys, the exponentials as many of theirs; a tile takes 7,500 (3.9 us): a
-// softmax warp's own instruction stream, one warp of either tile of rows on each of the SM's four schedulers, 0.4 instructions a cycle
-// (without the scales 6,000, without the conversions 7,000, without the exponentials 7,000).  A prompt of 2,048 tokens, 32 heads on 8: 84 us,
-// 410 TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
+//   scores            s = S * key scale * factor of the row (positive: a negative scale turns the query).
+//   value scales      of 32 keys with scales within 2^-11 of one another (or 0) go into the values: V' = code * scale * 2^(7 - e), e the power
+//       of two above the largest of them, P = 2^(s + e - R), and the sum takes P 2^-e.  V' is a normal f16 number, rounded
+//       to 11 bits like P (with the factor's rounding 3 * 2^-12 of a term in all).  Other keys, and pages that are not in the cache, have P =
+//       2^(s + log2(value scale) - R) and a second exponential for the sum: weights of values of very different scales keep
+//       their precision.
+// What bounds it: a tile of keys takes the tensor pipe 2,048 cycles, the exponentials as many of theirs, and PROMPT_CYCLES in all: a softmax
+// warp's own instruction stream, one warp of either tile of rows on each of the SM's four schedulers.  (With the value scales' logarithms and
+// reciprocals from shared memory, 16 bytes for four keys and warp that it hands out at 128 a cycle, 7,500.)  A prompt of 2,048 tokens, 32 heads on 8: PROMPT_US us,
+// PROMPT_RATE TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
 // All waits are bounded and report through this file's error word.
+#include <type_traits>
+
 #include "few_bits.cuh"
 #include "sm100.cuh"
 
@@ -34,15 +36,16 @@ constexpr int D = 128, ROWS = 128, KEYS = 128, SLICE = 16;
 constexpr int CONVERT = 4, FIRST_CONVERT = 8, ISSUER = FIRST_CONVERT + CONVERT, THREADS = 32 * (ISSUER + 1);
 constexpr int HALF_BYTES = 128 * 128, TILE_BYTES = 2 * HALF_BYTES;      // [128][64] f16 numbers, swizzled; a tile of 128 x 128
 constexpr float SLACK = 8.0f, LEAST = -80.0f;                           // see attention_kv8.cu
-constexpr float LARGE_SCALE = 65536.0f;
+constexpr int GROUP = 32;                                               // keys that share a power of two, a converting warp's
 
 // what the softmax needs to know of a tile's keys
 struct Scales {
-    float key[KEYS], log_value[KEYS], inverse[KEYS], value[KEYS];        // log2 of the value scale (-80 for 0, -inf: no such key), 2^-that
-    int apart[CONVERT];                                                  // per converting warp: whether a value scale is out of bounds
+    float key[KEYS], value[KEYS];                    // value -1: no such key
+    float log_power[KEYS / GROUP], inverse[KEYS / GROUP];        // e and 2^-e of 32 keys
+    int apart[KEYS / GROUP];                         // whether their value scales are too far apart for one
 };
 constexpr int SMEM = 6 * TILE_BYTES + 2 * (int)sizeof(Scales) + 20 * 8 + 1024;
-static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+static_assert(CONVERT * GROUP == KEYS && SMEM <= 227 * 1024, "shared memory of an SM");
 
 __device__ int g_error = 0;
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int code) { return mbar_wait_bounded(bar, parity, &g_error, code); }
@@ -97,6 +100,10 @@ __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ unsigned mul_f16(unsigned a, unsigned b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
 }
 // codes in the high bytes of two halves to f16 numbers 2^-8 times as large
 __device__ __forceinline__ unsigned widened(unsigned h) { return (h >> 1 & 0x3F803F80u) | (h & 0x80008000u); }
@@ -175,8 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
             return {((long)page * a.n_kv + kvh) * a.page_size + (j - p * a.page_size), max(lo_min - j, 0), min(pmax - j + 1, SLICE)};
         };
         uint4 k_raw[8], v_raw[8];
-        float k_s = 0.0f, v_s = 0.0f;
-        bool here = false;                                   // whether the lane's key is one
+        float k_s = 0.0f, v_s = 0.0f;                        // of the lane's key; value -1: its page is not in the cache
         auto load = [&](uint4 (&raw)[8], const unsigned char* pages, const Slice (&at)[2]) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
@@ -185,7 +191,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 raw[x] = r >= s.begin && r < s.end ? *reinterpret_cast<const uint4*>(pages + (s.vector + r) * D + 16 * c) : make_uint4(0, 0, 0, 0);
             }
         };
-        auto store = [&](const uint4 (&raw)[8], unsigned char* to) {
+        // (VALUES: times the rows' factors, an f16 number in both halves of the lane that has the row's key)
+        auto store = [&](const uint4 (&raw)[8], unsigned char* to, auto values, unsigned factor) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 const int r = first + 4 * x + row;
@@ -196,45 +203,58 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                     h[2 * e] = widened(__byte_perm(w[e], 0, 0x1404));
                     h[2 * e + 1] = widened(__byte_perm(w[e], 0, 0x3424));
                 }
+                if constexpr (decltype(values)::value) {
+                    const unsigned by = __shfl_sync(0xffffffffu, factor, 4 * x + row);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[e] = mul_f16(h[e], by);
+                }
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
             }
         };
-        auto load_scales = [&](const Slice (&at)[2]) {       // of the lane's key
-            const int r = lane & 15;
+        auto load_scales = [&](const Slice (&at)[2], int i) {
+            const int r = lane & 15, j = (t_begin + i) * KEYS + first + lane;
             const bool second = lane >= SLICE;
             const long vector = second ? at[1].vector : at[0].vector;
-            here = r >= (second ? at[1].begin : at[0].begin) && r < (second ? at[1].end : at[0].end);
+            const bool here = r >= (second ? at[1].begin : at[0].begin) && r < (second ? at[1].end : at[0].end);
             k_s = here ? a.k_scale[vector + r] : 0.0f;
-            v_s = here ? a.v_scale[vector + r] : 0.0f;
+            v_s = here ? a.v_scale[vector + r] : j >= lo_min && j <= pmax ? -1.0f : 0.0f;
         };
         Slice at[2] = {look_up(0, 0), look_up(0, 1)};
         load(k_raw, a.k_pages, at);
         load(v_raw, a.v_pages, at);
-        load_scales(at);
+        load_scales(at, 0);
         at[0] = look_up(1, 0);
         at[1] = look_up(1, 1);
         for (int i = 0; i < n_tiles; ++i) {
             const int s = i & 1;
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
             if (!ok) break;
-            store(k_raw, sk + s * TILE_BYTES);
+            store(k_raw, sk + s * TILE_BYTES, std::false_type(), 0u);
             handed_over(k_full0 + 8 * s);
             load(k_raw, a.k_pages, at);
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
             if (!ok) break;
-            store(v_raw, sv + s * TILE_BYTES);
-            const float log_value = fmaxf(lg2(v_s), LEAST);
-            const bool out_of_bounds = here && v_s != 0.0f && !(v_s >= 8.271806125530277e-25f && v_s <= LARGE_SCALE);
-            scales[s].key[first + lane] = k_s;
-            scales[s].value[first + lane] = v_s;
-            scales[s].log_value[first + lane] = here ? (v_s == v_s ? log_value : v_s) : -INFINITY;
-            scales[s].inverse[first + lane] = ex2(-log_value);
-            const bool any = __any_sync(0xffffffffu, out_of_bounds);
-            if (lane == 0) scales[s].apart[warp - FIRST_CONVERT] = any;
+            {
+                // the largest scale, the smallest but 0, both as bits (beyond every number's: one that is none, or no key)
+                const unsigned bits = __float_as_uint(v_s), most = __reduce_max_sync(0xffffffffu, bits);
+                const unsigned least = __reduce_min_sync(0xffffffffu, bits == 0 ? 0x7F800000u : bits);
+                const bool wide = most >= 0x7E000000u || (most != 0 && least + (11u << 23) < most) || (most != 0 && most < 0x06000000u);
+                const int e = most == 0 || wide ? 0 : (int)(most >> 23) - 126;
+                const float by = wide ? 1.0f : v_s * __uint_as_float((unsigned)(127 - e) << 23);
+                store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by));
+                scales[s].key[first + lane] = k_s;
+                scales[s].value[first + lane] = v_s;
+                if (lane == 0) {
+                    const int g = warp - FIRST_CONVERT;
+                    scales[s].log_power[g] = (float)e;
+                    scales[s].inverse[g] = __uint_as_float((unsigned)(127 - e) << 23);
+                    scales[s].apart[g] = wide;
+                }
+            }
             handed_over(v_full0 + 8 * s);
             load(v_raw, a.v_pages, at);
-            load_scales(at);
+            load_scales(at, i + 1);
             at[0] = look_up(i + 2, 0);
             at[1] = look_up(i + 2, 1);
         }
@@ -312,8 +332,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
             }
             largest = max(largest & 0xFFFF0000u, largest << 16);
             const int e = (int)(largest >> 23), up = largest == 0 ? 0 : 140 - e < 127 ? 140 - e : 127;
-            const float by = __uint_as_float((unsigned)(up + 127) << 23);
+            const float by = copysignf(__uint_as_float((unsigned)(up + 127) << 23), a.scale);
             factor = e == 255 ? __uint_as_float(0x7FC00000u) : 256.0f * (a.scale * 1.4426950408889634f / by);      // a query that is none
+            if (factor == 0.0f) factor = 1.17549435e-38f;      // (a hidden score times it stays one)
             unsigned char* to = sq + t * TILE_BYTES;
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
@@ -335,8 +356,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
-            const int4 far = *reinterpret_cast<const int4*>(of.apart);
-            const bool scales_apart = (far.x | far.y | far.z | far.w) != 0;
 #pragma unroll 1
             for (int h = 0; h < 2 && ok; ++h) {
                 const int in = 64 * h, key0 = (t_begin + i) * KEYS + in;
@@ -344,27 +363,45 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 tmem_ld32_issue(s_addr + in, v[0]);
                 tmem_ld32_issue(s_addr + in + 32, v[1]);
                 tmem_ld_wait();
-                // y = S * key scale * factor + log2 value scale
+                // t = S * key scale; s + e = t * factor + e is what the reference is one for.  Keys with scales far apart: that at once, each
+                // with its own logarithm
+                const bool all = key0 >= lo && key0 + 63 <= pos;
+                const int2 far = *reinterpret_cast<const int2*>(of.apart + 2 * h);
+                const float2 power = *reinterpret_cast<const float2*>(of.log_power + 2 * h);
+                float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 64; j += 4) {
-                    unsigned* x = v[j >> 5] + (j & 31);
-                    const float4 ks = *reinterpret_cast<const float4*>(of.key + in + j), lv = *reinterpret_cast<const float4*>(of.log_value + in + j);
-                    const float2 y0 = apart(fma2(mul2(two(__uint_as_float(x[0]), __uint_as_float(x[1])), two(ks.x, ks.y)), factor2, two(lv.x, lv.y)));
-                    const float2 y1 = apart(fma2(mul2(two(__uint_as_float(x[2]), __uint_as_float(x[3])), two(ks.z, ks.w)), factor2, two(lv.z, lv.w)));
-                    x[0] = __float_as_uint(y0.x); x[1] = __float_as_uint(y0.y); x[2] = __float_as_uint(y1.x); x[3] = __float_as_uint(y1.y);
-                }
-                if (!(key0 >= lo && key0 + 63 <= pos)) {
+                for (int b = 0; b < 2; ++b) {
+                    const bool wide = (b == 0 ? far.x : far.y) != 0;
 #pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (key0 + j < lo || key0 + j > pos) v[j >> 5][j & 31] = 0xff800000u;
-                }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    for (int j = 0; j < 32; j += 4) {
+                        unsigned* x = v[b] + j;
+                        const float4 ks = *reinterpret_cast<const float4*>(of.key + in + 32 * b + j);
+                        const float2 t0 = apart(mul2(two(__uint_as_float(x[0]), __uint_as_float(x[1])), two(ks.x, ks.y)));
+                        const float2 t1 = apart(mul2(two(__uint_as_float(x[2]), __uint_as_float(x[3])), two(ks.z, ks.w)));
+                        x[0] = __float_as_uint(t0.x); x[1] = __float_as_uint(t0.y); x[2] = __float_as_uint(t1.x); x[3] = __float_as_uint(t1.y);
+                    }
+                    if (wide) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    mx4[j & 3] = max3(mx4[j & 3], __uint_as_float(v[0][2 * j]), __uint_as_float(v[0][2 * j + 1]));
-                    mx4[(j + 2) & 3] = max3(mx4[(j + 2) & 3], __uint_as_float(v[1][2 * j]), __uint_as_float(v[1][2 * j + 1]));
+                        for (int j = 0; j < 32; ++j) {
+                            const float value = of.value[in + 32 * b + j];
+                            const float y = __uint_as_float(v[b][j]) * factor + fmaxf(lg2(value), LEAST) + (value - value);      // (none, if that is none)
+                            v[b][j] = __float_as_uint(value < 0.0f ? -INFINITY : y);
+                        }
+                    }
+                    if (!all) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (key0 + 32 * b + j < lo || key0 + 32 * b + j > pos) v[b][j] = 0xff800000u;
+                    }
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        m0 = max3(m0, __uint_as_float(v[b][j]), __uint_as_float(v[b][j + 1]));
+                        m1 = max3(m1, __uint_as_float(v[b][j + 2]), __uint_as_float(v[b][j + 3]));
+                    }
+                    m0 = fmaxf(m0, m1);
+                    mx = fmaxf(mx, wide ? m0 : m0 * factor + (b == 0 ? power.x : power.y));
                 }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 const bool move = mx > ref + SLACK || (ref == -INFINITY && mx > -INFINITY);
                 if ((i | h) != 0 && __any_sync(0xffffffffu, move)) {
                     // O stands still while its rows are scaled: in the first half, for S of this tile is there and all products
@@ -387,46 +424,40 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 }
                 if (move) ref = mx;
                 const float less = ref == -INFINITY ? 0.0f : -ref;
-                const unsigned long long less2 = two(less, less);
-                unsigned long long sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+                const float2 inverse = *reinterpret_cast<const float2*>(of.inverse + 2 * h);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     unsigned w[16];
-                    if (!scales_apart) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 inv = *reinterpret_cast<const float4*>(of.inverse + in + 32 * b + j);
-                            float2 x0 = apart(add2(two(__uint_as_float(v[b][j]), __uint_as_float(v[b][j + 1])), less2));
-                            float2 x1 = apart(add2(two(__uint_as_float(v[b][j + 2]), __uint_as_float(v[b][j + 3])), less2));
-                            x0.x = ex2(x0.x); x0.y = ex2(x0.y); x1.x = ex2(x1.x); x1.y = ex2(x1.y);
-                            sum2[0] = fma2(two(x0.x, x0.y), two(inv.x, inv.y), sum2[0]);
-                            sum2[1] = fma2(two(x1.x, x1.y), two(inv.z, inv.w), sum2[1]);
-                            w[j / 2] = f16_pair(x0.x, x0.y);
-                            w[j / 2 + 1] = f16_pair(x1.x, x1.y);
-                        }
-                    } else {
-                        unsigned again[32];      // S, which P has not reached yet
-                        tmem_ld32_issue(s_addr + in + 32 * b, again);
-                        tmem_ld_wait();
+                    if ((b == 0 ? far.x : far.y) == 0) {
+                        const float add = (b == 0 ? power.x : power.y) + less;
+                        const unsigned long long add_2 = two(add, add);
+                        unsigned long long sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            float e[2], p[2];
+                            float2 x = apart(fma2(two(__uint_as_float(v[b][j]), __uint_as_float(v[b][j + 1])), factor2, add_2));
+                            x.x = ex2(x.x); x.y = ex2(x.y);
+                            sum2[j / 2 & 1] = add2(sum2[j / 2 & 1], two(x.x, x.y));
+                            w[j / 2] = f16_pair(x.x, x.y);
+                        }
+                        const float2 sum = apart(add2(sum2[0], sum2[1]));
+                        l += (sum.x + sum.y) * (b == 0 ? inverse.x : inverse.y);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float p[2];
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                const int key = in + 32 * b + j + x;
+                                const float lv = lg2(of.value[in + 32 * b + j + x]), y = __uint_as_float(v[b][j + x]) + less;
                                 const bool hidden = v[b][j + x] == 0xff800000u;
-                                const float s = __uint_as_float(again[j + x]) * of.key[key] * factor + less;
-                                e[x] = hidden ? 0.0f : ex2(s);
-                                p[x] = hidden ? 0.0f : ex2(s + lg2(of.value[key]));
+                                const float s = y - fmaxf(lv, LEAST);
+                                l += hidden ? 0.0f : ex2(s);
+                                p[x] = hidden ? 0.0f : ex2(s + lv);
                             }
-                            sum2[0] = add2(sum2[0], two(e[0], e[1]));
                             w[j / 2] = f16_pair(p[0], p[1]);
                         }
                     }
                     tmem_st16(s_addr + 32 * h + 16 * b, w);
                 }
-                const float2 sum = apart(add2(sum2[0], sum2[1]));
-                l += sum.x + sum.y;
                 tmem_st_wait();
                 fence_before();
                 __syncwarp();
@@ -437,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
         if (ok && my_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * t, 0, 6));
         if (ok) {
             fence_after();
-            const float inv = l != 0.0f ? 256.0f / l : 0.0f;      // a row that sees no key: zeros
+            const float inv = l != 0.0f ? 0.0078125f / l : 0.0f;      // a row that sees no key: zeros
             __nv_bfloat16* dst = a.out + row * a.out_ld + (long)head * D;
 #pragma unroll 1
             for (int x = 0; x < D; x += 16) {

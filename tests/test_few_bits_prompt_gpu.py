@@ -162,3 +162,11 @@ def test_refusals_of_tiles():
         with pytest.raises(K.KernelError):
             K.paged_attention_kv8(q, pages, table, req, pos, 0.1, None, out, 64, tiles=tiles)
     assert K.kv8_tile_tokens(8, 2, 64, 1 << 20) == 8 and K.kv8_tile_tokens(8, 2, 128, 64) == 8 and K.kv8_tile_tokens(8, 2, 128, 1 << 20) == 64
+
+
+@pytest.mark.parametrize("most", [3, 10, 12, 40])
+def test_value_scales_of_every_size(most):
+    """Scales spread evenly (in their logarithm) over 2^-most .. 1: around what 32 keys may differ by to share a power of two."""
+    def change(pages, table, q):
+        pages.v_scale.mul_(torch.exp2(-most * torch.rand(pages.v_scale.shape, generator=torch.Generator(device="cuda").manual_seed(most), device="cuda")))
+    check((200,), (300,), 8, 2, 16, 0, seed=12, change=change, scale=0.5)
