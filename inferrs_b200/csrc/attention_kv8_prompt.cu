@@ -18,10 +18,11 @@
 //       to 11 bits like P (with the factor's rounding 3 * 2^-12 of a term in all).  Other keys, and pages that are not in the cache, have P =
 //       2^(s + log2(value scale) - R) and a second exponential for the sum: weights of values of very different scales keep
 //       their precision.
-// What bounds it: a tile of keys takes the tensor pipe 2,048 cycles, the exponentials as many of theirs, and PROMPT_CYCLES in all: a softmax
-// warp's own instruction stream, one warp of either tile of rows on each of the SM's four schedulers.  (With the value scales' logarithms and
-// reciprocals from shared memory, 16 bytes for four keys and warp that it hands out at 128 a cycle, 7,500.)  A prompt of 2,048 tokens, 32 heads on 8: PROMPT_US us,
-// PROMPT_RATE TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
+// What bounds it: a tile of keys takes the tensor pipe 2,048 cycles, the exponentials as many of theirs, and 6,500 in all: a softmax warp's own
+// instruction stream, one warp of either tile of rows on each of the SM's four schedulers (without the conversions 6,100, without the key
+// scales and the exponentials too 4,600; more registers for these warps change nothing).  With the value scales' logarithms and reciprocals
+// from shared memory, which hands out 16 bytes to a whole warp in four cycles, it was 7,500.  A prompt of 2,048 tokens, 32 heads on 8: 76 us, 450
+// TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
 // All waits are bounded and report through this file's error word.
 #include <type_traits>
 

@@ -50,7 +50,7 @@ struct Params {
     int scale_tiles;                         // 128-column tiles of scales per 128 rows
     const void* x;                           // rows that are brought to pieces inside: ldx elements apart, k numbers each
     long ldx;
-    int k;
+    int k, wide;                             // wide: rows start on 16 bytes
     int wait_first;                          // the kernel ahead may have written the weights: nothing is read before it is done
 };
 
@@ -217,14 +217,23 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
     if (i >= helpers) return true;
     for (int a = i; half == 0 && a < nkb && a < sh.stages; a += helpers) fetch_scales(a, a);      // before the kernel ahead is done
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    few::Eight<__nv_bfloat16> raw[PASSES];
+    uint4 raw[PASSES];
     const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(2 * half + (lane >> 4)) * p.ldx + 8 * g);
     auto fetch_x = [&](int i) {
         const int c = (kb0 + i) * 128;
 #pragma unroll
         for (int j = 0; j < PASSES; ++j) {
-            const bool in = 4 * j + 2 * half + (lane >> 4) < p.n_tok && i < nkb;
-            raw[j].load(x + (in ? 4L * j * p.ldx + c : 0), in ? p.k - c - 8 * g : 0);
+            raw[j] = make_uint4(0, 0, 0, 0);
+            if (4 * j + 2 * half + (lane >> 4) >= p.n_tok || i >= nkb) continue;
+            const __nv_bfloat16* src = x + 4L * j * p.ldx + c;
+            const int n = p.k - c - 8 * g;
+            if (p.wide && n >= 8) {
+                raw[j] = *reinterpret_cast<const uint4*>(src);
+            } else {
+                unsigned short* to = reinterpret_cast<unsigned short*>(&raw[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (e < n) to[e] = *reinterpret_cast<const unsigned short*>(src + e);
+            }
         }
     };
     if constexpr (INSIDE) fetch_x(i);
@@ -238,7 +247,7 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
                 if (4 * j + 2 * half >= p.n_tok) break;       // columns of no token: whatever the stage holds
-                const unsigned (&w)[4] = raw[j].w;
+                const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
                 unsigned m = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7FFF7FFFu);
@@ -664,10 +673,11 @@ template <int PARTS> __host__ __device__ __forceinline__ int pieces_scale_row(in
     return row / tokens * ((tokens * PARTS + 127) / 128 * 128) + row % tokens * PARTS;
 }
 // Rows as pieces: row PARTS * t + i of `pieces` [PARTS * n, kp] holds piece i of row t, kp = width rounded up to 128.  A
-// warp takes 256 columns of two rows: a lane eight numbers of each, four lanes a block of 32, sixteen a word of four scales.  Memory
-// bounds it where the conversions leave it time: 2,048 x 12,288 bfloat16 numbers, 101 MB, 29 us.
-constexpr int PIECES_ROWS = 2, PIECES_WARPS = 8;
-template <typename T, int PARTS>
+// warp takes 256 columns of one or two rows: a lane eight numbers, four lanes a block of 32, sixteen a word of four scales.  Memory
+// bounds it where the conversions leave it time: 2,048 x 12,288 bfloat16 numbers, 101 MB, 29 us with two rows, 33 with one; where
+// warps of one row do not fill the SMs, one is faster (512 x 4,096 4.6 and 5.3 us, 128 x 4,096 3.0 and 3.4).
+constexpr int PIECES_WARPS = 8;
+template <typename T, int PARTS, int PIECES_ROWS>
 __global__ void __launch_bounds__(32 * PIECES_WARPS) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int tokens,
                                                      uint2* __restrict__ pieces, unsigned* __restrict__ scales) {
     ib_grid_dependency_sync();
@@ -867,9 +877,10 @@ static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((
 
 template <typename T, int PARTS>
 static int make_pieces(const void* x, long ldx, int n, int k, int tokens, unsigned char* pieces, cudaStream_t stream) {
-    const dim3 grid(few::strips(n, k, PIECES_ROWS, PIECES_WARPS));
+    const bool one = (long)n * ((k + 255) / 256) <= SMS * 64;
+    const dim3 grid(few::strips(n, k, one ? 1 : 2, PIECES_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    ib_launch_early(pieces_kernel<T, PARTS>, grid, dim3(32 * PIECES_WARPS), 0, stream, (const T*)x, ldx, n, k, tokens, (uint2*)pieces,
+    ib_launch_early(one ? pieces_kernel<T, PARTS, 1> : pieces_kernel<T, PARTS, 2>, grid, dim3(32 * PIECES_WARPS), 0, stream, (const T*)x, ldx, n, k, tokens, (uint2*)pieces,
                     (unsigned*)(pieces + pieces_bytes(PARTS, n, k)));
     return ib_launch_status();
 }
@@ -927,6 +938,7 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     p.x = x;
     p.ldx = ldx;
     p.k = k;
+    p.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_kind ? 4 : 2) % 16 == 0;
     p.w_scales = (const unsigned char*)w_scales;
     if (x_kind == 0 && n <= INSIDE_ROWS) return launch_few<PIECES_BF16, 16, true>(w, nullptr, n, m, k, p, tile_rows, splits, stream, false);
     if (x_kind == 2) {
