@@ -62,10 +62,14 @@ __device__ __forceinline__ void cluster_wait() {
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void st_remote_f32(unsigned local_addr, unsigned rank, float v) {
-    unsigned remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_addr), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+// where CTA `rank` of the cluster has what stands at `local` here
+__device__ __forceinline__ unsigned at_rank(unsigned local, unsigned rank) {
+    unsigned there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(local), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ void st_remote_f32x4(unsigned there, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 // `bytes` (a multiple of 16) from global to shared memory
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
@@ -111,7 +115,7 @@ __device__ __forceinline__ void umma_scaled(unsigned d, unsigned long long a, un
 
 // the plan of a stage's shared and tensor memory
 template <int KIND, int BN> struct Plan {
-    static constexpr int TOKENS = BN / KIND;                             // of a tile
+    static constexpr int TOKENS = BN / KIND, PART = TOKENS + 4;          // of a tile; of a row of W's part of the sums, with room against bank conflicts
     static constexpr int B_BYTES = BN * 128;
     static constexpr int K_TILES = KIND != CODES ? 1 : 2;                // 128-column tiles of scales a stage
     static constexpr int B_GROUPS = (BN + 127) / 128;                    // 128-row tiles of scales
@@ -166,6 +170,44 @@ __device__ __forceinline__ void two_pieces(unsigned v, unsigned short& first, un
     const __half2 k32 = __float2half2_rn(32.0f);
     const __half2 left = __hmul2(k32, __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&back)));
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(second) : "r"(*reinterpret_cast<const unsigned*>(&left)));
+}
+
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMNS]) {
+#pragma unroll
+    for (int c = 0; c < COLUMNS / 16; ++c)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(r[16 * c]), "=r"(r[16 * c + 1]), "=r"(r[16 * c + 2]), "=r"(r[16 * c + 3]), "=r"(r[16 * c + 4]), "=r"(r[16 * c + 5]),
+                       "=r"(r[16 * c + 6]), "=r"(r[16 * c + 7]), "=r"(r[16 * c + 8]), "=r"(r[16 * c + 9]), "=r"(r[16 * c + 10]), "=r"(r[16 * c + 11]),
+                       "=r"(r[16 * c + 12]), "=r"(r[16 * c + 13]), "=r"(r[16 * c + 14]), "=r"(r[16 * c + 15])
+                     : "r"(from + 16 * c));
+    tmem_ld_wait();
+}
+
+constexpr int STORE_BYTES = 4096;      // a warp's piece of shared memory for results on their way out
+// A warp stores `count` tokens' results of up to 32 rows of W from f0 on, those below `end`, a lane a row: through shared memory, so that
+// a token's results go out in pieces of 16 bytes where y allows it (4,096 x 4,096 and 48 rows: FEW_STORE).
+template <typename T, int COUNT>
+__device__ __forceinline__ void store_rows(const Params& p, unsigned char* mine, const float (&v)[COUNT], int t0, int count, int f0, int end, int lane) {
+    T* rows = reinterpret_cast<T*>(mine);
+    static_assert(COUNT * 32 * sizeof(T) <= STORE_BYTES, "a warp's piece");
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        if constexpr (sizeof(T) == 4) rows[32 * j + lane] = v[j];
+        else rows[32 * j + lane] = __float2bfloat16_rn(v[j]);
+    }
+    __syncwarp();
+    constexpr int LANES = 2 * sizeof(T), PER = 32 / LANES, PIECE = 16 / (int)sizeof(T);      // lanes that a token's results take, tokens at a time
+    T* y = reinterpret_cast<T*>(p.y) + (long)t0 * p.ldy + f0;
+    if (p.y_wide && (end - f0 >= 32 || end % PIECE == 0)) {
+        const int r = lane / LANES, c = lane % LANES * PIECE;
+#pragma unroll
+        for (int j = 0; j < COUNT; j += PER)
+            if (j + r < count && f0 + c < end) *reinterpret_cast<uint4*>(y + (long)(j + r) * p.ldy + c) = *reinterpret_cast<const uint4*>(rows + 32 * (j + r) + c);
+    } else if (f0 + lane < end) {
+        for (int j = 0; j < count; ++j) y[(long)j * p.ldy + lane] = rows[32 * j + lane];
+    }
+    __syncwarp();
 }
 
 // ---- up to 64 rows: what counts is that every SM streams its share of the weights -----------------------------------------------
@@ -292,8 +334,8 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     unsigned char* a_tiles = b_tiles + stages * P::B_BYTES;
     unsigned char* sa_tiles = a_tiles + stages * a_bytes;
     unsigned char* sb_tiles = sa_tiles + stages * P::SA_BYTES;
-    float* recv = reinterpret_cast<float*>(sb_tiles + stages * P::SB_BYTES);     // [rank of the sender][token][rows owned]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(reinterpret_cast<unsigned char*>(recv) + (splits > 1 ? P::TOKENS * sh.tile_rows * 4 : 0));
+    float* recv = reinterpret_cast<float*>(sb_tiles + stages * P::SB_BYTES);     // [rank of the sender][rows owned][TOKENS, and four of room]
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(reinterpret_cast<unsigned char*>(recv) + (splits > 1 ? P::PART * sh.tile_rows * 4 : 0));
     const unsigned full0 = smem_u32(bars), empty0 = smem_u32(bars + stages), accum = smem_u32(bars + 2 * stages);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 2 * stages + 1);
 
@@ -380,25 +422,29 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
         if (ok && g_error == 0 && q * 32 < sh.tile_rows) {
-            constexpr int COLS = KIND == PIECES_F32 ? 80 : 16, STEP = COLS / KIND;     // accumulator columns at a time, their tokens
+            // accumulator columns at a time, their tokens; the stages' shared memory is free (one stage has 4 KB and more for every 32 rows)
+            constexpr int COLS = KIND == PIECES_F32 ? 80 : BN < 32 ? BN : 32, STEP = COLS / KIND;
+            unsigned char* mine = smem + q * STORE_BYTES;
+            const unsigned there = splits > 1 ? at_rank(smem_u32(recv + ((size_t)rank * owned + row % owned) * P::PART), (unsigned)(row / owned % splits)) : 0;
 #pragma unroll 1
             for (int c = 0; c * STEP < tokens; ++c) {
-                float v[COLS / 16][16];
-#pragma unroll
-                for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + ((unsigned)(q * 32) << 16) + COLS * c + 16 * i, v[i]);
+                unsigned r[COLS];
+                tmem_columns<COLS>(tmem + ((unsigned)(q * 32) << 16) + COLS * c, r);
+                float v[STEP];
 #pragma unroll
                 for (int j = 0; j < STEP; ++j) {
-                    float r = 0.0f;
+                    v[j] = 0.0f;
 #pragma unroll
-                    for (int i = KIND - 1; i >= 0; --i) r += v[(KIND * j + i) / 16][(KIND * j + i) % 16];
-                    const int t = c * STEP + j;
-                    if (t >= tokens) break;
-                    if (splits > 1) {
-                        if (row < sh.tile_rows)
-                            st_remote_f32(smem_u32(recv + ((size_t)rank * P::TOKENS + t) * owned + row % owned), (unsigned)(row / owned), r);
-                    } else if (row < rows) {
-                        store(p, t0 + t, row0 + row, r);
-                    }
+                    for (int i = KIND - 1; i >= 0; --i) v[j] += __uint_as_float(r[KIND * j + i]);
+                }
+                if (splits > 1) {
+#pragma unroll
+                    for (int j = 0; j < STEP; j += 4)
+                        if (row < sh.tile_rows && c * STEP + j < tokens) st_remote_f32x4(there + 4 * (c * STEP + j), v[j], v[j + 1], v[j + 2], v[j + 3]);
+                } else {
+                    const int count = tokens - c * STEP < STEP ? tokens - c * STEP : STEP;
+                    if (p.y_is_f32) store_rows<float, STEP>(p, mine, v, t0 + c * STEP, count, row0 + q * 32, row0 + rows, lane);
+                    else store_rows<__nv_bfloat16, STEP>(p, mine, v, t0 + c * STEP, count, row0 + q * 32, row0 + rows, lane);
                 }
             }
         }
@@ -407,12 +453,18 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
         cluster_arrive();
         cluster_wait();                      // every part of the rows that this CTA owns is in its shared memory
         if (warp >= 2 && warp < 6 && g_error == 0) {
-            for (int i = (int)threadIdx.x - 64; i < tokens * owned; i += 128) {
-                const int t = i / owned, r = i % owned, f = (int)rank * owned + r;
+            for (int i = (int)threadIdx.x - 64; i < (tokens + 3) / 4 * owned; i += 128) {
+                const int t = i / owned * 4, r = i % owned, f = (int)rank * owned + r;
                 if (f >= rows) continue;
-                float sum = 0.0f;
-                for (int part = 0; part < splits; ++part) sum += recv[((size_t)part * P::TOKENS + t) * owned + r];
-                store(p, t0 + t, row0 + f, sum);
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int part = 0; part < splits; ++part) {
+                    const float4 v = *reinterpret_cast<const float4*>(recv + ((size_t)part * owned + r) * P::PART + t);
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                }
+                store(p, t0 + t, row0 + f, sum.x);
+                if (t + 1 < tokens) store(p, t0 + t + 1, row0 + f, sum.y);
+                if (t + 2 < tokens) store(p, t0 + t + 2, row0 + f, sum.z);
+                if (t + 3 < tokens) store(p, t0 + t + 3, row0 + f, sum.w);
             }
         }
     }
@@ -421,18 +473,6 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     fence_before();
     __syncthreads();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.tmem_cols));
-}
-
-template <int COLUMNS>
-__device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMNS]) {
-#pragma unroll
-    for (int c = 0; c < COLUMNS / 16; ++c)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                     : "=r"(r[16 * c]), "=r"(r[16 * c + 1]), "=r"(r[16 * c + 2]), "=r"(r[16 * c + 3]), "=r"(r[16 * c + 4]), "=r"(r[16 * c + 5]),
-                       "=r"(r[16 * c + 6]), "=r"(r[16 * c + 7]), "=r"(r[16 * c + 8]), "=r"(r[16 * c + 9]), "=r"(r[16 * c + 10]), "=r"(r[16 * c + 11]),
-                       "=r"(r[16 * c + 12]), "=r"(r[16 * c + 13]), "=r"(r[16 * c + 14]), "=r"(r[16 * c + 15])
-                     : "r"(from + 16 * c));
-    tmem_ld_wait();
 }
 
 // ---- more rows ------------------------------------------------------------------------------------------------------------------
@@ -445,7 +485,7 @@ __device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMN
 // at which the tensor cores run under load, 1.3 to 1.6 GHz: 2,048 x 12,288 x 4,096 (bfloat16 rows) 130 us behind the 29 that bring x to
 // pieces, 3.2 PFLOP/s of 8-bit products (CTAs by themselves, one tile each: 170); 4-bit rows 2,048 x 4,096 x 24,576 72 to 81 us, 5.1 to 5.7
 // PFLOP/s (200).  Four CTAs that share x's tiles have room on 132 SMs and gain nothing.
-constexpr int PAIR = 2, STORE_BYTES = 4096;      // a warp's piece of shared memory for results on their way out
+constexpr int PAIR = 2;
 template <int KIND, int BN, int STAGES> struct Many {
     using P = Plan<KIND, BN>;
     static constexpr int B_BYTES = P::B_BYTES / PAIR;
@@ -457,12 +497,6 @@ template <int KIND, int BN, int STAGES> struct Many {
 __device__ __forceinline__ void umma_commit_pair(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"((unsigned short)3) : "memory");
-}
-// where the first CTA has what stands at `local` here
-__device__ __forceinline__ unsigned at_first(unsigned local) {
-    unsigned there;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(local));
-    return there;
 }
 // (relaxed: what it tells of is in registers; a release would wait for the results on their way to y)
 __device__ __forceinline__ void arrive_there(unsigned bar) {
@@ -476,32 +510,6 @@ __device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap
 __device__ __forceinline__ void tma_load_3d_pair(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-
-// A warp stores `count` tokens' results of its 32 rows of W, a lane a row: through shared memory, so that a token's results go out in
-// pieces of 16 bytes where y allows it.
-template <typename T, int COUNT>
-__device__ __forceinline__ void store_rows(const Params& p, unsigned char* mine, const float (&v)[COUNT], int t0, int count, int f0, int lane, bool wide) {
-    T* rows = reinterpret_cast<T*>(mine);
-    static_assert(COUNT * 32 * sizeof(T) <= STORE_BYTES, "a warp's piece");
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) {
-        if constexpr (sizeof(T) == 4) rows[32 * j + lane] = v[j];
-        else rows[32 * j + lane] = __float2bfloat16_rn(v[j]);
-    }
-    __syncwarp();
-    constexpr int LANES = 2 * sizeof(T), PER = 32 / LANES;      // lanes that a token's results take, tokens at a time
-    T* y = reinterpret_cast<T*>(p.y) + (long)t0 * p.ldy + f0;
-    if (wide) {
-        const int r = lane / LANES, c = lane % LANES;
-#pragma unroll
-        for (int j = 0; j < COUNT; j += PER)
-            if (j + r < count)
-                *reinterpret_cast<uint4*>(y + (long)(j + r) * p.ldy + c * (16 / (int)sizeof(T))) = *reinterpret_cast<const uint4*>(rows + 32 * (j + r) + c * (16 / (int)sizeof(T)));
-    } else if (f0 + lane < p.n_out) {
-        for (int j = 0; j < count; ++j) y[(long)j * p.ldy + lane] = rows[32 * j + lane];
-    }
-    __syncwarp();
 }
 
 template <int KIND, int BN, int STAGES>
@@ -548,7 +556,7 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     if (warp == 0 || warp == 6) {
         const bool leader = elected(), operands = warp == 0;
         constexpr unsigned W_TX = KIND != CODES ? A_BYTES / 2 : A_BYTES;     // what a tile of weights counts on its barrier
-        const unsigned full = at_first(full0);
+        const unsigned full = at_rank(full0, 0);
         int tile = first, tile_f = 0, row_x = 0, group = 0;
         auto enter = [&]() {      // (what lies behind the last rows reads as zeros)
             const int tile_t = tile / pairs_f;
@@ -633,7 +641,6 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
             fence_after();
             const int f0 = (tile % pairs_f * PAIR + rank) * BM + q * 32, t0 = tile / pairs_f * P::TOKENS;
             const int tokens = p.n_tok - t0 < P::TOKENS ? p.n_tok - t0 : P::TOKENS;
-            const bool wide = p.y_wide && f0 + 32 <= p.n_out;
             constexpr int STEP = KIND == PIECES_F32 ? 16 : 32 / KIND, COLUMNS = STEP * KIND;      // tokens and columns at a time
 #pragma unroll 1
             for (int c = 0; c * STEP < tokens; ++c) {
@@ -650,12 +657,12 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
                 if ((c + 1) * STEP >= tokens) {      // all is in registers
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive_there(at_first(drained0 + 8 * buffer));
+                    if (lane == 0) arrive_there(at_rank(drained0 + 8 * buffer, 0));
                 }
                 const int count = tokens - c * STEP < STEP ? tokens - c * STEP : STEP;
                 if (f0 >= p.n_out) continue;
-                if (p.y_is_f32) store_rows<float, STEP>(p, mine, v, t0 + c * STEP, count, f0, lane, wide);
-                else store_rows<__nv_bfloat16, STEP>(p, mine, v, t0 + c * STEP, count, f0, lane, wide);
+                if (p.y_is_f32) store_rows<float, STEP>(p, mine, v, t0 + c * STEP, count, f0, p.n_out, lane);
+                else store_rows<__nv_bfloat16, STEP>(p, mine, v, t0 + c * STEP, count, f0, p.n_out, lane);
             }
         }
     }
@@ -783,7 +790,7 @@ static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int
         }
     }
     const int stage = s.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES;
-    s.stages = (FEW_SMEM - 3072 - (s.splits > 1 ? P::TOKENS * s.tile_rows * 4 : 0)) / stage;
+    s.stages = (FEW_SMEM - 3072 - (s.splits > 1 ? P::PART * s.tile_rows * 4 : 0)) / stage;
     const int columns = (256 - BN) / P::SCALE_COLS;
     s.stages = s.stages < columns ? s.stages : columns;
     s.stages = s.stages < 16 ? s.stages : 16;
@@ -804,7 +811,7 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, sh.tile_rows, BN, p)) return r;
     if (sh.splits > 8 || sh.splits > p.num_kb || sh.tile_rows % sh.splits) return IB_ERR_ARGUMENT;
     size_t smem = 1024 + (size_t)sh.stages * (sh.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) +
-                  (sh.splits > 1 ? P::TOKENS * sh.tile_rows * 4 : 0) + 16 * sh.stages + 64;
+                  (sh.splits > 1 ? P::PART * sh.tile_rows * 4 : 0) + 16 * sh.stages + 64;
     // the products read 128 rows of A from where the last stage's tile starts, and no less than 128 rows of B are kept readable
     const size_t a_end = 1024 + (size_t)sh.stages * P::B_BYTES + (size_t)(sh.stages - 1) * sh.tile_rows * 128 + A_BYTES;
     const size_t b_end = 1024 + (size_t)(sh.stages - 1) * P::B_BYTES + 128 * 128;
@@ -848,7 +855,6 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     if (int r = make_scale_map(&map_sw, p.w_scales, p.scale_tiles, (m + BM - 1) / BM, P::K_TILES, 1)) return r;
     if (int r = make_scale_map(&map_sx, p.x_scales, p.scale_tiles, KIND == CODES ? (n + 127) / 128 : (n + P::TOKENS - 1) / P::TOKENS * P::B_GROUPS, P::K_TILES,
                                P::B_GROUPS)) return r;
-    p.y_wide = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy * (p.y_is_f32 ? 4 : 2) % 16 == 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(PAIR * (tiles < SMS / PAIR ? tiles : SMS / PAIR)));
     cfg.blockDim = dim3(THREADS + 32);
@@ -933,6 +939,7 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     p.y = y;
     p.ldy = ldy;
     p.y_is_f32 = y_is_f32;
+    p.y_wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy * (y_is_f32 ? 4 : 2) % 16 == 0;
     p.n_tok = n;
     p.n_out = m;
     p.x = x;
