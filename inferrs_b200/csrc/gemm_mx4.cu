@@ -33,7 +33,7 @@ namespace mx4 {
 using namespace sm100;
 
 constexpr int BM = 128, THREADS = 192, A_BYTES = BM * 128;
-constexpr int INSIDE_ROWS = 8;        // up to so many bfloat16 rows are brought to pieces inside the product
+constexpr int INSIDE_ROWS = 4;        // up to so many bfloat16 rows are brought to pieces inside the product
 // what a kernel's rows are: the number of pieces of a number, CODES for 4-bit rows
 enum { CODES = 1, PIECES_BF16 = 2, PIECES_F32 = 5 };
 
@@ -763,13 +763,14 @@ static int make_scale_map(CUtensorMap* map, const void* base, int tiles, int gro
     return r == CUDA_SUCCESS ? IB_OK : IB_ERR_UNSUPPORTED;
 }
 
-constexpr int SMS = 148, FEW_SMEM = 100 * 1024;      // of a CTA of the kernel for few rows: two share an SM
+constexpr int SMS = 148, FEW_SMEM = 100 * 1024, ALONE_SMEM = 200 * 1024;      // of a CTA of the kernel for few rows: two share an SM, or one has it
 
-// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA takes about 350 cycles
-// a stage whatever its tile's height (the issue of its copies and products) after a start of 4,000, two share an SM, their bytes
-// come at 44 a cycle, and parts cost their meeting, which grows with the rows of x.  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row
-// 32 x 1 10.9, 64 x 2 8.5, 128 x 4 6.9, 128 x 8 8.1; sixteen rows 11.8, 11.2, 9.9, 11.0; 48 rows 15.7, 18.7, 20.0 (128 x 4).
-// 4,096 x 24,576, one row: 88 x 1 13.3, 128 x 1 13.7; 48 rows 22.2, 25.3.
+// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA takes 250 cycles a stage
+// (the issue of its copies and products), what its bytes take at 42 a cycle, or the tensor core's time, after a start of 2,750; two
+// share an SM; its results cost 80 cycles a row of x, and parts their meeting, which grows with the rows of x too.  The numbers are
+// fitted to 4,700 products of 20 kinds (six matrices, 1 to 64 rows, every height and cut): what the rule takes is 3 % slower than the
+// best on average.  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row 128 x 1 9.4, 64 x 2 7.7, 128 x 4 6.2,
+// 128 x 8 6.7; 64 rows 128 x 1 14.9, 64 x 2 12.0, 128 x 4 10.2.  4,096 x 24,576, one row: 88 x 1 12.5, 128 x 1 12.8; 64 rows 19.0, 22.9.
 template <int KIND, int BN>
 static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int splits) {
     using P = Plan<KIND, BN>;
@@ -783,14 +784,17 @@ static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int
             const long columns = (all + sms - 1) / sms * sms / per_part;
             const int rows = lowered((m + columns - 1) / columns);
             const long ctas = (long)(m + rows - 1) / rows * per_part, each = (ctas + sms - 1) / sms, together = each < 2 ? each : 2;
-            const long bytes_cycles = (long)rows * (KIND == CODES ? 136 : 68) / 44 * together, stages = (num_kb + parts - 1) / parts;
-            const long cost = (each + 1) / 2 * (4000 + stages * (bytes_cycles > 350 ? bytes_cycles : 350)) +
-                              (parts == 1 ? 0 : (parts == 2 ? 1000 : parts == 4 ? 2000 : 5500) + 200 * (n < P::TOKENS ? n : P::TOKENS));
+            const long bytes = (long)(rows * (KIND == CODES ? 136 : 68) * together) / 42, products = 5L * BN * together / 2;
+            const long stages = (num_kb + parts - 1) / parts, stage = bytes > products ? bytes : products, x_rows = n < P::TOKENS ? n : P::TOKENS;
+            const long cost = (each + 1) / 2 * (2750 + stages * (stage > 250 ? stage : 250) + (parts == 1 ? 80 * x_rows : 0)) +
+                              (parts == 1 ? 0 : (parts == 2 ? 1000 : parts == 4 ? 1300 : 4350) + 100 * x_rows);
             if (best < 0 || cost < best) { best = cost; s.tile_rows = rows; s.splits = parts; }
         }
     }
     const int stage = s.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES;
-    s.stages = (FEW_SMEM - 3072 - (s.splits > 1 ? P::PART * s.tile_rows * 4 : 0)) / stage;
+    // a CTA by itself on its SM (4,096 x 4,096 and 64 rows, 128 x 4: 10.2 us, 15.2 with as little as where two share it; eight rows 6.3 and 6.9)
+    const int room = (long)(m + s.tile_rows - 1) / s.tile_rows * tiles_t * s.splits <= SMS ? ALONE_SMEM : FEW_SMEM;
+    s.stages = (room - 3072 - (s.splits > 1 ? P::PART * s.tile_rows * 4 : 0)) / stage;
     const int columns = (256 - BN) / P::SCALE_COLS;
     s.stages = s.stages < columns ? s.stages : columns;
     s.stages = s.stages < 16 ? s.stages : 16;

@@ -2547,7 +2547,7 @@ def dequantize_mx4(w: Mx4Matrix, out: torch.Tensor):
                                                           w.rows, w.width)), "dequantize_mx4")
 
 
-MX4_INSIDE_ROWS = 8      # up to so many bfloat16 rows the product needs no workspace (INSIDE_ROWS in csrc/gemm_mx4.cu)
+MX4_INSIDE_ROWS = 4      # up to so many bfloat16 rows the product needs no workspace (INSIDE_ROWS in csrc/gemm_mx4.cu)
 
 
 def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: int = 0):
