@@ -225,6 +225,7 @@ __device__ __forceinline__ void arrive_with_copies(unsigned bar) {
 
 struct Shape {
     int tile_rows, stages, splits, tmem_cols;
+    int x_rows;      // columns of the products that are brought: one tile of tokens alone needs no more than x has (the rest are not stored)
 };
 
 // (INSIDE) A thread takes eight numbers of a row of x, four threads a block of 32, a warp two rows at a time and every other
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
         const unsigned w_tx = KIND == CODES ? a_bytes : a_bytes / 2;     // what a tile of weights counts on its barrier
         auto load_w = [&](int i, int s) {
             if (!leader) return;
-            mbar_expect_tx(full0 + 8 * s, w_tx + (INSIDE ? 0 : P::B_BYTES + P::SB_BYTES));
+            mbar_expect_tx(full0 + 8 * s, w_tx + (INSIDE ? 0 : sh.x_rows * 128 + P::SB_BYTES));
             tma_load_2d_hint(smem_u32(a_tiles) + s * a_bytes, &map_w, (kb0 + i) * 128, row0, full0 + 8 * s, pol);
         };
         auto load_x = [&](int i, int s) {
@@ -775,7 +776,8 @@ template <int KIND, int BN>
 static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int splits) {
     using P = Plan<KIND, BN>;
     auto lowered = [](long rows) { return rows > 128 ? 128 : (int)(rows + 7) / 8 * 8; };
-    Shape s = {tile_rows > 0 ? tile_rows : 128, 1, splits > 0 ? splits : 1, 0};
+    // (rows that x has not, 32 together and more, also cost a copy dearly: float32, 4,096 x 24,576, six rows 28 us, seven 18, both 16 now)
+    Shape s = {tile_rows > 0 ? tile_rows : 128, 1, splits > 0 ? splits : 1, 0, tiles_t > 1 ? BN : (KIND * n + 7) / 8 * 8};
     if (tile_rows == 0 && splits == 0) {
         long best = -1;
         for (int parts = 1; parts <= 8 && (parts == 1 || 2 * parts <= num_kb); parts *= 2) {
@@ -812,7 +814,7 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
     const Shape sh = shape_for<KIND, BN>(n, m, (k + (KIND == CODES ? 255 : 127)) / (KIND == CODES ? 256 : 128), tiles_t, tile_rows, splits);
     CUtensorMap map_w, map_x;
-    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, sh.tile_rows, BN, p)) return r;
+    if (int r = make_maps<KIND>(&map_w, &map_x, w, x, n, m, k, sh.tile_rows, sh.x_rows, p)) return r;
     if (sh.splits > 8 || sh.splits > p.num_kb || sh.tile_rows % sh.splits) return IB_ERR_ARGUMENT;
     size_t smem = 1024 + (size_t)sh.stages * (sh.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES) +
                   (sh.splits > 1 ? P::PART * sh.tile_rows * 4 : 0) + 16 * sh.stages + 64;
