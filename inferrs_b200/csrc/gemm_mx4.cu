@@ -766,30 +766,31 @@ static int make_scale_map(CUtensorMap* map, const void* base, int tiles, int gro
 
 constexpr int SMS = 148, FEW_SMEM = 100 * 1024, ALONE_SMEM = 200 * 1024;      // of a CTA of the kernel for few rows: two share an SM, or one has it
 
-// How the weights of a product of few rows are cut: into tiles of at most 128 rows, and K into parts.  A CTA takes 250 cycles a stage
+// How the weights of a product of few rows are cut: into tiles of at most 128 rows, or K into parts.  A CTA takes 350 cycles a stage
 // (the issue of its copies and products), what its bytes take at 42 a cycle, or the tensor core's time, after a start of 2,750; two
 // share an SM; its results cost 80 cycles a row of x, and parts their meeting, which grows with the rows of x too.  The numbers are
 // fitted to 4,700 products of 20 kinds (six matrices, 1 to 64 rows, every height and cut): what the rule takes is 3 % slower than the
-// best on average.  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row 128 x 1 9.4, 64 x 2 7.7, 128 x 4 6.2,
+// best on average (lowered tiles in parts as well: 3.5 %).  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row 128 x 1 9.4, 64 x 2 7.7, 128 x 4 6.2,
 // 128 x 8 6.7; 64 rows 128 x 1 14.9, 64 x 2 12.0, 128 x 4 10.2.  4,096 x 24,576, one row: 88 x 1 12.5, 128 x 1 12.8; 64 rows 19.0, 22.9.
 template <int KIND, int BN>
 static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int splits) {
     using P = Plan<KIND, BN>;
     auto lowered = [](long rows) { return rows > 128 ? 128 : (int)(rows + 7) / 8 * 8; };
-    // (rows that x has not, 32 together and more, also cost a copy dearly: float32, 4,096 x 24,576, six rows 28 us, seven 18, both 16 now)
+    // (as many as a whole tile: float32, 4,096 x 24,576, six rows 28 us, seven 18; like this 16)
     Shape s = {tile_rows > 0 ? tile_rows : 128, 1, splits > 0 ? splits : 1, 0, tiles_t > 1 ? BN : (KIND * n + 7) / 8 * 8};
     if (tile_rows == 0 && splits == 0) {
         long best = -1;
         for (int parts = 1; parts <= 8 && (parts == 1 || 2 * parts <= num_kb); parts *= 2) {
-            // tiles of 128 rows, lowered until as many rounds of CTAs as they take are full (clusters find room on 128 SMs or so)
-            const long sms = parts > 1 ? 128 : SMS, per_part = (long)tiles_t * parts, all = (long)(m + 127) / 128 * per_part;
+            // alone: tiles of 128 rows, lowered until as many rounds of CTAs as they take are full; clusters of 2, 4 and 8 find room for
+            // 148, 132 and 120 CTAs
+            const long sms = parts == 4 ? 132 : parts == 8 ? 120 : SMS, per_part = (long)tiles_t * parts, all = (long)(m + 127) / 128 * per_part;
             const long columns = (all + sms - 1) / sms * sms / per_part;
-            const int rows = lowered((m + columns - 1) / columns);
+            const int rows = parts > 1 ? 128 : lowered((m + columns - 1) / columns);
             const long ctas = (long)(m + rows - 1) / rows * per_part, each = (ctas + sms - 1) / sms, together = each < 2 ? each : 2;
             const long bytes = (long)(rows * (KIND == CODES ? 136 : 68) * together) / 42, products = 5L * BN * together / 2;
             const long stages = (num_kb + parts - 1) / parts, stage = bytes > products ? bytes : products, x_rows = n < P::TOKENS ? n : P::TOKENS;
-            const long cost = (each + 1) / 2 * (2750 + stages * (stage > 250 ? stage : 250) + (parts == 1 ? 80 * x_rows : 0)) +
-                              (parts == 1 ? 0 : (parts == 2 ? 1000 : parts == 4 ? 1300 : 4350) + 100 * x_rows);
+            const long cost = (each + 1) / 2 * (2750 + stages * (stage > 350 ? stage : 350) + (parts == 1 ? 80 * x_rows : 0)) +
+                              (parts == 1 ? 0 : (parts == 2 ? 1200 : parts == 4 ? 1850 : 5850) + 100 * x_rows);
             if (best < 0 || cost < best) { best = cost; s.tile_rows = rows; s.splits = parts; }
         }
     }
