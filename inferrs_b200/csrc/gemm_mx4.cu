@@ -16,7 +16,7 @@
 // pieces are spread to a byte each on the way), and 512-byte tiles of scales, which the issuing thread copies into tensor
 // memory in front of the products that use them (every stage has its own columns, so none is overwritten early).
 // Accumulators are float32 in tensor memory.  Roles: warp 0 copies (warp 6 the scales, where they are tiles), warp 1 issues
-// products, warps 2..5 read back.  Up to eight bfloat16 rows are brought to pieces inside the product, by warps 6.. of every CTA while
+// products, warps 2..5 read back.  Up to four bfloat16 rows are brought to pieces inside the product, by warps 6.. of every CTA while
 // the weights stream in; more rows by a kernel of their own, and the product starts while that one runs.
 //
 // Up to 64 rows (few_rows_kernel), where low tiles would keep the tensor core longer than the weights take, K is cut over a cluster
@@ -33,7 +33,7 @@ namespace mx4 {
 using namespace sm100;
 
 constexpr int BM = 128, THREADS = 192, A_BYTES = BM * 128;
-constexpr int INSIDE_ROWS = 4;        // up to so many bfloat16 rows are brought to pieces inside the product
+constexpr int INSIDE_ROWS = 4;        // up to so many bfloat16 rows are brought to pieces inside the product (4,096 x 24,576: four rows 13.4 us, eight 16.2 and by themselves 13.3)
 // what a kernel's rows are: the number of pieces of a number, CODES for 4-bit rows
 enum { CODES = 1, PIECES_BF16 = 2, PIECES_F32 = 5 };
 
@@ -228,16 +228,15 @@ struct Shape {
     int x_rows;      // columns of the products that are brought: one tile of tokens alone needs no more than x has (the rest are not stored)
 };
 
-// (INSIDE) A thread takes eight numbers of a row of x, four threads a block of 32, a warp two rows at a time and every other
-// two; what it needs of its next stage is on its way.  The numbers go through f16, which holds a
+// (INSIDE) A thread takes eight numbers of a row of x, four threads a block of 32, a warp two rows; what it needs of its next stage is on
+// its way.  The numbers go through f16, which holds a
 // bfloat16 number's eight bits from 256 down to 2^-17 and below that what the second piece may still need.
 template <int KIND, int BN, bool INSIDE>
 __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, int row0, unsigned char* b_tiles, unsigned char* sa_tiles,
                                             unsigned char* sb_tiles, int kb0, int nkb, unsigned full0, unsigned empty0) {
     using P = Plan<KIND, BN>;
-    constexpr int PASSES = INSIDE ? P::TOKENS / 4 : 1;         // of a warp
     const int which = (int)(threadIdx.x - THREADS) >> 5, half = which >> 2;
-    const int lane = threadIdx.x & 31, g = lane & 15, rows = (p.n_out + 127) / 128 * 128 - row0;      // of scales there are
+    const int lane = threadIdx.x & 31, g = lane & 15, t = 2 * half + (lane >> 4), rows = (p.n_out + 127) / 128 * 128 - row0;      // of scales there are
     const unsigned* scales = reinterpret_cast<const unsigned*>(p.w_scales);
     // a stage's scales are on their way with its weights (the weights' scales come from as far as the weights do)
     auto fetch_scales = [&](int i, int s) {
@@ -260,23 +259,18 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
     if (i >= helpers) return true;
     for (int a = i; half == 0 && a < nkb && a < sh.stages; a += helpers) fetch_scales(a, a);      // before the kernel ahead is done
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    uint4 raw[PASSES];
-    const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)(2 * half + (lane >> 4)) * p.ldx + 8 * g);
+    uint4 raw;
+    const __nv_bfloat16* x = ib_after_wait(reinterpret_cast<const __nv_bfloat16*>(p.x) + (long)t * p.ldx + 8 * g);
     auto fetch_x = [&](int i) {
-        const int c = (kb0 + i) * 128;
+        const int c = (kb0 + i) * 128, n = p.k - c - 8 * g;
+        raw = make_uint4(0, 0, 0, 0);
+        if (t >= p.n_tok || i >= nkb) return;
+        if (p.wide && n >= 8) {
+            raw = *reinterpret_cast<const uint4*>(x + c);
+        } else {
+            unsigned short* to = reinterpret_cast<unsigned short*>(&raw);
 #pragma unroll
-        for (int j = 0; j < PASSES; ++j) {
-            raw[j] = make_uint4(0, 0, 0, 0);
-            if (4 * j + 2 * half + (lane >> 4) >= p.n_tok || i >= nkb) continue;
-            const __nv_bfloat16* src = x + 4L * j * p.ldx + c;
-            const int n = p.k - c - 8 * g;
-            if (p.wide && n >= 8) {
-                raw[j] = *reinterpret_cast<const uint4*>(src);
-            } else {
-                unsigned short* to = reinterpret_cast<unsigned short*>(&raw[j]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) if (e < n) to[e] = *reinterpret_cast<const unsigned short*>(src + e);
-            }
+            for (int e = 0; e < 8; ++e) if (e < n) to[e] = *reinterpret_cast<const unsigned short*>(x + c + e);
         }
     };
     if constexpr (INSIDE) fetch_x(i);
@@ -287,10 +281,8 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
         if (i >= sh.stages && !mbar_wait(empty0 + 8 * s, phase, 4)) return false;
         if (half == 0 && i >= sh.stages) fetch_scales(i, s);
         if constexpr (INSIDE) {
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) {
-                if (4 * j + 2 * half >= p.n_tok) break;       // columns of no token: whatever the stage holds
-                const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+            if (2 * half < p.n_tok) {      // (else columns of no token: whatever the stage holds)
+                const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
                 unsigned m = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7FFF7FFFu);
@@ -303,7 +295,7 @@ __device__ __forceinline__ bool fill_stages(const Params& p, const Shape& sh, in
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     two_pieces(byte == 255u ? 0u : f16_pair(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xFFFF0000u) * by), h[e], l[e]);
-                const int r = 2 * (4 * j + 2 * half + (lane >> 4));
+                const int r = 2 * t;
                 unsigned char* to = b_tiles + s * P::B_BYTES + (g & 1) * 8;
                 *reinterpret_cast<uint2*>(to + r * 128 + ((g >> 1) ^ (r & 7)) * 16) = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
                 *reinterpret_cast<uint2*>(to + (r + 1) * 128 + ((g >> 1) ^ ((r + 1) & 7)) * 16) = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
@@ -881,9 +873,11 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
 
-// tokens of a tile of the product that rows as pieces go through
-static int tile_tokens(int x_kind, int n) {
-    if (x_kind == 1) return n <= 64 ? 16 : 32;
+// Tokens of a tile of the product that rows as pieces go through.  17 to 64 float32 rows are several tiles of 16 that read the weights
+// again, or one or two of 32 on pairs of CTAs, which want many rows of W (us of 32 rows: 4,096 x 24,576 35 and 21, 4,096 x 4,096 10.3 and 11.6,
+// 12,288 x 4,096 17 and 25; 64 rows 45 and 30, 12.7 and 12.8, 26 and 27).
+static int tile_tokens(int x_kind, int n, int m) {
+    if (x_kind == 1) return n <= 16 || (n <= 64 && m <= 8192) ? 16 : 32;
     return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 96;
 }
 static long pieces_bytes(int parts, int n, int k) { return ((long)parts * n * ((k + 127) / 128 * 128) + 511) / 512 * 512; }
@@ -917,7 +911,8 @@ IB_EXPORT int ib_gemm_mx4_error_async(int* out, cudaStream_t stream) {
 // the bytes of workspace that ib_gemm_mx4 wants: pieces, then their scales (from a multiple of 512 on)
 IB_EXPORT long ib_gemm_mx4_workspace(int x_kind, int n, int k) {
     if (x_kind == 2 || (x_kind == 0 && n <= mx4::INSIDE_ROWS)) return 0;
-    const long tokens = mx4::tile_tokens(x_kind, n), parts = x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16;
+    // (tiles of 32 float32 tokens take the more room)
+    const long tokens = mx4::tile_tokens(x_kind, n, 1 << 24), parts = x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16;
     const long scale_rows = (n + tokens - 1) / tokens * ((tokens * parts + 127) / 128 * 128);      // whole tiles of tokens
     return mx4::pieces_bytes(x_kind == 1 ? mx4::PIECES_F32 : mx4::PIECES_BF16, n, k) + scale_rows / 128 * few::scale_tiles(k) * 512;
 }
@@ -963,7 +958,7 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
         return launch<CODES, 192, 5>(w, x, n, m, k, p, stream, false);
     }
     unsigned char* pieces = (unsigned char*)workspace;
-    const int tokens = tile_tokens(x_kind, n);
+    const int tokens = tile_tokens(x_kind, n, m);
     if (x_kind == 1) {
         p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
         if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, tokens, pieces, stream)) return r;
