@@ -28,12 +28,18 @@ struct StoreArgs {
     float eps;
 };
 
+// a number in float32 that rounds to fewer bits as it does: cut off, with the last bit set where something was
+__device__ __forceinline__ float sticky(double v) {
+    const float f = __double2float_rz(v);
+    return (double)f == v ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
 // Heads of 64, 128 or 256 numbers that turn as a whole, element i with i + d / 2, in bfloat16: a lane holds four numbers of the
 // first half of a head and the four they turn with, a warp 256 / D heads at a time and STEPS times, whose loads are all on their way
 // before the first is used; what belongs to the row (its place, its angles) is fetched once.  2,048 rows of 32 + 8 + 8 heads of 128:
-// 47 MB, 51 us with a warp a head through shared memory, 16 us like this.
+// 47 MB, 51 us with a warp a head through shared memory, 17 us like this.
 template <int D, int STEPS, typename WT>
-__global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
+__global__ void __launch_bounds__(32 * STORE_WARPS, 9) kv8_store_whole_kernel(
     const __nv_bfloat16* __restrict__ qkv, const WT* __restrict__ q_weight, const WT* __restrict__ k_weight,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table, const int* __restrict__ positions,
     const int* __restrict__ row_request, const int* __restrict__ block_table, unsigned char* __restrict__ k_pages,
@@ -64,6 +70,9 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
     }
     const int page = req >= 0 && req < a.n_req && pos / a.page_size < a.max_pages ? block_table[(long)req * a.max_pages + pos / a.page_size] : -1;
     const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+    // how far float32 may be off in a key's number times 448 / its largest: 8 last places of 448 (float32 weights: 16)
+    constexpr float OFF = sizeof(WT) == 4 ? 448.0f / 1048576.0f : 448.0f / 2097152.0f;
+    unsigned near = 0;        // the steps in which a key's number that far up has another code than one that far down
 #pragma unroll
     for (int t = 0; t < STEPS; ++t) {
         const int head = head0 + t * HEADS, kind = head < a.n_heads ? 0 : (head < a.n_heads + a.n_kv ? 1 : 2);   // 0 q, 1 k, 2 v
@@ -80,21 +89,24 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
         for (int e = 0; e < 4; ++e) ss += x[0][e] * x[0][e] + x[1][e] * x[1][e];
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        // the norm's factor comes last: it is one for the whole head, so no code depends on it, and a bfloat16 number times a bfloat16 weight
+        // is exact
+        float inv = 1.0f;
         if (kind != 2) {
             if (a.flags >> kind & 1) {
-                const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+                inv = 1.0f / sqrtf(ss / (float)D + a.eps);
                 const WT* w = kind == 0 ? q_weight : k_weight;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    x[0][e] = x[0][e] * inv * (w ? ib_to_float(w[i + e]) : 1.0f);
-                    x[1][e] = x[1][e] * inv * (w ? ib_to_float(w[D / 2 + i + e]) : 1.0f);
+                    x[0][e] *= w ? ib_to_float(w[i + e]) : 1.0f;
+                    x[1][e] *= w ? ib_to_float(w[D / 2 + i + e]) : 1.0f;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {       // products are rounded before they are added up, as everywhere in this file
+            for (int e = 0; e < 4; ++e) {
                 const float first = x[0][e], second = x[1][e];
-                x[0][e] = __fsub_rn(__fmul_rn(first, cs[e]), __fmul_rn(second, sn[e]));
-                x[1][e] = __fadd_rn(__fmul_rn(second, cs[e]), __fmul_rn(first, sn[e]));
+                x[0][e] = fmaf(first, cs[e], -(second * sn[e]));
+                x[1][e] = fmaf(second, cs[e], first * sn[e]);
             }
         }
         unsigned m = 0;
@@ -107,19 +119,56 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_whole_kernel(
             __nv_bfloat16* dst = q_out + ((long)row * a.n_heads + head) * D + i;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[h][0], x[h][1]), hi = __floats2bfloat162_rn(x[h][2], x[h][3]);
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[h][0] * inv, x[h][1] * inv), hi = __floats2bfloat162_rn(x[h][2] * inv, x[h][3] * inv);
                 *reinterpret_cast<uint2*>(dst + h * (D / 2)) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
             }
         } else if (page >= 0 && page < a.n_pages) {       // else a request that stands in to fill a batch
             const long place = ((long)page * a.n_kv + (head - a.n_heads) % a.n_kv) * a.page_size + pos % a.page_size;
-            float by, scale;
-            vector_scale(__uint_as_float(m), by, scale);
             unsigned char* dst = (kind == 1 ? k_pages : v_pages) + place * D + i;
+            float by, scale;
+            vector_scale(__uint_as_float(m) * inv, by, scale);
+            if (by != 0.0f) by = 448.0f / __uint_as_float(m);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 *reinterpret_cast<unsigned*>(dst + h * (D / 2)) = codes8x4(x[h][0] * by, x[h][1] * by, x[h][2] * by, x[h][3] * by);
+            if (kind == 1 && by != 0.0f) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    near |= (unsigned)(codes8x4(fmaf(x[h][0], by, OFF), fmaf(x[h][1], by, OFF), fmaf(x[h][2], by, OFF), fmaf(x[h][3], by, OFF)) !=
+                                       codes8x4(fmaf(x[h][0], by, -OFF), fmaf(x[h][1], by, -OFF), fmaf(x[h][2], by, -OFF), fmaf(x[h][3], by, -OFF))) << t;
+            }
             if (i == 0) (kind == 1 ? k_scale : v_scale)[place] = scale;
         }
+    }
+    // A key's codes are the nearest ones to what the float32 tables turn it to: where float32 leaves that open (one of twenty) the head is
+    // turned and divided once more in 64 bits.  (At the end, where little else is held: 2,048 rows of 32 + 8 + 8 heads of 128 17.4 us, in its
+    // place 18.8, not at all 16.3, all keys in 64 bits 25.)
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) near |= __shfl_xor_sync(0xffffffffu, near, o);
+    const unsigned steps = __reduce_or_sync(0xffffffffu, near);
+#pragma unroll 1
+    for (int t = 0; steps >> t != 0; ++t) {
+        if (!(steps >> t & 1)) continue;
+        const int head = near >> t & 1 ? head0 + t * HEADS : a.n_heads;
+        const __nv_bfloat16* src = qkv + (long)row * a.ldx + (long)head * D + i;
+        const WT* w = a.flags >> 1 & 1 ? k_weight : nullptr;
+        double y[2][4], top = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float first = __bfloat162float(src[e]) * (w ? ib_to_float(w[i + e]) : 1.0f);
+            const float second = __bfloat162float(src[D / 2 + e]) * (w ? ib_to_float(w[D / 2 + i + e]) : 1.0f);
+            y[0][e] = (double)first * cs[e] - (double)second * sn[e];
+            y[1][e] = (double)second * cs[e] + (double)first * sn[e];
+            top = fmax(top, fmax(fabs(y[0][e]), fabs(y[1][e])));
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const double by = 448.0 / top;
+        if (!(near >> t & 1)) continue;
+        unsigned char* dst = k_pages + (((long)page * a.n_kv + head - a.n_heads) * a.page_size + pos % a.page_size) * D + i;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<unsigned*>(dst + h * (D / 2)) = codes8x4(sticky(y[h][0] * by), sticky(y[h][1] * by), sticky(y[h][2] * by), sticky(y[h][3] * by));
     }
 }
 

@@ -543,3 +543,25 @@ def test_rows_that_start_anywhere(pad, offset, dtype):
         K.linear_mx4(x[:rows], m, got)
         K.linear_mx4(x[:rows].contiguous(), m, want)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("d,weights", [(64, "bf16"), (128, "bf16"), (128, "f32"), (256, "bf16")])
+def test_keys_take_the_nearest_codes(d, weights):
+    """Of keys that the kernel for whole heads turns, every code is the one that 64-bit arithmetic gives (a key of zeros beside them stays one)."""
+    from inferrs_b200 import kernels as K
+    n, heads, kv = 700, 3, 5
+    table, n_pages = table_for([n], 16, 1)
+    pages = K.Kv8Pages.zeros(n_pages, kv, 16, d, "cuda")
+    qkv = rand((n, (heads + 2 * kv) * d), 4).bfloat16()
+    qkv[5, heads * d:(heads + 2) * d] = 0
+    q_weight, k_weight = ((1 + 0.1 * rand((d,), s)).to(DT[weights]) for s in (5, 6))
+    angle = rand((n, d // 2), 7) * 3
+    pos, req = torch.arange(n, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    q = torch.empty((n, heads, d), dtype=torch.bfloat16, device="cuda")
+    K.qk_norm_rope_store_kv8(qkv, heads, kv, d, q_weight, k_weight, 1e-6, angle.cos(), angle.sin(), d, pos, req, table, pages, q)
+    want = plain.turned(qkv.double().reshape(n, heads + 2 * kv, d)[:, heads:heads + kv], k_weight, 1e-6, angle.cos(), angle.sin(), d, pos, False)
+    codes, _ = plain.to8(want)
+    got = pages.k.view(torch.uint8)[table[0].long()[(pos // 16).long()], :, (pos % 16).long()].view(torch.float8_e4m3fn).double()
+    wrong = int((got != codes).sum())
+    assert wrong == 0 if weights == "bf16" else wrong < 3      # (float32 weights: a product of 48 bits is rounded to 24)
+    assert bool((got[5, :2] == 0).all())
