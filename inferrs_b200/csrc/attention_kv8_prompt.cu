@@ -125,25 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
     const unsigned o_full0 = smem_u32(bars + 17);     // per tile of rows: O holds every key
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 19);
 
-    ib_grid_dependency_sync();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the last tiles of a prompt see the most keys: they come first, so that the grid's tail is short
-    const int tile = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv), kvh = (int)(blockIdx.x % a.n_kv);
-    const int req = a.tile_req[tile], row0 = a.tile_row0[tile], group = a.n_heads / a.n_kv;
-    const int n_tok = req >= 0 && req < a.n_req ? min(a.tokens, a.q_start[req + 1] - row0) : 0;
-    if (n_tok <= 0 || row0 < 0 || row0 + n_tok > a.n_rows) return;          // a place of the list without a tile
-    const int tpt = ROWS / group;                                            // tokens of a tile of rows
-    const int p0 = a.positions[row0], pmax = a.positions[row0 + n_tok - 1];
-    const int lo_min = ib_first_visible(p0, a.span), t_begin = lo_min / KEYS;
-    const int n_tok_t[2] = {n_tok < tpt ? n_tok : tpt, n_tok > tpt ? n_tok - tpt : 0};
-    int n_tiles_t[2];                                                        // tiles of keys that a tile of rows walks (none without a key)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int last = n_tok_t[t] > 0 ? a.positions[row0 + t * tpt + n_tok_t[t] - 1] : -1;
-        n_tiles_t[t] = last >= lo_min ? last / KEYS + 1 - t_begin : 0;
-    }
-    const int n_tiles = max(n_tiles_t[0], n_tiles_t[1]);
-
     if (threadIdx.x == 0) {
         mbar_init(q_full, 8);
         for (int s = 0; s < 2; ++s) {
@@ -161,6 +143,25 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
     fence_before();
     __syncthreads();
     fence_after();
+    // (not before: a CTA of the next kernel that came first could hold columns that this one waits for, and wait for its end)
+    ib_grid_dependency_sync();
+    // the last tiles of a prompt see the most keys: they come first, so that the grid's tail is short
+    const int tile = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv), kvh = (int)(blockIdx.x % a.n_kv);
+    const int req = a.tile_req[tile], row0 = a.tile_row0[tile], group = a.n_heads / a.n_kv;
+    const int n_tok = req >= 0 && req < a.n_req ? min(a.tokens, a.q_start[req + 1] - row0) : 0;
+    const bool work = n_tok > 0 && row0 >= 0 && row0 + n_tok <= a.n_rows;     // else a place of the list without a tile
+    const int tpt = ROWS / group;                                            // tokens of a tile of rows
+    const int p0 = work ? a.positions[row0] : -1, pmax = work ? a.positions[row0 + n_tok - 1] : -1;
+    const int lo_min = ib_first_visible(p0, a.span), t_begin = lo_min / KEYS;
+    const int n_tok_t[2] = {n_tok < tpt ? n_tok : tpt, n_tok > tpt ? n_tok - tpt : 0};
+    int n_tiles_t[2];                                                        // tiles of keys that a tile of rows walks (none without a key)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = work && n_tok_t[t] > 0 ? a.positions[row0 + t * tpt + n_tok_t[t] - 1] : -1;
+        n_tiles_t[t] = last >= lo_min ? last / KEYS + 1 - t_begin : 0;
+    }
+    const int n_tiles = max(n_tiles_t[0], n_tiles_t[1]);
+
     const unsigned tmem = *tmem_slot;      // columns 128 t: S and P of tile t; 256 + 128 t: O of tile t
     bool ok = true;
     // what was stored in shared memory is seen by the products of whoever hears of it through `bar`
@@ -170,7 +171,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
         if (lane == 0) mbar_arrive(bar);
     };
 
-    if (warp >= FIRST_CONVERT && warp < ISSUER) {
+    if (!work) {
+        // (down to the end, where the tensor memory is given back)
+    } else if (warp >= FIRST_CONVERT && warp < ISSUER) {
         // A warp brings 32 keys of every tile, two slices of 16 that lie in one page each: a lane 16 numbers of a row, four rows at a
         // time.  What no row of the tile sees, and what is not in the cache, is zeros.
         const int first = 32 * (warp - FIRST_CONVERT), row = lane >> 2 & 3, c = (lane & 3) | (lane >> 4) << 2;

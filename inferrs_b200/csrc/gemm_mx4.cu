@@ -186,7 +186,8 @@ __device__ __forceinline__ void tmem_columns(unsigned from, unsigned (&r)[COLUMN
 
 constexpr int STORE_BYTES = 4096;      // a warp's piece of shared memory for results on their way out
 // A warp stores `count` tokens' results of up to 32 rows of W from f0 on, those below `end`, a lane a row: through shared memory, so that
-// a token's results go out in pieces of 16 bytes where y allows it (4,096 x 4,096 and 48 rows: FEW_STORE).
+// a token's results go out in pieces of 16 bytes where y allows it (4,096 x 4,096 and 48 rows: 13.0 us, number by
+// number 15.5).
 template <typename T, int COUNT>
 __device__ __forceinline__ void store_rows(const Params& p, unsigned char* mine, const float (&v)[COUNT], int t0, int count, int f0, int end, int lane) {
     T* rows = reinterpret_cast<T*>(mine);
@@ -336,7 +337,6 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     const int row0 = blockIdx.x * sh.tile_rows, tile_t = blockIdx.y;
     const int kb0 = (int)((long)blockIdx.z * p.num_kb / splits), nkb = (int)((long)(blockIdx.z + 1) * p.num_kb / splits) - kb0;   // >= 1
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, INSIDE ? 35 : 33); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accum, 1);
@@ -348,6 +348,8 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
     }
     fence_before();
     __syncthreads();
+    // (not before: a CTA of the next kernel that came first could hold columns that this one waits for, and wait for its end)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     fence_after();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
@@ -527,7 +529,6 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nkb = p.num_kb;
     const int rank = blockIdx.x & 1, pairs_f = (p.n_out + PAIR * BM - 1) / (PAIR * BM), tiles = pairs_f * ((p.n_tok + P::TOKENS - 1) / P::TOKENS);
     const int first = blockIdx.x / PAIR, step = gridDim.x / PAIR, stages = (tiles - first + step - 1) / step * nkb;      // of this pair
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 2); mbar_init(empty0 + 8 * s, 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(filled0 + 8 * b, 1); mbar_init(drained0 + 8 * b, 4 * PAIR); }
@@ -539,6 +540,8 @@ __global__ void __launch_bounds__(THREADS + 32) gemm_kernel(const __grid_constan
     }
     fence_before();
     __syncthreads();
+    // (not before: a CTA of the next kernel that came first could hold columns that this one waits for, and wait for its end)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cluster_arrive();      // nothing is sent to the other CTA before its barriers stand
     cluster_wait();
     fence_after();
@@ -789,7 +792,7 @@ static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int
     const int stage = s.tile_rows * 128 + P::B_BYTES + P::SA_BYTES + P::SB_BYTES;
     // a CTA by itself on its SM (4,096 x 4,096 and 64 rows, 128 x 4: 10.2 us, 15.2 with as little as where two share it; eight rows 6.3 and 6.9)
     const int room = (long)(m + s.tile_rows - 1) / s.tile_rows * tiles_t * s.splits <= SMS ? ALONE_SMEM : FEW_SMEM;
-    s.stages = (room - 3072 - (s.splits > 1 ? P::PART * s.tile_rows * 4 : 0)) / stage;
+    s.stages = (room - 3 * 1024 - (s.splits > 1 ? P::PART * s.tile_rows * 4 : 0)) / stage;
     const int columns = (256 - BN) / P::SCALE_COLS;
     s.stages = s.stages < columns ? s.stages : columns;
     s.stages = s.stages < 16 ? s.stages : 16;
