@@ -565,3 +565,27 @@ def test_keys_take_the_nearest_codes(d, weights):
     wrong = int((got != codes).sum())
     assert wrong == 0 if weights == "bf16" else wrong < 3      # (float32 weights: a product of 48 bits is rounded to 24)
     assert bool((got[5, :2] == 0).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32", "mx4"])
+@pytest.mark.parametrize("n,k,m", [(2100, 300, 9000), (700, 4100, 8200), (50, 260, 8200), (33, 129, 8300), (64, 2080, 8448), (97, 64, 20000), (4000, 1, 513),
+                                   (193, 768, 256), (200, 2000, 127)])
+def test_products_of_many_tiles(n, k, m, kind):
+    """More tiles than pairs of CTAs, so that pairs take several and accumulators take turns; K of fewer stages than there is room for; a pair's
+    second half, or most of it, behind the last row of W."""
+    from inferrs_b200 import kernels as K
+    x = rand((n, k), 13)
+    w = K.quantize_mx4(0.02 * rand((m, k), 15))
+    dense = torch.empty((m, k), device="cuda")
+    K.dequantize_mx4(w, dense)
+    given = K.quantize_mx4(x) if kind == "mx4" else x.to(DT[kind])
+    x = plain.values4(x)[0].double() if kind == "mx4" else given.double()
+    want = x @ dense.double().t()
+    for out_type, pad in ((torch.bfloat16, 0), (torch.float32, 3)):
+        room = torch.full((n, m + pad), 7.0, device="cuda").to(out_type)
+        out = room[:, :m]
+        K.linear_mx4(given, w, out)
+        limit = product_limit(x, dense.double(), kind, out_type, want)
+        assert bool(((out.double() - want).abs() <= limit).all())
+        assert bool((room[:, m:] == 7).all())
+    assert K.few_bits_faults() == {}
