@@ -420,11 +420,13 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
     if (a.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// How many CTAs share a tile's keys: as many as run at once (four an SM), or twice as many for up to 32 single tokens, whose
-// lengths may differ: then they come longest first.  Clusters of 16 only where one round of them is all there is.
+// How many CTAs share a tile's keys: as many as run at once (four an SM), or twice as many for up to 32 single tokens with contexts that may
+// reach 8,192 keys: then they come longest first, and lengths that differ even out (us of as many and twice as many, 16 requests of
+// 32 heads on 8: all of 2,048 keys 19.1 and 25.7, 100 to 2,048 16.0 and 21.3; all of 8,192 50.8 and 55.6, 100 to 8,192 36.9 and 35.3, to 16,384
+// 65.9 and 53.6; 24 requests of 100 to 8,192 61.3 and 42.1).  Clusters of 16 only where one round of them is all there is.
 static int splits_for(long pairs, int max_len, bool ranked) {
     int s = 1;
-    while (s < 8 && pairs * s * 2 <= (ranked ? 2 : 1) * 148 * 4 && max_len >= 64 * s) s *= 2;
+    while (s < 8 && pairs * s * 2 <= (ranked && max_len >= 8192 ? 2 : 1) * 148 * 4 && max_len >= 64 * s) s *= 2;
     return s == 8 && pairs * 16 <= 148 && max_len >= 64 * 16 ? 16 : s;
 }
 
