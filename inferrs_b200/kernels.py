@@ -2553,8 +2553,9 @@ MX4_INSIDE_ROWS = 4      # up to so many bfloat16 rows the product needs no work
 def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: int = 0):
     """out = x @ w.T.  ``x`` is a tensor [rows, width] (float32 or bfloat16; its rows may lie apart), whose numbers keep
     their precision, or an :class:`Mx4Matrix`; sums are float32.  ``out`` [rows, features] may be float32 or bfloat16 and its
-    rows may lie apart.  Up to 64 rows (float32: any number) the kernel's tiles may be set: ``tile_rows`` rows of w (a multiple
-    of 8 up to 128) and ``splits`` CTAs that share K (1, 2, 4 or 8, a divisor of tile_rows); 0 lets the library choose."""
+    rows may lie apart.  Up to 64 rows (more than 16 of float32: with at most 8,192 rows of w) the kernel's tiles may be set:
+    ``tile_rows`` rows of w (a multiple of 8 up to 128) and ``splits`` CTAs that share K (1, 2, 4 or 8, a divisor of tile_rows); 0
+    lets the library choose.  More rows go through a kernel that takes neither."""
     ldy = _need_rows(out, "out", _BF16_F32)
     coded = isinstance(x, Mx4Matrix)
     ldx = x.width if coded else _need_rows(x, "x", _BF16_F32)
