@@ -14,7 +14,7 @@ namespace few {
 constexpr int QUANT_ROWS = 4, QUANT_WARPS = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width,
+__global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
                                                                     unsigned* __restrict__ codes, unsigned char* __restrict__ scales) {
     ib_grid_dependency_sync();
     const Strip at(width, QUANT_ROWS);
@@ -24,16 +24,14 @@ __global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __r
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
         const bool in = at.row0 + r < rows;
-        v[r].load(x + (long)(in ? at.row0 + r : 0) * ldx + at.column, in ? width - at.column : 0);
+        v[r].load(x + (long)(in ? at.row0 + r : 0) * ldx + at.column, in ? width - at.column : 0, wide != 0);
     }
 #pragma unroll
     for (int r = 0; r < QUANT_ROWS; ++r) {
         const int row = at.row0 + r;
         const unsigned byte = scale_byte(block_largest(v[r].largest()));
         const float by = __uint_as_float((254u - min(byte, 253u)) << 23);
-        unsigned c = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c |= codes2(v[r][2 * j] * by, v[r][2 * j + 1] * by) << (8 * j);
+        const unsigned c = codes4x8(v[r][0] * by, v[r][1] * by, v[r][2] * by, v[r][3] * by, v[r][4] * by, v[r][5] * by, v[r][6] * by, v[r][7] * by);
         if (row >= rows) break;
         if (at.g < pitch) codes[(long)row * pitch + at.g] = byte == 255u ? 0u : c;
         if ((lane & 3) == 0) scales[4 * scale_word(row, at.g >> 4, tiles) + (lane >> 2 & 3)] = (unsigned char)byte;
@@ -87,10 +85,11 @@ IB_EXPORT int ib_quantize_mx4(const IbQuantizeMx4* q) {
     const int x_is_f32 = (int)q->x_is_f32, rows = (int)q->rows, width = (int)q->width;
     if (rows < 0 || width <= 0 || ldx < width) return IB_ERR_ARGUMENT;
     if (rows == 0) return IB_OK;
+    const int wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_is_f32 ? 4 : 2) % 16 == 0;
     const dim3 grid(strips(rows, width, QUANT_ROWS, QUANT_WARPS));
     if (grid.x == 0) return IB_ERR_UNSUPPORTED;
-    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const float*)x, ldx, rows, width, (unsigned*)codes, (unsigned char*)scales);
-    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, (unsigned*)codes, (unsigned char*)scales);
+    if (x_is_f32) ib_launch_early(quantize_kernel<float>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const float*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
+    else ib_launch_early(quantize_kernel<__nv_bfloat16>, grid, dim3(32 * QUANT_WARPS), 0, stream, (const __nv_bfloat16*)x, ldx, rows, width, wide, (unsigned*)codes, (unsigned char*)scales);
     return ib_launch_status();
 }
 

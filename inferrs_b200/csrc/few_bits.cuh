@@ -54,10 +54,12 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
 __device__ __forceinline__ float scale_reciprocal(unsigned byte) {
     return byte == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - byte) << 23);
 }
-// two numbers as codes, nearest with ties to even, beyond 6 as 6; the first in the low half of the byte
-__device__ __forceinline__ unsigned codes2(float first, float second) {
+// eight numbers as codes, nearest with ties to even, beyond 6 as 6; the first in the lowest four bits
+__device__ __forceinline__ unsigned codes4x8(float a, float b, float c, float d, float e, float f, float g, float h) {
     unsigned r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(first), "f"(second));
+    asm("{\n\t.reg .b8 t, u, v, w;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 u, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 v, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 w, %8, %7;\n\tmov.b32 %0, {t, u, v, w};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f), "f"(g), "f"(h));
     return r;
 }
 // the values of two codes, the low half of the byte first
@@ -73,8 +75,8 @@ __device__ __forceinline__ __half2 values4x2(unsigned byte) {
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float v[8];
-    __device__ __forceinline__ void load(const float* p, int n) {
-        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+    __device__ __forceinline__ void load(const float* p, int n, bool wide = false) {
+        const unsigned off = wide ? 0u : (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
         if (n < 8 || (off & 7u)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
@@ -111,8 +113,8 @@ template <> struct Eight<float> {
 };
 template <> struct Eight<__nv_bfloat16> {
     unsigned w[4];      // two numbers each
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
-        const unsigned off = (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int n, bool wide = false) {
+        const unsigned off = wide ? 0u : (unsigned)reinterpret_cast<uintptr_t>(p) & 15u;
         const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
         if (n < 8) {
 #pragma unroll
