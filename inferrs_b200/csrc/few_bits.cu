@@ -9,8 +9,8 @@ namespace few {
 
 // A warp takes 256 columns of four rows: a lane eight numbers of each, four lanes a block of 32.  Memory bounds both kernels: every load of
 // the four rows is on its way before the first is used, and no index is divided by anything but once a block.  A matrix of 24,576 x 4,096
-// (bfloat16) there and back, 508 MB: 171 us a thread and eight
-// numbers at a time, 96 us now (53 there, 43 back; 5.3 TB/s).
+// (bfloat16) there and back, 508 MB: 171 us a thread and eight numbers at a time, 92 us now (5.5 TB/s); from cold caches two rows a
+// warp 64 and 53 us, four 55 and 47, eight 57 and 45.
 constexpr int QUANT_ROWS = 4, QUANT_WARPS = 8;
 
 template <typename T>
