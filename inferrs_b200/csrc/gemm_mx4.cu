@@ -17,7 +17,8 @@
 // memory in front of the products that use them (every stage has its own columns, so none is overwritten early).
 // Accumulators are float32 in tensor memory.  Roles: warp 0 copies (warp 6 the scales, where they are tiles), warp 1 issues
 // products, warps 2..5 read back.  Up to four bfloat16 rows are brought to pieces inside the product, by warps 6.. of every CTA while
-// the weights stream in; more rows by a kernel of their own, and the product starts while that one runs.
+// the weights stream in; more rows by a kernel of their own.  The product starts while that one runs, but reads weights before the kernels
+// ahead have ended only where the library's switch says that none of them writes any.
 //
 // Up to 64 rows (few_rows_kernel), where low tiles would keep the tensor core longer than the weights take, K is cut over a cluster
 // (1, 1, splits): every CTA sends its partial sums to their owners (each has an equal share of the tile's rows) through
@@ -804,7 +805,7 @@ static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int
 }
 
 template <int KIND, int BN, bool INSIDE>
-static int launch_few(const void* w, const void* x, int n, int m, int k, Params p, int tile_rows, int splits, cudaStream_t stream, bool early) {
+static int launch_few(const void* w, const void* x, int n, int m, int k, Params p, int tile_rows, int splits, cudaStream_t stream) {
     using P = Plan<KIND, BN>;
     const int tiles_t = (n + P::TOKENS - 1) / P::TOKENS;
     if (tiles_t > 65535) return IB_ERR_UNSUPPORTED;
@@ -839,13 +840,14 @@ static int launch_few(const void* w, const void* x, int n, int m, int k, Params 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    p.wait_first = !ib_pdl_enabled && !early;      // early: the kernel ahead is pieces_kernel
+    // (also behind pieces_kernel, which writes no weights: it lets this kernel start before it has waited itself, and what is ahead of it may write them)
+    p.wait_first = !ib_pdl_enabled;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<KIND, BN, INSIDE>, map_w, map_x, p, sh);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
 
 template <int KIND, int BN, int STAGES>
-static int launch(const void* w, const void* x, int n, int m, int k, Params p, cudaStream_t stream, bool early) {
+static int launch(const void* w, const void* x, int n, int m, int k, Params p, cudaStream_t stream) {
     using P = Plan<KIND, BN>;
     constexpr int SMEM = Many<KIND, BN, STAGES>::SMEM;
     static IbDeviceSet done;
@@ -871,7 +873,7 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    p.wait_first = !ib_pdl_enabled && !early;
+    p.wait_first = !ib_pdl_enabled;      // as in launch_few
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<KIND, BN, STAGES>, map_w, map_x, map_sw, map_sx, p);
     return e == cudaSuccess ? ib_launch_status() : (int)e;
 }
@@ -952,26 +954,26 @@ IB_EXPORT int ib_gemm_mx4(const IbGemmMx4* c) {
     p.k = k;
     p.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_kind ? 4 : 2) % 16 == 0;
     p.w_scales = (const unsigned char*)w_scales;
-    if (x_kind == 0 && n <= INSIDE_ROWS) return launch_few<PIECES_BF16, 16, true>(w, nullptr, n, m, k, p, tile_rows, splits, stream, false);
+    if (x_kind == 0 && n <= INSIDE_ROWS) return launch_few<PIECES_BF16, 16, true>(w, nullptr, n, m, k, p, tile_rows, splits, stream);
     if (x_kind == 2) {
         p.x_scales = (const unsigned char*)x_scales;
-        if (n <= 16) return launch_few<CODES, 16, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
-        if (n <= 32) return launch_few<CODES, 32, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
-        if (n <= 64) return launch_few<CODES, 64, false>(w, x, n, m, k, p, tile_rows, splits, stream, false);
-        return launch<CODES, 192, 5>(w, x, n, m, k, p, stream, false);
+        if (n <= 16) return launch_few<CODES, 16, false>(w, x, n, m, k, p, tile_rows, splits, stream);
+        if (n <= 32) return launch_few<CODES, 32, false>(w, x, n, m, k, p, tile_rows, splits, stream);
+        if (n <= 64) return launch_few<CODES, 64, false>(w, x, n, m, k, p, tile_rows, splits, stream);
+        return launch<CODES, 192, 5>(w, x, n, m, k, p, stream);
     }
     unsigned char* pieces = (unsigned char*)workspace;
     const int tokens = tile_tokens(x_kind, n, m);
     if (x_kind == 1) {
         p.x_scales = pieces + pieces_bytes(PIECES_F32, n, k);
         if (int r = make_pieces<float, PIECES_F32>(x, ldx, n, k, tokens, pieces, stream)) return r;
-        if (tokens == 16) return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-        return launch<PIECES_F32, 160, 6>(w, pieces, n, m, k, p, stream, true);
+        if (tokens == 16) return launch_few<PIECES_F32, 80, false>(w, pieces, n, m, k, p, tile_rows, splits, stream);
+        return launch<PIECES_F32, 160, 6>(w, pieces, n, m, k, p, stream);
     }
     p.x_scales = pieces + pieces_bytes(PIECES_BF16, n, k);
     if (int r = make_pieces<__nv_bfloat16, PIECES_BF16>(x, ldx, n, k, tokens, pieces, stream)) return r;
-    if (tokens == 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    if (tokens == 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    if (tokens == 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream, true);
-    return launch<PIECES_BF16, 192, 6>(w, pieces, n, m, k, p, stream, true);
+    if (tokens == 16) return launch_few<PIECES_BF16, 32, false>(w, pieces, n, m, k, p, tile_rows, splits, stream);
+    if (tokens == 32) return launch_few<PIECES_BF16, 64, false>(w, pieces, n, m, k, p, tile_rows, splits, stream);
+    if (tokens == 64) return launch_few<PIECES_BF16, 128, false>(w, pieces, n, m, k, p, tile_rows, splits, stream);
+    return launch<PIECES_BF16, 192, 6>(w, pieces, n, m, k, p, stream);
 }
