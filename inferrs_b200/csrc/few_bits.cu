@@ -17,6 +17,7 @@ template <typename T>
 __global__ void __launch_bounds__(32 * QUANT_WARPS) quantize_kernel(const T* __restrict__ x, long ldx, int rows, int width, int wide,
                                                                     unsigned* __restrict__ codes, unsigned char* __restrict__ scales) {
     ib_grid_dependency_sync();
+    x = ib_after_wait(x);
     const Strip at(width, QUANT_ROWS);
     const int lane = threadIdx.x & 31, tiles = scale_tiles(width);
     const long pitch = code_pitch(width) / 4;
@@ -42,6 +43,8 @@ template <typename T>
 __global__ void __launch_bounds__(32 * QUANT_WARPS) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales,
                                                          int rows, int width, T* __restrict__ out, long ldo) {
     ib_grid_dependency_sync();
+    codes = ib_after_wait(codes);
+    scales = ib_after_wait(scales);
     const Strip at(width, QUANT_ROWS);
     const int row0 = at.row0, g = at.g, lane = threadIdx.x & 31, tiles = scale_tiles(width);
     const long pitch = code_pitch(width) / 4;

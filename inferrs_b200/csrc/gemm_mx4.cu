@@ -685,6 +685,7 @@ template <typename T, int PARTS, int PIECES_ROWS>
 __global__ void __launch_bounds__(32 * PIECES_WARPS) pieces_kernel(const T* __restrict__ x, long ldx, int rows, int width, int tokens,
                                                      uint2* __restrict__ pieces, unsigned* __restrict__ scales) {
     ib_grid_dependency_sync();
+    x = ib_after_wait(x);
     const few::Strip at(width, PIECES_ROWS);
     const int row0 = at.row0, g = at.g, per_row = (width + 127) / 128 * 16, tiles = few::scale_tiles(width), lane = threadIdx.x & 31;
     few::Eight<T> raw[PIECES_ROWS];

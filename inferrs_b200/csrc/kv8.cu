@@ -50,12 +50,19 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 9) kv8_store_whole_kernel(
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = 4 * (lane % LANES);
     const int head0 = ((int)blockIdx.y * STORE_WARPS + warp) * HEADS * STEPS + lane / LANES, heads = a.n_heads + 2 * a.n_kv;
     if (a.wait_first) ib_grid_dependency_wait();
+    positions = ib_after_wait(positions);
+    row_request = ib_after_wait(row_request);
+    cos_table = ib_after_wait(cos_table);
+    sin_table = ib_after_wait(sin_table);
     const int pos = positions[row], req = row_request[row];
     const bool fault = pos < 0 || pos >= a.table_rows;
     const float4 c = fault ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(cos_table + (long)pos * (D / 2) + i);
     const float4 s = fault ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(sin_table + (long)pos * (D / 2) + i);
     ib_grid_dependency_wait();
     qkv = ib_after_wait(qkv);
+    q_weight = ib_after_wait(q_weight);
+    k_weight = ib_after_wait(k_weight);
+    block_table = ib_after_wait(block_table);
     if (fault) {
         if (threadIdx.x == 0) atomicCAS(&ib_kv8_row_fault_word, 0, row + 1);
         return;
@@ -188,10 +195,17 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
     float* sh = smem + warp * 2 * d;      // the head as it came, and turned
     float* turned = sh + d;
     if (a.wait_first) ib_grid_dependency_wait();
+    positions = ib_after_wait(positions);
     const int pos = positions[row];
     const bool fault = pos < 0 || (a.rot_dim > 0 && pos >= a.table_rows);
     ib_grid_dependency_wait();
     qkv = ib_after_wait(qkv);
+    q_weight = ib_after_wait(q_weight);
+    k_weight = ib_after_wait(k_weight);
+    block_table = ib_after_wait(block_table);
+    row_request = ib_after_wait(row_request);
+    cos_table = ib_after_wait(cos_table);
+    sin_table = ib_after_wait(sin_table);
     if (fault) {
         if (threadIdx.x == 0) atomicCAS(&ib_kv8_row_fault_word, 0, row + 1);
         return;
@@ -267,6 +281,14 @@ __global__ void __launch_bounds__(32 * SLOW_WARPS) kv8_attention_kernel(
     const int* __restrict__ row_request, const int* __restrict__ positions, T* __restrict__ out, const AttendArgs a) {
     __shared__ float part[SLOW_WARPS][512], part_m[SLOW_WARPS], part_l[SLOW_WARPS];
     ib_grid_dependency_sync();
+    q = ib_after_wait(q);
+    k_pages = ib_after_wait(k_pages);
+    v_pages = ib_after_wait(v_pages);
+    k_scale = ib_after_wait(k_scale);
+    v_scale = ib_after_wait(v_scale);
+    block_table = ib_after_wait(block_table);
+    row_request = ib_after_wait(row_request);
+    positions = ib_after_wait(positions);
     const int row = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.d;
     const int kvh = head / (a.n_heads / a.n_kv), pos = positions[row], req = row_request[row];
     const int lo = ib_first_visible(pos, a.span);

@@ -24,3 +24,21 @@ def test_products_wait_for_whoever_may_write_their_weights():
         for other in (False, True):          # whatever else the rule asks
             said = eval(rule.replace("!", " not ").replace("&&", " and ").replace("||", " or "), {n: n != "ib_pdl_enabled" and other for n in names})
             assert said, rule
+
+
+def test_no_kernel_reads_ahead_of_its_wait_through_a_restricted_pointer():
+    """Loads through a `const __restrict__` parameter may be moved ahead of the wait for the kernels ahead (common.cuh): every kernel of this
+    library, all of which start early, takes such a parameter through ib_after_wait, behind a wait, before it uses it."""
+    seen = 0
+    for name in ("few_bits.cu", "gemm_mx4.cu", "kv8.cu", "attention_kv8.cu", "attention_kv8_prompt.cu"):
+        for kernel in source(name).split("__global__ ")[1:]:
+            head, body = kernel.split(") {\n", 1)
+            body = body.split("\n}\n", 1)[0]
+            code = re.sub(r"//[^\n]*", "", body)
+            waits = [m.start() for m in re.finditer(r"ib_grid_dependency_(sync|wait)\(\)", code)]
+            for pointer in re.findall(r"const \w+\* __restrict__ (\w+)", head):
+                taken = code.find(f"{pointer} = ib_after_wait({pointer});")
+                used = re.search(rf"\b{pointer}\b", code)
+                assert taken >= 0 and used.start() == taken and any(w < taken for w in waits), (name, pointer)
+                seen += 1
+    assert seen >= 20
