@@ -368,7 +368,8 @@ IB_EXPORT int ib_qk_norm_rope_store_kv8(const IbStoreKv8* s) {
     if (n == 0) return IB_OK;
     const StoreArgs a = {ldx, n_heads, n_kv, d, norm_flags, rot_dim, interleaved, table_rows, max_pages, page_size, n_pages, n_req, !ib_pdl_enabled, eps};
     const int heads = n_heads + 2 * n_kv;
-    if (!is_f32 && !interleaved && rot_dim == d && (d == 64 || d == 128 || d == 256) && reinterpret_cast<uintptr_t>(qkv) % 8 == 0 && ldx % 4 == 0 &&
+    if (!is_f32 && !interleaved && rot_dim == d && (d == 64 || d == 128 || d == 256) &&
+        (reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) % 8 == 0 && ldx % 4 == 0 &&
         (reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) % 16 == 0) {
         // few rows: every warp a step of its own; many: three, so that what belongs to a row is fetched less often
         const int steps = (long)n * heads * d < 148L * 64 * 256 ? 1 : 3, per_block = STORE_WARPS * (256 / d) * steps;
