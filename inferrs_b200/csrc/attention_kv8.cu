@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
     if (a.tile_req != nullptr) {
         req = a.tile_req[tile];
         row0 = a.tile_row0[tile];
-        if (req >= 0) n_tok = min(a.tile_tokens, a.q_start[req + 1] - row0);
+        n_tok = req >= 0 && req < a.n_req ? min(a.tile_tokens, a.q_start[req + 1] - row0) : 0;
     } else {
         req = a.row_request[row0];
     }

@@ -2691,7 +2691,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
     one row and head at a time.
     ``tiles`` = (tile_req, tile_row0, n_tiles, q_start, tokens) lets rows of one request share what they read: tile i holds
     up to ``tokens`` (at most :func:`kv8_tile_tokens` of any number of rows) rows of request tile_req[i] (-1: none) from row tile_row0[i] on, and
-    request r's rows end at q_start[r + 1]."""
+    request r's rows end at q_start[r + 1] (a number for every request of the block table, and one)."""
     act = out.dtype
     out_ld = _need_rows(out, "out", _BF16_F32)
     if not (_lists(row_request, positions) and q.dtype is act and q.is_cuda and q.dim() == 3 and q.is_contiguous()
@@ -2716,8 +2716,10 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
             tile_req, tile_row0, n_tiles, q_start, tokens = tiles
             for name, t in (("tile_req", tile_req), ("tile_row0", tile_row0), ("q_start", q_start)):
                 _need(t, name, _I, 1)
-            if min(tile_req.shape[0], tile_row0.shape[0]) < n_tiles or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d, 1 << 30):
-                raise KernelError(f"paged_attention_kv8: {n_tiles} tiles of {tokens} tokens in lists of {tile_req.shape[0]}")
+            if not 0 <= n_tiles <= min(tile_req.shape[0], tile_row0.shape[0]) or q_start.shape[0] <= n_req \
+                    or not 1 <= tokens <= kv8_tile_tokens(nh, nkv, d, 1 << 30):
+                raise KernelError(f"paged_attention_kv8: {n_tiles} tiles of {tokens} tokens in lists of {tile_req.shape[0]}, starts "
+                                  f"of {q_start.shape[0] - 1} of {n_req} requests")
             tile_req, tile_row0, q_start = tile_req.data_ptr(), tile_row0.data_ptr(), q_start.data_ptr()
         code = lib.ib_paged_attention_kv8(_ATTENTION_CALL(
             q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),

@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_few_bits_gpu import rand, table_for
+import plain_few_bits as plain
+from test_few_bits_gpu import attention_limit, filled, rand, table_for
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,33 @@ def test_queries_go_anywhere(d, offset):
     again = torch.empty_like(want)
     store(rows, again)
     assert bool(((again.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("tokens", [8, 64])
+def test_tiles_of_requests_that_are_not_there(tokens):
+    """A list of starts that is too short, or a number of tiles that is none, is refused; a tile of a request beyond the table's is no tile."""
+    from inferrs_b200 import kernels as K
+    pages, table = filled([64, 64], 2, 128, 16, 1)
+    q, out = rand((128, 8, 128), 4).bfloat16(), torch.full((128, 1024), 7.0, dtype=torch.bfloat16, device="cuda")
+    numbers = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    pos, req = torch.arange(64, dtype=torch.int32, device="cuda").repeat(2), torch.arange(2, dtype=torch.int32, device="cuda").repeat_interleave(64)
+    tile_req, tile_row0, starts = numbers(0, 2, 5, -1, 1), numbers(0, 64, 64, 64, 64), numbers(0, 64, 128)
+
+    def call(n_tiles=5, starts=starts):
+        K.paged_attention_kv8(q, pages, table, req, pos, 0.1, None, out, 64, tiles=(tile_req, tile_row0, n_tiles, starts, tokens))
+
+    for bad in (dict(starts=starts[:2]), dict(starts=starts[:0]), dict(n_tiles=6), dict(n_tiles=-1)):
+        with pytest.raises(K.KernelError):
+            call(**bad)
+    codes, scales = [t.double() for t in (pages.k, pages.v)], [t.double() for t in (pages.k_scale, pages.v_scale)]
+    want, weight, size = plain.attention(q, *codes, *scales, table, req, pos, 0.1, 0)
+    limit = attention_limit(want, weight, size, 128, 64, torch.bfloat16)
+
+    def right():                               # of every row
+        return ((out.double().view(128, 8, 128) - want).abs() <= limit).all(-1).all(-1)
+
+    call(4)                                    # the first request's first tile alone
+    assert bool(right()[:tokens].all()) and bool((out[tokens:] == 7).all())
+    call()
+    assert bool(right()[64:64 + tokens].all())
+    assert K.few_bits_faults() == {}
