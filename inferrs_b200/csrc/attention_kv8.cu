@@ -115,10 +115,11 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
     } else {
         req = a.row_request[row0];
     }
-    const bool work = req >= 0 && n_tok > 0 && row0 >= 0 && row0 + n_tok <= a.n_rows;
+    // (a row by itself always has work: zeros where its request is none)
+    const bool work = n_tok > 0 && row0 >= 0 && row0 + n_tok <= a.n_rows;
     const int pos0 = work ? a.positions[row0] : -1, hi = work ? a.positions[row0 + n_tok - 1] : -1;
     const int lo = ib_first_visible(pos0, a.span), last_lo = ib_first_visible(hi, a.span);
-    const bool known = work && req < a.n_req;
+    const bool known = work && req >= 0 && req < a.n_req;
     const int base = lo & ~(KEYS - 1);          // slices start where a page may
     const int slices = known && hi >= lo ? (hi - base) / KEYS + 1 : 0;
     const int s0 = (int)((long)slices * rank / a.splits), s1 = (int)((long)slices * (rank + 1) / a.splits);

@@ -2685,7 +2685,7 @@ def paged_attention_kv8(q: torch.Tensor, pages: Kv8Pages, block_table: torch.Ten
                         tiles=None):
     """out[r, h*d:(h+1)*d] = attention of row r's head h over its request's cached keys in 8 bits up to positions[r].
     ``window``: see :func:`span_argument`.  ``max_kv_len``: no position is beyond it; how the keys are cut goes by it.  A row
-    that sees no key (a negative position, a request without pages) gets zeros.  The rows of ``out`` may lie apart.
+    that sees no key (a negative position, a request without pages or that is none) gets zeros.  The rows of ``out`` may lie apart.
 
     bfloat16 heads of 64, 128 and 256 numbers in pages of a multiple of 16 places run on the tensor cores, the rest in float32
     one row and head at a time.

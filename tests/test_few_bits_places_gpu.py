@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import plain_few_bits as plain
-from test_few_bits_gpu import attention_limit, filled, rand, table_for
+from test_few_bits_gpu import DT, attention_limit, filled, rand, table_for
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,18 @@ def test_tiles_of_requests_that_are_not_there(tokens):
     call()
     assert bool(right()[64:64 + tokens].all())
     assert K.few_bits_faults() == {}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_of_no_request_get_zeros(dtype):
+    """Rows whose request is -1, or beyond the table's, beside rows of requests."""
+    from inferrs_b200 import kernels as K
+    pages, table = filled([300, 64, 5], 2, 128, 16, 1)
+    q = rand((5, 8, 128), 4).to(DT[dtype])
+    pos = torch.tensor([299, 40, 63, 17, 4], dtype=torch.int32, device="cuda")
+    req = torch.tensor([0, -1, 1, 3, 2], dtype=torch.int32, device="cuda")
+    out, real = (torch.full((5, 1024), 7.0, dtype=DT[dtype], device="cuda") for _ in range(2))
+    K.paged_attention_kv8(q, pages, table, req, pos, 0.1, None, out, 300)
+    K.paged_attention_kv8(q, pages, table, req.clamp(0, 2), pos, 0.1, None, real, 300)
+    assert bool((out[[1, 3]] == 0).all())
+    assert torch.equal(out[[0, 2, 4]], real[[0, 2, 4]])
