@@ -230,12 +230,13 @@ __device__ __forceinline__ uint2 take_piece(float (&v)[8]) {
     }
     return c;
 }
-// What a vector with the largest magnitude `a` is multiplied by before its numbers are rounded, and its scale.  A vector
-// whose numbers are all below 2^-100 counts as zeros; one with an infinity or no number reads back as no numbers.
+// What a vector with the largest magnitude `a` is multiplied by before its numbers are rounded, and its scale.  0: its codes are
+// zeros.  A vector whose numbers are all below 2^-100 counts as zeros; one with an infinity or no number has a scale that is no
+// number, and reads back as none (codes that are none would reach, in the attention's products, rows that do not see the vector).
 __device__ __forceinline__ void vector_scale(float a, float& by, float& scale) {
-    const bool some = !(a < 7.888609052210118e-31f);
-    by = some ? 448.0f / a : 0.0f;
-    scale = some ? a / 448.0f : 0.0f;
+    const bool some = a >= 7.888609052210118e-31f, none = !(a <= 3.402823466e38f);
+    by = some && !none ? 448.0f / a : 0.0f;
+    scale = none ? __uint_as_float(0x7FC00000u) : some ? a / 448.0f : 0.0f;
 }
 
 }  // namespace few

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 9) kv8_store_whole_kernel(
             if (by != 0.0f) by = 448.0f / __uint_as_float(m);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<unsigned*>(dst + h * (D / 2)) = codes8x4(x[h][0] * by, x[h][1] * by, x[h][2] * by, x[h][3] * by);
+                *reinterpret_cast<unsigned*>(dst + h * (D / 2)) = by != 0.0f ? codes8x4(x[h][0] * by, x[h][1] * by, x[h][2] * by, x[h][3] * by) : 0u;
             if (kind == 1 && by != 0.0f) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
     vector_scale(__uint_as_float(m), by, scale);
     unsigned char* dst = (kind == 1 ? k_pages : v_pages) + place * d;
     for (int j = 4 * lane; j < d; j += 128)
-        *reinterpret_cast<unsigned*>(dst + j) = codes8x4(out[j] * by, out[j + 1] * by, out[j + 2] * by, out[j + 3] * by);
+        *reinterpret_cast<unsigned*>(dst + j) = by != 0.0f ? codes8x4(out[j] * by, out[j + 1] * by, out[j + 2] * by, out[j + 3] * by) : 0u;
     if (lane == 0) (kind == 1 ? k_scale : v_scale)[place] = scale;
 }
 

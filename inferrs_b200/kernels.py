@@ -2617,7 +2617,7 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
     """:func:`qk_norm_rope_store` for a cache in 8 bits: per-head norm of q and k (where a weight is given), rotation by
     position, q to ``q_out`` in its type, k and v into their pages.  With a the largest magnitude of a head's vector its
     scale is a / 448 and a number is x * (448 / a) rounded to the nearest code, ties to even.  A vector below 2^-100 is
-    stored as zeros; one with an infinity or no number reads back as no numbers.
+    stored as zeros; one with an infinity or no number as zeros with a scale that is no number, so it reads back as none.
 
     qkv [N, at least (n_heads + 2 n_kv_heads) * d] (float32 or bfloat16, columns behind them are not read); block_table
     int32 [R, max_pages].  A row whose position lies outside the rotation tables is left out
