@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 const int e = most == 0 || wide ? 0 : (int)(most >> 23) - 126;
                 const float by = wide ? 1.0f : v_s * __uint_as_float((unsigned)(127 - e) << 23);
                 store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by));
-                scales[s].key[first + lane] = k_s;
+                scales[s].key[first + lane] = fmaf(k_s, 0.0f, k_s);      // an infinite scale is none: a negative score times it would count as hidden
                 scales[s].value[first + lane] = v_s;
                 if (lane == 0) {
                     const int g = warp - FIRST_CONVERT;
