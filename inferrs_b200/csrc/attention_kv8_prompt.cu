@@ -11,6 +11,8 @@
 //       and store them in the swizzled form that the products read.  An e4m3 number's bits, moved seven to the left with the sign in its
 //       place, are the f16 number 2^-8 times as large, its small ones included: four integer instructions for two numbers, where the
 //       conversion instruction would compete with the exponentials (both run at a quarter of the other units' rate or less).
+//       A code that is no number would become 480: the largest magnitude is kept beside (one instruction for four codes, 2 % of the whole), and where
+//       it says that there is one, its vector's key scale becomes no number, so that whoever sees the vector gets none.
 //   queries           a row is multiplied by the power of two that brings its largest number to 2^13 .. 2^14, as in attention_kv8.cu.
 //   scores            s = S * key scale * factor of the row (positive: a negative scale turns the query).
 //   value scales      of 32 keys with scales within 2^-11 of one another (or 0) go into the values: V' = code * scale * 2^(7 - e), e the power
@@ -106,8 +108,11 @@ __device__ __forceinline__ unsigned mul_f16(unsigned a, unsigned b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const unsigned*>(&r);
 }
-// codes in the high bytes of two halves to f16 numbers 2^-8 times as large
-__device__ __forceinline__ unsigned widened(unsigned h) { return (h >> 1 & 0x3F803F80u) | (h & 0x80008000u); }
+// Codes in the high bytes of two halves to f16 numbers 2^-8 times as large: their magnitudes' bits, and the numbers.  A code that is no number
+// becomes 480 * 2^-8, the one magnitude above the largest number's.
+__device__ __forceinline__ unsigned magnitudes(unsigned h) { return h >> 1 & 0x3F803F80u; }
+__device__ __forceinline__ unsigned widened(unsigned h, unsigned m) { return m | (h & 0x80008000u); }
+constexpr unsigned NO_NUMBER = 0x3F80u;
 // where chunk c (eight f16 numbers) of a row stands in a tile
 __device__ __forceinline__ unsigned place(int row, int c) { return (unsigned)((c >> 3) * HALF_BYTES + row * 128 + ((c & 7) ^ (row & 7)) * 16); }
 
@@ -195,8 +200,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 raw[x] = r >= s.begin && r < s.end ? *reinterpret_cast<const uint4*>(pages + (s.vector + r) * D + 16 * c) : make_uint4(0, 0, 0, 0);
             }
         };
-        // (VALUES: times the rows' factors, an f16 number in both halves of the lane that has the row's key)
-        auto store = [&](const uint4 (&raw)[8], unsigned char* to, auto values, unsigned factor) {
+        // (VALUES: times the rows' factors, an f16 number in both halves of the lane that has the row's key.)  Whether some code is no number.
+        auto store = [&](const uint4 (&raw)[8], unsigned char* to, auto values, unsigned factor) -> bool {
+            unsigned largest = 0;
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 const int r = first + 4 * x + row;
@@ -204,8 +210,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 unsigned h[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    h[2 * e] = widened(__byte_perm(w[e], 0, 0x1404));
-                    h[2 * e + 1] = widened(__byte_perm(w[e], 0, 0x3424));
+                    const unsigned a = __byte_perm(w[e], 0, 0x1404), b = __byte_perm(w[e], 0, 0x3424);
+                    const unsigned ma = magnitudes(a), mb = magnitudes(b);
+                    largest = __vimax3_u16x2(largest, ma, mb);
+                    h[2 * e] = widened(a, ma);
+                    h[2 * e + 1] = widened(b, mb);
                 }
                 if constexpr (decltype(values)::value) {
                     const unsigned by = __shfl_sync(0xffffffffu, factor, 4 * x + row);
@@ -215,6 +224,17 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
             }
+            return __any_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16) == NO_NUMBER);
+        };
+        // Whether the vector whose scale the lane has holds such a code (looked at once more: this is rare).
+        auto mine_is_none = [&](const unsigned char* pages, int i) -> bool {
+            const Slice at = look_up(i, lane >> 4);
+            const int r = lane & 15;
+            unsigned found = 0;
+            if (r >= at.begin && r < at.end)
+#pragma unroll 1
+                for (int x = 0; x < D; x += 4) found |= (*reinterpret_cast<const unsigned*>(pages + (at.vector + r) * D + x) & 0x7F7F7F7Fu) + 0x01010101u;
+            return (found & 0x80808080u) != 0;
         };
         auto load_scales = [&](const Slice (&at)[2], int i) {
             const int r = lane & 15, j = (t_begin + i) * KEYS + first + lane;
@@ -234,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
             const int s = i & 1;
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
             if (!ok) break;
-            store(k_raw, sk + s * TILE_BYTES, std::false_type(), 0u);
+            if (store(k_raw, sk + s * TILE_BYTES, std::false_type(), 0u) && mine_is_none(a.k_pages, i)) k_s = __uint_as_float(0x7FC00000u);
             handed_over(k_full0 + 8 * s);
             load(k_raw, a.k_pages, at);
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
@@ -246,7 +266,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 const bool wide = most >= 0x7E000000u || (most != 0 && least + (11u << 23) < most) || (most != 0 && most < 0x06000000u);
                 const int e = most == 0 || wide ? 0 : (int)(most >> 23) - 126;
                 const float by = wide ? 1.0f : v_s * __uint_as_float((unsigned)(127 - e) << 23);
-                store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by));
+                // (a row that sees a value which is none gets none through its score: the values are stored by their scale already)
+                if (store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by)) && mine_is_none(a.v_pages, i))
+                    k_s = __uint_as_float(0x7FC00000u);
                 scales[s].key[first + lane] = fmaf(k_s, 0.0f, k_s);      // an infinite scale is none: a negative score times it would count as hidden
                 scales[s].value[first + lane] = v_s;
                 if (lane == 0) {

@@ -2575,7 +2575,8 @@ def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: i
 @dataclass
 class Kv8Pages:
     """Pages of keys and values in 8 bits: codes [pages, heads, page size, dim] (float8_e4m3fn) and one float32 scale per vector
-    [pages, heads, page size].  A number is its code times its vector's scale."""
+    [pages, heads, page size] (0 or more).  A number is its code times its vector's scale; a key whose scale, or one of whose codes, is
+    not a finite number is none, and so is what sees it (of a value with such a code: that number at least)."""
 
     k: torch.Tensor
     v: torch.Tensor

@@ -99,7 +99,7 @@ def test_attention_over_what_was_stored(dtype, d, form, span):
 
 @pytest.mark.parametrize("span", [0, 9, -16])
 @pytest.mark.parametrize("dtype,d,form", FORMS)
-@pytest.mark.parametrize("what", ["key scale"])
+@pytest.mark.parametrize("what", ["key scale", "key code", "value scale", "value code"])
 def test_attention_over_pages_that_others_have_filled(what, dtype, d, form, span):
     """Infinite scales, and codes that are no numbers beside a scale that is one."""
     from inferrs_b200 import kernels as K
