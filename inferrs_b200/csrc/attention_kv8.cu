@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
                 for (int n = 0; n < NT; ++n) mma_f16(sc[n][w & 1], a0, a1, a2, a3, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
             }
         }
-        const float ks[2] = {scales[g], scales[g + 8]};
+        const float ks[2] = {few::key_scale(scales[g]), few::key_scale(scales[g + 8])};
         const float lv[2] = {lg2(scales[KEYS + g]), lg2(scales[KEYS + g + 8])};
         const float least[2] = {fmaxf(lv[0], LEAST), fmaxf(lv[1], LEAST)};
         float p[NT][4];                         // [2 r + c]: key g + 8 r, column 2t + c

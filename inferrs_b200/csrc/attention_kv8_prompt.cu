@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 // (a row that sees a value which is none gets none through its score: the values are stored by their scale already)
                 if (store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by)) && mine_is_none(a.v_pages, i))
                     k_s = __uint_as_float(0x7FC00000u);
-                scales[s].key[first + lane] = fmaf(k_s, 0.0f, k_s);      // an infinite scale is none: a negative score times it would count as hidden
+                scales[s].key[first + lane] = few::key_scale(k_s);
                 scales[s].value[first + lane] = v_s;
                 if (lane == 0) {
                     const int g = warp - FIRST_CONVERT;

@@ -210,6 +210,9 @@ __device__ __forceinline__ float value8(unsigned char c) {
     const unsigned v = values8x2(c);
     return __low2float(*reinterpret_cast<const __half2*>(&v));
 }
+// A key's scale as the scores meet it: an infinite one is none.  (A sum of products times infinity is + or - infinity where the key's numbers
+// are infinities of both signs and zeros times infinity, and the negative one would count as a key that is not seen.)
+__device__ __forceinline__ float key_scale(float s) { return fmaf(s, 0.0f, s); }
 // Numbers as pieces (see gemm_mx4.cu): the first piece's scale byte of a block from the bits of its largest magnitude (the
 // largest then lies in 128 .. 256; every further piece's byte is five less, down to 0), and eight numbers' next piece, in
 // whose place 32 times what it leaves of them stays.

@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(32 * SLOW_WARPS) kv8_attention_kernel(
             const int j = lane + 32 * i;
             if (j < d) s = fmaf(qv[i], value8(k_pages[place * d + j]), s);
         }
-        s = ib_warp_sum(s) * k_scale[place];
+        s = ib_warp_sum(s) * key_scale(k_scale[place]);
         const float m2 = fmaxf(m, s), fade = m == -INFINITY ? 0.0f : expf(m - m2), p = expf(s - m2);
         const float pv = p * v_scale[place];
         l = l * fade + p;
