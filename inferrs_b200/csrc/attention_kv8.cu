@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         __syncwarp();
-        const unsigned char* at = ring + stage * P::STAGE;
+        unsigned char* at = ring + stage * P::STAGE;
         const float* scales = reinterpret_cast<const float*>(at + 2 * P::SLICE);
         const int j0 = base + s * KEYS;
         const bool there = present >> stage & 1;
@@ -237,14 +237,42 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
             }
         }
         const float ks[2] = {few::key_scale(scales[g]), few::key_scale(scales[g + 8])};
-        const float lv[2] = {lg2(scales[KEYS + g]), lg2(scales[KEYS + g + 8])};
-        const float least[2] = {fmaxf(lv[0], LEAST), fmaxf(lv[1], LEAST)};
+        float lv[2] = {lg2(scales[KEYS + g]), lg2(scales[KEYS + g + 8])};
+        float least[2] = {fmaxf(lv[0], LEAST), fmaxf(lv[1], LEAST)};
         float p[NT][4];                         // [2 r + c]: key g + 8 r, column 2t + c
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) p[n][x] = (sc[n][0][x] + sc[n][1][x]) * (ks[x >> 1] * factor[n][x & 1]);
         if (!all) {
+            if (n_tok > 1) {
+                // Some column does not see some key, and nothing times no number is none all the same: a value with such a code or scale becomes
+                // zeros, and the scores of its key none, for those who see it.  Two lanes look at a key's value.
+                uint4* half = reinterpret_cast<uint4*>(at + P::SLICE);
+                unsigned found = (__float_as_uint(scales[KEYS + (lane >> 1)]) & 0x7F800000u) == 0x7F800000u ? 0x80u : 0u;
+#pragma unroll 1
+                for (int c = 0; c < CHUNKS / 2; ++c) {
+                    const uint4 w = half[chunk_place<D>(lane >> 1, (lane & 1) * (CHUNKS / 2) + c)];
+                    found |= ((w.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w.y & 0x7F7F7F7Fu) + 0x01010101u) |
+                             ((w.z & 0x7F7F7F7Fu) + 0x01010101u) | ((w.w & 0x7F7F7F7Fu) + 0x01010101u);
+                }
+                unsigned none = __ballot_sync(0xffffffffu, (found & 0x80808080u) != 0);
+                if (none) {
+                    none |= (none >> 1 & 0x55555555u) | (none << 1 & 0xAAAAAAAAu);
+#pragma unroll 1
+                    for (int c = 0; c < CHUNKS / 2; ++c)
+                        if (none >> lane & 1) half[chunk_place<D>(lane >> 1, (lane & 1) * (CHUNKS / 2) + c)] = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (none >> (2 * g + 16 * r) & 1) {
+                            lv[r] = -INFINITY;
+                            least[r] = LEAST;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) p[n][2 * r] = p[n][2 * r + 1] = __uint_as_float(0x7FC00000u);
+                        }
+                }
+            }
             unsigned hidden = 0;
 #pragma unroll 1
             for (int x = 0; x < 4 * NT; ++x) {
