@@ -2665,6 +2665,11 @@ def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, hea
 KV8_HEAD_DIMS = (64, 128, 256)   # head sizes that the tensor cores' kernel takes
 
 
+def kv8_tiles_supported(head_dim: int, page_size: int) -> bool:
+    """Whether :func:`paged_attention_kv8` takes tiles of bfloat16 rows over such pages; others go row by row, whatever the tiles."""
+    return head_dim in KV8_HEAD_DIMS and page_size % 16 == 0
+
+
 # From so many CTAs on, tiles of 256 rows are the faster ones (us, 32 heads on 8, tiles of 32 and of 256): 8 CTAs, 64 tokens, 16 and 16 without
 # a context, 42 and 67 behind 2,000 tokens; 16 CTAs, 128 tokens, 32 and 16, 55 and 68, 77 and 120 behind 4,000; 24 CTAs, 192 tokens, 32 and 19, 79
 # and 71, 124 and 121.

@@ -309,7 +309,7 @@ class Attention:
                                         tiles=tiles)
 
         few = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim)
-        if ctx.decode_only or self.rt.dtype != torch.bfloat16:
+        if ctx.decode_only or self.rt.dtype != torch.bfloat16 or not kernels.kv8_tiles_supported(s.head_dim, pages.k.shape[2]):
             attend()
             return
         tokens = kernels.kv8_tile_tokens(s.n_heads, s.n_kv_heads, s.head_dim, ctx.extra.get("dispatch_rows", ctx.n_rows))
