@@ -37,9 +37,9 @@ class Runtime:
 
     device: torch.device
     dtype: torch.dtype
+    shared: Dict[Any, Any] = field(default_factory=dict)  # tables shared by parts with equal descriptions
     weight_bits: Optional[int] = None
     cache_bits: Optional[int] = None
-    shared: Dict[Any, Any] = field(default_factory=dict)  # tables shared by parts with equal descriptions
 
     def __post_init__(self):
         if self.weight_bits not in (None, 4):

@@ -42,3 +42,15 @@ def test_portions_go_in_tiles_and_single_tokens_beside_large_ones_by_themselves(
     assert calls_of_a_step(monkeypatch, 128, 32, [1, 30]) == [("req", "row0", 4, None, 8)]
     assert calls_of_a_step(monkeypatch, 128, 16, [1, 1]) == [None]
     assert calls_of_a_step(monkeypatch, 128, 16, [1, 900], torch.float32) == [None]
+
+
+def test_a_runtime_takes_its_arguments_in_the_order_that_it_had():
+    """The tables that parts share came third before there were options in few bits."""
+    tables = {"a": 1}
+    rt = Runtime(torch.device("cpu"), torch.float32, tables)
+    assert rt.shared is tables and rt.weight_bits is None and rt.cache_bits is None
+    rt = Runtime(torch.device("cpu"), torch.float32, weight_bits=4, cache_bits=8)
+    assert rt.shared == {} and (rt.weight_bits, rt.cache_bits) == (4, 8)
+    for bad in (dict(weight_bits=8), dict(cache_bits=4)):
+        with pytest.raises(ValueError):
+            Runtime(torch.device("cpu"), torch.float32, **bad)
