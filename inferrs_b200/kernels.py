@@ -2480,6 +2480,8 @@ class Mx4Matrix:
         if (codes.shape, scales.shape) != want:
             raise KernelError(f"a 4-bit matrix [{rows}, {width}] has codes and scales of shapes {want}, got "
                               f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.device != scales.device:
+            raise KernelError(f"a 4-bit matrix's codes are on {codes.device}, its scales on {scales.device}")
         self.rows, self.width, self.device = rows, width, codes.device
         self.codes_at, self.scales_at = codes.data_ptr(), scales.data_ptr()
         self._codes, self._scales, self._memory = codes, scales, None
@@ -2490,6 +2492,8 @@ class Mx4Matrix:
     def empty(cls, rows: int, width: int, device) -> "Mx4Matrix":
         if rows < 0 or width <= 0:
             raise KernelError(f"a 4-bit matrix has rows of at least one number, got [{rows}, {width}]")
+        if torch.device(device).type != "cuda":
+            raise KernelError(f"a 4-bit matrix is on a CUDA device (the kernels have no CPU implementation), got {device}")
         of_codes = rows * ((width + 127) // 128 * 64)
         m = cls.__new__(cls)
         m.rows, m.width, m._codes, m._scales = rows, width, None, None
@@ -2530,8 +2534,8 @@ def quantize_mx4(x: torch.Tensor, out: Optional[Mx4Matrix] = None) -> Mx4Matrix:
     rows, width = x.shape
     if out is None:
         out = Mx4Matrix.empty(rows, width, x.device)
-    elif out.rows != rows or out.width != width:
-        raise KernelError(f"quantize_mx4: x {(rows, width)} for a matrix {out.shape}")
+    elif out.rows != rows or out.width != width or out.device != x.device:
+        raise KernelError(f"quantize_mx4: x {(rows, width)} on {x.device} for a matrix {out.shape} on {out.device}")
     _check(_few_bits().ib_quantize_mx4(_QUANTIZE_CALL(x.data_ptr(), out.codes_at, out.scales_at, _stream(), x.dtype is _F32, ld,
                                                       rows, width)), "quantize_mx4")
     return out
@@ -2541,8 +2545,8 @@ def dequantize_mx4(w: Mx4Matrix, out: torch.Tensor):
     """out [rows, width] = the values that ``w`` stands for (float32 or bfloat16; rows may lie apart).  Both types hold them
     exactly, but for bfloat16's limits at the ends of the range."""
     ld = _need_rows(out, "out", _BF16_F32)
-    if out.shape != w.shape:
-        raise KernelError(f"dequantize_mx4: a matrix {w.shape} into {tuple(out.shape)}")
+    if out.shape != w.shape or out.device != w.device:
+        raise KernelError(f"dequantize_mx4: a matrix {w.shape} on {w.device} into {tuple(out.shape)} on {out.device}")
     _check(_few_bits().ib_dequantize_mx4(_DEQUANTIZE_CALL(w.codes_at, w.scales_at, out.data_ptr(), _stream(), out.dtype is _F32, ld,
                                                           w.rows, w.width)), "dequantize_mx4")
 
@@ -2560,12 +2564,13 @@ def linear_mx4(x, w: Mx4Matrix, out: torch.Tensor, tile_rows: int = 0, splits: i
     coded = isinstance(x, Mx4Matrix)
     ldx = x.width if coded else _need_rows(x, "x", _BF16_F32)
     n, k = x.shape
-    if k != w.width or out.shape != (n, w.rows):
-        raise KernelError(f"linear_mx4: x {(n, k)}, w {w.shape}, out {tuple(out.shape)}")
+    device = out.device
+    if k != w.width or out.shape != (n, w.rows) or w.device != device or x.device != device:
+        raise KernelError(f"linear_mx4: x {(n, k)} on {x.device}, w {w.shape} on {w.device}, out {tuple(out.shape)} on {device}")
     kind = 2 if coded else int(x.dtype is _F32)
     lib, workspace, at = _few_bits(), None, 0
     if kind == 1 or (kind == 0 and n > MX4_INSIDE_ROWS):
-        workspace = torch.empty(lib.ib_gemm_mx4_workspace(kind, n, k), dtype=torch.uint8, device=out.device)
+        workspace = torch.empty(lib.ib_gemm_mx4_workspace(kind, n, k), dtype=torch.uint8, device=device)
         at = workspace.data_ptr()
     _check(lib.ib_gemm_mx4(_GEMM_CALL(x.codes_at if coded else x.data_ptr(), x.scales_at if coded else 0, w.codes_at, w.scales_at,
                                       out.data_ptr(), at, _stream(), kind, ldx, n, w.rows, k, out.dtype is _F32, ldy, tile_rows,

@@ -54,3 +54,9 @@ def test_a_runtime_takes_its_arguments_in_the_order_that_it_had():
     for bad in (dict(weight_bits=8), dict(cache_bits=4)):
         with pytest.raises(ValueError):
             Runtime(torch.device("cpu"), torch.float32, **bad)
+
+
+def test_a_matrix_in_four_bits_is_on_a_gpu():
+    for device in ("cpu", torch.device("cpu"), "meta"):
+        with pytest.raises(kernels.KernelError):
+            kernels.Mx4Matrix.empty(4, 64, device)

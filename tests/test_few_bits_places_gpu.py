@@ -87,3 +87,19 @@ def test_rows_of_no_request_get_zeros(dtype):
     K.paged_attention_kv8(q, pages, table, req.clamp(0, 2), pos, 0.1, None, real, 300)
     assert bool((out[[1, 3]] == 0).all())
     assert torch.equal(out[[0, 2, 4]], real[[0, 2, 4]])
+
+
+def test_matrices_and_rows_on_different_devices_are_refused():
+    """Said by the matrix's device alone (nothing is launched)."""
+    from inferrs_b200 import kernels as K
+    x, out = rand((4, 64), 1), torch.empty((4, 4), device="cuda")
+    here, there = K.quantize_mx4(x), K.quantize_mx4(x)
+    there.device = torch.device("cuda", 1)
+    for call in (lambda: K.quantize_mx4(x, there), lambda: K.dequantize_mx4(there, torch.empty_like(x)), lambda: K.linear_mx4(x, there, out),
+                 lambda: K.linear_mx4(there, here, out)):
+        with pytest.raises(K.KernelError):
+            call()
+    K.linear_mx4(x, here, out)
+    K.linear_mx4(here, here, out)
+    K.dequantize_mx4(here, torch.empty_like(x))
+    assert K.quantize_mx4(x, here) is here
