@@ -2610,10 +2610,10 @@ class Kv8Pages:
 
     @classmethod
     def zeros(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device) -> "Kv8Pages":
-        codes = torch.zeros((2, n_pages, n_kv_heads, page_size, head_dim), dtype=torch.uint8, device=device)
-        scales = torch.zeros((2, n_pages, n_kv_heads, page_size), dtype=torch.float32, device=device)
-        codes = codes.view(torch.float8_e4m3fn)
-        return cls(codes[0], codes[1], scales[0], scales[1])
+        shape = (n_pages, n_kv_heads, page_size, head_dim)       # (keys and values each in a piece of memory: both start on 16 bytes)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        scales = torch.zeros((2,) + shape[:3], dtype=torch.float32, device=device)
+        return cls(k, v, scales[0], scales[1])
 
 
 def qk_norm_rope_store_kv8(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, q_weight: Optional[torch.Tensor],

@@ -103,3 +103,18 @@ def test_matrices_and_rows_on_different_devices_are_refused():
     K.linear_mx4(here, here, out)
     K.dequantize_mx4(here, torch.empty_like(x))
     assert K.quantize_mx4(x, here) is here
+
+
+@pytest.mark.parametrize("n_pages,kv,page,d", [(1, 1, 1, 4), (3, 1, 1, 12), (5, 3, 1, 20), (7, 1, 3, 4)])
+def test_pages_of_any_size_and_number(n_pages, kv, page, d):
+    """Keys and values start on 16 bytes whatever the pages before them take; a token in the last place is found again."""
+    from inferrs_b200 import kernels as K
+    pages = K.Kv8Pages.zeros(n_pages, kv, page, d, "cuda")
+    table = torch.arange(n_pages, dtype=torch.int32, device="cuda").view(1, -1)
+    qkv, q = rand((1, 3 * kv * d), 1), torch.empty((1, kv, d), device="cuda")
+    pos, req = torch.tensor([n_pages * page - 1], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.qk_norm_rope_store_kv8(qkv, kv, kv, d, None, None, 0.0, None, None, 0, pos, req, table, pages, q)
+    out = torch.empty((1, kv * d), device="cuda")
+    K.paged_attention_kv8(q, pages, table, req, pos, 1.0, 1, out, n_pages * page)      # a window of one key: its value
+    value = qkv.view(3, kv, d)[2]
+    assert bool(((out.view(kv, d) - value).abs() <= value.abs() * 2.0 ** -4 + value.abs().amax(-1, keepdim=True) * 2.0 ** -17).all())
