@@ -72,6 +72,10 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();      // (the threads of a warp arrive as one)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ unsigned lo8x2(unsigned w) { return few::values8x2((unsigned short)w); }
 __device__ __forceinline__ unsigned hi8x2(unsigned w) { return few::values8x2((unsigned short)(w >> 16)); }
 
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
         }
     }
     if (a.splits > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_barrier();
     } else {
         __syncthreads();
     }
@@ -444,9 +448,8 @@ __global__ void __launch_bounds__(THREADS, D > 128 || NT > 2 ? 2 : NT == 2 ? 3 :
             for (int e = 0; e < 4; ++e) reinterpret_cast<unsigned short*>(dst)[e] = h[e];
         }
     }
-    __syncwarp();
     // no CTA leaves while another may read its shared memory
-    if (a.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (a.splits > 1) cluster_barrier();
 }
 
 // How many CTAs share a tile's keys: as many as run at once (four an SM), or twice as many for up to 32 single tokens with contexts that may

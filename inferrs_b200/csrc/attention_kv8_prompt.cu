@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
 #pragma unroll 1
             for (int x = 0; x < D; x += 16) {
                 float o[16];
+                __syncwarp();      // rows of no token skip the stores
                 if (my_tiles > 0) tmem_ld16(o_addr + x, o);
                 unsigned w[8];
 #pragma unroll

@@ -425,6 +425,7 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
 #pragma unroll 1
             for (int c = 0; c * STEP < tokens; ++c) {
                 unsigned r[COLS];
+                __syncwarp();      // rows beyond the tile's skip the stores
                 tmem_columns<COLS>(tmem + ((unsigned)(q * 32) << 16) + COLS * c, r);
                 float v[STEP];
 #pragma unroll

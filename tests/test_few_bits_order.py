@@ -42,3 +42,15 @@ def test_no_kernel_reads_ahead_of_its_wait_through_a_restricted_pointer():
                 assert taken >= 0 and used.start() == taken and any(w < taken for w in waits), (name, pointer)
                 seen += 1
     assert seen >= 20
+
+
+def test_barriers_of_a_cluster_meet_whole_warps():
+    """The aligned forms ask that a warp's threads arrive as one; behind loops that some of them leave early only __syncwarp says so."""
+    seen = 0
+    for name in ("gemm_mx4.cu", "attention_kv8.cu"):
+        lines = [line for line in source(name).split("\n") if line.strip() and not line.strip().startswith("//")]
+        for i, line in enumerate(lines):
+            if "barrier.cluster.arrive.release.aligned" in line:
+                assert "__syncwarp();" in lines[i - 1] or "__syncwarp();" in line, (name, line)
+                seen += 1
+    assert seen >= 2
