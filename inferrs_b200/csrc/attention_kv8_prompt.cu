@@ -11,8 +11,8 @@
 //       and store them in the swizzled form that the products read.  An e4m3 number's bits, moved seven to the left with the sign in its
 //       place, are the f16 number 2^-8 times as large, its small ones included: four integer instructions for two numbers, where the
 //       conversion instruction would compete with the exponentials (both run at a quarter of the other units' rate or less).
-//       A code that is no number would become 480: the largest magnitude is kept beside (one instruction for four codes, 2 % of the whole), and where
-//       it says that there is one, its vector's key scale becomes no number, so that whoever sees the vector gets none.
+//       A code that is no number would become 480: the largest magnitude is kept beside (one instruction for four codes, 2 to 4 % of the whole), and
+//       where it says that there is one, its vector's key scale becomes no number, so that whoever sees the vector gets none.
 //   queries           a row is multiplied by the power of two that brings its largest number to 2^13 .. 2^14, as in attention_kv8.cu.
 //   scores            s = S * key scale * factor of the row (positive: a negative scale turns the query).
 //   value scales      of 32 keys with scales within 2^-11 of one another (or 0) go into the values: V' = code * scale * 2^(7 - e), e the power
@@ -200,9 +200,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 raw[x] = r >= s.begin && r < s.end ? *reinterpret_cast<const uint4*>(pages + (s.vector + r) * D + 16 * c) : make_uint4(0, 0, 0, 0);
             }
         };
-        // (VALUES: times the rows' factors, an f16 number in both halves of the lane that has the row's key.)  Whether some code is no number.
-        auto store = [&](const uint4 (&raw)[8], unsigned char* to, auto values, unsigned factor) -> bool {
-            unsigned largest = 0;
+        // (VALUES: times the rows' factors, an f16 number in both halves of the lane that has the row's key)
+        unsigned largest = 0;                                // magnitude of the tile's codes so far, the even and the odd ones
+        auto store = [&](const uint4 (&raw)[8], unsigned char* to, auto values, unsigned factor) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 const int r = first + 4 * x + row;
@@ -224,7 +224,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(to + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
             }
-            return __any_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16) == NO_NUMBER);
         };
         // Whether the vector whose scale the lane has holds such a code (looked at once more: this is rare).
         auto mine_is_none = [&](const unsigned char* pages, int i) -> bool {
@@ -254,7 +253,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
             const int s = i & 1;
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
             if (!ok) break;
-            if (store(k_raw, sk + s * TILE_BYTES, std::false_type(), 0u) && mine_is_none(a.k_pages, i)) k_s = __uint_as_float(0x7FC00000u);
+            largest = 0;
+            store(k_raw, sk + s * TILE_BYTES, std::false_type(), 0u);
             handed_over(k_full0 + 8 * s);
             load(k_raw, a.k_pages, at);
             if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty0 + 8 * s, ((i >> 1) - 1) & 1, 1));
@@ -266,8 +266,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const Args a) {
                 const bool wide = most >= 0x7E000000u || (most != 0 && least + (11u << 23) < most) || (most != 0 && most < 0x06000000u);
                 const int e = most == 0 || wide ? 0 : (int)(most >> 23) - 126;
                 const float by = wide ? 1.0f : v_s * __uint_as_float((unsigned)(127 - e) << 23);
+                store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by));
                 // (a row that sees a value which is none gets none through its score: the values are stored by their scale already)
-                if (store(v_raw, sv + s * TILE_BYTES, std::true_type(), f16_pair(32768.0f * by, 32768.0f * by)) && mine_is_none(a.v_pages, i))
+                if (__any_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16) == NO_NUMBER) && (mine_is_none(a.k_pages, i) || mine_is_none(a.v_pages, i)))
                     k_s = __uint_as_float(0x7FC00000u);
                 scales[s].key[first + lane] = few::key_scale(k_s);
                 scales[s].value[first + lane] = v_s;
