@@ -7,7 +7,7 @@
 // bounds it are the warps' own instruction streams, about five cycles an instruction and warp, so sixteen warps share an SM and
 // none does more than it must.  A warp that fills the rings of the others cannot keep up (206 instructions for 32 keys: a thousand
 // cycles), with TMA neither (165 cycles a box of 16 keys): 64 requests of 2,048 keys, 32 heads on 8 of 128 numbers, 82 and 75 us;
-// this form 50, 5.6 TB/s.
+// this form 50, 5.5 TB/s.
 //
 //   scores   S = K Q^T: codes become f16 pairs exactly (mma.sync has no e4m3 products of its own on this machine: it converts
 //            both operands every time, 867 instead of 830 instructions a stage); a query row is multiplied by the power of two that
@@ -19,7 +19,10 @@
 //            holds it (value scales below 2^-80 count as that for the reference).  It moves only when a number has
 //            outgrown it by 2^8 (a vote of the warp says whether any has).
 //   values   O = V^T P^T in f16, which holds the codes exactly: two keys' codes are interleaved byte by byte, P is turned with
-//            movmatrix; sums in float32.
+//            movmatrix; sums in float32.  P is rounded to f16's 11 bits, three more than a bfloat16 result keeps; below 2^-25 of the
+//            reference's weight it is lost (the sum, in float32, counts it).
+//   no numbers  a key whose scale is not finite has no score (a negative sum times infinity would count as hidden).  Where some
+//            column of a tile does not see some key, a value that is none becomes zeros and its key's scores none.
 //
 // Warps join through shared memory, the parts of one tile's keys (up to 16 CTAs, a cluster) through distributed shared
 // memory in the order of the ranks: nothing is left in global memory, and the same call gives the same bits.

@@ -20,11 +20,12 @@
 //       to 11 bits like P (with the factor's rounding 3 * 2^-12 of a term in all).  Other keys, and pages that are not in the cache, have P =
 //       2^(s + log2(value scale) - R) and a second exponential for the sum: weights of values of very different scales keep
 //       their precision.
-// What bounds it: a tile of keys takes the tensor pipe 2,048 cycles, the exponentials as many of theirs, and 6,500 in all: a softmax warp's own
-// instruction stream, one warp of either tile of rows on each of the SM's four schedulers (without the conversions 6,100, without the key
-// scales and the exponentials too 4,600; more registers for these warps change nothing).  With the value scales' logarithms and reciprocals
-// from shared memory, which hands out 16 bytes to a whole warp in four cycles, it was 7,500.  A prompt of 2,048 tokens, 32 heads on 8: 76 us, 450
-// TFLOP/s (attention_kv8.cu's tiles of 32 rows 264 us; bfloat16 pages 49 us).
+// What bounds it: a tile of keys takes the tensor pipe 2,048 cycles, the exponentials as many of theirs, and 6,500 in all (about 6,800 with the
+// question for codes that are no numbers): a softmax warp's own instruction stream, one warp of either tile of rows on each of the SM's
+// four schedulers (without the conversions 6,100, without the key scales and the exponentials too 4,600; more registers for these warps
+// change nothing).  With the value scales' logarithms and reciprocals
+// from shared memory, which hands out 16 bytes to a whole warp in four cycles, it was 7,500.  A prompt of 2,048 tokens, 32 heads on 8: 80 us, 430
+// TFLOP/s (attention_kv8.cu's tiles of 32 rows 272 us; bfloat16 pages 49 us).
 // All waits are bounded and report through this file's error word.
 #include <type_traits>
 

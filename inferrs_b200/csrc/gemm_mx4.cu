@@ -34,7 +34,9 @@ namespace mx4 {
 using namespace sm100;
 
 constexpr int BM = 128, THREADS = 192, A_BYTES = BM * 128;
-constexpr int INSIDE_ROWS = 4;        // up to so many bfloat16 rows are brought to pieces inside the product (4,096 x 24,576: four rows 13.4 us, eight 16.2 and by themselves 13.3)
+// up to so many bfloat16 rows are brought to pieces inside the product (4,096 x 24,576: four rows 13.4 us, eight 16.2 and by themselves 13.3, 13.7 outside
+// captured steps)
+constexpr int INSIDE_ROWS = 4;
 // what a kernel's rows are: the number of pieces of a number, CODES for 4-bit rows
 enum { CODES = 1, PIECES_BF16 = 2, PIECES_F32 = 5 };
 
@@ -418,7 +420,8 @@ __global__ void __launch_bounds__(THREADS + (INSIDE ? 256 : 128)) few_rows_kerne
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
         if (ok && g_error == 0 && q * 32 < sh.tile_rows) {
-            // accumulator columns at a time, their tokens; the stages' shared memory is free (one stage has 4 KB and more for every 32 rows)
+            // accumulator columns at a time, their tokens; the stages' shared memory is free (one stage has what a warp's tokens take for every 32
+            // rows begun: 4 KB where B's tile does, 2 KB at most with 16 columns)
             constexpr int COLS = KIND == PIECES_F32 ? 80 : BN < 32 ? BN : 32, STEP = COLS / KIND;
             unsigned char* mine = smem + q * STORE_BYTES;
             const unsigned there = splits > 1 ? at_rank(smem_u32(recv + ((size_t)rank * owned + row % owned) * P::PART), (unsigned)(row / owned % splits)) : 0;
@@ -769,7 +772,8 @@ constexpr int SMS = 148, FEW_SMEM = 100 * 1024, ALONE_SMEM = 200 * 1024;      //
 // share an SM; its results cost 80 cycles a row of x, and parts their meeting, which grows with the rows of x too.  The numbers are
 // fitted to 4,700 products of 20 kinds (six matrices, 1 to 64 rows, every height and cut): what the rule takes is 3 % slower than the
 // best on average (lowered tiles in parts as well: 3.5 %).  Us of a product in a row of products, tiles x parts: 4,096 x 4,096, one row 128 x 1 9.4, 64 x 2 7.7, 128 x 4 6.2,
-// 128 x 8 6.7; 64 rows 128 x 1 14.9, 64 x 2 12.0, 128 x 4 10.2.  4,096 x 24,576, one row: 88 x 1 12.5, 128 x 1 12.8; 64 rows 19.0, 22.9.
+// 128 x 8 6.7; 64 rows 128 x 1 14.9, 64 x 2 12.0, 128 x 4 10.2.  4,096 x 24,576, one row: 88 x 1 12.5, 128 x 1 12.8; 64 rows 19.0, 22.9.  (More than four
+// rows: as in captured steps; a call that waits for the rows' way to pieces takes about 1 us more, with every shape.)
 template <int KIND, int BN>
 static Shape shape_for(int n, int m, int num_kb, int tiles_t, int tile_rows, int splits) {
     using P = Plan<KIND, BN>;
@@ -882,7 +886,7 @@ static int launch(const void* w, const void* x, int n, int m, int k, Params p, c
 
 // Tokens of a tile of the product that rows as pieces go through.  17 to 64 float32 rows are several tiles of 16 that read the weights
 // again, or one or two of 32 on pairs of CTAs, which want many rows of W (us of 32 rows: 4,096 x 24,576 35 and 21, 4,096 x 4,096 10.3 and 11.6,
-// 12,288 x 4,096 17 and 25; 64 rows 45 and 30, 12.7 and 12.8, 26 and 27).
+// 12,288 x 4,096 17 and 25; 64 rows 45 and 30, 12.7 and 12.8, 26 and 27; between 4,096 and 24,576 rows of W it was not measured).
 static int tile_tokens(int x_kind, int n, int m) {
     if (x_kind == 1) return n <= 16 || (n <= 64 && m <= 8192) ? 16 : 32;
     return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 96;

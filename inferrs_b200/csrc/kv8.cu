@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 9) kv8_store_whole_kernel(
 }
 
 // Everything else, a warp per head of a row: norm, rotation in float32; queries are stored in their type, keys and values as codes
-// with a scale per vector.
+// with a scale per vector.  (A key's codes are the nearest ones to what float32 gives: one may be the neighbour of the kernel's above.)
 template <typename T, typename WT>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv8_store_kernel(
     const T* __restrict__ qkv, const WT* __restrict__ q_weight, const WT* __restrict__ k_weight,

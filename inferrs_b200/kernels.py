@@ -2675,9 +2675,9 @@ def kv8_tiles_supported(head_dim: int, page_size: int) -> bool:
     return head_dim in KV8_HEAD_DIMS and page_size % 16 == 0
 
 
-# From so many CTAs on, tiles of 256 rows are the faster ones (us, 32 heads on 8, tiles of 32 and of 256): 8 CTAs, 64 tokens, 16 and 16 without
-# a context, 42 and 67 behind 2,000 tokens; 16 CTAs, 128 tokens, 32 and 16, 55 and 68, 77 and 120 behind 4,000; 24 CTAs, 192 tokens, 32 and 19, 79
-# and 71, 124 and 121.
+# From so many CTAs on, tiles of 256 rows are the faster ones whatever the context (us, 32 heads on 8, tiles of 32 and of 256): 8 CTAs, 64 tokens, 17
+# and 16 without a context, 44 and 69 behind 2,000 tokens; 16 CTAs, 128 tokens, 34 and 16, 57 and 70, 80 and 124 behind 4,000; 24 CTAs, 192 tokens, 34
+# and 19, 82 and 72, 129 and 124.  (The context is not asked, so a first portion of 128 tokens goes in the slower one.)
 KV8_PROMPT_MIN_CTAS = 24
 
 
