@@ -1,0 +1,165 @@
+// Moving what the paged cache holds, in all layers at once: whole pages (a request is forked), and tokens that are kept while
+// others between them go (the path of a tree of drafted tokens, a context that is thinned out).
+//
+// Both kernels move bytes and know nothing of numbers: a tensor is [outer, pages, page], a page [heads, places, vector].  What
+// they cannot do without is each byte read once and written once.
+#include "common.cuh"
+
+namespace moves {
+
+struct Pages {
+    unsigned char* base;
+    long outer, n_pages, page_bytes;     // the tensor [outer][n_pages][page_bytes]
+};
+
+template <typename U, int N>
+__global__ void __launch_bounds__(256) copy_pages_kernel(Pages P, const int* __restrict__ source, const int* __restrict__ target,
+                                                         int n_pairs, int chunks) {
+    const long page_units = P.page_bytes / (long)sizeof(U);
+    const long at = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x - at * chunks);
+    const int pair = (int)(at % n_pairs);
+    const long outer = at / n_pairs;
+    const int from = source[pair], to = target[pair];
+    if (from < 0 || to < 0 || from >= P.n_pages || to >= P.n_pages || from == to) return;
+    const U* src = reinterpret_cast<const U*>(P.base) + (outer * P.n_pages + from) * page_units;
+    U* dst = reinterpret_cast<U*>(P.base) + (outer * P.n_pages + to) * page_units;
+    U held[N];
+    const long first = (long)chunk * (256 * N) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (first + i * 256 < page_units) held[i] = src[first + i * 256];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (first + i * 256 < page_units) dst[first + i * 256] = held[i];
+}
+
+// Token kept[r, i] behind context[r] goes to place context[r] + i.  The places are ascending, so a token never moves back and
+// never beyond one that follows it: chunk by chunk, with all loads of a chunk ahead of its stores, nothing is overwritten before
+// it has been read (a chunk's stores end below the places that the next chunk reads).  One CTA for a head of one request in
+// one plane, so chunks of the same vectors never run at once.
+template <typename U, int N>
+__global__ void __launch_bounds__(256) keep_tokens_kernel(Pages P, int heads, int places, int units,      // units per vector
+                                                          const int* __restrict__ table, int max_pages,
+                                                          const int* __restrict__ context, const int* __restrict__ kept,
+                                                          int max_kept, const int* __restrict__ n_kept) {
+    const int r = blockIdx.z, head = blockIdx.y;
+    const long outer = blockIdx.x;
+    int n = n_kept[r];
+    n = n < max_kept ? n : max_kept;
+    const long first = context[r];
+    const int per = units < (int)blockDim.x ? units : (int)blockDim.x;       // threads that share a vector
+    const int step = blockDim.x / per;                                       // vectors that the CTA takes side by side
+    const int mine = threadIdx.x / per;
+    U* plane = reinterpret_cast<U*>(P.base) + outer * P.n_pages * heads * places * units;
+    const int* bt = table + (long)r * max_pages;
+    auto vector_at = [&](long place) -> U* {
+        if (place < 0) return nullptr;
+        const long slot = place / places;
+        if (slot >= max_pages) return nullptr;
+        const int page = bt[slot];
+        if (page < 0 || page >= P.n_pages) return nullptr;
+        return plane + (((long)page * heads + head) * places + (place - slot * places)) * units;
+    };
+    for (int unit0 = 0; unit0 < units; unit0 += per) {
+        const int unit = unit0 + (int)(threadIdx.x - mine * per);
+        const bool some = mine < step && unit < units;
+        for (int i0 = 0; i0 < n; i0 += step * N) {
+            U held[N];
+            U* to[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int i = i0 + k * step + mine;
+                to[k] = nullptr;
+                if (!some || i >= n) continue;
+                const int from = kept[(long)r * max_kept + i];
+                if (from == i) continue;
+                const U* src = vector_at(first + from);
+                to[k] = vector_at(first + i);
+                if (src == nullptr) to[k] = nullptr;
+                if (to[k] != nullptr) held[k] = src[unit];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (to[k] != nullptr) to[k][unit] = held[k];
+        }
+        __syncthreads();
+    }
+}
+
+// the widest unit that both the address and the length are a multiple of
+static int unit_of(const void* p, long bytes) {
+    const unsigned long long a = (unsigned long long)p | (unsigned long long)bytes;
+    for (int u = 16; u > 1; u /= 2)
+        if (a % u == 0) return u;
+    return 1;
+}
+
+}  // namespace moves
+
+using namespace moves;
+
+struct IbCopyPages {
+    unsigned char* base;
+    const int *source, *target;
+    cudaStream_t stream;
+    long outer, n_pages, page_bytes, n_pairs;
+};
+
+template <typename U>
+static int copy_pages_as(const IbCopyPages& a) {
+    const Pages P{a.base, a.outer, a.n_pages, a.page_bytes};
+    const long units = a.page_bytes / (long)sizeof(U), pages = a.outer * a.n_pairs;
+    const long chunks = (units + 256 * 4 - 1) / (256 * 4);
+    if (pages * chunks > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
+    copy_pages_kernel<U, 4><<<(unsigned)(pages * chunks), 256, 0, a.stream>>>(P, a.source, a.target, (int)a.n_pairs, (int)chunks);
+    return ib_launch_status();
+}
+
+IB_EXPORT int ib_copy_pages(const void* call) {
+    const IbCopyPages a = *static_cast<const IbCopyPages*>(call);
+    if (a.outer < 0 || a.n_pages < 0 || a.page_bytes < 0 || a.n_pairs < 0 || a.n_pairs > 0x7fffffffL) return IB_ERR_ARGUMENT;
+    if (a.outer == 0 || a.n_pages == 0 || a.page_bytes == 0 || a.n_pairs == 0) return IB_OK;
+    switch (unit_of(a.base, a.page_bytes)) {
+        case 16: return copy_pages_as<uint4>(a);
+        case 8: return copy_pages_as<uint2>(a);
+        case 4: return copy_pages_as<unsigned>(a);
+        case 2: return copy_pages_as<unsigned short>(a);
+        default: return copy_pages_as<unsigned char>(a);
+    }
+}
+
+struct IbKeepTokens {
+    unsigned char* base;
+    const int *table, *context, *kept, *n_kept;
+    cudaStream_t stream;
+    long outer, n_pages, heads, places, vector_bytes, requests, max_pages, max_kept;
+};
+
+template <typename U>
+static int keep_tokens_as(const IbKeepTokens& a) {
+    const int units = (int)(a.vector_bytes / (long)sizeof(U));
+    const Pages P{a.base, a.outer, a.n_pages, a.heads * a.places * a.vector_bytes};
+    const dim3 grid((unsigned)a.outer, (unsigned)a.heads, (unsigned)a.requests);
+    int threads = 256;
+    while (threads > 32 && (long)(threads / 2) >= a.max_kept * units) threads /= 2;
+    keep_tokens_kernel<U, 4><<<grid, threads, 0, a.stream>>>(P, (int)a.heads, (int)a.places, units, a.table, (int)a.max_pages, a.context,
+                                                             a.kept, (int)a.max_kept, a.n_kept);
+    return ib_launch_status();
+}
+
+IB_EXPORT int ib_keep_tokens(const void* call) {
+    const IbKeepTokens a = *static_cast<const IbKeepTokens*>(call);
+    if (a.outer < 0 || a.n_pages < 0 || a.heads < 0 || a.places <= 0 || a.vector_bytes < 0 || a.requests < 0 || a.max_pages < 0 || a.max_kept < 0)
+        return IB_ERR_ARGUMENT;
+    if (a.outer == 0 || a.n_pages == 0 || a.heads == 0 || a.vector_bytes == 0 || a.requests == 0 || a.max_pages == 0 || a.max_kept == 0) return IB_OK;
+    if (a.outer > 0x7fffffffL || a.heads > 65535 || a.requests > 65535 || a.places > 0x7fffffffL || a.vector_bytes > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
+    switch (unit_of(a.base, a.vector_bytes)) {
+        case 16: return keep_tokens_as<uint4>(a);
+        case 8: return keep_tokens_as<uint2>(a);
+        case 4: return keep_tokens_as<unsigned>(a);
+        case 2: return keep_tokens_as<unsigned short>(a);
+        default: return keep_tokens_as<unsigned char>(a);
+    }
+}

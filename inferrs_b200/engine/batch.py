@@ -96,6 +96,32 @@ class BatchError(ValueError):
     pass
 
 
+def tree_masks(trees: Sequence[Sequence[int]], words: Optional[int] = None):
+    """(masks, depths) of drafted tokens: int32 arrays [rows, words] and [rows].  ``trees[r][i]`` is the parent of request r's i-th
+    drafted token among them (an earlier one), or -1 where it follows the context.  A token sees itself and its ancestors: bit
+    j % 32 of word j // 32 stands for the request's j-th drafted token.  Its depth is the number of its ancestors: it stands
+    at position context + depth.  ``words`` sets a width that does not depend on the trees (a step of fixed shapes)."""
+    most = max((len(t) for t in trees), default=0)
+    need = max(1, -(-most // 32))
+    if words is None:
+        words = need
+    elif words < need:
+        raise BatchError(f"masks of {words} words hold {32 * words} drafted tokens, a request has {most}")
+    n = sum(len(t) for t in trees)
+    masks, depths = np.zeros((n, words), dtype=np.uint32), np.zeros(n, dtype=np.int32)
+    at = 0
+    for r, tree in enumerate(trees):
+        for i, parent in enumerate(tree):
+            if not -1 <= parent < i:
+                raise BatchError(f"drafted token {i} of entry {r}: its parent is an earlier one or -1, got {parent}")
+            if parent >= 0:
+                masks[at + i] = masks[at + parent]
+                depths[at + i] = depths[at + parent] + 1
+            masks[at + i, i // 32] |= np.uint32(1 << (i % 32))
+        at += len(tree)
+    return masks.view(np.int32), depths
+
+
 def sorted_tiles(q_lens: Sequence[int], starts: Sequence[int], tokens_per_tile: int, portions_only: bool):
     """The step's rows cut into tiles of at most ``tokens_per_tile`` tokens of one request each, as
     (position of the tile's last token, request, first row); ``starts[r]`` is the position of request r's first token

@@ -8,6 +8,7 @@ functions: without a CUDA device, ``nvcc`` or a successful build they raise.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from dataclasses import dataclass
 from typing import Optional
@@ -2759,6 +2760,185 @@ def few_bits_faults(reset: bool = True) -> dict:
     values = (_FEW_BITS_LIB.ib_kv8_row_fault(int(reset)), _FEW_BITS_LIB.ib_gemm_mx4_error(int(reset)),
               _FEW_BITS_LIB.ib_attention_kv8_error(int(reset)))
     return {name: v for name, v in zip(FEW_BITS_WORDS, values) if v}
+
+
+# ---- drafted tokens, forked requests, log probabilities (csrc/attention_tree.cu, cache_moves.cu, log_probs.cu) ----------
+_DRAFTS_LIB = None
+_DRAFTS_CALLS = ("ib_paged_attention_tree", "ib_copy_pages", "ib_keep_tokens", "ib_token_log_probs")
+# The calls take their arguments as one structure of 8-byte fields (IbTreeAttention, IbCopyPages, IbKeepTokens, IbTokenLogProbs
+# in csrc/), like those of the kernels in few bits.
+_TREE_CALL = struct.Struct("=24qd").pack
+_COPY_CALL = struct.Struct("=8q").pack
+_KEEP_CALL = struct.Struct("=14q").pack
+_LOG_PROBS_CALL = struct.Struct("=13q").pack
+
+
+def _drafts():
+    global _DRAFTS_LIB
+    if _DRAFTS_LIB is None:
+        lib = load_library("drafts")
+        for fn in _DRAFTS_CALLS:
+            getattr(lib, fn).argtypes = [ctypes.c_char_p]
+            getattr(lib, fn).restype = c_int
+        _DRAFTS_LIB = lib
+    return _DRAFTS_LIB
+
+
+def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The current stream, where all tensors given are on its device."""
+    stream = _stream()
+    here = _DEVICE_INDEX if _RAW_STREAM is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current stream is one of cuda:{here}")
+    return stream
+
+
+def paged_attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                         q_start: torch.Tensor, context: torch.Tensor, positions: Optional[torch.Tensor], seen: torch.Tensor,
+                         scale: float, window: Optional[int], out: torch.Tensor, max_tree: int, max_kv_len: int):
+    """Attention of drafted tokens over their requests' pages.  Rows q_start[r] .. q_start[r + 1] - 1 are the drafted tokens of
+    request r; ``context[r]`` keys are in its pages ahead of them, and the i-th drafted token's key and value are at place
+    context[r] + i.  out[row, h*d:(h+1)*d] = the attention of the row's head h over
+
+    * the context: all of it, or with ``window`` (see :func:`span_argument`) what a token at positions[row] sees of it,
+    * the drafted tokens of its own request that its mask names: bit j % 32 of seen[row, j // 32] stands for the j-th
+      (:func:`inferrs_b200.engine.batch.tree_masks` makes the masks of a tree).
+
+    q [N, heads, d] and the pages [pages, kv_heads, page size, d] are all float32 or all bfloat16, d up to 512; block_table
+    int32 [R, max_pages], q_start int32 [R + 1] (ascending), context int32 [R], positions int32 [N] (only read with a window), seen int32
+    [N, words].  ``max_tree``: no request has more drafted tokens (rows beyond it may be left out); ``max_kv_len``: how the keys are
+    cut goes by it.  A row that sees no key gets zeros; a key without a page is none; rows from q_start[R] on are left as they
+    were.  The rows of ``out`` may lie apart."""
+    act = out.dtype
+    out_ld = _need_rows(out, "out", _BF16_F32)
+    if not (_lists(q_start, context) and q.dtype is act and k_pages.dtype is act and v_pages.dtype is act and q.dim() == 3
+            and k_pages.dim() == 4 and q.is_contiguous() and k_pages.is_contiguous() and v_pages.is_contiguous() and q.is_cuda
+            and k_pages.is_cuda and v_pages.is_cuda and block_table.dtype is _I32 and block_table.dim() == 2
+            and block_table.is_contiguous() and seen.dtype is _I32 and seen.dim() == 2 and seen.is_contiguous()):
+        _need(q, "q", (act,), 3)
+        _need(k_pages, "k_pages", (act,), 4)
+        _need(v_pages, "v_pages", (act,), 4)
+        _need(block_table, "block_table", _I, 2)
+        _need(q_start, "q_start", _I, 1)
+        _need(context, "context", _I, 1)
+        _need(seen, "seen", _I, 2)
+    n, nh, d = q.shape
+    n_pages, nkv, page_size, dk = k_pages.shape
+    n_req, max_pages = block_table.shape
+    span = int(window) if window else 0
+    if span and positions is None:
+        raise KernelError("paged_attention_tree: a window goes by the rows' positions")
+    _need(positions, "positions", _I, 1, optional=True)
+    if dk != d or v_pages.shape != k_pages.shape or nkv == 0 or nh % nkv or out.shape != (n, nh * d) or context.shape[0] != n_req \
+            or q_start.shape[0] != n_req + 1 or seen.shape[0] != n or (positions is not None and positions.shape[0] != n):
+        raise KernelError(f"paged_attention_tree: q {tuple(q.shape)}, pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)}, block table "
+                          f"{tuple(block_table.shape)}, q_start {tuple(q_start.shape)}, context {tuple(context.shape)}, seen "
+                          f"{tuple(seen.shape)}, out {tuple(out.shape)}")
+    if max_tree < 0 or max_kv_len < 0:
+        raise KernelError(f"paged_attention_tree: at most {max_tree} drafted tokens over {max_kv_len} keys")
+    stream = _one_device("paged_attention_tree", q, k_pages, v_pages, block_table, q_start, context, positions, seen, out)
+    code = _drafts().ib_paged_attention_tree(_TREE_CALL(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), context.data_ptr(),
+        0 if positions is None else positions.data_ptr(), seen.data_ptr(), out.data_ptr(), stream, act is _F32, out_ld, n, n_req, nh, nkv, d,
+        max_pages, page_size, n_pages, seen.shape[1], span, max_tree, max_kv_len, scale))
+    if code == -1:
+        raise KernelError(f"paged_attention_tree takes heads of up to 512 numbers and caches of fewer than 2^31 keys; got heads of {d}, "
+                          f"{n_pages} pages of {page_size} places and {nkv} heads, requests of {max_pages} pages")
+    _check(code, "paged_attention_tree")
+
+
+def _page_axes(what: str, pages: torch.Tensor, axis: int, behind: int):
+    """(planes ahead of the axis, pages) of a contiguous tensor with at least ``behind`` axes behind the one that counts pages."""
+    if not (pages.is_cuda and pages.is_contiguous() and 0 <= axis < pages.dim() - behind):
+        raise KernelError(f"{what}: pages must be a contiguous CUDA tensor with at least {behind} axes behind the one that counts its "
+                          f"pages, got {tuple(pages.shape)} on {pages.device}, axis {axis}")
+    return math.prod(pages.shape[:axis]), pages.shape[axis]
+
+
+def copy_pages(pages: torch.Tensor, axis: int, source: torch.Tensor, target: torch.Tensor):
+    """Page target[i] becomes a copy of page source[i], in every plane ahead of ``axis``, the axis of ``pages`` that counts pages
+    (any type; contiguous).  source and target int32 [n].  A page may be copied to many; no target may stand twice in the list or
+    be a source too (but of itself).  A pair with a page that is not there is left out."""
+    outer, n_pages = _page_axes("copy_pages", pages, axis, 0)
+    _need(source, "source", _I, 1)
+    _need(target, "target", _I, 1)
+    if source.shape != target.shape:
+        raise KernelError(f"copy_pages: {source.shape[0]} sources for {target.shape[0]} targets")
+    stream = _one_device("copy_pages", pages, source, target)
+    page_bytes = math.prod(pages.shape[axis + 1:]) * pages.element_size()
+    _check(_drafts().ib_copy_pages(_COPY_CALL(pages.data_ptr(), source.data_ptr(), target.data_ptr(), stream, outer, n_pages, page_bytes,
+                                              source.shape[0])), "copy_pages")
+
+
+def keep_tokens(pages: torch.Tensor, axis: int, block_table: torch.Tensor, context: torch.Tensor, kept: torch.Tensor,
+                n_kept: torch.Tensor):
+    """What is cached at place context[r] + kept[r, i] of request r goes to place context[r] + i, for i < n_kept[r], in every plane
+    ahead of ``axis``, the axis of ``pages`` that counts pages; behind it stand heads, a page's places, and the vector's numbers
+    (or none: a scale per vector).  Any type; contiguous.
+
+    block_table int32 [R, max_pages]; context int32 [R]; kept int32 [R, most], ascending in each row's first n_kept[r] (from 0 on,
+    none twice), n_kept int32 [R].  A place without a page is left out.  No page may stand in the tables of two requests at
+    places from context[r] on."""
+    outer, n_pages = _page_axes("keep_tokens", pages, axis, 2)
+    _need(block_table, "block_table", _I, 2)
+    _need(context, "context", _I, 1)
+    _need(kept, "kept", _I, 2)
+    _need(n_kept, "n_kept", _I, 1)
+    n_req, max_pages = block_table.shape
+    if context.shape[0] != n_req or kept.shape[0] != n_req or n_kept.shape[0] != n_req:
+        raise KernelError(f"keep_tokens: block table {tuple(block_table.shape)}, context {tuple(context.shape)}, kept "
+                          f"{tuple(kept.shape)}, n_kept {tuple(n_kept.shape)}")
+    heads, places = pages.shape[axis + 1], pages.shape[axis + 2]
+    if places == 0:
+        return
+    stream = _one_device("keep_tokens", pages, block_table, context, kept, n_kept)
+    vector_bytes = math.prod(pages.shape[axis + 3:]) * pages.element_size()
+    _check(_drafts().ib_keep_tokens(_KEEP_CALL(
+        pages.data_ptr(), block_table.data_ptr(), context.data_ptr(), kept.data_ptr(), n_kept.data_ptr(), stream, outer, n_pages, heads,
+        places, vector_bytes, n_req, max_pages, kept.shape[1])), "keep_tokens")
+
+
+MAX_TOP_LOG_PROBS = 32      # most likely tokens that :func:`token_log_probs` gives at most
+
+
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, log_probs: torch.Tensor, entropy: Optional[torch.Tensor] = None,
+                    top_ids: Optional[torch.Tensor] = None, top_log_probs: Optional[torch.Tensor] = None):
+    """log_probs[r, i] = log of the probability that softmax(logits[r]) gives to token tokens[r, i]; entropy[r] = that
+    distribution's entropy in nats; top_ids[r] = its most likely tokens, the likeliest first and of equal ones the lower id first,
+    with their log probabilities (up to 32 of them).
+
+    logits [R, V] float32 or bfloat16 (rows may lie apart), tokens int32 [R, n]; log_probs and top_log_probs float32, top_ids int32
+    [R, k], entropy float32 [R].  A token outside the vocabulary has minus infinity.  A logit that is no number counts as minus
+    infinity and is never among the likeliest; where those are fewer than k, -1 and minus infinity fill up.  A row whose largest
+    logit is infinite, of either sign, has no distribution: NaN."""
+    ld = _need_rows(logits, "logits", _BF16_F32)
+    _need(tokens, "tokens", _I, 2)
+    _need(log_probs, "log_probs", (_F32,), 2)
+    _need(entropy, "entropy", (_F32,), 1, optional=True)
+    rows, vocab = logits.shape
+    top = 0
+    if (top_ids is None) != (top_log_probs is None):
+        raise KernelError("token_log_probs: top_ids and top_log_probs come together")
+    if top_ids is not None:
+        _need(top_ids, "top_ids", _I, 2)
+        _need(top_log_probs, "top_log_probs", (_F32,), 2)
+        top = top_ids.shape[1]
+        if top > MAX_TOP_LOG_PROBS or top_ids.shape != (rows, top) or top_log_probs.shape != (rows, top):
+            raise KernelError(f"token_log_probs: the most likely tokens of {rows} rows, {MAX_TOP_LOG_PROBS} at most, go to "
+                              f"{tuple(top_ids.shape)} and {tuple(top_log_probs.shape)}")
+    if tokens.shape[0] != rows or log_probs.shape != tokens.shape or (entropy is not None and entropy.shape[0] != rows):
+        raise KernelError(f"token_log_probs: logits {(rows, vocab)}, tokens {tuple(tokens.shape)}, log_probs {tuple(log_probs.shape)}, "
+                          f"entropy {None if entropy is None else tuple(entropy.shape)}")
+    if rows == 0:
+        return
+    if not 0 < vocab <= 1 << 30:
+        raise KernelError(f"token_log_probs: a vocabulary has 1 to 2^30 tokens, got {vocab}")
+    stream = _one_device("token_log_probs", logits, tokens, log_probs, entropy, top_ids, top_log_probs)
+    _check(_drafts().ib_token_log_probs(_LOG_PROBS_CALL(
+        logits.data_ptr(), tokens.data_ptr(), log_probs.data_ptr(), 0 if entropy is None else entropy.data_ptr(),
+        top_ids.data_ptr() if top else 0, top_log_probs.data_ptr() if top else 0, stream, logits.dtype is _F32, ld, rows, vocab,
+        tokens.shape[1], top)), "token_log_probs")
 
 
 # ---- the kernels' error words, all of them ------------------------------------------------------------------
