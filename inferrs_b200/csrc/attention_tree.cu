@@ -9,74 +9,9 @@
 // All heads of a key/value head's group and all tokens of the tree share what they read of the cache, so the rows of a tile are
 // (token, head of the group) pairs, counted token by token.  The keys are cut into as many parts as the machine has room for:
 // the CTAs of a cluster take one each and join their sums through distributed shared memory, in the order of the parts.
-#include "common.cuh"
-#include "sm100.cuh"
+#include "tree.cuh"
 
 namespace tree {
-
-constexpr int MAX_CLUSTER = 8;
-
-struct Args {
-    const void *q, *k, *v;
-    const int *table, *q_start, *context, *positions, *seen;
-    void* out;
-    long out_ld;
-    int n_rows, n_requests, n_heads, n_kv, dim, max_pages, page_size, n_pages, words, span, tiles_of_rows;
-    float scale_log2;          // scale * log2(e)
-};
-
-// what a CTA works for
-struct Work {
-    int req, head, row_tile, part, parts;
-};
-
-// a request's rows, keys and drafted tokens
-struct Span {
-    int row0, n_tree, context, keys;
-};
-__device__ __forceinline__ Span span_of(const Args& A, int req) {
-    Span s;
-    const int a = A.q_start[req], b = A.q_start[req + 1];
-    s.row0 = a < 0 ? 0 : a;
-    const int end = b < A.n_rows ? b : A.n_rows;
-    s.n_tree = end > s.row0 ? end - s.row0 : 0;
-    const int c = A.context[req];
-    s.context = c < 0 ? 0 : c;
-    const long room = (long)A.max_pages * A.page_size;      // places beyond the block table hold no keys
-    if (s.context > room) s.context = (int)room;
-    const long all = (long)s.context + s.n_tree;
-    s.keys = (int)(all < room ? all : room);
-    return s;
-}
-
-__device__ __forceinline__ int first_key(const Args& A, const Span& s, int token) {
-    return A.span == 0 ? 0 : ib_first_visible(A.positions[s.row0 + token], A.span);
-}
-
-// bits j .. j + 31 of a row's mask, where bits below 0 and from n_tree on are not set
-__device__ __forceinline__ unsigned mask_bits(const Args& A, const Span& s, const int* row_words, int j) {
-    const int at = j >> 5, shift = j & 31;        // (an arithmetic shift: rounds down)
-    const unsigned a = at >= 0 && at < A.words ? (unsigned)row_words[at] : 0u;
-    const unsigned b = shift && at + 1 >= 0 && at + 1 < A.words ? (unsigned)row_words[at + 1] : 0u;
-    unsigned bits = __funnelshift_r(a, b, shift);
-    const int left = s.n_tree - j;
-    if (left < 32) bits &= left <= 0 ? 0u : (1u << left) - 1u;
-    return bits;
-}
-
-__device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {
-    unsigned a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // ---- any type and head size: 32-bit arithmetic, 16 rows a CTA, four for each warp ----------------------------------------
 constexpr int ROWS = 16, KEYS = 32, WARPS = 4, MINE = ROWS / WARPS;
@@ -238,24 +173,6 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     if (parts > 1) cluster_sync();                // nobody leaves while others read its sums
 }
 
-template <typename... KArgs, typename... Given>
-static int launch_cluster(void (*kernel)(KArgs...), long ctas, int cluster, int threads, size_t smem, cudaStream_t stream, Given... args) {
-    if (ctas > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-    return ib_launch_status();
-}
-
 template <typename T, int PER>
 static int launch_rows(const Args& A, int max_keys, cudaStream_t stream) {
     static IbDeviceSet done;
@@ -285,15 +202,6 @@ static int rows_of_type(Args A, int max_tree, int max_keys, cudaStream_t stream)
 
 }  // namespace tree
 
-struct IbTreeAttention {
-    const void *q, *k, *v;
-    const int *table, *q_start, *context, *positions, *seen;
-    void* out;
-    cudaStream_t stream;
-    long f32, out_ld, n_rows, n_requests, n_heads, n_kv, dim, max_pages, page_size, n_pages, words, span, max_tree, max_keys;
-    double scale;
-};
-
 IB_EXPORT int ib_paged_attention_tree(const void* call) {
     using namespace tree;
     const IbTreeAttention c = *static_cast<const IbTreeAttention*>(call);
@@ -314,5 +222,10 @@ IB_EXPORT int ib_paged_attention_tree(const void* call) {
     A.max_pages = (int)c.max_pages; A.page_size = (int)c.page_size; A.n_pages = (int)c.n_pages; A.words = (int)c.words; A.span = (int)c.span;
     A.scale_log2 = (float)(c.scale * 1.4426950408889634);
     const int keys = (int)(c.max_keys < 0x7fffffffL ? c.max_keys : 0x7fffffffL);
+    A.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)c.page_size) : -1;
+    if (!c.f32) {
+        const int code = ib_tree_tcgen05(A, (int)tree, keys, c.stream);
+        if (code != IB_ERR_UNSUPPORTED) return code;
+    }
     return c.f32 ? rows_of_type<float>(A, (int)tree, keys, c.stream) : rows_of_type<__nv_bfloat16>(A, (int)tree, keys, c.stream);
 }

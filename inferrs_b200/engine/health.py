@@ -20,7 +20,8 @@ class KernelHealth:
     def __init__(self, dtype: torch.dtype, every: int = 16):
         self.dtype = dtype
         self.every = every                   # steps between two looks when no request ends
-        self.host = torch.zeros((len(kernels.ERROR_WORDS + kernels.FEW_BITS_WORDS),), dtype=torch.int32).pin_memory()
+        self.names = kernels.ERROR_WORDS + kernels.FEW_BITS_WORDS + kernels.DRAFTS_WORDS
+        self.host = torch.zeros((len(self.names),), dtype=torch.int32).pin_memory()
         self.event: Optional[torch.cuda.Event] = None
 
     @property
@@ -42,9 +43,8 @@ class KernelHealth:
             return None
         self.event.synchronize()
         self.event = None
-        names = kernels.ERROR_WORDS + kernels.FEW_BITS_WORDS
-        words = self.host[:len(names)].tolist()
-        return {name: int(v) for name, v in zip(names, words) if v}
+        words = self.host[:len(self.names)].tolist()
+        return {name: int(v) for name, v in zip(self.names, words) if v}
 
     def reset(self) -> Dict[str, int]:
         """Clear the words on the device (waits for it); returns what was set."""

@@ -2780,6 +2780,8 @@ def _drafts():
         for fn in _DRAFTS_CALLS:
             getattr(lib, fn).argtypes = [ctypes.c_char_p]
             getattr(lib, fn).restype = c_int
+        lib.ib_attention_tree_error.argtypes, lib.ib_attention_tree_error.restype = [c_int], c_int
+        lib.ib_attention_tree_error_async.argtypes, lib.ib_attention_tree_error_async.restype = [c_void_p, c_void_p], c_int
         _DRAFTS_LIB = lib
     return _DRAFTS_LIB
 
@@ -2846,6 +2848,11 @@ def paged_attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
         raise KernelError(f"paged_attention_tree takes heads of up to 512 numbers and caches of fewer than 2^31 keys; got heads of {d}, "
                           f"{n_pages} pages of {page_size} places and {nkv} heads, requests of {max_pages} pages")
     _check(code, "paged_attention_tree")
+
+
+def attention_tree_error(reset: bool = True) -> int:
+    """0, or the code of the first bounded wait that ran out in the kernel above (synchronises)."""
+    return _drafts().ib_attention_tree_error(int(reset))
 
 
 def _page_axes(what: str, pages: torch.Tensor, axis: int, behind: int):
@@ -2948,11 +2955,14 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, log_probs: torch
 ERROR_WORDS = ("a row's position outside the rotation tables", "prefill attention (tcgen05)",
                "prefill attention (two query tiles)", "decode attention", "matrix product (tcgen05)",
                "chain of matrix products")
+# ... and, where a program has used them, behind those of the kernels in few bits
+DRAFTS_WORDS = ("attention of drafted tokens",)
 
 
 def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
     """Ask for every error word of the kernel libraries, in the order of ``ERROR_WORDS``, to be copied into ``host``
-    (pinned int32, at least ``len(ERROR_WORDS)`` long; with room for them, those of the kernels in few bits follow) behind
+    (pinned int32, at least ``len(ERROR_WORDS)`` long; with room for them, those of the kernels in few bits and of the drafted
+    tokens' attention follow) behind
     the work that the current stream holds.  The caller
     records an event after this call and reads ``host`` once the event has come."""
     if host.dtype != torch.int32 or host.numel() < len(ERROR_WORDS) or not host.is_pinned():
@@ -2973,6 +2983,13 @@ def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
                 code = fn(at + 4 * (len(ERROR_WORDS) + i), stream)
                 if code != 0:
                     raise KernelError(f"error_words_async: CUDA error {code}")
+    behind = len(ERROR_WORDS) + len(FEW_BITS_WORDS)
+    if host.numel() >= behind + len(DRAFTS_WORDS):       # and that of the drafted tokens' attention
+        host[behind] = 0
+        if _DRAFTS_LIB is not None:
+            code = _DRAFTS_LIB.ib_attention_tree_error_async(at + 4 * behind, stream)
+            if code != 0:
+                raise KernelError(f"error_words_async: CUDA error {code}")
     for i, fn in enumerate(calls):
         code = fn(at + 4 * i, stream)
         if code != 0:
@@ -2996,6 +3013,10 @@ def reset_error_words(act_dtype: torch.dtype) -> dict:
         if v:
             found[name] = v
     found.update(few_bits_faults(reset=True))
+    if _DRAFTS_LIB is not None:
+        v = attention_tree_error(True)
+        if v:
+            found[DRAFTS_WORDS[0]] = v
     for counters in _DECODE_COUNTERS.values():
         counters.zero_()
     return found
