@@ -12,7 +12,7 @@
 //
 // What bounds it is what comes from memory: a tile of 128 keys and values of 128 numbers is 64 KB, 2,900 cycles of an SM's share of the
 // copy bandwidth, and needs 1,100 cycles of products and as many of exponentials for every 128 rows.  Keys and values come through
-// a ring of tiles that four warps fill with cp.async, 16 bytes a lane: rows of a page lie anywhere, pages have any size, and where there is
+// a ring of tiles that two warps fill with cp.async, 16 bytes a lane: rows of a page lie anywhere, pages have any size, and where there is
 // no key zeros are written.  Ring places come in the order in which the products take them.
 //
 // What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So in tiles that some row does
@@ -28,7 +28,8 @@ using namespace tree;
 typedef __nv_bfloat16 bf16;
 
 constexpr int ROWS = 128, KEYS = 128;
-constexpr int PRODUCERS = 8, ISSUER = 12, THREADS = 13 * 32;      // warps 0..7: softmax, 8..11: the ring, 12: products
+constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
+constexpr int EACH = 4 / N_PRODUCERS;          // rows of a tile that a warp brings, in 32
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
 constexpr int MOST_PARTS = 8;
 constexpr int RANKED = 1024;          // requests that are put in order of their length
@@ -46,7 +47,7 @@ template <int D, int NQ> struct Shape {
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
     static constexpr int SMEM = 1024 + TILES + 256;
-    static_assert(SUMS + 4 * ROWS * 4 <= TILES, "the sums, references and denominators take the place of the tiles");
+    static_assert(SUMS + 4 * ROWS * 4 + 16 * NQ * ROWS * 4 <= TILES, "the sums, references, denominators and factors take the place of the tiles");
     // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
     static_assert(SMEM > 116 * 1024 && SMEM <= 232448, "one CTA an SM");
 };
@@ -61,7 +62,7 @@ static_assert(sizeof(Small) <= 256, "");
 __device__ __forceinline__ void cp16(unsigned dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// an arrival when all that this thread has asked for so far is there
+// an arrival when all that this thread has asked for so far is there (who waits for it needs fence_async before products read it)
 __device__ __forceinline__ void cp_arrive(unsigned bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -111,6 +112,69 @@ __device__ __forceinline__ bool clean_rows(unsigned tile, int w, int lane) {
     return any;
 }
 
+// Columns of this warp's lanes of tensor memory, and the wait for them: in one piece, since the compiler may put registers aside
+// between the two, before they hold what was asked for
+__device__ __forceinline__ void tmem_ld64(unsigned taddr, unsigned (&r)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29"
+                 ",%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%"
+                 "57,%58,%59,%60,%61,%62,%63}"
+                 ", [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29"
+                 ",%30,%31}"
+                 ", [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// two neighbouring numbers at once
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pair(float a, float b) {
+    u64 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void apart(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// One lane of the warp, the same every time
+__device__ __forceinline__ bool elected() {
+    unsigned r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// operand descriptors: desc_k_major and desc_mn_major (groups of 64 numbers ROWS * 128 bytes apart) of sm100.cuh, from the address in 16 bytes
+__device__ __forceinline__ u64 words(unsigned lo, unsigned hi) {
+    u64 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+constexpr unsigned K_HI = (unsigned)(1024 >> 4) | 1u << 14 | 2u << 29, V_HI = K_HI, K_LO = 1u << 16, V_LO = (unsigned)(ROWS * 128 >> 4) << 16;
+
 struct Place {
     const int* bt;
     int head, keys;
@@ -123,36 +187,67 @@ __device__ __forceinline__ int key_index(const Args& A, const Place& p, int j) {
     return (page * A.n_kv + p.head) * A.page_size + (j - slot * A.page_size);
 }
 
-// which of the 32 keys from jb on a row sees; lo: the first key of the context that it sees
-__device__ unsigned visible(const Args& A, const Span& S, const Place& p, const int* words, int lo, int jb, bool bad_pages) {
-    const int a = max(lo - jb, 0), b = min(S.context - jb, 32);
-    unsigned bits = 0;
-    if (b > a) bits = (b == 32 ? 0xffffffffu : (1u << b) - 1u) & ~((1u << a) - 1u);
-    if (jb + 32 > S.context) {
-        unsigned drafted = mask_bits(A, S, words, jb - S.context);
-        const int left = S.keys - jb;
-        if (left < 32) drafted &= left <= 0 ? 0u : (1u << left) - 1u;
-        bits |= drafted;
+// which of the 32 N keys from jb on a row sees; lo: the first key of the context that it sees
+template <int N>
+__device__ __forceinline__ void visible(const Args& A, const Span& S, const Place& p, const int* row_words, int lo, int jb, bool bad_pages,
+                                        unsigned (&see)[N]) {
+    const int first = jb - S.context, at = first >> 5, shift = first & 31;        // (rounds down)
+    unsigned w[N + 1];
+#pragma unroll
+    for (int c = 0; c <= N; ++c) w[c] = at + c >= 0 && at + c < A.words ? (unsigned)row_words[at + c] : 0u;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        const int j = jb + 32 * c, a = max(lo - j, 0), b = min(S.context - j, 32), left = S.keys - j;
+        unsigned bits = b > a ? (b == 32 ? 0xffffffffu : (1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
+        if (b < 32) {              // (a drafted token behind the tree's last one is behind the keys too)
+            const unsigned drafted = __funnelshift_r(w[c], w[c + 1], shift);
+            bits |= left >= 32 ? drafted : left > 0 ? drafted & ((1u << left) - 1u) : 0u;
+        }
+        see[c] = bits;
     }
     if (bad_pages)
-        for (int k = 0; k < 32; ++k)
-            if ((bits >> k & 1u) && key_index(A, p, jb + k) < 0) bits &= ~(1u << k);
-    return bits;
+        for (int c = 0; c < N; ++c)
+            for (int k = 0; k < 32; ++k)
+                if ((see[c] >> k & 1u) && key_index(A, p, jb + 32 * c + k) < 0) see[c] &= ~(1u << k);
 }
 
 __device__ __forceinline__ float4 remote_f32x4(const float* local, unsigned rank) {
     float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote(local, rank)) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote(local, rank)));
     return v;
 }
-__device__ __forceinline__ float2 remote_f32x2(const float* local, unsigned rank) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote(local, rank)) : "memory");
+__device__ __forceinline__ int remote_i32(const int* local, unsigned rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(local, rank)));
     return v;
 }
 
+// A row's numbers e .. e + 3 with the infinite values and no numbers that it sees in tiles that not all rows see
+template <int D>
+__device__ __noinline__ float4 with_bad_values(const Args& A, const Span S, const Place place, float4 o, int token, int e, int t_first,
+                                               int n_tiles, int lo_max) {
+    const int lo = first_key(A, S, token);
+    const int* words = A.seen + (long)(S.row0 + token) * A.words;
+    float v[4] = {o.x, o.y, o.z, o.w};
+    for (int t = t_first; t < t_first + n_tiles; ++t) {
+        if (!(t * KEYS < lo_max || (t + 1) * KEYS > S.context)) continue;
+        for (int c = 0; c < 4; ++c) {
+            unsigned see[1];
+            visible(A, S, place, words, lo, t * KEYS + 32 * c, true, see);
+            for (; see[0]; see[0] &= see[0] - 1) {
+                const bf16* x = static_cast<const bf16*>(A.v) + (long)key_index(A, place, t * KEYS + 32 * c + __ffs(see[0]) - 1) * D + e;
+                for (int k = 0; k < 4; ++k) {
+                    const float add = __bfloat162float(x[k]);
+                    if (!(fabsf(add) < INFINITY)) v[k] += add;
+                }
+            }
+        }
+    }
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
 template <int D, int NQ>
-__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int parts, int ranked) {
+__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ Args A, int parts, int ranked) {
     typedef Shape<D, NQ> Sh;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -194,20 +289,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
         sm.bad_values = 0;
     }
     if (warp == ISSUER) {
-        if (lane == 0) {
-            for (int i = 0; i < Sh::STAGES; ++i) { mbar_init(smem_u32(&sm.full[i]), 128); mbar_init(smem_u32(&sm.empty[i]), 1); }
-            for (int g = 0; g < 2; ++g) {
-                const int used = NQ == 2 ? rows - g * ROWS : rows;
-                mbar_init(smem_u32(&sm.s_full[g]), 1);
-                mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : (used + 31) / 32);
-            }
-            mbar_init(smem_u32(&sm.o_full), 1);
-            mbar_init(smem_u32(&sm.q_full), 128);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == PRODUCERS && lane == 0) {
+        for (int i = 0; i < Sh::STAGES; ++i) { mbar_init(smem_u32(&sm.full[i]), 32 * N_PRODUCERS); mbar_init(smem_u32(&sm.empty[i]), 1); }
+        for (int g = 0; g < 2; ++g) {
+            const int used = NQ == 2 ? rows - g * ROWS : rows;
+            mbar_init(smem_u32(&sm.s_full[g]), 1);
+            mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : (used + 31) / 32);
+        }
+        mbar_init(smem_u32(&sm.o_full), 1);
+        mbar_init(smem_u32(&sm.q_full), 32 * N_PRODUCERS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
     __syncthreads();
@@ -233,18 +326,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
     auto partly = [&](int t) { return t * KEYS < lo_max || (t + 1) * KEYS > S.context; };
     bool ok = true;
 
-    if (warp >= PRODUCERS && warp < ISSUER) {
+    if (warp >= PRODUCERS && warp < PRODUCERS + N_PRODUCERS) {
         const int w = warp - PRODUCERS;
         const bf16* q = static_cast<const bf16*>(A.q);
 #pragma unroll
         for (int g = 0; g < NQ; ++g) {
-            const int r = g * ROWS + w * 32 + lane;
-            int index = -1;
-            if (r < rows) {
-                const int at = first_row + r, token = at / group;
-                index = (S.row0 + token) * A.n_heads + head * group + at - token * group;
+#pragma unroll
+            for (int h = 0; h < EACH; ++h) {
+                const int r = g * ROWS + (w * EACH + h) * 32 + lane;
+                int index = -1;
+                if (r < rows) {
+                    const int at = first_row + r, token = at / group;
+                    index = (S.row0 + token) * A.n_heads + head * group + at - token * group;
+                }
+                load_rows<D>(sq + g * Sh::TILE, q, index, w * EACH + h, lane);
             }
-            load_rows<D>(sq + g * Sh::TILE, q, index, w, lane);
         }
         cp_arrive(smem_u32(&sm.q_full));
         // the ring's entries in the order of the products: with two sets of rows K0 V0 K1 V1 .., else K0 K1 V0 K2 V1 .. V(n-1)
@@ -258,76 +354,103 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
             return e == 0 ? 0 : (e & 1) ? (e + 1) >> 1 : (e - 2) >> 1;
         };
         bool values = false;
-        int t = 0, index = -1;
-        if (n > 0) {
-            t = tile_of(0, values);
-            index = key_index(A, place, (t_begin + t) * KEYS + w * 32 + lane);
-        }
+        int index[EACH], index_next[EACH];        // this lane's rows of the entry's tile, and of the next one's: the table's answer takes a while
+        auto look_up = [&](int e, int (&to)[EACH]) {
+            bool unused;
+            const int j = (t_begin + tile_of(e, unused)) * KEYS + w * EACH * 32 + lane;
+#pragma unroll
+            for (int h = 0; h < EACH; ++h) to[h] = e < 2 * n ? key_index(A, place, j + 32 * h) : -1;
+        };
+        look_up(0, index_next);
         int slot = 0, turn = 0;
         for (int e = 0; e < 2 * n; ++e) {
             if (turn > 0 && !mbar_wait(smem_u32(&sm.empty[slot]), (turn - 1) & 1, 1)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const unsigned dst = ring + slot * Sh::TILE, bar = smem_u32(&sm.full[slot]);
-            load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), index, w, lane);
+            const int t = tile_of(e, values);
+#pragma unroll
+            for (int h = 0; h < EACH; ++h) index[h] = index_next[h];
+            look_up(e + 1, index_next);
+            const unsigned dst = ring + slot * Sh::TILE;
+#pragma unroll
+            for (int h = 0; h < EACH; ++h) load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), index[h], w * EACH + h, lane);
             if (values && partly(t_begin + t)) {
                 cp_wait_all();
-                if (clean_rows<D>(dst, w, lane)) sm.bad_values = 1;
-                mbar_arrive(bar);
+#pragma unroll
+                for (int h = 0; h < EACH; ++h)
+                    if (clean_rows<D>(dst, w * EACH + h, lane)) sm.bad_values = 1;
+                mbar_arrive(smem_u32(&sm.full[slot]));
             } else {
-                cp_arrive(bar);
-            }
-            if (e + 1 < 2 * n) {
-                t = tile_of(e + 1, values);
-                index = key_index(A, place, (t_begin + t) * KEYS + w * 32 + lane);
+                cp_arrive(smem_u32(&sm.full[slot]));
             }
             if (++slot == Sh::STAGES) { slot = 0; ++turn; }
         }
         cp_wait_all();
     } else if (warp == ISSUER) {
-        if (lane == 0) {
-            constexpr unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(ROWS >> 4) << 24);
-            constexpr unsigned idesc_s = idesc | ((unsigned)(KEYS >> 3) << 17), idesc_o = idesc | (1u << 16) | ((unsigned)(D >> 3) << 17);
-            auto k_entry = [&](int t) { return NQ == 2 ? 2 * t : t == 0 ? 0 : 2 * t - 1; };
-            auto v_entry = [&](int t) { return NQ == 2 ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1); };
-            const int last = NQ == 2 && count1 > 0 ? 1 : 0;            // with two sets of rows: the stream that is done with a tile last
-            auto arrived = [&](int e) {
-                if (!mbar_wait(smem_u32(&sm.full[e % Sh::STAGES]), (e / Sh::STAGES) & 1, 2)) return false;
-                fence_async();
-                fence_after();
-                return true;
-            };
-            auto scores = [&](int g, int i) {                          // of the stream's i-th tile
-                const int e = k_entry(NQ == 2 ? i : 2 * i + g);
-                if (!arrived(e)) return false;
-                const unsigned k = ring + (e % Sh::STAGES) * Sh::TILE, rows_q = sq + (NQ == 2 ? g * Sh::TILE : 0);
+        // the warp runs its loops as a whole, so that addresses and descriptors are the same for all lanes; one lane issues
+        constexpr unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(ROWS >> 4) << 24);
+        constexpr unsigned idesc_s = idesc | ((unsigned)(KEYS >> 3) << 17), idesc_o = idesc | (1u << 16) | ((unsigned)(D >> 3) << 17);
+        const bool leader = elected();
+        // (an address of a cluster's CTA has its rank above the 18 bits that a descriptor takes)
+        const unsigned ring0 = __shfl_sync(0xffffffffu, (ring & 0x3FFFF) >> 4, 0), q0 = __shfl_sync(0xffffffffu, (sq & 0x3FFFF) >> 4, 0);
+        const unsigned tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int last = NQ == 2 && count1 > 0 ? 1 : 0;            // with two sets of rows: the stream that is done with a tile last
+        struct Turn { int slot; unsigned phase; };
+        Turn k_at = {0, 0}, v_at = {0, 0};                         // the next keys and values: places in the ring
+        auto step = [&](Turn& u, int by) {
+            u.slot += by;
+            if (u.slot >= Sh::STAGES) { u.slot -= Sh::STAGES; u.phase ^= 1; }
+        };
+        step(v_at, NQ == 2 ? 1 : n == 1 ? 1 : 2);
+        auto arrived = [&](const Turn& u) {
+            if (!mbar_wait(smem_u32(&sm.full[u.slot]), u.phase, 2)) return false;
+            fence_async();
+            fence_after();
+            return true;
+        };
+        auto scores = [&](int g) {
+            if (!arrived(k_at)) return false;
+            if (leader) {
+                const unsigned k = ring0 + k_at.slot * (Sh::TILE >> 4), rows_q = q0 + (NQ == 2 ? g * (Sh::TILE >> 4) : 0);
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s) {
-                    const unsigned off = (s >> 2) * (ROWS * 128) + (s & 3) * 32;
-                    umma(tmem + g * 128, desc_k_major(rows_q + off), desc_k_major(k + off), idesc_s, s != 0);
+                    const unsigned off = ((s >> 2) * (ROWS * 128) + (s & 3) * 32) >> 4;
+                    umma(tm + g * 128, words(rows_q + off + K_LO, K_HI), words(k + off + K_LO, K_HI), idesc_s, s != 0);
                 }
                 umma_commit(smem_u32(&sm.s_full[g]));
-                if (NQ == 1 || g == last) umma_commit(smem_u32(&sm.empty[e % Sh::STAGES]));
-                return true;
-            };
-            ok = mbar_wait(smem_u32(&sm.q_full), 0, 3);
-            for (int g = 0; g < 2 && ok; ++g)
-                if ((g ? count1 : count0) > 0) ok = scores(g, 0);
-            for (int i = 0; i < count0 && ok; ++i) {
-                for (int g = 0; g < 2 && ok; ++g) {
-                    if (i >= (g ? count1 : count0)) continue;
-                    const int e = v_entry(NQ == 2 ? i : 2 * i + g);
-                    if (!mbar_wait(smem_u32(&sm.p_full[g]), i & 1, 4) || !arrived(e)) { ok = false; break; }
-                    const unsigned v = ring + (e % Sh::STAGES) * Sh::TILE;
+                if (NQ == 1 || g == last) umma_commit(smem_u32(&sm.empty[k_at.slot]));
+            }
+            return true;
+        };
+        ok = mbar_wait(smem_u32(&sm.q_full), 0, 3);
+        // keys: K0 [V0] K1 [V1] .. with two sets of rows; K0 K1 [V0] K2 [V1] .. else.  Values likewise, the last one behind the one before it.
+        int k_next = 0, v_next = 0;
+        auto k_done = [&]() { step(k_at, NQ == 2 ? 2 : k_next == 0 ? 1 : 2); ++k_next; };
+        auto v_done = [&]() { step(v_at, NQ == 2 ? 2 : v_next + 2 < n ? 2 : 1); ++v_next; };
+        for (int g = 0; g < 2 && ok; ++g)
+            if ((g ? count1 : count0) > 0) {
+                ok = scores(g);
+                if (NQ == 1 || g == last) k_done();
+            }
+        for (int i = 0; i < count0 && ok; ++i) {
+            for (int g = 0; g < 2 && ok; ++g) {
+                if (i >= (g ? count1 : count0)) continue;
+                if (!mbar_wait(smem_u32(&sm.p_full[g]), i & 1, 4) || !arrived(v_at)) { ok = false; break; }
+                if (leader) {
+                    const unsigned v = ring0 + v_at.slot * (Sh::TILE >> 4);
 #pragma unroll
                     for (int s = 0; s < KEYS / 16; ++s)
-                        umma_ts(tmem + 256 + g * 128, tmem + g * 128 + s * 8, desc_mn_major(v + s * 16 * 128, ROWS * 128), idesc_o, (i | s) != 0);
-                    if (NQ == 1 || g == last) umma_commit(smem_u32(&sm.empty[e % Sh::STAGES]));
-                    if (i + 1 < (g ? count1 : count0)) ok = scores(g, i + 1);
+                        umma_ts(tm + 256 + g * 128, tm + g * 128 + s * 8, words(v + s * (16 * 128 >> 4) + V_LO, V_HI), idesc_o, (i | s) != 0);
+                    if (NQ == 1 || g == last) umma_commit(smem_u32(&sm.empty[v_at.slot]));
+                }
+                if (NQ == 1 || g == last) v_done();
+                if (i + 1 < (g ? count1 : count0)) {
+                    ok = scores(g);
+                    if (NQ == 1 || g == last) k_done();
                 }
             }
-            umma_commit(smem_u32(&sm.o_full));
         }
+        if (leader) umma_commit(smem_u32(&sm.o_full));
         __syncwarp();
     } else {
         const int g = warp >> 2, r = (warp & 3) * 32 + lane;
@@ -351,31 +474,42 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
             const unsigned s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * 128;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < count; ++i) {
+                const int t = t_begin + (NQ == 2 ? i : 2 * i + g), j0 = t * KEYS;
+                const bool plain = __all_sync(0xffffffffu, !bad && j0 >= lo && j0 + KEYS <= S.context);
+                unsigned see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                if (!plain) visible(A, S, place, words, lo, j0, bad, see);
                 if (!mbar_wait(smem_u32(&sm.s_full[g]), i & 1, 5)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 fence_after();
-                const int t = t_begin + (NQ == 2 ? i : 2 * i + g), j0 = t * KEYS;
-                const bool plain = __all_sync(0xffffffffu, !bad && j0 >= lo && j0 + KEYS <= S.context);
-                unsigned see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-                if (!plain) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) see[c] = visible(A, S, place, words, lo, j0 + 32 * c, bad);
-                }
-                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    unsigned x[32];
-                    tmem_ld32_issue(s_at + 32 * c, x);
-                    tmem_ld_wait();
+                // 128 scores and what else a thread keeps are more than its registers: half of them stay, half come twice
+                auto hide = [&](auto& x, int at, int c) {
                     if (!plain) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (!(see[c] >> k & 1u)) x[k] = 0xff800000u;
+                            if (!(see[c] >> k & 1u)) x[at + k] = 0xff800000u;
                     }
+                };
+                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto look = [&](const auto& x, int at) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) top4[k & 3] = fmaxf(top4[k & 3], __uint_as_float(x[k]));
-                }
+                    for (int k = 0; k < 32; k += 8)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            top4[c] = max3(top4[c], __uint_as_float(x[at + k + 2 * c]), __uint_as_float(x[at + k + 2 * c + 1]));
+                };
+                unsigned x[64], y[32];
+                tmem_ld64(s_at, x);
+                hide(x, 0, 0);
+                hide(x, 32, 1);
+                look(x, 0);
+                look(x, 32);
+                tmem_ld32(s_at + 64, y);
+                hide(y, 0, 2);
+                look(y, 0);
+                tmem_ld32(s_at + 96, y);
+                hide(y, 0, 3);
+                look(y, 0);
                 const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * A.scale_log2;     // (the scale is positive)
                 const bool move = top > m + STEP || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
@@ -384,8 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
 #pragma unroll 1
                         for (int e = 0; e < D; e += 32) {
                             unsigned x[32];
-                            tmem_ld32_issue(o_at + e, x);
-                            tmem_ld_wait();
+                            tmem_ld32(o_at + e, x);
 #pragma unroll
                             for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * c);
                             tmem_st32(o_at + e, x);
@@ -396,28 +529,31 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
                     if (move) m = top;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    unsigned x[32], p[16];
-                    tmem_ld32_issue(s_at + 32 * c, x);
-                    tmem_ld_wait();
-                    if (!plain) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!(see[c] >> k & 1u)) x[k] = 0xff800000u;
-                    }
-                    float add[2] = {0.0f, 0.0f};
+                const u64 factor = pair(A.scale_log2, A.scale_log2), less = pair(-ref, -ref);
+                u64 add[2] = {0, 0};
+                auto weigh = [&](const unsigned* x, int c) {
+                    unsigned p[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float a = ex2(fmaf(__uint_as_float(x[2 * k]), A.scale_log2, -ref));
-                        const float b = ex2(fmaf(__uint_as_float(x[2 * k + 1]), A.scale_log2, -ref));
-                        add[0] += a;
-                        add[1] += b;
+                        float a, b;
+                        apart(fma2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), factor, less), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        add[k & 1] = add2(add[k & 1], pair(a, b));
                         p[k] = pack_bf16(a, b);
                     }
-                    l += add[0] + add[1];
                     tmem_st16(s_at + 16 * c, p);
-                }
+                };
+                weigh(x, 0);
+                weigh(x + 32, 1);
+                tmem_ld64(s_at + 64, x);
+                hide(x, 0, 2);
+                hide(x, 32, 3);
+                weigh(x, 2);
+                weigh(x + 32, 3);
+                float a, b;
+                apart(add2(add[0], add[1]), a, b);
+                l += a + b;
                 tmem_st_wait();
                 fence_before();
                 __syncwarp();
@@ -431,8 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
 #pragma unroll
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
-                    tmem_ld32_issue(o_at + e, x);
-                    tmem_ld_wait();
+                    tmem_ld32(o_at + e, x);
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
                         *reinterpret_cast<uint4*>(row + e + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
@@ -448,73 +583,69 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const Args A, int part
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
-    // join: CTA `part` writes every parts-th row; a lane holds D / 32 neighbouring numbers of a row
-    constexpr int PER = D / 32, STREAMS = NQ == 2 ? 1 : 2;
+    // Join: CTA `part` writes every parts-th row.  First the factor of every sum of these rows, a thread a row, then the rows' numbers,
+    // four a thread: loads that wait for nothing but their factor.
+    constexpr int STREAMS = NQ == 2 ? 1 : 2, MOST_SUMS = STREAMS * MOST_PARTS;
+    const int n_sums = parts * STREAMS, mine = rows > part ? (rows - part + parts - 1) / parts : 0;
+    float* factors = part_l + 2 * ROWS;                           // [sum][this CTA's row]
     bool bad_values = false;
-    for (int c = 0; c < parts; ++c) {
-        int v;
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(&sm.bad_values, c)) : "memory");
-        bad_values |= v != 0;
-    }
-    for (int row = part + warp * parts; row < rows; row += parts * (THREADS / 32)) {
-        const int g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
-        // lane p looks at the p-th of the row's sums
-        const int n_sums = parts * STREAMS;
-        float m = -INFINITY, l = 0.0f;
-        if (lane < n_sums) {
-            m = remote_f32(&part_m[(g0 + lane % STREAMS) * ROWS + r], lane / STREAMS);
-            l = remote_f32(&part_l[(g0 + lane % STREAMS) * ROWS + r], lane / STREAMS);
-        }
-        const float top = ib_warp_max(m), ref = top == -INFINITY ? 0.0f : top;
-        const float f = l == 0.0f ? 0.0f : ex2(m - ref);
-        const float total = ib_warp_sum(l == 0.0f ? 0.0f : l * f);
-        float o[PER];
+    for (int c = 0; c < parts; ++c) bad_values |= remote_i32(&sm.bad_values, c) != 0;
+    for (int i = tid; i < mine; i += THREADS) {
+        const int row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
+        float m[MOST_SUMS], l[MOST_SUMS], top = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-        for (int p = 0; p < n_sums; ++p) {
-            if (__shfl_sync(0xffffffffu, l, p) == 0.0f) continue;         // none of its keys is seen
-            const float fp = __shfl_sync(0xffffffffu, f, p);
-            const float* from = sums + ((g0 + p % STREAMS) * ROWS + r) * Sh::OLD + lane * PER;
-            if constexpr (PER == 4) {
-                const float4 x = remote_f32x4(from, p / STREAMS);
-                o[0] = fmaf(x.x, fp, o[0]); o[1] = fmaf(x.y, fp, o[1]); o[2] = fmaf(x.z, fp, o[2]); o[3] = fmaf(x.w, fp, o[3]);
-            } else {
-                const float2 x = remote_f32x2(from, p / STREAMS);
-                o[0] = fmaf(x.x, fp, o[0]); o[1] = fmaf(x.y, fp, o[1]);
-            }
+        for (int p = 0; p < MOST_SUMS; ++p) {
+            if (p >= n_sums) continue;
+            m[p] = remote_f32(&part_m[(g0 + p % STREAMS) * ROWS + r], p / STREAMS);
+            l[p] = remote_f32(&part_l[(g0 + p % STREAMS) * ROWS + r], p / STREAMS);
+        }
+#pragma unroll
+        for (int p = 0; p < MOST_SUMS; ++p)
+            if (p < n_sums) top = fmaxf(top, m[p]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int p = 0; p < MOST_SUMS; ++p) {
+            if (p >= n_sums) continue;
+            m[p] = l[p] == 0.0f ? 0.0f : ex2(m[p] - ref);         // (no sum is there where none of its keys is seen)
+            if (l[p] != 0.0f) total = fmaf(l[p], m[p], total);
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] *= inv;
-        const int at = first_row + row, token = at / group;
-        if (bad_values) {             // infinite values and no numbers that the row sees in tiles that not all rows see
-            const int lo = first_key(A, S, token);
-            const int* words = A.seen + (long)(S.row0 + token) * A.words;
-            for (int t = t_first; t < t_first + all_tiles; ++t) {
-                if (!partly(t)) continue;
-                for (int c = 0; c < 4; ++c) {
-                    unsigned see = visible(A, S, place, words, lo, t * KEYS + 32 * c, true);
-                    for (; see; see &= see - 1) {
-                        const int index = key_index(A, place, t * KEYS + 32 * c + __ffs(see) - 1);
+        for (int p = 0; p < MOST_SUMS; ++p)
+            if (p < n_sums) factors[p * (NQ * ROWS) + i] = m[p] * inv;
+    }
+    __syncthreads();
+    constexpr int QUADS = D / 4, BATCH = 4;
+    const bool wide = (reinterpret_cast<uintptr_t>(A.out) | (uintptr_t)(A.out_ld * 2)) % 8 == 0;
+    for (int first = tid; first < mine * QUADS; first += THREADS * BATCH) {
+        float4 o[BATCH];
 #pragma unroll
-                        for (int e = 0; e < PER; ++e) {
-                            const float v = __bfloat162float(static_cast<const bf16*>(A.v)[(long)index * D + lane * PER + e]);
-                            if (!(fabsf(v) < INFINITY)) o[e] += v;
-                        }
-                    }
-                }
+        for (int u = 0; u < BATCH; ++u) {
+            o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int item = first + u * THREADS, i = item / QUADS, e = (item - i * QUADS) * 4;
+            if (i >= mine) continue;
+            const int row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
+            for (int p = 0; p < n_sums; ++p) {
+                const float f = factors[p * (NQ * ROWS) + i];
+                const float* from = sums + ((g0 + p % STREAMS) * ROWS + r) * Sh::OLD + e;
+                if (f == 0.0f) continue;
+                const float4 x = parts == 1 ? *reinterpret_cast<const float4*>(from) : remote_f32x4(from, p / STREAMS);
+                o[u].x = fmaf(x.x, f, o[u].x); o[u].y = fmaf(x.y, f, o[u].y); o[u].z = fmaf(x.z, f, o[u].z); o[u].w = fmaf(x.w, f, o[u].w);
             }
         }
-        bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + lane * PER;
-        unsigned packed[PER / 2];
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) packed[e / 2] = pack_bf16(o[e], o[e + 1]);
-        if ((reinterpret_cast<uintptr_t>(A.out) | (uintptr_t)(A.out_ld * 2)) % (PER * 2) == 0) {
-            if constexpr (PER == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
-            else *reinterpret_cast<unsigned*>(dst) = packed[0];
-        } else {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) dst[e] = __float2bfloat16_rn(o[e]);
+        for (int u = 0; u < BATCH; ++u) {
+            const int item = first + u * THREADS, i = item / QUADS, e = (item - i * QUADS) * 4;
+            if (i >= mine) continue;
+            const int row = part + i * parts, at = first_row + row, token = at / group;
+            if (bad_values) o[u] = with_bad_values<D>(A, S, place, o[u], token, e, t_first, all_tiles, lo_max);
+            bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
+            if (wide) {
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[u].x, o[u].y), pack_bf16(o[u].z, o[u].w));
+            } else {
+                dst[0] = __float2bfloat16_rn(o[u].x); dst[1] = __float2bfloat16_rn(o[u].y);
+                dst[2] = __float2bfloat16_rn(o[u].z); dst[3] = __float2bfloat16_rn(o[u].w);
+            }
         }
     }
     cluster_sync();                   // nobody leaves while others read its sums

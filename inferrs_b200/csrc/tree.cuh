@@ -58,7 +58,7 @@ __device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {
 }
 __device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
     float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)));
     return v;
 }
 __device__ __forceinline__ void cluster_sync() {
