@@ -12,11 +12,11 @@
 //
 // What bounds it is what comes from memory: a tile of 128 keys and values of 128 numbers is 64 KB, 2,900 cycles of an SM's share of the
 // copy bandwidth, and needs 1,100 cycles of products and as many of exponentials for every 128 rows.  Keys and values come through
-// a ring of tiles that two warps fill with cp.async, 16 bytes a lane: rows of a page lie anywhere, pages have any size, and where there is
-// no key zeros are written.  Ring places come in the order in which the products take them.
+// a ring of tiles that two warps fill, in the order in which the products take them: by TMA, a box for every page, and where pages
+// have an odd size with cp.async, 16 bytes a lane.  Where there is no key zeros are written.
 //
-// What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So in tiles that some row does
-// not see in full the warps that fill the ring look at the values that they brought, put zeros in the place of those that are
+// What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So the values of tiles that
+// some row does not see in full come with cp.async, and the warps that fill the ring look at what they brought, put zeros in the place of those that are
 // infinite or no numbers, and the rows that see such a value get it added at the end, from its page.
 #include "sm100.cuh"
 #include "tree.cuh"
@@ -29,7 +29,6 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
-constexpr int EACH = 4 / N_PRODUCERS;          // rows of a tile that a warp brings, in 32
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
 constexpr int MOST_PARTS = 8;
 constexpr int RANKED = 1024;          // requests that are put in order of their length
@@ -47,7 +46,7 @@ template <int D, int NQ> struct Shape {
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
     static constexpr int SMEM = 1024 + TILES + 256;
-    static_assert(SUMS + 4 * ROWS * 4 + 16 * NQ * ROWS * 4 <= TILES, "the sums, references, denominators and factors take the place of the tiles");
+    static_assert(SUMS + 4 * ROWS * 4 + 16 * ROWS * 4 + NQ * ROWS * 8 <= TILES, "the sums, references, denominators, factors and the rows' places take the place of the tiles");
     // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
     static_assert(SMEM > 116 * 1024 && SMEM <= 232448, "one CTA an SM");
 };
@@ -69,29 +68,29 @@ __device__ __forceinline__ void cp_arrive(unsigned bar) {
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Vectors of D numbers to rows 32 w .. 32 w + 31 of a tile; `index` is the place of this lane's row among the vectors at `base` (-1: zeros)
+// Vectors of D numbers to rows 16 g .. 16 g + 15 of a tile; lanes `from` .. `from` + 15 hold their places among the vectors at `base`
+// (-1: zeros)
 template <int D>
-__device__ __forceinline__ void load_rows(unsigned tile, const bf16* base, int index, int w, int lane) {
+__device__ __forceinline__ void load_rows(unsigned tile, const bf16* base, int index, int from, int g, int lane) {
     constexpr int CHUNKS = D / 8, STEP_ROWS = 32 / CHUNKS;
     const int c = lane % CHUNKS, sub = lane / CHUNKS;
-    const unsigned at = tile + (unsigned)((c >> 3) * (ROWS * 128) + w * 32 * 128);
+    const unsigned at = tile + (unsigned)((c >> 3) * (ROWS * 128) + g * 16 * 128);
 #pragma unroll
-    for (int i = 0; i < 32 / STEP_ROWS; ++i) {
-        const int r = i * STEP_ROWS + sub;
-        const int from = __shfl_sync(0xffffffffu, index, r);
-        cp16(at + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (long)(from < 0 ? 0 : from) * D + c * 8, from < 0 ? 0 : 16);
+    for (int i = 0; i < 16 / STEP_ROWS; ++i) {
+        const int r = i * STEP_ROWS + sub, place = __shfl_sync(0xffffffffu, index, from + r);
+        cp16(at + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (long)(place < 0 ? 0 : place) * D + c * 8, place < 0 ? 0 : 16);
     }
 }
 
-// Zeros for what is no finite number among what this lane has loaded with load_rows; true if there was any
+// Zeros for what is no finite number among what this lane has loaded with load_rows to the g-th 16 rows; true if there was any
 template <int D>
-__device__ __forceinline__ bool clean_rows(unsigned tile, int w, int lane) {
+__device__ __forceinline__ bool clean_rows(unsigned tile, int g, int lane) {
     constexpr int CHUNKS = D / 8, STEP_ROWS = 32 / CHUNKS;
     const int c = lane % CHUNKS, sub = lane / CHUNKS;
-    const unsigned at = tile + (unsigned)((c >> 3) * (ROWS * 128) + w * 32 * 128);
+    const unsigned at = tile + (unsigned)((c >> 3) * (ROWS * 128) + g * 16 * 128);
     bool any = false;
-#pragma unroll 4
-    for (int i = 0; i < 32 / STEP_ROWS; ++i) {
+#pragma unroll
+    for (int i = 0; i < 16 / STEP_ROWS; ++i) {
         const int r = i * STEP_ROWS + sub;
         const unsigned a = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         unsigned v[4];
@@ -247,7 +246,8 @@ __device__ __noinline__ float4 with_bad_values(const Args& A, const Span S, cons
 }
 
 template <int D, int NQ>
-__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ Args A, int parts, int ranked) {
+__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                          const __grid_constant__ Args A, int parts, int ranked, int box) {
     typedef Shape<D, NQ> Sh;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -258,6 +258,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const unsigned sq = smem_u32(smem), ring = sq + NQ * Sh::TILE;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if (threadIdx.x == PRODUCERS * 32 && box > 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
     int unit = blockIdx.x / parts;
     const int part = blockIdx.x - unit * parts;
     const int head = unit % A.n_kv;
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : (used + 31) / 32);
         }
         mbar_init(smem_u32(&sm.o_full), 1);
-        mbar_init(smem_u32(&sm.q_full), 32 * N_PRODUCERS);
+        mbar_init(smem_u32(&sm.q_full), 256);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int lo_min = A.span != 0 ? min(sm.lo_min, S.context) : 0, lo_max = A.span != 0 ? sm.lo_max : 0;
     const unsigned tmem = sm.tmem;
     const int t_first = lo_min / KEYS, all_tiles = (S.keys + KEYS - 1) / KEYS - t_first;
-    const int t_begin = t_first + (int)((long)all_tiles * part / parts), t_end = t_first + (int)((long)all_tiles * (part + 1) / parts);
+    const int t_begin = t_first + all_tiles * part / parts, t_end = t_first + all_tiles * (part + 1) / parts;      // (fewer than 2^24 tiles)
     const int n = t_end - t_begin;
     // tiles that each stream takes
     const int count0 = NQ == 2 ? n : (n + 1) / 2, count1 = NQ == 2 ? (rows > ROWS ? n : 0) : n / 2;
@@ -328,21 +332,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 
     if (warp >= PRODUCERS && warp < PRODUCERS + N_PRODUCERS) {
         const int w = warp - PRODUCERS;
-        const bf16* q = static_cast<const bf16*>(A.q);
-#pragma unroll
-        for (int g = 0; g < NQ; ++g) {
-#pragma unroll
-            for (int h = 0; h < EACH; ++h) {
-                const int r = g * ROWS + (w * EACH + h) * 32 + lane;
-                int index = -1;
-                if (r < rows) {
-                    const int at = first_row + r, token = at / group;
-                    index = (S.row0 + token) * A.n_heads + head * group + at - token * group;
-                }
-                load_rows<D>(sq + g * Sh::TILE, q, index, w * EACH + h, lane);
-            }
-        }
-        cp_arrive(smem_u32(&sm.q_full));
         // the ring's entries in the order of the products: with two sets of rows K0 V0 K1 V1 .., else K0 K1 V0 K2 V1 .. V(n-1)
         auto tile_of = [&](int e, bool& values) -> int {
             if (NQ == 2) {
@@ -353,13 +342,22 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (e == 2 * n - 1) return n - 1;
             return e == 0 ? 0 : (e & 1) ? (e + 1) >> 1 : (e - 2) >> 1;
         };
-        bool values = false;
-        int index[EACH], index_next[EACH];        // this lane's rows of the entry's tile, and of the next one's: the table's answer takes a while
-        auto look_up = [&](int e, int (&to)[EACH]) {
-            bool unused;
-            const int j = (t_begin + tile_of(e, unused)) * KEYS + w * EACH * 32 + lane;
-#pragma unroll
-            for (int h = 0; h < EACH; ++h) to[h] = e < 2 * n ? key_index(A, place, j + 32 * h) : -1;
+        const int beyond = A.n_pages * A.n_kv * A.page_size;          // a box that starts here is zeros
+        auto in_boxes = [&](int t, bool values) { return box > 0 && !(values && partly(t)); };
+        // An entry's places: of the box that this lane brings, or of two rows.  They are looked up an entry ahead: the table's answer takes a while.
+        int index[2], index_next[2];
+        auto look_up = [&](int e, int (&to)[2]) {
+            to[0] = to[1] = -1;
+            if (e >= 2 * n) return;
+            bool values;
+            const int t = t_begin + tile_of(e, values), j = t * KEYS;
+            if (in_boxes(t, values)) {
+                if (lane * box < KEYS) to[0] = key_index(A, place, j + lane * box);
+                if (to[0] < 0) to[0] = beyond;
+            } else {
+                to[0] = key_index(A, place, j + w * 64 + lane);
+                to[1] = key_index(A, place, j + w * 64 + 32 + lane);
+            }
         };
         look_up(0, index_next);
         int slot = 0, turn = 0;
@@ -367,21 +365,32 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (turn > 0 && !mbar_wait(smem_u32(&sm.empty[slot]), (turn - 1) & 1, 1)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int t = tile_of(e, values);
-#pragma unroll
-            for (int h = 0; h < EACH; ++h) index[h] = index_next[h];
+            bool values;
+            const int t = t_begin + tile_of(e, values);
+            index[0] = index_next[0];
+            index[1] = index_next[1];
             look_up(e + 1, index_next);
-            const unsigned dst = ring + slot * Sh::TILE;
-#pragma unroll
-            for (int h = 0; h < EACH; ++h) load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), index[h], w * EACH + h, lane);
-            if (values && partly(t_begin + t)) {
-                cp_wait_all();
-#pragma unroll
-                for (int h = 0; h < EACH; ++h)
-                    if (clean_rows<D>(dst, w * EACH + h, lane)) sm.bad_values = 1;
-                mbar_arrive(smem_u32(&sm.full[slot]));
+            const unsigned dst = ring + slot * Sh::TILE, full = smem_u32(&sm.full[slot]);
+            if (in_boxes(t, values)) {
+                // one warp a sub-tile of 64 numbers, one lane a box
+                if (lane == 0 && w < D / 64) mbar_expect_tx(full, ROWS * 128);
+                else mbar_arrive(full);
+                __syncwarp();
+                if (lane * box < KEYS && w < D / 64)
+                    tma_load_2d(dst + w * (ROWS * 128) + lane * box * 128, values ? &map_v : &map_k, w * 64, index[0], full);
             } else {
-                cp_arrive(smem_u32(&sm.full[slot]));
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), index[h >> 1], 16 * (h & 1), w * 4 + h, lane);
+                if (values && partly(t)) {
+                    cp_wait_all();
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        if (clean_rows<D>(dst, w * 4 + h, lane)) sm.bad_values = 1;
+                    mbar_arrive(full);
+                } else {
+                    cp_arrive(full);
+                }
             }
             if (++slot == Sh::STAGES) { slot = 0; ++turn; }
         }
@@ -453,6 +462,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         if (leader) umma_commit(smem_u32(&sm.o_full));
         __syncwarp();
     } else {
+        // the queries: 16 rows a warp and set
+#pragma unroll
+        for (int s = 0; s < NQ; ++s) {
+            const int r = s * ROWS + warp * 16 + (lane & 15), at = first_row + r, token = at / group;
+            const int index = r < rows ? (S.row0 + token) * A.n_heads + head * group + at - token * group : -1;
+            load_rows<D>(sq + s * Sh::TILE, static_cast<const bf16*>(A.q), index, 0, warp, lane);
+        }
+        cp_arrive(smem_u32(&sm.q_full));
         const int g = warp >> 2, r = (warp & 3) * 32 + lane;
         const int used = NQ == 2 ? min(rows - g * ROWS, ROWS) : rows, count = g ? count1 : count0;
         if ((warp & 3) * 32 < used) {
@@ -562,7 +579,35 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (!mbar_wait(smem_u32(&sm.o_full), 0, 6)) ok = false;       // every product is done: the tiles' memory is free
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            if (count > 0 && ok) {
+            if (NQ == 2 && parts == 1 && !sm.bad_values) {
+                // no other sums of these rows: they go out from here, a thread a row
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
+                const bool wide = ((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 16 == 0;
+#pragma unroll 1
+                for (int e = 0; e < D; e += 32) {
+                    unsigned x[32];
+                    tmem_ld32(o_at + e, x);
+                    if (!ok || !mine) continue;
+                    unsigned y[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float a = count > 0 ? __uint_as_float(x[2 * k]) * inv : 0.0f, b = count > 0 ? __uint_as_float(x[2 * k + 1]) * inv : 0.0f;
+                        y[k] = pack_bf16(a, b);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) {
+                        if (wide) {
+                            *reinterpret_cast<uint4*>(dst + e + 2 * k) = make_uint4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                        } else {
+                            for (int i = 0; i < 4; ++i) {
+                                reinterpret_cast<unsigned short*>(dst)[e + 2 * (k + i)] = (unsigned short)y[k + i];
+                                reinterpret_cast<unsigned short*>(dst)[e + 2 * (k + i) + 1] = (unsigned short)(y[k + i] >> 16);
+                            }
+                        }
+                    }
+                }
+            } else if (count > 0 && ok) {
                 float* row = sums + (g * ROWS + r) * Sh::OLD;
 #pragma unroll
                 for (int e = 0; e < D; e += 32) {
@@ -583,63 +628,63 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
-    // Join: CTA `part` writes every parts-th row.  First the factor of every sum of these rows, a thread a row, then the rows' numbers,
-    // four a thread: loads that wait for nothing but their factor.
+    if (NQ == 2 && parts == 1 && !sm.bad_values) return;
+    // Join: CTA `part` writes every parts-th row.  First the factor of every sum of these rows, as many lanes a row as it has sums, and
+    // where the row goes; then a warp a row, four at a time: loads that wait for nothing but their factor.
     constexpr int STREAMS = NQ == 2 ? 1 : 2, MOST_SUMS = STREAMS * MOST_PARTS;
     const int n_sums = parts * STREAMS, mine = rows > part ? (rows - part + parts - 1) / parts : 0;
     float* factors = part_l + 2 * ROWS;                           // [sum][this CTA's row]
-    bool bad_values = false;
-    for (int c = 0; c < parts; ++c) bad_values |= remote_i32(&sm.bad_values, c) != 0;
-    for (int i = tid; i < mine; i += THREADS) {
-        const int row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
-        float m[MOST_SUMS], l[MOST_SUMS], top = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int p = 0; p < MOST_SUMS; ++p) {
-            if (p >= n_sums) continue;
-            m[p] = remote_f32(&part_m[(g0 + p % STREAMS) * ROWS + r], p / STREAMS);
-            l[p] = remote_f32(&part_l[(g0 + p % STREAMS) * ROWS + r], p / STREAMS);
+    long* places = reinterpret_cast<long*>(factors + MOST_SUMS * NQ * ROWS);
+    int lanes = 1;
+    while (lanes < n_sums) lanes *= 2;
+    bool bad = false;
+    for (int first = warp * (32 / lanes); first < mine; first += THREADS / 32 * (32 / lanes)) {
+        const int i = first + lane / lanes, p = lane % lanes, row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
+        float m = -INFINITY, l = 0.0f;
+        if (i < mine && p < n_sums) {
+            const int at = (g0 + p % STREAMS) * ROWS + r;
+            m = remote_f32(part_m + at, p / STREAMS);
+            l = remote_f32(part_l + at, p / STREAMS);
+            bad |= remote_i32(&sm.bad_values, p / STREAMS) != 0;
         }
-#pragma unroll
-        for (int p = 0; p < MOST_SUMS; ++p)
-            if (p < n_sums) top = fmaxf(top, m[p]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int p = 0; p < MOST_SUMS; ++p) {
-            if (p >= n_sums) continue;
-            m[p] = l[p] == 0.0f ? 0.0f : ex2(m[p] - ref);         // (no sum is there where none of its keys is seen)
-            if (l[p] != 0.0f) total = fmaf(l[p], m[p], total);
+        float top = m;
+        for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float f = l == 0.0f ? 0.0f : ex2(m - (top == -INFINITY ? 0.0f : top));       // (no sum is there where none of its keys is seen)
+        float total = l == 0.0f ? 0.0f : l * f;
+        for (int o = lanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (i < mine && p < n_sums) factors[p * (NQ * ROWS) + i] = total == 0.0f ? 0.0f : f / total;
+        if (i < mine && p == 0) {
+            const int at = first_row + row, token = at / group;
+            places[i] = (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
         }
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-        for (int p = 0; p < MOST_SUMS; ++p)
-            if (p < n_sums) factors[p * (NQ * ROWS) + i] = m[p] * inv;
     }
-    __syncthreads();
-    constexpr int QUADS = D / 4, BATCH = 4;
-    const bool wide = (reinterpret_cast<uintptr_t>(A.out) | (uintptr_t)(A.out_ld * 2)) % 8 == 0;
-    for (int first = tid; first < mine * QUADS; first += THREADS * BATCH) {
+    const bool bad_values = __syncthreads_or(bad);
+    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, BATCH = 4;      // lanes of a row, rows of a warp's step
+    const bool wide = ((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0;
+    const int e = lane % LANES * 4;
+    for (int first = warp * STEP_ROWS + lane / LANES; first < mine; first += THREADS / 32 * STEP_ROWS * BATCH) {
         float4 o[BATCH];
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
             o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int item = first + u * THREADS, i = item / QUADS, e = (item - i * QUADS) * 4;
+            const int i = first + u * (THREADS / 32 * STEP_ROWS);
             if (i >= mine) continue;
-            const int row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
+            const int row = part + i * parts;                    // (with 256 rows the second stream's follow the first one's)
+            const float* from = sums + row * Sh::OLD + e;
             for (int p = 0; p < n_sums; ++p) {
                 const float f = factors[p * (NQ * ROWS) + i];
-                const float* from = sums + ((g0 + p % STREAMS) * ROWS + r) * Sh::OLD + e;
+                const float* x_at = from + p % STREAMS * (ROWS * Sh::OLD);
                 if (f == 0.0f) continue;
-                const float4 x = parts == 1 ? *reinterpret_cast<const float4*>(from) : remote_f32x4(from, p / STREAMS);
+                const float4 x = parts == 1 ? *reinterpret_cast<const float4*>(x_at) : remote_f32x4(x_at, p / STREAMS);
                 o[u].x = fmaf(x.x, f, o[u].x); o[u].y = fmaf(x.y, f, o[u].y); o[u].z = fmaf(x.z, f, o[u].z); o[u].w = fmaf(x.w, f, o[u].w);
             }
         }
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
-            const int item = first + u * THREADS, i = item / QUADS, e = (item - i * QUADS) * 4;
+            const int i = first + u * (THREADS / 32 * STEP_ROWS);
             if (i >= mine) continue;
-            const int row = part + i * parts, at = first_row + row, token = at / group;
-            if (bad_values) o[u] = with_bad_values<D>(A, S, place, o[u], token, e, t_first, all_tiles, lo_max);
-            bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
+            if (bad_values) o[u] = with_bad_values<D>(A, S, place, o[u], (first_row + part + i * parts) / group, e, t_first, all_tiles, lo_max);
+            bf16* dst = static_cast<bf16*>(A.out) + places[i] + e;
             if (wide) {
                 *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[u].x, o[u].y), pack_bf16(o[u].z, o[u].w));
             } else {
@@ -648,7 +693,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             }
         }
     }
-    cluster_sync();                   // nobody leaves while others read its sums
+    if (parts > 1) cluster_sync();    // nobody leaves while others read its sums
 }
 
 template <int D, int NQ>
@@ -661,8 +706,22 @@ static int launch(Args A, int max_tree, int max_keys, cudaStream_t stream) {
     long parts = 148 / pairs;
     if (parts > tiles) parts = tiles;
     parts = parts < 1 ? 1 : parts > MOST_PARTS ? MOST_PARTS : parts;
+    // boxes of a page's places, or of 128 in larger pages, where whole ones make a tile and start on eight rows
+    int box = A.page_shift >= 3 ? (A.page_size < KEYS ? A.page_size : KEYS) : 0;
+    CUtensorMap map_k = {}, map_v = {};
+    if (box > 0) {
+        const EncodeTiled encode = encode_fn();
+        const cuuint64_t dims[2] = {D, (cuuint64_t)A.n_pages * A.n_kv * A.page_size}, strides[1] = {D * 2};
+        const cuuint32_t sizes[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+        for (int values = 0; values < 2 && box > 0; ++values)
+            if (dims[1] == 0 || encode == nullptr
+                || encode(values ? &map_v : &map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(values ? A.v : A.k), dims, strides, sizes, steps,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+                       != CUDA_SUCCESS)
+                box = 0;
+    }
     const int ranked = A.n_requests > 1 && A.n_requests <= RANKED && pairs * parts > 148;
-    return launch_cluster(tree_kernel<D, NQ>, pairs * parts, (int)parts, THREADS, Shape<D, NQ>::SMEM, stream, A, (int)parts, ranked);
+    return launch_cluster(tree_kernel<D, NQ>, pairs * parts, (int)parts, THREADS, Shape<D, NQ>::SMEM, stream, map_k, map_v, A, (int)parts, ranked, box);
 }
 
 }  // namespace tree_tc
