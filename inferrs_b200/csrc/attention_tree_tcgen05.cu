@@ -88,27 +88,32 @@ __device__ __forceinline__ bool clean_rows(unsigned tile, int g, int lane) {
     constexpr int CHUNKS = D / 8, STEP_ROWS = 32 / CHUNKS;
     const int c = lane % CHUNKS, sub = lane / CHUNKS;
     const unsigned at = tile + (unsigned)((c >> 3) * (ROWS * 128) + g * 16 * 128);
-    bool any = false;
+    // bit 15 of a half carries over where all bits of its exponent are set
+    auto hits = [](unsigned v) { return ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+    unsigned v[16 / STEP_ROWS][4], any = 0;
 #pragma unroll
     for (int i = 0; i < 16 / STEP_ROWS; ++i) {
         const int r = i * STEP_ROWS + sub;
-        const unsigned a = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        unsigned v[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
-        unsigned hit = 0;      // bit 15 of a half carries over where all bits of its exponent are set
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i][0]), "=r"(v[i][1]), "=r"(v[i][2]), "=r"(v[i][3])
+                     : "r"(at + r * 128 + (((c & 7) ^ (r & 7)) << 4)) : "memory");
+    }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hit |= ((v[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-        if (hit) {
-            any = true;
-#pragma unroll
+    for (int i = 0; i < 16 / STEP_ROWS; ++i) any |= hits(v[i][0]) | hits(v[i][1]) | hits(v[i][2]) | hits(v[i][3]);
+    if (any) {
+#pragma unroll 1
+        for (int i = 0; i < 16 / STEP_ROWS; ++i) {
+            const int r = i * STEP_ROWS + sub;
+            const unsigned a = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
-                const unsigned h = ((v[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                v[k] &= ~((h >> 15) * 0xffffu);
+                unsigned x;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(a + 4 * k) : "memory");
+                x &= ~((hits(x) >> 15) * 0xffffu);
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(a + 4 * k), "r"(x) : "memory");
             }
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
         }
     }
-    return any;
+    return any != 0;
 }
 
 // Columns of this warp's lanes of tensor memory, and the wait for them: in one piece, since the compiler may put registers aside
@@ -286,6 +291,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int first_row = row_tile * (NQ * ROWS);
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (rows <= 0) return;            // (the whole cluster leaves)
+    // up to 64 rows stand twice among the 128: the second ones' threads take the second half of a tile's keys, and are joined like a part
+    const int copies = NQ == 1 && rows <= ROWS / 2 ? 2 : 1, block = ROWS / copies;
 
     if (tid == 0) {
         sm.lo_min = 0x7fffffff;
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         for (int g = 0; g < 2; ++g) {
             const int used = NQ == 2 ? rows - g * ROWS : rows;
             mbar_init(smem_u32(&sm.s_full[g]), 1);
-            mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : (used + 31) / 32);
+            mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : copies * ((used + 31) / 32));
         }
         mbar_init(smem_u32(&sm.o_full), 1);
         mbar_init(smem_u32(&sm.q_full), 256);
@@ -465,14 +472,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         // the queries: 16 rows a warp and set
 #pragma unroll
         for (int s = 0; s < NQ; ++s) {
-            const int r = s * ROWS + warp * 16 + (lane & 15), at = first_row + r, token = at / group;
+            const int r = s * ROWS + ((warp * 16 + (lane & 15)) & (block - 1)), at = first_row + r, token = at / group;
             const int index = r < rows ? (S.row0 + token) * A.n_heads + head * group + at - token * group : -1;
             load_rows<D>(sq + s * Sh::TILE, static_cast<const bf16*>(A.q), index, 0, warp, lane);
         }
         cp_arrive(smem_u32(&sm.q_full));
-        const int g = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int g = warp >> 2, line = (warp & 3) * 32 + lane, r = line & (block - 1);
+        const int copy = (warp & 3) * 32 / block;
         const int used = NQ == 2 ? min(rows - g * ROWS, ROWS) : rows, count = g ? count1 : count0;
-        if ((warp & 3) * 32 < used) {
+        if (((warp & 3) * 32 & (block - 1)) < used) {
             const bool mine = r < used;
             const int at = first_row + (NQ == 2 ? g * ROWS : 0) + (mine ? r : 0), token = at / group;
             const int lo = first_key(A, S, token);
@@ -502,9 +510,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 // 128 scores and what else a thread keeps are more than its registers: half of them stay, half come twice
                 auto hide = [&](auto& x, int at, int c) {
                     if (!plain) {
+                        const unsigned bits = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (!(see[c] >> k & 1u)) x[at + k] = 0xff800000u;
+                            if (!(bits >> k & 1u)) x[at + k] = 0xff800000u;
                     }
                 };
                 float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -515,18 +524,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                         for (int c = 0; c < 4; ++c)
                             top4[c] = max3(top4[c], __uint_as_float(x[at + k + 2 * c]), __uint_as_float(x[at + k + 2 * c + 1]));
                 };
-                unsigned x[64], y[32];
-                tmem_ld64(s_at, x);
-                hide(x, 0, 0);
-                hide(x, 32, 1);
+                unsigned x[64];
+                tmem_ld64(s_at + 64 * copy, x);
+                hide(x, 0, 2 * copy);
+                hide(x, 32, 2 * copy + 1);
                 look(x, 0);
                 look(x, 32);
-                tmem_ld32(s_at + 64, y);
-                hide(y, 0, 2);
-                look(y, 0);
-                tmem_ld32(s_at + 96, y);
-                hide(y, 0, 3);
-                look(y, 0);
+                if (copies == 1) {
+                    unsigned y[32];
+                    tmem_ld32(s_at + 64, y);
+                    hide(y, 0, 2);
+                    look(y, 0);
+                    tmem_ld32(s_at + 96, y);
+                    hide(y, 0, 3);
+                    look(y, 0);
+                }
                 const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * A.scale_log2;     // (the scale is positive)
                 const bool move = top > m + STEP || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
@@ -561,13 +573,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     }
                     tmem_st16(s_at + 16 * c, p);
                 };
-                weigh(x, 0);
-                weigh(x + 32, 1);
-                tmem_ld64(s_at + 64, x);
-                hide(x, 0, 2);
-                hide(x, 32, 3);
-                weigh(x, 2);
-                weigh(x + 32, 3);
+                weigh(x, 2 * copy);
+                weigh(x + 32, 2 * copy + 1);
+                if (copies == 1) {
+                    tmem_ld64(s_at + 64, x);
+                    hide(x, 0, 2);
+                    hide(x, 32, 3);
+                    weigh(x, 2);
+                    weigh(x + 32, 3);
+                } else {              // the other copy's keys
+                    unsigned zeros[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) zeros[k] = 0;
+                    tmem_st16(s_at + 32 * (copy ^ 1), zeros);
+                    tmem_st16(s_at + 32 * (copy ^ 1) + 16, zeros);
+                }
                 float a, b;
                 apart(add2(add[0], add[1]), a, b);
                 l += a + b;
@@ -608,7 +628,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     }
                 }
             } else if (count > 0 && ok) {
-                float* row = sums + (g * ROWS + r) * Sh::OLD;
+                float* row = sums + (g * ROWS + line) * Sh::OLD;
 #pragma unroll
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
@@ -618,8 +638,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                         *reinterpret_cast<uint4*>(row + e + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
                 }
             }
-            part_m[g * ROWS + r] = m;
-            part_l[g * ROWS + r] = l;
+            part_m[g * ROWS + line] = m;
+            part_l[g * ROWS + line] = l;
         }
         fence_before();
     }
@@ -630,36 +650,37 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     }
     if (NQ == 2 && parts == 1 && !sm.bad_values) return;
     // Join: CTA `part` writes every parts-th row.  First the factor of every sum of these rows, as many lanes a row as it has sums, and
-    // where the row goes; then a warp a row, four at a time: loads that wait for nothing but their factor.
-    constexpr int STREAMS = NQ == 2 ? 1 : 2, MOST_SUMS = STREAMS * MOST_PARTS;
-    const int n_sums = parts * STREAMS, mine = rows > part ? (rows - part + parts - 1) / parts : 0;
-    float* factors = part_l + 2 * ROWS;                           // [sum][this CTA's row]
-    long* places = reinterpret_cast<long*>(factors + MOST_SUMS * NQ * ROWS);
+    // where the row goes; then a warp a row, two at a time: loads that wait for nothing but their factor.
+    constexpr int STREAMS = NQ == 2 ? 1 : 2;
+    const int here = STREAMS * copies, here_log = (NQ == 1) + (copies == 2), n_sums = parts * here, mine = rows > part ? (rows - part + parts - 1) / parts : 0;
+    float* factors = part_l + 2 * ROWS;                           // [sum][this CTA's row], 16 * ROWS of them at most
+    long* places = reinterpret_cast<long*>(factors + 16 * ROWS);
+    const int row_stride = NQ * block;                            // (rows of one sum)
     int lanes = 1;
     while (lanes < n_sums) lanes *= 2;
     bool bad = false;
     for (int first = warp * (32 / lanes); first < mine; first += THREADS / 32 * (32 / lanes)) {
-        const int i = first + lane / lanes, p = lane % lanes, row = part + i * parts, g0 = NQ == 2 ? row / ROWS : 0, r = row - g0 * ROWS;
+        const int i = first + lane / lanes, p = lane & (lanes - 1), row = part + i * parts;
         float m = -INFINITY, l = 0.0f;
         if (i < mine && p < n_sums) {
-            const int at = (g0 + p % STREAMS) * ROWS + r;
-            m = remote_f32(part_m + at, p / STREAMS);
-            l = remote_f32(part_l + at, p / STREAMS);
-            bad |= remote_i32(&sm.bad_values, p / STREAMS) != 0;
+            const int at = (p & (here - 1)) * block + row;       // (a stream's copies lie one behind the other)
+            m = remote_f32(part_m + at, p >> here_log);
+            l = remote_f32(part_l + at, p >> here_log);
+            bad |= remote_i32(&sm.bad_values, p >> here_log) != 0;
         }
         float top = m;
         for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float f = l == 0.0f ? 0.0f : ex2(m - (top == -INFINITY ? 0.0f : top));       // (no sum is there where none of its keys is seen)
         float total = l == 0.0f ? 0.0f : l * f;
         for (int o = lanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (i < mine && p < n_sums) factors[p * (NQ * ROWS) + i] = total == 0.0f ? 0.0f : f / total;
+        if (i < mine && p < n_sums) factors[p * row_stride + i] = total == 0.0f ? 0.0f : f / total;
         if (i < mine && p == 0) {
             const int at = first_row + row, token = at / group;
             places[i] = (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
         }
     }
     const bool bad_values = __syncthreads_or(bad);
-    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, BATCH = 4;      // lanes of a row, rows of a warp's step
+    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, BATCH = 2;      // lanes of a row, rows of a warp's step
     const bool wide = ((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0;
     const int e = lane % LANES * 4;
     for (int first = warp * STEP_ROWS + lane / LANES; first < mine; first += THREADS / 32 * STEP_ROWS * BATCH) {
@@ -671,12 +692,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (i >= mine) continue;
             const int row = part + i * parts;                    // (with 256 rows the second stream's follow the first one's)
             const float* from = sums + row * Sh::OLD + e;
-            for (int p = 0; p < n_sums; ++p) {
-                const float f = factors[p * (NQ * ROWS) + i];
-                const float* x_at = from + p % STREAMS * (ROWS * Sh::OLD);
-                if (f == 0.0f) continue;
-                const float4 x = parts == 1 ? *reinterpret_cast<const float4*>(x_at) : remote_f32x4(x_at, p / STREAMS);
-                o[u].x = fmaf(x.x, f, o[u].x); o[u].y = fmaf(x.y, f, o[u].y); o[u].z = fmaf(x.z, f, o[u].z); o[u].w = fmaf(x.w, f, o[u].w);
+            // (a sum that is not there has the factor 0, and what stands in its place is not used)
+            for (int p0 = 0; p0 < n_sums; p0 += 4) {
+                float4 x[4];
+                float f[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int p = p0 + k < n_sums ? p0 + k : p0;
+                    const float* x_at = from + (p & (here - 1)) * (block * Sh::OLD);
+                    f[k] = p0 + k < n_sums ? factors[p * row_stride + i] : 0.0f;
+                    x[k] = remote_f32x4(x_at, p >> here_log);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (f[k] == 0.0f) continue;
+                    o[u].x = fmaf(x[k].x, f[k], o[u].x); o[u].y = fmaf(x[k].y, f[k], o[u].y);
+                    o[u].z = fmaf(x[k].z, f[k], o[u].z); o[u].w = fmaf(x[k].w, f[k], o[u].w);
+                }
             }
         }
 #pragma unroll
