@@ -46,7 +46,7 @@ template <int D, int NQ> struct Shape {
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
     static constexpr int SMEM = 1024 + TILES + 256;
-    static_assert(SUMS + 4 * ROWS * 4 + 16 * ROWS * 4 + NQ * ROWS * 8 <= TILES, "the sums, references, denominators, factors and the rows' places take the place of the tiles");
+    static_assert(SUMS + 6 * ROWS * 4 <= TILES, "the sums, references and denominators take the place of the tiles");
     // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
     static_assert(SMEM > 116 * 1024 && SMEM <= 232448, "one CTA an SM");
 };
@@ -643,89 +643,96 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         }
         fence_before();
     }
-    cluster_sync();
+    __syncthreads();
     if (warp == ISSUER) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
     if (NQ == 2 && parts == 1 && !sm.bad_values) return;
-    // Join: CTA `part` writes every parts-th row.  First the factor of every sum of these rows, as many lanes a row as it has sums, and
-    // where the row goes; then a warp a row, two at a time: loads that wait for nothing but their factor.
-    constexpr int STREAMS = NQ == 2 ? 1 : 2;
-    const int here = STREAMS * copies, here_log = (NQ == 1) + (copies == 2), n_sums = parts * here, mine = rows > part ? (rows - part + parts - 1) / parts : 0;
-    float* factors = part_l + 2 * ROWS;                           // [sum][this CTA's row], 16 * ROWS of them at most
-    long* places = reinterpret_cast<long*>(factors + 16 * ROWS);
-    const int row_stride = NQ * block;                            // (rows of one sum)
-    int lanes = 1;
-    while (lanes < n_sums) lanes *= 2;
-    bool bad = false;
-    for (int first = warp * (32 / lanes); first < mine; first += THREADS / 32 * (32 / lanes)) {
-        const int i = first + lane / lanes, p = lane & (lanes - 1), row = part + i * parts;
-        float m = -INFINITY, l = 0.0f;
-        if (i < mine && p < n_sums) {
-            const int at = (p & (here - 1)) * block + row;       // (a stream's copies lie one behind the other)
-            m = remote_f32(part_m + at, p >> here_log);
-            l = remote_f32(part_l + at, p >> here_log);
-            bad |= remote_i32(&sm.bad_values, p >> here_log) != 0;
+    // Join: first the sums that this CTA has of a row (of two streams, of two copies), then, a share of the rows for each, those of the
+    // cluster's CTAs.  Sixteen or 32 lanes a row, four numbers each; every sum comes in the same order whatever the grid.
+    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, PASS = THREADS / 32 * STEP_ROWS;
+    const int here = (NQ == 1 ? 2 : 1) * copies, line0 = warp * STEP_ROWS + lane / LANES, e = lane % LANES * 4;
+    auto write = [&](int row, float4 o, float total, bool bad_values) {
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        const int at = first_row + row, token = at / group;
+        if (bad_values) o = with_bad_values<D>(A, S, place, o, token, e, t_first, all_tiles, lo_max);
+        bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
+        if (((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+        } else {
+            dst[0] = __float2bfloat16_rn(o.x); dst[1] = __float2bfloat16_rn(o.y);
+            dst[2] = __float2bfloat16_rn(o.z); dst[3] = __float2bfloat16_rn(o.w);
         }
-        float top = m;
-        for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float f = l == 0.0f ? 0.0f : ex2(m - (top == -INFINITY ? 0.0f : top));       // (no sum is there where none of its keys is seen)
-        float total = l == 0.0f ? 0.0f : l * f;
-        for (int o = lanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (i < mine && p < n_sums) factors[p * row_stride + i] = total == 0.0f ? 0.0f : f / total;
-        if (i < mine && p == 0) {
-            const int at = first_row + row, token = at / group;
-            places[i] = (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
-        }
-    }
-    const bool bad_values = __syncthreads_or(bad);
-    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, BATCH = 2;      // lanes of a row, rows of a warp's step
-    const bool wide = ((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0;
-    const int e = lane % LANES * 4;
-    for (int first = warp * STEP_ROWS + lane / LANES; first < mine; first += THREADS / 32 * STEP_ROWS * BATCH) {
-        float4 o[BATCH];
+    };
+    // (a sum whose l is 0 is not there: what stands in its place is not used)
+    auto add = [](float4& o, const float4& x, float f) {
+        o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    };
+    float *own_m = here > 1 ? part_l + 2 * ROWS : part_m, *own_l = here > 1 ? own_m + ROWS : part_l;      // of what this CTA has of a row
+    if (here > 1 || parts == 1) {
+#pragma unroll 2
+        for (int row = line0; row < rows; row += PASS) {
+            float4 x[4], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float m[4], l[4], top = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-            o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int i = first + u * (THREADS / 32 * STEP_ROWS);
-            if (i >= mine) continue;
-            const int row = part + i * parts;                    // (with 256 rows the second stream's follow the first one's)
-            const float* from = sums + row * Sh::OLD + e;
-            // (a sum that is not there has the factor 0, and what stands in its place is not used)
-            for (int p0 = 0; p0 < n_sums; p0 += 4) {
-                float4 x[4];
-                float f[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int p = p0 + k < n_sums ? p0 + k : p0;
-                    const float* x_at = from + (p & (here - 1)) * (block * Sh::OLD);
-                    f[k] = p0 + k < n_sums ? factors[p * row_stride + i] : 0.0f;
-                    x[k] = remote_f32x4(x_at, p >> here_log);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (f[k] == 0.0f) continue;
-                    o[u].x = fmaf(x[k].x, f[k], o[u].x); o[u].y = fmaf(x[k].y, f[k], o[u].y);
-                    o[u].z = fmaf(x[k].z, f[k], o[u].z); o[u].w = fmaf(x[k].w, f[k], o[u].w);
-                }
+            for (int s = 0; s < 4; ++s) {
+                const int line = row + (s < here ? s : 0) * block;       // (a stream's copies lie one behind the other)
+                m[s] = s < here ? part_m[line] : -INFINITY;
+                l[s] = s < here ? part_l[line] : 0.0f;
+                x[s] = *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e);
+                top = fmaxf(top, m[s]);
             }
-        }
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-            const int i = first + u * (THREADS / 32 * STEP_ROWS);
-            if (i >= mine) continue;
-            if (bad_values) o[u] = with_bad_values<D>(A, S, place, o[u], (first_row + part + i * parts) / group, e, t_first, all_tiles, lo_max);
-            bf16* dst = static_cast<bf16*>(A.out) + places[i] + e;
-            if (wide) {
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[u].x, o[u].y), pack_bf16(o[u].z, o[u].w));
+            for (int s = 0; s < 4; ++s) {
+                if (l[s] == 0.0f) continue;
+                const float f = ex2(m[s] - (top == -INFINITY ? 0.0f : top));
+                total = fmaf(l[s], f, total);
+                add(o, x[s], f);
+            }
+            if (parts == 1) {
+                write(row, o, total, sm.bad_values != 0);
             } else {
-                dst[0] = __float2bfloat16_rn(o[u].x); dst[1] = __float2bfloat16_rn(o[u].y);
-                dst[2] = __float2bfloat16_rn(o[u].z); dst[3] = __float2bfloat16_rn(o[u].w);
+                *reinterpret_cast<float4*>(sums + row * Sh::OLD + e) = o;
+                if (e == 0) { own_m[row] = top; own_l[row] = total; }
             }
         }
     }
-    if (parts > 1) cluster_sync();    // nobody leaves while others read its sums
+    if (parts == 1) return;
+    cluster_sync();
+    bool bad_values = false;
+    for (int first = part + warp * STEP_ROWS * parts; first < rows; first += PASS * parts) {
+        const int mine = first + lane / LANES * parts, row = mine < rows ? mine : first;        // (the warp stays together)
+        float4 x[MOST_PARTS], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < MOST_PARTS; ++p)
+            if (p < parts) x[p] = remote_f32x4(sums + row * Sh::OLD + e, p);
+        const int p = lane % LANES;
+        float m = -INFINITY, l = 0.0f;
+        int bad = 0;
+        if (p < parts) {
+            m = remote_f32(own_m + row, p);
+            l = remote_f32(own_l + row, p);
+            bad = remote_i32(&sm.bad_values, p);
+        }
+        bad_values = __any_sync(0xffffffffu, bad);
+        float top = m;
+#pragma unroll
+        for (int k = MOST_PARTS / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float f = l == 0.0f ? 0.0f : ex2(m - (top == -INFINITY ? 0.0f : top));
+        float total = l == 0.0f ? 0.0f : l * f;
+#pragma unroll
+        for (int k = MOST_PARTS / 2; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+        total = __shfl_sync(0xffffffffu, total, 0, LANES);
+#pragma unroll
+        for (int p = 0; p < MOST_PARTS; ++p) {
+            const float fp = __shfl_sync(0xffffffffu, f, p, LANES);
+            if (p < parts && fp != 0.0f) add(o, x[p], fp);
+        }
+        if (mine < rows) write(row, o, total, bad_values);
+    }
+    cluster_sync();                   // nobody leaves while others read its sums
 }
 
 template <int D, int NQ>
