@@ -202,30 +202,48 @@ static int rows_of_type(Args A, int max_tree, int max_keys, cudaStream_t stream)
 
 }  // namespace tree
 
-IB_EXPORT int ib_paged_attention_tree(const void* call) {
-    using namespace tree;
-    const IbTreeAttention c = *static_cast<const IbTreeAttention*>(call);
+// A refusal, or IB_OK and the arguments as the kernels take them (n_rows 0: there is nothing to do)
+static int tree_args(const IbTreeAttention& c, tree::Args& A, int& max_tree, int& max_keys) {
     if (c.n_rows < 0 || c.n_requests < 0 || c.n_kv <= 0 || c.n_heads <= 0 || c.n_heads % c.n_kv || c.dim <= 0 || c.page_size <= 0 || c.max_tree < 0
         || c.max_pages < 0 || c.n_pages < 0 || c.words < 0)
         return IB_ERR_ARGUMENT;
     if (c.dim > 512 || c.n_rows * c.n_heads > 0x7fffffffL || c.n_requests > 0x7fffffffL || c.max_pages * c.page_size > 0x7fffffffL
         || c.n_pages * c.n_kv * c.page_size > 0x7fffffffL)
         return IB_ERR_UNSUPPORTED;
-    if (c.n_rows == 0 || c.n_requests == 0 || c.max_tree == 0) return IB_OK;
-    const long tree = c.max_tree < c.n_rows ? c.max_tree : c.n_rows;
-    Args A;
     A.q = c.q; A.k = c.k; A.v = c.v;
     A.table = c.table; A.q_start = c.q_start; A.context = c.context; A.positions = c.positions; A.seen = c.seen;
     A.out = c.out;
     A.out_ld = c.out_ld;
-    A.n_rows = (int)c.n_rows; A.n_requests = (int)c.n_requests; A.n_heads = (int)c.n_heads; A.n_kv = (int)c.n_kv; A.dim = (int)c.dim;
+    A.n_rows = c.n_requests && c.max_tree ? (int)c.n_rows : 0;
+    A.n_requests = (int)c.n_requests; A.n_heads = (int)c.n_heads; A.n_kv = (int)c.n_kv; A.dim = (int)c.dim;
     A.max_pages = (int)c.max_pages; A.page_size = (int)c.page_size; A.n_pages = (int)c.n_pages; A.words = (int)c.words; A.span = (int)c.span;
+    A.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctzl(c.page_size) : -1;
     A.scale_log2 = (float)(c.scale * 1.4426950408889634);
-    const int keys = (int)(c.max_keys < 0x7fffffffL ? c.max_keys : 0x7fffffffL);
-    A.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)c.page_size) : -1;
+    max_tree = (int)(c.max_tree < c.n_rows ? c.max_tree : c.n_rows);
+    max_keys = (int)(c.max_keys < 0x3fffffffL ? c.max_keys : 0x3fffffffL);
+    return IB_OK;
+}
+
+// the bytes of workspace that a call needs (0: none), or a refusal
+IB_EXPORT long ib_paged_attention_tree_workspace(const void* call) {
+    const IbTreeAttention c = *static_cast<const IbTreeAttention*>(call);
+    tree::Args A;
+    int max_tree, max_keys;
+    if (const int code = tree_args(c, A, max_tree, max_keys)) return code;
+    if (A.n_rows == 0 || c.f32) return 0;
+    const long bytes = ib_tree_tcgen05(A, max_tree, max_keys, nullptr, true, c.stream);
+    return bytes == IB_ERR_UNSUPPORTED ? 0 : bytes;
+}
+
+IB_EXPORT int ib_paged_attention_tree(const void* call) {
+    const IbTreeAttention c = *static_cast<const IbTreeAttention*>(call);
+    tree::Args A;
+    int max_tree, max_keys;
+    if (const int code = tree_args(c, A, max_tree, max_keys)) return code;
+    if (A.n_rows == 0) return IB_OK;
     if (!c.f32) {
-        const int code = ib_tree_tcgen05(A, (int)tree, keys, c.stream);
-        if (code != IB_ERR_UNSUPPORTED) return code;
+        const long code = ib_tree_tcgen05(A, max_tree, max_keys, c.workspace, false, c.stream);
+        if (code != IB_ERR_UNSUPPORTED) return (int)code;
     }
-    return c.f32 ? rows_of_type<float>(A, (int)tree, keys, c.stream) : rows_of_type<__nv_bfloat16>(A, (int)tree, keys, c.stream);
+    return c.f32 ? tree::rows_of_type<float>(A, max_tree, max_keys, c.stream) : tree::rows_of_type<__nv_bfloat16>(A, max_tree, max_keys, c.stream);
 }

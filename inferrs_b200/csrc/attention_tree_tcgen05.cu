@@ -31,6 +31,7 @@ constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
 constexpr int MOST_PARTS = 8;
+constexpr int SLICE = 16, MOST_SLICES = 64;
 constexpr int RANKED = 1024;          // requests that are put in order of their length
 
 __device__ int g_error = 0;
@@ -45,6 +46,7 @@ template <int D, int NQ> struct Shape {
     static constexpr int OLD = D + 4;                              // floats between two rows of the sums: 16-byte stores of 8 lanes meet no bank twice
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
+    static constexpr int SLICE_SUMS = 2 * ROWS * (D + 2) + 4;      // floats of a slice's sums in the scratch: o [D / 4][line][4], m and l [line][2], whether it met bad values
     static constexpr int SMEM = 1024 + TILES + 256;
     static_assert(SUMS + 6 * ROWS * 4 <= TILES, "the sums, references and denominators take the place of the tiles");
     // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
@@ -250,9 +252,42 @@ __device__ __noinline__ float4 with_bad_values(const Args& A, const Span S, cons
     return make_float4(v[0], v[1], v[2], v[3]);
 }
 
+// The sum (m, l, x) joins a row's (top, total, o).  (A sum whose l is 0 is not there: what stands in its place is not used.)
+__device__ __forceinline__ void join(float& top, float& total, float4& o, float m, float l, const float4& x) {
+    if (l == 0.0f) return;
+    const float to = fmaxf(top, m), ref = to == -INFINITY ? 0.0f : to, a = ex2(top - ref), b = ex2(m - ref);
+    total = fmaf(l, b, total * a);
+    o.x = fmaf(x.x, b, o.x * a); o.y = fmaf(x.y, b, o.y * a); o.z = fmaf(x.z, b, o.z * a); o.w = fmaf(x.w, b, o.w * a);
+    top = to;
+}
+
+// numbers e .. e + 3 of a row (counted token by token) to their place
+template <int D>
+__device__ __forceinline__ void write_row(const Args& A, const Span& S, const Place& place, int at, int head, int e, float4 o, float total, bool bad_values,
+                                          int t_first, int n_tiles, int lo_max) {
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const int group = A.n_heads / A.n_kv, token = at / group;
+    if (bad_values) o = with_bad_values<D>(A, S, place, o, token, e, t_first, n_tiles, lo_max);
+    bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
+    if (((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    } else {
+        dst[0] = __float2bfloat16_rn(o.x); dst[1] = __float2bfloat16_rn(o.y);
+        dst[2] = __float2bfloat16_rn(o.z); dst[3] = __float2bfloat16_rn(o.w);
+    }
+}
+
+// In how many slices a request's tiles are cut where there may be `most`: of SLICE tiles or more
+__device__ __forceinline__ int slices_of(int tiles, int most) {
+    const int n = (tiles + SLICE - 1) / SLICE;
+    return n < 1 ? 1 : n > most ? most : n;
+}
+
 template <int D, int NQ>
 __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                          const __grid_constant__ Args A, int parts, int ranked, int box) {
+                                                          const __grid_constant__ Args A, int slices, int ranked, int box,
+                                                          float* scratch) {
     typedef Shape<D, NQ> Sh;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -267,8 +302,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    int unit = blockIdx.x / parts;
-    const int part = blockIdx.x - unit * parts;
+    // `slices` CTAs for the same rows: a cluster whose CTAs take a part of the keys each, or, with a scratch, as many as the keys need
+    int unit = blockIdx.x / slices;
+    const int part = blockIdx.x - unit * slices;
     const int head = unit % A.n_kv;
     unit /= A.n_kv;
     const int row_tile = unit % A.tiles_of_rows;
@@ -291,6 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int first_row = row_tile * (NQ * ROWS);
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (rows <= 0) return;            // (the whole cluster leaves)
+    if (scratch != nullptr && part > 0 && (long)part * SLICE * KEYS >= S.keys) return;       // (there are no more slices than this)
     // up to 64 rows stand twice among the 128: the second ones' threads take the second half of a tile's keys, and are joined like a part
     const int copies = NQ == 1 && rows <= ROWS / 2 ? 2 : 1, block = ROWS / copies;
 
@@ -328,8 +365,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int lo_min = A.span != 0 ? min(sm.lo_min, S.context) : 0, lo_max = A.span != 0 ? sm.lo_max : 0;
     const unsigned tmem = sm.tmem;
     const int t_first = lo_min / KEYS, all_tiles = (S.keys + KEYS - 1) / KEYS - t_first;
+    const int parts = scratch != nullptr ? slices_of(all_tiles, slices) : slices;
     const int t_begin = t_first + all_tiles * part / parts, t_end = t_first + all_tiles * (part + 1) / parts;      // (fewer than 2^24 tiles)
-    const int n = t_end - t_begin;
+    const int n = part < parts ? t_end - t_begin : 0;
+    const bool none = part >= parts;  // (with a window that leaves fewer slices: no keys, no rows to write)
     // tiles that each stream takes
     const int count0 = NQ == 2 ? n : (n + 1) / 2, count1 = NQ == 2 ? (rows > ROWS ? n : 0) : n / 2;
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
@@ -599,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (!mbar_wait(smem_u32(&sm.o_full), 0, 6)) ok = false;       // every product is done: the tiles' memory is free
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            if (NQ == 2 && parts == 1 && !sm.bad_values) {
+            if (NQ == 2 && parts == 1 && !none && !sm.bad_values) {
                 // no other sums of these rows: they go out from here, a thread a row
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
@@ -627,6 +666,20 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                         }
                     }
                 }
+            } else if (scratch != nullptr && parts > 1) {
+                // the sums of a slice, numbers four by four, so that a warp's stores lie side by side
+                float* to = scratch + (((long)(req * A.tiles_of_rows + row_tile) * A.n_kv + head) * slices + part) * Sh::SLICE_SUMS;
+                const int all = g * ROWS + line;
+#pragma unroll 1
+                for (int e = 0; e < D && count > 0; e += 32) {
+                    unsigned x[32];
+                    tmem_ld32(o_at + e, x);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4*>(to + ((e + k) / 4 * (2 * ROWS) + all) * 4) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                }
+                *reinterpret_cast<float2*>(to + 2 * ROWS * D + 2 * all) = make_float2(m, ok ? l : NAN);
+                if (tid == 0) to[2 * ROWS * (D + 2)] = sm.bad_values ? 1.0f : 0.0f;
             } else if (count > 0 && ok) {
                 float* row = sums + (g * ROWS + line) * Sh::OLD;
 #pragma unroll
@@ -648,48 +701,25 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
-    if (NQ == 2 && parts == 1 && !sm.bad_values) return;
+    if (none || (scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
     // Join: first the sums that this CTA has of a row (of two streams, of two copies), then, a share of the rows for each, those of the
     // cluster's CTAs.  Sixteen or 32 lanes a row, four numbers each; every sum comes in the same order whatever the grid.
     constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, PASS = THREADS / 32 * STEP_ROWS;
     const int here = (NQ == 1 ? 2 : 1) * copies, line0 = warp * STEP_ROWS + lane / LANES, e = lane % LANES * 4;
-    auto write = [&](int row, float4 o, float total, bool bad_values) {
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        const int at = first_row + row, token = at / group;
-        if (bad_values) o = with_bad_values<D>(A, S, place, o, token, e, t_first, all_tiles, lo_max);
-        bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
-        if (((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-        } else {
-            dst[0] = __float2bfloat16_rn(o.x); dst[1] = __float2bfloat16_rn(o.y);
-            dst[2] = __float2bfloat16_rn(o.z); dst[3] = __float2bfloat16_rn(o.w);
-        }
-    };
-    // (a sum whose l is 0 is not there: what stands in its place is not used)
-    auto add = [](float4& o, const float4& x, float f) {
-        o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    auto write = [&](int row, const float4& o, float total, bool bad) {
+        write_row<D>(A, S, place, first_row + row, head, e, o, total, bad, t_first, all_tiles, lo_max);
     };
     float *own_m = here > 1 ? part_l + 2 * ROWS : part_m, *own_l = here > 1 ? own_m + ROWS : part_l;      // of what this CTA has of a row
+    // (loops as they stand: this code runs once, and what an unrolled one gains it loses to the instructions' own way from memory)
     if (here > 1 || parts == 1) {
-#pragma unroll 2
+#pragma unroll 1
         for (int row = line0; row < rows; row += PASS) {
-            float4 x[4], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float m[4], l[4], top = -INFINITY, total = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int line = row + (s < here ? s : 0) * block;       // (a stream's copies lie one behind the other)
-                m[s] = s < here ? part_m[line] : -INFINITY;
-                l[s] = s < here ? part_l[line] : 0.0f;
-                x[s] = *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e);
-                top = fmaxf(top, m[s]);
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                if (l[s] == 0.0f) continue;
-                const float f = ex2(m[s] - (top == -INFINITY ? 0.0f : top));
-                total = fmaf(l[s], f, total);
-                add(o, x[s], f);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+            for (int s = 0; s < here; ++s) {
+                const int line = row + s * block;                // (a stream's copies lie one behind the other)
+                join(top, total, o, part_m[line], part_l[line], *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e));
             }
             if (parts == 1) {
                 write(row, o, total, sm.bad_values != 0);
@@ -702,49 +732,86 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     if (parts == 1) return;
     cluster_sync();
     bool bad_values = false;
-    for (int first = part + warp * STEP_ROWS * parts; first < rows; first += PASS * parts) {
-        const int mine = first + lane / LANES * parts, row = mine < rows ? mine : first;        // (the warp stays together)
-        float4 x[MOST_PARTS], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int p = 0; p < MOST_PARTS; ++p)
-            if (p < parts) x[p] = remote_f32x4(sums + row * Sh::OLD + e, p);
-        const int p = lane % LANES;
-        float m = -INFINITY, l = 0.0f;
-        int bad = 0;
-        if (p < parts) {
-            m = remote_f32(own_m + row, p);
-            l = remote_f32(own_l + row, p);
-            bad = remote_i32(&sm.bad_values, p);
-        }
-        bad_values = __any_sync(0xffffffffu, bad);
-        float top = m;
-#pragma unroll
-        for (int k = MOST_PARTS / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        const float f = l == 0.0f ? 0.0f : ex2(m - (top == -INFINITY ? 0.0f : top));
-        float total = l == 0.0f ? 0.0f : l * f;
-#pragma unroll
-        for (int k = MOST_PARTS / 2; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
-        total = __shfl_sync(0xffffffffu, total, 0, LANES);
-#pragma unroll
-        for (int p = 0; p < MOST_PARTS; ++p) {
-            const float fp = __shfl_sync(0xffffffffu, f, p, LANES);
-            if (p < parts && fp != 0.0f) add(o, x[p], fp);
-        }
-        if (mine < rows) write(row, o, total, bad_values);
+    for (int p = 0; p < parts; ++p) bad_values |= remote_i32(&sm.bad_values, p) != 0;
+#pragma unroll 1
+    for (int row = part + line0 * parts; row < rows; row += PASS * parts) {
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+        for (int p = 0; p < parts; ++p)
+            join(top, total, o, remote_f32(own_m + row, p), remote_f32(own_l + row, p), remote_f32x4(sums + row * Sh::OLD + e, p));
+        write(row, o, total, bad_values);
     }
     cluster_sync();                   // nobody leaves while others read its sums
 }
 
+// The rows whose keys were cut into slices by CTAs that do not run together: their sums lie in memory, slice by slice.  A thread
+// takes 16 numbers of a row, a warp 32 rows.
 template <int D, int NQ>
-static int launch(Args A, int max_tree, int max_keys, cudaStream_t stream) {
-    static IbDeviceSet done;
-    if (const int code = ib_allow_dynamic_smem(done, tree_kernel<D, NQ>, Shape<D, NQ>::SMEM)) return code;
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args A, int slices, const float* __restrict__ scratch) {
+    constexpr int CHUNKS = NQ * ROWS * (D / 16) / 256, SUMS = Shape<D, NQ>::SLICE_SUMS;
+    const int unit = blockIdx.x / CHUNKS, at = blockIdx.x % CHUNKS * 256 + threadIdx.x, row = at % (NQ * ROWS), e = at / (NQ * ROWS) * 16;
+    const int head = unit % A.n_kv, row_tile = unit / A.n_kv % A.tiles_of_rows, req = unit / A.n_kv / A.tiles_of_rows;
+    const Span S = span_of(A, req);
+    const int group = A.n_heads / A.n_kv, first_row = row_tile * (NQ * ROWS);
+    const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
+    if (row >= rows) return;
+    int lo_min = 0, lo_max = 0;
+    if (A.span != 0) {
+        lo_min = 0x7fffffff;
+        for (int t = first_row / group; t <= (first_row + rows - 1) / group; ++t) {
+            const int lo = first_key(A, S, t);
+            lo_min = min(lo_min, lo);
+            lo_max = max(lo_max, lo);
+        }
+        lo_min = min(lo_min, S.context);
+    }
+    const int t_first = lo_min / KEYS, all_tiles = (S.keys + KEYS - 1) / KEYS - t_first, parts = slices_of(all_tiles, slices);
+    if (parts == 1) return;           // (its rows are written)
+    const int copies = NQ == 1 && rows <= ROWS / 2 ? 2 : 1, here = (NQ == 1 ? 2 : 1) * copies;
+    float4 o[4] = {};
+    float top = -INFINITY, total = 0.0f;
+    bool bad_values = false;
+    const float* from = scratch + (long)unit * slices * SUMS;
+    for (int p = 0; p < parts * here; ++p) {
+        const float* slice = from + (long)(p / here) * SUMS;
+        const int line = row + p % here * (ROWS / copies);
+        const float2 ml = *reinterpret_cast<const float2*>(slice + 2 * ROWS * D + 2 * line);
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(slice + ((e / 4 + k) * (2 * ROWS) + line) * 4);
+        bad_values |= slice[2 * ROWS * (D + 2)] != 0.0f;
+        const float before = top, sum = total;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            top = before;
+            total = sum;
+            join(top, total, o[k], ml.x, ml.y, x[k]);
+        }
+    }
+    const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) write_row<D>(A, S, place, first_row + row, head, e + 4 * k, o[k], total, bad_values, t_first, all_tiles, lo_max);
+}
+
+template <int D, int NQ>
+static long launch(Args A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream) {
     A.tiles_of_rows = (int)(((long)max_tree * (A.n_heads / A.n_kv) + NQ * ROWS - 1) / (NQ * ROWS));
     const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
     const int tiles = (max_keys + KEYS - 1) / KEYS;
-    long parts = 148 / pairs;
+    // One wave of CTAs: as many parts as there are SMs for, a cluster each.  More than that: requests differ in length, and clusters would wait
+    // for as many free SMs at once; slices of 16 tiles or more, the longest requests first, are joined by a kernel of their own.
+    const bool waves = 2 * pairs > 148 && tiles > 2 * SLICE;
+    long parts = waves ? (tiles + SLICE - 1) / SLICE : 148 / pairs;
     if (parts > tiles) parts = tiles;
-    parts = parts < 1 ? 1 : parts > MOST_PARTS ? MOST_PARTS : parts;
+    const long most = waves ? MOST_SLICES : MOST_PARTS;
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    const long needed = waves && parts > 1 ? pairs * parts * Shape<D, NQ>::SLICE_SUMS * 4 : 0;
+    if (ask) return needed;
+    float* scratch = needed ? static_cast<float*>(workspace) : nullptr;
+    if (needed && workspace == nullptr) return IB_ERR_ARGUMENT;
+    static IbDeviceSet done;
+    if (const int code = ib_allow_dynamic_smem(done, tree_kernel<D, NQ>, Shape<D, NQ>::SMEM)) return code;
     // boxes of a page's places, or of 128 in larger pages, where whole ones make a tile and start on eight rows
     int box = A.page_shift >= 3 ? (A.page_size < KEYS ? A.page_size : KEYS) : 0;
     CUtensorMap map_k = {}, map_v = {};
@@ -760,18 +827,24 @@ static int launch(Args A, int max_tree, int max_keys, cudaStream_t stream) {
                 box = 0;
     }
     const int ranked = A.n_requests > 1 && A.n_requests <= RANKED && pairs * parts > 148;
-    return launch_cluster(tree_kernel<D, NQ>, pairs * parts, (int)parts, THREADS, Shape<D, NQ>::SMEM, stream, map_k, map_v, A, (int)parts, ranked, box);
+    const int code = launch_cluster(tree_kernel<D, NQ>, pairs * parts, scratch ? 1 : (int)parts, THREADS, Shape<D, NQ>::SMEM, stream, map_k, map_v, A,
+                                    (int)parts, ranked, box, scratch);
+    if (code != IB_OK || scratch == nullptr) return code;
+    const long blocks = pairs * (NQ * ROWS * (D / 16) / 256);
+    if (blocks > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
+    tree_join_kernel<D, NQ><<<(unsigned)blocks, 256, 0, stream>>>(A, (int)parts, scratch);
+    return ib_launch_status();
 }
 
 }  // namespace tree_tc
 
-int ib_tree_tcgen05(tree::Args A, int max_tree, int max_keys, cudaStream_t stream) {
+long ib_tree_tcgen05(tree::Args A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream) {
     using namespace tree_tc;
     const uintptr_t at = reinterpret_cast<uintptr_t>(A.q) | reinterpret_cast<uintptr_t>(A.k) | reinterpret_cast<uintptr_t>(A.v);
     if ((A.dim != 64 && A.dim != 128) || at % 16 || !(A.scale_log2 > 0.0f)) return IB_ERR_UNSUPPORTED;
     const bool two = (long)max_tree * (A.n_heads / A.n_kv) > ROWS;
-    if (A.dim == 128) return two ? launch<128, 2>(A, max_tree, max_keys, stream) : launch<128, 1>(A, max_tree, max_keys, stream);
-    return two ? launch<64, 2>(A, max_tree, max_keys, stream) : launch<64, 1>(A, max_tree, max_keys, stream);
+    if (A.dim == 128) return two ? launch<128, 2>(A, max_tree, max_keys, workspace, ask, stream) : launch<128, 1>(A, max_tree, max_keys, workspace, ask, stream);
+    return two ? launch<64, 2>(A, max_tree, max_keys, workspace, ask, stream) : launch<64, 1>(A, max_tree, max_keys, workspace, ask, stream);
 }
 
 IB_EXPORT int ib_attention_tree_error(int reset) {

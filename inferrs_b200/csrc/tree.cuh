@@ -78,7 +78,7 @@ static int launch_cluster(void (*kernel)(KArgs...), long ctas, int cluster, int 
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
     return ib_launch_status();
 }
@@ -89,10 +89,12 @@ struct IbTreeAttention {
     const void *q, *k, *v;
     const int *table, *q_start, *context, *positions, *seen;
     void* out;
+    void* workspace;           // of ib_paged_attention_tree_workspace bytes
     cudaStream_t stream;
     long f32, out_ld, n_rows, n_requests, n_heads, n_kv, dim, max_pages, page_size, n_pages, words, span, max_tree, max_keys;
     double scale;
 };
 
-// heads of 64 or 128 numbers in bfloat16 (attention_tree_tcgen05.cu); IB_ERR_UNSUPPORTED where it does not take the call
-int ib_tree_tcgen05(tree::Args A, int max_tree, int max_keys, cudaStream_t stream);
+// Heads of 64 or 128 numbers in bfloat16 (attention_tree_tcgen05.cu): IB_ERR_UNSUPPORTED where it does not take the call; if
+// asked, the bytes of workspace that the call needs (nothing is launched), else what the launch says.
+long ib_tree_tcgen05(tree::Args A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream);

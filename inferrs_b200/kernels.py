@@ -2767,7 +2767,7 @@ _DRAFTS_LIB = None
 _DRAFTS_CALLS = ("ib_paged_attention_tree", "ib_copy_pages", "ib_keep_tokens", "ib_token_log_probs")
 # The calls take their arguments as one structure of 8-byte fields (IbTreeAttention, IbCopyPages, IbKeepTokens, IbTokenLogProbs
 # in csrc/), like those of the kernels in few bits.
-_TREE_CALL = struct.Struct("=24qd").pack
+_TREE_CALL = struct.Struct("=25qd").pack
 _COPY_CALL = struct.Struct("=8q").pack
 _KEEP_CALL = struct.Struct("=14q").pack
 _LOG_PROBS_CALL = struct.Struct("=13q").pack
@@ -2780,6 +2780,7 @@ def _drafts():
         for fn in _DRAFTS_CALLS:
             getattr(lib, fn).argtypes = [ctypes.c_char_p]
             getattr(lib, fn).restype = c_int
+        lib.ib_paged_attention_tree_workspace.argtypes, lib.ib_paged_attention_tree_workspace.restype = [ctypes.c_char_p], c_long
         lib.ib_attention_tree_error.argtypes, lib.ib_attention_tree_error.restype = [c_int], c_int
         lib.ib_attention_tree_error_async.argtypes, lib.ib_attention_tree_error_async.restype = [c_void_p, c_void_p], c_int
         _DRAFTS_LIB = lib
@@ -2840,14 +2841,22 @@ def paged_attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     if max_tree < 0 or max_kv_len < 0:
         raise KernelError(f"paged_attention_tree: at most {max_tree} drafted tokens over {max_kv_len} keys")
     stream = _one_device("paged_attention_tree", q, k_pages, v_pages, block_table, q_start, context, positions, seen, out)
-    code = _drafts().ib_paged_attention_tree(_TREE_CALL(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), context.data_ptr(),
-        0 if positions is None else positions.data_ptr(), seen.data_ptr(), out.data_ptr(), stream, act is _F32, out_ld, n, n_req, nh, nkv, d,
-        max_pages, page_size, n_pages, seen.shape[1], span, max_tree, max_kv_len, scale))
+    lib, workspace = _drafts(), None
+    pointers = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), context.data_ptr(),
+                0 if positions is None else positions.data_ptr(), seen.data_ptr(), out.data_ptr())
+    sizes = (stream, act is _F32, out_ld, n, n_req, nh, nkv, d, max_pages, page_size, n_pages, seen.shape[1], span, max_tree, max_kv_len, scale)
+    if max_kv_len > TREE_SLICE:
+        needed = lib.ib_paged_attention_tree_workspace(_TREE_CALL(*pointers, 0, *sizes))
+        if needed > 0:
+            workspace = torch.empty(needed, dtype=torch.uint8, device=q.device)
+    code = lib.ib_paged_attention_tree(_TREE_CALL(*pointers, 0 if workspace is None else workspace.data_ptr(), *sizes))
     if code == -1:
         raise KernelError(f"paged_attention_tree takes heads of up to 512 numbers and caches of fewer than 2^31 keys; got heads of {d}, "
                           f"{n_pages} pages of {page_size} places and {nkv} heads, requests of {max_pages} pages")
     _check(code, "paged_attention_tree")
+
+
+TREE_SLICE = 4096      # keys up to which the call above needs no workspace (2 SLICE tiles in csrc/attention_tree_tcgen05.cu)
 
 
 def attention_tree_error(reset: bool = True) -> int:

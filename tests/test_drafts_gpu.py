@@ -106,6 +106,26 @@ def test_tree_attention(case, span):
     check(c, attend(c, span), span)
 
 
+@pytest.mark.parametrize("d,heads,kv,most,span", [(128, 16, 8, 9, None), (64, 16, 8, 20, None), (128, 8, 8, 40, 4200), (128, 16, 8, 70, None),
+                                                  (64, 32, 8, 64, None), (128, 32, 8, 100, None)])
+def test_tree_attention_requests_of_very_different_length(d, heads, kv, most, span):
+    """More CTAs than run at once: the long requests' keys go in slices that are joined by a kernel of their own."""
+    rng = random.Random(most)
+    contexts = [0, 2300, 5, 4500, 130, 64, 7, 2000, 33, 1]
+    trees = [rng.randrange(1, most + 1) for _ in contexts]
+    trees[3], trees[4], trees[5] = most, 0, 1
+    c = drafted(21, contexts, trees, heads, kv, d, 16, BF, spare=2)
+    assert c["longest"] > kernels.TREE_SLICE and 2 * len(contexts) * kv > 148
+    out = attend(c, span)
+    check(c, out, span)
+    c["v"][c["table"][3, 4500 // 16], :, 4500 % 16] = float("nan")      # the first drafted token of the longest one
+    got = attend(c, span).float().view(out.shape[0], heads, d)
+    start = int(c["q_start"][3])
+    hit = torch.zeros(out.shape[0], dtype=torch.bool, device=DEV)
+    hit[start:start + most] = (c["seen"][start:start + most, 0] & 1).bool()
+    assert torch.isnan(got[hit]).all() and torch.isfinite(got[~hit]).all()
+
+
 def test_tree_attention_many_requests_and_splits():
     rng = random.Random(3)
     contexts = [rng.choice([0, 1, 17, 200, 900]) for _ in range(40)]
