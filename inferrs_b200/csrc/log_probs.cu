@@ -8,17 +8,19 @@
 //
 // The logits are read once.  The k most likely tokens come out of the same pass: a key is the logit's bits made ascending, the
 // place's complement below them (of equal logits the lower place is ahead).  A bound that at least k keys of the row reach is
-// kept; what passes it is noted in shared memory, and now and then the k best of the noted ones give a higher bound.  The first
-// bound is the k-th largest of 64 groups' largest keys; expected are k to 2 k notes from the first 8,192 logits and k more
+// kept; what passes it is noted in shared memory, and behind chunks 2, 5, 11, 23 .. the k best of the noted ones give a higher bound.  The first
+// bound is the k-th largest of 64 groups' largest keys; expected are k to 2 k notes from the first 4,096 logits and k more
 // for every doubling behind them.
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace lp {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;         // that look at logits; one warp more fetches them
+constexpr int RING = 4096;           // 16-byte vectors that may be on their way or waiting
 constexpr int MAX_TOP = 32;
 constexpr int NOTES = 1024;          // room for noted keys
-constexpr int GROUPS = 64;           // groups of 8 threads whose largest keys give the first bound
+constexpr int GROUPS = 64;           // groups of 4 threads whose largest keys give the first bound
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOWEST = -200.0f;    // e^-200 is 0 in 32 bits, and 0 times it is 0
 
@@ -43,13 +45,27 @@ struct Board {
 };
 
 struct Shared {
+    uint4 ring[RING];
+    unsigned long long full[8], empty[8];
     Board board;
     u64 notes[NOTES];
     u64 groups[GROUPS];
     u64 bound;
-    int n_notes;
+    int n_notes, lost;        // lost: a note did not fit
     float red[3][THREADS / 32];
 };
+
+__device__ int g_error = 0;
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int code) { return sm100::mbar_wait_bounded(bar, parity, &g_error, code); }
+
+// the threads that look at logits meet; whether any of them has `mine`
+__device__ __forceinline__ bool meet(bool mine) {
+    int any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((int)mine) : "memory");
+    return any != 0;
+}
+static_assert(THREADS == 256, "");
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
@@ -95,6 +111,7 @@ __device__ __forceinline__ void rank_notes(const u64* notes, int n, int k, u64* 
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const u64 mine = notes[i];
         int ahead = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) ahead += notes[j] > mine;
         if (ahead < k) best[ahead] = mine;
     }
@@ -111,7 +128,7 @@ struct Args {
     int rows, vocab, given, top;
 };
 
-template <typename T> struct Wide;
+template <typename T> struct Wide;      // logits of a vector, vectors of a thread's share of a chunk
 template <> struct Wide<float> {
     static constexpr int N = 4, VECTORS = 4;
     static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
@@ -131,37 +148,98 @@ template <> struct Wide<__nv_bfloat16> {
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int cluster) {
+__global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A, int cluster) {
     constexpr int N = Wide<T>::N, VECTORS = Wide<T>::VECTORS, EACH = N * VECTORS;      // logits that a thread takes at once
-    __shared__ Shared sh;
+    constexpr int CHUNK = THREADS * VECTORS, STAGES = RING / CHUNK;
+    static_assert(STAGES <= 8, "");
+    extern __shared__ __align__(128) unsigned char raw[];
+    Shared& sh = *reinterpret_cast<Shared*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / cluster;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     const T* x = static_cast<const T*>(A.logits) + (long)row * A.ld;
-    // this CTA's stretch [lo, hi), cut on whole vectors counted from the 16-byte boundary at or before the row's start
+    // this CTA's stretch of the row: vectors v_lo .. v_hi, counted from the 16-byte boundary at or before the row's start
     const int skew = (int)(((unsigned long long)x / sizeof(T)) % N);
     const int vectors = (A.vocab + skew + N - 1) / N;
     const int v_lo = (int)((long)vectors * rank / cluster), v_hi = (int)((long)vectors * (rank + 1) / cluster);
-    const int hi = min(A.vocab, v_hi * N - skew), lo = max(0, v_lo * N - skew);
+    // the whole ones among them; at the row's ends a vector may hold what is not the row's
+    const int w_lo = v_lo == 0 && skew ? 1 : v_lo, w_hi = min(v_hi, (A.vocab + skew) / N);
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            sm100::mbar_init(sm100::smem_u32(&sh.full[s]), 1);
+            sm100::mbar_init(sm100::smem_u32(&sh.empty[s]), THREADS / 32);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sh.n_notes = sh.lost = 0;
+    }
+    __syncthreads();
 
     float m = -INFINITY, s = 0.0f, w = 0.0f;
     u64 bound = 0;                    // keys below it are not noted
     float bound_v = -INFINITY;
-    if (TOP && tid == 0) sh.n_notes = 0;
     int round = 0, next_look = 2;
-    for (int v0 = v_lo; v0 < v_hi; v0 += THREADS * VECTORS, ++round) {
+    bool ok = true;
+    auto note = [&](u64 key) {
+        if (key < bound) return;
+        const int at = atomicAdd(&sh.n_notes, 1);
+        if (at < NOTES) sh.notes[at] = key;
+        else sh.lost = 1;
+    };
+    // the k best of what is noted take its place and give the next bound (the threads have met)
+    auto prune = [&]() {
+        const int n = min(sh.n_notes, NOTES);
+        rank_notes(sh.notes, n, A.top, sh.board.best);
+        meet(false);
+        const int left = min(n, A.top);
+        if (tid < left) sh.notes[tid] = sh.board.best[tid];
+        if (tid == 0) sh.n_notes = left;
+        if (left == A.top) {
+            bound = max(bound, sh.board.best[A.top - 1]);
+            bound_v = bound ? value_of(bound) : -INFINITY;
+        }
+        meet(false);
+    };
+    // the given tokens' logits, on their way meanwhile
+    float given = -INFINITY;
+    if (rank == 0 && tid < A.given) {
+        const int t = A.tokens[(long)row * A.given + tid];
+        if (t >= 0 && t < A.vocab) given = fmaxf(ib_to_float(x[t]), -INFINITY);
+    }
+    if (warp == THREADS / 32) {       // the logits come as bulk copies: three CTAs of an SM have up to 192 KB on their way
+        if (lane == 0) {
+            for (int v0 = v_lo; v0 < v_hi && ok; v0 += CHUNK, ++round) {
+                const int stage = round % STAGES;
+                if (round >= STAGES) ok = mbar_wait(sm100::smem_u32(&sh.empty[stage]), (round / STAGES - 1) & 1, 1);
+                if (!ok) break;
+                const int from = max(v0, w_lo), to = min(v0 + CHUNK, w_hi);
+                const unsigned bytes = to > from ? (unsigned)(to - from) * 16u : 0u, full = sm100::smem_u32(&sh.full[stage]);
+                sm100::mbar_expect_tx(full, bytes);
+                if (bytes)
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                 ::"r"(sm100::smem_u32(&sh.ring[stage * CHUNK + from - v0])), "l"(x + ((long)from * N - skew)), "r"(bytes), "r"(full) : "memory");
+            }
+        }
+        __syncwarp();
+    } else
+    for (int v0 = v_lo; v0 < v_hi; v0 += CHUNK, ++round) {
+        const int stage = round % STAGES;
+        if (ok && !mbar_wait(sm100::smem_u32(&sh.full[stage]), (round / STAGES) & 1, 2)) ok = false;
         float e[EACH];
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) {
-            const int at = (v0 + i * THREADS + tid) * N - skew;
-            if (at >= lo && at + N <= hi) {
-                const uint4 v = __ldcs(reinterpret_cast<const uint4*>(x + at));
-                Wide<T>::unpack(v, e + i * N);
+            const int v = v0 + i * THREADS + tid;
+            if (v >= w_lo && v < w_hi) {
+                Wide<T>::unpack(sh.ring[stage * CHUNK + i * THREADS + tid], e + i * N);
             } else {
 #pragma unroll
-                for (int c = 0; c < N; ++c) e[i * N + c] = at + c >= lo && at + c < hi ? ib_to_float(x[at + c]) : NAN;
+                for (int c = 0; c < N; ++c) {
+                    const int at = v * N - skew + c;
+                    e[i * N + c] = v < v_hi && at >= 0 && at < A.vocab ? ib_to_float(x[at]) : NAN;
+                }
             }
         }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&sh.empty[stage]));
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) top = fmaxf(top, e[i]);
@@ -185,56 +263,52 @@ __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int
                 for (int i = 0; i < EACH; ++i)
                     if (e[i] == e[i]) best = max(best, key_of(e[i], place(i)));
 #pragma unroll
-                for (int o = 4; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-                if ((tid & 7) == 0) sh.groups[tid >> 3] = best;
-                __syncthreads();
+                for (int o = 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+                if ((tid & 3) == 0) sh.groups[tid >> 2] = best;
+                meet(false);
                 if (tid < GROUPS) {
                     const u64 mine = sh.groups[tid];
                     int ahead = 0;
+#pragma unroll 8
                     for (int j = 0; j < GROUPS; ++j) ahead += sh.groups[j] > mine || (sh.groups[j] == mine && j < tid);
                     if (ahead == A.top - 1) sh.bound = mine;       // (0 where fewer groups hold a number)
                 }
-                __syncthreads();
+                meet(false);
                 bound = sh.bound;
                 bound_v = bound ? value_of(bound) : -INFINITY;
             }
-            unsigned todo = 0;
             if (top >= bound_v) {
 #pragma unroll
                 for (int i = 0; i < EACH; ++i)
-                    if (e[i] >= bound_v && key_of(e[i], place(i)) >= bound) todo |= 1u << i;
+                    if (e[i] >= bound_v) note(key_of(e[i], place(i)));
             }
-            for (;;) {
-                bool full = false;
-                if (todo) {
-#pragma unroll
-                    for (int i = 0; i < EACH; ++i) {
-                        if (!(todo >> i & 1) || full) continue;
-                        const u64 key = key_of(e[i], place(i));
-                        if (key >= bound) {
-                            const int at = atomicAdd(&sh.n_notes, 1);
-                            if (at < NOTES) sh.notes[at] = key; else full = true;
-                        }
-                        if (!full) todo &= ~(1u << i);
-                    }
-                }
-                const bool again = __syncthreads_or(full);
-                if (!again && round < next_look) break;
-                // the k best of what is noted take its place and give the next bound
-                const int n = min(sh.n_notes, NOTES);
-                rank_notes(sh.notes, n, A.top, sh.board.best);
-                __syncthreads();
-                const int left = min(n, A.top);
-                if (tid < left) sh.notes[tid] = sh.board.best[tid];
-                if (tid == 0) sh.n_notes = left;
-                if (left == A.top) {
-                    bound = max(bound, sh.board.best[A.top - 1]);
-                    bound_v = bound ? value_of(bound) : -INFINITY;
-                }
-                __syncthreads();
-                if (!again) { next_look = 2 * round + 1; break; }
+            if (round == next_look) {
+                meet(false);
+                prune();
+                next_look = 2 * round + 1;
             }
         }
+    }
+    __syncthreads();
+    if (TOP && sh.lost) {
+        // More notes than there is room for (logits that ascend do that): from the best bound so far on, the stretch again, a few at a time,
+        // with a look whenever the room could run out.  Nothing is lost: of what does not fit the k best are kept each time.
+        if (tid < THREADS) {
+            meet(false);
+            prune();
+            if (tid == 0) sh.n_notes = 0;
+            meet(false);
+            const int lo = max(0, v_lo * N - skew), hi = min(A.vocab, v_hi * N - skew);
+            for (int at0 = lo; at0 < hi; at0 += THREADS) {
+                const float v = at0 + tid < hi ? ib_to_float(x[at0 + tid]) : NAN;
+                if (v >= bound_v) note(key_of(v, at0 + tid));
+                meet(false);
+                const bool look = sh.n_notes > NOTES - THREADS;
+                meet(false);
+                if (look) prune();
+            }
+        }
+        __syncthreads();
     }
 
     // the CTA's m, S and W
@@ -242,9 +316,9 @@ __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int
     move_reference(m, top, s, w);
     s = ib_warp_sum(s);
     w = ib_warp_sum(w);
-    if (lane == 0) { sh.red[0][warp] = top; sh.red[1][warp] = s; sh.red[2][warp] = w; }
+    if (lane == 0 && warp < THREADS / 32) { sh.red[0][warp] = top; sh.red[1][warp] = ok ? s : NAN; sh.red[2][warp] = w; }
     __syncthreads();
-    if (TOP) rank_notes(sh.notes, min(sh.n_notes, NOTES), A.top, sh.board.best);
+    if (TOP && tid < THREADS) rank_notes(sh.notes, min(sh.n_notes, NOTES), A.top, sh.board.best);
     if (warp == 0) {
         const int n = THREADS / 32;
         float m1 = lane < n ? sh.red[0][lane] : -INFINITY, s1 = lane < n ? sh.red[1][lane] : 0.0f, w1 = lane < n ? sh.red[2][lane] : 0.0f;
@@ -271,26 +345,28 @@ __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int
         const bool none = !(fabsf(all) < INFINITY);
         const float log_total = none ? NAN : logf(total);
         if (tid == 0 && A.entropy) A.entropy[row] = log_total - weighed / total;
-        for (int i = tid; i < A.given; i += THREADS) {
-            const int t = A.tokens[(long)row * A.given + i];
-            float v = -INFINITY;
-            if (t >= 0 && t < A.vocab) v = fmaxf(ib_to_float(x[t]), -INFINITY);
+        for (int i = tid; i < A.given; i += THREADS + 32) {
+            float v = given;
+            if (i != tid) {
+                const int t = A.tokens[(long)row * A.given + i];
+                v = t >= 0 && t < A.vocab ? fmaxf(ib_to_float(x[t]), -INFINITY) : -INFINITY;
+            }
             A.log_probs[(long)row * A.given + i] = (v - all) - log_total;
         }
         if constexpr (TOP) {
             if (cluster > 1) {      // the best of the CTAs' best
+                const int all_keys = cluster * A.top;
                 u64 mine = 0;
-                int of = 0;
-                if (tid < cluster * MAX_TOP) {
-                    of = tid / MAX_TOP;
-                    const int i = tid % MAX_TOP;
+                if (tid < all_keys) {
+                    const int of = tid / A.top, i = tid - of * A.top;
                     if (i < remote_i32(&sh.board.n, of)) mine = remote_u64(&sh.board.best[i], of);
                     sh.notes[tid] = mine;
                 }
                 __syncthreads();
-                if (tid < cluster * MAX_TOP && mine) {
+                if (mine) {
                     int ahead = 0;
-                    for (int j = 0; j < cluster * MAX_TOP; ++j) ahead += sh.notes[j] > mine;
+#pragma unroll 8
+                    for (int j = 0; j < all_keys; ++j) ahead += sh.notes[j] > mine;
                     if (ahead < A.top) {
                         A.top_ids[(long)row * A.top + ahead] = place_of(mine);
                         A.top_log_probs[(long)row * A.top + ahead] = (value_of(mine) - all) - log_total;
@@ -298,12 +374,12 @@ __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int
                 }
                 int have = 0;
                 for (int c = 0; c < cluster; ++c) have += remote_i32(&sh.board.n, c);
-                for (int i = have + tid; i < A.top; i += THREADS) {
+                for (int i = have + tid; i < A.top; i += THREADS + 32) {
                     A.top_ids[(long)row * A.top + i] = -1;
                     A.top_log_probs[(long)row * A.top + i] = -INFINITY;
                 }
             } else {
-                for (int i = tid; i < A.top; i += THREADS) {
+                for (int i = tid; i < A.top; i += THREADS + 32) {
                     const bool some = i < sh.board.n;
                     A.top_ids[(long)row * A.top + i] = some ? place_of(sh.board.best[i]) : -1;
                     A.top_log_probs[(long)row * A.top + i] = some ? (value_of(sh.board.best[i]) - all) - log_total : -INFINITY;
@@ -316,9 +392,12 @@ __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const Args A, int
 
 template <typename T, bool TOP>
 static int launch(const Args& a, int cluster, cudaStream_t stream) {
+    static IbDeviceSet done;
+    if (const int code = ib_allow_dynamic_smem(done, log_probs_kernel<T, TOP>, sizeof(Shared))) return code;
     cudaLaunchConfig_t cfg = {};
+    cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.gridDim = dim3((unsigned)(a.rows * cluster));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(THREADS + 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -349,9 +428,23 @@ IB_EXPORT int ib_token_log_probs(const void* call) {
     if (c.top > MAX_TOP || c.vocab > 0x40000000L || c.rows > 0x7fffffffL / MAX_CLUSTER || c.given > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
     if (c.rows == 0) return IB_OK;
     const Args a{c.logits, c.tokens, c.log_probs, c.entropy, c.top_ids, c.top_log_probs, c.ld, (int)c.rows, (int)c.vocab, (int)c.given, (int)c.top};
-    // as many CTAs for a row as the machine has room for (two on each of 148 SMs), each with at least 4,096 logits
+    // as many CTAs for a row as the machine has room for (three on each of 148 SMs), each with at least a chunk's logits
     int cluster = 1;
-    while (cluster < MAX_CLUSTER && c.rows * cluster * 2 <= 296 && c.vocab >= 4096L * cluster * 2) cluster *= 2;
+    while (cluster < MAX_CLUSTER && c.rows * cluster * 2 <= 444 && c.vocab >= 4096L * cluster * 2) cluster *= 2;
     if (c.f32) return c.top ? launch<float, true>(a, cluster, c.stream) : launch<float, false>(a, cluster, c.stream);
     return c.top ? launch<__nv_bfloat16, true>(a, cluster, c.stream) : launch<__nv_bfloat16, false>(a, cluster, c.stream);
+}
+
+IB_EXPORT int ib_log_probs_error(int reset) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, lp::g_error, sizeof(int));
+    if (e != cudaSuccess) return -(int)e;
+    if (reset && v != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(lp::g_error, &zero, sizeof(int));
+    }
+    return v;
+}
+IB_EXPORT int ib_log_probs_error_async(int* out, cudaStream_t stream) {
+    return (int)cudaMemcpyFromSymbolAsync(out, lp::g_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
 }

@@ -2781,8 +2781,9 @@ def _drafts():
             getattr(lib, fn).argtypes = [ctypes.c_char_p]
             getattr(lib, fn).restype = c_int
         lib.ib_paged_attention_tree_workspace.argtypes, lib.ib_paged_attention_tree_workspace.restype = [ctypes.c_char_p], c_long
-        lib.ib_attention_tree_error.argtypes, lib.ib_attention_tree_error.restype = [c_int], c_int
-        lib.ib_attention_tree_error_async.argtypes, lib.ib_attention_tree_error_async.restype = [c_void_p, c_void_p], c_int
+        for fn in ("ib_attention_tree_error", "ib_log_probs_error"):
+            getattr(lib, fn).argtypes, getattr(lib, fn).restype = [c_int], c_int
+            getattr(lib, fn + "_async").argtypes, getattr(lib, fn + "_async").restype = [c_void_p, c_void_p], c_int
         _DRAFTS_LIB = lib
     return _DRAFTS_LIB
 
@@ -2957,6 +2958,11 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, log_probs: torch
         tokens.shape[1], top)), "token_log_probs")
 
 
+def log_probs_error(reset: bool = True) -> int:
+    """0, or the code of the first bounded wait that ran out in the kernel above (synchronises)."""
+    return _drafts().ib_log_probs_error(int(reset))
+
+
 # ---- the kernels' error words, all of them ------------------------------------------------------------------
 # A bounded wait that ran out, or a row whose position lay outside the rotation tables, leaves a code in a word
 # on the device.  The functions above read one word each and wait for the device; these read all of them the way
@@ -2965,13 +2971,13 @@ ERROR_WORDS = ("a row's position outside the rotation tables", "prefill attentio
                "prefill attention (two query tiles)", "decode attention", "matrix product (tcgen05)",
                "chain of matrix products")
 # ... and, where a program has used them, behind those of the kernels in few bits
-DRAFTS_WORDS = ("attention of drafted tokens",)
+DRAFTS_WORDS = ("attention of drafted tokens", "log probabilities")
 
 
 def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
     """Ask for every error word of the kernel libraries, in the order of ``ERROR_WORDS``, to be copied into ``host``
-    (pinned int32, at least ``len(ERROR_WORDS)`` long; with room for them, those of the kernels in few bits and of the drafted
-    tokens' attention follow) behind
+    (pinned int32, at least ``len(ERROR_WORDS)`` long; with room for them, those of the kernels in few bits and for drafted
+    tokens follow) behind
     the work that the current stream holds.  The caller
     records an event after this call and reads ``host`` once the event has come."""
     if host.dtype != torch.int32 or host.numel() < len(ERROR_WORDS) or not host.is_pinned():
@@ -2993,12 +2999,13 @@ def error_words_async(host: torch.Tensor, act_dtype: torch.dtype):
                 if code != 0:
                     raise KernelError(f"error_words_async: CUDA error {code}")
     behind = len(ERROR_WORDS) + len(FEW_BITS_WORDS)
-    if host.numel() >= behind + len(DRAFTS_WORDS):       # and that of the drafted tokens' attention
-        host[behind] = 0
+    if host.numel() >= behind + len(DRAFTS_WORDS):       # and those of the kernels for drafted tokens
+        host[behind:behind + len(DRAFTS_WORDS)] = 0
         if _DRAFTS_LIB is not None:
-            code = _DRAFTS_LIB.ib_attention_tree_error_async(at + 4 * behind, stream)
-            if code != 0:
-                raise KernelError(f"error_words_async: CUDA error {code}")
+            for i, fn in enumerate((_DRAFTS_LIB.ib_attention_tree_error_async, _DRAFTS_LIB.ib_log_probs_error_async)):
+                code = fn(at + 4 * (behind + i), stream)
+                if code != 0:
+                    raise KernelError(f"error_words_async: CUDA error {code}")
     for i, fn in enumerate(calls):
         code = fn(at + 4 * i, stream)
         if code != 0:
@@ -3023,9 +3030,10 @@ def reset_error_words(act_dtype: torch.dtype) -> dict:
             found[name] = v
     found.update(few_bits_faults(reset=True))
     if _DRAFTS_LIB is not None:
-        v = attention_tree_error(True)
-        if v:
-            found[DRAFTS_WORDS[0]] = v
+        for name, fn in zip(DRAFTS_WORDS, (attention_tree_error, log_probs_error)):
+            v = fn(True)
+            if v:
+                found[name] = v
     for counters in _DECODE_COUNTERS.values():
         counters.zero_()
     return found

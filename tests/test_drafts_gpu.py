@@ -404,7 +404,7 @@ def test_log_probs_hard_rows(dtype, rows):
              torch.where(up < 29.9, -inf, up), torch.where(up < 29.99, torch.finfo(dtype).min, up), torch.full((vocab,), -inf, device=DEV),
              torch.where(up == up[5], inf, up), torch.where(up == up[5], nan, up), torch.full((vocab,), nan, device=DEV),
              torch.where(up > 0.004, nan, up), torch.where(up > 0.004, -inf, -up), torch.where(up == 0, -0.0, 0.0), 1e4 + up, up * 1e30,
-             torch.where(up.long() % 2 == 0, up, -up)]
+             torch.where(up.long() % 2 == 0, up, -up), torch.where(up < 12, up, 50 - up), up.flip(0).roll(9000)]
     x = torch.stack(kinds).to(dtype)
     x = x.repeat(-(-rows // len(kinds)), 1)[:max(rows, len(kinds))].contiguous()
     t = torch.randint(-3, vocab + 3, (x.shape[0], 4), device=DEV).to(torch.int32)
