@@ -1,6 +1,6 @@
 // Log probabilities of given tokens, the distribution's entropy and its most likely tokens, for every row of logits.
 //
-// With m the row's largest logit, z = x - m, S = sum e^z and W = sum e^z z:
+// With m the row's largest logit, z = x - m, S = sum e^z and W = sum e^z z (kept in powers of two):
 //   log p(t) = z_t - log S        entropy = -sum p log p = log S - W / S
 // S and W are sums of numbers of one sign and lose nothing to cancellation.  Every thread keeps m, S and W of what it has seen
 // in 32 bits; when its m grows by g, S becomes S e^-g and W becomes (W - S g) e^-g.  A logit that is no number counts as minus
@@ -22,7 +22,7 @@ constexpr int MAX_TOP = 32;
 constexpr int NOTES = 1024;          // room for noted keys
 constexpr int GROUPS = 64;           // groups of 4 threads whose largest keys give the first bound
 constexpr int MAX_CLUSTER = 8;
-constexpr float LOWEST = -200.0f;    // e^-200 is 0 in 32 bits, and 0 times it is 0
+constexpr float LOWEST = -300.0f;    // 2^-300 is 0 in 32 bits, and 0 times it is 0
 
 typedef unsigned long long u64;
 
@@ -96,24 +96,54 @@ __device__ __forceinline__ u64 remote_u64(const u64* local, unsigned rank) {
     return v;
 }
 
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
 // S and W from reference m to reference to >= m (S = W = 0 where m is minus infinity)
 __device__ __forceinline__ void move_reference(float m, float to, float& s, float& w) {
     if (m == to || m == -INFINITY) return;
-    const float g = m - to;
-    const float c = __expf(g);
+    const float g = (m - to) * LOG2E, c = sm100::ex2(g);
     w = c > 0.0f ? c * fmaf(s, g, w) : 0.0f;
     s *= c;
 }
 
+// two neighbouring numbers at once
+__device__ __forceinline__ u64 pair(float a, float b) {
+    u64 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void apart(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+    u64 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // The k best of the first n notes to best[0 .. min(k, n)) in descending order, by counting the keys ahead of each (keys differ:
-// they hold their places).  The whole CTA calls it between two barriers.
+// they hold their places), four threads a key where there are few.  The threads that look at logits call it between two meetings.
 __device__ __forceinline__ void rank_notes(const u64* notes, int n, int k, u64* best) {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const u64 mine = notes[i];
+    const int share = n <= THREADS / 4 ? 4 : 1, part = threadIdx.x & (share - 1);
+    for (int i0 = 0; i0 < n; i0 += THREADS / share) {
+        const int i = i0 + threadIdx.x / share;
+        const u64 mine = i < n ? notes[i] : ~0ull;
         int ahead = 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) ahead += notes[j] > mine;
-        if (ahead < k) best[ahead] = mine;
+        for (int j = part; j < n; j += share) ahead += notes[j] > mine;
+        if (share == 4) {
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
+        }
+        if (i < n && part == 0 && ahead < k) best[ahead] = mine;
     }
 }
 
@@ -177,6 +207,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
     float m = -INFINITY, s = 0.0f, w = 0.0f;
     u64 bound = 0;                    // keys below it are not noted
     float bound_v = -INFINITY;
+    const int rounds = (v_hi - v_lo + CHUNK - 1) / CHUNK;
     int round = 0, next_look = 2;
     bool ok = true;
     auto note = [&](u64 key) {
@@ -238,8 +269,6 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                 }
             }
         }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&sh.empty[stage]));
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) top = fmaxf(top, e[i]);
@@ -248,13 +277,23 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
             m = top;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        const u64 less = pair(-ref, -ref), factor = pair(LOG2E, LOG2E);
+        u64 s2 = 0, w2 = 0;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const float z = fmaxf(e[i] - ref, LOWEST);
-            const float p = __expf(z);
-            s += p;
-            w = fmaf(p, z, w);
+        for (int i = 0; i < EACH; i += 2) {
+            float a, b;
+            apart(mul2(add2(pair(e[i], e[i + 1]), less), factor), a, b);       // (log2(e) z; the difference is taken first: large logits lose nothing)
+            a = fmaxf(a, LOWEST);
+            b = fmaxf(b, LOWEST);
+            const u64 p = pair(sm100::ex2(a), sm100::ex2(b));
+            s2 = add2(s2, p);
+            w2 = fma2(p, pair(a, b), w2);
         }
+        float a, b;
+        apart(s2, a, b);
+        s += a + b;
+        apart(w2, a, b);
+        w += a + b;
         if constexpr (TOP) {
             auto place = [&](int i) { return (v0 + (i / N) * THREADS + tid) * N - skew + i % N; };
             if (round == 0) {      // the first bound
@@ -266,28 +305,39 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                 for (int o = 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
                 if ((tid & 3) == 0) sh.groups[tid >> 2] = best;
                 meet(false);
-                if (tid < GROUPS) {
-                    const u64 mine = sh.groups[tid];
-                    int ahead = 0;
+                const int group = tid >> 2;
+                const u64 mine = sh.groups[group];
+                int ahead = 0;
 #pragma unroll 8
-                    for (int j = 0; j < GROUPS; ++j) ahead += sh.groups[j] > mine || (sh.groups[j] == mine && j < tid);
-                    if (ahead == A.top - 1) sh.bound = mine;       // (0 where fewer groups hold a number)
-                }
+                for (int j = tid & 3; j < GROUPS; j += 4) ahead += sh.groups[j] > mine || (sh.groups[j] == mine && j < group);
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
+                if ((tid & 3) == 0 && ahead == A.top - 1) sh.bound = mine;       // (0 where fewer groups hold a number)
                 meet(false);
                 bound = sh.bound;
                 bound_v = bound ? value_of(bound) : -INFINITY;
             }
-            if (top >= bound_v) {
+            if (top >= bound_v) {      // (few threads come here: a loop that is short to fetch)
+                unsigned todo = 0;
 #pragma unroll
-                for (int i = 0; i < EACH; ++i)
-                    if (e[i] >= bound_v) note(key_of(e[i], place(i)));
+                for (int i = 0; i < EACH; ++i) todo |= e[i] >= bound_v ? 1u << i : 0u;
+#pragma unroll 1
+                for (; todo; todo &= todo - 1) {
+                    const int i = __ffs(todo) - 1, v = v0 + i / N * THREADS + tid, at = v * N - skew + i % N;
+                    const T* from = v >= w_lo && v < w_hi ? reinterpret_cast<const T*>(&sh.ring[stage * CHUNK + i / N * THREADS + tid]) + i % N : x + at;
+                    note(key_of(ib_to_float(*from), at));
+                }
             }
-            if (round == next_look) {
-                meet(false);
-                prune();
+            if (round == next_look) {      // (not when fewer logits are to come than have been: the last look is near)
+                if (round < rounds - round) {
+                    meet(false);
+                    prune();
+                }
                 next_look = 2 * round + 1;
             }
         }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&sh.empty[stage]));
     }
     __syncthreads();
     if (TOP && sh.lost) {
@@ -344,7 +394,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         }
         const bool none = !(fabsf(all) < INFINITY);
         const float log_total = none ? NAN : logf(total);
-        if (tid == 0 && A.entropy) A.entropy[row] = log_total - weighed / total;
+        if (tid == 0 && A.entropy) A.entropy[row] = log_total - LN2 * (weighed / total);
         for (int i = tid; i < A.given; i += THREADS + 32) {
             float v = given;
             if (i != tid) {
