@@ -16,19 +16,32 @@ namespace tree {
 // ---- any type and head size: 32-bit arithmetic, 16 rows a CTA, four for each warp ----------------------------------------
 constexpr int ROWS = 16, KEYS = 32, WARPS = 4, MINE = ROWS / WARPS;
 
+// Shared memory: the rows' queries (later the part's sums), two tiles of keys and values as they lie in the cache, in rows that start 16 bytes
+// off a multiple of 128 (a lane a key: eight lanes' 16 bytes meet all banks), references and denominators.
 __host__ __device__ __forceinline__ int padded(int dim) { return (dim + 3) / 4 * 4; }
-__host__ __device__ __forceinline__ size_t rows_smem(int dim) {
-    return sizeof(float) * (size_t)(ROWS * padded(dim) + KEYS * (padded(dim) + 4) + KEYS * padded(dim) + 2 * ROWS);
+template <typename T> __host__ __device__ __forceinline__ int row_bytes(int dim) { return (dim * (int)sizeof(T) + 15) / 16 * 16 + 16; }
+// two tiles, one that is used and one that is on its way, where there is room for them
+template <typename T> __host__ __device__ __forceinline__ int turns(int dim) { return row_bytes<T>(dim) <= 1088 ? 2 : 1; }
+template <typename T> __host__ __device__ __forceinline__ size_t rows_smem(int dim) {
+    return sizeof(float) * (size_t)(ROWS * padded(dim) + 2 * ROWS) + 2 * turns<T>(dim) * (size_t)KEYS * row_bytes<T>(dim);
 }
 
-template <typename T, int PER>       // PER numbers of a head per lane
-__global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts) {
-    extern __shared__ __align__(16) float smem[];
-    const int d = A.dim, dp = padded(d);
-    float* sq = smem;                             // [ROWS][dp], later the part's sums
-    float* sk = sq + ROWS * dp;                   // [KEYS][dp + 4]
-    float* sv = sk + KEYS * (dp + 4);             // [KEYS][dp]
-    float* sml = sv + KEYS * dp;                  // [2][ROWS]
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+
+// What bounds it are instructions (a product of 32 bits takes one for 32 of them), few CTAs' latency, or what comes from memory where there are
+// few rows: 328 heads of requests with 2,000 keys each and eight rows, 754 MB, go at the copy's rate.  PER numbers of a head per lane, four
+// neighbours where that is a multiple of four.
+template <typename T, int PER>
+__global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts, bool wide) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int d = A.dim, dp = padded(d), rb = row_bytes<T>(d);
+    float* sq = reinterpret_cast<float*>(raw);    // [ROWS][dp], later the part's sums
+    float* sml = sq + ROWS * dp;                  // [2][ROWS]
+    unsigned char* tiles = reinterpret_cast<unsigned char*>(sml + 2 * ROWS);      // [2 in turn][keys, values][KEYS][rb]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int b = blockIdx.x;
     const int part = b % parts;
@@ -42,16 +55,6 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     if (rows <= 0) return;                        // (the whole cluster leaves)
     const int used = rows < ROWS ? rows : ROWS;
 
-    const T* q = static_cast<const T*>(A.q);
-    for (int i = tid; i < ROWS * dp; i += WARPS * 32) {
-        const int r = i / dp, e = i - r * dp;
-        float x = 0.0f;
-        if (r < used && e < d) {
-            const int at = first_row + r, token = at / group;
-            x = ib_to_float(q[((long)(S.row0 + token) * A.n_heads + head * group + at - token * group) * d + e]) * A.scale_log2;
-        }
-        sq[i] = x;
-    }
     // the warp's rows: their tokens, and the first key that each sees (and any of the tile's)
     int token[MINE], lo[MINE], lo_min = 0x7fffffff;
 #pragma unroll
@@ -60,10 +63,52 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         token[r] = warp * MINE + r < used ? at / group : -1;
         lo[r] = token[r] >= 0 ? first_key(A, S, token[r]) : 0;
     }
-    for (int t = first_row / group; t <= (first_row + used - 1) / group; ++t) lo_min = min(lo_min, first_key(A, S, t));
+    if (A.span == 0) lo_min = 0;
+    else for (int t = first_row / group; t <= (first_row + used - 1) / group; ++t) lo_min = min(lo_min, first_key(A, S, t));
     lo_min = min(lo_min, S.context);              // (the drafted tokens are looked at in any case)
     const int t0 = lo_min / KEYS, n_tiles = (S.keys + KEYS - 1) / KEYS - t0;
     const int begin = t0 + (int)((long)n_tiles * part / parts), end = t0 + (int)((long)n_tiles * (part + 1) / parts);
+    const int* bt = A.table + (long)req * A.max_pages;
+    auto look_up = [&](int t) -> long {           // where this lane's key of a tile lies
+        const int j = t * KEYS + lane;
+        if (t >= end || j >= S.keys) return -1;
+        const int slot = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size, page = bt[slot];
+        return page >= 0 && page < A.n_pages ? ((long)page * A.n_kv + head) * A.page_size + j - slot * A.page_size : -1;
+    };
+    auto load = [&](int t, long at) {             // a warp brings every fourth of the tile's keys
+        unsigned char* tile = tiles + (t & (turns<T>(d) - 1)) * (2 * KEYS * rb);
+#pragma unroll 2
+        for (int i = 0; i < KEYS / WARPS; ++i) {
+            const int key = i * WARPS + warp;
+            const long from = __shfl_sync(0xffffffffu, at, key);
+            const T* k = static_cast<const T*>(A.k) + (from < 0 ? 0 : from) * d;
+            const T* v = static_cast<const T*>(A.v) + (from < 0 ? 0 : from) * d;
+            unsigned char *to_k = tile + key * rb, *to_v = to_k + KEYS * rb;
+            if (wide) {
+                for (int c = lane; c < d * (int)sizeof(T) / 16; c += 32) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to_k + c * 16)),
+                                 "l"(reinterpret_cast<const uint4*>(k) + c), "r"(from < 0 ? 0 : 16) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to_v + c * 16)),
+                                 "l"(reinterpret_cast<const uint4*>(v) + c), "r"(from < 0 ? 0 : 16) : "memory");
+                }
+            } else {
+                for (int e = lane; e < dp; e += 32) {
+                    const bool some = from >= 0 && e < d;
+                    reinterpret_cast<T*>(to_k)[e] = some ? k[e] : ib_from_float<T>(0.0f);
+                    reinterpret_cast<T*>(to_v)[e] = some ? v[e] : ib_from_float<T>(0.0f);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    long at = look_up(begin), at_next = look_up(begin + 1);
+    load(begin, at);
+    const T* q = static_cast<const T*>(A.q);
+    for (int i = warp; i < ROWS; i += WARPS) {
+        const int row = first_row + i, tok = row / group;
+        const T* from = q + ((long)(S.row0 + tok) * A.n_heads + head * group + row - tok * group) * d;
+        for (int e = lane; e < dp; e += 32) sq[i * dp + e] = i < used && e < d ? ib_to_float(from[e]) * A.scale_log2 : 0.0f;
+    }
 
     float acc[MINE][PER], m[MINE], l[MINE];
 #pragma unroll
@@ -73,33 +118,31 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
 #pragma unroll
         for (int i = 0; i < PER; ++i) acc[r][i] = 0.0f;
     }
-    const int* bt = A.table + (long)req * A.max_pages;
+    // number i of this lane
+    auto number = [&](int i) { return PER % 4 == 0 ? (i / 4) * 128 + lane * 4 + i % 4 : lane + 32 * i; };
     for (int t = begin; t < end; ++t) {
         const int j = t * KEYS + lane;            // every lane's own key
-        long at = -1;
-        if (j < S.keys) {
-            const int page = bt[j / A.page_size];
-            if (page >= 0 && page < A.n_pages) at = ((long)page * A.n_kv + head) * A.page_size + j % A.page_size;
-        }
-        __syncthreads();                          // the tile before has been read
-        for (int i = 0; i < KEYS / WARPS; ++i) {
-            const int key = warp * (KEYS / WARPS) + i;
-            const long from = __shfl_sync(0xffffffffu, at, key);
-            for (int e = lane; e < dp; e += 32) {
-                const bool some = from >= 0 && e < d;
-                sk[key * (dp + 4) + e] = some ? ib_to_float(static_cast<const T*>(A.k)[from * d + e]) : 0.0f;
-                sv[key * dp + e] = some ? ib_to_float(static_cast<const T*>(A.v)[from * d + e]) : 0.0f;
-            }
+        const long next = at_next;
+        at_next = look_up(t + 2);
+        const bool ahead = turns<T>(d) == 2;
+        if (ahead) {
+            load(t + 1, next);                    // (behind the last tile zeros)
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         __syncthreads();
+        const unsigned char* tile = tiles + (t & (turns<T>(d) - 1)) * (2 * KEYS * rb);
+        const T* sk = reinterpret_cast<const T*>(tile + lane * rb);
         float dot[MINE];
 #pragma unroll
         for (int r = 0; r < MINE; ++r) dot[r] = 0.0f;
+#pragma unroll 4
         for (int e = 0; e < dp; e += 4) {
-            const float4 kk = *reinterpret_cast<const float4*>(sk + lane * (dp + 4) + e);
+            const float4 kk = four(sk + e);
 #pragma unroll
             for (int r = 0; r < MINE; ++r) {
-                const float4 qq = *reinterpret_cast<const float4*>(sq + (warp * MINE + r) * dp + e);
+                const float4 qq = four(sq + (warp * MINE + r) * dp + e);
                 dot[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, dot[r]))));
             }
         }
@@ -121,21 +164,35 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
             for (int i = 0; i < PER; ++i) acc[r][i] *= c;
             m[r] = to;
         }
+#pragma unroll 4
         for (int key = 0; key < KEYS; ++key) {
+            const T* sv = reinterpret_cast<const T*>(tile + (KEYS + key) * rb);
             float pk[MINE];
 #pragma unroll
             for (int r = 0; r < MINE; ++r) pk[r] = __shfl_sync(0xffffffffu, p[r], key);
+            float x[PER];
+            if constexpr (PER % 4 == 0) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int e = lane + 32 * i;
-                if (e >= d) continue;
-                const float x = sv[key * dp + e];
+                for (int i = 0; i < PER; i += 4) {
+                    const float4 v = number(i) < d ? four(sv + number(i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+                }
+            } else {
 #pragma unroll
-                for (int r = 0; r < MINE; ++r)
-                    if (pk[r] != 0.0f) acc[r][i] = fmaf(pk[r], x, acc[r][i]);      // what a row does not see cannot reach it
+                for (int i = 0; i < PER; ++i) x[i] = number(i) < d ? ib_to_float(sv[number(i)]) : 0.0f;
             }
+#pragma unroll
+            for (int r = 0; r < MINE; ++r)
+                if (pk[r] != 0.0f) {              // (the same for the warp; what a row does not see cannot reach it)
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) acc[r][i] = fmaf(pk[r], x[i], acc[r][i]);
+                }
         }
+        at = next;
+        __syncthreads();                          // the tile has been read
+        if (!ahead) load(t + 1, next);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     // join the parts: each CTA writes every parts-th row
     __syncthreads();
 #pragma unroll
@@ -143,7 +200,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         const int row = warp * MINE + r;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < d) sq[row * dp + lane + 32 * i] = acc[r][i];
+            if (number(i) < d) sq[row * dp + number(i)] = acc[r][i];
         if (lane == 0) { sml[row] = m[r]; sml[ROWS + row] = l[r]; }
     }
     if (parts > 1) cluster_sync(); else __syncthreads();
@@ -161,14 +218,14 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
             total = fmaf(lc, f, total);
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (lane + 32 * i < d) o[i] = fmaf(remote_f32(&sq[row * dp + lane + 32 * i], c), f, o[i]);
+                if (number(i) < d) o[i] = fmaf(remote_f32(&sq[row * dp + number(i)], c), f, o[i]);
         }
         const int at = first_row + row, tok = at / group;
         T* dst = static_cast<T*>(A.out) + (long)(S.row0 + tok) * A.out_ld + (long)(head * group + at - tok * group) * d;
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < d) dst[lane + 32 * i] = ib_from_float<T>(o[i] * inv);
+            if (number(i) < d) dst[number(i)] = ib_from_float<T>(o[i] * inv);
     }
     if (parts > 1) cluster_sync();                // nobody leaves while others read its sums
 }
@@ -176,15 +233,13 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
 template <typename T, int PER>
 static int launch_rows(const Args& A, int max_keys, cudaStream_t stream) {
     static IbDeviceSet done;
-    const size_t smem = rows_smem(A.dim);
-    if (smem > 48 * 1024) {
-        const int code = ib_allow_dynamic_smem(done, tree_rows_kernel<T, PER>, rows_smem(32 * PER));
-        if (code != IB_OK) return code;
-    }
+    const size_t smem = rows_smem<T>(A.dim);
+    if (const int code = ib_allow_dynamic_smem(done, tree_rows_kernel<T, PER>, rows_smem<T>(32 * PER))) return code;
     const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
     int parts = 1;
     while (parts < MAX_CLUSTER && pairs * parts * 2 <= 592 && max_keys >= 2 * KEYS * parts * 2) parts *= 2;
-    return launch_cluster(tree_rows_kernel<T, PER>, pairs * parts, parts, WARPS * 32, smem, stream, A, parts);
+    const bool wide = (reinterpret_cast<uintptr_t>(A.k) | reinterpret_cast<uintptr_t>(A.v) | (uintptr_t)(A.dim * sizeof(T))) % 16 == 0;
+    return launch_cluster(tree_rows_kernel<T, PER>, pairs * parts, parts, WARPS * 32, smem, stream, A, parts, wide);
 }
 
 template <typename T>

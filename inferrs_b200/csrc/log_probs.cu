@@ -6,11 +6,12 @@
 // in 32 bits; when its m grows by g, S becomes S e^-g and W becomes (W - S g) e^-g.  A logit that is no number counts as minus
 // infinity, as it does for the sampler; a row whose largest logit is infinite has no distribution, and NaN as its numbers.
 //
-// The logits are read once.  The k most likely tokens come out of the same pass: a key is the logit's bits made ascending, the
-// place's complement below them (of equal logits the lower place is ahead).  A bound that at least k keys of the row reach is
-// kept; what passes it is noted in shared memory, and behind chunks 2, 5, 11, 23 .. the k best of the noted ones give a higher bound.  The first
-// bound is the k-th largest of 64 groups' largest keys; expected are k to 2 k notes from the first 4,096 logits and k more
-// for every doubling behind them.
+// The logits are read once.  The k most likely tokens come out of the same pass, by blocks of 16 neighbouring logits, a thread's share of a
+// chunk: the k blocks whose largest logits are the largest (of equal ones the earlier block) hold the k most likely tokens, because every block
+// ahead of a token's own has a token that is ahead of it.  A block's key is its largest logit's bits made ascending, the complement of its place
+// below them.  A bound that at least k keys reach is kept; the key of a block that passes it is noted in shared memory, and behind chunks
+// 2, 5, 11 .. the k best of the noted ones give a higher bound.  The first bound is the k-th largest of 64 groups' largest keys; expected are k
+// to 2 k notes from the first 4,096 logits and k more for every doubling behind them.  At the end the k blocks are looked through.
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -65,7 +66,7 @@ __device__ __forceinline__ bool meet(bool mine) {
                  : "=r"(any) : "r"((int)mine) : "memory");
     return any != 0;
 }
-static_assert(THREADS == 256, "");
+static_assert(THREADS == 256, "the barrier's number of threads");
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
@@ -82,17 +83,17 @@ __device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {
 }
 __device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
     float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)));
     return v;
 }
 __device__ __forceinline__ int remote_i32(const int* local, unsigned rank) {
     int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(local, rank)) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(local, rank)));
     return v;
 }
 __device__ __forceinline__ u64 remote_u64(const u64* local, unsigned rank) {
     u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(local, rank)) : "memory");
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(local, rank)));
     return v;
 }
 
@@ -206,12 +207,10 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
 
     float m = -INFINITY, s = 0.0f, w = 0.0f;
     u64 bound = 0;                    // keys below it are not noted
-    float bound_v = -INFINITY;
     const int rounds = (v_hi - v_lo + CHUNK - 1) / CHUNK;
     int round = 0, next_look = 2;
     bool ok = true;
     auto note = [&](u64 key) {
-        if (key < bound) return;
         const int at = atomicAdd(&sh.n_notes, 1);
         if (at < NOTES) sh.notes[at] = key;
         else sh.lost = 1;
@@ -224,10 +223,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         const int left = min(n, A.top);
         if (tid < left) sh.notes[tid] = sh.board.best[tid];
         if (tid == 0) sh.n_notes = left;
-        if (left == A.top) {
-            bound = max(bound, sh.board.best[A.top - 1]);
-            bound_v = bound ? value_of(bound) : -INFINITY;
-        }
+        if (left == A.top) bound = max(bound, sh.board.best[A.top - 1]);
         meet(false);
     };
     // the given tokens' logits, on their way meanwhile
@@ -258,9 +254,10 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         float e[EACH];
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) {
-            const int v = v0 + i * THREADS + tid;
+            // (a thread's vectors are neighbours; in an order of its own, so that eight threads' meet all banks)
+            const int v = v0 + tid * VECTORS + ((i + lane / (8 / VECTORS)) & (VECTORS - 1));
             if (v >= w_lo && v < w_hi) {
-                Wide<T>::unpack(sh.ring[stage * CHUNK + i * THREADS + tid], e + i * N);
+                Wide<T>::unpack(sh.ring[stage * CHUNK + v - v0], e + i * N);
             } else {
 #pragma unroll
                 for (int c = 0; c < N; ++c) {
@@ -269,9 +266,16 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&sh.empty[stage]));
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) top = fmaxf(top, e[i]);
+        bool any = false;          // (a logit of minus infinity is one, no number is none)
+        if (TOP && top == -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) any |= e[i] == e[i];
+        }
         if (top > m) {
             move_reference(m, top, s, w);
             m = top;
@@ -295,12 +299,9 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         apart(w2, a, b);
         w += a + b;
         if constexpr (TOP) {
-            auto place = [&](int i) { return (v0 + (i / N) * THREADS + tid) * N - skew + i % N; };
+            const u64 key = top > -INFINITY || any ? key_of(top, v0 + tid * VECTORS) : 0;
             if (round == 0) {      // the first bound
-                u64 best = 0;
-#pragma unroll
-                for (int i = 0; i < EACH; ++i)
-                    if (e[i] == e[i]) best = max(best, key_of(e[i], place(i)));
+                u64 best = key;
 #pragma unroll
                 for (int o = 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
                 if ((tid & 3) == 0) sh.groups[tid >> 2] = best;
@@ -315,50 +316,64 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                 if ((tid & 3) == 0 && ahead == A.top - 1) sh.bound = mine;       // (0 where fewer groups hold a number)
                 meet(false);
                 bound = sh.bound;
-                bound_v = bound ? value_of(bound) : -INFINITY;
             }
-            if (top >= bound_v) {      // (few threads come here: a loop that is short to fetch)
-                unsigned todo = 0;
-#pragma unroll
-                for (int i = 0; i < EACH; ++i) todo |= e[i] >= bound_v ? 1u << i : 0u;
-#pragma unroll 1
-                for (; todo; todo &= todo - 1) {
-                    const int i = __ffs(todo) - 1, v = v0 + i / N * THREADS + tid, at = v * N - skew + i % N;
-                    const T* from = v >= w_lo && v < w_hi ? reinterpret_cast<const T*>(&sh.ring[stage * CHUNK + i / N * THREADS + tid]) + i % N : x + at;
-                    note(key_of(ib_to_float(*from), at));
-                }
-            }
-            if (round == next_look) {      // (not when fewer logits are to come than have been: the last look is near)
-                if (round < rounds - round) {
+            if (key >= bound && key) note(key);
+            if (round == next_look) {      // (not when few logits are to come: the last look is near)
+                if (3 * round < rounds) {
                     meet(false);
                     prune();
                 }
                 next_look = 2 * round + 1;
             }
         }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&sh.empty[stage]));
     }
     __syncthreads();
-    if (TOP && sh.lost) {
-        // More notes than there is room for (logits that ascend do that): from the best bound so far on, the stretch again, a few at a time,
-        // with a look whenever the room could run out.  Nothing is lost: of what does not fit the k best are kept each time.
-        if (tid < THREADS) {
+    if (TOP && tid < THREADS) {
+        auto logit = [&](int v, int c) {       // logit c of the block that starts with vector v
+            const int at = v * N - skew + c;
+            return v + c / N < v_hi && at >= 0 && at < A.vocab ? ib_to_float(x[at]) : NAN;
+        };
+        if (sh.lost) {
+            // More notes than there is room for (logits that ascend do that): from the best bound so far on, the blocks again, with a look whenever
+            // the room could run out.  Nothing is lost then.
             meet(false);
             prune();
             if (tid == 0) sh.n_notes = 0;
             meet(false);
-            const int lo = max(0, v_lo * N - skew), hi = min(A.vocab, v_hi * N - skew);
-            for (int at0 = lo; at0 < hi; at0 += THREADS) {
-                const float v = at0 + tid < hi ? ib_to_float(x[at0 + tid]) : NAN;
-                if (v >= bound_v) note(key_of(v, at0 + tid));
+            for (int v0 = v_lo; v0 < v_hi; v0 += CHUNK) {
+                const int v = v0 + tid * VECTORS;
+                float top = -INFINITY;
+                bool any = false;
+                for (int c = 0; c < EACH; ++c) {
+                    const float z = logit(v, c);
+                    top = fmaxf(top, z);
+                    any |= z == z;
+                }
+                if (any && key_of(top, v) >= bound) note(key_of(top, v));
                 meet(false);
                 const bool look = sh.n_notes > NOTES - THREADS;
                 meet(false);
                 if (look) prune();
             }
+            meet(false);
         }
-        __syncthreads();
+        // the k best blocks' logits: those that reach the k-th block's largest one
+        prune();
+        const int blocks = sh.n_notes;
+        const float least = blocks == A.top ? value_of(bound) : -INFINITY;
+        meet(false);
+        if (tid == 0) sh.n_notes = 0;
+        meet(false);
+        for (int i = tid; i < blocks * EACH; i += THREADS) {
+            const int v = place_of(sh.board.best[i / EACH]), c = i % EACH;
+            const float z = logit(v, c);
+            if (z >= least) note(key_of(z, v * N - skew + c));      // (at most 512: there is room)
+        }
+        meet(false);
+        rank_notes(sh.notes, sh.n_notes, A.top, sh.groups);
+        meet(false);
+        if (tid < A.top) sh.board.best[tid] = sh.groups[tid];
+        if (tid == 0) sh.n_notes = min(sh.n_notes, A.top);
     }
 
     // the CTA's m, S and W
@@ -368,7 +383,6 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
     w = ib_warp_sum(w);
     if (lane == 0 && warp < THREADS / 32) { sh.red[0][warp] = top; sh.red[1][warp] = ok ? s : NAN; sh.red[2][warp] = w; }
     __syncthreads();
-    if (TOP && tid < THREADS) rank_notes(sh.notes, min(sh.n_notes, NOTES), A.top, sh.board.best);
     if (warp == 0) {
         const int n = THREADS / 32;
         float m1 = lane < n ? sh.red[0][lane] : -INFINITY, s1 = lane < n ? sh.red[1][lane] : 0.0f, w1 = lane < n ? sh.red[2][lane] : 0.0f;
@@ -378,20 +392,31 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         w1 = ib_warp_sum(w1);
         if (lane == 0) {
             sh.board.m = all; sh.board.s = s1; sh.board.w = w1;
-            sh.board.n = TOP ? min(min(sh.n_notes, NOTES), A.top) : 0;
+            sh.board.n = TOP ? sh.n_notes : 0;
         }
     }
     if (cluster > 1) cluster_sync(); else __syncthreads();
     if (rank == 0) {
-        // every thread adds the CTAs' sums in the same order
-        float all = -INFINITY, total = 0.0f, weighed = 0.0f;
-        for (int c = 0; c < cluster; ++c) all = fmaxf(all, cluster > 1 ? remote_f32(&sh.board.m, c) : sh.board.m);
-        for (int c = 0; c < cluster; ++c) {
-            float sc = cluster > 1 ? remote_f32(&sh.board.s, c) : sh.board.s, wc = cluster > 1 ? remote_f32(&sh.board.w, c) : sh.board.w;
-            move_reference(cluster > 1 ? remote_f32(&sh.board.m, c) : sh.board.m, all, sc, wc);
-            total += sc;
-            weighed += wc;
+        // lane c looks at the c-th CTA's sums; all warps add them in the same order
+        float mc = -INFINITY, total = 0.0f, weighed = 0.0f;
+        int have = 0;
+        if (lane < cluster) {
+            mc = remote_f32(&sh.board.m, lane);
+            total = remote_f32(&sh.board.s, lane);
+            weighed = remote_f32(&sh.board.w, lane);
+            have = remote_i32(&sh.board.n, lane);
         }
+        const float all = ib_warp_max(mc);
+        move_reference(mc, all, total, weighed);
+#pragma unroll
+        for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+            weighed += __shfl_xor_sync(0xffffffffu, weighed, o);
+            have += __shfl_xor_sync(0xffffffffu, have, o);
+        }
+        total = __shfl_sync(0xffffffffu, total, 0);
+        weighed = __shfl_sync(0xffffffffu, weighed, 0);
+        have = __shfl_sync(0xffffffffu, have, 0);
         const bool none = !(fabsf(all) < INFINITY);
         const float log_total = none ? NAN : logf(total);
         if (tid == 0 && A.entropy) A.entropy[row] = log_total - LN2 * (weighed / total);
@@ -405,13 +430,11 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         }
         if constexpr (TOP) {
             if (cluster > 1) {      // the best of the CTAs' best
-                const int all_keys = cluster * A.top;
+                const int all_keys = cluster * A.top, of = tid / A.top, i = tid - of * A.top;
                 u64 mine = 0;
-                if (tid < all_keys) {
-                    const int of = tid / A.top, i = tid - of * A.top;
-                    if (i < remote_i32(&sh.board.n, of)) mine = remote_u64(&sh.board.best[i], of);
-                    sh.notes[tid] = mine;
-                }
+                const int theirs = tid < all_keys ? remote_i32(&sh.board.n, of) : 0;
+                if (i < theirs) mine = remote_u64(&sh.board.best[i], of);
+                if (tid < all_keys) sh.notes[tid] = mine;
                 __syncthreads();
                 if (mine) {
                     int ahead = 0;
@@ -422,8 +445,6 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                         A.top_log_probs[(long)row * A.top + ahead] = (value_of(mine) - all) - log_total;
                     }
                 }
-                int have = 0;
-                for (int c = 0; c < cluster; ++c) have += remote_i32(&sh.board.n, c);
                 for (int i = have + tid; i < A.top; i += THREADS + 32) {
                     A.top_ids[(long)row * A.top + i] = -1;
                     A.top_log_probs[(long)row * A.top + i] = -INFINITY;
