@@ -36,14 +36,14 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(Pages P, const int* __r
 
 // Token kept[r, i] behind context[r] goes to place context[r] + i.  The places are ascending, so a token never moves back and
 // never beyond one that follows it: chunk by chunk, with all loads of a chunk ahead of its stores, nothing is overwritten before
-// it has been read (a chunk's stores end below the places that the next chunk reads).  One CTA for a head of one request in
-// one plane, so chunks of the same vectors never run at once.
+// it has been read (a chunk's stores end below the places that the next chunk reads).  One CTA for one or several heads of one
+// request in one plane, so chunks of the same vectors never run at once.
 template <typename U, int N>
-__global__ void __launch_bounds__(256) keep_tokens_kernel(Pages P, int heads, int places, int units,      // units per vector
+__global__ void __launch_bounds__(256) keep_tokens_kernel(Pages P, int heads, int places, int shift, int units, int together,      // log2: of the places or -1, of a CTA's heads
                                                           const int* __restrict__ table, int max_pages,
                                                           const int* __restrict__ context, const int* __restrict__ kept,
                                                           int max_kept, const int* __restrict__ n_kept) {
-    const int r = blockIdx.z, head = blockIdx.y;
+    const int r = blockIdx.z, head0 = blockIdx.y << together;
     const long outer = blockIdx.x;
     int n = n_kept[r];
     n = n < max_kept ? n : max_kept;
@@ -53,36 +53,45 @@ __global__ void __launch_bounds__(256) keep_tokens_kernel(Pages P, int heads, in
     const int mine = threadIdx.x / per;
     U* plane = reinterpret_cast<U*>(P.base) + outer * P.n_pages * heads * places * units;
     const int* bt = table + (long)r * max_pages;
-    auto vector_at = [&](long place) -> U* {
-        if (place < 0) return nullptr;
-        const long slot = place / places;
-        if (slot >= max_pages) return nullptr;
+    auto vector_at = [&](int head, long place) -> int {                      // a vector's place in the plane, -1: there is no page
+        if (place < 0 || place > 0x7fffffffL) return -1;
+        const int slot = shift >= 0 ? (int)place >> shift : (int)place / places;
+        if (slot >= max_pages) return -1;
         const int page = bt[slot];
-        if (page < 0 || page >= P.n_pages) return nullptr;
-        return plane + (((long)page * heads + head) * places + (place - slot * places)) * units;
+        return page >= 0 && page < P.n_pages ? (page * heads + head) * places + ((int)place - slot * places) : -1;
     };
     for (int unit0 = 0; unit0 < units; unit0 += per) {
         const int unit = unit0 + (int)(threadIdx.x - mine * per);
         const bool some = mine < step && unit < units;
-        for (int i0 = 0; i0 < n; i0 += step * N) {
-            U held[N];
-            U* to[N];
+        // a chunk's places are looked up while the chunk before it is on its way
+        auto look_up = [&](int i0, int (&from)[N], int (&to)[N]) {
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const int i = i0 + k * step + mine;
-                to[k] = nullptr;
+                const int q = i0 + k * step + mine, i = q >> together, head = head0 + (q & ((1 << together) - 1));
+                from[k] = to[k] = -1;
                 if (!some || i >= n) continue;
-                const int from = kept[(long)r * max_kept + i];
-                if (from == i) continue;
-                const U* src = vector_at(first + from);
-                to[k] = vector_at(first + i);
-                if (src == nullptr) to[k] = nullptr;
-                if (to[k] != nullptr) held[k] = src[unit];
+                const int old = kept[(long)r * max_kept + i];
+                if (old == i) continue;
+                from[k] = vector_at(head, first + old);
+                to[k] = vector_at(head, first + i);
             }
-            __syncthreads();
+        };
+        int from[N], to[N];
+        look_up(0, from, to);
+        for (int i0 = 0; i0 < n << together; i0 += step * N) {
+            U held[N];
 #pragma unroll
             for (int k = 0; k < N; ++k)
-                if (to[k] != nullptr) to[k][unit] = held[k];
+                if (from[k] >= 0 && to[k] >= 0) held[k] = plane[(long)from[k] * units + unit];
+            int from_next[N], to_next[N];
+            look_up(i0 + step * N, from_next, to_next);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if (from[k] >= 0 && to[k] >= 0) plane[(long)to[k] * units + unit] = held[k];
+                from[k] = from_next[k];
+                to[k] = to_next[k];
+            }
         }
         __syncthreads();
     }
@@ -141,10 +150,14 @@ template <typename U>
 static int keep_tokens_as(const IbKeepTokens& a) {
     const int units = (int)(a.vector_bytes / (long)sizeof(U));
     const Pages P{a.base, a.outer, a.n_pages, a.heads * a.places * a.vector_bytes};
-    const dim3 grid((unsigned)a.outer, (unsigned)a.heads, (unsigned)a.requests);
+    // heads in one CTA: as many as make up for short lists, while there are CTAs for every SM
+    int together = 0;
+    while (a.heads % (2L << together) == 0 && a.max_kept * units << together < 1024 && a.outer * (a.heads >> together) * a.requests >= 2 * 8 * 148) ++together;
+    const dim3 grid((unsigned)a.outer, (unsigned)(a.heads >> together), (unsigned)a.requests);
     int threads = 256;
-    while (threads > 32 && (long)(threads / 2) >= a.max_kept * units) threads /= 2;
-    keep_tokens_kernel<U, 4><<<grid, threads, 0, a.stream>>>(P, (int)a.heads, (int)a.places, units, a.table, (int)a.max_pages, a.context,
+    while (threads > 32 && (long)(threads / 2) >= a.max_kept * units << together) threads /= 2;
+    const int shift = (a.places & (a.places - 1)) == 0 ? __builtin_ctzl(a.places) : -1;
+    keep_tokens_kernel<U, 2><<<grid, threads, 0, a.stream>>>(P, (int)a.heads, (int)a.places, shift, units, together, a.table, (int)a.max_pages, a.context,
                                                              a.kept, (int)a.max_kept, a.n_kept);
     return ib_launch_status();
 }
@@ -154,7 +167,9 @@ IB_EXPORT int ib_keep_tokens(const void* call) {
     if (a.outer < 0 || a.n_pages < 0 || a.heads < 0 || a.places <= 0 || a.vector_bytes < 0 || a.requests < 0 || a.max_pages < 0 || a.max_kept < 0)
         return IB_ERR_ARGUMENT;
     if (a.outer == 0 || a.n_pages == 0 || a.heads == 0 || a.vector_bytes == 0 || a.requests == 0 || a.max_pages == 0 || a.max_kept == 0) return IB_OK;
-    if (a.outer > 0x7fffffffL || a.heads > 65535 || a.requests > 65535 || a.places > 0x7fffffffL || a.vector_bytes > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
+    if (a.max_kept > 0x7fffffffL / 64) return IB_ERR_UNSUPPORTED;
+    if (a.outer > 0x7fffffffL || a.heads > 65535 || a.requests > 65535 || a.places > 0x7fffffffL || a.vector_bytes > 0x7fffffffL
+        || a.n_pages * a.heads * a.places > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
     switch (unit_of(a.base, a.vector_bytes)) {
         case 16: return keep_tokens_as<uint4>(a);
         case 8: return keep_tokens_as<uint2>(a);
