@@ -17,6 +17,7 @@ from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .. import kernels
 from ..kernels import Kv8Pages
 from .manager import GroupLayout
 
@@ -152,6 +153,30 @@ class CacheStorage:
     def side_state(self, cache_id: int, owner: Any) -> torch.Tensor:
         """The per-request state [slots, ...] that the description ``owner`` keeps under this cache id."""
         return self.side_states[(cache_id, owner)]
+
+    def _page_tensors(self, group: int):
+        """(tensor, the axis that counts its pages) of everything that holds a group's pages."""
+        yield self.kv[group], 2
+        if self.scales:
+            yield self.scales[group], 2
+        if self.values[group] is not None:
+            yield self.values[group], 1
+
+    def copy_pages(self, group: int, source: torch.Tensor, target: torch.Tensor):
+        """In all of a group's caches page target[i] becomes a copy of page source[i] (int32, on the device)."""
+        for t, axis in self._page_tensors(group):
+            kernels.copy_pages(t, axis, source, target)
+
+    def keep_tokens(self, group: int, block_table: torch.Tensor, context: torch.Tensor, kept: torch.Tensor, n_kept: torch.Tensor):
+        """In all of a group's caches what is at place context[r] + kept[r, i] of a request goes to place context[r] + i (see
+        :func:`inferrs_b200.kernels.keep_tokens`)."""
+        for t, axis in self._page_tensors(group):
+            kernels.keep_tokens(t, axis, block_table, context, kept, n_kept)
+
+    def copy_slot(self, source: int, target: int):
+        """The fixed-size states of one slot become those of another."""
+        for t in list(self.states.values()) + list(self.side_states.values()):
+            t[target].copy_(t[source])
 
     def clear_slot(self, slot: int):
         """A new request takes the slot: its fixed-size states start at zero."""

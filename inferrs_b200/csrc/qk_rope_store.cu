@@ -53,7 +53,7 @@ __global__ void qk_norm_rope_store_kernel(
     const act_t* __restrict__ qkv, int row_stride, int n_heads, int n_kv_heads, int head_dim, int v_dim, int store_kv,
     const WT* __restrict__ q_weight, const WT* __restrict__ k_weight, int norm_flags, float eps,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table, int rot_dim, int interleaved, int table_rows,
-    const int* __restrict__ positions, const int* __restrict__ row_request,
+    const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ row_request,
     const int* __restrict__ block_table, int max_pages, int page_size, int n_pages,
     act_t* __restrict__ k_pages, act_t* __restrict__ v_pages, act_t* __restrict__ q_out,
     const float* __restrict__ bias, int value_is_key) {
@@ -65,7 +65,7 @@ __global__ void qk_norm_rope_store_kernel(
     const int half = rot_dim / 2;
     float* sh = smem + warp * 2 * d;      // the head as it came, and turned
     float* turned = sh + d;
-    const int pos = positions[row];
+    const int pos = positions[row], at = places ? places[row] : pos;      // what it turns by, and where its key and value go
     const int heads_total = n_heads + (store_kv ? 2 * n_kv_heads : 0);
     // a position outside the rotation tables: the row is left out and the fault is recorded
     if (pos < 0 || (rot_dim > 0 && pos >= table_rows)) { ib_note_row_fault(row); ib_grid_dependency_wait(); return; }
@@ -74,9 +74,9 @@ __global__ void qk_norm_rope_store_kernel(
     long kv_place = -1;  // (page, kv head 0, slot) counted in heads' rows
     if (store_kv) {
         const int req = row_request[row];
-        const int page = pos / page_size < max_pages ? block_table[(long)req * max_pages + pos / page_size] : -1;
+        const int page = at >= 0 && at / page_size < max_pages ? block_table[(long)req * max_pages + at / page_size] : -1;
         if (page >= 0 && page < n_pages)
-            kv_place = (long)page * n_kv_heads * page_size + (pos % page_size);
+            kv_place = (long)page * n_kv_heads * page_size + (at % page_size);
     }
     const bool clear_tail = kv_place >= 0 && ib_last_row_of_request(row_request, row, gridDim.x);
     const bool norm_after = (norm_flags & 4) != 0;
@@ -95,7 +95,7 @@ __global__ void qk_norm_rope_store_kernel(
             for (int j = lane; j < v_dim; j += 32)
                 dst[j] = bias ? ib_from_float<act_t>(ib_to_float(src[j]) + bias[col + j]) : src[j];
             if (clear_tail) {
-                const int behind = (page_size - 1 - pos % page_size) * v_dim;
+                const int behind = (page_size - 1 - at % page_size) * v_dim;
                 for (int j = lane; j < behind; j += 32) dst[v_dim + j] = ib_from_float<act_t>(0.0f);
             }
             continue;
@@ -154,7 +154,7 @@ __global__ void qk_norm_rope_store_d128_kernel(
     const __nv_bfloat16* __restrict__ qkv, int row_stride, int n_heads, int n_kv_heads, int store_kv,
     const WT* __restrict__ q_weight, const WT* __restrict__ k_weight, float eps,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table, int table_rows,
-    const int* __restrict__ positions, const int* __restrict__ row_request,
+    const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ row_request,
     const int* __restrict__ block_table, int max_pages, int page_size, int n_pages,
     __nv_bfloat16* __restrict__ k_pages, __nv_bfloat16* __restrict__ v_pages, __nv_bfloat16* __restrict__ q_out) {
     // the step's description, the tables and the weights are written by no kernel: they are fetched while the
@@ -165,13 +165,13 @@ __global__ void qk_norm_rope_store_d128_kernel(
     const int heads_total = n_heads + (store_kv ? 2 * n_kv_heads : 0);
     const int head0 = (blockIdx.y * QRS_WARPS + warp) * HPW;
     if (head0 >= heads_total) return;
-    const int pos = positions[row];
+    const int pos = positions[row], at = places ? places[row] : pos;      // what it turns by, and where its key and value go
     if (pos < 0 || pos >= table_rows) { ib_note_row_fault(row); ib_grid_dependency_wait(); return; }
     long kv_base = -1;  // element offset of (page, kv head 0, place in the page, 0)
     if (store_kv && head0 + HPW > n_heads) {
         const int req = row_request[row];
-        const int page = pos / page_size < max_pages ? block_table[(long)req * max_pages + pos / page_size] : -1;
-        if (page >= 0 && page < n_pages) kv_base = ((long)page * n_kv_heads * page_size + (pos % page_size)) * 128;
+        const int page = at >= 0 && at / page_size < max_pages ? block_table[(long)req * max_pages + at / page_size] : -1;
+        if (page >= 0 && page < n_pages) kv_base = ((long)page * n_kv_heads * page_size + (at % page_size)) * 128;
     }
     const bool clear_tail = kv_base >= 0 && ib_last_row_of_request(row_request, row, gridDim.x);
     // element i < 64 pairs with i + 64: lanes 0..15 hold the first halves, lanes 16..31 the second
@@ -228,7 +228,7 @@ __global__ void qk_norm_rope_store_d128_kernel(
         *reinterpret_cast<__nv_bfloat162*>(&o.y) = __floats2bfloat162_rn(x[2], x[3]);
         *reinterpret_cast<uint2*>(dst + 4 * lane) = o;
         if (kind == 2 && clear_tail)
-            for (int k = 1; k < page_size - pos % page_size; ++k)
+            for (int k = 1; k < page_size - at % page_size; ++k)
                 *reinterpret_cast<uint2*>(dst + k * 128 + 4 * lane) = make_uint2(0u, 0u);
     }
 }
@@ -244,7 +244,7 @@ __global__ void qk_norm_rope_store_d128_wide_kernel(
     const __nv_bfloat16* __restrict__ qkv, int row_stride, int n_heads, int n_kv_heads, int store_kv,
     const WT* __restrict__ q_weight, const WT* __restrict__ k_weight, float eps,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table, int table_rows,
-    const int* __restrict__ positions, const int* __restrict__ row_request,
+    const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ row_request,
     const int* __restrict__ block_table, int max_pages, int page_size, int n_pages,
     __nv_bfloat16* __restrict__ k_pages, __nv_bfloat16* __restrict__ v_pages, __nv_bfloat16* __restrict__ q_out) {
     constexpr int HPW = 8;                       // heads per warp
@@ -254,13 +254,13 @@ __global__ void qk_norm_rope_store_d128_wide_kernel(
     const int heads_total = n_heads + (store_kv ? 2 * n_kv_heads : 0);
     const int head0 = (blockIdx.y * (blockDim.x >> 5) + warp) * HPW;
     if (head0 >= heads_total) return;
-    const int pos = positions[row];
+    const int pos = positions[row], at = places ? places[row] : pos;      // what it turns by, and where its key and value go
     if (pos < 0 || pos >= table_rows) { ib_note_row_fault(row); ib_grid_dependency_wait(); return; }
     long kv_base = -1;
     if (store_kv && head0 + HPW > n_heads) {
         const int req = row_request[row];
-        const int page = pos / page_size < max_pages ? block_table[(long)req * max_pages + pos / page_size] : -1;
-        if (page >= 0 && page < n_pages) kv_base = ((long)page * n_kv_heads * page_size + (pos % page_size)) * 128;
+        const int page = at >= 0 && at / page_size < max_pages ? block_table[(long)req * max_pages + at / page_size] : -1;
+        if (page >= 0 && page < n_pages) kv_base = ((long)page * n_kv_heads * page_size + (at % page_size)) * 128;
     }
     const bool clear_tail = kv_base >= 0 && ib_last_row_of_request(row_request, row, gridDim.x);
     const int sub = lane >> 4, l16 = lane & 15;  // which of the two heads of a pass, and the place in it
@@ -355,7 +355,7 @@ __global__ void qk_norm_rope_store_d128_wide_kernel(
         *reinterpret_cast<uint2*>(dst + e0) = o_lo;
         *reinterpret_cast<uint2*>(dst + 64 + e0) = o_hi;
         if (kind == 2 && clear_tail)
-            for (int k = 1; k < page_size - pos % page_size; ++k) {
+            for (int k = 1; k < page_size - at % page_size; ++k) {
                 *reinterpret_cast<uint2*>(dst + k * 128 + e0) = make_uint2(0u, 0u);
                 *reinterpret_cast<uint2*>(dst + k * 128 + 64 + e0) = make_uint2(0u, 0u);
             }
@@ -373,7 +373,7 @@ template <bool INTERLEAVED>
 __global__ void qk_rope_store_shared_kernel(
     const act_t* __restrict__ qk, long row_stride, int n_heads, int n_kv_heads, int d, const float* __restrict__ bias,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table, int rot_dim, int table_rows,
-    const int* __restrict__ positions, const int* __restrict__ row_request, const int* __restrict__ block_table,
+    const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ row_request, const int* __restrict__ block_table,
     int max_pages, int page_size, int n_pages, act_t* __restrict__ k_pages, act_t* __restrict__ v_pages,
     act_t* __restrict__ q_out) {
     constexpr int VEC = 16 / (int)sizeof(act_t);
@@ -381,13 +381,13 @@ __global__ void qk_rope_store_shared_kernel(
     // the step's description, the tables and the biases are written by no kernel: they are read while the kernel
     // before this one still runs
     const int row = blockIdx.x;
-    const int pos = positions[row];
+    const int pos = positions[row], at = places ? places[row] : pos;      // what it turns by, and where its key and value go
     if (pos < 0 || (rot_dim > 0 && pos >= table_rows)) { ib_note_row_fault(row); ib_grid_dependency_wait(); return; }
-    const int slot = pos % page_size;
+    const int slot = at % page_size;
     long kv_place = -1;
     {
         const int req = row_request[row];
-        const int page = pos / page_size < max_pages ? block_table[(long)req * max_pages + pos / page_size] : -1;
+        const int page = at >= 0 && at / page_size < max_pages ? block_table[(long)req * max_pages + at / page_size] : -1;
         if (page >= 0 && page < n_pages) kv_place = (long)page * n_kv_heads * page_size + slot;
     }
     const bool clear_tail = kv_place >= 0 && ib_last_row_of_request(row_request, row, gridDim.x);
@@ -469,12 +469,13 @@ __global__ void qk_rope_store_shared_kernel(
     }
 }
 
-// bias: float over the columns of qkv (or null).  value_is_key: qkv holds queries and keys; a value is its key before the
+// places: where in its request a row's key and value go (null: at its position).  bias: float over the columns of qkv (or null).  value_is_key: qkv holds queries and keys; a value is its key before the
 // norm and the rotation (v_dim is then head_dim).
 IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows, int n_heads, int n_kv_heads,
                                     int head_dim, int v_dim, int store_kv, const void* q_weight, const void* k_weight,
                                     int weight_is_f32, int norm_flags, float eps, const float* cos_table, const float* sin_table,
-                                    int rot_dim, int interleaved, int table_rows, const int* positions, const int* row_request,
+                                    int rot_dim, int interleaved, int table_rows, const int* positions, const int* places,
+                                    const int* row_request,
                                     const int* block_table, int max_pages, int page_size, int n_pages,
                                     void* k_pages, void* v_pages, void* q_out, const float* bias, int value_is_key,
                                     cudaStream_t stream) {
@@ -494,7 +495,7 @@ IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows,
             if (threads > 256) threads = 256;
 #define IB_LAUNCH_SHARED(INTER)                                                                                      \
     ib_launch(qk_rope_store_shared_kernel<INTER>, n_rows, threads, 0, stream, (const act_t*)qkv, (long)row_stride,   \
-              n_heads, n_kv_heads, head_dim, bias, cos_table, sin_table, rot_dim, table_rows, positions, row_request, \
+              n_heads, n_kv_heads, head_dim, bias, cos_table, sin_table, rot_dim, table_rows, positions, places, row_request, \
               block_table, max_pages, page_size, n_pages, (act_t*)k_pages, (act_t*)v_pages, (act_t*)q_out)
             if (interleaved) IB_LAUNCH_SHARED(true); else IB_LAUNCH_SHARED(false);
 #undef IB_LAUNCH_SHARED
@@ -513,7 +514,7 @@ IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows,
 #define IB_LAUNCH_D128(WT, HPW)                                                                                    \
     ib_launch(qk_norm_rope_store_d128_kernel<WT, HPW>, dim3(n_rows, (heads_total + QRS_WARPS * HPW - 1) / (QRS_WARPS * HPW)), \
               32 * QRS_WARPS, 0, stream, (const __nv_bfloat16*)qkv, row_stride, n_heads, n_kv_heads, store_kv,          \
-              (const WT*)q_weight, (const WT*)k_weight, eps, cos_table, sin_table, table_rows, positions, row_request,  \
+              (const WT*)q_weight, (const WT*)k_weight, eps, cos_table, sin_table, table_rows, positions, places, row_request,  \
               block_table, max_pages, page_size, n_pages, (__nv_bfloat16*)k_pages, (__nv_bfloat16*)v_pages,            \
               (__nv_bfloat16*)q_out)
         // few rows: one head per warp, for the shortest chain; many rows: eight heads per warp and sixteen bytes
@@ -527,7 +528,7 @@ IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows,
 #define IB_LAUNCH_WIDE(WT)                                                                                            \
     ib_launch(qk_norm_rope_store_d128_wide_kernel<WT>, wide_grid, 32 * warps, 0, stream, (const __nv_bfloat16*)qkv,   \
               row_stride, n_heads, n_kv_heads, store_kv, (const WT*)q_weight, (const WT*)k_weight, eps, cos_table,     \
-              sin_table, table_rows, positions, row_request, block_table, max_pages, page_size, n_pages,               \
+              sin_table, table_rows, positions, places, row_request, block_table, max_pages, page_size, n_pages,               \
               (__nv_bfloat16*)k_pages, (__nv_bfloat16*)v_pages, (__nv_bfloat16*)q_out)
             if (weight_is_f32) IB_LAUNCH_WIDE(float); else IB_LAUNCH_WIDE(__nv_bfloat16);
 #undef IB_LAUNCH_WIDE
@@ -543,12 +544,12 @@ IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows,
     if (weight_is_f32)
         ib_launch(qk_norm_rope_store_kernel<float>, grid, 32 * QRS_WARPS, smem, stream,
             (const act_t*)qkv, row_stride, n_heads, n_kv_heads, head_dim, v_dim, store_kv, (const float*)q_weight,
-            (const float*)k_weight, norm_flags, eps, cos_table, sin_table, rot_dim, interleaved, table_rows, positions, row_request, block_table,
+            (const float*)k_weight, norm_flags, eps, cos_table, sin_table, rot_dim, interleaved, table_rows, positions, places, row_request, block_table,
             max_pages, page_size, n_pages, (act_t*)k_pages, (act_t*)v_pages, (act_t*)q_out, bias, value_is_key);
     else
         ib_launch(qk_norm_rope_store_kernel<__nv_bfloat16>, grid, 32 * QRS_WARPS, smem, stream,
             (const act_t*)qkv, row_stride, n_heads, n_kv_heads, head_dim, v_dim, store_kv, (const __nv_bfloat16*)q_weight,
-            (const __nv_bfloat16*)k_weight, norm_flags, eps, cos_table, sin_table, rot_dim, interleaved, table_rows, positions, row_request,
+            (const __nv_bfloat16*)k_weight, norm_flags, eps, cos_table, sin_table, rot_dim, interleaved, table_rows, positions, places, row_request,
             block_table,
             max_pages, page_size, n_pages, (act_t*)k_pages, (act_t*)v_pages, (act_t*)q_out, bias, value_is_key);
     return ib_launch_status();

@@ -29,6 +29,29 @@ class StepEntry:
 
 
 @dataclass
+class DraftEntry:
+    """Drafted tokens of one request: a token's parent is an earlier one among them, or -1 where it follows what the cache holds."""
+
+    rid: Hashable
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
+@dataclass
+class Drafts:
+    """Device tensors (int32) of a step of drafted tokens, beside the step's context, whose positions are those of the tree.
+
+    places [N]       where in its request a row's keys and values go: the place in the list behind what the cache holds
+    context [R]      tokens of request r that the cache holds
+    seen [N, words]  the rows' masks (:func:`tree_masks`)
+    """
+
+    places: torch.Tensor
+    context: torch.Tensor
+    seen: torch.Tensor
+
+
+@dataclass
 class StepContext:
     """Device tensors (int32) and host numbers that describe a step to the parts.
 
@@ -120,6 +143,27 @@ def tree_masks(trees: Sequence[Sequence[int]], words: Optional[int] = None):
             masks[at + i, i // 32] |= np.uint32(1 << (i % 32))
         at += len(tree)
     return masks.view(np.int32), depths
+
+
+def build_drafts(entries: Sequence[DraftEntry], manager: CacheManager, storage: CacheStorage, vocab_size: int, max_positions: int,
+                 device: torch.device) -> StepContext:
+    """The step of the entries' drafted tokens, all of whose logits are wanted.  Pages must already be reserved."""
+    for e in entries:
+        if len(e.parents) != len(e.tokens):
+            raise BatchError(f"request {e.rid!r}: {len(e.parents)} parents for {len(e.tokens)} drafted tokens")
+    masks, depths = tree_masks([e.parents for e in entries])
+    reach = max(int(d) for d in depths) + 1 if len(depths) else 0
+    for g, need in enumerate(storage.needs):
+        if need.window is not None and reach > need.window:
+            raise BatchError(f"drafted tokens {reach} deep do not fit a window of {need.window}")
+    context = [manager.n_tokens(e.rid) for e in entries]
+    ctx = build_context([StepEntry(e.rid, e.tokens, range(len(e.tokens))) for e in entries], manager, storage, vocab_size, max_positions, device)
+    places = ctx.positions.clone()
+    positions = np.repeat(np.asarray(context, dtype=np.int32), [len(e.tokens) for e in entries]) + depths
+    ctx.positions.copy_(torch.from_numpy(positions.astype(np.int32)))
+    ctx.extra["drafts"] = Drafts(places=places, context=torch.tensor(context, dtype=torch.int32, device=device),
+                                 seen=torch.from_numpy(masks).to(device))
+    return ctx
 
 
 def sorted_tiles(q_lens: Sequence[int], starts: Sequence[int], tokens_per_tile: int, portions_only: bool):

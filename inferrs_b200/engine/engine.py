@@ -15,7 +15,8 @@ import torch
 
 from ..config.base import generation_eos_ids
 from ..runtime import Runtime, parse_dtype
-from ..sampling.params import SamplingParams
+from .. import kernels
+from ..sampling.params import MOST_LOGPROBS, SamplingParams, TokenLogProbs
 from ..sampling.sampler import Sampler
 from .batch import StepEntry
 from .health import KernelHealth
@@ -148,14 +149,25 @@ class Engine:
         logits = self.runner.step(entries, own_output=False, carry=(before[1], sources) if carried else None)
         self.scheduler.advance(plan)
         sampling = [(e, s) for e, s in zip(plan, sources) if e.samples]
-        ids = host = event = None
+        ids = host = event = scores = None
         if sampling:
+            # rows whose log probabilities are wanted: the logits as they are, before the sampler's penalties change them
+            asked = [i for i, (e, _) in enumerate(sampling) if e.request.params.logprobs is not None]
+            plain = None
+            if asked:
+                at = torch.tensor(asked, dtype=torch.int64).to(logits.device)
+                plain = logits.index_select(0, at)
             pending = [int(s >= 0) for _, s in sampling]
             # a pending token is looked up on the device, where the step before left it
             pending_from = (before[1], [max(s, 0) for _, s in sampling]) if any(pending) else None
             ids = self.sampler.sample(logits, [e.request.params for e, _ in sampling],
                                       [e.request.seed for e, _ in sampling], [e.request for e, _ in sampling],
                                       pending, pending_from=pending_from)
+            if asked:
+                scores = self._scores(plain, ids.index_select(0, at).view(-1, 1), max(sampling[i][0].request.params.logprobs for i in asked))
+                if self.overlap:
+                    pinned = torch.empty(scores.shape, dtype=torch.float32, pin_memory=True)
+                    scores = pinned.copy_(scores, non_blocking=True)
             if self.overlap and ids.device.type == "cuda":
                 # the token ids start their way to pinned memory now; an event says when they are there
                 host = self._pinned.pop() if self._pinned else \
@@ -165,11 +177,52 @@ class Engine:
                 event.record()
         self.n_steps += 1
         self.n_tokens_run += sum(e.n for e in plan)
-        return plan, ids, host, event
+        return plan, ids, host, event, scores
+
+    def _scores(self, logits: torch.Tensor, tokens: torch.Tensor, top: int) -> torch.Tensor:
+        """float32 [rows, 2 + 2 top] on the device: log probability of the rows' tokens [rows, 1], entropy, the likeliest tokens' ids (as
+        numbers, exact up to 2^24) and log probabilities."""
+        n, dev = logits.shape[0], logits.device
+        log_probs = torch.empty((n, 1), dtype=torch.float32, device=dev)
+        entropy = torch.empty((n,), dtype=torch.float32, device=dev)
+        ids = torch.empty((n, top), dtype=torch.int32, device=dev)
+        best = torch.empty((n, top), dtype=torch.float32, device=dev)
+        kernels.token_log_probs(logits, tokens, log_probs, entropy, ids if top else None, best if top else None)
+        return torch.cat((log_probs, entropy[:, None], ids.to(torch.float32), best), dim=1)
+
+    @staticmethod
+    def _token_log_probs(token: int, row: Sequence[float], top: int) -> TokenLogProbs:
+        """One row of :meth:`_scores`, which may hold more of the likeliest tokens than this request asks for."""
+        n = (len(row) - 2) // 2
+        pairs = [(int(i), p) for i, p in zip(row[2:2 + n], row[2 + n:]) if i >= 0]
+        return TokenLogProbs(token, row[0], row[1], pairs[:top])
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenLogProbs]]:
+        """For every prompt the log probabilities that the model gives to its tokens from the second one on, each behind those
+        before it, with the ``top`` likeliest tokens at its place.  Needs a free slot and pages for one prompt at a time."""
+        if not 0 <= top <= MOST_LOGPROBS:
+            raise ValueError(f"top must be within 0 and {MOST_LOGPROBS}, got {top}")
+        out, portion = [], self.scheduler.max_tokens_per_step
+        for prompt in prompts:
+            prompt = [int(t) for t in prompt]
+            rid, found = ("score", next(self._ids)), []
+            self.runner.admit(rid)
+            try:
+                for start in range(0, len(prompt) - 1, portion):
+                    part = prompt[start:start + portion]
+                    following = prompt[start + 1:start + portion + 1]
+                    logits = self.runner.step([StepEntry(rid, part, list(range(len(following))))], own_output=False)
+                    ids = torch.tensor(following, dtype=torch.int32).to(logits.device)
+                    rows = self._scores(logits, ids.view(-1, 1), top).cpu().tolist()
+                    found += [self._token_log_probs(t, r, top) for t, r in zip(following, rows)]
+            finally:
+                self.runner.release(rid)
+            out.append(found)
+        return out
 
     def _finish(self, step) -> List[Request]:
         """Read a launched step's tokens and record them; returns the requests that ended with it."""
-        plan, ids, host, event = step
+        plan, ids, host, event, scores = step
         tokens: List[int] = []
         if ids is not None:
             if event is not None:
@@ -180,12 +233,16 @@ class Engine:
                 tokens = ids.cpu().tolist()
         # a request that ended while this step was already on its way ran in vain: it is left out
         alive, kept, it = [], [], iter(tokens)
+        rows = iter(scores.cpu().tolist() if scores is not None else ())
         for e in plan:
             tok = next(it) if e.samples else None
+            row = next(rows) if e.samples and e.request.params.logprobs is not None else None
             if e.request.finish_reason is None:
                 alive.append(e)
                 if e.samples:
                     kept.append(tok)
+                if row is not None:
+                    e.request.log_probs.append(self._token_log_probs(tok, row, e.request.params.logprobs))
             else:
                 self.n_steps_in_vain += 1
         return self.scheduler.deliver(alive, kept)

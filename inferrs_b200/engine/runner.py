@@ -12,7 +12,7 @@ The reference's nearest counterparts are ``CausalLM::forward_paged``
 """
 from __future__ import annotations
 
-from typing import Dict, Hashable, List, Optional, Sequence
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence
 
 import torch
 
@@ -20,7 +20,7 @@ from ..cache.manager import CacheManager, OutOfPages
 from ..cache.storage import CacheStorage, bytes_of_vectors
 from ..parts.spec import ModelSpec
 from ..runtime import Runtime
-from .batch import StepContext, StepEntry, build_context
+from .batch import BatchError, DraftEntry, StepContext, StepEntry, build_context, build_drafts
 from .model import Model, cache_needs, side_state_needs
 
 
@@ -48,6 +48,7 @@ class ModelRunner:
         self.manager = CacheManager(self.storage.layouts, page_size, self.storage.n_pages, max_requests)
         self.page_size = page_size
         self.steps_run = 0
+        self._drafted: Dict[Hashable, int] = {}      # drafted tokens of the requests' last step of drafts, until some are kept
         # decode steps are replayed as CUDA graphs when every part says its launches do not depend on
         # host-side values of the step (``graph_safe``)
         parts = [p for b in self.model.blocks for p in b.parts()] + [self.model.final_norm]
@@ -89,7 +90,31 @@ class ModelRunner:
         return slot
 
     def release(self, rid: Hashable):
+        self._drafted.pop(rid, None)
         self.manager.release(rid)
+
+    def fork(self, rid: Hashable, new_rid: Hashable) -> int:
+        """A new live request that holds what ``rid`` holds: its pages (copied, in all layers) and its fixed-size states.  Returns the
+        new request's slot; raises OutOfPages, and leaves everything as it was, where there is no room."""
+        n, slot = self.manager.n_tokens(rid), self.manager.slot(rid)
+        new_slot = self.manager.admit(new_rid)
+        try:
+            done = 0
+            while done < n:              # in portions, so that pages behind a window come back before the next ones are taken
+                k = min(n - done, 64 * self.page_size)
+                self.manager.reserve({new_rid: k})
+                self.manager.commit(new_rid, k)
+                done += k
+        except OutOfPages:
+            self.manager.release(new_rid)
+            raise
+        for g in range(len(self.manager.groups)):
+            pairs = [(a, b) for a, b in zip(self.manager.block_table(rid, g), self.manager.block_table(new_rid, g)) if a >= 0 and b >= 0]
+            if pairs and self.storage.members[g]:
+                both = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.rt.device)
+                self.storage.copy_pages(g, both[0], both[1])
+        self.storage.copy_slot(slot, new_slot)
+        return new_slot
 
     def has(self, rid: Hashable) -> bool:
         return self.manager.has(rid)
@@ -166,7 +191,56 @@ class ModelRunner:
     def commit(self, entries: Sequence[StepEntry]):
         for e in entries:
             self.manager.commit(e.rid, len(e.tokens))
+            self._drafted.pop(e.rid, None)       # (the step has written over drafted tokens that nobody kept)
         self.steps_run += 1
+
+    # ---- drafted tokens -------------------------------------------------------------------
+    def takes_drafts(self) -> bool:
+        """Whether the model's layers can run trees of drafted tokens (see :meth:`step_drafts`)."""
+        return not self.storage.states and not self.storage.side_states and all(
+            p.takes_drafts() if hasattr(p, "takes_drafts") else not hasattr(p, "cache_need")       # (a mixer says so itself)
+            for b in self.model.blocks for p in b.parts())
+
+    def step_drafts(self, entries: Sequence[DraftEntry]) -> torch.Tensor:
+        """float32 logits [number of drafted tokens, vocab] of trees of drafted tokens, each behind what its request holds and its
+        own ancestors.  Nothing of them is held yet: :meth:`keep_drafts` says what stays, and the next step without it writes over them."""
+        if not self.takes_drafts():
+            raise BatchError("this model has layers that cannot run a tree of drafted tokens")
+        wants = {e.rid: len(e.tokens) for e in entries}
+        if len(wants) != len(entries):
+            raise ValueError("a request appears twice in one step")
+        self.manager.reserve(wants)
+        ctx = build_drafts(entries, self.manager, self.storage, self.spec.vocab_size, self.spec.max_positions, self.rt.device)
+        logits = self.model.forward(ctx)
+        self._drafted.update(wants)
+        self.steps_run += 1
+        return logits
+
+    def keep_drafts(self, kept: Mapping[Hashable, Sequence[int]]):
+        """Of each request's drafted tokens those with the given places in their list stay, from the tree's root on down one path:
+        their keys and values move together behind what the request held.  A request without any keeps nothing."""
+        for rid, places in kept.items():
+            if rid not in self._drafted:
+                raise BatchError(f"request {rid!r} has no drafted tokens")
+            if any(not 0 <= p < self._drafted[rid] for p in places) or any(a >= b for a, b in zip(places, list(places)[1:])):
+                raise BatchError(f"request {rid!r}: the tokens that stay are ascending places among {self._drafted[rid]}, got {list(places)}")
+        moved = [rid for rid, places in kept.items() if list(places) != list(range(len(places)))]
+        if moved:
+            lists = [list(kept[rid]) for rid in moved]
+            most = max(len(x) for x in lists)
+            ints = lambda x: torch.tensor(x, dtype=torch.int32).to(self.rt.device)      # noqa: E731
+            context, n_kept = ints([self.manager.n_tokens(rid) for rid in moved]), ints([len(x) for x in lists])
+            places = ints([x + [0] * (most - len(x)) for x in lists])
+            for g in range(len(self.manager.groups)):
+                if not self.storage.members[g]:
+                    continue
+                tables = [self.manager.block_table(rid, g) for rid in moved]
+                width = max(len(t) for t in tables)
+                self.storage.keep_tokens(g, ints([t + [-1] * (width - len(t)) for t in tables]), context, places, n_kept)
+        for rid, places in kept.items():
+            if len(places):
+                self.manager.commit(rid, len(places))
+            del self._drafted[rid]
 
     def _decode_graph_takes(self, entries: Sequence[StepEntry]) -> bool:
         return self.graphs is not None and all(len(e.tokens) == 1 for e in entries) \

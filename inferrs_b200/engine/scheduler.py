@@ -45,6 +45,7 @@ class Request:
     n_preempted: int = 0
     order: int = 0                  # arrival number: smaller is older
     handle: int = -1                # the number by which native code knows the request
+    log_probs: list = field(default_factory=list)    # of the output's tokens, where the options ask for them (TokenLogProbs)
 
     @property
     def tokens(self) -> List[int]:

@@ -40,7 +40,7 @@ _SIGNATURES = {
     "ib_act_to_float": [c_void_p, c_void_p, c_long, c_void_p],
     "ib_qk_norm_rope_store": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
                               c_float,
-                              c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                              c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
     "ib_paged_attention_generic": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
                                    c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int, c_void_p,
@@ -701,7 +701,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_di
                        k_pages: Optional[torch.Tensor], v_pages: Optional[torch.Tensor], q_out: torch.Tensor,
                        interleaved: bool = False, norm_q: Optional[bool] = None, norm_k: Optional[bool] = None,
                        norm_after_rotation: bool = False, bias: Optional[torch.Tensor] = None,
-                       value_is_key: bool = False):
+                       value_is_key: bool = False, places: Optional[torch.Tensor] = None):
     """Per-head norm of q and k, rotation by position, q to ``q_out``, k and v into their pages.  Element ``i`` of
     a head's first ``rot_dim / 2`` turns with element ``i + rot_dim / 2``; ``interleaved``: element ``2i`` with ``2i + 1``.
 
@@ -709,7 +709,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_di
     given); a normed kind without a weight is divided and nothing else.  ``norm_after_rotation``: the norm comes
     after the rotation instead of before it.  Values may have another size than keys (the last size of ``v_pages``).
     ``bias`` (float32, one number per column of q, k and v) is added first.  ``value_is_key``: there are no value columns;
-    a value is its key as it was projected (with its bias), before norm and rotation.
+    a value is its key as it was projected (with its bias), before norm and rotation.  ``places`` (int32 [N]): a row's key and
+    value go to that place of its request instead of to its position (drafted tokens, several of which may share a position).
 
     qkv [N, at least n_heads * d + n_kv_heads * (d + dv)] (queries only when ``store_kv`` is False; columns behind
     them, a gate's for instance, are not read);
@@ -721,6 +722,9 @@ def qk_norm_rope_store(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_di
     _need(positions, "positions", _I, 1)
     _need(row_request, "row_request", _I, 1)
     n = qkv.shape[0]
+    _need(places, "places", _I, 1, optional=True)
+    if places is not None and places.shape[0] != n:
+        raise KernelError(f"qk_norm_rope_store: {places.shape[0]} places for {n} rows")
     v_dim = head_dim
     if store_kv:
         _need(v_pages, "v_pages", (act,), 4)
@@ -768,7 +772,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_di
     _check(_core(act).ib_qk_norm_rope_store(
         _p(qkv), ld, n, n_heads, n_kv_heads, head_dim, v_dim, int(store_kv), _p(q_weight), _p(k_weight),
         int(wdt == torch.float32), flags, float(eps), _p(cos) if rot_dim else None, _p(sin) if rot_dim else None, rot_dim,
-        int(bool(interleaved)), table_rows, _p(positions), _p(row_request), _p(block_table) if store_kv else None, max_pages, page_size,
+        int(bool(interleaved)), table_rows, _p(positions), _p(places), _p(row_request), _p(block_table) if store_kv else None, max_pages, page_size,
         n_pages, _p(k_pages) if store_kv else None, _p(v_pages) if store_kv else None, _p(q_out), _p(bias),
         int(bool(value_is_key)), _stream()), "qk_norm_rope_store")
 

@@ -252,10 +252,34 @@ class Attention:
     def middle(self, ctx, cache_id: int, h, proj: torch.Tensor, out: torch.Tensor, shares=None):
         self.attend(ctx, cache_id, proj, out)
 
+    def takes_drafts(self) -> bool:
+        """Whether this layer can run a tree of drafted tokens: grouped-query attention over all keys or a window, with its own keys and
+        values as the cache holds them, and nothing that shapes the scores."""
+        s = self.spec
+        return not (self.fused or self.talking or not s.own_kv or s.value_is_key or s.value_blend is not None or s.value_publish is not None
+                    or self.value_dim != s.head_dim or s.chunk or s.keep_first or self.rt.cache_bits is not None
+                    or any(x is not None for x in (self.head_scale, self.sinks, self.slopes, s.score_cap, s.head_gate)))
+
+    def _attend_drafts(self, ctx, cache_id: int, qkv: torch.Tensor, out: torch.Tensor, drafts):
+        """The same for trees of drafted tokens: a row turns by its depth in the tree, its key and value go to its place in the list."""
+        s = self.spec
+        k_pages, v_pages, group = ctx.storage.pages(cache_id)
+        table = ctx.block_tables[group]
+        q = torch.empty((qkv.shape[0], s.n_heads, s.head_dim), dtype=self.rt.dtype, device=qkv.device)
+        kernels.qk_norm_rope_store(qkv, s.n_heads, s.n_kv_heads, s.head_dim, True, self.q_weight, self.k_weight, self.eps, self.cos,
+                                   self.sin, self.rot_dim, ctx.positions, ctx.row_request, table, k_pages, v_pages, q,
+                                   interleaved=self.interleaved, norm_q=s.q_norm is not None, norm_k=s.k_norm is not None,
+                                   norm_after_rotation=s.norm_after_rotation, bias=self.store_bias, places=drafts.places)
+        kernels.paged_attention_tree(q, k_pages, v_pages, table, ctx.q_start, drafts.context, ctx.positions, drafts.seen, s.scale, self.span,
+                                     out, max_tree=ctx.max_q_len, max_kv_len=ctx.max_kv_len)
+
     def attend(self, ctx, cache_id: int, qkv: torch.Tensor, out: torch.Tensor):
         """From the projected rows to the heads side by side in ``out`` (whose rows may lie apart)."""
         s = self.spec
         n = qkv.shape[0]
+        if "drafts" in ctx.extra:
+            self._attend_drafts(ctx, cache_id, qkv, out, ctx.extra["drafts"])
+            return
         if self.rt.cache_bits is not None:
             self._attend_kv8(ctx, cache_id, qkv, out)
             return

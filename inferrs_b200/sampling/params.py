@@ -5,9 +5,23 @@ from __future__ import annotations
 import sys
 from array import array
 from dataclasses import dataclass, field
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 GREEDY_EPS = 1e-5  # temperatures below this pick the largest logit (sampler.rs:114, :176-179)
+
+
+MOST_LOGPROBS = 32       # likeliest tokens that can be asked for (kernels.MAX_TOP_LOG_PROBS)
+
+
+@dataclass
+class TokenLogProbs:
+    """What the model's distribution says of one token: its log probability, the distribution's entropy (nats), and the likeliest tokens
+    with theirs.  It is the distribution before temperature, penalties and cuts."""
+
+    token: int
+    log_prob: float
+    entropy: float
+    top: List[Tuple[int, float]] = field(default_factory=list)
 
 
 @dataclass
@@ -24,6 +38,7 @@ class SamplingParams:
     stop_token_ids: Tuple[int, ...] = ()  # the reference's extra_stop_token_ids
     seed: Optional[int] = None           # None: a fresh random seed per request
     ignore_eos: bool = False             # the reference's bypass_stop_tokens
+    logprobs: Optional[int] = None       # log probabilities of the generated tokens, with so many of the likeliest ones; None: off
 
     def __post_init__(self):
         if self.temperature < 0:
@@ -38,6 +53,8 @@ class SamplingParams:
             raise ValueError(f"max_tokens must be positive, got {self.max_tokens}")
         if self.repeat_last_n < 0:
             raise ValueError(f"repeat_last_n must be >= 0, got {self.repeat_last_n}")
+        if self.logprobs is not None and not 0 <= self.logprobs <= MOST_LOGPROBS:
+            raise ValueError(f"logprobs must be within 0 and {MOST_LOGPROBS} (or None), got {self.logprobs}")
         self.stop_token_ids = tuple(int(t) for t in self.stop_token_ids)
 
     @classmethod
