@@ -48,7 +48,8 @@ template <int D, int NQ> struct Shape {
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
     static constexpr int SLICE_SUMS = 2 * ROWS * (D + 2) + 4;      // floats of a slice's sums in the scratch: o [D / 4][line][4], m and l [line][2], whether it met bad values
     static constexpr int SMEM = 1024 + TILES + 256;
-    static_assert(SUMS + 6 * ROWS * 4 <= TILES, "the sums, references and denominators take the place of the tiles");
+    static_assert((NQ == 1 ? SUMS + 4 * ROWS * 4 : 0) + (NQ * ROWS + 8) * (OLD + 4) * 4 <= TILES, "the sums take the place of the tiles");
+    static_assert(SUMS + 4 * ROWS * 4 <= TILES, "the CTA's own sums too");
     // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
     static_assert(SMEM > 116 * 1024 && SMEM <= 232448, "one CTA an SM");
 };
@@ -217,15 +218,8 @@ __device__ __forceinline__ void visible(const Args& A, const Span& S, const Plac
                 if ((see[c] >> k & 1u) && key_index(A, p, jb + 32 * c + k) < 0) see[c] &= ~(1u << k);
 }
 
-__device__ __forceinline__ float4 remote_f32x4(const float* local, unsigned rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote(local, rank)));
-    return v;
-}
-__device__ __forceinline__ int remote_i32(const int* local, unsigned rank) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(local, rank)));
-    return v;
+__device__ __forceinline__ void remote_store(unsigned to, const float4& v) {      // into a CTA of the cluster (see remote)
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // A row's numbers e .. e + 3 with the infinite values and no numbers that it sees in tiles that not all rows see
@@ -259,6 +253,24 @@ __device__ __forceinline__ void join(float& top, float& total, float4& o, float 
     total = fmaf(l, b, total * a);
     o.x = fmaf(x.x, b, o.x * a); o.y = fmaf(x.y, b, o.y * a); o.z = fmaf(x.z, b, o.z * a); o.w = fmaf(x.w, b, o.w * a);
     top = to;
+}
+
+// N sums at once
+template <int N>
+__device__ __forceinline__ void join(const float (&m)[N], const float (&l)[N], const float4 (&x)[N], float& top, float& total, float4& o) {
+    top = m[0];
+#pragma unroll
+    for (int s = 1; s < N; ++s) top = fmaxf(top, m[s]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    total = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        if (l[s] == 0.0f) continue;
+        const float f = ex2(m[s] - ref);
+        total = fmaf(l[s], f, total);
+        o.x = fmaf(x[s].x, f, o.x); o.y = fmaf(x[s].y, f, o.y); o.z = fmaf(x[s].z, f, o.z); o.w = fmaf(x[s].w, f, o.w);
+    }
 }
 
 // numbers e .. e + 3 of a row (counted token by token) to their place
@@ -372,6 +384,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     // tiles that each stream takes
     const int count0 = NQ == 2 ? n : (n + 1) / 2, count1 = NQ == 2 ? (rows > ROWS ? n : 0) : n / 2;
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
+    // what the cluster's CTAs send this one: `most` rows of each (their sums; references, denominators and whether they met bad values).  With 128
+    // rows it lies behind the CTA's own sums.
+    const int most = (rows + parts - 1) / parts;
+    float* inbox = NQ == 1 ? part_l + 2 * ROWS : sums;
+    float* inbox_ml = inbox + parts * most * Sh::OLD;
     // keys that some row does not see
     auto partly = [&](int t) { return t * KEYS < lo_max || (t + 1) * KEYS > S.context; };
     bool ok = true;
@@ -638,6 +655,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (!mbar_wait(smem_u32(&sm.o_full), 0, 6)) ok = false;       // every product is done: the tiles' memory is free
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
+            if (scratch == nullptr && parts > 1) cluster_sync();          // the cluster's tiles are free: sums may go to any CTA
             if (NQ == 2 && parts == 1 && !none && !sm.bad_values) {
                 // no other sums of these rows: they go out from here, a thread a row
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -680,69 +698,92 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 }
                 *reinterpret_cast<float2*>(to + 2 * ROWS * D + 2 * all) = make_float2(m, ok ? l : NAN);
                 if (tid == 0) to[2 * ROWS * (D + 2)] = sm.bad_values ? 1.0f : 0.0f;
-            } else if (count > 0 && ok) {
-                float* row = sums + (g * ROWS + line) * Sh::OLD;
-#pragma unroll
+            } else if (NQ == 2 && parts > 1) {
+                // the only sums of a row that this CTA has: they go to the CTA that writes the row, a thread a row
+                const int row = g * ROWS + r, i = row / parts, owner = row - i * parts;
+                const unsigned to = remote(inbox + (part * most + i) * Sh::OLD, owner);
+#pragma unroll 1
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
                     tmem_ld32(o_at + e, x);
+                    if (!mine) continue;
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<uint4*>(row + e + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                        remote_store(to + (e + k) * 4, make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]), __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])));
                 }
+                if (mine) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(m, ok ? l : NAN, sm.bad_values ? 1.0f : 0.0f, 0.0f));
+            } else {
+                if (count > 0 && ok) {
+                    float* row = sums + (g * ROWS + line) * Sh::OLD;
+#pragma unroll
+                    for (int e = 0; e < D; e += 32) {
+                        unsigned x[32];
+                        tmem_ld32(o_at + e, x);
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<uint4*>(row + e + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                    }
+                }
+                part_m[g * ROWS + line] = m;
+                part_l[g * ROWS + line] = ok ? l : NAN;
             }
-            part_m[g * ROWS + line] = m;
-            part_l[g * ROWS + line] = l;
+        } else if (scratch == nullptr && parts > 1) {
+            cluster_sync();
         }
         fence_before();
     }
+    if (warp >= PRODUCERS && scratch == nullptr && parts > 1) cluster_sync();
     __syncthreads();
     if (warp == ISSUER) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
     if (none || (scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
-    // Join: first the sums that this CTA has of a row (of two streams, of two copies), then, a share of the rows for each, those of the
-    // cluster's CTAs.  Sixteen or 32 lanes a row, four numbers each; every sum comes in the same order whatever the grid.
+    // Join: first the sums that this CTA has of a row (of two streams, of two copies), which go to the CTA that writes the row (every parts-th),
+    // and there those of the cluster's CTAs.  What goes out is not waited for; a look into another CTA's memory takes 700 cycles.  Sixteen or
+    // 32 lanes a row, four numbers each; every sum comes in the same order whatever the grid.
     constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, PASS = THREADS / 32 * STEP_ROWS;
     const int here = (NQ == 1 ? 2 : 1) * copies, line0 = warp * STEP_ROWS + lane / LANES, e = lane % LANES * 4;
-    auto write = [&](int row, const float4& o, float total, bool bad) {
-        write_row<D>(A, S, place, first_row + row, head, e, o, total, bad, t_first, all_tiles, lo_max);
-    };
-    float *own_m = here > 1 ? part_l + 2 * ROWS : part_m, *own_l = here > 1 ? own_m + ROWS : part_l;      // of what this CTA has of a row
-    // (loops as they stand: this code runs once, and what an unrolled one gains it loses to the instructions' own way from memory)
-    if (here > 1 || parts == 1) {
+    if (NQ == 1 || parts == 1) {
 #pragma unroll 1
         for (int row = line0; row < rows; row += PASS) {
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float top = -INFINITY, total = 0.0f;
-#pragma unroll 1
-            for (int s = 0; s < here; ++s) {
-                const int line = row + s * block;                // (a stream's copies lie one behind the other)
-                join(top, total, o, part_m[line], part_l[line], *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e));
+            float4 x[4], o;
+            float m[4], l[4], top, total;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int line = row + (s < here ? s : 0) * block;        // (a stream's copies lie one behind the other)
+                m[s] = part_m[line];
+                l[s] = s < here ? part_l[line] : 0.0f;
+                x[s] = *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e);
             }
+            join<4>(m, l, x, top, total, o);
             if (parts == 1) {
-                write(row, o, total, sm.bad_values != 0);
+                write_row<D>(A, S, place, first_row + row, head, e, o, total, sm.bad_values != 0, t_first, all_tiles, lo_max);
             } else {
-                *reinterpret_cast<float4*>(sums + row * Sh::OLD + e) = o;
-                if (e == 0) { own_m[row] = top; own_l[row] = total; }
+                const int i = row / parts, owner = row - i * parts;
+                remote_store(remote(inbox + (part * most + i) * Sh::OLD + e, owner), o);
+                if (e == 0) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(top, total, sm.bad_values ? 1.0f : 0.0f, 0.0f));
             }
         }
     }
     if (parts == 1) return;
     cluster_sync();
-    bool bad_values = false;
-    for (int p = 0; p < parts; ++p) bad_values |= remote_i32(&sm.bad_values, p) != 0;
 #pragma unroll 1
-    for (int row = part + line0 * parts; row < rows; row += PASS * parts) {
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float top = -INFINITY, total = 0.0f;
-#pragma unroll 1
-        for (int p = 0; p < parts; ++p)
-            join(top, total, o, remote_f32(own_m + row, p), remote_f32(own_l + row, p), remote_f32x4(sums + row * Sh::OLD + e, p));
-        write(row, o, total, bad_values);
+    for (int i = line0; part + i * parts < rows; i += PASS) {
+        float4 x[MOST_PARTS], o;
+        float m[MOST_PARTS], l[MOST_PARTS], top, total, bad = 0.0f;
+#pragma unroll
+        for (int p = 0; p < MOST_PARTS; ++p) {
+            const int at = (p < parts ? p : 0) * most + i;
+            const float4 ml = *reinterpret_cast<const float4*>(inbox_ml + at * 4);
+            m[p] = ml.x;
+            l[p] = p < parts ? ml.y : 0.0f;
+            bad = fmaxf(bad, ml.z);
+            x[p] = *reinterpret_cast<const float4*>(inbox + at * Sh::OLD + e);
+        }
+        join<MOST_PARTS>(m, l, x, top, total, o);
+        write_row<D>(A, S, place, first_row + part + i * parts, head, e, o, total, bad != 0.0f, t_first, all_tiles, lo_max);
     }
-    cluster_sync();                   // nobody leaves while others read its sums
 }
 
 // The rows whose keys were cut into slices by CTAs that do not run together: their sums lie in memory, slice by slice.  A thread
