@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     b /= A.tiles_of_rows;
     const int head = b % A.n_kv, req = b / A.n_kv;
     const Span S = span_of(A, req);
-    const int group = A.n_heads / A.n_kv;
+    const int group = A.group;
     const int first_row = row_tile * ROWS, rows = S.n_tree * group - first_row;
     if (rows <= 0) return;                        // (the whole cluster leaves)
     const int used = rows < ROWS ? rows : ROWS;
@@ -244,7 +244,7 @@ static int launch_rows(const Args& A, int max_keys, cudaStream_t stream) {
 
 template <typename T>
 static int rows_of_type(Args A, int max_tree, int max_keys, cudaStream_t stream) {
-    A.tiles_of_rows = (int)(((long)max_tree * (A.n_heads / A.n_kv) + ROWS - 1) / ROWS);
+    A.tiles_of_rows = (int)(((long)max_tree * A.group + ROWS - 1) / ROWS);
     const int per = (A.dim + 31) / 32;
     if (per <= 1) return launch_rows<T, 1>(A, max_keys, stream);
     if (per <= 2) return launch_rows<T, 2>(A, max_keys, stream);
@@ -273,6 +273,8 @@ static int tree_args(const IbTreeAttention& c, tree::Args& A, int& max_tree, int
     A.n_requests = (int)c.n_requests; A.n_heads = (int)c.n_heads; A.n_kv = (int)c.n_kv; A.dim = (int)c.dim;
     A.max_pages = (int)c.max_pages; A.page_size = (int)c.page_size; A.n_pages = (int)c.n_pages; A.words = (int)c.words; A.span = (int)c.span;
     A.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctzl(c.page_size) : -1;
+    A.group = A.n_heads / A.n_kv;
+    A.group_shift = (A.group & (A.group - 1)) == 0 ? __builtin_ctz((unsigned)A.group) : -1;
     A.scale_log2 = (float)(c.scale * 1.4426950408889634);
     max_tree = (int)(c.max_tree < c.n_rows ? c.max_tree : c.n_rows);
     max_keys = (int)(c.max_keys < 0x3fffffffL ? c.max_keys : 0x3fffffffL);

@@ -194,6 +194,14 @@ __device__ __forceinline__ int key_index(const Args& A, const Place& p, int j) {
     return (page * A.n_kv + p.head) * A.page_size + (j - slot * A.page_size);
 }
 
+// those of the 32 keys from j on whose bit is set and whose page is there
+__device__ __noinline__ unsigned with_page(const Args& A, const Place p, int j, unsigned bits) {
+#pragma unroll 1
+    for (unsigned left = bits; left; left &= left - 1)
+        if (key_index(A, p, j + __ffs(left) - 1) < 0) bits &= ~(left & -left);
+    return bits;
+}
+
 // which of the 32 N keys from jb on a row sees; lo: the first key of the context that it sees
 template <int N>
 __device__ __forceinline__ void visible(const Args& A, const Span& S, const Place& p, const int* row_words, int lo, int jb, bool bad_pages,
@@ -212,10 +220,10 @@ __device__ __forceinline__ void visible(const Args& A, const Span& S, const Plac
         }
         see[c] = bits;
     }
-    if (bad_pages)
-        for (int c = 0; c < N; ++c)
-            for (int k = 0; k < 32; ++k)
-                if ((see[c] >> k & 1u) && key_index(A, p, jb + 32 * c + k) < 0) see[c] &= ~(1u << k);
+    if (bad_pages) {               // (rare, and long if it were unrolled: code that is fetched costs time even where it is not run)
+#pragma unroll
+        for (int c = 0; c < N; ++c) see[c] = with_page(A, p, jb + 32 * c, see[c]);
+    }
 }
 
 __device__ __forceinline__ void remote_store(unsigned to, const float4& v) {      // into a CTA of the cluster (see remote)
@@ -229,8 +237,10 @@ __device__ __noinline__ float4 with_bad_values(const Args& A, const Span S, cons
     const int lo = first_key(A, S, token);
     const int* words = A.seen + (long)(S.row0 + token) * A.words;
     float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll 1
     for (int t = t_first; t < t_first + n_tiles; ++t) {
         if (!(t * KEYS < lo_max || (t + 1) * KEYS > S.context)) continue;
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             unsigned see[1];
             visible(A, S, place, words, lo, t * KEYS + 32 * c, true, see);
@@ -246,47 +256,42 @@ __device__ __noinline__ float4 with_bad_values(const Args& A, const Span S, cons
     return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// The sum (m, l, x) joins a row's (top, total, o).  (A sum whose l is 0 is not there: what stands in its place is not used.)
-__device__ __forceinline__ void join(float& top, float& total, float4& o, float m, float l, const float4& x) {
+// The sum (m, l, the numbers at x and every 32 behind them) joins a row's (top, total, o).  (A sum whose l is 0 is not there: what stands in its
+// place is not used.)
+template <int QUADS>
+__device__ __forceinline__ void join(float& top, float& total, float4 (&o)[QUADS], float m, float l, const float* x, int step = 32) {
     if (l == 0.0f) return;
+    float4 v[QUADS];
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) v[k] = *reinterpret_cast<const float4*>(x + k * step);
     const float to = fmaxf(top, m), ref = to == -INFINITY ? 0.0f : to, a = ex2(top - ref), b = ex2(m - ref);
     total = fmaf(l, b, total * a);
-    o.x = fmaf(x.x, b, o.x * a); o.y = fmaf(x.y, b, o.y * a); o.z = fmaf(x.z, b, o.z * a); o.w = fmaf(x.w, b, o.w * a);
     top = to;
-}
-
-// N sums at once
-template <int N>
-__device__ __forceinline__ void join(const float (&m)[N], const float (&l)[N], const float4 (&x)[N], float& top, float& total, float4& o) {
-    top = m[0];
 #pragma unroll
-    for (int s = 1; s < N; ++s) top = fmaxf(top, m[s]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    total = 0.0f;
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-        if (l[s] == 0.0f) continue;
-        const float f = ex2(m[s] - ref);
-        total = fmaf(l[s], f, total);
-        o.x = fmaf(x[s].x, f, o.x); o.y = fmaf(x[s].y, f, o.y); o.z = fmaf(x[s].z, f, o.z); o.w = fmaf(x[s].w, f, o.w);
+    for (int k = 0; k < QUADS; ++k) {
+        o[k].x = fmaf(v[k].x, b, o[k].x * a); o[k].y = fmaf(v[k].y, b, o[k].y * a);
+        o[k].z = fmaf(v[k].z, b, o[k].z * a); o[k].w = fmaf(v[k].w, b, o[k].w * a);
     }
 }
 
-// numbers e .. e + 3 of a row (counted token by token) to their place
-template <int D>
-__device__ __forceinline__ void write_row(const Args& A, const Span& S, const Place& place, int at, int head, int e, float4 o, float total, bool bad_values,
-                                          int t_first, int n_tiles, int lo_max) {
+// numbers e .. e + 3 of a row (counted token by token), and every `step` behind them, to their place
+template <int D, int QUADS>
+__device__ __forceinline__ void write_row(const Args& A, const Span& S, const Place& place, int at, int head, int e, int step, float4 (&o)[QUADS],
+                                          float total, bool bad_values, int t_first, int n_tiles, int lo_max) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    const int group = A.n_heads / A.n_kv, token = at / group;
-    if (bad_values) o = with_bad_values<D>(A, S, place, o, token, e, t_first, n_tiles, lo_max);
+    const int group = A.group, token = A.group_shift >= 0 ? at >> A.group_shift : at / group;
     bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D + e;
-    if (((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-    } else {
-        dst[0] = __float2bfloat16_rn(o.x); dst[1] = __float2bfloat16_rn(o.y);
-        dst[2] = __float2bfloat16_rn(o.z); dst[3] = __float2bfloat16_rn(o.w);
+    const bool wide = ((unsigned)reinterpret_cast<uintptr_t>(A.out) | (unsigned)A.out_ld * 2) % 8 == 0;
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) {
+        float4 v = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+        if (bad_values) v = with_bad_values<D>(A, S, place, v, token, e + k * step, t_first, n_tiles, lo_max);
+        if (wide) {
+            *reinterpret_cast<uint2*>(dst + k * step) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+        } else {
+            bf16* to = dst + k * step;
+            to[0] = __float2bfloat16_rn(v.x); to[1] = __float2bfloat16_rn(v.y); to[2] = __float2bfloat16_rn(v.z); to[3] = __float2bfloat16_rn(v.w);
+        }
     }
 }
 
@@ -323,11 +328,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     int req = unit / A.tiles_of_rows;
     if (ranked) {                     // the longest contexts first: the grid's last CTAs are short ones
         int* lengths = reinterpret_cast<int*>(smem);
+#pragma unroll 1
         for (int i = tid; i < A.n_requests; i += THREADS) lengths[i] = A.context[i];
         __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < A.n_requests; i += THREADS) {
             const int mine = lengths[i];
             int ahead = 0;
+#pragma unroll 4
             for (int j = 0; j < A.n_requests; ++j) ahead += lengths[j] > mine || (lengths[j] == mine && j < i);
             if (ahead == req) sm.req = i;
         }
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         req = sm.req;
     }
     const Span S = span_of(A, req);
-    const int group = A.n_heads / A.n_kv;
+    const int group = A.group;
     const int first_row = row_tile * (NQ * ROWS);
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (rows <= 0) return;            // (the whole cluster leaves)
@@ -352,7 +360,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp == PRODUCERS && lane == 0) {
+#pragma unroll 1
         for (int i = 0; i < Sh::STAGES; ++i) { mbar_init(smem_u32(&sm.full[i]), 32 * N_PRODUCERS); mbar_init(smem_u32(&sm.empty[i]), 1); }
+#pragma unroll 1
         for (int g = 0; g < 2; ++g) {
             const int used = NQ == 2 ? rows - g * ROWS : rows;
             mbar_init(smem_u32(&sm.s_full[g]), 1);
@@ -367,6 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     fence_after();
     if (A.span != 0) {                // the first keys that the CTA's rows see: the least and the greatest
         const int t0 = first_row / group, t1 = (first_row + rows - 1) / group;
+#pragma unroll 1
         for (int t = t0 + tid; t <= t1; t += THREADS) {
             const int lo = first_key(A, S, t);
             atomicMin(&sm.lo_min, lo);
@@ -386,7 +397,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
     // what the cluster's CTAs send this one: `most` rows of each (their sums; references, denominators and whether they met bad values).  With 128
     // rows it lies behind the CTA's own sums.
-    const int most = (rows + parts - 1) / parts;
+    const int most = (rows + parts - 1) / parts, over = 65536 / parts + 1;
+    auto share_of = [&](int row) { return row * over >> 16; };        // row / parts, for rows below 256 and up to eight parts
     float* inbox = NQ == 1 ? part_l + 2 * ROWS : sums;
     float* inbox_ml = inbox + parts * most * Sh::OLD;
     // keys that some row does not see
@@ -442,12 +454,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 if (lane * box < KEYS && w < D / 64)
                     tma_load_2d(dst + w * (ROWS * 128) + lane * box * 128, values ? &map_v : &map_k, w * 64, index[0], full);
             } else {
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < 4; ++h)
-                    load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), index[h >> 1], 16 * (h & 1), w * 4 + h, lane);
+                    load_rows<D>(dst, static_cast<const bf16*>(values ? A.v : A.k), h < 2 ? index[0] : index[1], 16 * (h & 1), w * 4 + h, lane);
                 if (values && partly(t)) {
                     cp_wait_all();
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 4; ++h)
                         if (clean_rows<D>(dst, w * 4 + h, lane)) sm.bad_values = 1;
                     mbar_arrive(full);
@@ -545,7 +557,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             bool bad = false;
             if (n > 0) {
                 const int j0 = max(t_begin * KEYS, lo_min), j1 = min(t_end * KEYS, S.keys);
-                for (int slot = j0 / A.page_size + lane; (long)slot * A.page_size < j1; slot += 32) {
+#pragma unroll 1
+                for (int slot = A.page_shift >= 0 ? (j0 >> A.page_shift) + lane : j0 / A.page_size + lane; (long)slot * A.page_size < j1; slot += 32) {
                     const int page = place.bt[slot];
                     if (page < 0 || page >= A.n_pages) bad = true;
                 }
@@ -698,9 +711,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 }
                 *reinterpret_cast<float2*>(to + 2 * ROWS * D + 2 * all) = make_float2(m, ok ? l : NAN);
                 if (tid == 0) to[2 * ROWS * (D + 2)] = sm.bad_values ? 1.0f : 0.0f;
-            } else if (NQ == 2 && parts > 1) {
+            } else if (NQ == 2) {
                 // the only sums of a row that this CTA has: they go to the CTA that writes the row, a thread a row
-                const int row = g * ROWS + r, i = row / parts, owner = row - i * parts;
+                const int row = g * ROWS + r, i = share_of(row), owner = row - i * parts;
                 const unsigned to = remote(inbox + (part * most + i) * Sh::OLD, owner);
 #pragma unroll 1
                 for (int e = 0; e < D; e += 32) {
@@ -740,49 +753,40 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     }
     if (none || (scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
     // Join: first the sums that this CTA has of a row (of two streams, of two copies), which go to the CTA that writes the row (every parts-th),
-    // and there those of the cluster's CTAs.  What goes out is not waited for; a look into another CTA's memory takes 700 cycles.  Sixteen or
-    // 32 lanes a row, four numbers each; every sum comes in the same order whatever the grid.
-    constexpr int LANES = D / 4, STEP_ROWS = 32 / LANES, PASS = THREADS / 32 * STEP_ROWS;
-    const int here = (NQ == 1 ? 2 : 1) * copies, line0 = warp * STEP_ROWS + lane / LANES, e = lane % LANES * 4;
-    if (NQ == 1 || parts == 1) {
+    // and there those of the cluster's CTAs.  What goes out is not waited for; a look into another CTA's memory takes 700 cycles.  Eight lanes
+    // a row, and loops as they stand: this code runs once, and unrolled ones wait for their instructions (ten cycles each) longer than they
+    // save.  Every sum comes in the same order whatever the grid.
+    constexpr int QUADS = D / 32, PASS = THREADS / 8;
+    const int line0 = tid >> 3, e = (lane & 7) * 4;              // a lane's numbers: e .. e + 3 and every 32 behind them
+    if (NQ == 1) {
 #pragma unroll 1
         for (int row = line0; row < rows; row += PASS) {
-            float4 x[4], o;
-            float m[4], l[4], top, total;
+            float4 o[QUADS] = {};
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+            for (int line = row; line < 2 * ROWS; line += block)          // (a stream's copies lie one behind the other)
+                join<QUADS>(top, total, o, part_m[line], part_l[line], sums + line * Sh::OLD + e);
+            const int i = share_of(row), owner = row - i * parts;
+            const unsigned to = remote(inbox + (part * most + i) * Sh::OLD + e, owner);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int line = row + (s < here ? s : 0) * block;        // (a stream's copies lie one behind the other)
-                m[s] = part_m[line];
-                l[s] = s < here ? part_l[line] : 0.0f;
-                x[s] = *reinterpret_cast<const float4*>(sums + line * Sh::OLD + e);
-            }
-            join<4>(m, l, x, top, total, o);
-            if (parts == 1) {
-                write_row<D>(A, S, place, first_row + row, head, e, o, total, sm.bad_values != 0, t_first, all_tiles, lo_max);
-            } else {
-                const int i = row / parts, owner = row - i * parts;
-                remote_store(remote(inbox + (part * most + i) * Sh::OLD + e, owner), o);
-                if (e == 0) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(top, total, sm.bad_values ? 1.0f : 0.0f, 0.0f));
-            }
+            for (int k = 0; k < QUADS; ++k) remote_store(to + k * 128, o[k]);
+            if (e == 0) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(top, total, sm.bad_values ? 1.0f : 0.0f, 0.0f));
         }
     }
-    if (parts == 1) return;
-    cluster_sync();
+    if (parts > 1) cluster_sync();
+    else __syncthreads();
 #pragma unroll 1
     for (int i = line0; part + i * parts < rows; i += PASS) {
-        float4 x[MOST_PARTS], o;
-        float m[MOST_PARTS], l[MOST_PARTS], top, total, bad = 0.0f;
-#pragma unroll
-        for (int p = 0; p < MOST_PARTS; ++p) {
-            const int at = (p < parts ? p : 0) * most + i;
+        float4 o[QUADS] = {};
+        float top = -INFINITY, total = 0.0f, bad = 0.0f;
+#pragma unroll 1
+        for (int p = 0; p < parts; ++p) {
+            const int at = p * most + i;
             const float4 ml = *reinterpret_cast<const float4*>(inbox_ml + at * 4);
-            m[p] = ml.x;
-            l[p] = p < parts ? ml.y : 0.0f;
             bad = fmaxf(bad, ml.z);
-            x[p] = *reinterpret_cast<const float4*>(inbox + at * Sh::OLD + e);
+            join<QUADS>(top, total, o, ml.x, ml.y, inbox + at * Sh::OLD + e);
         }
-        join<MOST_PARTS>(m, l, x, top, total, o);
-        write_row<D>(A, S, place, first_row + part + i * parts, head, e, o, total, bad != 0.0f, t_first, all_tiles, lo_max);
+        write_row<D, QUADS>(A, S, place, first_row + part + i * parts, head, e, 32, o, total, bad != 0.0f, t_first, all_tiles, lo_max);
     }
 }
 
@@ -794,12 +798,13 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     const int unit = blockIdx.x / CHUNKS, at = blockIdx.x % CHUNKS * 256 + threadIdx.x, row = at % (NQ * ROWS), e = at / (NQ * ROWS) * 16;
     const int head = unit % A.n_kv, row_tile = unit / A.n_kv % A.tiles_of_rows, req = unit / A.n_kv / A.tiles_of_rows;
     const Span S = span_of(A, req);
-    const int group = A.n_heads / A.n_kv, first_row = row_tile * (NQ * ROWS);
+    const int group = A.group, first_row = row_tile * (NQ * ROWS);
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (row >= rows) return;
     int lo_min = 0, lo_max = 0;
     if (A.span != 0) {
         lo_min = 0x7fffffff;
+#pragma unroll 1
         for (int t = first_row / group; t <= (first_row + rows - 1) / group; ++t) {
             const int lo = first_key(A, S, t);
             lo_min = min(lo_min, lo);
@@ -814,25 +819,16 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     float top = -INFINITY, total = 0.0f;
     bool bad_values = false;
     const float* from = scratch + (long)unit * slices * SUMS;
+#pragma unroll 2
     for (int p = 0; p < parts * here; ++p) {
         const float* slice = from + (long)(p / here) * SUMS;
         const int line = row + p % here * (ROWS / copies);
         const float2 ml = *reinterpret_cast<const float2*>(slice + 2 * ROWS * D + 2 * line);
-        float4 x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(slice + ((e / 4 + k) * (2 * ROWS) + line) * 4);
         bad_values |= slice[2 * ROWS * (D + 2)] != 0.0f;
-        const float before = top, sum = total;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            top = before;
-            total = sum;
-            join(top, total, o[k], ml.x, ml.y, x[k]);
-        }
+        join<4>(top, total, o, ml.x, ml.y, slice + (e / 4 * (2 * ROWS) + line) * 4, 2 * ROWS * 4);
     }
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) write_row<D>(A, S, place, first_row + row, head, e + 4 * k, o[k], total, bad_values, t_first, all_tiles, lo_max);
+    write_row<D, 4>(A, S, place, first_row + row, head, e, 4, o, total, bad_values, t_first, all_tiles, lo_max);
 }
 
 template <int D, int NQ>

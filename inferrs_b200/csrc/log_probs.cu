@@ -132,13 +132,14 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
 
 // The k best of the first n notes to best[0 .. min(k, n)) in descending order, by counting the keys ahead of each (keys differ:
 // they hold their places), four threads a key where there are few.  The threads that look at logits call it between two meetings.
-__device__ __forceinline__ void rank_notes(const u64* notes, int n, int k, u64* best) {
-    const int share = n <= THREADS / 4 ? 4 : 1, part = threadIdx.x & (share - 1);
-    for (int i0 = 0; i0 < n; i0 += THREADS / share) {
-        const int i = i0 + threadIdx.x / share;
+__device__ __noinline__ void rank_notes(const u64* notes, int n, int k, u64* best) {
+    const int log = n <= THREADS / 4 ? 2 : 0, share = 1 << log, part = threadIdx.x & (share - 1);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += THREADS >> log) {
+        const int i = i0 + (threadIdx.x >> log);
         const u64 mine = i < n ? notes[i] : ~0ull;
         int ahead = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (int j = part; j < n; j += share) ahead += notes[j] > mine;
         if (share == 4) {
             ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);

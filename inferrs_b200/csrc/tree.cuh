@@ -14,6 +14,7 @@ struct Args {
     long out_ld;
     int n_rows, n_requests, n_heads, n_kv, dim, max_pages, page_size, n_pages, words, span, tiles_of_rows;
     int page_shift;            // log2 of the page size, -1: it is no power of two
+    int group, group_shift;    // query heads of a key/value head, their log2 or -1
     float scale_log2;          // scale * log2(e)
 };
 
