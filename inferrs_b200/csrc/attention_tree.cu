@@ -13,17 +13,15 @@
 
 namespace tree {
 
-// ---- any type and head size: 32-bit arithmetic, 16 rows a CTA, four for each warp ----------------------------------------
-constexpr int ROWS = 16, KEYS = 32, WARPS = 4, MINE = ROWS / WARPS;
+// ---- any type and head size: 32-bit arithmetic, eight or 16 rows a CTA, two or four for each warp ----------------------------------------
+constexpr int KEYS = 32, WARPS = 4;
 
-// Shared memory: the rows' queries (later the part's sums), two tiles of keys and values as they lie in the cache, in rows that start 16 bytes
+// Shared memory: the rows' queries (later the part's sums), a tile of keys and values as they lie in the cache, in rows that start 16 bytes
 // off a multiple of 128 (a lane a key: eight lanes' 16 bytes meet all banks), references and denominators.
 __host__ __device__ __forceinline__ int padded(int dim) { return (dim + 3) / 4 * 4; }
 template <typename T> __host__ __device__ __forceinline__ int row_bytes(int dim) { return (dim * (int)sizeof(T) + 15) / 16 * 16 + 16; }
-// two tiles, one that is used and one that is on its way, where there is room for them
-template <typename T> __host__ __device__ __forceinline__ int turns(int dim) { return row_bytes<T>(dim) <= 1088 ? 2 : 1; }
-template <typename T> __host__ __device__ __forceinline__ size_t rows_smem(int dim) {
-    return sizeof(float) * (size_t)(ROWS * padded(dim) + 2 * ROWS) + 2 * turns<T>(dim) * (size_t)KEYS * row_bytes<T>(dim);
+template <typename T> __host__ __device__ __forceinline__ size_t rows_smem(int dim, int rows) {
+    return sizeof(float) * (size_t)(rows * padded(dim) + 2 * rows) + 2 * (size_t)KEYS * row_bytes<T>(dim);
 }
 
 __device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
@@ -32,16 +30,18 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
     return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-// What bounds it are instructions (a product of 32 bits takes one for 32 of them), few CTAs' latency, or what comes from memory where there are
-// few rows: 328 heads of requests with 2,000 keys each and eight rows, 754 MB, go at the copy's rate.  PER numbers of a head per lane, four
-// neighbours where that is a multiple of four.
-template <typename T, int PER>
+// What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles, four fifths of them waits), so what counts is
+// how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows: 355 us, with two 443),
+// and eight rows a CTA where there are no more or few CTAs (the same: 264 us; 2 trees of 13 over up to 777: 31.5 and 35.6).  PER numbers of a
+// head per lane, four neighbours where that is a multiple of four.
+template <typename T, int PER, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts, bool wide) {
+    constexpr int MINE = ROWS / WARPS;
     extern __shared__ __align__(16) unsigned char raw[];
     const int d = A.dim, dp = padded(d), rb = row_bytes<T>(d);
     float* sq = reinterpret_cast<float*>(raw);    // [ROWS][dp], later the part's sums
     float* sml = sq + ROWS * dp;                  // [2][ROWS]
-    unsigned char* tiles = reinterpret_cast<unsigned char*>(sml + 2 * ROWS);      // [2 in turn][keys, values][KEYS][rb]
+    unsigned char* tile = reinterpret_cast<unsigned char*>(sml + 2 * ROWS);       // [keys, values][KEYS][rb]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int b = blockIdx.x;
     const int part = b % parts;
@@ -64,10 +64,12 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         lo[r] = token[r] >= 0 ? first_key(A, S, token[r]) : 0;
     }
     if (A.span == 0) lo_min = 0;
-    else for (int t = first_row / group; t <= (first_row + used - 1) / group; ++t) lo_min = min(lo_min, first_key(A, S, t));
+    else
+#pragma unroll 1
+    for (int t = first_row / group; t <= (first_row + used - 1) / group; ++t) lo_min = min(lo_min, first_key(A, S, t));
     lo_min = min(lo_min, S.context);              // (the drafted tokens are looked at in any case)
     const int t0 = lo_min / KEYS, n_tiles = (S.keys + KEYS - 1) / KEYS - t0;
-    const int begin = t0 + (int)((long)n_tiles * part / parts), end = t0 + (int)((long)n_tiles * (part + 1) / parts);
+    const int begin = t0 + n_tiles * part / parts, end = t0 + n_tiles * (part + 1) / parts;       // (fewer than 2^26 tiles)
     const int* bt = A.table + (long)req * A.max_pages;
     auto look_up = [&](int t) -> long {           // where this lane's key of a tile lies
         const int j = t * KEYS + lane;
@@ -75,9 +77,8 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         const int slot = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size, page = bt[slot];
         return page >= 0 && page < A.n_pages ? ((long)page * A.n_kv + head) * A.page_size + j - slot * A.page_size : -1;
     };
-    auto load = [&](int t, long at) {             // a warp brings every fourth of the tile's keys
-        unsigned char* tile = tiles + (t & (turns<T>(d) - 1)) * (2 * KEYS * rb);
-#pragma unroll 2
+    auto load = [&](long at) {                    // a warp brings every fourth of the tile's keys
+#pragma unroll 1
         for (int i = 0; i < KEYS / WARPS; ++i) {
             const int key = i * WARPS + warp;
             const long from = __shfl_sync(0xffffffffu, at, key);
@@ -85,6 +86,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
             const T* v = static_cast<const T*>(A.v) + (from < 0 ? 0 : from) * d;
             unsigned char *to_k = tile + key * rb, *to_v = to_k + KEYS * rb;
             if (wide) {
+#pragma unroll 1
                 for (int c = lane; c < d * (int)sizeof(T) / 16; c += 32) {
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to_k + c * 16)),
                                  "l"(reinterpret_cast<const uint4*>(k) + c), "r"(from < 0 ? 0 : 16) : "memory");
@@ -92,6 +94,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
                                  "l"(reinterpret_cast<const uint4*>(v) + c), "r"(from < 0 ? 0 : 16) : "memory");
                 }
             } else {
+#pragma unroll 1
                 for (int e = lane; e < dp; e += 32) {
                     const bool some = from >= 0 && e < d;
                     reinterpret_cast<T*>(to_k)[e] = some ? k[e] : ib_from_float<T>(0.0f);
@@ -99,14 +102,15 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
                 }
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     long at = look_up(begin), at_next = look_up(begin + 1);
-    load(begin, at);
+    load(at);
     const T* q = static_cast<const T*>(A.q);
+#pragma unroll 1
     for (int i = warp; i < ROWS; i += WARPS) {
         const int row = first_row + i, tok = row / group;
         const T* from = q + ((long)(S.row0 + tok) * A.n_heads + head * group + row - tok * group) * d;
+#pragma unroll 1
         for (int e = lane; e < dp; e += 32) sq[i * dp + e] = i < used && e < d ? ib_to_float(from[e]) * A.scale_log2 : 0.0f;
     }
 
@@ -124,20 +128,13 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         const int j = t * KEYS + lane;            // every lane's own key
         const long next = at_next;
         at_next = look_up(t + 2);
-        const bool ahead = turns<T>(d) == 2;
-        if (ahead) {
-            load(t + 1, next);                    // (behind the last tile zeros)
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        const unsigned char* tile = tiles + (t & (turns<T>(d) - 1)) * (2 * KEYS * rb);
         const T* sk = reinterpret_cast<const T*>(tile + lane * rb);
         float dot[MINE];
 #pragma unroll
         for (int r = 0; r < MINE; ++r) dot[r] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int e = 0; e < dp; e += 4) {
             const float4 kk = four(sk + e);
 #pragma unroll
@@ -190,7 +187,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         }
         at = next;
         __syncthreads();                          // the tile has been read
-        if (!ahead) load(t + 1, next);
+        if (t + 1 < end) load(next);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     // join the parts: each CTA writes every parts-th row
@@ -204,13 +201,16 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         if (lane == 0) { sml[row] = m[r]; sml[ROWS + row] = l[r]; }
     }
     if (parts > 1) cluster_sync(); else __syncthreads();
+#pragma unroll 1
     for (int row = part + warp * parts; row < used; row += WARPS * parts) {
         float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
         for (int c = 0; c < parts; ++c) top = fmaxf(top, remote_f32(&sml[row], c));
         const float ref = top == -INFINITY ? 0.0f : top;
         float o[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+#pragma unroll 1
         for (int c = 0; c < parts; ++c) {
             const float lc = remote_f32(&sml[ROWS + row], c);
             if (lc == 0.0f) continue;             // this part of the keys holds none that the row sees
@@ -230,29 +230,32 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     if (parts > 1) cluster_sync();                // nobody leaves while others read its sums
 }
 
-template <typename T, int PER>
-static int launch_rows(const Args& A, int max_keys, cudaStream_t stream) {
+template <typename T, int PER, int ROWS>
+static int launch_rows(Args A, int max_tree, int max_keys, cudaStream_t stream) {
     static IbDeviceSet done;
-    const size_t smem = rows_smem<T>(A.dim);
-    if (const int code = ib_allow_dynamic_smem(done, tree_rows_kernel<T, PER>, rows_smem<T>(32 * PER))) return code;
+    if (const int code = ib_allow_dynamic_smem(done, tree_rows_kernel<T, PER, ROWS>, rows_smem<T>(32 * PER, ROWS))) return code;
+    A.tiles_of_rows = (int)(((long)max_tree * A.group + ROWS - 1) / ROWS);
     const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
-    int parts = 1;
-    while (parts < MAX_CLUSTER && pairs * parts * 2 <= 592 && max_keys >= 2 * KEYS * parts * 2) parts *= 2;
+    int parts = 1;       // about ten CTAs an SM, two or more that run and as many that follow them
+    while (parts < MAX_CLUSTER && pairs * parts * 2 <= 10 * 148 && max_keys >= 2 * KEYS * parts * 2) parts *= 2;
     const bool wide = (reinterpret_cast<uintptr_t>(A.k) | reinterpret_cast<uintptr_t>(A.v) | (uintptr_t)(A.dim * sizeof(T))) % 16 == 0;
-    return launch_cluster(tree_rows_kernel<T, PER>, pairs * parts, parts, WARPS * 32, smem, stream, A, parts, wide);
+    return launch_cluster(tree_rows_kernel<T, PER, ROWS>, pairs * parts, parts, WARPS * 32, rows_smem<T>(A.dim, ROWS), stream, A, parts, wide);
+}
+
+template <typename T, int PER>
+static int rows_of_heads(const Args& A, int max_tree, int max_keys, cudaStream_t stream) {
+    const long rows = (long)max_tree * A.group;
+    const bool few = rows <= 8 || (long)A.n_requests * A.n_kv * ((rows + 7) / 8) <= 148;
+    return few ? launch_rows<T, PER, 8>(A, max_tree, max_keys, stream) : launch_rows<T, PER, 16>(A, max_tree, max_keys, stream);
 }
 
 template <typename T>
-static int rows_of_type(Args A, int max_tree, int max_keys, cudaStream_t stream) {
-    A.tiles_of_rows = (int)(((long)max_tree * A.group + ROWS - 1) / ROWS);
+static int rows_of_type(const Args& A, int max_tree, int max_keys, cudaStream_t stream) {
     const int per = (A.dim + 31) / 32;
-    if (per <= 1) return launch_rows<T, 1>(A, max_keys, stream);
-    if (per <= 2) return launch_rows<T, 2>(A, max_keys, stream);
-    if (per <= 3) return launch_rows<T, 3>(A, max_keys, stream);
-    if (per <= 4) return launch_rows<T, 4>(A, max_keys, stream);
-    if (per <= 6) return launch_rows<T, 6>(A, max_keys, stream);
-    if (per <= 8) return launch_rows<T, 8>(A, max_keys, stream);
-    return launch_rows<T, 16>(A, max_keys, stream);
+    if (per <= 2) return rows_of_heads<T, 2>(A, max_tree, max_keys, stream);
+    if (per <= 4) return rows_of_heads<T, 4>(A, max_tree, max_keys, stream);
+    if (per <= 8) return rows_of_heads<T, 8>(A, max_tree, max_keys, stream);
+    return rows_of_heads<T, 16>(A, max_tree, max_keys, stream);
 }
 
 }  // namespace tree
