@@ -55,7 +55,7 @@ template <int D, int NQ> struct Shape {
 };
 
 struct Small {                 // what stands behind the tiles
-    unsigned long long full[8], empty[8], s_full[2], p_full[2], o_full, q_full;
+    unsigned long long full[8], empty[8], s_full[2], p_full[2][2], o_full, q_full;
     unsigned tmem;
     int req, lo_min, lo_max, bad_values;
 };
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         for (int g = 0; g < 2; ++g) {
             const int used = NQ == 2 ? rows - g * ROWS : rows;
             mbar_init(smem_u32(&sm.s_full[g]), 1);
-            mbar_init(smem_u32(&sm.p_full[g]), used <= 0 ? 1 : used >= ROWS ? 4 : copies * ((used + 31) / 32));
+            for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&sm.p_full[g][h]), used <= 0 ? 1 : used >= ROWS ? 4 : copies * ((used + 31) / 32));
         }
         mbar_init(smem_u32(&sm.o_full), 1);
         mbar_init(smem_u32(&sm.q_full), 256);
@@ -519,11 +519,19 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         for (int i = 0; i < count0 && ok; ++i) {
             for (int g = 0; g < 2 && ok; ++g) {
                 if (i >= (g ? count1 : count0)) continue;
-                if (!mbar_wait(smem_u32(&sm.p_full[g]), i & 1, 4) || !arrived(v_at)) { ok = false; break; }
+                // the products with the first half's P run while the threads make the second half's
+                const unsigned v = ring0 + v_at.slot * (Sh::TILE >> 4);
+                if (!mbar_wait(smem_u32(&sm.p_full[g][0]), i & 1, 4) || !arrived(v_at)) { ok = false; break; }
                 if (leader) {
-                    const unsigned v = ring0 + v_at.slot * (Sh::TILE >> 4);
 #pragma unroll
-                    for (int s = 0; s < KEYS / 16; ++s)
+                    for (int s = 0; s < KEYS / 32; ++s)
+                        umma_ts(tm + 256 + g * 128, tm + g * 128 + s * 8, words(v + s * (16 * 128 >> 4) + V_LO, V_HI), idesc_o, (i | s) != 0);
+                }
+                if (!mbar_wait(smem_u32(&sm.p_full[g][1]), i & 1, 4)) { ok = false; break; }
+                fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int s = KEYS / 32; s < KEYS / 16; ++s)
                         umma_ts(tm + 256 + g * 128, tm + g * 128 + s * 8, words(v + s * (16 * 128 >> 4) + V_LO, V_HI), idesc_o, (i | s) != 0);
                     if (NQ == 1 || g == last) umma_commit(smem_u32(&sm.empty[v_at.slot]));
                 }
@@ -644,7 +652,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 };
                 weigh(x, 2 * copy);
                 weigh(x + 32, 2 * copy + 1);
+                auto hand_over = [&](int h) {
+                    tmem_st_wait();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[g][h]));
+                };
                 if (copies == 1) {
+                    hand_over(0);
                     tmem_ld64(s_at + 64, x);
                     hide(x, 0, 2);
                     hide(x, 32, 3);
@@ -656,14 +671,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     for (int k = 0; k < 16; ++k) zeros[k] = 0;
                     tmem_st16(s_at + 32 * (copy ^ 1), zeros);
                     tmem_st16(s_at + 32 * (copy ^ 1) + 16, zeros);
+                    hand_over(0);
                 }
                 float a, b;
                 apart(add2(add[0], add[1]), a, b);
                 l += a + b;
-                tmem_st_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[g]));
+                hand_over(1);
             }
             if (!mbar_wait(smem_u32(&sm.o_full), 0, 6)) ok = false;       // every product is done: the tiles' memory is free
             ok = __all_sync(0xffffffffu, ok);
