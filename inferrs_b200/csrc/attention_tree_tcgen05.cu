@@ -31,7 +31,7 @@ constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
 constexpr int MOST_PARTS = 8;
-constexpr int SLICE = 16, MOST_SLICES = 64;
+constexpr int SLICE = 24, MOST_SLICES = 64;      // tiles (see launch)
 constexpr int RANKED = 1024;          // requests that are put in order of their length
 
 __device__ int g_error = 0;
@@ -850,7 +850,9 @@ static long launch(Args A, int max_tree, int max_keys, void* workspace, bool ask
     const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
     const int tiles = (max_keys + KEYS - 1) / KEYS;
     // One wave of CTAs: as many parts as there are SMs for, a cluster each.  More than that: requests differ in length, and clusters would wait
-    // for as many free SMs at once; slices of 16 tiles or more, the longest requests first, are joined by a kernel of their own.
+    // for as many free SMs at once; slices of 24 tiles or more, the longest requests first, are joined by a kernel of their own.  (Trees of 64,
+    // 32 heads on 8, 16 requests of 100 to 16,384 keys: slices of 12, 16, 24, 32 tiles 190, 180, 167, 178 us, whole requests 246; all of 16,384:
+    // 325, 306, 305, 299; of 100 to 4,500: 67, 73, and whole ones, which 24 leaves them, 73.)
     const bool waves = 2 * pairs > 148 && tiles > 2 * SLICE;
     long parts = waves ? (tiles + SLICE - 1) / SLICE : 148 / pairs;
     if (parts > tiles) parts = tiles;

@@ -2861,7 +2861,7 @@ def paged_attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     _check(code, "paged_attention_tree")
 
 
-TREE_SLICE = 4096      # keys up to which the call above needs no workspace (2 SLICE tiles in csrc/attention_tree_tcgen05.cu)
+TREE_SLICE = 6144      # keys up to which the call above needs no workspace (2 SLICE tiles in csrc/attention_tree_tcgen05.cu)
 
 
 def attention_tree_error(reset: bool = True) -> int:

@@ -54,14 +54,17 @@ def tree_attention(q, k, v, table, q_start, context, positions, seen, scale, spa
             s = torch.where(mask, s, torch.full_like(s, float("-inf")))
             p = torch.where(mask, torch.exp(s - torch.where(some, s.max(1).values, 0.0)[:, None]), torch.zeros_like(s))
             p = p / torch.where(some, p.sum(1), 1.0)[:, None]
-            clean = torch.where(mask.any(0)[:, None], vv[:, g], torch.zeros_like(vv[:, g]))
-            parts = torch.where(mask[:, :, None], p[:, :, None] * clean[None], torch.zeros((), dtype=torch.float64))
-            o[rows, h] = parts.sum(1)
+            # (what a row does not see is left out, whatever stands there)
+            finite = torch.where(torch.isfinite(vv[:, g]), vv[:, g], 0.0)
+            mean, spread = p @ finite, p @ finite.abs()
+            for x in torch.nonzero(~torch.isfinite(vv[:, g]).all(1)).flatten().tolist():
+                mean[mask[:, x]] += torch.where(torch.isfinite(vv[x, g]), 0.0, vv[x, g])
+            o[rows, h] = mean
             size = (q[rows, h].abs() @ kk[:, g].abs().t() * abs(scale)).nan_to_num(0.0, 0.0, 0.0)
             delta = ((d + 2) * size + s.abs().nan_to_num(0.0, 0.0, 0.0) + 4).masked_fill(~mask, 0).max(1).values * 2.0 ** -24
-            off[rows, h] = (2 * delta + 2 * len(place) * 2.0 ** -24)[:, None] * parts.abs().sum(1)
+            off[rows, h] = (2 * delta + 2 * len(place) * 2.0 ** -24)[:, None] * spread
             if rounded:
-                off[rows, h] += 2.0 ** -8 * parts.abs().sum(1)
+                off[rows, h] += 2.0 ** -8 * spread
     return o, off
 
 

@@ -106,19 +106,19 @@ def test_tree_attention(case, span):
     check(c, attend(c, span), span)
 
 
-@pytest.mark.parametrize("d,heads,kv,most,span", [(128, 16, 8, 9, None), (64, 16, 8, 20, None), (128, 8, 8, 40, 4200), (128, 16, 8, 70, None),
+@pytest.mark.parametrize("d,heads,kv,most,span", [(128, 16, 8, 9, None), (64, 16, 8, 20, None), (128, 8, 8, 40, 6200), (128, 16, 8, 70, None),
                                                   (64, 32, 8, 64, None), (128, 32, 8, 100, None)])
 def test_tree_attention_requests_of_very_different_length(d, heads, kv, most, span):
     """More CTAs than run at once: the long requests' keys go in slices that are joined by a kernel of their own."""
     rng = random.Random(most)
-    contexts = [0, 2300, 5, 4500, 130, 64, 7, 2000, 33, 1]
+    contexts = [0, 3300, 5, 6500, 130, 64, 7, 2000, 33, 1]
     trees = [rng.randrange(1, most + 1) for _ in contexts]
     trees[3], trees[4], trees[5] = most, 0, 1
     c = drafted(21, contexts, trees, heads, kv, d, 16, BF, spare=2)
     assert c["longest"] > kernels.TREE_SLICE and 2 * len(contexts) * kv > 148
     out = attend(c, span)
     check(c, out, span)
-    c["v"][c["table"][3, 4500 // 16], :, 4500 % 16] = float("nan")      # the first drafted token of the longest one
+    c["v"][c["table"][3, 6500 // 16], :, 6500 % 16] = float("nan")      # the first drafted token of the longest one
     got = attend(c, span).float().view(out.shape[0], heads, d)
     start = int(c["q_start"][3])
     hit = torch.zeros(out.shape[0], dtype=torch.bool, device=DEV)
