@@ -21,7 +21,7 @@ constexpr int KEYS = 32, WARPS = 4;
 __host__ __device__ __forceinline__ int padded(int dim) { return (dim + 3) / 4 * 4; }
 template <typename T> __host__ __device__ __forceinline__ int row_bytes(int dim) { return (dim * (int)sizeof(T) + 15) / 16 * 16 + 16; }
 template <typename T> __host__ __device__ __forceinline__ size_t rows_smem(int dim, int rows) {
-    return sizeof(float) * (size_t)(rows * padded(dim) + 2 * rows) + 2 * (size_t)KEYS * row_bytes<T>(dim);
+    return sizeof(float) * (size_t)(rows * padded(dim) + 2 * rows + KEYS * rows) + 2 * (size_t)KEYS * row_bytes<T>(dim);
 }
 
 __device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     const int d = A.dim, dp = padded(d), rb = row_bytes<T>(d);
     float* sq = reinterpret_cast<float*>(raw);    // [ROWS][dp], later the part's sums
     float* sml = sq + ROWS * dp;                  // [2][ROWS]
-    unsigned char* tile = reinterpret_cast<unsigned char*>(sml + 2 * ROWS);       // [keys, values][KEYS][rb]
+    float* sp = sml + 2 * ROWS;                   // [WARPS][KEYS][MINE]: the softmax's numbers
+    unsigned char* tile = reinterpret_cast<unsigned char*>(sp + KEYS * ROWS);     // [keys, values][KEYS][rb]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int b = blockIdx.x;
     const int part = b % parts;
@@ -161,12 +162,21 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
             for (int i = 0; i < PER; ++i) acc[r][i] *= c;
             m[r] = to;
         }
+        float* mine = sp + warp * KEYS * MINE;    // (one look gives a key's numbers of all the warp's rows)
+#pragma unroll
+        for (int r = 0; r < MINE; ++r) mine[lane * MINE + r] = p[r];
+        __syncwarp();
 #pragma unroll 4
         for (int key = 0; key < KEYS; ++key) {
             const T* sv = reinterpret_cast<const T*>(tile + (KEYS + key) * rb);
             float pk[MINE];
-#pragma unroll
-            for (int r = 0; r < MINE; ++r) pk[r] = __shfl_sync(0xffffffffu, p[r], key);
+            if constexpr (MINE == 4) {
+                const float4 v = four(mine + key * 4);
+                pk[0] = v.x; pk[1] = v.y; pk[2] = v.z; pk[3] = v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(mine + key * 2);
+                pk[0] = v.x; pk[1] = v.y;
+            }
             float x[PER];
             if constexpr (PER % 4 == 0) {
 #pragma unroll
