@@ -47,11 +47,12 @@ template <int D, int NQ> struct Shape {
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
     static constexpr int SLICE_SUMS = 2 * ROWS * (D + 2) + 4;      // floats of a slice's sums in the scratch: o [D / 4][line][4], m and l [line][2], whether it met bad values
-    static constexpr int SMEM = 1024 + TILES + 256;
+    static constexpr int SMEM = 232448;                            // all that a CTA may have
+    static_assert(1024 + TILES + 256 <= SMEM, "");
     static_assert((NQ == 1 ? SUMS + 4 * ROWS * 4 : 0) + (NQ * ROWS + 8) * (OLD + 4) * 4 <= TILES, "the sums take the place of the tiles");
     static_assert(SUMS + 4 * ROWS * 4 <= TILES, "the CTA's own sums too");
-    // one CTA an SM: a second one would wait for the first one's tensor memory while others of its cluster wait for it
-    static_assert(SMEM > 116 * 1024 && SMEM <= 232448, "one CTA an SM");
+    // One CTA an SM, and no other kernel's that holds tensor memory beside it: a CTA that waits for tensor memory holds up its cluster, which may
+    // hold the tensor memory that the other one's cluster waits for.
 };
 
 struct Small {                 // what stands behind the tiles
