@@ -30,7 +30,7 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
     return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-// What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles, four fifths of them waits), so what counts is
+// What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles for some 2,000 instructions), so what counts is
 // how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows: 355 us, with two 443),
 // and eight rows a CTA where there are no more or few CTAs (the same: 264 us; 2 trees of 13 over up to 777: 31.5 and 35.6).  PER numbers of a
 // head per lane, four neighbours where that is a multiple of four.
@@ -278,7 +278,9 @@ static int tree_args(const IbTreeAttention& c, tree::Args& A, int& max_tree, int
     if (c.dim > 512 || c.n_rows * c.n_heads > 0x7fffffffL || c.n_requests > 0x7fffffffL || c.max_pages * c.page_size > 0x7fffffffL
         || c.n_pages * c.n_kv * c.page_size > 0x7fffffffL)
         return IB_ERR_UNSUPPORTED;
-    A.q = c.q; A.k = c.k; A.v = c.v;
+    A.q = c.q;
+    A.k = c.n_pages ? c.k : c.q;      // (a cache without pages: nothing is read, but copies of no bytes want an address)
+    A.v = c.n_pages ? c.v : c.q;
     A.table = c.table; A.q_start = c.q_start; A.context = c.context; A.positions = c.positions; A.seen = c.seen;
     A.out = c.out;
     A.out_ld = c.out_ld;

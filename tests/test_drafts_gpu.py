@@ -19,6 +19,12 @@ def ints(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    assert kernels.attention_tree_error() == 0 and kernels.log_probs_error() == 0
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 def drafted(seed, contexts, trees, heads, kv, d, page, dtype, chain=False, spare=0, words=None):
     """Everything that a call takes, with pages in no order, leftovers in the places that hold no key, and rows behind the last."""
@@ -89,6 +95,9 @@ SHAPES = [
     ([50], [9], 4, 2, 33, 7, BF),
     ([140], [11], 4, 2, 256, 16, BF),
     ([130, 64], [11, 5], 8, 2, 128, 48, BF),
+    ([130, 300], [11, 5], 8, 2, 128, 4, BF),
+    ([500, 300, 7], [11, 80, 3], 8, 2, 128, 256, BF),
+    ([500, 129], [11, 70], 8, 2, 64, 128, BF),
     ([300, 77], [13, 8], 16, 8, 128, 16, F32),
     ([0, 31, 32, 33], [1, 2, 3, 64], 4, 2, 64, 16, F32),
     ([45], [20], 6, 2, 36, 5, F32),
@@ -218,6 +227,65 @@ def test_tree_attention_rows_that_lie_apart_and_other_scales(dtype, d):
     for scale in (0.5, -0.1, 1e-6):
         check(c, attend(c, scale=scale), scale=scale)
     assert (attend(c, positions=False) == attend(c)).all()
+
+
+def moved(t, by):
+    """The same numbers in memory that starts ``by`` of them off a boundary."""
+    flat = torch.empty((t.numel() + by,), dtype=t.dtype, device=DEV)
+    flat[by:].copy_(t.flatten())
+    return flat[by:].view(t.shape)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (BF, 64), (BF, 80), (F32, 128), (F32, 20)])
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_tree_attention_tensors_that_start_anywhere(dtype, d, which):
+    c = drafted(15, [150, 7], [9, 12], 4, 2, d, 16, dtype)
+    for by in (1, 4):
+        c[which] = moved(c[which], by)
+        check(c, attend(c))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (BF, 96), (F32, 64)])
+def test_tree_attention_a_cache_without_pages_and_calls_without_rows(dtype, d):
+    c = drafted(16, [50, 7], [3, 4], 4, 2, d, 16, dtype)
+    empty = dict(c, k=c["k"][:0], v=c["v"][:0])
+    assert (attend(empty) == 0).all()
+    none = dict(c, q=c["q"][:0].contiguous(), q_start=ints([0, 0, 0]), positions=c["positions"][:0], seen=c["seen"][:0])
+    assert attend(none).shape[0] == 0
+    lying = dict(c, q_start=ints([-5, 3, 2 ** 31 - 1]), context=ints([-3, 2 ** 31 - 1]))     # read as far as there is anything
+    attend(lying)
+
+
+def test_what_the_calls_refuse():
+    c = drafted(17, [50, 7], [3, 4], 4, 2, 64, 16, BF)
+    for name, bad in (("q", c["q"].float()), ("q", c["q"].transpose(0, 1)), ("k", c["k"][..., :32]), ("v", c["v"][:3]), ("table", c["table"].long()),
+                      ("table", c["table"][:1]), ("q_start", c["q_start"][:2]), ("context", c["context"].float()), ("seen", c["seen"][:2]),
+                      ("seen", c["seen"].cpu()), ("context", c["context"].cpu()), ("positions", c["positions"][:1])):
+        with pytest.raises(kernels.KernelError):
+            attend(dict(c, **{name: bad}), out=torch.zeros((7, 256), dtype=BF, device=DEV))
+    with pytest.raises(kernels.KernelError):
+        attend(c, span=9, positions=False)
+    with pytest.raises(kernels.KernelError):
+        attend(c, out=torch.zeros((7, 128), dtype=BF, device=DEV))
+    wide = drafted(18, [5], [3], 2, 1, 520, 16, F32)
+    with pytest.raises(kernels.KernelError):
+        attend(wide)
+    pages = torch.zeros((2, 5, 2, 16, 8), device=DEV)
+    for args in ((pages, 5, ints([0]), ints([1])), (pages, 1, ints([0]), ints([1, 2])), (pages, 1, ints([0]).long(), ints([1])),
+                 (pages[:, ::2], 1, ints([0]), ints([1])), (pages, 1, ints([0]).cpu(), ints([1]))):
+        with pytest.raises(kernels.KernelError):
+            kernels.copy_pages(*args)
+    t, n = ints([[0, 1]]), ints([1])
+    for args in ((pages, 3, t, n, t, n), (pages, 1, t, n, ints([[0], [1]]), n), (pages, 1, t, ints([1, 2]), t, n), (pages, 1, t.long(), n, t, n)):
+        with pytest.raises(kernels.KernelError):
+            kernels.keep_tokens(*args)
+    x, one = torch.zeros((3, 50), device=DEV), torch.zeros((3, 1), device=DEV)
+    k33 = (ints([[0] * 33] * 3), torch.zeros((3, 33), device=DEV))
+    for args in ((x.half(), ints([[1]] * 3), one), (x, ints([[1]] * 2), one), (x, ints([[1, 2]] * 3), one), (x.t(), ints([[1]] * 50), one),
+                 (x, ints([[1]] * 3), one, torch.zeros(2, device=DEV)), (x, ints([[1]] * 3), one, None, *k33),
+                 (x, ints([[1]] * 3), one, None, k33[0][:, :4].contiguous()), (x[:, :0], ints([[1]] * 3), one)):
+        with pytest.raises(kernels.KernelError):
+            kernels.token_log_probs(*args)
 
 
 @pytest.mark.parametrize("dtype,d", [(BF, 128), (BF, 128), (F32, 64)])
