@@ -31,8 +31,9 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
 }
 
 // What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles for some 2,000 instructions), so what counts is
-// how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows: 355 us, with two 443),
-// and eight rows a CTA where there are no more or few CTAs (the same: 264 us; 2 trees of 13 over up to 777: 31.5 and 35.6).  PER numbers of a
+// how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows, when that was changed: 355 us, with two 443),
+// and eight rows a CTA where there are no more or few CTAs (with eight and with sixteen: 41 requests of 2,000 keys 245 and 386 us; 2 trees of 13
+// over up to 777 29.0 and 31.8; 2 trees of 64 over up to 1,000 with 64 heads 262 and 200).  PER numbers of a
 // head per lane, four neighbours where that is a multiple of four.
 template <typename T, int PER, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts, bool wide) {

@@ -10,10 +10,17 @@
 //   O += P V    in tensor memory, P from there, V as it lies in its page.
 // While one stream's threads compute their P the other's products run.
 //
-// What bounds it is what comes from memory: a tile of 128 keys and values of 128 numbers is 64 KB, 2,900 cycles of an SM's share of the
-// copy bandwidth, and needs 1,100 cycles of products and as many of exponentials for every 128 rows.  Keys and values come through
-// a ring of tiles that two warps fill, in the order in which the products take them: by TMA, a box for every page, and where pages
-// have an odd size with cp.async, 16 bytes a lane.  Where there is no key zeros are written.
+// A tile of 128 keys and values of 128 numbers is 64 KB, 2,900 cycles of an SM's share of the copy bandwidth, and needs 1,100 cycles of
+// products and as many of exponentials for every 128 rows.  Keys and values come through a ring of tiles that two warps fill, in the
+// order in which the products take them: by TMA, a box for every page, and where pages have an odd size with cp.async, 16 bytes a
+// lane.  Where there is no key zeros are written.
+//
+// What bounds it.  16 trees of 64 over up to 16,384 keys, 32 heads on 8 of 128 (171 us; the bytes alone 90): with 256 rows the tensor cores, whose
+// products of 128 x 128 x 16 take 85 to 100 cycles where 64 would do, 3,300 a tile, and 16 us of the join.  8 trees of 16 over 2,048 keys (21.3 us;
+// 10.6): memory while the ring runs, on 128 of 148 SMs, and about 10,000 of 38,000 cycles before and behind it.  One tree of 8 over 300
+// keys (8.7 us): the chain start, one tile (6,000 cycles), join (5,000), much of it waiting for instructions that run once.  Up to 64 rows standing twice
+// among the 128, so that more threads shared the exponentials, gained nothing once a tile's halves were handed over one by one (21.8 us; 16
+// trees of 16 over 8,192 keys 135, as it is 123).
 //
 // What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So the values of tiles that
 // some row does not see in full come with cp.async, and the warps that fill the ring look at what they brought, put zeros in the place of those that are
@@ -349,8 +356,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (rows <= 0) return;            // (the whole cluster leaves)
     if (scratch != nullptr && part > 0 && (long)part * SLICE * KEYS >= S.keys) return;       // (there are no more slices than this)
-    // up to 64 rows stand twice among the 128: the second ones' threads take the second half of a tile's keys, and are joined like a part
-    const int copies = NQ == 1 && rows <= ROWS / 2 ? 2 : 1, block = ROWS / copies;
 
     if (tid == 0) {
         sm.lo_min = 0x7fffffff;
@@ -367,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         for (int g = 0; g < 2; ++g) {
             const int used = NQ == 2 ? rows - g * ROWS : rows;
             mbar_init(smem_u32(&sm.s_full[g]), 1);
-            for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&sm.p_full[g][h]), used <= 0 ? 1 : used >= ROWS ? 4 : copies * ((used + 31) / 32));
+            for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&sm.p_full[g][h]), used <= 0 ? 1 : used >= ROWS ? 4 : (used + 31) / 32);
         }
         mbar_init(smem_u32(&sm.o_full), 1);
         mbar_init(smem_u32(&sm.q_full), 256);
@@ -549,15 +554,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         // the queries: 16 rows a warp and set
 #pragma unroll
         for (int s = 0; s < NQ; ++s) {
-            const int r = s * ROWS + ((warp * 16 + (lane & 15)) & (block - 1)), at = first_row + r, token = at / group;
+            const int r = s * ROWS + warp * 16 + (lane & 15), at = first_row + r, token = at / group;
             const int index = r < rows ? (S.row0 + token) * A.n_heads + head * group + at - token * group : -1;
             load_rows<D>(sq + s * Sh::TILE, static_cast<const bf16*>(A.q), index, 0, warp, lane);
         }
         cp_arrive(smem_u32(&sm.q_full));
-        const int g = warp >> 2, line = (warp & 3) * 32 + lane, r = line & (block - 1);
-        const int copy = (warp & 3) * 32 / block;
+        const int g = warp >> 2, r = (warp & 3) * 32 + lane;
         const int used = NQ == 2 ? min(rows - g * ROWS, ROWS) : rows, count = g ? count1 : count0;
-        if (((warp & 3) * 32 & (block - 1)) < used) {
+        if ((warp & 3) * 32 < used) {
             const bool mine = r < used;
             const int at = first_row + (NQ == 2 ? g * ROWS : 0) + (mine ? r : 0), token = at / group;
             const int lo = first_key(A, S, token);
@@ -603,20 +607,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                             top4[c] = max3(top4[c], __uint_as_float(x[at + k + 2 * c]), __uint_as_float(x[at + k + 2 * c + 1]));
                 };
                 unsigned x[64];
-                tmem_ld64(s_at + 64 * copy, x);
-                hide(x, 0, 2 * copy);
-                hide(x, 32, 2 * copy + 1);
+                tmem_ld64(s_at, x);
+                hide(x, 0, 0);
+                hide(x, 32, 1);
                 look(x, 0);
                 look(x, 32);
-                if (copies == 1) {
-                    unsigned y[32];
-                    tmem_ld32(s_at + 64, y);
-                    hide(y, 0, 2);
-                    look(y, 0);
-                    tmem_ld32(s_at + 96, y);
-                    hide(y, 0, 3);
-                    look(y, 0);
-                }
+                unsigned y[32];
+                tmem_ld32(s_at + 64, y);
+                hide(y, 0, 2);
+                look(y, 0);
+                tmem_ld32(s_at + 96, y);
+                hide(y, 0, 3);
+                look(y, 0);
                 const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * A.scale_log2;     // (the scale is positive)
                 const bool move = top > m + STEP || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
@@ -651,29 +653,20 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     }
                     tmem_st16(s_at + 16 * c, p);
                 };
-                weigh(x, 2 * copy);
-                weigh(x + 32, 2 * copy + 1);
+                weigh(x, 0);
+                weigh(x + 32, 1);
                 auto hand_over = [&](int h) {
                     tmem_st_wait();
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[g][h]));
                 };
-                if (copies == 1) {
-                    hand_over(0);
-                    tmem_ld64(s_at + 64, x);
-                    hide(x, 0, 2);
-                    hide(x, 32, 3);
-                    weigh(x, 2);
-                    weigh(x + 32, 3);
-                } else {              // the other copy's keys
-                    unsigned zeros[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) zeros[k] = 0;
-                    tmem_st16(s_at + 32 * (copy ^ 1), zeros);
-                    tmem_st16(s_at + 32 * (copy ^ 1) + 16, zeros);
-                    hand_over(0);
-                }
+                hand_over(0);
+                tmem_ld64(s_at + 64, x);
+                hide(x, 0, 2);
+                hide(x, 32, 3);
+                weigh(x, 2);
+                weigh(x + 32, 3);
                 float a, b;
                 apart(add2(add[0], add[1]), a, b);
                 l += a + b;
@@ -714,7 +707,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             } else if (scratch != nullptr && parts > 1) {
                 // the sums of a slice, numbers four by four, so that a warp's stores lie side by side
                 float* to = scratch + (((long)(req * A.tiles_of_rows + row_tile) * A.n_kv + head) * slices + part) * Sh::SLICE_SUMS;
-                const int all = g * ROWS + line;
+                const int all = g * ROWS + r;
 #pragma unroll 1
                 for (int e = 0; e < D && count > 0; e += 32) {
                     unsigned x[32];
@@ -741,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 if (mine) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(m, ok ? l : NAN, sm.bad_values ? 1.0f : 0.0f, 0.0f));
             } else {
                 if (count > 0 && ok) {
-                    float* row = sums + (g * ROWS + line) * Sh::OLD;
+                    float* row = sums + (g * ROWS + r) * Sh::OLD;
 #pragma unroll
                     for (int e = 0; e < D; e += 32) {
                         unsigned x[32];
@@ -751,8 +744,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                             *reinterpret_cast<uint4*>(row + e + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
                     }
                 }
-                part_m[g * ROWS + line] = m;
-                part_l[g * ROWS + line] = ok ? l : NAN;
+                part_m[g * ROWS + r] = m;
+                part_l[g * ROWS + r] = ok ? l : NAN;
             }
         } else if (scratch == nullptr && parts > 1) {
             cluster_sync();
@@ -766,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
     if (none || (scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
-    // Join: first the sums that this CTA has of a row (of two streams, of two copies), which go to the CTA that writes the row (every parts-th),
+    // Join: first the sums that this CTA has of a row (of two streams), which go to the CTA that writes the row (every parts-th),
     // and there those of the cluster's CTAs.  What goes out is not waited for; a look into another CTA's memory takes 700 cycles.  Eight lanes
     // a row, and loops as they stand: this code runs once, and unrolled ones wait for their instructions (ten cycles each) longer than they
     // save.  Every sum comes in the same order whatever the grid.
@@ -778,7 +771,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             float4 o[QUADS] = {};
             float top = -INFINITY, total = 0.0f;
 #pragma unroll 1
-            for (int line = row; line < 2 * ROWS; line += block)          // (a stream's copies lie one behind the other)
+            for (int line = row; line < 2 * ROWS; line += ROWS)
                 join<QUADS>(top, total, o, part_m[line], part_l[line], sums + line * Sh::OLD + e);
             const int i = share_of(row), owner = row - i * parts;
             const unsigned to = remote(inbox + (part * most + i) * Sh::OLD + e, owner);
@@ -808,7 +801,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 // takes 16 numbers of a row, a warp 32 rows.
 template <int D, int NQ>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args A, int slices, const float* __restrict__ scratch) {
-    constexpr int CHUNKS = NQ * ROWS * (D / 16) / 256, SUMS = Shape<D, NQ>::SLICE_SUMS;
+    constexpr int CHUNKS = NQ * ROWS * (D / 16) / 256, SUMS = Shape<D, NQ>::SLICE_SUMS, STREAMS = NQ == 1 ? 2 : 1;      // that have a row's sums
     const int unit = blockIdx.x / CHUNKS, at = blockIdx.x % CHUNKS * 256 + threadIdx.x, row = at % (NQ * ROWS), e = at / (NQ * ROWS) * 16;
     const int head = unit % A.n_kv, row_tile = unit / A.n_kv % A.tiles_of_rows, req = unit / A.n_kv / A.tiles_of_rows;
     const Span S = span_of(A, req);
@@ -828,15 +821,14 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     }
     const int t_first = lo_min / KEYS, all_tiles = (S.keys + KEYS - 1) / KEYS - t_first, parts = slices_of(all_tiles, slices);
     if (parts == 1) return;           // (its rows are written)
-    const int copies = NQ == 1 && rows <= ROWS / 2 ? 2 : 1, here = (NQ == 1 ? 2 : 1) * copies;
     float4 o[4] = {};
     float top = -INFINITY, total = 0.0f;
     bool bad_values = false;
     const float* from = scratch + (long)unit * slices * SUMS;
 #pragma unroll 2
-    for (int p = 0; p < parts * here; ++p) {
-        const float* slice = from + (long)(p / here) * SUMS;
-        const int line = row + p % here * (ROWS / copies);
+    for (int p = 0; p < parts * STREAMS; ++p) {
+        const float* slice = from + (long)(p / STREAMS) * SUMS;
+        const int line = row + p % STREAMS * ROWS;
         const float2 ml = *reinterpret_cast<const float2*>(slice + 2 * ROWS * D + 2 * line);
         bad_values |= slice[2 * ROWS * (D + 2)] != 0.0f;
         join<4>(top, total, o, ml.x, ml.y, slice + (e / 4 * (2 * ROWS) + line) * 4, 2 * ROWS * 4);
