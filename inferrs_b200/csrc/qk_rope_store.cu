@@ -469,8 +469,9 @@ __global__ void qk_rope_store_shared_kernel(
     }
 }
 
-// places: where in its request a row's key and value go (null: at its position).  bias: float over the columns of qkv (or null).  value_is_key: qkv holds queries and keys; a value is its key before the
-// norm and the rotation (v_dim is then head_dim).
+// places: where in its request a row's key and value go (null: at its position); they ascend within a request, whose last row has the values
+// behind its place in its page cleared.  bias: float over the columns of qkv (or null).  value_is_key: qkv holds queries and keys; a value is
+// its key before the norm and the rotation (v_dim is then head_dim).
 IB_EXPORT int ib_qk_norm_rope_store(const void* qkv, int row_stride, int n_rows, int n_heads, int n_kv_heads,
                                     int head_dim, int v_dim, int store_kv, const void* q_weight, const void* k_weight,
                                     int weight_is_f32, int norm_flags, float eps, const float* cos_table, const float* sin_table,

@@ -48,7 +48,7 @@ class ModelRunner:
         self.manager = CacheManager(self.storage.layouts, page_size, self.storage.n_pages, max_requests)
         self.page_size = page_size
         self.steps_run = 0
-        self._drafted: Dict[Hashable, int] = {}      # drafted tokens of the requests' last step of drafts, until some are kept
+        self._drafted: Dict[Hashable, List[int]] = {}      # the parents of the requests' drafted tokens, until some are kept
         # decode steps are replayed as CUDA graphs when every part says its launches do not depend on
         # host-side values of the step (``graph_safe``)
         parts = [p for b in self.model.blocks for p in b.parts()] + [self.model.final_norm]
@@ -212,7 +212,7 @@ class ModelRunner:
         self.manager.reserve(wants)
         ctx = build_drafts(entries, self.manager, self.storage, self.spec.vocab_size, self.spec.max_positions, self.rt.device)
         logits = self.model.forward(ctx)
-        self._drafted.update(wants)
+        self._drafted.update((e.rid, [int(p) for p in e.parents]) for e in entries)
         self.steps_run += 1
         return logits
 
@@ -222,8 +222,11 @@ class ModelRunner:
         for rid, places in kept.items():
             if rid not in self._drafted:
                 raise BatchError(f"request {rid!r} has no drafted tokens")
-            if any(not 0 <= p < self._drafted[rid] for p in places) or any(a >= b for a, b in zip(places, list(places)[1:])):
-                raise BatchError(f"request {rid!r}: the tokens that stay are ascending places among {self._drafted[rid]}, got {list(places)}")
+            parents, before = self._drafted[rid], -1
+            for p in places:
+                if not 0 <= p < len(parents) or parents[p] != before:
+                    raise BatchError(f"request {rid!r}: the tokens that stay are a path through its {len(parents)} drafted ones, got {list(places)}")
+                before = p
         moved = [rid for rid, places in kept.items() if list(places) != list(range(len(places)))]
         if moved:
             lists = [list(kept[rid]) for rid in moved]

@@ -710,7 +710,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_di
     after the rotation instead of before it.  Values may have another size than keys (the last size of ``v_pages``).
     ``bias`` (float32, one number per column of q, k and v) is added first.  ``value_is_key``: there are no value columns;
     a value is its key as it was projected (with its bias), before norm and rotation.  ``places`` (int32 [N]): a row's key and
-    value go to that place of its request instead of to its position (drafted tokens, several of which may share a position).
+    value go to that place of its request instead of to its position (drafted tokens, several of which may share a position);
+    a request's places ascend, because the values behind its last row's place are cleared to the end of that page.
 
     qkv [N, at least n_heads * d + n_kv_heads * (d + dv)] (queries only when ``store_kv`` is False; columns behind
     them, a gate's for instance, are not read);

@@ -7,7 +7,7 @@ import torch
 import plain_qwen3
 from helpers import CONFIG_A, CONFIG_B, CONFIG_C, CONFIG_D, PAGE_SIZE, random_tokens, rel_err
 from inferrs_b200 import Engine, SamplingParams, kernels
-from inferrs_b200.cache.manager import OutOfPages
+from inferrs_b200.cache.manager import CacheError, OutOfPages
 from inferrs_b200.engine.batch import BatchError, DraftEntry, StepEntry
 from inferrs_b200.engine.loading import load_model_dir
 from inferrs_b200.engine.runner import ModelRunner
@@ -180,3 +180,91 @@ def test_prompts_are_scored(model_dirs, dtype):
     assert engine.runner.manager.n_live == 0
     with pytest.raises(ValueError):
         engine.score(prompts, top=33)
+
+
+def test_what_stays_is_a_path(model_dirs):
+    runner = make_runner(model_dirs["A"], torch.float32, PAGE_SIZE["A"])
+    runner.admit(0)
+    runner.step([StepEntry(0, [1, 2, 3], [])])
+    runner.step_drafts([DraftEntry(0, [5, 6, 7, 8], [-1, 0, 0, 1])])
+    for bad in ([1], [0, 3], [0, 1, 2], [0, 2, 3], [0, 1, 3, 3]):
+        with pytest.raises(BatchError):
+            runner.keep_drafts({0: bad})
+    runner.keep_drafts({0: [0, 1, 3]})
+    assert runner.n_tokens(0) == 6
+    with pytest.raises(BatchError):
+        runner.step_drafts([])
+    with pytest.raises(CacheError):
+        runner.step_drafts([DraftEntry(0, [], [])])
+    with pytest.raises(ValueError):
+        runner.step_drafts([DraftEntry(0, [1], [-1]), DraftEntry(0, [2], [-1])])
+    assert runner.n_tokens(0) == 6
+    runner.manager.check_invariants()
+
+
+@pytest.mark.parametrize("name", ["A", "D"])
+def test_drafting_choosing_keeping_and_forking_give_the_greedy_tokens(model_dirs, name):
+    """Trees whose tokens are half right, the model's choice among them, the path that it chose, and a fork that goes on alike: the
+    tokens and log probabilities are those of one token after another."""
+    vocab, n = CONFIGS[name]["vocab_size"], 14
+    runner = make_runner(model_dirs[name], torch.float32, PAGE_SIZE[name])
+    prompts = [random_tokens(11, vocab, seed=31), random_tokens(2 * PAGE_SIZE[name], vocab, seed=32)]
+    greedy, wanted = [], []
+    for prompt in prompts:
+        tokens, log_probs = list(prompt), []
+        for _ in range(n + 6):
+            row = torch.log_softmax(plain_logits(model_dirs[name], tokens, torch.float32)[-1].double(), -1)
+            tokens.append(int(row.argmax()))
+            log_probs.append(float(row.max()))
+        greedy.append(tokens[len(prompt):])
+        wanted.append(log_probs)
+
+    def choose(logits):
+        rows = logits.shape[0]
+        ids = torch.empty((rows, 1), dtype=torch.int32, device=logits.device)
+        best = torch.empty((rows, 1), dtype=torch.float32, device=logits.device)
+        given = torch.empty((rows, 1), dtype=torch.float32, device=logits.device)
+        kernels.token_log_probs(logits, torch.zeros_like(ids), given, None, ids, best)
+        return ids[:, 0].tolist(), best[:, 0].tolist()
+
+    rids, out, scores = [0, 1], [[], []], [[], []]
+    for r in rids:
+        runner.admit(r)
+    ids, best = choose(runner.step([StepEntry(r, prompts[r], [len(prompts[r]) - 1]) for r in rids]))
+    for r in rids:
+        out[r].append(ids[r])
+        scores[r].append(best[r])
+    turn = 0
+    while min(map(len, out)) < n:
+        if turn == 2:                  # a third request goes on from the second one, and the second one ends
+            runner.fork(1, 2)
+            runner.release(1)
+            rids = [0, 2]
+        entries = []
+        for i, r in enumerate(rids):
+            right = greedy[i][len(out[i]):] + [0] * 4
+            wrong = (right[0] + 1) % vocab
+            # the last token, a wrong one and the right one behind it, then two more right ones or (in turn) a wrong one
+            entries.append(DraftEntry(r, [out[i][-1], wrong, right[0], wrong, right[1], right[2] if turn % 2 else wrong], [-1, 0, 0, 1, 2, 4]))
+        ids, best = choose(runner.step_drafts(entries))
+        kept = {}
+        for i, r in enumerate(rids):
+            e, at, path = entries[i], 6 * i, [0]
+            while True:
+                out[i].append(ids[at + path[-1]])
+                scores[i].append(best[at + path[-1]])
+                following = [k for k in range(6) if e.parents[k] == path[-1] and e.tokens[k] == out[i][-1]]
+                if not following:
+                    break
+                path.append(following[0])
+            kept[r] = path
+            assert path[:3] == [0, 2, 4]
+        runner.keep_drafts(kept)
+        turn += 1
+    assert turn >= 3
+    for i in range(2):
+        assert out[i][:n] == greedy[i][:n]
+        # logits off by the engine's bound, relative to the largest one, move a log probability by twice that at most
+        off = 2 * TOL[torch.float32] * float(plain_logits(model_dirs[name], prompts[i] + greedy[i], torch.float32).abs().max())
+        assert all(abs(a - b) <= off for a, b in zip(scores[i][:n], wanted[i]))
+    runner.manager.check_invariants()

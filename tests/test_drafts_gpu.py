@@ -320,6 +320,33 @@ def test_tree_attention_replayed_and_on_another_stream(dtype, d):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("name", ["clusters", "slices", "rows"])
+def test_calls_on_two_streams_at_once(name):
+    """Two kinds of work side by side give what each gives alone."""
+    sizes = {"clusters": ([900, 300], [40, 9], 8, 2, 128, 16, BF), "slices": ([7000] * 12, [16] * 12, 32, 8, 64, 16, BF),
+             "rows": ([500, 20], [7, 30], 8, 2, 64, 16, F32)}
+    cases = [drafted(21, *sizes[name]), drafted(22, [1500, 7], [30, 60], 16, 2, 128, 16, BF)]
+    alone = [attend(c) for c in cases]
+    logits = torch.randn((40, 60000), device=DEV, generator=torch.Generator(DEV).manual_seed(3))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got, given = [[], []], []
+    for _ in range(12):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(attend(cases[i]))
+        with torch.cuda.stream(streams[2]):
+            lp, ids, best = torch.empty((40, 1), device=DEV), torch.empty((40, 4), dtype=torch.int32, device=DEV), torch.empty((40, 4), device=DEV)
+            kernels.token_log_probs(logits, torch.zeros((40, 1), dtype=torch.int32, device=DEV), lp, None, ids, best)
+            given.append((lp, ids, best))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in got[i])
+    values, order = logits.sort(dim=1, descending=True, stable=True)
+    for lp, ids, best in given:
+        assert torch.equal(ids.long(), order[:, :4]) and all(torch.equal(a, b) for a, b in zip((lp, ids, best), given[0]))
+
+
 def test_tree_attention_a_chain_is_a_prompts_portion():
     """Drafted tokens without branches see what a portion of a prompt sees: the framework's own attention gives the same."""
     contexts, n = [211, 64, 5], 6
@@ -501,3 +528,50 @@ def test_log_probs_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+# ---- where keys and values go ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("dtype,d,value_is_key,norm", [(BF, 128, False, True), (BF, 128, True, True), (BF, 64, False, False), (BF, 80, True, False),
+                                                       (F32, 128, False, True), (F32, 64, True, True)])
+def test_keys_and_values_go_to_their_places(rows, dtype, d, value_is_key, norm):
+    """With places a row's query, key and value are what they are without, and the key and value lie at the place."""
+    g = torch.Generator().manual_seed(rows + d)
+    nh, nkv, page = 4, 2, 16
+    starts = [0, rows // 2, rows]
+    request = [0] * (rows // 2) + [1] * (rows - rows // 2)
+    positions = [i - starts[r] + 3 for i, r in enumerate(request)]
+    places = []
+    for r in range(2):                    # ascending, with gaps
+        count = starts[r + 1] - starts[r]
+        places += sorted(int(x) + 1 for x in torch.randperm(2 * count, generator=g)[:count])
+    places[1] = -1                        # nowhere
+    per = -(-(rows + 3) // page)
+    table = torch.randperm(2 * per, generator=g).view(2, per).int().to(DEV)
+    qkv = torch.randn((rows, (nh + nkv * (1 if value_is_key else 2)) * d), generator=g).to(dtype).to(DEV)
+    weight = (1 + 0.1 * torch.randn((d,), generator=g)).to(dtype).to(DEV) if norm else None
+    angle = torch.rand((rows + 3, d // 2), generator=g)
+    cos, sin = angle.cos().to(DEV), angle.sin().to(DEV)
+
+    def run(at):
+        k, v = torch.full((2 * per, nkv, page, d), 9.0, dtype=dtype, device=DEV), torch.full((2 * per, nkv, page, d), 9.0, dtype=dtype, device=DEV)
+        q = torch.empty((rows, nh, d), dtype=dtype, device=DEV)
+        kernels.qk_norm_rope_store(qkv, nh, nkv, d, True, weight, weight, 1e-6, cos, sin, d, ints(positions), ints(request), table, k, v, q,
+                                   value_is_key=value_is_key, places=None if at is None else ints(at))
+        return q, k, v
+
+    q0, k0, v0 = run(None)
+    assert all(torch.equal(a, b) for a, b in zip(run(positions), (q0, k0, v0)))
+    q, k, v = run(places)
+    assert torch.equal(q, q0)
+    pages = table.cpu()
+    written = torch.zeros((2 * per, page), dtype=torch.bool)
+    for i, (r, p, a) in enumerate(zip(request, positions, places)):
+        if a < 0:
+            continue
+        page0, page1 = int(pages[r, p // page]), int(pages[r, a // page])
+        written[page1, a % page] = True
+        assert torch.equal(k[page1, :, a % page], k0[page0, :, p % page]) and torch.equal(v[page1, :, a % page], v0[page0, :, p % page])
+    # what lies behind a row's place in its page may be cleared; all else is as it was
+    left = ~written.to(DEV)[:, None, :, None].expand_as(k)
+    assert ((k == 9) | (k == 0))[left].all() and ((v == 9) | (v == 0))[left].all()
