@@ -136,6 +136,33 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
     return d;
 }
 
+// the logits e, the largest of which is `top`, to a thread's m, S and W
+template <int EACH>
+__device__ __forceinline__ void add_block(const float* e, float top, float& m, float& s, float& w) {
+    if (top > m) {
+        move_reference(m, top, s, w);
+        m = top;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const u64 less = pair(-ref, -ref), factor = pair(LOG2E, LOG2E);
+    u64 s2 = 0, w2 = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i += 2) {
+        float a, b;
+        apart(mul2(add2(pair(e[i], e[i + 1]), less), factor), a, b);       // (log2(e) z; the difference is taken first: large logits lose nothing)
+        a = fmaxf(a, LOWEST);
+        b = fmaxf(b, LOWEST);
+        const u64 p = pair(sm100::ex2(a), sm100::ex2(b));
+        s2 = add2(s2, p);
+        w2 = fma2(p, pair(a, b), w2);
+    }
+    float a, b;
+    apart(s2, a, b);
+    s += a + b;
+    apart(w2, a, b);
+    w += a + b;
+}
+
 // The k best of the first n notes to best[0 .. min(k, n)) in descending order, by counting the keys ahead of each (keys differ:
 // they hold their places), four threads a key where there are few.  The threads that look at logits call it between two meetings.
 __device__ __noinline__ void rank_notes(const u64* notes, int n, int k, u64* best) {
@@ -283,28 +310,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
 #pragma unroll
             for (int i = 0; i < EACH; ++i) any |= e[i] == e[i];
         }
-        if (top > m) {
-            move_reference(m, top, s, w);
-            m = top;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const u64 less = pair(-ref, -ref), factor = pair(LOG2E, LOG2E);
-        u64 s2 = 0, w2 = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; i += 2) {
-            float a, b;
-            apart(mul2(add2(pair(e[i], e[i + 1]), less), factor), a, b);       // (log2(e) z; the difference is taken first: large logits lose nothing)
-            a = fmaxf(a, LOWEST);
-            b = fmaxf(b, LOWEST);
-            const u64 p = pair(sm100::ex2(a), sm100::ex2(b));
-            s2 = add2(s2, p);
-            w2 = fma2(p, pair(a, b), w2);
-        }
-        float a, b;
-        apart(s2, a, b);
-        s += a + b;
-        apart(w2, a, b);
-        w += a + b;
+        add_block<EACH>(e, top, m, s, w);
         if constexpr (TOP) {
             const u64 key = top > -INFINITY || any ? key_of(top, v0 + tid * VECTORS) : 0;
             if (round == 0) {      // the first bound
@@ -468,8 +474,108 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
     if (cluster > 1) cluster_sync();        // nobody leaves while rank 0 reads
 }
 
+// The same with a warp a row, for many rows of few logits: a lane takes every 32nd block of 16, all of whose keys stay in its registers.  The likeliest
+// tokens come one by one: the block with the best key is looked at by 16 lanes, and its next logit's key takes that one's place.
+constexpr int LANE_BLOCKS = 16, SHORT = LANE_BLOCKS * 512;      // a lane's blocks at most; logits of a row, counted from the 16-byte boundary
+
+__device__ __forceinline__ u64 warp_best(u64 key) {
+    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32));
+    return (u64)high << 32 | __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
+}
+
+template <typename T, bool TOP, int BLOCKS>
+__global__ void __launch_bounds__(128) short_rows_kernel(const Args A) {
+    constexpr int N = Wide<T>::N, VECTORS = Wide<T>::VECTORS, EACH = N * VECTORS;
+    static_assert(EACH == 16, "");
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= A.rows) return;
+    const T* x = static_cast<const T*>(A.logits) + row * A.ld;
+    const int skew = (int)(((unsigned long long)x / sizeof(T)) % N), end = A.vocab + skew;      // places are counted from the boundary
+    const T* from = x - skew;
+    float m = -INFINITY, s = 0.0f, w = 0.0f;
+    u64 keys[BLOCKS];
+    uint4 next[VECTORS];
+    auto fetch = [&](int place) {
+        if (place >= skew && place + EACH <= end)
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) next[i] = *reinterpret_cast<const uint4*>(from + place + i * N);
+    };
+    fetch(lane * EACH);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        keys[b] = 0;
+        if (b * 32 * EACH >= end) continue;
+        const int place = (b * 32 + lane) * EACH;
+        float e[EACH];
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i) Wide<T>::unpack(next[i], e + i * N);
+        if (place < skew || place + EACH > end) {
+#pragma unroll
+            for (int c = 0; c < EACH; ++c) e[c] = place + c >= skew && place + c < end ? ib_to_float(from[place + c]) : NAN;
+        }
+        fetch(place + 32 * EACH);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) top = fmaxf(top, e[i]);
+        bool any = top > -INFINITY;        // (a logit of minus infinity is one, no number is none)
+        if (TOP && !any) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) any |= e[i] == e[i];
+        }
+        add_block<EACH>(e, top, m, s, w);
+        if (TOP && any) keys[b] = key_of(top, place);
+    }
+    const float all = ib_warp_max(m);
+    move_reference(m, all, s, w);
+    s = ib_warp_sum(s);
+    w = ib_warp_sum(w);
+    const bool none = !(fabsf(all) < INFINITY);
+    const float log_total = none ? NAN : logf(s);
+    if (lane == 0 && A.entropy) A.entropy[row] = log_total - LN2 * (w / s);
+    for (int i = lane; i < A.given; i += 32) {
+        const int t = A.tokens[row * A.given + i];
+        const float v = t >= 0 && t < A.vocab ? fmaxf(ib_to_float(x[t]), -INFINITY) : -INFINITY;
+        A.log_probs[row * A.given + i] = (v - all) - log_total;
+    }
+    if constexpr (TOP) {
+        u64 mine = 0;                      // the lane-th likeliest
+#pragma unroll 1
+        for (int i = 0; i < A.top; ++i) {
+            u64 best = 0;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) best = max(best, keys[b]);
+            best = warp_best(best);
+            if (best == 0) break;
+            // a block's key is that of a logit that comes next, or, before the first one was taken, no less than its largest logit's
+            const int block = place_of(best) / EACH, place = block * EACH + (lane & (EACH - 1));
+            u64 key = 0;
+            if (place >= skew && place < end) {
+                const float z = ib_to_float(from[place]);
+                key = z == z ? key_of(z, place) : 0;
+            }
+            if (key > best) key = 0;
+            const u64 first = warp_best(key), second = warp_best(key == first ? 0 : key);
+            if (lane == i) mine = first;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+                if (b * 32 + lane == block) keys[b] = second;
+        }
+        if (lane < A.top) {
+            A.top_ids[row * A.top + lane] = mine ? place_of(mine) - skew : -1;
+            A.top_log_probs[row * A.top + lane] = mine ? (value_of(mine) - all) - log_total : -INFINITY;
+        }
+    }
+}
+
 template <typename T, bool TOP>
 static int launch(const Args& a, int cluster, cudaStream_t stream) {
+    if (cluster == 0) {
+        const unsigned grid = (unsigned)((a.rows + 3L) / 4);
+        if (a.vocab + 7 <= SHORT / 2) short_rows_kernel<T, TOP, LANE_BLOCKS / 2><<<grid, 128, 0, stream>>>(a);
+        else short_rows_kernel<T, TOP, LANE_BLOCKS><<<grid, 128, 0, stream>>>(a);
+        return ib_launch_status();
+    }
     static IbDeviceSet done;
     if (const int code = ib_allow_dynamic_smem(done, log_probs_kernel<T, TOP>, sizeof(Shared))) return code;
     cudaLaunchConfig_t cfg = {};
@@ -506,11 +612,14 @@ IB_EXPORT int ib_token_log_probs(const void* call) {
     if (c.top > MAX_TOP || c.vocab > 0x40000000L || c.rows > 0x7fffffffL / MAX_CLUSTER || c.given > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
     if (c.rows == 0) return IB_OK;
     const Args a{c.logits, c.tokens, c.log_probs, c.entropy, c.top_ids, c.top_log_probs, c.ld, (int)c.rows, (int)c.vocab, (int)c.given, (int)c.top};
+    // A warp for a row of few logits where there are more rows than the SMs hold CTAs, or few logits and few tokens wanted of them.  (A CTA and a
+    // warp a row: 4,096 rows of 1,000 with the five likeliest 60.6 and 10.1 us, of 8,000 73 and 39; 500 rows of 8,000 13.8 and 10.9, with 32
+    // 18.2 and 18.9; 300 rows of 1,000 8.2 and 4.7, of 8,000 9.0 and 10.9, of 1,000 with 32 9.3 and 10.9.)
+    int cluster = c.vocab + 7 <= SHORT && (c.rows > 444 || (c.vocab <= 2048 && c.top <= 8)) ? 0 : 1;
     // As many CTAs for a row as the machine has room for (three on each of 148 SMs), each with at least a chunk's logits.  (1, 2, 4, 8 CTAs a row, the
     // five most likely tokens: 128 rows of 151,936 logits 30, 22.5, 29, 36 us; one row 28, 18.8, 13.4, 10.1; one of 16,384 8.0, 7.8, 7.2, 7.4;
     // one of 4,000 6.2, 7.1, 7.2, 7.2.)
-    int cluster = 1;
-    while (cluster < MAX_CLUSTER && c.rows * cluster * 2 <= 444 && c.vocab >= 4096L * cluster * 2) cluster *= 2;
+    while (cluster > 0 && cluster < MAX_CLUSTER && c.rows * cluster * 2 <= 444 && c.vocab >= 4096L * cluster * 2) cluster *= 2;
     if (c.f32) return c.top ? launch<float, true>(a, cluster, c.stream) : launch<float, false>(a, cluster, c.stream);
     return c.top ? launch<__nv_bfloat16, true>(a, cluster, c.stream) : launch<__nv_bfloat16, false>(a, cluster, c.stream);
 }

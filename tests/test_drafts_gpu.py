@@ -513,6 +513,40 @@ def test_log_probs_hard_rows(dtype, rows):
             same(got[r], want[r], vocab, min(big, 1e5) * 4)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,vocab,given,top,skew", [
+    (445, 1, 1, 1, 0), (445, 15, 40, 32, 1), (450, 16, 1, 16, 0), (446, 300, 1, 20, 3), (1001, 512, 2, 5, 7), (447, 513, 1, 32, 8), (500, 4089, 1, 8, 1),
+    (500, 4090, 1, 8, 0), (445, 8185, 1, 32, 5), (445, 8186, 1, 3, 5), (3, 2048, 1, 8, 2), (1, 300, 1, 0, 3), (9, 2049, 3, 8, 1), (2, 40, 33, 8, 0)])
+def test_log_probs_of_few_logits_a_row(dtype, rows, vocab, given, top, skew):
+    g = torch.Generator(device=DEV).manual_seed(vocab + rows)
+    wide = torch.full((rows, vocab + 9 + skew), 1e4, device=DEV).to(dtype)
+    x = wide[:, skew:skew + vocab]
+    x.copy_(3 * torch.randn((rows, vocab), generator=g, device=DEV))
+    compare(x, torch.randint(0, vocab, (rows, given), generator=g, device=DEV).to(torch.int32), top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("vocab,top,rows", [(700, 20, 460), (700, 8, 19), (8000, 32, 460), (2000, 8, 460), (20, 32, 460)])
+def test_log_probs_hard_rows_of_few_logits(dtype, vocab, top, rows):
+    inf, nan = float("inf"), float("nan")
+    at = torch.arange(vocab, device=DEV)
+    up = at.to(F32) / 64
+    kinds = [torch.zeros(vocab, device=DEV), torch.full((vocab,), -3.5, device=DEV), up, up.flip(0), torch.where(at == 7, 90.0, 0.0),
+             torch.where(at < vocab - 5, -inf, up), torch.where(at < vocab - 5, torch.finfo(dtype).min, up), torch.full((vocab,), -inf, device=DEV),
+             torch.where(at == 5, inf, up), torch.where(at == 5, nan, up), torch.full((vocab,), nan, device=DEV), torch.where(at > 4, nan, up),
+             torch.where(at > 4, -inf, -up), torch.where(at == 0, -0.0, 0.0), 1e4 + up, up * 1e30, torch.where(at % 2 == 0, up, -up),
+             torch.where(at % 16 == 3, 5.0, nan), up.flip(0).roll(vocab // 3)]
+    x = torch.stack(kinds).to(dtype).repeat(-(-rows // len(kinds)), 1)[:rows].contiguous()
+    t = torch.randint(-3, vocab + 3, (rows, 4), device=DEV).to(torch.int32)
+    lp, h, ids, best = scored(x, t, top)
+    wlp, wh, wids, wbest = plain.log_probs(x, t, top)
+    assert torch.equal(ids.cpu().long(), wids)
+    for got, want in ((lp, wlp), (best, wbest), (h[:, None], wh[:, None])):
+        for r in range(rows):              # (rows that start elsewhere within 16 bytes are added up in another order)
+            big = float(x[r].float().nan_to_num(0.0, 0.0, 0.0).abs().max())
+            same(got[r], want[r], vocab, min(big, 1e5) * 4)
+
+
 def test_log_probs_replayed():
     x = torch.randn((4, 40000), device=DEV)
     t = torch.randint(0, 40000, (4, 1), device=DEV).to(torch.int32)
