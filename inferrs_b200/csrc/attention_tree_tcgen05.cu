@@ -25,6 +25,7 @@
 // What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So the values of tiles that
 // some row does not see in full come with cp.async, and the warps that fill the ring look at what they brought, put zeros in the place of those that are
 // infinite or no numbers, and the rows that see such a value get it added at the end, from its page.
+#include "clusters.cuh"
 #include "sm100.cuh"
 #include "tree.cuh"
 
@@ -37,7 +38,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
-constexpr int MOST_PARTS = 8;
+constexpr int MOST_PARTS = IB_MAX_CLUSTER;
 constexpr int SLICE = 24, MOST_SLICES = 64;      // tiles (see launch)
 constexpr int RANKED = 1024;          // requests that are put in order of their length
 
@@ -837,26 +838,41 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     write_row<D, 4>(A, S, place, first_row + row, head, e, 4, o, total, bad_values, t_first, all_tiles, lo_max);
 }
 
+// How a call is cut: row tiles of NQ x 128 rows, a part of the keys for each CTA, in clusters or (waves) in slices
+struct Cut { long pairs, parts; int tiles_of_rows, tiles; bool waves; };
+
 template <int D, int NQ>
-static long launch(Args A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream) {
-    A.tiles_of_rows = (int)(((long)max_tree * (A.n_heads / A.n_kv) + NQ * ROWS - 1) / (NQ * ROWS));
-    const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
-    const int tiles = (max_keys + KEYS - 1) / KEYS;
+static int cut_of(const Args& A, int max_tree, int max_keys, Cut& c) {
+    static IbDeviceSet done;
+    if (const int code = ib_allow_dynamic_smem(done, tree_kernel<D, NQ>, Shape<D, NQ>::SMEM)) return code;
+    c.tiles_of_rows = (int)(((long)max_tree * (A.n_heads / A.n_kv) + NQ * ROWS - 1) / (NQ * ROWS));
+    c.pairs = (long)A.n_requests * A.n_kv * c.tiles_of_rows;
+    long keys = max_keys;
+    if (A.span > 0 && keys > (long)A.span + max_tree + KEYS) keys = (long)A.span + max_tree + KEYS;
+    c.tiles = (int)((keys + KEYS - 1) / KEYS);
     // One wave of CTAs: as many parts as there are SMs for, a cluster each.  More than that: requests differ in length, and clusters would wait
     // for as many free SMs at once; slices of 24 tiles or more, the longest requests first, are joined by a kernel of their own.  (Trees of 64,
     // 32 heads on 8, 16 requests of 100 to 16,384 keys: slices of 12, 16, 24, 32 tiles 190, 180, 167, 178 us, whole requests 246; all of 16,384:
     // 325, 306, 305, 299; of 100 to 4,500: 67, 73, and whole ones, which 24 leaves them, 73.)
-    const bool waves = 2 * pairs > 148 && tiles > 2 * SLICE;
-    long parts = waves ? (tiles + SLICE - 1) / SLICE : 148 / pairs;
-    if (parts > tiles) parts = tiles;
-    const long most = waves ? MOST_SLICES : MOST_PARTS;
-    parts = parts < 1 ? 1 : parts > most ? most : parts;
-    const long needed = waves && parts > 1 ? pairs * parts * Shape<D, NQ>::SLICE_SUMS * 4 : 0;
+    c.waves = 2 * c.pairs > 148 && c.tiles > 2 * SLICE;
+    c.parts = c.waves ? (c.tiles + SLICE - 1) / SLICE : 148 / c.pairs;
+    if (c.parts > c.tiles) c.parts = c.tiles;
+    const long most = c.waves ? MOST_SLICES : MOST_PARTS;
+    c.parts = c.parts < 1 ? 1 : c.parts > most ? most : c.parts;
+    // (Clusters that do not all run at once take twice the time: 5 requests of 20 pairs with a window 26.2 us in clusters of seven, 16.2 in six.)
+    static IbClusters clusters;
+    while (!c.waves && c.parts > 1 && ib_clusters_at_once(clusters, tree_kernel<D, NQ>, (int)c.parts, THREADS, Shape<D, NQ>::SMEM) < c.pairs) --c.parts;
+    return IB_OK;
+}
+
+template <int D, int NQ>
+static long launch(Args A, const Cut& c, void* workspace, bool ask, cudaStream_t stream) {
+    const long pairs = c.pairs, parts = c.parts;
+    A.tiles_of_rows = c.tiles_of_rows;
+    const long needed = c.waves && parts > 1 ? pairs * parts * Shape<D, NQ>::SLICE_SUMS * 4 : 0;
     if (ask) return needed;
     float* scratch = needed ? static_cast<float*>(workspace) : nullptr;
     if (needed && workspace == nullptr) return IB_ERR_ARGUMENT;
-    static IbDeviceSet done;
-    if (const int code = ib_allow_dynamic_smem(done, tree_kernel<D, NQ>, Shape<D, NQ>::SMEM)) return code;
     // boxes of a page's places, or of 128 in larger pages, where whole ones make a tile and start on eight rows
     int box = A.page_shift >= 3 ? (A.page_size < KEYS ? A.page_size : KEYS) : 0;
     CUtensorMap map_k = {}, map_v = {};
@@ -881,15 +897,28 @@ static long launch(Args A, int max_tree, int max_keys, void* workspace, bool ask
     return ib_launch_status();
 }
 
+// Two sets of rows share a CTA's keys, or each has CTAs of its own, with half as many parts and a shorter start and join.  In tiles of keys a CTA,
+// n1 and n2, one set takes about 10 + 1.25 n1 us and two take 14 + 1.85 n2.  (Trees of 64, 32 heads on 8 of 128; one set and two: 1 request of 2,000
+// keys 15.0 and 21.5 us, 4 21.5 and 23.7, 8 31.6 and 28.9; 4 of 30,000 156 and 117.  5 chains of 37, 20 heads on 4 of 64, window 1,500: 15.0 and 16.2.)
+template <int D>
+static long launch(const Args& A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream) {
+    Cut one, two;
+    if (const int code = cut_of<D, 1>(A, max_tree, max_keys, one)) return code;
+    if ((long)max_tree * (A.n_heads / A.n_kv) > ROWS) {
+        if (const int code = cut_of<D, 2>(A, max_tree, max_keys, two)) return code;
+        const long n1 = one.waves ? one.pairs * one.tiles / 148 : (one.tiles + one.parts - 1) / one.parts, n2 = (two.tiles + two.parts - 1) / two.parts;
+        if (2 * two.pairs > 148 || 2 * n1 > 3 * n2 + 6) return launch<D, 2>(A, two, workspace, ask, stream);
+    }
+    return launch<D, 1>(A, one, workspace, ask, stream);
+}
+
 }  // namespace tree_tc
 
 long ib_tree_tcgen05(tree::Args A, int max_tree, int max_keys, void* workspace, bool ask, cudaStream_t stream) {
     using namespace tree_tc;
     const uintptr_t at = reinterpret_cast<uintptr_t>(A.q) | reinterpret_cast<uintptr_t>(A.k) | reinterpret_cast<uintptr_t>(A.v);
     if ((A.dim != 64 && A.dim != 128) || at % 16 || !(A.scale_log2 > 0.0f)) return IB_ERR_UNSUPPORTED;
-    const bool two = (long)max_tree * (A.n_heads / A.n_kv) > ROWS;
-    if (A.dim == 128) return two ? launch<128, 2>(A, max_tree, max_keys, workspace, ask, stream) : launch<128, 1>(A, max_tree, max_keys, workspace, ask, stream);
-    return two ? launch<64, 2>(A, max_tree, max_keys, workspace, ask, stream) : launch<64, 1>(A, max_tree, max_keys, workspace, ask, stream);
+    return A.dim == 128 ? launch<128>(A, max_tree, max_keys, workspace, ask, stream) : launch<64>(A, max_tree, max_keys, workspace, ask, stream);
 }
 
 IB_EXPORT int ib_attention_tree_error(int reset) {

@@ -18,7 +18,7 @@
 // bound it (186 us with five).  A warp of its own fetches (bulk copies into 64 KB, three CTAs an SM), and a logit costs one exponential and half
 // of a packed instruction of each other kind.  Few rows are bound by the chain from the first copy through the bounds to the join of a row's CTAs: one
 // row takes 6.6 us, 10.1 with the five most likely tokens.
-#include "common.cuh"
+#include "clusters.cuh"
 #include "sm100.cuh"
 
 namespace lp {
@@ -28,7 +28,6 @@ constexpr int RING = 4096;           // 16-byte vectors that may be on their way
 constexpr int MAX_TOP = 32;
 constexpr int NOTES = 1024;          // room for noted keys
 constexpr int GROUPS = 64;           // groups of 4 threads whose largest keys give the first bound
-constexpr int MAX_CLUSTER = 8;
 constexpr float LOWEST = -300.0f;    // 2^-300 is 0 in 32 bits, and 0 times it is 0
 
 typedef unsigned long long u64;
@@ -422,7 +421,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         const float all = ib_warp_max(mc);
         move_reference(mc, all, total, weighed);
 #pragma unroll
-        for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) {
+        for (int o = IB_MAX_CLUSTER / 2; o > 0; o >>= 1) {
             total += __shfl_xor_sync(0xffffffffu, total, o);
             weighed += __shfl_xor_sync(0xffffffffu, weighed, o);
             have += __shfl_xor_sync(0xffffffffu, have, o);
@@ -569,8 +568,8 @@ __global__ void __launch_bounds__(128) short_rows_kernel(const Args A) {
 }
 
 template <typename T, bool TOP>
-static int launch(const Args& a, int cluster, cudaStream_t stream) {
-    if (cluster == 0) {
+static int launch(const Args& a, bool short_rows, cudaStream_t stream) {
+    if (short_rows) {
         const unsigned grid = (unsigned)((a.rows + 3L) / 4);
         if (a.vocab + 7 <= SHORT / 2) short_rows_kernel<T, TOP, LANE_BLOCKS / 2><<<grid, 128, 0, stream>>>(a);
         else short_rows_kernel<T, TOP, LANE_BLOCKS><<<grid, 128, 0, stream>>>(a);
@@ -578,6 +577,13 @@ static int launch(const Args& a, int cluster, cudaStream_t stream) {
     }
     static IbDeviceSet done;
     if (const int code = ib_allow_dynamic_smem(done, log_probs_kernel<T, TOP>, sizeof(Shared))) return code;
+    // As many CTAs for a row as the machine has room for (three on each of 148 SMs, clusters that run at once), each with at least a chunk's logits.
+    // (1, 2, 4, 8 CTAs a row, the five most likely tokens: 128 rows of 151,936 logits 30, 22.5, 29, 36 us; one row 28, 18.8, 13.4, 10.1; one of 16,384
+    // 8.0, 7.8, 7.2, 7.4; one of 4,000 6.2, 7.1, 7.2, 7.2.  50 rows, whose clusters of eight take two turns, 21.1, of four 15.7.)
+    static IbClusters clusters;
+    int cluster = 1;
+    while (cluster < IB_MAX_CLUSTER && (long)a.rows * cluster * 2 <= 444 && a.vocab >= 4096L * cluster * 2) cluster *= 2;
+    while (cluster > 1 && ib_clusters_at_once(clusters, log_probs_kernel<T, TOP>, cluster, THREADS + 32, sizeof(Shared)) < a.rows) cluster /= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.gridDim = dim3((unsigned)(a.rows * cluster));
@@ -609,19 +615,15 @@ IB_EXPORT int ib_token_log_probs(const void* call) {
     using namespace lp;
     const IbTokenLogProbs c = *static_cast<const IbTokenLogProbs*>(call);
     if (c.rows < 0 || c.vocab <= 0 || c.given < 0 || c.top < 0) return IB_ERR_ARGUMENT;
-    if (c.top > MAX_TOP || c.vocab > 0x40000000L || c.rows > 0x7fffffffL / MAX_CLUSTER || c.given > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
+    if (c.top > MAX_TOP || c.vocab > 0x40000000L || c.rows > 0x7fffffffL / IB_MAX_CLUSTER || c.given > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
     if (c.rows == 0) return IB_OK;
     const Args a{c.logits, c.tokens, c.log_probs, c.entropy, c.top_ids, c.top_log_probs, c.ld, (int)c.rows, (int)c.vocab, (int)c.given, (int)c.top};
     // A warp for a row of few logits where there are more rows than the SMs hold CTAs, or few logits and few tokens wanted of them.  (A CTA and a
     // warp a row: 4,096 rows of 1,000 with the five likeliest 60.6 and 10.1 us, of 8,000 73 and 39; 500 rows of 8,000 13.8 and 10.9, with 32
     // 18.2 and 18.9; 300 rows of 1,000 8.2 and 4.7, of 8,000 9.0 and 10.9, of 1,000 with 32 9.3 and 10.9.)
-    int cluster = c.vocab + 7 <= SHORT && (c.rows > 444 || (c.vocab <= 2048 && c.top <= 8)) ? 0 : 1;
-    // As many CTAs for a row as the machine has room for (three on each of 148 SMs), each with at least a chunk's logits.  (1, 2, 4, 8 CTAs a row, the
-    // five most likely tokens: 128 rows of 151,936 logits 30, 22.5, 29, 36 us; one row 28, 18.8, 13.4, 10.1; one of 16,384 8.0, 7.8, 7.2, 7.4;
-    // one of 4,000 6.2, 7.1, 7.2, 7.2.)
-    while (cluster > 0 && cluster < MAX_CLUSTER && c.rows * cluster * 2 <= 444 && c.vocab >= 4096L * cluster * 2) cluster *= 2;
-    if (c.f32) return c.top ? launch<float, true>(a, cluster, c.stream) : launch<float, false>(a, cluster, c.stream);
-    return c.top ? launch<__nv_bfloat16, true>(a, cluster, c.stream) : launch<__nv_bfloat16, false>(a, cluster, c.stream);
+    const bool short_rows = c.vocab + 7 <= SHORT && (c.rows > 444 || (c.vocab <= 2048 && c.top <= 8));
+    if (c.f32) return c.top ? launch<float, true>(a, short_rows, c.stream) : launch<float, false>(a, short_rows, c.stream);
+    return c.top ? launch<__nv_bfloat16, true>(a, short_rows, c.stream) : launch<__nv_bfloat16, false>(a, short_rows, c.stream);
 }
 
 IB_EXPORT int ib_log_probs_error(int reset) {

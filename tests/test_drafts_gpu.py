@@ -135,6 +135,37 @@ def test_tree_attention_requests_of_very_different_length(d, heads, kv, most, sp
     assert torch.isnan(got[hit]).all() and torch.isfinite(got[~hit]).all()
 
 
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (128, 24), (64, 256)])
+@pytest.mark.parametrize("requests,span", [(5, None), (5, 900), (5, -700), (10, None), (10, 64)])
+def test_tree_attention_many_rows_over_many_keys(d, page, requests, span):
+    """Enough CTAs that two sets of rows share their keys: in clusters (5 requests) and alone (10)."""
+    contexts, trees = ([1100, 900, 0, 1000, 130], [40, 37, 33, 40, 1])
+    if requests == 10:
+        contexts, trees = contexts[1:] + [300, 5, 128, 127, 400, 64], trees[1:] + [40, 39, 2, 0, 36, 40]
+    c = drafted(31, contexts, trees, 32, 8, d, page, BF, chain=page == 24, spare=1)
+    out = attend(c, span)
+    check(c, out, span)
+    # a value that is no number: the rows that see it, no others
+    c["v"][c["table"][0, contexts[0] // page], :, contexts[0] % page] = float("nan")
+    c["v"][c["table"][1, 3 // page], :, 3 % page] = float("inf")
+    got = attend(c, span)
+    finite = torch.isfinite(got.float().view(got.shape[0], 32, d)).all(2).all(1)
+    hit = torch.zeros(out.shape[0], dtype=torch.bool, device=DEV)
+    hit[:trees[0]] = (c["seen"][:trees[0], 0] & 1).bool()
+    rows = slice(trees[0], trees[0] + trees[1])
+    at = c["positions"][rows]
+    if contexts[1] <= 3:                  # (place 3 is a drafted token)
+        hit[rows] = (c["seen"][rows, 0] >> (3 - contexts[1]) & 1).bool()
+    else:
+        hit[rows] = True if span is None else at - span < 3 if span > 0 else at // -span == 0
+    assert torch.equal(finite, ~hit)
+    assert torch.equal(got[~hit], out[~hit])
+    c["table"][0, 2] = -1                 # a page that is not there
+    c["v"][c["table"][0, contexts[0] // page], :, contexts[0] % page] = 1.0
+    c["v"][c["table"][1, 3 // page], :, 3 % page] = 1.0
+    check(c, attend(c, span), span)
+
+
 def test_tree_attention_many_requests_and_splits():
     rng = random.Random(3)
     contexts = [rng.choice([0, 1, 17, 200, 900]) for _ in range(40)]
