@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
 
     float m = -INFINITY, s = 0.0f, w = 0.0f;
     u64 bound = 0;                    // keys below it are not noted
+    float least = -INFINITY;          // its value
     const int rounds = (v_hi - v_lo + CHUNK - 1) / CHUNK;
     int round = 0, next_look = 2;
     bool ok = true;
@@ -256,7 +257,10 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         const int left = min(n, A.top);
         if (tid < left) sh.notes[tid] = sh.board.best[tid];
         if (tid == 0) sh.n_notes = left;
-        if (left == A.top) bound = max(bound, sh.board.best[A.top - 1]);
+        if (left == A.top) {
+            bound = max(bound, sh.board.best[A.top - 1]);
+            least = value_of(bound);
+        }
         meet(false);
     };
     // the given tokens' logits, on their way meanwhile
@@ -285,13 +289,14 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         const int stage = round % STAGES;
         if (ok && !mbar_wait(sm100::smem_u32(&sh.full[stage]), (round / STAGES) & 1, 2)) ok = false;
         float e[EACH];
+        // (a thread's vectors are neighbours; in an order of its own, so that eight threads' meet all banks)
 #pragma unroll
-        for (int i = 0; i < VECTORS; ++i) {
-            // (a thread's vectors are neighbours; in an order of its own, so that eight threads' meet all banks)
-            const int v = v0 + tid * VECTORS + ((i + lane / (8 / VECTORS)) & (VECTORS - 1));
-            if (v >= w_lo && v < w_hi) {
-                Wide<T>::unpack(sh.ring[stage * CHUNK + v - v0], e + i * N);
-            } else {
+        for (int i = 0; i < VECTORS; ++i) Wide<T>::unpack(sh.ring[stage * CHUNK + tid * VECTORS + ((i + lane / (8 / VECTORS)) & (VECTORS - 1))], e + i * N);
+        if (v0 < w_lo || v0 + CHUNK > w_hi) {      // at a row's ends some vectors are not whole
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) {
+                const int v = v0 + tid * VECTORS + ((i + lane / (8 / VECTORS)) & (VECTORS - 1));
+                if (v >= w_lo && v < w_hi) continue;
 #pragma unroll
                 for (int c = 0; c < N; ++c) {
                     const int at = v * N - skew + c;
@@ -304,16 +309,18 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) top = fmaxf(top, e[i]);
-        bool any = false;          // (a logit of minus infinity is one, no number is none)
-        if (TOP && top == -INFINITY) {
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) any |= e[i] == e[i];
-        }
         add_block<EACH>(e, top, m, s, w);
         if constexpr (TOP) {
-            const u64 key = top > -INFINITY || any ? key_of(top, v0 + tid * VECTORS) : 0;
+            auto key = [&]() -> u64 {      // (a logit of minus infinity is one, no number is none)
+                bool any = top > -INFINITY;
+                if (!any) {
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) any |= e[i] == e[i];
+                }
+                return any ? key_of(top, v0 + tid * VECTORS) : 0;
+            };
             if (round == 0) {      // the first bound
-                u64 best = key;
+                u64 best = key();
 #pragma unroll
                 for (int o = 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
                 if ((tid & 3) == 0) sh.groups[tid >> 2] = best;
@@ -328,8 +335,12 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
                 if ((tid & 3) == 0 && ahead == A.top - 1) sh.bound = mine;       // (0 where fewer groups hold a number)
                 meet(false);
                 bound = sh.bound;
+                if (bound) least = value_of(bound);
             }
-            if (key >= bound && key) note(key);
+            if (top >= least) {
+                const u64 mine = key();
+                if (mine >= bound && mine) note(mine);
+            }
             if (round == next_look) {      // (not when few logits are to come: the last look is near)
                 if (3 * round < rounds) {
                     meet(false);
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
         // the k best blocks' logits: those that reach the k-th block's largest one
         prune();
         const int blocks = sh.n_notes;
-        const float least = blocks == A.top ? value_of(bound) : -INFINITY;
+        if (blocks < A.top) least = -INFINITY;
         meet(false);
         if (tid == 0) sh.n_notes = 0;
         meet(false);
