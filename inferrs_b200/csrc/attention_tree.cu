@@ -33,11 +33,11 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
 // What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles for some 2,000 instructions), so what counts is
 // how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows, when that was changed: 355 us, with two 443),
 // and eight rows a CTA where there are no more or few CTAs (with eight and with sixteen: 41 requests of 2,000 keys 245 and 386 us; 2 trees of 13
-// over up to 777 29.0 and 31.8; 2 trees of 64 over up to 1,000 with 64 heads 262 and 200).  PER numbers of a
+// over up to 777 26.5 and about 29; 2 trees of 64 over up to 1,000 with 64 heads 262 and 200).  PER numbers of a
 // head per lane, four neighbours where that is a multiple of four.
 template <typename T, int PER, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts, bool wide) {
-    constexpr int MINE = ROWS / WARPS;
+    constexpr int MINE = ROWS / WARPS, SIDE = PER <= 4 ? 4 : 16 / PER;
     extern __shared__ __align__(16) unsigned char raw[];
     const int d = A.dim, dp = padded(d), rb = row_bytes<T>(d);
     float* sq = reinterpret_cast<float*>(raw);    // [ROWS][dp], later the part's sums
@@ -214,22 +214,27 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
     if (parts > 1) cluster_sync(); else __syncthreads();
 #pragma unroll 1
     for (int row = part + warp * parts; row < used; row += WARPS * parts) {
-        float top = -INFINITY, total = 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < parts; ++c) top = fmaxf(top, remote_f32(&sml[row], c));
-        const float ref = top == -INFINITY ? 0.0f : top;
+        // a lane looks at a part's reference and denominator, then all look at some parts' sums at once: a look into another CTA takes 700 cycles
+        const float mc = lane < parts ? remote_f32(&sml[row], lane) : -INFINITY, lc = lane < parts ? remote_f32(&sml[ROWS + row], lane) : 0.0f;
+        const float top = ib_warp_max(mc), ref = top == -INFINITY ? 0.0f : top;
+        const float f = lc == 0.0f ? 0.0f : exp2f(mc - ref);           // (0: this part of the keys holds none that the row sees)
+        const float total = ib_warp_sum(lc * f);
         float o[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) o[i] = 0.0f;
 #pragma unroll 1
-        for (int c = 0; c < parts; ++c) {
-            const float lc = remote_f32(&sml[ROWS + row], c);
-            if (lc == 0.0f) continue;             // this part of the keys holds none that the row sees
-            const float f = exp2f(remote_f32(&sml[row], c) - ref);
-            total = fmaf(lc, f, total);
+        for (int c = 0; c < parts; c += SIDE) {
+            float v[SIDE][PER];
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (number(i) < d) o[i] = fmaf(remote_f32(&sq[row * dp + number(i)], c), f, o[i]);
+            for (int k = 0; k < SIDE; ++k)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[k][i] = c + k < parts && number(i) < d ? remote_f32(&sq[row * dp + number(i)], c + k) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < SIDE; ++k) {
+                const float fc = __shfl_sync(0xffffffffu, f, c + k);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) o[i] = fmaf(v[k][i], fc, o[i]);
+            }
         }
         const int at = first_row + row, tok = at / group;
         T* dst = static_cast<T*>(A.out) + (long)(S.row0 + tok) * A.out_ld + (long)(head * group + at - tok * group) * d;
