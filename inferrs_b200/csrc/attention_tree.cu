@@ -31,10 +31,12 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
 }
 
 // What bounds it are the warps' own chains of instructions (a tile takes one about 8,000 cycles for some 2,000 instructions), so what counts is
-// how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows, when that was changed: 355 us, with two 443),
-// and eight rows a CTA where there are no more or few CTAs (with eight and with sixteen: 41 requests of 2,000 keys 245 and 386 us; 2 trees of 13
-// over up to 777 26.5 and about 29; 2 trees of 64 over up to 1,000 with 64 heads 262 and 200).  PER numbers of a
-// head per lane, four neighbours where that is a multiple of four.
+// how many share an SM: one tile of shared memory a CTA, not two (41 requests of 2,000 keys, 32 heads on 8, eight rows, when that was changed:
+// 355 us, with two 443), and eight rows a CTA where there are no more or few CTAs (with eight and with sixteen: 41 requests of 2,000 keys 245 and
+// 386 us; 2 trees of 13 over up to 777 26.5 and 29; 2 trees of 64 over up to 1,000 with 64 heads 262 and 200).  Four groups of warps with a tile
+// each in one CTA, where there are few pairs, were slower below some 4,000 keys (1 request of 300 keys 21.5 us, 14.7 as it is; of 9,000 115 and 142).
+// Loops of 16 as they stand below took 3 to 5 % off loops of 8 and 4 (41 requests 238 us, 2 trees of 13 25.8).  PER numbers of a head per lane, four
+// neighbours where that is a multiple of four.
 template <typename T, int PER, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int parts, bool wide) {
     constexpr int MINE = ROWS / WARPS, SIDE = PER <= 4 ? 4 : 16 / PER;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         float dot[MINE];
 #pragma unroll
         for (int r = 0; r < MINE; ++r) dot[r] = 0.0f;
-#pragma unroll 8
+#pragma unroll 16
         for (int e = 0; e < dp; e += 4) {
             const float4 kk = four(sk + e);
 #pragma unroll
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
 #pragma unroll
         for (int r = 0; r < MINE; ++r) mine[lane * MINE + r] = p[r];
         __syncwarp();
-#pragma unroll 4
+#pragma unroll 16
         for (int key = 0; key < KEYS; ++key) {
             const T* sv = reinterpret_cast<const T*>(tile + (KEYS + key) * rb);
             float pk[MINE];

@@ -13,11 +13,11 @@
 // 2, 5, 11 .. the k best of the noted ones give a higher bound.  The first bound is the k-th largest of 64 groups' largest keys; expected are k
 // to 2 k notes from the first 4,096 logits and k more for every doubling behind them.  At the end the k blocks are looked through.
 //
-// Many rows of 32 bits are bound by memory: 2,048 rows of 151,936 logits take 181 us without and 196 with the most likely token (190 at the
-// copy rate, which counts a write for every read), 235 with the 32 most likely ones; in bfloat16, which are half the bytes, the instructions
-// bound it (186 us with five).  A warp of its own fetches (bulk copies into 64 KB, three CTAs an SM), and a logit costs one exponential and half
-// of a packed instruction of each other kind.  Few rows are bound by the chain from the first copy through the bounds to the join of a row's CTAs: one
-// row takes 6.6 us, 10.1 with the five most likely tokens.
+// Many rows of 32 bits are bound by memory: 2,048 rows of 151,936 logits take 179 us without and 191 with the most likely token (190 at the
+// copy rate, which counts a write for every read), 218 with the 32 most likely ones; in bfloat16, which are half the bytes, the instructions
+// bound it (172 us with five).  A warp of its own fetches (bulk copies into 64 KB, three CTAs an SM), and a logit costs one exponential and half
+// of a packed instruction of each other kind.  Few rows are bound by the chain from the first copy through the bounds to the join of a row's CTAs:
+// one row takes 6.6 us, 10 with the five most likely tokens.
 #include "clusters.cuh"
 #include "sm100.cuh"
 
