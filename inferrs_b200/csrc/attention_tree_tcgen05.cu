@@ -356,12 +356,32 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const int first_row = row_tile * (NQ * ROWS);
     const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
     if (rows <= 0) return;            // (the whole cluster leaves)
-    if (scratch != nullptr && part > 0 && (long)part * SLICE * KEYS >= S.keys) return;       // (there are no more slices than this)
 
     if (tid == 0) {
         sm.lo_min = 0x7fffffff;
         sm.lo_max = 0;
         sm.bad_values = 0;
+    }
+    // the first keys that the CTA's rows see: the least and the greatest
+    auto first_keys = [&]() {
+        const int t0 = first_row / group, t1 = (first_row + rows - 1) / group;
+#pragma unroll 1
+        for (int t = t0 + tid; t <= t1; t += THREADS) {
+            const int lo = first_key(A, S, t);
+            atomicMin(&sm.lo_min, lo);
+            atomicMax(&sm.lo_max, lo);
+        }
+        __syncthreads();
+    };
+    if (scratch != nullptr) {
+        // A CTA that no slice is left for has no rows to write and no place for sums: it leaves before it takes anything.  What is left behind a
+        // span's first keys may be fewer slices than the request's keys alone would give, one even.
+        if (A.span != 0) {
+            __syncthreads();
+            first_keys();
+        }
+        const int t0 = A.span != 0 ? min(sm.lo_min, S.context) / KEYS : 0;
+        if (part >= slices_of((S.keys + KEYS - 1) / KEYS - t0, slices)) return;
     }
     if (warp == ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
@@ -382,23 +402,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     fence_before();
     __syncthreads();
     fence_after();
-    if (A.span != 0) {                // the first keys that the CTA's rows see: the least and the greatest
-        const int t0 = first_row / group, t1 = (first_row + rows - 1) / group;
-#pragma unroll 1
-        for (int t = t0 + tid; t <= t1; t += THREADS) {
-            const int lo = first_key(A, S, t);
-            atomicMin(&sm.lo_min, lo);
-            atomicMax(&sm.lo_max, lo);
-        }
-        __syncthreads();
-    }
+    if (A.span != 0 && scratch == nullptr) first_keys();
     const int lo_min = A.span != 0 ? min(sm.lo_min, S.context) : 0, lo_max = A.span != 0 ? sm.lo_max : 0;
     const unsigned tmem = sm.tmem;
     const int t_first = lo_min / KEYS, all_tiles = (S.keys + KEYS - 1) / KEYS - t_first;
     const int parts = scratch != nullptr ? slices_of(all_tiles, slices) : slices;
     const int t_begin = t_first + all_tiles * part / parts, t_end = t_first + all_tiles * (part + 1) / parts;      // (fewer than 2^24 tiles)
-    const int n = part < parts ? t_end - t_begin : 0;
-    const bool none = part >= parts;  // (with a window that leaves fewer slices: no keys, no rows to write)
+    const int n = t_end - t_begin;
     // tiles that each stream takes
     const int count0 = NQ == 2 ? n : (n + 1) / 2, count1 = NQ == 2 ? (rows > ROWS ? n : 0) : n / 2;
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
@@ -677,7 +687,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
             if (scratch == nullptr && parts > 1) cluster_sync();          // the cluster's tiles are free: sums may go to any CTA
-            if (NQ == 2 && parts == 1 && !none && !sm.bad_values) {
+            if (NQ == 2 && parts == 1 && !sm.bad_values) {
                 // no other sums of these rows: they go out from here, a thread a row
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 bf16* dst = static_cast<bf16*>(A.out) + (long)(S.row0 + token) * A.out_ld + (long)(head * group + at - token * group) * D;
@@ -759,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
-    if (none || (scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
+    if ((scratch != nullptr && parts > 1) || (NQ == 2 && parts == 1 && !sm.bad_values)) return;
     // Join: first the sums that this CTA has of a row (of two streams), which go to the CTA that writes the row (every parts-th),
     // and there those of the cluster's CTAs.  What goes out is not waited for; a look into another CTA's memory takes 700 cycles.  Eight lanes
     // a row, and loops as they stand: this code runs once, and unrolled ones wait for their instructions (ten cycles each) longer than they
