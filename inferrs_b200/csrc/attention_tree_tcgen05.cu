@@ -39,7 +39,8 @@ constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
 constexpr int MOST_PARTS = IB_MAX_CLUSTER;
-constexpr int SLICE = 24, MOST_SLICES = 64;      // tiles (see launch)
+constexpr int SLICE = 24, MOST_SLICES = 64;      // tiles (see cut_of)
+constexpr long MOST_SCRATCH = 256L << 20;        // bytes of all slices' sums (see cut_of)
 constexpr int RANKED = 1024;          // requests that are put in order of their length
 
 __device__ int g_error = 0;
@@ -54,7 +55,9 @@ template <int D, int NQ> struct Shape {
     static constexpr int OLD = D + 4;                              // floats between two rows of the sums: 16-byte stores of 8 lanes meet no bank twice
     static constexpr int TILES = (NQ + STAGES) * TILE;
     static constexpr int SUMS = 2 * ROWS * OLD * 4;
-    static constexpr int SLICE_SUMS = 2 * ROWS * (D + 2) + 4;      // floats of a slice's sums in the scratch: o [D / 4][line][4], m and l [line][2], whether it met bad values
+    // floats of a slice's sums in the scratch, where a tile has up to `most` rows: o [D / 4][line][4], m and l [line][2], whether it met bad values
+    static __host__ __device__ constexpr int lines(int most) { return NQ == 1 ? 2 * most : most; }
+    static __host__ __device__ constexpr int slice_sums(int most) { return lines(most) * (D + 2) + 4; }
     static constexpr int SMEM = 232448;                            // all that a CTA may have
     static_assert(1024 + TILES + 256 <= SMEM, "");
     static_assert((NQ == 1 ? SUMS + 4 * ROWS * 4 : 0) + (NQ * ROWS + 8) * (OLD + 4) * 4 <= TILES, "the sums take the place of the tiles");
@@ -313,7 +316,7 @@ __device__ __forceinline__ int slices_of(int tiles, int most) {
 template <int D, int NQ>
 __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                           const __grid_constant__ Args A, int slices, int ranked, int box,
-                                                          float* scratch) {
+                                                          float* scratch, int slice_rows) {
     typedef Shape<D, NQ> Sh;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     const Span S = span_of(A, req);
     const int group = A.group;
     const int first_row = row_tile * (NQ * ROWS);
-    const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
+    const int rows = min(S.n_tree * group - first_row, slice_rows);      // (NQ * ROWS, or what the scratch has room for)
     if (rows <= 0) return;            // (the whole cluster leaves)
 
     if (tid == 0) {
@@ -717,18 +720,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 }
             } else if (scratch != nullptr && parts > 1) {
                 // the sums of a slice, numbers four by four, so that a warp's stores lie side by side
-                float* to = scratch + (((long)(req * A.tiles_of_rows + row_tile) * A.n_kv + head) * slices + part) * Sh::SLICE_SUMS;
-                const int all = g * ROWS + r;
+                float* to = scratch + (((long)(req * A.tiles_of_rows + row_tile) * A.n_kv + head) * slices + part) * Sh::slice_sums(slice_rows);
+                const int lines = Sh::lines(slice_rows), all = g * (NQ == 2 ? ROWS : slice_rows) + r;
 #pragma unroll 1
                 for (int e = 0; e < D && count > 0; e += 32) {
                     unsigned x[32];
                     tmem_ld32(o_at + e, x);
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<uint4*>(to + ((e + k) / 4 * (2 * ROWS) + all) * 4) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                        *reinterpret_cast<uint4*>(to + ((e + k) / 4 * lines + all) * 4) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
                 }
-                *reinterpret_cast<float2*>(to + 2 * ROWS * D + 2 * all) = make_float2(m, ok ? l : NAN);
-                if (tid == 0) to[2 * ROWS * (D + 2)] = sm.bad_values ? 1.0f : 0.0f;
+                *reinterpret_cast<float2*>(to + lines * D + 2 * all) = make_float2(m, ok ? l : NAN);
+                if (tid == 0) to[lines * (D + 2)] = sm.bad_values ? 1.0f : 0.0f;
             } else if (NQ == 2) {
                 // the only sums of a row that this CTA has: they go to the CTA that writes the row, a thread a row
                 const int row = g * ROWS + r, i = share_of(row), owner = row - i * parts;
@@ -811,13 +814,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 // The rows whose keys were cut into slices by CTAs that do not run together: their sums lie in memory, slice by slice.  A thread
 // takes 16 numbers of a row, a warp 32 rows.
 template <int D, int NQ>
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args A, int slices, const float* __restrict__ scratch) {
-    constexpr int CHUNKS = NQ * ROWS * (D / 16) / 256, SUMS = Shape<D, NQ>::SLICE_SUMS, STREAMS = NQ == 1 ? 2 : 1;      // that have a row's sums
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args A, int slices, int slice_rows, const float* __restrict__ scratch) {
+    constexpr int CHUNKS = NQ * ROWS * (D / 16) / 256, STREAMS = NQ == 1 ? 2 : 1;      // that have a row's sums
     const int unit = blockIdx.x / CHUNKS, at = blockIdx.x % CHUNKS * 256 + threadIdx.x, row = at % (NQ * ROWS), e = at / (NQ * ROWS) * 16;
     const int head = unit % A.n_kv, row_tile = unit / A.n_kv % A.tiles_of_rows, req = unit / A.n_kv / A.tiles_of_rows;
     const Span S = span_of(A, req);
     const int group = A.group, first_row = row_tile * (NQ * ROWS);
-    const int rows = min(S.n_tree * group - first_row, NQ * ROWS);
+    const int rows = min(S.n_tree * group - first_row, slice_rows), lines = Shape<D, NQ>::lines(slice_rows), sums = Shape<D, NQ>::slice_sums(slice_rows);
     if (row >= rows) return;
     int lo_min = 0, lo_max = 0;
     if (A.span != 0) {
@@ -835,21 +838,21 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     float4 o[4] = {};
     float top = -INFINITY, total = 0.0f;
     bool bad_values = false;
-    const float* from = scratch + (long)unit * slices * SUMS;
+    const float* from = scratch + (long)unit * slices * sums;
 #pragma unroll 2
     for (int p = 0; p < parts * STREAMS; ++p) {
-        const float* slice = from + (long)(p / STREAMS) * SUMS;
-        const int line = row + p % STREAMS * ROWS;
-        const float2 ml = *reinterpret_cast<const float2*>(slice + 2 * ROWS * D + 2 * line);
-        bad_values |= slice[2 * ROWS * (D + 2)] != 0.0f;
-        join<4>(top, total, o, ml.x, ml.y, slice + (e / 4 * (2 * ROWS) + line) * 4, 2 * ROWS * 4);
+        const float* slice = from + (long)(p / STREAMS) * sums;
+        const int line = row + p % STREAMS * slice_rows;
+        const float2 ml = *reinterpret_cast<const float2*>(slice + lines * D + 2 * line);
+        bad_values |= slice[lines * (D + 2)] != 0.0f;
+        join<4>(top, total, o, ml.x, ml.y, slice + (e / 4 * lines + line) * 4, lines * 4);
     }
     const Place place = {A.table + (long)req * A.max_pages, head, S.keys};
     write_row<D, 4>(A, S, place, first_row + row, head, e, 4, o, total, bad_values, t_first, all_tiles, lo_max);
 }
 
 // How a call is cut: row tiles of NQ x 128 rows, a part of the keys for each CTA, in clusters or (waves) in slices
-struct Cut { long pairs, parts; int tiles_of_rows, tiles; bool waves; };
+struct Cut { long pairs, parts; int tiles_of_rows, tiles, slice_rows; bool waves; };
 
 template <int D, int NQ>
 static int cut_of(const Args& A, int max_tree, int max_keys, Cut& c) {
@@ -867,7 +870,22 @@ static int cut_of(const Args& A, int max_tree, int max_keys, Cut& c) {
     c.waves = 2 * c.pairs > 148 && c.tiles > 2 * SLICE;
     c.parts = c.waves ? (c.tiles + SLICE - 1) / SLICE : 148 / c.pairs;
     if (c.parts > c.tiles) c.parts = c.tiles;
-    const long most = c.waves ? MOST_SLICES : MOST_PARTS;
+    // A slice has lines for the rows that a tile of the largest tree has, 32 by 32 as warps write them, and all slices together have 256 MB: the longest
+    // request may be one of many short ones, for which as many slices are set aside, and CTAs that find none cost time too.  (No bound, 1 GB, 256,
+    // 64 MB: 64 requests of up to 2,000 keys and one of 131,072, trees of 4, 699 MB without: 554, 554, 298, 547 us; trees of 40, 1,748 MB: 564, 410, 314,
+    // 1,782; 256 requests, trees of 4, 2,796 MB: 3,216, 1,358, 554, 1,700; 100 requests of 100 to 32,400 keys, trees of 40: 1,647, 1,645, 1,538, 1,412.)
+    const long rows = (long)max_tree * (A.n_heads / A.n_kv);
+    c.slice_rows = c.waves && rows < NQ * ROWS ? (int)(rows + 31) / 32 * 32 : NQ * ROWS;
+    long most = MOST_PARTS;
+    if (c.waves) {
+        most = MOST_SCRATCH / (c.pairs * Shape<D, NQ>::slice_sums(c.slice_rows) * 4L);
+        if (most > MOST_SLICES) most = MOST_SLICES;
+        if (most < 2) {               // (whole requests)
+            c.waves = false;
+            c.slice_rows = NQ * ROWS;
+            most = 1;
+        }
+    }
     c.parts = c.parts < 1 ? 1 : c.parts > most ? most : c.parts;
     // (Clusters that do not all run at once take twice the time: 5 requests of 20 pairs with a window 26.2 us in clusters of seven, 16.2 in six.)
     static IbClusters clusters;
@@ -879,7 +897,7 @@ template <int D, int NQ>
 static long launch(Args A, const Cut& c, void* workspace, bool ask, cudaStream_t stream) {
     const long pairs = c.pairs, parts = c.parts;
     A.tiles_of_rows = c.tiles_of_rows;
-    const long needed = c.waves && parts > 1 ? pairs * parts * Shape<D, NQ>::SLICE_SUMS * 4 : 0;
+    const long needed = c.waves ? pairs * parts * Shape<D, NQ>::slice_sums(c.slice_rows) * 4 : 0;
     if (ask) return needed;
     float* scratch = needed ? static_cast<float*>(workspace) : nullptr;
     if (needed && workspace == nullptr) return IB_ERR_ARGUMENT;
@@ -899,11 +917,11 @@ static long launch(Args A, const Cut& c, void* workspace, bool ask, cudaStream_t
     }
     const int ranked = A.n_requests > 1 && A.n_requests <= RANKED && pairs * parts > 148;
     const int code = launch_cluster(tree_kernel<D, NQ>, pairs * parts, scratch ? 1 : (int)parts, THREADS, Shape<D, NQ>::SMEM, stream, map_k, map_v, A,
-                                    (int)parts, ranked, box, scratch);
+                                    (int)parts, ranked, box, scratch, c.slice_rows);
     if (code != IB_OK || scratch == nullptr) return code;
     const long blocks = pairs * (NQ * ROWS * (D / 16) / 256);
     if (blocks > 0x7fffffffL) return IB_ERR_UNSUPPORTED;
-    tree_join_kernel<D, NQ><<<(unsigned)blocks, 256, 0, stream>>>(A, (int)parts, scratch);
+    tree_join_kernel<D, NQ><<<(unsigned)blocks, 256, 0, stream>>>(A, (int)parts, c.slice_rows, scratch);
     return ib_launch_status();
 }
 
