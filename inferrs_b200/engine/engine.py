@@ -53,6 +53,8 @@ class Engine:
                          sure or is no replayed graph, the tokens are read first.
     """
 
+    _ended_aside: Sequence[Request] = ()     # requests that ended outside of a step: the next one returns them
+
     def __init__(self, model_dir: Optional[str] = None, dtype: str = "bf16", block_size: int = 16,
                  num_blocks: Optional[int] = None, paged_attention: float = 0.9, max_batch_size: int = 32,
                  max_tokens_per_step: int = 2048, max_seq_len: int = 0, prefill_chunk: Optional[int] = None,
@@ -119,7 +121,7 @@ class Engine:
         return self.scheduler.abort(rid)
 
     def has_work(self) -> bool:
-        return not self.scheduler.idle or self._in_flight is not None
+        return not self.scheduler.idle or self._in_flight is not None or bool(self._ended_aside)
 
     def warm_up(self, batch_sizes: Optional[Sequence[int]] = None) -> List[int]:
         """Capture the decode graphs for the given numbers of requests (all, if none is given) before the
@@ -199,7 +201,9 @@ class Engine:
 
     def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenLogProbs]]:
         """For every prompt the log probabilities that the model gives to its tokens from the second one on, each behind those
-        before it, with the ``top`` likeliest tokens at its place.  Needs a free slot and pages for one prompt at a time."""
+        before it, with the ``top`` likeliest tokens at its place.  Needs a free slot and pages for one prompt at a time.  Raises
+        KernelFault where a kernel reported that it left rows unwritten; live requests then end with reason "error" like behind a step of
+        theirs (the next :meth:`step` returns them)."""
         if not 0 <= top <= MOST_LOGPROBS:
             raise ValueError(f"top must be within 0 and {MOST_LOGPROBS}, got {top}")
         out, portion = [], self.scheduler.max_tokens_per_step
@@ -218,7 +222,16 @@ class Engine:
             finally:
                 self.runner.release(rid)
             out.append(found)
+        self._look_behind_scores()
         return out
+
+    def _look_behind_scores(self):
+        known = len(self.kernel_errors)
+        if self.health is not None and self.health.pending:      # (asked for before the last of the scores' kernels came: it does not say all)
+            self._ended_aside = [*self._ended_aside, *self._look_at_kernels(wait=True)]
+        self._ended_aside = [*self._ended_aside, *self._look_at_kernels(wait=True)]
+        if len(self.kernel_errors) > known:
+            raise KernelFault(f"a kernel reported an error while prompts were scored: {self.kernel_errors[-1]}")
 
     def _finish(self, step) -> List[Request]:
         """Read a launched step's tokens and record them; returns the requests that ended with it."""
@@ -305,7 +318,8 @@ class Engine:
         A request may end with reason "error": a kernel reported that it left rows unwritten (``stats()`` says
         which); a request that a call before returned as finished is marked so too if it ended since the last
         look that found nothing."""
-        failed = self._look_at_kernels()
+        failed = [*self._ended_aside, *self._look_at_kernels()]
+        self._ended_aside = ()
         if failed:
             return failed
         finished = self._step()
