@@ -222,16 +222,11 @@ class Engine:
             finally:
                 self.runner.release(rid)
             out.append(found)
-        self._look_behind_scores()
-        return out
-
-    def _look_behind_scores(self):
         known = len(self.kernel_errors)
-        if self.health is not None and self.health.pending:      # (asked for before the last of the scores' kernels came: it does not say all)
-            self._ended_aside = [*self._ended_aside, *self._look_at_kernels(wait=True)]
-        self._ended_aside = [*self._ended_aside, *self._look_at_kernels(wait=True)]
+        self._ended_aside = [*self._ended_aside, *self._look_behind_all()]
         if len(self.kernel_errors) > known:
             raise KernelFault(f"a kernel reported an error while prompts were scored: {self.kernel_errors[-1]}")
+        return out
 
     def _finish(self, step) -> List[Request]:
         """Read a launched step's tokens and record them; returns the requests that ended with it."""
@@ -301,6 +296,12 @@ class Engine:
             r.finish_reason = "error"
         self._unchecked, self._checked_up_to = [], 0
         return failed
+
+    def _look_behind_all(self) -> List[Request]:
+        """A look that says all of what was launched so far: one that is on its way already was asked for before the last of it."""
+        h = getattr(self, "health", None)
+        earlier = self._look_at_kernels(wait=True) if h is not None and h.pending else []
+        return earlier + self._look_at_kernels(wait=True)
 
     def _ask_about_kernels(self, ended: Sequence[Request]):
         h = getattr(self, "health", None)
@@ -378,7 +379,7 @@ class Engine:
         while len(done) < len(rids) and self.has_work():
             for r in self.step():
                 done[r.rid] = r
-        for r in self._look_at_kernels(wait=True):      # the device is idle now: this look costs nothing
+        for r in self._look_behind_all():      # the device is idle now: this look costs nothing
             done[r.rid] = r
         out = [done[r] for r in rids]
         if return_requests:

@@ -75,3 +75,21 @@ def test_scores_beside_live_requests_change_nothing(overlap):
     for i in range(3):
         assert (done[i].output, done[i].finish_reason) == plain_generate(prompts[i], params[i], ())
     manager.check_invariants()
+
+
+def test_generation_looks_behind_its_last_step():
+    """A look that was on its way before the last step says nothing of that step: the one at the end is asked for behind it."""
+    eng, _ = engine(False, fail_at=2)
+    eng.health.every = 1
+    asked = []
+    queue = eng.health.queue
+
+    def queued():
+        asked.append(eng.n_steps)
+        queue()
+
+    eng.health.queue = queued
+    eng.health.poll = lambda wait=False, poll=eng.health.poll: poll(wait) if wait else None      # (the first answer never comes by itself)
+    with pytest.raises(KernelFault):
+        eng.generate([[1, 2, 3]], SamplingParams(temperature=0.0, max_tokens=6))
+    assert asked == [1, eng.n_steps]
