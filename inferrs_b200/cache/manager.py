@@ -80,7 +80,7 @@ def host_library():
             "ibh_cache_n_free_slots": [p], "ibh_cache_n_free_pages": [p, i], "ibh_cache_slot": [p, l],
             "ibh_cache_n_tokens": [p, l], "ibh_cache_block_table": [p, l, i, p, i],
             "ibh_cache_pages_needed": [p, l, i, p], "ibh_cache_can_reserve": [p, i, p, p],
-            "ibh_cache_reserve": [p, i, p, p], "ibh_cache_commit": [p, l, i], "ibh_cache_release": [p, l],
+            "ibh_cache_reserve": [p, i, p, p], "ibh_cache_commit": [p, l, i], "ibh_cache_trim": [p, l, i], "ibh_cache_release": [p, l],
             "ibh_cache_check": [p, ctypes.c_char_p, i],
             "ibh_cache_fit_in_order": [p, i, p, p, p],
             "ibh_describe_decode": [p, i, p, p, i, p, i, i, p, i, p],
@@ -274,6 +274,12 @@ class CacheManager:
             raise CacheError(f"request {rid!r}: commit of {n_new} tokens beyond those reserved")
         if code != 0:
             raise CacheError(f"commit: the native cache manager answered {code}")
+
+    def trim(self, rid: Hashable, n_new: int = 0):
+        """The request will bring ``n_new`` more tokens at most: pages that were taken for others are free again."""
+        code = self._lib.ibh_cache_trim(self._h, self._handle(rid), int(n_new))
+        if code != 0:
+            raise CacheError(f"trim: the native cache manager answered {code}")
 
     def release(self, rid: Hashable):
         """The request is over: all its pages and its slot are free again."""

@@ -170,6 +170,22 @@ struct Cache {
         return OK;
     }
 
+    // The request will bring n_new more tokens at most: the pages behind them are free again.
+    int trim(int64_t rid, int n_new) {
+        Request* r = get(rid);
+        if (r == nullptr) return ERR_UNKNOWN_REQUEST;
+        if (n_new < 0) return ERR_BAD_COUNT;
+        const size_t keep = (size_t)pages_for(r->n_tokens + n_new);
+        for (size_t g = 0; g < pools.size(); ++g) {
+            std::vector<int>& t = r->tables[g];
+            for (size_t i = keep; i < t.size(); ++i)
+                if (t[i] != RELEASED && !pools[g].give_back(t[i])) return ERR_DOUBLE_FREE;
+            if (t.size() > keep) t.resize(keep);
+        }
+        r->n_reserved = std::min(r->n_reserved, r->n_tokens + n_new);
+        return OK;
+    }
+
     int release(int64_t rid) {
         auto it = requests.find(rid);
         if (it == requests.end()) return ERR_UNKNOWN_REQUEST;
@@ -319,6 +335,7 @@ IBH_EXPORT int ibh_cache_reserve(void* h, int n, const int64_t* rids, const int*
 }
 
 IBH_EXPORT int ibh_cache_commit(void* h, int64_t rid, int n_new) { return static_cast<Cache*>(h)->commit(rid, n_new); }
+IBH_EXPORT int ibh_cache_trim(void* h, int64_t rid, int n_new) { return static_cast<Cache*>(h)->trim(rid, n_new); }
 IBH_EXPORT int ibh_cache_release(void* h, int64_t rid) { return static_cast<Cache*>(h)->release(rid); }
 
 IBH_EXPORT int ibh_cache_check(void* h, char* msg, int cap) {

@@ -176,6 +176,14 @@ class ModelRunner:
         return done
 
     # ---- the step -----------------------------------------------------------
+    def _reserve(self, wants: Mapping[Hashable, int]):
+        """Take the pages for a step, all or nothing.  The step writes over drafted tokens that nobody kept, and gives back what only they
+        needed: a replayed step's block tables have room for the tokens that a request holds, and no more."""
+        self.manager.reserve(wants)
+        for rid in [r for r in self._drafted if r in wants]:
+            self.manager.trim(rid, wants[rid])
+            del self._drafted[rid]
+
     def prepare(self, entries: Sequence[StepEntry], fixed_pages: Optional[Sequence[int]] = None) -> StepContext:
         """Reserve pages for all entries (all or nothing: OutOfPages leaves the cache untouched) and
         build the step's description."""
@@ -184,14 +192,13 @@ class ModelRunner:
             if e.rid in wants:
                 raise ValueError(f"request {e.rid!r} appears twice in one step")
             wants[e.rid] = len(e.tokens)
-        self.manager.reserve(wants)
+        self._reserve(wants)
         return build_context(entries, self.manager, self.storage, self.spec.vocab_size, self.spec.max_positions,
                              self.rt.device, fixed_pages)
 
     def commit(self, entries: Sequence[StepEntry]):
         for e in entries:
             self.manager.commit(e.rid, len(e.tokens))
-            self._drafted.pop(e.rid, None)       # (the step has written over drafted tokens that nobody kept)
         self.steps_run += 1
 
     # ---- drafted tokens -------------------------------------------------------------------
@@ -210,7 +217,15 @@ class ModelRunner:
         if len(wants) != len(entries):
             raise ValueError("a request appears twice in one step")
         self.manager.reserve(wants)
-        ctx = build_drafts(entries, self.manager, self.storage, self.spec.vocab_size, self.spec.max_positions, self.rt.device)
+        try:
+            ctx = build_drafts(entries, self.manager, self.storage, self.spec.vocab_size, self.spec.max_positions, self.rt.device)
+        except Exception:
+            for rid in wants:                 # as it was: with the pages of earlier drafts that may still be kept
+                self.manager.trim(rid, len(self._drafted.get(rid, ())))
+            raise
+        for rid, n in wants.items():
+            self.manager.trim(rid, n)
+            self._drafted.pop(rid, None)
         logits = self.model.forward(ctx)
         self._drafted.update((e.rid, [int(p) for p in e.parents]) for e in entries)
         self.steps_run += 1
@@ -243,6 +258,7 @@ class ModelRunner:
         for rid, places in kept.items():
             if len(places):
                 self.manager.commit(rid, len(places))
+            self.manager.trim(rid)
             del self._drafted[rid]
 
     def _decode_graph_takes(self, entries: Sequence[StepEntry]) -> bool:
@@ -275,7 +291,7 @@ class ModelRunner:
             wants = {e.rid: 1 for e in entries}
             if len(wants) != len(entries):
                 raise ValueError("a request appears twice in one step")
-            self.manager.reserve(wants)
+            self._reserve(wants)
             logits = self.graphs.run(entries, carry)
             if own_output:
                 logits = logits.clone()
@@ -283,7 +299,7 @@ class ModelRunner:
             wants = {e.rid: len(e.tokens) for e in entries}
             if len(wants) != len(entries):
                 raise ValueError("a request appears twice in one step")
-            self.manager.reserve(wants)
+            self._reserve(wants)
             logits = self.portion_graphs.run(entries, carry)
             if own_output:
                 logits = logits.clone()

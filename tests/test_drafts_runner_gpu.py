@@ -1,0 +1,40 @@
+"""Drafted tokens and forks beside replayed steps."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helpers import CONFIG_A, PAGE_SIZE, random_tokens, rel_err
+from inferrs_b200.engine.batch import DraftEntry, StepEntry
+from inferrs_b200.engine.loading import load_model_dir
+from inferrs_b200.engine.runner import ModelRunner
+from inferrs_b200.runtime import Runtime
+from test_drafts_engine_gpu import TOL, plain_logits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keep", [True, False])
+def test_replayed_steps_behind_a_tree_that_reached_beyond_their_tables(model_dirs, dtype, keep):
+    """The block tables of replayed steps end with the longest context that the runner was told; a tree may be wider than what is left of it."""
+    page, vocab = PAGE_SIZE["A"], CONFIG_A["vocab_size"]
+    rt = Runtime.cuda(dtype)
+    spec, weights, _ = load_model_dir(model_dirs["A"], rt)
+    runner = ModelRunner(spec, weights, rt, page_size=page, n_pages=32, max_requests=2, max_context=3 * page)
+    assert runner.graphs is not None and runner.graphs.fixed_pages == [3]
+    prompt = random_tokens(3 * page - 3, vocab, seed=1)
+    runner.admit(0)
+    runner.step([StepEntry(0, prompt, [])])
+    drafts = random_tokens(2 * page, vocab, seed=2)
+    logits = runner.step_drafts([DraftEntry(0, drafts, [-1] + [0] * (2 * page - 1))])
+    assert rel_err(logits[-1].cpu(), plain_logits(model_dirs["A"], prompt + [drafts[0], drafts[-1]], dtype)[-1]) < TOL[dtype]
+    tokens = list(prompt)
+    if keep:
+        runner.keep_drafts({0: [0]})
+        tokens.append(drafts[0])
+    for token in (3, 4):
+        tokens.append(token)
+        got = runner.step([StepEntry(0, [token], [0])])
+        assert rel_err(got[0].cpu(), plain_logits(model_dirs["A"], tokens, dtype)[-1]) < TOL[dtype]
+    assert runner.graphs.captured and runner.n_tokens(0) == len(tokens)
