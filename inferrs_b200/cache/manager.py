@@ -80,7 +80,7 @@ def host_library():
             "ibh_cache_n_free_slots": [p], "ibh_cache_n_free_pages": [p, i], "ibh_cache_slot": [p, l],
             "ibh_cache_n_tokens": [p, l], "ibh_cache_block_table": [p, l, i, p, i],
             "ibh_cache_pages_needed": [p, l, i, p], "ibh_cache_can_reserve": [p, i, p, p],
-            "ibh_cache_reserve": [p, i, p, p], "ibh_cache_commit": [p, l, i], "ibh_cache_trim": [p, l, i], "ibh_cache_release": [p, l],
+            "ibh_cache_reserve": [p, i, p, p], "ibh_cache_commit": [p, l, i], "ibh_cache_trim": [p, l, i], "ibh_cache_fork": [p, l, l], "ibh_cache_release": [p, l],
             "ibh_cache_check": [p, ctypes.c_char_p, i],
             "ibh_cache_fit_in_order": [p, i, p, p, p],
             "ibh_describe_decode": [p, i, p, p, i, p, i, i, p, i, p],
@@ -203,6 +203,24 @@ class CacheManager:
             raise CacheError(f"request {rid!r}: the native cache manager answered {slot}")
         self._next_handle += 1
         self._handles[rid] = handle
+        return slot
+
+    def fork(self, rid: Hashable, new_rid: Hashable) -> int:
+        """Make ``new_rid`` a live request of as many tokens as ``rid``, with pages of its own at the places where ``rid`` has them; returns its
+        slot.  What the pages and the slot hold is the caller's to copy.  OutOfPages changes nothing."""
+        if new_rid in self._handles:
+            raise CacheError(f"request {new_rid!r} is already live")
+        handle = self._next_handle
+        slot = self._lib.ibh_cache_fork(self._h, self._handle(rid), handle)
+        if slot == _ERR_NO_SLOT:
+            raise OutOfPages(f"no free state slot ({self.max_requests} requests are live)")
+        if slot == _ERR_OUT_OF_PAGES:
+            held = [sum(p != RELEASED for p in self.block_table(rid, g)) for g in range(len(self.groups))]
+            raise OutOfPages(f"pages held per group {held}, free {[p.n_free for p in self.pools]}")
+        if slot < 0:
+            raise CacheError(f"fork: the native cache manager answered {slot}")
+        self._next_handle += 1
+        self._handles[new_rid] = handle
         return slot
 
     def slot(self, rid: Hashable) -> int:

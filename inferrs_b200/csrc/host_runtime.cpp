@@ -170,6 +170,28 @@ struct Cache {
         return OK;
     }
 
+    // Request `to` gets a state slot (returned, >= 0) and a page of its own for every page that holds tokens of `from`; where a window has passed
+    // a page of one, there is none of the other.  Nothing is taken where pages or slots are short.
+    int fork(int64_t from, int64_t to) {
+        const Request* r = get(from);
+        if (r == nullptr) return ERR_UNKNOWN_REQUEST;
+        if (requests.count(to)) return ERR_ALREADY_LIVE;
+        if (free_slots.empty()) return ERR_NO_SLOT;
+        const size_t pages = (size_t)pages_for(r->n_tokens);
+        for (size_t g = 0; g < pools.size(); ++g) {
+            const auto end = r->tables[g].begin() + pages;
+            if (pages - std::count(r->tables[g].begin(), end, RELEASED) > (size_t)pools[g].n_free()) return ERR_OUT_OF_PAGES;
+        }
+        const int slot = admit(to);
+        r = get(from);                    // (the map may have moved)
+        Request* t = get(to);
+        for (size_t g = 0; g < pools.size(); ++g)
+            for (size_t i = 0; i < pages; ++i)
+                t->tables[g].push_back(r->tables[g][i] == RELEASED ? RELEASED : pools[g].take());
+        t->n_tokens = t->n_reserved = r->n_tokens;
+        return slot;
+    }
+
     // The request will bring n_new more tokens at most: the pages behind them are free again.
     int trim(int64_t rid, int n_new) {
         Request* r = get(rid);
@@ -335,6 +357,7 @@ IBH_EXPORT int ibh_cache_reserve(void* h, int n, const int64_t* rids, const int*
 }
 
 IBH_EXPORT int ibh_cache_commit(void* h, int64_t rid, int n_new) { return static_cast<Cache*>(h)->commit(rid, n_new); }
+IBH_EXPORT int ibh_cache_fork(void* h, int64_t from, int64_t to) { return static_cast<Cache*>(h)->fork(from, to); }
 IBH_EXPORT int ibh_cache_trim(void* h, int64_t rid, int n_new) { return static_cast<Cache*>(h)->trim(rid, n_new); }
 IBH_EXPORT int ibh_cache_release(void* h, int64_t rid) { return static_cast<Cache*>(h)->release(rid); }
 

@@ -16,7 +16,7 @@ from typing import Dict, Hashable, List, Mapping, Optional, Sequence
 
 import torch
 
-from ..cache.manager import CacheManager, OutOfPages
+from ..cache.manager import CacheManager
 from ..cache.storage import CacheStorage, bytes_of_vectors
 from ..parts.spec import ModelSpec
 from ..runtime import Runtime
@@ -96,24 +96,17 @@ class ModelRunner:
     def fork(self, rid: Hashable, new_rid: Hashable) -> int:
         """A new live request that holds what ``rid`` holds: its pages (copied, in all layers) and its fixed-size states.  Returns the
         new request's slot; raises OutOfPages, and leaves everything as it was, where there is no room."""
-        n, slot = self.manager.n_tokens(rid), self.manager.slot(rid)
-        new_slot = self.manager.admit(new_rid)
+        new_slot = self.manager.fork(rid, new_rid)
         try:
-            done = 0
-            while done < n:              # in portions, so that pages behind a window come back before the next ones are taken
-                k = min(n - done, 64 * self.page_size)
-                self.manager.reserve({new_rid: k})
-                self.manager.commit(new_rid, k)
-                done += k
-        except OutOfPages:
+            for g in range(len(self.manager.groups)):
+                pairs = [(a, b) for a, b in zip(self.manager.block_table(rid, g), self.manager.block_table(new_rid, g)) if a >= 0]
+                if pairs and self.storage.members[g]:
+                    both = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.rt.device)
+                    self.storage.copy_pages(g, both[0], both[1])
+            self.storage.copy_slot(self.manager.slot(rid), new_slot)
+        except Exception:
             self.manager.release(new_rid)
             raise
-        for g in range(len(self.manager.groups)):
-            pairs = [(a, b) for a, b in zip(self.manager.block_table(rid, g), self.manager.block_table(new_rid, g)) if a >= 0 and b >= 0]
-            if pairs and self.storage.members[g]:
-                both = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.rt.device)
-                self.storage.copy_pages(g, both[0], both[1])
-        self.storage.copy_slot(slot, new_slot)
         return new_slot
 
     def has(self, rid: Hashable) -> bool:

@@ -142,3 +142,76 @@ def test_a_step_without_room_leaves_drafts_that_can_be_kept(model_dirs, monkeypa
     runner.keep_drafts({0: [0, page - 1]})
     assert runner.n_tokens(0) == page + 2
     runner.manager.check_invariants()
+
+
+# ---- forks --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seed", range(8))
+def test_the_book_of_a_fork(seed):
+    """A fork has as many tokens, its own pages where the other one has pages, and none where a window has passed; it needs no room beyond that."""
+    rng = random.Random(100 + seed)
+    page = rng.choice([1, 4, 16])
+    window, keep = rng.choice([1, 7, 40]), rng.choice([0, 5])
+    m = CacheManager([GroupLayout("full"), GroupLayout("window", window=window, keep_first=keep)], page, [400, 400], 3)
+    m.admit("a")
+    n = 0
+    for _ in range(rng.randrange(0, 40)):
+        k = rng.randrange(1, 9)
+        m.reserve({"a": k})
+        m.commit("a", k)
+        n += k
+    m.reserve({"a": 30})                  # (taken for a step that has not been)
+    m.fork("a", "b")
+    assert m.n_tokens("b") == n and m.slot("b") != m.slot("a")
+    for g in range(2):
+        a, b = m.block_table("a", g), m.block_table("b", g)
+        assert len(b) == -(-n // page) and [x < 0 for x in b] == [x < 0 for x in a[:len(b)]]
+        assert not set(x for x in b if x >= 0) & set(a)
+    m.check_invariants()
+    with pytest.raises(CacheError):
+        m.fork("a", "b")
+    with pytest.raises(CacheError):
+        m.fork("nobody", "c")
+    assert not m.has("c")
+    if all(p.n_free >= sum(x >= 0 for x in m.block_table("b", g)) for g, p in enumerate(m.pools)):
+        m.fork("b", "c")
+    else:
+        with pytest.raises(OutOfPages):
+            m.fork("b", "c")
+        m.admit("c")
+    with pytest.raises(OutOfPages):       # no slot
+        m.fork("a", "d")
+    for rid in "abc":
+        m.release(rid)
+    assert [p.n_free for p in m.pools] == [400, 400] and m.n_free_slots == 3
+    m.check_invariants()
+
+
+def test_a_fork_behind_a_window_needs_the_window_alone():
+    """A long request whose layers all have a window holds few pages: a pool with exactly as many left takes its fork."""
+    page, window = 4, 16
+    m = CacheManager([GroupLayout("window", window=window)], page, [12], 2)
+    m.admit("a")
+    for _ in range(500):
+        m.reserve({"a": 1})
+        m.commit("a", 1)
+    held = sum(p >= 0 for p in m.block_table("a", 0))
+    assert held <= 6 and len(m.block_table("a", 0)) == 125
+    m.fork("a", "b")
+    assert m.pools[0].n_free == 12 - 2 * held
+    m.release("b")
+    m.admit("c")
+    m.reserve({"c": page * (12 - 2 * held + 1)})
+    m.release("a")
+    m.check_invariants()
+
+
+def test_a_fork_that_has_no_room_changes_nothing():
+    m = CacheManager([GroupLayout("full"), GroupLayout("window", window=8)], 4, [10, 10], 3)
+    m.admit("a")
+    m.reserve({"a": 24})
+    m.commit("a", 24)
+    free = [p.n_free for p in m.pools]
+    with pytest.raises(OutOfPages):
+        m.fork("a", "b")
+    assert not m.has("b") and [p.n_free for p in m.pools] == free and m.n_free_slots == 2
+    m.check_invariants()
