@@ -147,7 +147,8 @@ def tree_masks(trees: Sequence[Sequence[int]], words: Optional[int] = None):
 
 def build_drafts(entries: Sequence[DraftEntry], manager: CacheManager, storage: CacheStorage, vocab_size: int, max_positions: int,
                  device: torch.device) -> StepContext:
-    """The step of the entries' drafted tokens, all of whose logits are wanted.  Pages must already be reserved."""
+    """The step of the entries' drafted tokens, all of whose logits are wanted.  Pages must already be reserved.  A tree is as long as it is deep:
+    its tokens may be more than the model has positions left."""
     for e in entries:
         if len(e.parents) != len(e.tokens):
             raise BatchError(f"request {e.rid!r}: {len(e.parents)} parents for {len(e.tokens)} drafted tokens")
@@ -157,7 +158,14 @@ def build_drafts(entries: Sequence[DraftEntry], manager: CacheManager, storage: 
         if need.window is not None and reach > need.window:
             raise BatchError(f"drafted tokens {reach} deep do not fit a window of {need.window}")
     context = [manager.n_tokens(e.rid) for e in entries]
-    ctx = build_context([StepEntry(e.rid, e.tokens, range(len(e.tokens))) for e in entries], manager, storage, vocab_size, max_positions, device)
+    at = 0
+    for e, held in zip(entries, context):
+        deep = 1 + max((int(d) for d in depths[at:at + len(e.tokens)]), default=-1)
+        if held + deep > max_positions:
+            raise BatchError(f"request {e.rid!r}: {held} tokens and drafted ones {deep} deep exceed the model's {max_positions} positions")
+        at += len(e.tokens)
+    ctx = build_context([StepEntry(e.rid, e.tokens, range(len(e.tokens))) for e in entries], manager, storage, vocab_size,
+                        max_positions + len(masks), device)       # (places in the cache, which ends with the block tables)
     places = ctx.positions.clone()
     positions = np.repeat(np.asarray(context, dtype=np.int32), [len(e.tokens) for e in entries]) + depths
     ctx.positions.copy_(torch.from_numpy(positions.astype(np.int32)))

@@ -215,3 +215,40 @@ def test_a_fork_that_has_no_room_changes_nothing():
         m.fork("a", "b")
     assert not m.has("b") and [p.n_free for p in m.pools] == free and m.n_free_slots == 2
     m.check_invariants()
+
+
+# ---- the end of a model's positions -------------------------------------------------------------------------------------
+def test_a_wide_tree_at_the_end_of_the_positions(model_dirs, monkeypatch):
+    """Two positions are left and nine tokens are drafted, none deeper than the second one; a third level is refused."""
+    drafts_refs.install(monkeypatch)
+    page, vocab, most = PAGE_SIZE["A"], CONFIG_A["vocab_size"], CONFIG_A["max_position_embeddings"]
+    runner = make_runner(model_dirs["A"], page, n_pages=2 * most // page, max_requests=2)
+    prompt = random_tokens(most - 2, vocab, seed=7)
+    runner.admit(0)
+    runner.step([StepEntry(0, prompt, [])])
+    runner.admit(1)
+    runner.step([StepEntry(1, [1, 2, 3], [])])
+    tree = [-1, 0, 0, 0, -1, 4, 4, -1, 7]
+    drafts = random_tokens(len(tree), vocab, seed=8)
+    logits = runner.step_drafts([DraftEntry(1, [4] * 6, [-1, 0, 1, 2, 3, 4]), DraftEntry(0, drafts, tree)])
+    for i in (3, 6, 8):
+        assert rel_err(logits[6 + i], last_logits(model_dirs["A"], prompt + [drafts[tree[i]], drafts[i]])) < 1e-4
+    runner.keep_drafts({0: [4, 6], 1: []})
+    assert runner.n_tokens(0) == most
+    with pytest.raises(BatchError, match="positions"):
+        runner.step_drafts([DraftEntry(0, [1], [-1])])
+    assert pages_held(runner, 0) == [most // page]
+    runner.manager.check_invariants()
+
+
+def test_a_tree_that_is_too_deep_is_refused(model_dirs, monkeypatch):
+    drafts_refs.install(monkeypatch)
+    page, most = PAGE_SIZE["A"], CONFIG_A["max_position_embeddings"]
+    runner = make_runner(model_dirs["A"], page, n_pages=2 * most // page, max_requests=2)
+    runner.admit(0)
+    runner.step([StepEntry(0, [1] * (most - 2), [])])
+    held = pages_held(runner, 0)
+    with pytest.raises(BatchError, match="positions"):
+        runner.step_drafts([DraftEntry(0, [1, 2, 3], [-1, 0, 1])])
+    assert pages_held(runner, 0) == held
+    runner.step_drafts([DraftEntry(0, [1, 2, 3], [-1, 0, 0])])

@@ -38,3 +38,24 @@ def test_replayed_steps_behind_a_tree_that_reached_beyond_their_tables(model_dir
         got = runner.step([StepEntry(0, [token], [0])])
         assert rel_err(got[0].cpu(), plain_logits(model_dirs["A"], tokens, dtype)[-1]) < TOL[dtype]
     assert runner.graphs.captured and runner.n_tokens(0) == len(tokens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_wide_tree_at_the_end_of_the_positions(model_dirs, dtype):
+    page, vocab, most = PAGE_SIZE["A"], CONFIG_A["vocab_size"], CONFIG_A["max_position_embeddings"]
+    rt = Runtime.cuda(dtype)
+    spec, weights, _ = load_model_dir(model_dirs["A"], rt)
+    runner = ModelRunner(spec, weights, rt, page_size=page, n_pages=most // page + 8, max_requests=2)
+    prompt = random_tokens(most - 3, vocab, seed=7)
+    runner.admit(0)
+    runner.step([StepEntry(0, prompt, [])])
+    tree = [-1] + [0] * 20
+    drafts = random_tokens(len(tree), vocab, seed=8)
+    logits = runner.step_drafts([DraftEntry(0, drafts, tree)])
+    for i in (0, 1, 20):
+        tokens = prompt + drafts[:1] + ([drafts[i]] if i else [])
+        assert rel_err(logits[i].cpu(), plain_logits(model_dirs["A"], tokens, dtype)[-1]) < TOL[dtype]
+    runner.keep_drafts({0: [0, 20]})
+    got = runner.step([StepEntry(0, [9], [0])])
+    assert rel_err(got[0].cpu(), plain_logits(model_dirs["A"], prompt + [drafts[0], drafts[20], 9], dtype)[-1]) < TOL[dtype]
+    assert runner.n_tokens(0) == most
