@@ -16,7 +16,7 @@ import torch
 from ..config.base import generation_eos_ids
 from ..runtime import Runtime, parse_dtype
 from .. import kernels
-from ..sampling.params import MOST_LOGPROBS, SamplingParams, TokenLogProbs
+from ..sampling.params import SamplingParams, TokenLogProbs, count_of_likeliest
 from ..sampling.sampler import Sampler
 from .batch import StepEntry
 from .health import KernelHealth
@@ -204,8 +204,7 @@ class Engine:
         before it, with the ``top`` likeliest tokens at its place.  Needs a free slot and pages for one prompt at a time.  Raises
         KernelFault where a kernel reported that it left rows unwritten; live requests then end with reason "error" like behind a step of
         theirs (the next :meth:`step` returns them)."""
-        if not 0 <= top <= MOST_LOGPROBS:
-            raise ValueError(f"top must be within 0 and {MOST_LOGPROBS}, got {top}")
+        top = count_of_likeliest("top", top)
         out, portion = [], self.scheduler.max_tokens_per_step
         for prompt in prompts:
             prompt = [int(t) for t in prompt]

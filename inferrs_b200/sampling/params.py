@@ -2,6 +2,7 @@
 (inferrs/src/sampler.rs:27-112)."""
 from __future__ import annotations
 
+import operator
 import sys
 from array import array
 from dataclasses import dataclass, field
@@ -11,6 +12,17 @@ GREEDY_EPS = 1e-5  # temperatures below this pick the largest logit (sampler.rs:
 
 
 MOST_LOGPROBS = 32       # likeliest tokens that can be asked for (kernels.MAX_TOP_LOG_PROBS)
+
+
+def count_of_likeliest(name: str, n) -> int:
+    """``n`` as a number of likeliest tokens, or ValueError."""
+    try:
+        n = operator.index(n)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number, got {n!r}") from None
+    if not 0 <= n <= MOST_LOGPROBS:
+        raise ValueError(f"{name} must be within 0 and {MOST_LOGPROBS}, got {n}")
+    return n
 
 
 @dataclass
@@ -53,8 +65,8 @@ class SamplingParams:
             raise ValueError(f"max_tokens must be positive, got {self.max_tokens}")
         if self.repeat_last_n < 0:
             raise ValueError(f"repeat_last_n must be >= 0, got {self.repeat_last_n}")
-        if self.logprobs is not None and not 0 <= self.logprobs <= MOST_LOGPROBS:
-            raise ValueError(f"logprobs must be within 0 and {MOST_LOGPROBS} (or None), got {self.logprobs}")
+        if self.logprobs is not None:
+            self.logprobs = count_of_likeliest("logprobs", self.logprobs)
         self.stop_token_ids = tuple(int(t) for t in self.stop_token_ids)
 
     @classmethod

@@ -93,3 +93,16 @@ def test_generation_looks_behind_its_last_step():
     with pytest.raises(KernelFault):
         eng.generate([[1, 2, 3]], SamplingParams(temperature=0.0, max_tokens=6))
     assert asked == [1, eng.n_steps]
+
+
+def test_how_many_of_the_likeliest_tokens_can_be_asked_for():
+    """A number that is none is refused where it is given, not in the middle of a step that other requests share."""
+    for good in (0, 1, 32, torch.tensor(3)):
+        assert SamplingParams(logprobs=good).logprobs == int(good) and type(SamplingParams(logprobs=good).logprobs) is int
+    assert SamplingParams().logprobs is None
+    eng, manager = engine(False)
+    for bad in (-1, 33, 2.5, 2.0, "3", [1]):
+        with pytest.raises(ValueError):
+            SamplingParams(logprobs=bad)
+        with pytest.raises(ValueError):
+            eng.score([[1, 2]], top=bad)
