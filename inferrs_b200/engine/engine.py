@@ -104,16 +104,20 @@ class Engine:
         self._last_look = 0
 
     # ---- requests -------------------------------------------------------------------
+    def _checked(self, prompt: Sequence[int]) -> List[int]:
+        prompt = [int(t) for t in prompt]
+        for t in prompt:
+            if not 0 <= t < self.spec.vocab_size:
+                raise ValueError(f"token id {t} is outside the vocabulary of {self.spec.vocab_size}")
+        return prompt
+
     def add_request(self, prompt: Sequence[int], sampling: Optional[SamplingParams] = None,
                     rid: Optional[Hashable] = None) -> Hashable:
         sampling = sampling or SamplingParams()
         if rid is None:
             rid = next(self._ids)
         seed = sampling.seed if sampling.seed is not None else self._rng.getrandbits(63)
-        prompt = [int(t) for t in prompt]
-        for t in prompt:
-            if not 0 <= t < self.spec.vocab_size:
-                raise ValueError(f"token id {t} is outside the vocabulary of {self.spec.vocab_size}")
+        prompt = self._checked(prompt)
         self.scheduler.add(Request(rid=rid, prompt=prompt, params=sampling, seed=seed))
         return rid
 
@@ -206,8 +210,8 @@ class Engine:
         theirs (the next :meth:`step` returns them)."""
         top = count_of_likeliest("top", top)
         out, portion = [], self.scheduler.max_tokens_per_step
+        prompts = [self._checked(prompt) for prompt in prompts]
         for prompt in prompts:
-            prompt = [int(t) for t in prompt]
             rid, found = ("score", next(self._ids)), []
             self.runner.admit(rid)
             try:

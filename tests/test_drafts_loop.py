@@ -106,3 +106,14 @@ def test_how_many_of_the_likeliest_tokens_can_be_asked_for():
             SamplingParams(logprobs=bad)
         with pytest.raises(ValueError):
             eng.score([[1, 2]], top=bad)
+
+
+def test_a_prompt_to_score_is_checked_before_anything_runs():
+    """Also its last token, which no step runs where the tokens ahead of it fill whole portions."""
+    eng, manager = engine(False)
+    portion = eng.scheduler.max_tokens_per_step
+    for prompt in ([1] * portion + [VOCAB], [1, VOCAB, 2], [-1, 2]):
+        with pytest.raises(ValueError):
+            eng.score([[1, 2, 3], prompt])
+    assert eng.runner.hash == {} and manager.n_live == 0
+    assert eng.score([[], [1]]) == [[], []]
