@@ -75,3 +75,12 @@ def test_trees_that_are_larger_than_the_call_says():
     for r in range(len(trees)):
         rows = slice(start[r], start[r + 1])
         assert right[rows][:9].all() and (right[rows] | (got[rows] == 7.0).flatten(1).all(1)).all()
+
+
+@pytest.mark.parametrize("requests", [63, 64, 65, 130])
+def test_requests_in_order_of_their_length_and_as_they_come(requests):
+    """The CTAs of few requests take the longest ones first, those of more take them as they come; equal lengths among both."""
+    contexts = [(i * 37) % 11 * 40 for i in range(requests)]
+    trees = [1 + i % 5 for i in range(requests)]
+    c = drafted(71, contexts, trees, 8, 4, 128, 16, BF)
+    check(c, attend(c))
