@@ -1,6 +1,7 @@
 """Drafted tokens and forks through the runner on the CPU, with plain statements in the kernels' place."""
 from __future__ import annotations
 
+import dataclasses
 import random
 
 import pytest
@@ -11,8 +12,10 @@ import plain_qwen3
 from helpers import CONFIG_A, CONFIG_B, PAGE_SIZE, random_tokens, rel_err
 from inferrs_b200.cache.manager import CacheError, CacheManager, GroupLayout, OutOfPages
 from inferrs_b200.engine.batch import BatchError, DraftEntry, StepEntry
-from inferrs_b200.engine.loading import load_model_dir
+from inferrs_b200.engine.loading import load_model_dir, spec_from_config
+from inferrs_b200.engine.model import declared_tensors
 from inferrs_b200.engine.runner import ModelRunner
+from inferrs_b200.parts.spec import ScheduleEntry
 from inferrs_b200.runtime import Runtime
 
 CONFIGS = {"A": CONFIG_A, "B": CONFIG_B}
@@ -252,3 +255,78 @@ def test_a_tree_that_is_too_deep_is_refused(model_dirs, monkeypatch):
         runner.step_drafts([DraftEntry(0, [1, 2, 3], [-1, 0, 1])])
     assert pages_held(runner, 0) == held
     runner.step_drafts([DraftEntry(0, [1, 2, 3], [-1, 0, 0])])
+
+
+# ---- windows ------------------------------------------------------------------------------------------------------------
+def windowed_runner(config, window, page, rt, seed=6):
+    """A model whose second layer has a window and whose first two layers run twice."""
+    spec, _ = spec_from_config(config)
+    layers = list(spec.layers)
+    layers[1] = layers[1].with_part("mixer", dataclasses.replace(layers[1].mixer, window=window))
+    order = [0, 1, 0, 1] + list(range(2, len(layers)))
+    spec = dataclasses.replace(spec, layers=tuple(layers), schedule=tuple(ScheduleEntry(layer=x, cache=i) for i, x in enumerate(order)))
+    g = torch.Generator().manual_seed(seed)
+    weights = {d.name: (1.0 + 0.1 * torch.randn(d.shape, generator=g) if len(d.shape) == 1 else
+                        torch.randn(d.shape, generator=g) * d.shape[-1] ** -0.5).to(rt.dtype).to(rt.device) for d in declared_tensors(spec)}
+    return ModelRunner(spec, weights, rt, page_size=page, n_pages=96, max_requests=4)
+
+
+def check_windows(make, window, page, bound, n_prompt=70):
+    """Trees behind contexts that windows have passed: every drafted token's logits are those of its path one token after another, the kept path
+    goes on, and so does a fork behind it; a tree deeper than a window is refused."""
+    runner, plain = make(), make()
+    vocab = runner.spec.vocab_size
+    assert runner.takes_drafts() and sorted(x.window or 0 for x in runner.storage.layouts) == [0, window]
+    prompts = [random_tokens(n, vocab, seed=n) for n in (n_prompt, 3)]
+    trees = [[-1, 0, 0, 1, -1, 4, 3, 6][:window + 4], [-1, 0, 1]]
+    drafts = [random_tokens(len(t), vocab, seed=20 + i) for i, t in enumerate(trees)]
+    for i, p in enumerate(prompts):
+        runner.admit(i)
+        runner.step([StepEntry(i, p, [])])
+    if window <= 40:
+        assert any(x < 0 for g, layout in enumerate(runner.storage.layouts) if layout.window for x in runner.manager.block_table(0, g))
+
+    def one_by_one(tokens, n_wanted):
+        plain.admit("p")
+        plain.step([StepEntry("p", tokens[:-n_wanted], [])])
+        rows = [plain.step([StepEntry("p", [t], [0])]).clone() for t in tokens[-n_wanted:]]
+        plain.release("p")
+        return torch.cat(rows)
+
+    def path(tree, j):
+        return (path(tree, tree[j]) if tree[j] >= 0 else []) + [j]
+
+    logits = runner.step_drafts([DraftEntry(i, d, t) for i, (d, t) in enumerate(zip(drafts, trees))])
+    at = 0
+    for i, tree in enumerate(trees):
+        for j in range(len(tree)):
+            way = path(tree, j)
+            want = one_by_one(prompts[i] + [drafts[i][k] for k in way], len(way))
+            assert rel_err(logits[at + j].cpu(), want[-1].cpu()) < bound, (i, j)
+        at += len(tree)
+    runner.keep_drafts({0: path(trees[0], 6), 1: [0]})
+    runner.fork(0, 2)
+    held = {0: prompts[0] + [drafts[0][k] for k in path(trees[0], 6)], 1: prompts[1] + drafts[1][:1]}
+    held[2] = list(held[0])
+    chain = {0: [5, 6, 7], 1: [8, 9], 2: [1, 2, 3, 4]}
+    got = runner.step_drafts([DraftEntry(r, c, list(range(-1, len(c) - 1))) for r, c in chain.items()])
+    at = 0
+    for r, c in chain.items():
+        want = one_by_one(held[r] + c, len(c))
+        assert rel_err(got[at:at + len(c)].cpu(), want.cpu()) < bound, r
+        at += len(c)
+    runner.keep_drafts({r: list(range(len(c))) for r, c in chain.items()})
+    for r, c in chain.items():
+        got = runner.step([StepEntry(r, [7], [0])])
+        assert rel_err(got[0].cpu(), one_by_one(held[r] + c + [7], 1)[0].cpu()) < bound, r
+    with pytest.raises(BatchError, match="window"):
+        runner.step_drafts([DraftEntry(0, [1] * (window + 1), list(range(-1, window)))])
+    runner.step_drafts([DraftEntry(0, [1] * window, list(range(-1, window - 1)))])
+    runner.manager.check_invariants()
+
+
+@pytest.mark.parametrize("window,page", [(24, 4), (17, 16), (5, 4)])
+def test_trees_through_layers_with_windows(monkeypatch, window, page):
+    drafts_refs.install(monkeypatch)
+    rt = Runtime(torch.device("cpu"), torch.float32)
+    check_windows(lambda: windowed_runner(CONFIG_A, window, page, rt), window, page, 1e-4)

@@ -4,12 +4,14 @@ from __future__ import annotations
 import pytest
 import torch
 
-from helpers import CONFIG_A, PAGE_SIZE, random_tokens, rel_err
+from helpers import CONFIG_A, CONFIG_B, CONFIG_C, CONFIG_D, PAGE_SIZE, random_tokens, rel_err
+from inferrs_b200 import kernels
 from inferrs_b200.engine.batch import DraftEntry, StepEntry
 from inferrs_b200.engine.loading import load_model_dir
 from inferrs_b200.engine.runner import ModelRunner
 from inferrs_b200.runtime import Runtime
 from test_drafts_engine_gpu import TOL, plain_logits
+from test_drafts_runner import check_windows, windowed_runner
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +61,11 @@ def test_a_wide_tree_at_the_end_of_the_positions(model_dirs, dtype):
     got = runner.step([StepEntry(0, [9], [0])])
     assert rel_err(got[0].cpu(), plain_logits(model_dirs["A"], prompt + [drafts[0], drafts[20], 9], dtype)[-1]) < TOL[dtype]
     assert runner.n_tokens(0) == most
+
+
+@pytest.mark.parametrize("config,window,n_prompt", [(CONFIG_B, 24, 70), (CONFIG_C, 17, 90), (CONFIG_D, 24, 70), (CONFIG_D, 130, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_trees_through_layers_with_windows(config, window, n_prompt, dtype):
+    rt = Runtime.cuda(dtype)
+    check_windows(lambda: windowed_runner(config, window, 16, rt), window, 16, TOL[dtype], n_prompt)
+    assert kernels.attention_tree_error() == 0
