@@ -640,6 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 const bool move = top > m + STEP || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
                     const float c = move ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
+                    __syncwarp();
                     if (i > 0) {      // (the stream's products are done: the one that gave S came behind them)
 #pragma unroll 1
                         for (int e = 0; e < D; e += 32) {
@@ -677,6 +678,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[g][h]));
+                    __syncwarp();
                 };
                 hand_over(0);
                 tmem_ld64(s_at + 64, x);
@@ -701,6 +703,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 #pragma unroll 1
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
+                    __syncwarp();      // rows of no token skip the stores
                     tmem_ld32(o_at + e, x);
                     if (!ok || !mine) continue;
                     unsigned y[16];
@@ -742,6 +745,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 #pragma unroll 1
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
+                    __syncwarp();
                     tmem_ld32(o_at + e, x);
                     if (!mine) continue;
 #pragma unroll

@@ -79,6 +79,7 @@ __device__ __forceinline__ unsigned cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();      // (the threads of a warp arrive as one)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {

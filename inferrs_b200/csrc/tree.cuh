@@ -63,6 +63,7 @@ __device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
     return v;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();      // (the threads of a warp arrive as one)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
