@@ -213,11 +213,11 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
             if (number(i) < d) sq[row * dp + number(i)] = acc[r][i];
         if (lane == 0) { sml[row] = m[r]; sml[ROWS + row] = l[r]; }
     }
-    if (parts > 1) cluster_sync(); else __syncthreads();
+    if (parts > 1) ib_cluster_sync(); else __syncthreads();
 #pragma unroll 1
     for (int row = part + warp * parts; row < used; row += WARPS * parts) {
         // a lane looks at a part's reference and denominator, then all look at some parts' sums at once: a look into another CTA takes 700 cycles
-        const float mc = lane < parts ? remote_f32(&sml[row], lane) : -INFINITY, lc = lane < parts ? remote_f32(&sml[ROWS + row], lane) : 0.0f;
+        const float mc = lane < parts ? ib_cluster_f32(&sml[row], lane) : -INFINITY, lc = lane < parts ? ib_cluster_f32(&sml[ROWS + row], lane) : 0.0f;
         const float top = ib_warp_max(mc), ref = top == -INFINITY ? 0.0f : top;
         const float f = lc == 0.0f ? 0.0f : exp2f(mc - ref);           // (0: this part of the keys holds none that the row sees)
         const float total = ib_warp_sum(lc * f);
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
 #pragma unroll
             for (int k = 0; k < SIDE; ++k)
 #pragma unroll
-                for (int i = 0; i < PER; ++i) v[k][i] = c + k < parts && number(i) < d ? remote_f32(&sq[row * dp + number(i)], c + k) : 0.0f;
+                for (int i = 0; i < PER; ++i) v[k][i] = c + k < parts && number(i) < d ? ib_cluster_f32(&sq[row * dp + number(i)], c + k) : 0.0f;
 #pragma unroll
             for (int k = 0; k < SIDE; ++k) {
                 const float fc = __shfl_sync(0xffffffffu, f, c + k);
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(WARPS * 32) tree_rows_kernel(const Args A, int
         for (int i = 0; i < PER; ++i)
             if (number(i) < d) dst[number(i)] = ib_from_float<T>(o[i] * inv);
     }
-    if (parts > 1) cluster_sync();                // nobody leaves while others read its sums
+    if (parts > 1) ib_cluster_sync();                // nobody leaves while others read its sums
 }
 
 template <typename T, int PER, int ROWS>
@@ -255,7 +255,7 @@ static int launch_rows(Args A, int max_tree, int max_keys, cudaStream_t stream) 
     A.tiles_of_rows = (int)(((long)max_tree * A.group + ROWS - 1) / ROWS);
     const long pairs = (long)A.n_requests * A.n_kv * A.tiles_of_rows;
     int parts = 1;       // about ten CTAs an SM, two or more that run and as many that follow them
-    while (parts < MAX_CLUSTER && pairs * parts * 2 <= 10 * 148 && max_keys >= 2 * KEYS * parts * 2) parts *= 2;
+    while (parts < IB_MAX_CLUSTER && pairs * parts * 2 <= 10 * 148 && max_keys >= 2 * KEYS * parts * 2) parts *= 2;
     const bool wide = (reinterpret_cast<uintptr_t>(A.k) | reinterpret_cast<uintptr_t>(A.v) | (uintptr_t)(A.dim * sizeof(T))) % 16 == 0;
     return launch_cluster(tree_rows_kernel<T, PER, ROWS>, pairs * parts, parts, WARPS * 32, rows_smem<T>(A.dim, ROWS), stream, A, parts, wide);
 }

@@ -25,7 +25,6 @@
 // What no row sees must not reach it: a product cannot leave a value out, and 0 times infinity is no number.  So the values of tiles that
 // some row does not see in full come with cp.async, and the warps that fill the ring look at what they brought, put zeros in the place of those that are
 // infinite or no numbers, and the rows that see such a value get it added at the end, from its page.
-#include "clusters.cuh"
 #include "sm100.cuh"
 #include "tree.cuh"
 
@@ -38,7 +37,6 @@ typedef __nv_bfloat16 bf16;
 constexpr int ROWS = 128, KEYS = 128;
 constexpr int PRODUCERS = 8, N_PRODUCERS = 2, ISSUER = 10, THREADS = 11 * 32;     // warps 0..7: softmax, 8 and 9: the ring, 10: products
 constexpr float STEP = 8.0f;          // how far (log2) a row's maximum may outgrow its reference
-constexpr int MOST_PARTS = IB_MAX_CLUSTER;
 constexpr int SLICE = 24, MOST_SLICES = 64;      // tiles (see cut_of)
 constexpr long MOST_SCRATCH = 256L << 20;        // bytes of all slices' sums (see cut_of)
 // Requests that are put in order of their length: every CTA does it for itself, a thread n / 352 times n comparisons.  (In order and as they come, trees
@@ -241,7 +239,7 @@ __device__ __forceinline__ void visible(const Args& A, const Span& S, const Plac
     }
 }
 
-__device__ __forceinline__ void remote_store(unsigned to, const float4& v) {      // into a CTA of the cluster (see remote)
+__device__ __forceinline__ void remote_store(unsigned to, const float4& v) {      // into a CTA of the cluster (see ib_cluster_address)
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
@@ -694,7 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (!mbar_wait(smem_u32(&sm.o_full), 0, 6)) ok = false;       // every product is done: the tiles' memory is free
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            if (scratch == nullptr && parts > 1) cluster_sync();          // the cluster's tiles are free: sums may go to any CTA
+            if (scratch == nullptr && parts > 1) ib_cluster_sync();          // the cluster's tiles are free: sums may go to any CTA
             if (NQ == 2 && parts == 1 && !sm.bad_values) {
                 // no other sums of these rows: they go out from here, a thread a row
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -741,7 +739,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             } else if (NQ == 2) {
                 // the only sums of a row that this CTA has: they go to the CTA that writes the row, a thread a row
                 const int row = g * ROWS + r, i = share_of(row), owner = row - i * parts;
-                const unsigned to = remote(inbox + (part * most + i) * Sh::OLD, owner);
+                const unsigned to = ib_cluster_address(inbox + (part * most + i) * Sh::OLD, owner);
 #pragma unroll 1
                 for (int e = 0; e < D; e += 32) {
                     unsigned x[32];
@@ -752,7 +750,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                     for (int k = 0; k < 32; k += 4)
                         remote_store(to + (e + k) * 4, make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]), __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])));
                 }
-                if (mine) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(m, ok ? l : NAN, sm.bad_values ? 1.0f : 0.0f, 0.0f));
+                if (mine) remote_store(ib_cluster_address(inbox_ml + (part * most + i) * 4, owner), make_float4(m, ok ? l : NAN, sm.bad_values ? 1.0f : 0.0f, 0.0f));
             } else {
                 if (count > 0 && ok) {
                     float* row = sums + (g * ROWS + r) * Sh::OLD;
@@ -769,11 +767,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 part_l[g * ROWS + r] = ok ? l : NAN;
             }
         } else if (scratch == nullptr && parts > 1) {
-            cluster_sync();
+            ib_cluster_sync();
         }
         fence_before();
     }
-    if (warp >= PRODUCERS && scratch == nullptr && parts > 1) cluster_sync();
+    if (warp >= PRODUCERS && scratch == nullptr && parts > 1) ib_cluster_sync();
     __syncthreads();
     if (warp == ISSUER) {
         fence_after();
@@ -795,13 +793,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             for (int line = row; line < 2 * ROWS; line += ROWS)
                 join<QUADS>(top, total, o, part_m[line], part_l[line], sums + line * Sh::OLD + e);
             const int i = share_of(row), owner = row - i * parts;
-            const unsigned to = remote(inbox + (part * most + i) * Sh::OLD + e, owner);
+            const unsigned to = ib_cluster_address(inbox + (part * most + i) * Sh::OLD + e, owner);
 #pragma unroll
             for (int k = 0; k < QUADS; ++k) remote_store(to + k * 128, o[k]);
-            if (e == 0) remote_store(remote(inbox_ml + (part * most + i) * 4, owner), make_float4(top, total, sm.bad_values ? 1.0f : 0.0f, 0.0f));
+            if (e == 0) remote_store(ib_cluster_address(inbox_ml + (part * most + i) * 4, owner), make_float4(top, total, sm.bad_values ? 1.0f : 0.0f, 0.0f));
         }
     }
-    if (parts > 1) cluster_sync();
+    if (parts > 1) ib_cluster_sync();
     else __syncthreads();
 #pragma unroll 1
     for (int i = line0; part + i * parts < rows; i += PASS) {
@@ -883,7 +881,7 @@ static int cut_of(const Args& A, int max_tree, int max_keys, Cut& c) {
     // 1,782; 256 requests, trees of 4, 2,796 MB: 3,216, 1,358, 554, 1,700; 100 requests of 100 to 32,400 keys, trees of 40: 1,647, 1,645, 1,538, 1,412.)
     const long rows = (long)max_tree * (A.n_heads / A.n_kv);
     c.slice_rows = c.waves && rows < NQ * ROWS ? (int)(rows + 31) / 32 * 32 : NQ * ROWS;
-    long most = MOST_PARTS;
+    long most = IB_MAX_CLUSTER;
     if (c.waves) {
         most = MOST_SCRATCH / (c.pairs * Shape<D, NQ>::slice_sums(c.slice_rows) * 4L);
         if (most > MOST_SLICES) most = MOST_SLICES;

@@ -1,8 +1,24 @@
-// How many clusters of CTAs run at once.
+// Clusters of CTAs: their barrier, a look into another CTA's shared memory, and how many of them run at once.
 #pragma once
 #include "common.cuh"
 
 constexpr int IB_MAX_CLUSTER = 8;
+
+__device__ __forceinline__ void ib_cluster_sync() {
+    __syncwarp();      // (the threads of a warp arrive as one)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// where the CTA of that rank has what this one has at `local`
+__device__ __forceinline__ unsigned ib_cluster_address(const void* local, unsigned rank) {
+    unsigned a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float ib_cluster_f32(const float* local, unsigned rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ib_cluster_address(local, rank)));
+    return v;
+}
 
 struct IbClusters { std::atomic<int> known[64][IB_MAX_CLUSTER + 1] = {}; };      // by device and size; 0: not asked yet
 

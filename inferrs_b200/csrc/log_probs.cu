@@ -78,28 +78,14 @@ __device__ __forceinline__ unsigned cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();      // (the threads of a warp arrive as one)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {
-    unsigned a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)));
-    return v;
-}
 __device__ __forceinline__ int remote_i32(const int* local, unsigned rank) {
     int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote(local, rank)));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ib_cluster_address(local, rank)));
     return v;
 }
 __device__ __forceinline__ u64 remote_u64(const u64* local, unsigned rank) {
     u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(local, rank)));
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(ib_cluster_address(local, rank)));
     return v;
 }
 
@@ -419,15 +405,15 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
             sh.board.n = TOP ? sh.n_notes : 0;
         }
     }
-    if (cluster > 1) cluster_sync(); else __syncthreads();
+    if (cluster > 1) ib_cluster_sync(); else __syncthreads();
     if (rank == 0) {
         // lane c looks at the c-th CTA's sums; all warps add them in the same order
         float mc = -INFINITY, total = 0.0f, weighed = 0.0f;
         int have = 0;
         if (lane < cluster) {
-            mc = remote_f32(&sh.board.m, lane);
-            total = remote_f32(&sh.board.s, lane);
-            weighed = remote_f32(&sh.board.w, lane);
+            mc = ib_cluster_f32(&sh.board.m, lane);
+            total = ib_cluster_f32(&sh.board.s, lane);
+            weighed = ib_cluster_f32(&sh.board.w, lane);
             have = remote_i32(&sh.board.n, lane);
         }
         const float all = ib_warp_max(mc);
@@ -482,7 +468,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) log_probs_kernel(const Args A
             }
         }
     }
-    if (cluster > 1) cluster_sync();        // nobody leaves while rank 0 reads
+    if (cluster > 1) ib_cluster_sync();        // nobody leaves while rank 0 reads
 }
 
 // The same with a warp a row, for many rows of few logits: a lane takes every 32nd block of 16, all of whose keys stay in its registers.  The likeliest

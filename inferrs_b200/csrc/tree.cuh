@@ -1,11 +1,9 @@
 // What the kernels for attention of drafted tokens share (attention_tree.cu says what they compute).
 #pragma once
 
-#include "common.cuh"
+#include "clusters.cuh"
 
 namespace tree {
-
-constexpr int MAX_CLUSTER = 8;
 
 struct Args {
     const void *q, *k, *v;
@@ -50,21 +48,6 @@ __device__ __forceinline__ unsigned mask_bits(const Args& A, const Span& s, cons
     const int left = s.n_tree - j;
     if (left < 32) bits &= left <= 0 ? 0u : (1u << left) - 1u;
     return bits;
-}
-
-__device__ __forceinline__ unsigned remote(const void* local, unsigned rank) {
-    unsigned a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float remote_f32(const float* local, unsigned rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(local, rank)));
-    return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();      // (the threads of a warp arrive as one)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename... KArgs, typename... Given>
