@@ -294,7 +294,8 @@ static int tree_args(const IbTreeAttention& c, tree::Args& A, int& max_tree, int
     A.out_ld = c.out_ld;
     A.n_rows = c.n_requests && c.max_tree ? (int)c.n_rows : 0;
     A.n_requests = (int)c.n_requests; A.n_heads = (int)c.n_heads; A.n_kv = (int)c.n_kv; A.dim = (int)c.dim;
-    A.max_pages = (int)c.max_pages; A.page_size = (int)c.page_size; A.n_pages = (int)c.n_pages; A.words = (int)c.words; A.span = (int)c.span;
+    A.max_pages = (int)c.max_pages; A.page_size = (int)c.page_size; A.n_pages = (int)c.n_pages; A.words = (int)c.words;
+    A.span = (int)(c.span > 0x7fffffffL ? 0x7fffffffL : c.span < -0x7fffffffL ? -0x7fffffffL : c.span);       // (wider than any context)
     A.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctzl(c.page_size) : -1;
     A.group = A.n_heads / A.n_kv;
     A.group_shift = (A.group & (A.group - 1)) == 0 ? __builtin_ctz((unsigned)A.group) : -1;

@@ -23,3 +23,11 @@ def test_lists_that_say_too_much(dtype, d):
     c["most"] = 7
     assert torch.equal(attend(dict(c, q_start=ints([0, 9, 5]))), attend(dict(c, q_start=ints([0, 7, 7]))))
     assert kernels.attention_tree_error() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F32, 64)])
+def test_windows_wider_than_any_context(dtype, d):
+    c = drafted(16, [50, 300], [3, 4], 4, 2, d, 16, dtype)
+    whole = attend(c)
+    for span in (2 ** 31 - 1, 2 ** 31, 2 ** 31 + 5, 2 ** 40, 2 ** 32 + 7, -2 ** 31, -2 ** 32 - 9):
+        assert torch.equal(attend(c, span), whole), span
