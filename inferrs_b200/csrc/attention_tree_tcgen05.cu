@@ -15,7 +15,8 @@
 // order in which the products take them: by TMA, a box for every page, and where pages have an odd size with cp.async, 16 bytes a
 // lane.  Where there is no key zeros are written.
 //
-// What bounds it.  16 trees of 64 over up to 16,384 keys, 32 heads on 8 of 128 (171 us; the bytes alone 90): with 256 rows the tensor cores, whose
+// What bounds it.  16 trees of 64 over up to 16,384 keys, 32 heads on 8 of 128 (165 to 190 us by the order of the requests, 207 where the power limit
+// holds the clock at 1.6 GHz; the bytes alone 90): with 256 rows the tensor cores, whose
 // products of 128 x 128 x 16 take 85 to 100 cycles where 64 would do, 3,300 a tile, and 16 us of the join.  8 trees of 16 over 2,048 keys (21.3 us;
 // 10.6): memory while the ring runs, on 128 of 148 SMs, and about 10,000 of 38,000 cycles before and behind it.  One tree of 8 over 300
 // keys (8.7 us): the chain start, one tile (6,000 cycles), join (5,000), much of it waiting for instructions that run once.  Up to 64 rows standing twice
@@ -870,7 +871,7 @@ static int cut_of(const Args& A, int max_tree, int max_keys, Cut& c) {
     c.tiles = (int)((keys + KEYS - 1) / KEYS);
     // One wave of CTAs: as many parts as there are SMs for, a cluster each.  More than that: requests differ in length, and clusters would wait
     // for as many free SMs at once; slices of 24 tiles or more, the longest requests first, are joined by a kernel of their own.  (Trees of 64,
-    // 32 heads on 8, 16 requests of 100 to 16,384 keys: slices of 12, 16, 24, 32 tiles 190, 180, 167, 178 us, whole requests 246; all of 16,384:
+    // 32 heads on 8, 16 requests of 100 to 16,384 keys: slices of 12, 16, 24, 32 tiles 190, 180, 167, 178 us in short runs, whole requests 246; all of 16,384:
     // 325, 306, 305, 299; of 100 to 4,500: 67, 73, and whole ones, which 24 leaves them, 73.)
     c.waves = 2 * c.pairs > 148 && c.tiles > 2 * SLICE;
     c.parts = c.waves ? (c.tiles + SLICE - 1) / SLICE : 148 / c.pairs;

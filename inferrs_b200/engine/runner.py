@@ -203,7 +203,8 @@ class ModelRunner:
 
     def step_drafts(self, entries: Sequence[DraftEntry]) -> torch.Tensor:
         """float32 logits [number of drafted tokens, vocab] of trees of drafted tokens, each behind what its request holds and its
-        own ancestors.  Nothing of them is held yet: :meth:`keep_drafts` says what stays, and the next step without it writes over them."""
+        own ancestors.  Nothing of them is held yet: :meth:`keep_drafts` says what stays, and the next step without it writes over them.  What
+        the kernels report about themselves is the caller's to look at, as behind :meth:`step` (``kernels.reset_error_words``)."""
         if not self.takes_drafts():
             raise BatchError("this model has layers that cannot run a tree of drafted tokens")
         wants = {e.rid: len(e.tokens) for e in entries}

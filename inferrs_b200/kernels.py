@@ -2818,7 +2818,12 @@ def paged_attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     int32 [R, max_pages], q_start int32 [R + 1] (ascending), context int32 [R], positions int32 [N] (only read with a window), seen int32
     [N, words].  ``max_tree``: no request has more drafted tokens (rows beyond it may be left out); ``max_kv_len``: how the keys are
     cut goes by it.  A row that sees no key gets zeros; a key without a page is none; rows from q_start[R] on are left as they
-    were.  The rows of ``out`` may lie apart."""
+    were.  The rows of ``out`` may lie apart.
+
+    Scores, references and sums are held in 32 bits.  In bfloat16 with heads of 64 or 128 the softmax's numbers are rounded to bfloat16 before
+    the product with the values (2^-8 of each at most, as in the framework's other attention in that type), and the sums that divide are not;
+    in float32, and with other heads, nothing is rounded before the end.  Many requests over long contexts take up to 256 MB of workspace from
+    torch's allocator for the time of the call."""
     act = out.dtype
     out_ld = _need_rows(out, "out", _BF16_F32)
     if not (_lists(q_start, context) and q.dtype is act and k_pages.dtype is act and v_pages.dtype is act and q.dim() == 3
