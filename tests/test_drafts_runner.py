@@ -330,3 +330,95 @@ def test_trees_through_layers_with_windows(monkeypatch, window, page):
     drafts_refs.install(monkeypatch)
     rt = Runtime(torch.device("cpu"), torch.float32)
     check_windows(lambda: windowed_runner(CONFIG_A, window, page, rt), window, page, 1e-4)
+
+
+# ---- everything in any order --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seed", range(6))
+def test_steps_trees_forks_and_ends_in_any_order(model_dirs, monkeypatch, seed):
+    """Requests that come, go on, draft, keep some of it or none, fork and end in random order: every row that is looked at has the logits of its
+    request's tokens, and a request without drafts holds the pages of its tokens."""
+    drafts_refs.install(monkeypatch)
+    rng = random.Random(seed)
+    page, vocab = PAGE_SIZE["A"], CONFIG_A["vocab_size"]
+    runner = make_runner(model_dirs["A"], page, n_pages=40, max_requests=4)
+    held, drafted, new = {}, {}, iter(range(10 ** 6))
+
+    def some():
+        return rng.sample(sorted(held), rng.randrange(1, len(held) + 1)) if held else []
+
+    def path(rid):
+        tokens, tree = drafted[rid]
+        way, at = [], -1
+        while True:
+            children = [i for i, p in enumerate(tree) if p == at]
+            if not children or rng.random() < 0.3:
+                return way
+            at = rng.choice(children)
+            way.append(at)
+
+    def look(logits, row, tokens):
+        if rng.random() < 0.25:
+            assert rel_err(logits[row], last_logits(model_dirs["A"], tokens)) < 1e-4
+
+    for _ in range(120):
+        what = rng.random()
+        try:
+            if what < 0.12 and runner.manager.n_free_slots:
+                rid = next(new)
+                runner.admit(rid)
+                prompt = random_tokens(rng.randrange(1, 14), vocab, seed=rid)
+                held[rid] = []
+                logits = runner.step([StepEntry(rid, prompt, [len(prompt) - 1])])
+                held[rid] = prompt
+                look(logits, 0, prompt)
+            elif what < 0.35 and held:
+                entries = [StepEntry(r, random_tokens(rng.choice([1, 1, 1, 5]), vocab, seed=rng.randrange(10 ** 6)), [0]) for r in some()]
+                logits = runner.step(entries)
+                for i, e in enumerate(entries):
+                    look(logits, i, held[e.rid] + list(e.tokens[:1]))
+                    held[e.rid] = held[e.rid] + list(e.tokens)
+                    drafted.pop(e.rid, None)
+            elif what < 0.62 and held:
+                entries = []
+                for r in some():
+                    n = rng.randrange(1, 11)
+                    entries.append(DraftEntry(r, random_tokens(n, vocab, seed=rng.randrange(10 ** 6)), [rng.randrange(-1, i) for i in range(n)]))
+                logits = runner.step_drafts(entries)
+                row = 0
+                for e in entries:
+                    drafted[e.rid] = (list(e.tokens), list(e.parents))
+                    for i in range(len(e.tokens)):
+                        way, at = [], i
+                        while at >= 0:
+                            way, at = [e.tokens[at]] + way, e.parents[at]
+                        look(logits, row, held[e.rid] + way)
+                        row += 1
+            elif what < 0.85 and drafted:
+                kept = {r: path(r) for r in rng.sample(sorted(drafted), rng.randrange(1, len(drafted) + 1))}
+                runner.keep_drafts(kept)
+                for r, way in kept.items():
+                    tokens = drafted.pop(r)[0]
+                    held[r] = held[r] + [tokens[k] for k in way]
+            elif what < 0.93 and held and runner.manager.n_free_slots:
+                r, rid = rng.choice(sorted(held)), next(new)
+                runner.fork(r, rid)
+                held[rid] = list(held[r])
+            elif held:
+                r = rng.choice(sorted(held))
+                runner.release(r)
+                del held[r]
+                drafted.pop(r, None)
+        except OutOfPages:
+            empty = [r for r in held if not held[r]]
+            for r in empty or rng.sample(sorted(held), 1):
+                runner.release(r)
+                del held[r]
+                drafted.pop(r, None)
+        runner.manager.check_invariants()
+        for r, tokens in held.items():
+            assert runner.n_tokens(r) == len(tokens)
+            if r not in drafted:
+                assert pages_held(runner, r) == [-(-len(tokens) // page)]
+    for r in list(held):
+        runner.release(r)
+    assert [p.n_free for p in runner.manager.pools] == [40]
